@@ -196,6 +196,44 @@ int32_t olmax_cross_entropy_reduce(olmax_stream_t stream, const void* logits, vo
                                    int64_t T, int32_t V, int64_t ld, int64_t ldd, int32_t logits_f32,
                                    int32_t ignore_index, float softcap, float dloss, int32_t reduction);
 
+/* ---- Log probabilities of given tokens, beside the cross entropy: what evaluation, policy-gradient losses and a teacher's pass take
+ * from logits.  No counterpart in the reference (its cross_entropy_loss, src/olmax/nn/functional.py:70-91, returns -logprob of the labels).
+ * z = cap(x) / temperature, cap(x) = softcap * tanh(x / softcap) where softcap > 0; p = softmax(z) over the V logits of a row.
+ * logprobs [T] (optional; needs targets) = ln p[target], 0 for a target outside [0, V); entropy [T] = - sum p ln p;
+ * stats [T, 3] = {m = max z, ln sum exp(z - m), entropy}, what the backward call takes (its first two add up to the log-normaliser);
+ * top_ids / top_logprobs [T, top] (top 0 to 128, at most V): the largest logits x in order, ties to the lowest index.  A row whose target
+ * is ignore_index is not read: zeros, ids of -1, log probabilities of minus infinity.  Logits of minus infinity are tokens of no
+ * probability; a row of nothing else has entropy 0 and log probabilities of minus infinity.  A NaN or an infinite score makes a row's values NaN
+ * (the ids stay different tokens).  targets NULL: no row is left out.  logits: any row stride >= V and any alignment of their type.
+ * All fp32; results do not depend on the order in which anything runs. */
+int64_t olmax_token_logprobs_workspace_bytes(int64_t T, int32_t V, int32_t top, int32_t logits_f32);
+int32_t olmax_token_logprobs(olmax_stream_t stream, const void* logits, const int32_t* targets, float* logprobs,
+                             float* entropy, float* stats, int32_t* top_ids, float* top_logprobs,
+                             void* workspace, int64_t workspace_bytes, int64_t T, int32_t V, int64_t ld,
+                             int32_t top, int32_t logits_f32, int32_t ignore_index, float temperature,
+                             float softcap);
+/* dlogits [T, V] (type of the logits; may be them, with the same stride) from the cotangents dlogprobs [T] and dentropy [T] (optional).  Rows of
+ * an ignored target get zeros, a target outside [0, V) has no log probability to follow. */
+int32_t olmax_token_logprobs_bwd(olmax_stream_t stream, const void* logits, const int32_t* targets,
+                                 const float* stats, const float* dlogprobs, const float* dentropy,
+                                 void* dlogits, int64_t T, int32_t V, int64_t ld, int64_t ldd,
+                                 int32_t logits_f32, int32_t ignore_index, float temperature, float softcap);
+
+/* ---- Distillation from a teacher's top logits: the cross entropy's place in a step that learns from a teacher.  No counterpart in the reference.
+ * top_ids / top_logprobs [T, k], k 1 to 128, are the teacher's tokens and what it says of them (olmax_token_logprobs writes both).
+ * tail 0, renormalize: q = softmax over the k numbers / temperature; L = sum q ln(q / p[id]).  tail 1, bucket: q = exp(top_logprobs), and all
+ * other tokens are one event: L = sum q ln(q / p[id]) + r ln(r / s), r = 1 - sum q (0 below 2^-20), s = sum of the other tokens' p (V up to 2^20 - 32).
+ * p is the student's softmax of cap(logits) / temperature.  A row whose first id is negative is left out (no loss, zero gradient); other ids
+ * outside [0, V), and those named before in the row, are dropped.  A row without a logit above minus infinity has no loss and no gradient.
+ * reduction 0 mean over the rows that are not left out, 1 sum, 2 none (loss [T], cotangent dloss * dloss_rows[t]).  dlogits (optional; type of the
+ * logits; may be them, with the same stride) receives dloss * dL/dlogits.  (Softened targets are commonly weighted by temperature^2: through dloss.) */
+int64_t olmax_distill_workspace_bytes(int64_t T);
+int32_t olmax_distill(olmax_stream_t stream, const void* logits, void* dlogits, const int32_t* top_ids,
+                      const float* top_logprobs, float* loss, const float* dloss_rows, void* workspace,
+                      int64_t workspace_bytes, int64_t T, int32_t V, int32_t k, int64_t ld, int64_t ldd,
+                      int32_t logits_f32, int32_t tail, float temperature, float softcap, float dloss,
+                      int32_t reduction);
+
 /* ---- LM head + cross entropy, forward and backward in one call (three GEMMs around a row kernel;
  * the bf16 logits [T, V] are materialised once in the workspace and overwritten by their gradient,
  * never as fp32 and never twice): LMHead.forward,
@@ -207,6 +245,27 @@ int32_t olmax_lmhead_ce(olmax_stream_t stream, const void* h, const void* W, con
                         float* loss, void* dh, void* dW, void* workspace, int64_t workspace_bytes,
                         int64_t T, int32_t d, int32_t V, int32_t ignore_index, float softcap,
                         int32_t dw_f32);
+
+/* The LM head with olmax_token_logprobs, its backward pass, and with olmax_distill (reduction mean): h [T, d], W [V, d] bf16, the logits h W^T
+ * summed and kept in fp32.  The backward call runs the product again.  dh [T, d] bf16 and dW [V, d] (bf16, or fp32 with
+ * dw_f32 != 0) may be NULL to skip. */
+int64_t olmax_lmhead_logprobs_workspace_bytes(int64_t T, int32_t d, int32_t V, int32_t top);
+int32_t olmax_lmhead_logprobs(olmax_stream_t stream, const void* h, const void* W, const int32_t* targets,
+                              float* logprobs, float* entropy, float* stats, int32_t* top_ids,
+                              float* top_logprobs, void* workspace, int64_t workspace_bytes, int64_t T,
+                              int32_t d, int32_t V, int32_t top, int32_t ignore_index, float temperature,
+                              float softcap);
+int64_t olmax_lmhead_logprobs_bwd_workspace_bytes(int64_t T, int32_t d, int32_t V);
+int32_t olmax_lmhead_logprobs_bwd(olmax_stream_t stream, const void* h, const void* W, const int32_t* targets,
+                                  const float* stats, const float* dlogprobs, const float* dentropy, void* dh,
+                                  void* dW, void* workspace, int64_t workspace_bytes, int64_t T, int32_t d,
+                                  int32_t V, int32_t ignore_index, float temperature, float softcap,
+                                  int32_t dw_f32);
+int64_t olmax_lmhead_distill_workspace_bytes(int64_t T, int32_t d, int32_t V);
+int32_t olmax_lmhead_distill(olmax_stream_t stream, const void* h, const void* W, const int32_t* top_ids,
+                             const float* top_logprobs, float* loss, void* dh, void* dW, void* workspace,
+                             int64_t workspace_bytes, int64_t T, int32_t d, int32_t V, int32_t k, int32_t tail,
+                             float temperature, float softcap, float dloss, int32_t dw_f32);
 
 /* ---- Synthetic token batches: _randomize_start_offsets, src/olmax/data/utils.py:12-33:
  * inputs[b, s] = (s + start_offsets[b]) mod V, targets = inputs + 1 (so a target equals V when

@@ -66,6 +66,12 @@ _SIGNATURES = {
     "olmax_fill_zero": "PPL",
     "olmax_attn_fwd": "PPPPPPIIIIILLLLIF",
     "olmax_attn_bwd": "PPPPPPPPPPPLIIIIILLLLLLLLIF",
+    "olmax_token_logprobs": "PPPPPPPPPLLILIIIFF",
+    "olmax_token_logprobs_bwd": "PPPPPPPLILLIIFF",
+    "olmax_distill": "PPPPPPPPLLIILLIIFFFI",
+    "olmax_lmhead_logprobs": "PPPPPPPPPPLLIIIIFF",
+    "olmax_lmhead_logprobs_bwd": "PPPPPPPPPPLLIIIFFI",
+    "olmax_lmhead_distill": "PPPPPPPPPLLIIIIFFFI",
 }
 _typed = {}
 

@@ -192,6 +192,9 @@ int olmax_gemm_grads(hipStream_t s, const bf16* dy, const bf16* w, const bf16* x
 int olmax_lmhead_ce_scratch(hipStream_t stream, const void* h, const void* W, const int32_t* labels, float* loss, void* dh, void* dW,
                             void* workspace, int64_t workspace_bytes, int64_t T, int32_t d, int32_t V, int32_t ignore_index,
                             float softcap, int32_t dw_f32, GemmScratch scratch);
+// lmhead_ce.hip: dh [T, d] = dlogits W and dW [V, d] = dlogits^T h of dlogits [T, V] whose rows are zero up to a multiple of 8; either may be null
+int olmax_lmhead_products(hipStream_t stream, const bf16* dlogits, const bf16* W, const bf16* h, bf16* dh, void* dW, int T, int d, int V, int64_t ldl,
+                          bool dw_f32, GemmScratch scratch = GemmScratch());
 // elementwise.hip: pieces of the flat buffers too small for a launch each; one launch takes a table of them.  off: first element in
 // parameter layout, goff: of its gradient in the bf16 or (g_f32) fp32 buffer
 struct FlatRange {

@@ -464,6 +464,14 @@ extern "C" int64_t olmax_lmhead_ce_workspace_bytes(int64_t T, int32_t V) {
   return ((T * logits_stride(V) * 2 + 255) / 256) * 256 + olmax_cross_entropy_workspace_bytes(T);
 }
 
+int olmax_lmhead_products(hipStream_t stream, const bf16* dlogits, const bf16* W, const bf16* h, bf16* dh, void* dW, int T, int d, int V, int64_t ldl,
+                          bool dw_f32, GemmScratch scratch) {
+  if (dh && dW) return olmax_gemm_grads(stream, dlogits, W, h, dh, nullptr, dW, T, d, V, ldl, d, d, d, 0, d, dw_f32, true, scratch);
+  if (dh) return olmax_gemm_padded(stream, dlogits, W, dh, nullptr, T, d, V, ldl, d, d, 0, true, false, false, true, scratch);
+  if (dW) return olmax_gemm_padded(stream, dlogits, h, dW, nullptr, V, d, T, ldl, d, d, 0, false, false, dw_f32, true, scratch);
+  return OLMAX_OK;
+}
+
 // Fused LM head + cross entropy, forward and backward in one call:
 //   logits = h W^T (bf16) ; loss = CE(softcap(logits), labels) ;
 //   dlogits overwrites logits in the workspace ; dh = dlogits W ; dW = dlogits^T h.
@@ -486,17 +494,7 @@ int olmax_lmhead_ce_scratch(hipStream_t stream, const void* h, const void* W, co
   rc = cross_entropy(stream, logits, need_grad ? logits : nullptr, labels, loss, nullptr, nullptr, ce_ws,
                      olmax_cross_entropy_workspace_bytes(T), T, V, ldl, ldl, 0, ignore_index, softcap, 1.f, 0, true);
   if (rc) return rc;
-  if (dh && dW)
-    return olmax_gemm_grads(stream, logits, wp, hp, (bf16*)dh, nullptr, dW, (int)T, d, V, ldl, d, d, d, 0, d, dw_f32 != 0, true, scratch);
-  if (dh) {
-    rc = olmax_gemm_padded(stream, logits, wp, dh, nullptr, (int)T, d, V, ldl, d, d, 0, true, false, false, true, scratch);
-    if (rc) return rc;
-  }
-  if (dW) {
-    rc = olmax_gemm_padded(stream, logits, hp, dW, nullptr, V, d, (int)T, ldl, d, d, 0, false, false, dw_f32 != 0, true, scratch);
-    if (rc) return rc;
-  }
-  return OLMAX_OK;
+  return olmax_lmhead_products(stream, logits, wp, hp, (bf16*)dh, dW, (int)T, d, V, ldl, dw_f32 != 0, scratch);
 }
 
 extern "C" int32_t olmax_lmhead_ce(hipStream_t stream, const void* h, const void* W,

@@ -1,0 +1,570 @@
+// Log probabilities of given tokens, the entropy of their distributions and the most likely alternatives, with the gradient.
+//
+// z = cap(x) / temperature (rows.h), p = softmax(z):  logprob = z[target] - m - ln S,  entropy = ln S - sum p (z - m),
+// alternatives = the `top` largest logits, in order, ties to the lowest index.
+#include "rows.h"
+#include <algorithm>
+
+using namespace rows;
+
+namespace {
+
+constexpr int TH = 256;       // threads of a workgroup
+constexpr int UNROLL = 4;     // vectors of a thread that are in flight, and reduced against one maximum
+constexpr int MAX_TOP = 128;
+constexpr int CAND = 1024;    // candidates for the alternatives that a workgroup can hold
+constexpr int JOINED = 2048;  // of all parts of a row
+
+// Rises with the value; -0 is 0.
+__device__ __forceinline__ unsigned key_of(float x) {
+  const unsigned b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+constexpr unsigned KEY_NEG_INF = 0x007fffffu;
+// A candidate: larger for a larger value, and among equal ones for a lower index; 0: none.
+__device__ __forceinline__ uint64_t entry_of(unsigned key, int index) { return ((uint64_t)key << 32) | (0xffffffffu - (unsigned)index); }
+__device__ __forceinline__ int index_of(uint64_t e) { return (int)(0xffffffffu - (unsigned)e); }
+
+struct Lds {
+  alignas(16) unsigned best[TH];  // key of each thread's largest
+  uint64_t cand[CAND];
+  unsigned hist[256];
+  Stat red[TH / 64];
+  int n, sums[TH / 64];
+};
+
+// A lower bound of the k-th largest value that the workgroup has seen, from the largest of each thread: at least k values are not below the k-th
+// largest of those.  Found on the upper 16 bits of the keys, by bits: each wave counts all TH of them, four a lane.
+__device__ __forceinline__ unsigned kth_best(unsigned* best, unsigned own, int k) {
+  __syncthreads();
+  best[threadIdx.x] = own;
+  __syncthreads();
+  const u32x4 q = *reinterpret_cast<const u32x4*>(best + (threadIdx.x & 63) * 4);
+  unsigned at = 0;
+#pragma unroll
+  for (int bit = 15; bit >= 0; bit--) {
+    const unsigned tried = at | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) n += __popcll(__ballot((q[j] >> 16) >= tried));
+    if (n >= k) at = tried;
+  }
+  return max(at << 16, KEY_NEG_INF);
+}
+
+// The exact way, for rows with more values that tie at the bound than there is room: the k largest of elements [lo, hi) above minus infinity go
+// to cand, in any order; returns how many.  The k-th largest key by four passes of 8 bits, then all above it, then as many equal ones as are
+// missing, from the lowest index on.
+template <typename T>
+__device__ int select_exact(const T* zr, int lo, int hi, int k, Lds& l) {
+  unsigned at = 0;
+  int need = k;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    __syncthreads();
+    l.hist[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = lo + threadIdx.x; i < hi; i += TH) {
+      const float x = (float)zr[i];
+      if (!(x > -INFINITY)) continue;
+      const unsigned key = key_of(x);
+      if (shift == 24 || (key >> (shift + 8)) == (at >> (shift + 8))) atomicAdd(&l.hist[(key >> shift) & 255], 1u);
+    }
+    __syncthreads();
+    int b = 255, above = 0;
+    for (; b > 0; b--) {
+      const int n = (int)l.hist[b];
+      if (above + n >= need) break;
+      above += n;
+    }
+    need -= above;
+    at |= (unsigned)b << shift;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) l.n = 0;
+  __syncthreads();
+  for (int i = lo + threadIdx.x; i < hi; i += TH) {
+    const float x = (float)zr[i];
+    if (x > -INFINITY && key_of(x) > at) l.cand[atomicAdd(&l.n, 1)] = entry_of(key_of(x), i);
+  }
+  __syncthreads();
+  const int above = l.n;
+  int got = 0;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int base = lo; base < hi && got < need; base += TH) {
+    const int i = base + threadIdx.x;
+    const float x = i < hi ? (float)zr[i] : -INFINITY;
+    const bool eq = x > -INFINITY && key_of(x) == at;
+    const uint64_t votes = __ballot(eq);
+    __syncthreads();
+    if (lane == 0) l.sums[wave] = __popcll(votes);
+    __syncthreads();
+    int before = got + __popcll(votes & ((1ull << lane) - 1));
+    for (int w = 0; w < wave; w++) before += l.sums[w];
+    if (eq && before < need) l.cand[above + before] = entry_of(at, i);
+    for (int w = 0; w < TH / 64; w++) got += l.sums[w];
+  }
+  __syncthreads();
+  return above + min(got, need);
+}
+
+// Leaves of cand[0 .. n) those whose key is at least `bound`, in any order, and returns how many.  Each thread holds its share meanwhile.
+template <int ROOM>
+__device__ __forceinline__ int narrow(uint64_t* cand, int n, unsigned bound, int* counter) {
+  uint64_t own[ROOM / TH];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < ROOM / TH; i++) {
+    const int at = i * TH + threadIdx.x;
+    own[i] = at < n ? cand[at] : 0;
+  }
+  if (threadIdx.x == 0) *counter = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < ROOM / TH; i++)
+    if (own[i] && (unsigned)(own[i] >> 32) >= bound) cand[atomicAdd(counter, 1)] = own[i];
+  __syncthreads();
+  return *counter;
+}
+
+// emit(rank, entry) for the k largest of cand[0 .. n): an entry's rank is the number of larger ones (all are different).
+template <typename F>
+__device__ __forceinline__ void ranked(const uint64_t* cand, int n, int k, F emit) {
+  for (int i = threadIdx.x; i < n; i += TH) {
+    const uint64_t e = cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += cand[j] > e;
+    if (rank < k) emit(rank, e);
+  }
+}
+
+// What a row's outputs are written from.
+struct Out {
+  float *logprobs, *entropy, *stats, *top_logprobs;  // logprobs and the top ones may be null
+  int32_t* top_ids;
+};
+__device__ __forceinline__ void write_skipped(const Out& o, int64_t row, int k) {
+  if (threadIdx.x == 0) {
+    if (o.logprobs) o.logprobs[row] = 0.f;
+    o.entropy[row] = 0.f;
+  }
+  if (threadIdx.x < 3) o.stats[row * 3 + threadIdx.x] = 0.f;
+  if (o.top_ids && (int)threadIdx.x < k) {
+    o.top_ids[row * k + threadIdx.x] = -1;
+    o.top_logprobs[row * k + threadIdx.x] = -INFINITY;
+  }
+}
+// a: statistics of the whole row.  A row without a score above minus infinity has no distribution: log probabilities of minus infinity, entropy 0.
+template <typename T, bool CAP>
+__device__ __forceinline__ void write_row(const Out& o, int64_t row, const T* zr, int target, int V, const Scale& c, const Stat& a) {
+  const bool none = a.s == 0.f;
+  const float log_sum = log_of(a.s), entropy = none ? 0.f : log_sum - a.t / a.s;
+  if (threadIdx.x == 0) {
+    if (o.logprobs) o.logprobs[row] = target < 0 || target >= V ? 0.f : none ? -INFINITY : behind<CAP>((float)zr[target], c, a.m) - log_sum;
+    o.entropy[row] = entropy;
+    o.stats[row * 3] = a.m;
+    o.stats[row * 3 + 1] = none ? 0.f : log_sum;
+    o.stats[row * 3 + 2] = entropy;
+  }
+}
+// The n <= k largest logits above minus infinity are cand[0 .. n) or are the largest of them; the rest of k slots gets the lowest indices that are not among them.
+template <bool CAP>
+__device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, const uint64_t* cand, int n, const Scale& c, const Stat& a) {
+  int32_t* ids = o.top_ids + row * k;
+  float* lp = o.top_logprobs + row * k;
+  const float log_sum = log_of(a.s);
+  const bool none = a.s == 0.f;
+  ranked(cand, n, k, [&](int rank, uint64_t e) {
+    ids[rank] = index_of(e);
+    lp[rank] = none ? -INFINITY : behind<CAP>(value_of((unsigned)(e >> 32)), c, a.m) - log_sum;
+  });
+  if (n < k && (int)threadIdx.x < k) {  // (the first k indices hold at least k - n others)
+    int below = 0;
+    bool there = false;
+    for (int j = 0; j < n; j++) {
+      const int id = index_of(cand[j]);
+      below += id < (int)threadIdx.x;
+      there |= id == (int)threadIdx.x;
+    }
+    const int rank = n + (int)threadIdx.x - below;
+    if (!there && rank < k) {
+      ids[rank] = threadIdx.x;
+      lp[rank] = none ? -INFINITY : behind<CAP>(-INFINITY, c, a.m) - log_sum;
+    }
+  }
+}
+
+// One workgroup to a row, or to one of `parts` equal shares of it; a part leaves its statistics and its candidates for score_join_kernel.
+template <typename T, bool CAP, bool TOP>
+__global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out, uint64_t* __restrict__ part_top,
+                                                        Stat* __restrict__ part_stat, int V, int64_t ld, int32_t ignore_index, Scale c, int k, int parts) {
+  constexpr int N = Vec<T>::N, SPAN = TH * UNROLL;
+  __shared__ Lds l;
+  const int64_t row = blockIdx.x / parts;
+  const int part = blockIdx.x % parts;
+  const int target = targets ? targets[row] : -1;
+  if (targets && target == ignore_index) {  // (the join writes for a row in parts)
+    if (parts == 1) write_skipped(out, row, k);
+    return;
+  }
+  const T* zr = logits + row * ld;
+  const Cut cutting = cut<T, N>(zr, V);
+  const T* body = zr + cutting.head;
+  const int per = (cutting.nvec + parts - 1) / parts;
+  const int v0 = min(part * per, cutting.nvec), v1 = min(v0 + per, cutting.nvec);
+  if (TOP && threadIdx.x == 0) l.n = 0;
+  Raw<T, N> next[UNROLL];
+  auto fetch = [&](int at) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      const int v = at + u * TH + threadIdx.x;
+      if (v < v1) next[u].load(body + (int64_t)v * N);
+    }
+  };
+  fetch(v0);
+  Stat a = Stat::none();
+  float most = -INFINITY;  // of the logits themselves
+  unsigned bound = KEY_NEG_INF;
+  float bound_value = -INFINITY;
+  auto offer = [&](float x, int i) {
+    if (x >= bound_value && x > -INFINITY) {
+      const int at = atomicAdd(&l.n, 1);
+      if (at < CAND) l.cand[at] = entry_of(key_of(x), i);
+    }
+  };
+  // the single elements at the row's ends, one to a thread
+  const bool has_edge = part == 0 && (int)threadIdx.x < cutting.edges;
+  const int edge = has_edge ? cutting.edge(threadIdx.x, V) : 0;
+  const float edge_x = has_edge ? (float)zr[edge] : -INFINITY;
+  if (has_edge) {
+    if (edge_x > -INFINITY) most = edge_x;
+    if (CAP || edge_x > -INFINITY) a.m = score<CAP>(edge_x, c);
+    const float d = behind<CAP>(edge_x, c, a.ref()), e = exp_of(d);
+    a.s = e;
+    a.t = e * fmaxf(d, -200.f);
+  }
+  const int chunks = max(1, (v1 - v0 + SPAN - 1) / SPAN);
+  for (int ch = 0; ch < chunks; ch++) {
+    const int at = v0 + ch * SPAN;
+    Raw<T, N> now[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) now[u] = next[u];
+    if (ch + 1 < chunks) fetch(at + SPAN);
+    float cm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      if (at + u * TH + (int)threadIdx.x >= v1) continue;
+      float x[N];
+      now[u].unpack(x);
+#pragma unroll
+      for (int e = 0; e < N; e++) cm = fmaxf(cm, x[e]);
+    }
+    if (cm > most || (CAP && a.m == -INFINITY)) {  // (a soft-cap makes a score of minus infinity too)
+      most = fmaxf(most, cm);
+      a.raise(score<CAP>(most, c));
+    }
+    const float ref = a.ref();
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      if (at + u * TH + (int)threadIdx.x >= v1) continue;
+      float x[N], t[N];
+      now[u].unpack(x);
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const float d = behind<CAP>(x[e], c, ref);
+        x[e] = exp_of(d);
+        t[e] = x[e] * fmaxf(d, -200.f);
+      }
+#pragma unroll
+      for (int w = N / 2; w > 0; w >>= 1)
+#pragma unroll
+        for (int e = 0; e < w; e++) x[e] += x[e + w], t[e] += t[e + w];
+      a.s += x[0];
+      a.t += t[0];
+    }
+    if (TOP) {
+      if ((ch & (ch + 1)) == 0) {  // 1, 2, 4, .. chunks seen: about k candidates between two bounds
+        bound = kth_best(l.best, key_of(most), k);
+        bound_value = value_of(bound);
+      }
+      if (ch == 0 && has_edge) offer(edge_x, edge);
+      if (cm >= bound_value) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+          const int v = at + u * TH + threadIdx.x;
+          if (v >= v1) continue;
+          float x[N];
+          now[u].unpack(x);
+#pragma unroll
+          for (int e = 0; e < N; e++) offer(x[e], cutting.head + v * N + e);
+        }
+      }
+    }
+  }
+  const Stat all = block_join<TH / 64>(a, l.red);
+  int n = 0;
+  if (TOP) {
+    if (((chunks - 1) & chunks) != 0) bound = kth_best(l.best, key_of(most), k);  // of all that was seen
+    __syncthreads();
+    n = l.n;
+    if (n > CAND) {
+      const int first = part == 0 ? 0 : cutting.head + v0 * N;  // part 0 has the edges: the row's first elements and its last
+      const int last = cutting.head + v1 * N;
+      if (parts == 1) {
+        n = select_exact(zr, 0, V, k, l);
+      } else {
+        n = select_exact(zr, first, last, k, l);
+        if (part == 0) {  // the rest behind the last vector joins the k largest of the others (cand has room: k + 7 <= CAND)
+          const int rest = cutting.edges - cutting.head;
+          __syncthreads();
+          if (threadIdx.x == 0) l.n = n;
+          __syncthreads();
+          if ((int)threadIdx.x < rest) {
+            const int i = V - rest + threadIdx.x;
+            const float x = (float)zr[i];
+            if (x > -INFINITY) l.cand[atomicAdd(&l.n, 1)] = entry_of(key_of(x), i);
+          }
+          __syncthreads();
+          n = l.n;
+        }
+      }
+    } else {
+      n = narrow<CAND>(l.cand, n, bound, &l.n);
+    }
+  }
+  if (parts == 1) {
+    write_row<T, CAP>(out, row, zr, target, V, c, all);
+    if (TOP) write_top<CAP>(out, row, k, l.cand, n, c, all);
+    return;
+  }
+  if (threadIdx.x == 0) part_stat[blockIdx.x] = all;
+  if (TOP) {
+    uint64_t* mine = part_top + (int64_t)blockIdx.x * k;
+    ranked(l.cand, n, k, [&](int rank, uint64_t e) { mine[rank] = e; });
+    for (int i = n + threadIdx.x; i < k; i += TH) mine[i] = 0;
+  }
+}
+
+// The parts of a row, one workgroup a row.
+template <typename T, bool CAP, bool TOP>
+__global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out,
+                                                        const uint64_t* __restrict__ part_top, const Stat* __restrict__ part_stat, int V, int64_t ld,
+                                                        int32_t ignore_index, Scale c, int k, int parts) {
+  __shared__ uint64_t cand[JOINED];
+  __shared__ alignas(16) unsigned best[TH];
+  __shared__ Stat red[TH / 64];
+  __shared__ int counter;
+  const int64_t row = blockIdx.x;
+  const int target = targets ? targets[row] : -1;
+  if (targets && target == ignore_index) {
+    write_skipped(out, row, k);
+    return;
+  }
+  Stat a = Stat::none();
+  if ((int)threadIdx.x < parts) a = part_stat[row * parts + threadIdx.x];
+  uint64_t most = 0;
+  if (TOP)
+    for (int i = threadIdx.x; i < parts * k; i += TH) {
+      const uint64_t e = part_top[row * parts * k + i];
+      cand[i] = e;
+      most = max(most, e);
+    }
+  a = block_join<TH / 64>(a, red);
+  write_row<T, CAP>(out, row, logits + row * ld, target, V, c, a);
+  if (TOP) {
+    const unsigned bound = kth_best(best, max((unsigned)(most >> 32), KEY_NEG_INF), k);
+    const int n = narrow<JOINED>(cand, parts * k, bound, &counter);
+    write_top<CAP>(out, row, k, cand, n, c, a);
+  }
+}
+
+// d loss / d logits of logprob and entropy: dz_i = g (delta_it - p_i) - h p_i (ln p_i + H), from the statistics that the forward pass kept.
+// A workgroup takes one of `parts` shares of a row.
+template <typename T, typename TO, bool CAP, bool ENT>
+__global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const int32_t* __restrict__ targets,
+                                                        const float* __restrict__ stats, const float* __restrict__ dlogprobs,
+                                                        const float* __restrict__ dentropy, int V, int64_t ld, int64_t ldd, int32_t ignore_index, Scale c,
+                                                        int parts, int pad) {
+  constexpr int N = Vec<TO>::N;
+  const int64_t row = blockIdx.x / parts;
+  const int part = blockIdx.x % parts;
+  const T* zr = logits + row * ld;
+  TO* dr = dlogits + row * ldd;
+  const Cut cutting = cut<TO, N>(dr, V);
+  const int per = (cutting.nvec + parts - 1) / parts;
+  const int v0 = min(part * per, cutting.nvec), v1 = min(v0 + per, cutting.nvec);
+  const int target = targets[row];
+  const float m = stats[row * 3], log_sum = stats[row * 3 + 1], entropy = stats[row * 3 + 2];
+  const bool skipped = target == ignore_index || m == -INFINITY;  // no distribution: no gradient
+  const float g = skipped || target < 0 || target >= V ? 0.f : dlogprobs[row], h = skipped || !ENT ? 0.f : dentropy[row];
+  auto grad = [&](float x, int i) {
+    float chain = c.inv_tau, y = x;
+    if (CAP) {
+      const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f);
+      y = c.cap * t;
+      chain *= 1.f - t * t;
+    }
+    const float logp = __builtin_fmaf(y, c.inv_tau, -m) - log_sum;
+    const float p = exp_of(logp);
+    float d = -p * (ENT ? __builtin_fmaf(h, fmaxf(logp, -200.f) + entropy, g) : g);
+    if (i == target) d += g;
+    return d * chain;
+  };
+  for (int v = v0 + threadIdx.x; v < v1; v += TH) {
+    float x[N];
+    const int i = cutting.head + v * N;
+    if (!skipped) {
+      Raw<T, N> r;
+      r.load(zr + i);
+      r.unpack(x);
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) x[e] = skipped ? 0.f : grad(x[e], i + e);
+    *reinterpret_cast<u32x4*>(dr + i) = Vec<TO>::pack(x);
+  }
+  if (part == 0 && (int)threadIdx.x < cutting.edges) {
+    const int i = cutting.edge(threadIdx.x, V);
+    dr[i] = (TO)(skipped ? 0.f : grad((float)zr[i], i));
+  }
+  if (part == 0 && (int)threadIdx.x < pad) dr[V + threadIdx.x] = (TO)0.f;
+}
+
+Scale scale_of(float temperature, float softcap) {
+  Scale c;
+  c.cap = softcap;
+  c.cap_k = softcap > 0.f ? 2.f * LOG2E / softcap : 0.f;
+  c.inv_tau = 1.f / temperature;
+  return c;
+}
+
+// Shares of a row in the forward pass: rows that fill the GPU by themselves are whole.
+int parts_of(int64_t T, int V, int top, bool f32) {
+  const int64_t vecs = V / (f32 ? 4 : 8);
+  int64_t p = std::min<int64_t>(1024 / T, vecs / (TH * 2));
+  if (top > 0) p = std::min<int64_t>(p, JOINED / top);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(p, 64));
+}
+
+}  // namespace
+
+extern "C" int64_t olmax_token_logprobs_workspace_bytes(int64_t T, int32_t V, int32_t top, int32_t logits_f32) {
+  if (T <= 0 || V <= 0) return 0;
+  const int parts = parts_of(T, V, top, logits_f32 != 0);
+  return parts == 1 ? 0 : T * parts * ((int64_t)std::max(top, 0) * 8 + (int64_t)sizeof(Stat));
+}
+
+extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, const int32_t* targets, float* logprobs, float* entropy, float* stats,
+                                        int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes, int64_t T, int32_t V,
+                                        int64_t ld, int32_t top, int32_t logits_f32, int32_t ignore_index, float temperature, float softcap) {
+  OLMAX_CHECK(logits && entropy && stats && (!logprobs || targets), OLMAX_ERR_ARG, "olmax_token_logprobs: null pointer");
+  OLMAX_CHECK(T > 0 && V > 0 && ld >= V && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_token_logprobs: bad shape T=%ld V=%d ld=%ld", (long)T, V, (long)ld);
+  OLMAX_CHECK(top >= 0 && top <= MAX_TOP && top <= V && (top == 0 || (top_ids && top_logprobs)), OLMAX_ERR_ARG,
+              "olmax_token_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, top);
+  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_token_logprobs: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(((uintptr_t)logits & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_token_logprobs: logits not aligned to their type");
+  const int parts = parts_of(T, V, top, logits_f32 != 0);
+  OLMAX_CHECK(workspace_bytes >= olmax_token_logprobs_workspace_bytes(T, V, top, logits_f32) && (parts == 1 || (workspace && aligned16(workspace))), OLMAX_ERR_WORKSPACE,
+              "olmax_token_logprobs: workspace needs %ld bytes, 16-byte aligned", (long)olmax_token_logprobs_workspace_bytes(T, V, top, logits_f32));
+  uint64_t* part_top = (uint64_t*)workspace;
+  Stat* part_stat = (Stat*)((char*)workspace + (parts == 1 ? 0 : T * parts * (int64_t)top * 8));
+  const Out out{logprobs, entropy, stats, top ? top_logprobs : nullptr, top ? top_ids : nullptr};
+  const Scale c = scale_of(temperature, softcap);
+#define SCORE(TY, CAPV, TOPV)                                                                                                                             \
+  do {                                                                                                                                                    \
+    hipLaunchKernelGGL((score_rows_kernel<TY, CAPV, TOPV>), dim3((unsigned)(T * parts)), dim3(TH), 0, stream, (const TY*)logits, targets, out, part_top, \
+                       part_stat, V, ld, ignore_index, c, top, parts);                                                                                    \
+    if (parts > 1)                                                                                                                                        \
+      hipLaunchKernelGGL((score_join_kernel<TY, CAPV, TOPV>), dim3((unsigned)T), dim3(TH), 0, stream, (const TY*)logits, targets, out,                    \
+                         (const uint64_t*)part_top, (const Stat*)part_stat, V, ld, ignore_index, c, top, parts);                                          \
+  } while (0)
+#define SCORE_T(TY, CAPV) do { if (top) SCORE(TY, CAPV, true); else SCORE(TY, CAPV, false); } while (0)
+#define SCORE_C(TY) do { if (softcap > 0.f) SCORE_T(TY, true); else SCORE_T(TY, false); } while (0)
+  if (logits_f32) SCORE_C(float); else SCORE_C(bf16);
+#undef SCORE
+#undef SCORE_T
+#undef SCORE_C
+  OLMAX_LAUNCH_CHECK();
+  return OLMAX_OK;
+}
+
+// grads_bf16: the gradient of fp32 logits as bf16 (the LM head's products take it); pad: zeros behind each of its rows
+static int token_logprobs_bwd(hipStream_t stream, const void* logits, const int32_t* targets, const float* stats, const float* dlogprobs,
+                              const float* dentropy, void* dlogits, int64_t T, int32_t V, int64_t ld, int64_t ldd, bool logits_f32, bool grads_f32,
+                              int32_t ignore_index, float temperature, float softcap, int pad) {
+  const Scale c = scale_of(temperature, softcap);
+  const int parts = (int)std::max<int64_t>(1, V / (grads_f32 ? 4 : 8) / (TH * 8));
+  OLMAX_CHECK(T * parts < (1LL << 31), OLMAX_ERR_SHAPE, "olmax_token_logprobs_bwd: T=%ld rows of V=%d are too many", (long)T, V);
+#define GRAD(TY, TO, CAPV, ENTV)                                                                                                                             \
+  hipLaunchKernelGGL((score_grad_kernel<TY, TO, CAPV, ENTV>), dim3((unsigned)(T * parts)), dim3(TH), 0, stream, (const TY*)logits, (TO*)dlogits, targets, stats, \
+                     dlogprobs, dentropy, V, ld, ldd, ignore_index, c, parts, pad)
+#define GRAD_E(TY, TO, CAPV) do { if (dentropy) GRAD(TY, TO, CAPV, true); else GRAD(TY, TO, CAPV, false); } while (0)
+#define GRAD_C(TY, TO) do { if (softcap > 0.f) GRAD_E(TY, TO, true); else GRAD_E(TY, TO, false); } while (0)
+  if (logits_f32 && grads_f32) GRAD_C(float, float); else if (logits_f32) GRAD_C(float, bf16); else GRAD_C(bf16, bf16);
+#undef GRAD
+#undef GRAD_E
+#undef GRAD_C
+  OLMAX_LAUNCH_CHECK();
+  return OLMAX_OK;
+}
+
+extern "C" int32_t olmax_token_logprobs_bwd(hipStream_t stream, const void* logits, const int32_t* targets, const float* stats, const float* dlogprobs,
+                                            const float* dentropy, void* dlogits, int64_t T, int32_t V, int64_t ld, int64_t ldd, int32_t logits_f32,
+                                            int32_t ignore_index, float temperature, float softcap) {
+  OLMAX_CHECK(logits && targets && stats && dlogprobs && dlogits, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: null pointer");
+  OLMAX_CHECK(T > 0 && V > 0 && ld >= V && ldd >= V && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_token_logprobs_bwd: bad shape T=%ld V=%d", (long)T, V);
+  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK((((uintptr_t)logits | (uintptr_t)dlogits) & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_token_logprobs_bwd: operands not aligned to their type");
+  OLMAX_CHECK(logits != dlogits || ld == ldd, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: in place wants one row stride");
+  return token_logprobs_bwd(stream, logits, targets, stats, dlogprobs, dentropy, dlogits, T, V, ld, ldd, logits_f32 != 0, logits_f32 != 0, ignore_index,
+                            temperature, softcap, 0);
+}
+
+// ---- with the LM head's product.  The logits are fp32 in the workspace: the framework's bf16 ones are off by 2^-9 of themselves, as much in a
+// log probability as policies of two steps may be apart.
+static int64_t head_stride(int32_t V) { return ((int64_t)V + 63) / 64 * 64; }  // whole lines of bf16 and fp32
+static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+extern "C" int64_t olmax_lmhead_logprobs_workspace_bytes(int64_t T, int32_t d, int32_t V, int32_t top) {
+  if (T <= 0 || V <= 0) return 0;
+  return up256(T * head_stride(V) * 4) + olmax_token_logprobs_workspace_bytes(T, V, top, 1);
+}
+
+extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, const void* W, const int32_t* targets, float* logprobs, float* entropy,
+                                         float* stats, int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes, int64_t T,
+                                         int32_t d, int32_t V, int32_t top, int32_t ignore_index, float temperature, float softcap) {
+  OLMAX_CHECK(h && W && workspace, OLMAX_ERR_ARG, "olmax_lmhead_logprobs: null pointer");
+  OLMAX_CHECK(T > 0 && d > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs: bad shape T=%ld d=%d V=%d", (long)T, d, V);
+  OLMAX_CHECK(workspace_bytes >= olmax_lmhead_logprobs_workspace_bytes(T, d, V, top) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
+              "olmax_lmhead_logprobs: workspace needs %ld bytes, 256-byte aligned", (long)olmax_lmhead_logprobs_workspace_bytes(T, d, V, top));
+  const int64_t ld = head_stride(V), at = up256(T * ld * 4);
+  // (the arguments of the rows are checked before the product is launched)
+  OLMAX_CHECK(entropy && stats && (!logprobs || targets) && top >= 0 && top <= MAX_TOP && top <= V && (top == 0 || (top_ids && top_logprobs)) && temperature >= 1e-6f &&
+                  temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG,
+              "olmax_lmhead_logprobs: wants entropy and stats, targets for logprobs, 0 to %d alternatives, a temperature within 1e-6 and 1e6, a softcap that is not negative", MAX_TOP);
+  if (int rc = olmax_gemm_padded(stream, (const bf16*)h, (const bf16*)W, workspace, nullptr, (int)T, V, d, d, d, ld, 0, true, true, true, false)) return rc;
+  return olmax_token_logprobs(stream, workspace, targets, logprobs, entropy, stats, top_ids, top_logprobs, (char*)workspace + at, workspace_bytes - at, T, V,
+                              ld, top, 1, ignore_index, temperature, softcap);
+}
+
+extern "C" int64_t olmax_lmhead_logprobs_bwd_workspace_bytes(int64_t T, int32_t d, int32_t V) {
+  if (T <= 0 || V <= 0) return 0;
+  return up256(T * head_stride(V) * 4) + up256(T * head_stride(V) * 2);
+}
+
+extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, const void* W, const int32_t* targets, const float* stats,
+                                             const float* dlogprobs, const float* dentropy, void* dh, void* dW, void* workspace, int64_t workspace_bytes,
+                                             int64_t T, int32_t d, int32_t V, int32_t ignore_index, float temperature, float softcap, int32_t dw_f32) {
+  OLMAX_CHECK(h && W && targets && stats && dlogprobs && workspace && (dh || dW), OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: null pointer");
+  OLMAX_CHECK(T > 0 && d > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs_bwd: bad shape T=%ld d=%d V=%d", (long)T, d, V);
+  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(workspace_bytes >= olmax_lmhead_logprobs_bwd_workspace_bytes(T, d, V) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
+              "olmax_lmhead_logprobs_bwd: workspace needs %ld bytes, 256-byte aligned", (long)olmax_lmhead_logprobs_bwd_workspace_bytes(T, d, V));
+  const int64_t ld = head_stride(V);
+  const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
+  bf16* grads = (bf16*)((char*)workspace + up256(T * ld * 4));
+  if (int rc = olmax_gemm_padded(stream, hp, wp, workspace, nullptr, (int)T, V, d, d, d, ld, 0, true, true, true, false)) return rc;
+  if (int rc = token_logprobs_bwd(stream, workspace, targets, stats, dlogprobs, dentropy, grads, T, V, ld, ld, true, false, ignore_index, temperature, softcap,
+                                  (8 - V % 8) % 8))
+    return rc;
+  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0);
+}

@@ -1,0 +1,127 @@
+// What the kernels on rows of logits share that are neither the cross entropy's nor bound to whole vectors: scores, streaming
+// softmax statistics, 16-byte access to rows of any alignment.
+//
+// Scores z = cap(x) / temperature, cap(x) = softcap * tanh(x / softcap) or x.  A thread's statistics are of what it has seen:
+//   m   largest score (the reference that exponentials are taken against), s = sum exp(z - m), t = sum exp(z - m) (z - m)
+// so that ln sum exp z = m + ln s, and the entropy of softmax(z) is ln s - t / s.  Everything is fp32.  z - m is formed by one fma from the
+// logit, so that rows at the type's lowest value or about 1e30 are exact where scores near the largest are; a score of minus infinity has
+// exp = 0 and adds nothing to t (z - m is cut at -200, where exp is 0 in fp32).
+#pragma once
+#include "common.h"
+
+namespace rows {
+
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;  // 16 bytes at any element
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// 16 bytes of a row as numbers
+template <typename T> struct Vec;
+template <> struct Vec<bf16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const u32x4& w, float* f) {
+    Pack8 t;
+    t.u = w;
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = bf2f(t.e[e]);
+  }
+  static __device__ __forceinline__ u32x4 pack(const float* f) {
+    Pack8 t;
+#pragma unroll
+    for (int e = 0; e < 8; e++) t.e[e] = f2bf(f[e]);
+    return t.u;
+  }
+};
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const u32x4& w, float* f) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) f[e] = __uint_as_float(w[e]);
+  }
+  static __device__ __forceinline__ u32x4 pack(const float* f) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = __float_as_uint(f[e]);
+    return w;
+  }
+};
+// N numbers of a row as they are loaded: 16 or (N fp32 numbers for 16 bytes of bf16) 32 bytes
+template <typename T, int N> struct Raw {
+  static constexpr int W = N / Vec<T>::N;
+  u32x4 w[W];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = *reinterpret_cast<const u32x4_any*>(p + i * Vec<T>::N);
+  }
+  __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+    for (int i = 0; i < W; i++) Vec<T>::unpack(w[i], f + i * Vec<T>::N);
+  }
+};
+
+// A row of n elements as `head` single ones, nvec vectors of N that begin at 16-byte boundaries of T, and the rest
+struct Cut {
+  int head, nvec, edges;  // edges: head and rest
+  __device__ __forceinline__ int edge(int e, int n) const { return e < head ? e : n - (edges - e); }  // element of edge e
+};
+template <typename T, int N> __device__ __forceinline__ Cut cut(const T* row, int n) {
+  Cut c;
+  c.head = min(n, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T));
+  c.nvec = (n - c.head) / N;
+  c.edges = n - c.nvec * N;
+  return c;
+}
+
+struct Scale {
+  float cap, cap_k, inv_tau;  // cap_k = 2 log2(e) / cap
+};
+template <bool CAP> __device__ __forceinline__ float capped(float x, const Scale& c) {
+  return CAP ? c.cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f)) : x;
+}
+template <bool CAP> __device__ __forceinline__ float score(float x, const Scale& c) { return capped<CAP>(x, c) * c.inv_tau; }
+// z - m
+template <bool CAP> __device__ __forceinline__ float behind(float x, const Scale& c, float m) { return __builtin_fmaf(capped<CAP>(x, c), c.inv_tau, -m); }
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
+__device__ __forceinline__ float log_of(float s) { return __builtin_amdgcn_logf(s) * LN2; }
+
+// Statistics of what a thread has seen; m = -inf: nothing above minus infinity yet.
+struct Stat {
+  float m, s, t;
+  static __device__ __forceinline__ Stat none() { return Stat{-INFINITY, 0.f, 0.f}; }
+  __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }  // against which every exponential of such a thread is 0
+  // the largest score is m2 now
+  __device__ __forceinline__ void raise(float m2) {
+    if (m != -INFINITY) {
+      const float d = m - m2, f = exp_of(d);
+      t = f * (t + s * fmaxf(d, -200.f));
+      s *= f;
+    }
+    m = m2;
+  }
+  __device__ __forceinline__ void join(const Stat& o) {
+    Stat b = o;
+    if (b.m > m) raise(b.m);
+    else if (m > b.m) b.raise(m);
+    s += b.s;
+    t += b.t;
+  }
+};
+template <int NW> __device__ __forceinline__ Stat block_join(Stat a, Stat* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    Stat b;
+    b.m = __shfl_xor(a.m, o, 64);
+    b.s = __shfl_xor(a.s, o, 64);
+    b.t = __shfl_xor(a.t, o, 64);
+    a.join(b);
+  }
+  if (NW == 1) return a;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+  __syncthreads();
+  a = red[0];
+#pragma unroll
+  for (int i = 1; i < NW; i++) a.join(red[i]);
+  return a;
+}
+
+}  // namespace rows

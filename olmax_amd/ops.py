@@ -8,7 +8,7 @@ operands may be row-strided views (stride(1) must be 1).
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -312,6 +312,196 @@ def lmhead_ce(h, W, labels, *, softcap: float = 0.0, ignore_index: int = -100, w
     check(L.olmax_lmhead_ce(stream_ptr(), ptr(h), ptr(W), ptr(labels), ptr(loss), ptr(dh), ptr(dW), ptr(ws),
                             i64(nbytes), i64(T), i32(d), i32(V), i32(ignore_index), f32(softcap),
                             i32(1 if (dW is not None and dW.dtype == torch.float32) else 0)))
+    return loss, dh, dW
+
+
+# ----------------------------------------------------------------------------- log probabilities, distillation
+class TokenLogprobs(NamedTuple):
+    """What a row's softmax says: log probability of its target (None without targets), entropy, statistics for the backward call
+    ([T, 3]: largest score, log of the sum of exponentials behind it, entropy), and the alternatives [T, top] (None without)."""
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    stats: torch.Tensor
+    top_logprobs: Optional[torch.Tensor]
+    top_ids: Optional[torch.Tensor]
+
+
+_TAIL = {"renormalize": 0, "bucket": 1}
+_sizes = {}
+
+
+def _want(ok, what: str):
+    if not ok:
+        raise _lib.OlmaxHipError(what)
+
+
+def _size(name: str, *args) -> int:
+    """A workspace query of the library."""
+    f = _sizes.get(name)
+    if f is None:
+        f = getattr(_L(), name)
+        f.restype, f.argtypes = i64, [i64] + [i32] * (len(args) - 1)
+        _sizes[name] = f
+    return f(*args)
+
+
+def _place(*ts):
+    """GPU tensors of the current device, whose stream the call is enqueued on."""
+    _need_gpu(*ts)
+    here = torch._C._cuda_getDevice()
+    for t in ts:
+        _want(t is None or t.device.index == here, "olmax_amd ops: a tensor is on another GPU than the current one")
+
+
+def _logits(t, like=None):
+    _want(t.dim() == 2 and t.stride(1) == 1 and t.dtype in (BF16, torch.float32), "expected logits [T, V] in bf16 or fp32 with contiguous rows")
+    _want(t.stride(0) >= t.shape[1] or t.shape[0] == 1, "rows of logits overlap")
+    _want(like is None or (t.shape == like.shape and t.dtype == like.dtype), "gradients have the shape and type of the logits")
+    return t, max(t.stride(0), t.shape[1])
+
+
+def _row_of(t, T: int, what: str, dtype=torch.float32):
+    _want(t is None or (t.dtype == dtype and t.shape == (T,) and t.is_contiguous()), f"{what}: expected a contiguous {dtype} tensor [{T}]")
+    return None if t is None else t.data_ptr()
+
+
+def _head(h, W):
+    _want(h.dim() == 2 and W.dim() == 2 and h.is_contiguous() and W.is_contiguous() and h.dtype == BF16 and W.dtype == BF16 and h.shape[1] == W.shape[1],
+          "expected contiguous bf16 hidden states [T, d] and LM head [V, d]")
+    return h.shape[0], h.shape[1], W.shape[0]
+
+
+def _teacher(top_ids, top_logprobs, T: int) -> int:
+    _want(top_ids.dim() == 2 and top_ids.shape[0] == T and top_ids.dtype == torch.int32 and top_ids.is_contiguous(), "top_ids: expected a contiguous int32 tensor [T, k]")
+    _want(top_logprobs.shape == top_ids.shape and top_logprobs.dtype == torch.float32 and top_logprobs.is_contiguous(),
+          "top_logprobs: expected a contiguous fp32 tensor of top_ids' shape")
+    return top_ids.shape[1]
+
+
+def _tail(tail: str) -> int:
+    _want(tail in _TAIL, f"tail must be 'renormalize' or 'bucket' (got {tail!r})")
+    return _TAIL[tail]
+
+
+def _outputs(T: int, targets, top: int, like):
+    new = lambda *shape: torch.empty(shape, device=like.device, dtype=torch.float32)  # noqa: E731
+    _row_of(targets, T, "targets", torch.int32)
+    _want(top >= 0, "top must not be negative")
+    ids = torch.empty((T, top), device=like.device, dtype=torch.int32) if top else None
+    return TokenLogprobs(None if targets is None else new(T), new(T), new(T, 3), new(T, top) if top else None, ids)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def token_logprobs(logits, targets=None, *, top: int = 0, temperature: float = 1.0, softcap: float = 0.0, ignore_index: int = -100) -> TokenLogprobs:
+    """Log probabilities of targets [T] int32 under the softmax of cap(logits) / temperature, cap(x) = softcap * tanh(x / softcap), the entropy of each row,
+    and its `top` (up to 128) most likely tokens in order (ties to the lowest index) with their log probabilities.
+
+    logits [T, V] bf16 or fp32, any row stride.  Rows whose target is ignore_index are not read: zeros, ids -1, log probabilities of the
+    alternatives minus infinity.  A target outside [0, V) has log probability 0 and no gradient, as in cross_entropy."""
+    _place(logits, targets)
+    logits, ld = _logits(logits)
+    T, V = logits.shape
+    r = _outputs(T, targets, top, logits)
+    f32_ = 1 if logits.dtype == torch.float32 else 0
+    nbytes = _size("olmax_token_logprobs_workspace_bytes", T, V, top, f32_)
+    ws = torch.empty(nbytes, device=logits.device, dtype=torch.uint8) if nbytes else None
+    check(typed("olmax_token_logprobs")(raw_stream(), logits.data_ptr(), _ptr(targets), _ptr(r.logprobs), r.entropy.data_ptr(), r.stats.data_ptr(), _ptr(r.top_ids),
+                                        _ptr(r.top_logprobs), _ptr(ws), nbytes, T, V, ld, top, f32_, ignore_index, temperature, softcap))
+    return r
+
+
+def token_logprobs_bwd(logits, targets, stats, dlogprobs, *, dentropy=None, temperature: float = 1.0, softcap: float = 0.0, ignore_index: int = -100,
+                       inplace: bool = False, out=None):
+    """d / d logits of sum(dlogprobs * logprobs) + sum(dentropy * entropy), from the stats that token_logprobs returned for the same logits.  `inplace`
+    overwrites the logits."""
+    _place(logits, targets, stats, dlogprobs, dentropy, out)
+    logits, ld = _logits(logits)
+    T, V = logits.shape
+    _want(stats.dtype == torch.float32 and stats.shape == (T, 3) and stats.is_contiguous(), f"stats: expected a contiguous fp32 tensor [{T}, 3]")
+    if out is None:
+        out = logits if inplace else torch.empty((T, V), device=logits.device, dtype=logits.dtype)
+    out, ldd = _logits(out, logits)
+    check(typed("olmax_token_logprobs_bwd")(raw_stream(), logits.data_ptr(), _row_of(targets, T, "targets", torch.int32), stats.data_ptr(),
+                                            _row_of(dlogprobs, T, "dlogprobs"), _row_of(dentropy, T, "dentropy"), out.data_ptr(), T, V, ld, ldd,
+                                            1 if logits.dtype == torch.float32 else 0, ignore_index, temperature, softcap))
+    return out
+
+
+def distill(logits, top_ids, top_logprobs, *, tail: str = "renormalize", temperature: float = 1.0, softcap: float = 0.0, want_grad: bool = True,
+            inplace: bool = False, dloss: float = 1.0, reduction: str = "mean", dloss_rows=None):
+    """Divergence KL(teacher || student) from a teacher's k (up to 128) best tokens: top_ids [T, k] int32 and top_logprobs [T, k] fp32 as token_logprobs(top=k)
+    returns them.  Returns (loss, dlogits or None), loss a scalar, or [T] for reduction "none".
+
+    tail "renormalize": the teacher is softmax(top_logprobs / temperature) over its k tokens (logits do as well).  "bucket": its
+    probabilities are exp(top_logprobs), and the other tokens are one event with the rest.  The student is softmax(cap(logits) / temperature).  Rows whose
+    first id is negative are left out; other ids outside [0, V) and repeated ones are dropped.  Softened losses are commonly weighted by
+    temperature ** 2: dloss scales the gradient (not the loss), per row dloss_rows with reduction "none"."""
+    _place(logits, top_ids, top_logprobs, dloss_rows)
+    logits, ld = _logits(logits)
+    T, V = logits.shape
+    k = _teacher(top_ids, top_logprobs, T)
+    _want(reduction in ("mean", "sum", "none"), f"unknown reduction {reduction!r}")
+    red = ("mean", "sum", "none").index(reduction)
+    nbytes = _size("olmax_distill_workspace_bytes", T)
+    ws = torch.empty(nbytes, device=logits.device, dtype=torch.uint8)
+    loss = torch.empty((T,) if red == 2 else (), device=logits.device, dtype=torch.float32)
+    d, ldd = None, 0
+    if want_grad:
+        d = logits if inplace else torch.empty((T, V), device=logits.device, dtype=logits.dtype)
+        d, ldd = _logits(d)
+    check(typed("olmax_distill")(raw_stream(), logits.data_ptr(), _ptr(d), top_ids.data_ptr(), top_logprobs.data_ptr(), loss.data_ptr(),
+                                 _row_of(dloss_rows, T, "dloss_rows"), ws.data_ptr(), nbytes, T, V, k, ld, ldd, 1 if logits.dtype == torch.float32 else 0, _tail(tail),
+                                 temperature, softcap, dloss, red))
+    return loss, d
+
+
+def lmhead_logprobs(h, W, targets=None, *, top: int = 0, temperature: float = 1.0, softcap: float = 0.0, ignore_index: int = -100) -> TokenLogprobs:
+    """token_logprobs of h W^T (h [T, d], W [V, d] bf16), summed and kept in fp32."""
+    _place(h, W, targets)
+    T, d, V = _head(h, W)
+    r = _outputs(T, targets, top, h)
+    nbytes = _size("olmax_lmhead_logprobs_workspace_bytes", T, d, V, top)
+    ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
+    check(typed("olmax_lmhead_logprobs")(raw_stream(), h.data_ptr(), W.data_ptr(), _ptr(targets), _ptr(r.logprobs), r.entropy.data_ptr(), r.stats.data_ptr(),
+                                         _ptr(r.top_ids), _ptr(r.top_logprobs), ws.data_ptr(), nbytes, T, d, V, top, ignore_index, temperature, softcap))
+    return r
+
+
+def _head_grads(h, W, want_dh: bool, want_dw: bool, dw_f32: bool):
+    dh = torch.empty_like(h) if want_dh else None
+    return dh, torch.empty(W.shape, device=h.device, dtype=torch.float32 if dw_f32 else BF16) if want_dw else None
+
+
+def lmhead_logprobs_bwd(h, W, targets, stats, dlogprobs, *, dentropy=None, temperature: float = 1.0, softcap: float = 0.0, ignore_index: int = -100,
+                        want_dh: bool = True, want_dw: bool = True, dw_f32: bool = False):
+    """Gradients of lmhead_logprobs (see token_logprobs_bwd): returns (dh, dW).  The logits are formed again."""
+    _place(h, W, targets, stats, dlogprobs, dentropy)
+    T, d, V = _head(h, W)
+    _want(stats.dtype == torch.float32 and stats.shape == (T, 3) and stats.is_contiguous(), f"stats: expected a contiguous fp32 tensor [{T}, 3]")
+    nbytes = _size("olmax_lmhead_logprobs_bwd_workspace_bytes", T, d, V)
+    ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
+    dh, dW = _head_grads(h, W, want_dh, want_dw, dw_f32)
+    check(typed("olmax_lmhead_logprobs_bwd")(raw_stream(), h.data_ptr(), W.data_ptr(), _row_of(targets, T, "targets", torch.int32), stats.data_ptr(),
+                                             _row_of(dlogprobs, T, "dlogprobs"), _row_of(dentropy, T, "dentropy"), _ptr(dh), _ptr(dW), ws.data_ptr(), nbytes, T, d, V,
+                                             ignore_index, temperature, softcap, 1 if dw_f32 else 0))
+    return dh, dW
+
+
+def lmhead_distill(h, W, top_ids, top_logprobs, *, tail: str = "renormalize", temperature: float = 1.0, softcap: float = 0.0, dloss: float = 1.0,
+                   want_dh: bool = True, want_dw: bool = True, dw_f32: bool = False):
+    """distill (reduction "mean") of h W^T, forward and backward in one call as lmhead_ce: returns (loss, dh, dW)."""
+    _place(h, W, top_ids, top_logprobs)
+    T, d, V = _head(h, W)
+    k = _teacher(top_ids, top_logprobs, T)
+    nbytes = _size("olmax_lmhead_distill_workspace_bytes", T, d, V)
+    ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
+    loss = torch.empty((), device=h.device, dtype=torch.float32)
+    dh, dW = _head_grads(h, W, want_dh, want_dw, dw_f32)
+    check(typed("olmax_lmhead_distill")(raw_stream(), h.data_ptr(), W.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(), loss.data_ptr(), _ptr(dh), _ptr(dW),
+                                        ws.data_ptr(), nbytes, T, d, V, k, _tail(tail), temperature, softcap, dloss, 1 if dw_f32 else 0))
     return loss, dh, dW
 
 

@@ -298,6 +298,123 @@ def lm_head_ce(h: Tensor, w: Tensor, labels: Tensor, *, softcap: float = 0.0, rt
 
 
 # --------------------------------------------------------------------------- embedding
+def token_scores(logits: Tensor, temperature: float = 1.0, softcap: float = 0.0) -> Tensor:
+    """cap(logits) / temperature in the logits' own precision.  (No counterpart in the reference, as all up to distill_bwd.)"""
+    return (softcap * torch.tanh(logits / softcap) if softcap > 0 else logits) / temperature
+
+
+def _log_softmax(z: Tensor) -> Tensor:
+    """The largest score is taken off first: behind a row of the type's lowest value even 64 bits have no room for a logarithm."""
+    z = z - z.max(1, keepdim=True).values
+    return z - torch.logsumexp(z, 1, keepdim=True)
+
+
+def token_logprobs_fwd(logits: Tensor, targets: Optional[Tensor] = None, *, top: int = 0, temperature: float = 1.0, softcap: float = 0.0,
+                       ignore_index: int = -100):
+    """(logprobs, entropy, top_logprobs, top_ids) of each row.  Top tokens by the logit itself, ties to the lowest index, minus infinity (and NaN) last.  Rows of an
+    ignored target: zeros, ids -1, minus infinity; a row of minus infinities has no distribution: entropy 0, log probabilities of minus infinity."""
+    T, V = logits.shape
+    z = token_scores(logits, temperature, softcap)
+    none = (z == -math.inf).all(1)
+    logp = torch.where(none[:, None], -math.inf, _log_softmax(z))
+    p = logp.exp()
+    entropy = -torch.where(p == 0, torch.zeros_like(p), p * logp).sum(1)
+    lp = None
+    skip = torch.zeros(T, dtype=torch.bool)
+    if targets is not None:
+        inside = (targets >= 0) & (targets < V)
+        lp = torch.where(inside, logp.gather(1, targets.clamp(0, V - 1).long()[:, None])[:, 0], torch.zeros_like(entropy))
+        skip = targets == ignore_index
+        lp = torch.where(skip, torch.zeros_like(lp), lp)
+    entropy = torch.where(skip, torch.zeros_like(entropy), entropy)
+    ids = torch.sort(torch.nan_to_num(logits, nan=-math.inf, posinf=math.inf, neginf=-math.inf), dim=1, descending=True, stable=True).indices[:, :top]
+    best = torch.where(skip[:, None], -math.inf, logp.gather(1, ids))
+    return lp, entropy, best, torch.where(skip[:, None], -1, ids)
+
+
+def token_logprobs_bwd(logits: Tensor, targets: Tensor, dlogprobs: Tensor, dentropy: Optional[Tensor] = None, *, temperature: float = 1.0, softcap: float = 0.0,
+                       ignore_index: int = -100) -> Tensor:
+    """dz_i = g (delta_it - p_i) - h p_i (ln p_i + H), times dz / dx."""
+    T, V = logits.shape
+    z = token_scores(logits, temperature, softcap)
+    none = (z == -math.inf).all(1)
+    logp = _log_softmax(z)
+    p = torch.where(none[:, None], 0.0, logp.exp())
+    plogp = torch.where(p == 0, torch.zeros_like(p), p * logp)
+    skip = (targets == ignore_index) | none
+    inside = (targets >= 0) & (targets < V) & ~skip
+    g = torch.where(inside, dlogprobs, torch.zeros_like(dlogprobs))[:, None]
+    h = torch.zeros_like(g) if dentropy is None else torch.where(skip, torch.zeros_like(dentropy), dentropy)[:, None]
+    d = -g * p - h * (plogp - p * plogp.sum(1, keepdim=True))
+    d = d.scatter_add(1, targets.clamp(0, V - 1).long()[:, None], g)
+    if softcap > 0:
+        d = d * (1 - torch.tanh(logits / softcap) ** 2)
+    return d / temperature
+
+
+def _teacher(ids: Tensor, t: Tensor, V: int, tail: str, temperature: float):
+    """q of each of the k entries (0 for those that are dropped), ln q, r, which entries count."""
+    k = ids.shape[1]
+    ok = (ids >= 0) & (ids < V)
+    again = (ids[:, :, None] == ids[:, None, :]) & torch.tril(torch.ones(k, k, dtype=torch.bool), -1)
+    ok = ok & ~again.any(2)
+    if tail == "renormalize":
+        logq = torch.log_softmax(torch.where(ok, t / temperature, -math.inf), 1)
+        q = torch.where(ok, logq.exp(), 0.0)
+        return q, logq, torch.zeros_like(q[:, 0]), ok
+    q = torch.where(ok, t.exp(), 0.0)
+    r = 1 - q.sum(1)
+    return q, t, torch.where(r < 2.0 ** -20, torch.zeros_like(r), r), ok
+
+
+def distill_fwd(logits: Tensor, top_ids: Tensor, top_logprobs: Tensor, *, tail: str = "renormalize", temperature: float = 1.0, softcap: float = 0.0,
+                reduction: str = "mean") -> Tensor:
+    """sum_j q_j ln(q_j / p_j) (+ r ln(r / s) of the other tokens together); rows whose first id is negative count nowhere."""
+    T, V = logits.shape
+    ids = top_ids.long()
+    q, logq, r, ok = _teacher(ids, top_logprobs, V, tail, temperature)
+    z = token_scores(logits, temperature, softcap)
+    none = (z == -math.inf).all(1)
+    logp = _log_softmax(z)
+    at = ids.clamp(0, V - 1)
+    per = torch.where(q > 0, q * (logq - logp.gather(1, at)), torch.zeros_like(q)).sum(1)
+    if tail == "bucket":
+        hidden = torch.zeros(T, V + 1, dtype=torch.bool).scatter(1, torch.where(ok, at, V), True)[:, :V]  # (V: nowhere)
+        log_s = torch.logsumexp(torch.where(hidden, -math.inf, logp), 1)
+        per = per + torch.where(r > 0, r * (r.log() - log_s), torch.zeros_like(r))
+    kept = ids[:, 0] >= 0
+    per = torch.where(kept & ~none, per, torch.zeros_like(per))
+    if reduction == "none":
+        return per
+    return per.sum() / (kept.sum().clamp(min=1) if reduction == "mean" else 1)
+
+
+def distill_bwd(logits: Tensor, top_ids: Tensor, top_logprobs: Tensor, *, tail: str = "renormalize", temperature: float = 1.0, softcap: float = 0.0,
+                reduction: str = "mean", dloss=1.0) -> Tensor:
+    """dz_i = w p_i - q_i for the teacher's tokens, p_i (w - r / s) for the others, w = sum q + r (0 where nothing is left of the teacher)."""
+    T, V = logits.shape
+    ids = top_ids.long()
+    q, _, r, ok = _teacher(ids, top_logprobs, V, tail, temperature)
+    z = token_scores(logits, temperature, softcap)
+    none = (z == -math.inf).all(1)
+    p = torch.where(none[:, None], 0.0, torch.softmax(z, 1))
+    at = torch.where(ok, ids, V)
+    w = q.sum(1) + r
+    outside = w[:, None].expand(T, V)
+    if tail == "bucket":
+        hidden = torch.zeros(T, V + 1, dtype=torch.bool).scatter(1, at, True)[:, :V]
+        s = torch.where(hidden, 0.0, p).sum(1)
+        outside = torch.where(hidden, w[:, None], (w - torch.where(r > 0, r / s, 0.0))[:, None])
+    d = torch.cat([p * outside, torch.zeros(T, 1, dtype=p.dtype)], 1).scatter_add(1, at, -q)[:, :V]
+    kept = (ids[:, 0] >= 0) & ~none
+    n = (ids[:, 0] >= 0).sum().clamp(min=1) if reduction == "mean" else 1
+    scale = torch.as_tensor(dloss, dtype=p.dtype).expand(T) / n
+    d = d * torch.where(kept, scale, torch.zeros_like(scale))[:, None]
+    if softcap > 0:
+        d = d * (1 - torch.tanh(logits / softcap) ** 2)
+    return d / temperature
+
+
 def embed_fwd(ids: Tensor, w: Tensor) -> Tensor:
     """src/olmax/nn/embedding.py:30-32 — row gather."""
     return w[ids.long()]
