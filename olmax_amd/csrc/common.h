@@ -181,6 +181,7 @@ struct GemmScratch {
   void* p = nullptr;
   int64_t bytes = 0;
 };
+constexpr int64_t PRODUCT_SCRATCH = 64ll << 20;  // what the gradients of the LM head are given
 // gemm.hip: olmax_gemm_bf16 with an A whose rows are readable (and, k-contiguous, zero) up to a multiple of 8
 int olmax_gemm_padded(hipStream_t stream, const bf16* a, const bf16* b, void* C, const bf16* r, int M, int N, int K,
                       int64_t lda, int64_t ldb, int64_t ldc, int64_t ldr, bool a_kc, bool b_kc, bool out_f32, bool a_padded,

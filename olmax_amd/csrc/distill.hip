@@ -287,5 +287,5 @@ extern "C" int32_t olmax_lmhead_distill(hipStream_t stream, const void* h, const
   if (int rc = distill(stream, workspace, dh || dW ? grads : nullptr, top_ids, top_logprobs, loss, nullptr, row_ws, T, V, k, ld, ld, true, false, tail, temperature,
                        softcap, dloss, 0, (8 - V % 8) % 8))
     return rc;
-  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0);
+  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0, GemmScratch{workspace, std::min<int64_t>(T * ld * 4, PRODUCT_SCRATCH)});
 }

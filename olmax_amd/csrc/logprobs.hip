@@ -566,5 +566,6 @@ extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, 
   if (int rc = token_logprobs_bwd(stream, workspace, targets, stats, dlogprobs, dentropy, grads, T, V, ld, ld, true, false, ignore_index, temperature, softcap,
                                   (8 - V % 8) % 8))
     return rc;
-  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0);
+  // (the fp32 logits are done with.  Without shared reductions the few long ones of dh take 60 % more: dh and dW of 1024 x 4096 x 100352 1.78 -> 1.34 ms)
+  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0, GemmScratch{workspace, std::min<int64_t>(T * ld * 4, PRODUCT_SCRATCH)});
 }
