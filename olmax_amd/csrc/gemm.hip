@@ -31,7 +31,7 @@
 // round-robin over the 8 XCDs, so id i is remapped to (i % 8) * (grid/8) + i / 8, giving
 // every XCD one contiguous run of tiles; runs walk the tile grid in column groups so that
 // the A row-panels and B column-panels a single L2 sees are re-used.
-#include "common.h"
+#include "rows.h"
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -86,6 +86,11 @@ std::mutex g_prof_mu;
 // are, 1 KB per instruction, to Cv[part][tile][wave][i][j][lane] for gemm_split_sum_kernel.  With `sums` (both gradients in one launch) the
 // operands are already those of a part, and its accumulators go there.
 //
+// EPI == 7 and 8 form a row's part of the softmax of the LM head's logits from the accumulators (HeadRows): 7 the statistics of each row over the tile's 256 columns
+// (largest score, sum of exponentials, entropy's sum) and the targets' logits, 8 the logits' gradient in their place.  A lane has 16 of a row's 64 columns in a wave, four lanes
+// share a row, four waves a tile's: two exchanges between lanes and one through LDS.  An exponential costs the vector unit about what one k-tile's issue does; of the 100 us that a
+// round of tiles of K = 4096 takes they are 3.
+//
 // RAG: 1 where M or N, 2 where K is not a multiple of the tile.  The last tile of a row or column is
 // moved back so that it ends with the matrix (the loop then reads nothing outside it and is the same
 // code) and stores only what no other tile stores.  The partial k-tile at the end of K is taken FIRST, ahead of
@@ -103,11 +108,12 @@ __device__ __forceinline__ void gemm_tile(
     const bf16* __restrict__ R, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc,
     int64_t ldr, int tiles_m, int tiles_n, int c_vec, const float* __restrict__ cos_t,
     const float* __restrict__ sin_t, int seq_len, int rope_cols, int order, int pid, const int nwg, unsigned char* smem, int block = 0, float* park = nullptr,
-    float* sums = nullptr) {
+    float* sums = nullptr, const HeadRows* head = nullptr) {
   constexpr int GLU = (EPI == 1 || EPI == 2) ? EPI : (EPI == 4 ? 1 : (EPI == 5 ? 2 : 0));
   constexpr bool GLU_BWD = EPI == 4 || EPI == 5;
   constexpr bool ROPE = EPI == 3;
   constexpr bool SPLIT = EPI == 6;
+  constexpr bool ROW_STATS = EPI == 7, ROW_GRADS = EPI == 8;
   static_assert(EPI == 0 || SPLIT || (BN == 256 && WN == 64 && B_KC && !HAS_RES && !OUT_F32), "fused epilogues: 256-wide NT tiles only");
   constexpr int NW = (BM / WM) * (BN / WN);
   constexpr int TM = WM / 16, TN = WN / 16;  // accumulators of 16x16 per wave
@@ -672,6 +678,92 @@ __device__ __forceinline__ void gemm_tile(
   // ---- epilogue.  The MFMAs ran with their operands swapped (B fragment as the instruction's A),
   // so each accumulator is a transposed 16x16 tile: lane -> row l16e, columns 4*g16e + r, i.e. four
   // consecutive columns of one row of C per lane.
+  if constexpr (ROW_STATS) {
+    int targets[TM];
+#pragma unroll
+    for (int i = 0; i < TM; i++) targets[i] = head->targets ? head->targets[m0 + wm * WM + i * 16 + l16e] : -1;
+    __syncthreads();  // every wave is done reading the operand stages
+    rows::Stat* strip = reinterpret_cast<rows::Stat*>(smem);  // [WAVES_N][BM]
+    const rows::Scale c{head->cap, head->cap_k, head->inv_tau};
+    const bool cap = head->cap > 0.f;
+    const int first = wn * WN + g16e * 4;  // this lane's first column of the block
+    auto here = [&](int j, int r) { return !RAG || first + j * 16 + r >= col_lo; };
+    auto of_row = [&](auto capped, const f32x4* x, int row, int target) {
+      constexpr bool CAP = decltype(capped)::value;
+      float most = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) most = here(j, r) ? fmaxf(most, x[j][r]) : most;
+      most = fmaxf(most, __shfl_xor(most, 16, 64));
+      most = half_swap_max(most);
+      rows::Stat a = rows::Stat::none();
+      if (CAP || most > -INFINITY) a.m = rows::score<CAP>(most, c);
+      const float ref = a.ref();
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float d = rows::behind<CAP>(x[j][r], c, ref), e = here(j, r) ? rows::exp_of(d) : 0.f;
+          a.s += e;
+          a.t += e * fmaxf(d, -200.f);
+        }
+      a.s += __shfl_xor(a.s, 16, 64);
+      a.t += __shfl_xor(a.t, 16, 64);
+      a.s = half_swap_sum(a.s);
+      a.t = half_swap_sum(a.t);
+      if (g16e == 0) strip[wn * BM + row] = a;
+      const int at = target - n0 - first;  // of the lane's columns: 0 to 3, 16 to 19, ..
+      if (at >= 0 && at < WN && (at & 12) == 0 && target - n0 >= col_lo && stores_row(row)) {
+        float logit = 0.f;
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) logit = at == j * 16 + r ? x[j][r] : logit;
+        head->target_logit[m0 + row] = logit;
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      const int row = wm * WM + i * 16 + l16e;
+      if (cap) of_row(std::true_type(), acc[i], row, targets[i]);
+      else of_row(std::false_type(), acc[i], row, targets[i]);
+    }
+    __syncthreads();
+    if (tid < BM && stores_row(tid)) {
+      rows::Stat a = strip[tid];
+#pragma unroll
+      for (int w = 1; w < WAVES_N; w++) a.join(strip[w * BM + tid]);
+      reinterpret_cast<rows::Stat*>(head->parts)[(int64_t)tile_n * M + m0 + tid] = a;
+    }
+    return;
+  }
+  if constexpr (ROW_GRADS) {
+    // d = p (-g - h (ln p + H)), and g more at the target, times the scores' slope; then out as any bf16 result
+    const rows::Scale c{head->cap, head->cap_k, head->inv_tau};
+    const bool cap = head->cap > 0.f;
+    const int first = n0 + wn * WN + g16e * 4;
+    auto of_row = [&](auto capped, f32x4* x, int64_t row) {
+      constexpr bool CAP = decltype(capped)::value;
+      const float m = head->stats[row * 3], log_sum = head->stats[row * 3 + 1], entropy = head->stats[row * 3 + 2];
+      const int target = head->targets[row];
+      const bool skipped = target == head->ignore_index || m == -INFINITY;
+      const float g = target < 0 || target >= head->V || skipped ? 0.f : head->dlogprobs[row], h = head->dentropy && !skipped ? head->dentropy[row] : 0.f;
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[j][r] = rows::score_grad<CAP, true>(x[j][r], c, m, log_sum, entropy, g, h, first + j * 16 + r == target);
+      if (skipped)
+#pragma unroll
+        for (int j = 0; j < TN; j++) x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      const int64_t row = m0 + wm * WM + i * 16 + l16e;
+      if (cap) of_row(std::true_type(), acc[i], row);
+      else of_row(std::false_type(), acc[i], row);
+    }
+  }
   if (GLU) {
     bf16* act = const_cast<bf16*>(R);
     bf16* gu = reinterpret_cast<bf16*>(Cv);
@@ -901,6 +993,14 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) GEMM_VGPR_CAP void gemm
                                                                     sin_t, seq_len, rope_cols, order, blockIdx.x, gridDim.x, smem);
 }
 
+template <int EPI, int RAG>
+__global__ __launch_bounds__(512) void gemm_head_kernel(const bf16* __restrict__ A, const bf16* __restrict__ B, bf16* __restrict__ C, int M, int N, int K, int64_t ldc, int tiles_m,
+                                                        int tiles_n, int order, const HeadRows rows) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  gemm_tile<256, 256, 128, 64, true, true, false, false, EPI, RAG>(A, B, C, nullptr, M, N, K, K, K, ldc, 0, tiles_m, tiles_n, 1, nullptr, nullptr, 1, 0, order, blockIdx.x,
+                                                                   gridDim.x, smem, 0, nullptr, nullptr, &rows);
+}
+
 // dX = dY W (+ R) and dW = dY^T X in one launch of T x T tiles: the second starts on the CUs that the first's last round of tiles
 // leaves idle.  Workgroups [0, n_first) are the product with the longer reduction (and padding up to a whole number of XCDs).
 // us in a block's backward pass, two calls -> one, T x in x out: tiles of 128: 3000 x 1024 x 3072 76 -> 47, 3000 x 2816 x 1024 65 -> 42, 4096 x 1024 x 3072 92 -> 60;
@@ -1023,6 +1123,36 @@ int launch_glu(hipStream_t s, const bf16* A, const bf16* B, bf16* gu, bf16* act,
     rec.bytes = 2.0 * ((double)M * K + 2.0 * F * K + (double)M * F * ((gu ? 3 : 1) + (dact ? 1 : 0)));
     rec.key = 256 | (1 << 12) | (1 << 13) | (1 << 16);
     rec.M = M; rec.N = 2 * F; rec.K = K;
+    std::lock_guard<std::mutex> lk(g_prof_mu);
+    g_prof.push_back(rec);
+  }
+  OLMAX_LAUNCH_CHECK();
+  return OLMAX_OK;
+}
+
+template <int EPI>
+int launch_head(hipStream_t s, const bf16* A, const bf16* B, bf16* C, int M, int N, int K, int64_t ldc, const HeadRows& rows) {
+  constexpr int SMEM = 2 * (256 + 256) * BK * 2;
+  auto whole = gemm_head_kernel<EPI, 0>, ragged = gemm_head_kernel<EPI, 1>, kragged = gemm_head_kernel<EPI, 2>;
+  static std::once_flag attr_once;
+  std::call_once(attr_once, [&] {
+    for (auto k : {whole, ragged, kragged}) (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  });
+  auto kern = K % BK ? kragged : (M % 256 || N % 256) ? ragged : whole;
+  const int tm = (M + 255) / 256, tn = (N + 255) / 256, order = tile_order(tm, tn, true, true, N, K);
+  ProfRec rec{};
+  if (g_prof_on) {
+    (void)hipEventCreate(&rec.e0);
+    (void)hipEventCreate(&rec.e1);
+    (void)hipEventRecord(rec.e0, s);
+  }
+  hipLaunchKernelGGL(kern, dim3(order_grid(order, tm, tn)), dim3(512), SMEM, s, A, B, C, M, N, K, ldc, tm, tn, order, rows);
+  if (g_prof_on) {
+    (void)hipEventRecord(rec.e1, s);
+    rec.flops = 2.0 * M * N * K;
+    rec.bytes = 2.0 * ((double)M * K + (double)N * K + (EPI == 8 ? (double)M * N : 0.0));
+    rec.key = 256 | (1 << 12) | (1 << 13) | (1 << 20);
+    rec.M = M; rec.N = N; rec.K = K;
     std::lock_guard<std::mutex> lk(g_prof_mu);
     g_prof.push_back(rec);
   }
@@ -1510,6 +1640,22 @@ int olmax_gemm_padded(hipStream_t stream, const bf16* a, const bf16* b, void* C,
   if (b_kc) GO(false, true);
   GO(false, false);
 #undef GO
+}
+
+int olmax_gemm_head_columns(int M, int N, int K) {
+  if (M < 256 || N < 256 || K < BK || K % 8) return 0;
+  int parts;
+  float cost;
+  if (pick_tile(M, N, K, true, true, true, 0, &parts, &cost) != 256) return 0;
+  const int tm = (M + 255) / 256;
+  const Cut cut = find_cut(tm, (N + 255) / 256);  // (a cut along the rows is not taken: a row's statistics would come from two launches for all columns)
+  return cut.cn ? cut.cn * 256 : N;
+}
+int olmax_gemm_head_stats(hipStream_t s, const bf16* h, const bf16* w, int M, int N, int K, const HeadRows& rows) {
+  return launch_head<7>(s, h, w, nullptr, M, N, K, 0, rows);
+}
+int olmax_gemm_head_grads(hipStream_t s, const bf16* h, const bf16* w, bf16* d, int64_t ldd, int M, int N, int K, const HeadRows& rows) {
+  return launch_head<8>(s, h, w, d, M, N, K, ldd, rows);
 }
 
 // The two products of olmax_gemm_grads as one launch: what it costs in each kernel that can run it.  Measured, with the two calls, on 312

@@ -154,18 +154,17 @@ __device__ __forceinline__ void write_skipped(const Out& o, int64_t row, int k) 
     o.top_logprobs[row * k + threadIdx.x] = -INFINITY;
   }
 }
-// a: statistics of the whole row.  A row without a score above minus infinity has no distribution: log probabilities of minus infinity, entropy 0.
-template <typename T, bool CAP>
-__device__ __forceinline__ void write_row(const Out& o, int64_t row, const T* zr, int target, int V, const Scale& c, const Stat& a) {
+// a: statistics of the whole row, x: the target's logit, if there is one.  A row without a score above minus infinity has no distribution: log probabilities of minus
+// infinity, entropy 0.  By one thread.
+template <bool CAP>
+__device__ __forceinline__ void write_row(const Out& o, int64_t row, bool has_target, float x, const Scale& c, const Stat& a) {
   const bool none = a.s == 0.f;
   const float log_sum = log_of(a.s), entropy = none ? 0.f : log_sum - a.t / a.s;
-  if (threadIdx.x == 0) {
-    if (o.logprobs) o.logprobs[row] = target < 0 || target >= V ? 0.f : none ? -INFINITY : behind<CAP>((float)zr[target], c, a.m) - log_sum;
-    o.entropy[row] = entropy;
-    o.stats[row * 3] = a.m;
-    o.stats[row * 3 + 1] = none ? 0.f : log_sum;
-    o.stats[row * 3 + 2] = entropy;
-  }
+  if (o.logprobs) o.logprobs[row] = !has_target ? 0.f : none ? -INFINITY : behind<CAP>(x, c, a.m) - log_sum;
+  o.entropy[row] = entropy;
+  o.stats[row * 3] = a.m;
+  o.stats[row * 3 + 1] = none ? 0.f : log_sum;
+  o.stats[row * 3 + 2] = entropy;
 }
 // The n <= k largest logits above minus infinity are cand[0 .. n) or are the largest of them; the rest of k slots gets the lowest indices that are not among them.
 template <bool CAP>
@@ -194,7 +193,7 @@ __device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, cons
   }
 }
 
-// One workgroup to a row, or to one of `parts` equal shares of it; a part leaves its statistics and its candidates for score_join_kernel.
+// One workgroup to a row, or to one of `parts` equal shares of it; with part_stat a share leaves its statistics and its candidates for a kernel that joins them.
 template <typename T, bool CAP, bool TOP>
 __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out, uint64_t* __restrict__ part_top,
                                                         Stat* __restrict__ part_stat, int V, int64_t ld, int32_t ignore_index, Scale c, int k, int parts) {
@@ -204,7 +203,7 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
   const int part = blockIdx.x % parts;
   const int target = targets ? targets[row] : -1;
   if (targets && target == ignore_index) {  // (the join writes for a row in parts)
-    if (parts == 1) write_skipped(out, row, k);
+    if (!part_stat) write_skipped(out, row, k);
     return;
   }
   const T* zr = logits + row * ld;
@@ -332,8 +331,9 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
       n = narrow<CAND>(l.cand, n, bound, &l.n);
     }
   }
-  if (parts == 1) {
-    write_row<T, CAP>(out, row, zr, target, V, c, all);
+  if (!part_stat) {
+    const bool has_target = target >= 0 && target < V;
+    if (threadIdx.x == 0) write_row<CAP>(out, row, has_target, has_target ? (float)zr[target] : 0.f, c, all);
     if (TOP) write_top<CAP>(out, row, k, l.cand, n, c, all);
     return;
   }
@@ -370,7 +370,8 @@ __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ lo
       most = max(most, e);
     }
   a = block_join<TH / 64>(a, red);
-  write_row<T, CAP>(out, row, logits + row * ld, target, V, c, a);
+  const bool has_target = target >= 0 && target < V;
+  if (threadIdx.x == 0) write_row<CAP>(out, row, has_target, has_target ? (float)logits[row * ld + target] : 0.f, c, a);
   if (TOP) {
     const unsigned bound = kth_best(best, max((unsigned)(most >> 32), KEY_NEG_INF), k);
     const int n = narrow<JOINED>(cand, parts * k, bound, &counter);
@@ -378,13 +379,55 @@ __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ lo
   }
 }
 
+// The rows of an LM head whose product left statistics of 256 columns a tile (olmax_gemm_head_stats), [tiles][rows], and, for the last columns, logits (`rest`, from column
+// `fused` on) with statistics of their own: 16 rows a workgroup, each sixteenth of a wave takes every 64th tile.  (64 rows a workgroup, a lane each: 20 us for 2048 rows of
+// 384 tiles, so 8.)
+template <bool CAP>
+__global__ __launch_bounds__(1024) void head_join_kernel(const Stat* __restrict__ tiles, int n_tiles, const Stat* __restrict__ rest_stat, const float* __restrict__ rest,
+                                                         int64_t ld_rest, const float* __restrict__ target_logit, const int32_t* __restrict__ targets, Out out, int64_t rows,
+                                                         int V, int fused, int32_t ignore_index, Scale c) {
+  __shared__ Stat part[16][16];
+  const int wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x * 16ll + (threadIdx.x & 15);
+  Stat a = Stat::none();
+  if (row < rows)
+    for (int i = threadIdx.x >> 4; i < n_tiles; i += 64) a.join(tiles[(int64_t)i * rows + row]);
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) {
+    Stat b;
+    b.m = __shfl_xor(a.m, o, 64);
+    b.s = __shfl_xor(a.s, o, 64);
+    b.t = __shfl_xor(a.t, o, 64);
+    a.join(b);
+  }
+  if ((threadIdx.x & 63) < 16) part[wave][threadIdx.x & 15] = a;
+  __syncthreads();
+  if (threadIdx.x >= 16 || row >= rows) return;
+  const int target = targets ? targets[row] : -1;
+  if (targets && target == ignore_index) {
+    if (out.logprobs) out.logprobs[row] = 0.f;
+    out.entropy[row] = 0.f;
+    for (int i = 0; i < 3; i++) out.stats[row * 3 + i] = 0.f;
+    return;
+  }
+  for (int w = 1; w < 16; w++) a.join(part[w][threadIdx.x]);
+  if (fused < V) a.join(rest_stat[row]);
+  const bool has_target = target >= 0 && target < V;
+  write_row<CAP>(out, row, has_target, !has_target ? 0.f : target < fused ? target_logit[row] : rest[row * ld_rest + target - fused], c, a);
+}
+
+__global__ __launch_bounds__(256) void zero_columns_kernel(bf16* __restrict__ d, int64_t rows, int64_t ld, int n) {
+  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+  if (i < rows * n) d[i / n * ld + i % n] = (bf16)0.f;
+}
+
 // d loss / d logits of logprob and entropy: dz_i = g (delta_it - p_i) - h p_i (ln p_i + H), from the statistics that the forward pass kept.
-// A workgroup takes one of `parts` shares of a row.
+// A workgroup takes one of `parts` shares of a row.  first: the column of the whole row that these logits begin with (they are its last).
 template <typename T, typename TO, bool CAP, bool ENT>
 __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const int32_t* __restrict__ targets,
                                                         const float* __restrict__ stats, const float* __restrict__ dlogprobs,
                                                         const float* __restrict__ dentropy, int V, int64_t ld, int64_t ldd, int32_t ignore_index, Scale c,
-                                                        int parts, int pad) {
+                                                        int parts, int pad, int first) {
   constexpr int N = Vec<TO>::N;
   const int64_t row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
@@ -396,20 +439,8 @@ __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ lo
   const int target = targets[row];
   const float m = stats[row * 3], log_sum = stats[row * 3 + 1], entropy = stats[row * 3 + 2];
   const bool skipped = target == ignore_index || m == -INFINITY;  // no distribution: no gradient
-  const float g = skipped || target < 0 || target >= V ? 0.f : dlogprobs[row], h = skipped || !ENT ? 0.f : dentropy[row];
-  auto grad = [&](float x, int i) {
-    float chain = c.inv_tau, y = x;
-    if (CAP) {
-      const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f);
-      y = c.cap * t;
-      chain *= 1.f - t * t;
-    }
-    const float logp = __builtin_fmaf(y, c.inv_tau, -m) - log_sum;
-    const float p = exp_of(logp);
-    float d = -p * (ENT ? __builtin_fmaf(h, fmaxf(logp, -200.f) + entropy, g) : g);
-    if (i == target) d += g;
-    return d * chain;
-  };
+  const float g = skipped || target < 0 || target >= first + V ? 0.f : dlogprobs[row], h = skipped || !ENT ? 0.f : dentropy[row];
+  auto grad = [&](float x, int i) { return score_grad<CAP, ENT>(x, c, m, log_sum, entropy, g, h, first + i == target); };
   for (int v = v0 + threadIdx.x; v < v1; v += TH) {
     float x[N];
     const int i = cutting.head + v * N;
@@ -466,7 +497,7 @@ extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, 
   OLMAX_CHECK(workspace_bytes >= olmax_token_logprobs_workspace_bytes(T, V, top, logits_f32) && (parts == 1 || (workspace && aligned16(workspace))), OLMAX_ERR_WORKSPACE,
               "olmax_token_logprobs: workspace needs %ld bytes, 16-byte aligned", (long)olmax_token_logprobs_workspace_bytes(T, V, top, logits_f32));
   uint64_t* part_top = (uint64_t*)workspace;
-  Stat* part_stat = (Stat*)((char*)workspace + (parts == 1 ? 0 : T * parts * (int64_t)top * 8));
+  Stat* part_stat = parts == 1 ? nullptr : (Stat*)((char*)workspace + T * parts * (int64_t)top * 8);
   const Out out{logprobs, entropy, stats, top ? top_logprobs : nullptr, top ? top_ids : nullptr};
   const Scale c = scale_of(temperature, softcap);
 #define SCORE(TY, CAPV, TOPV)                                                                                                                             \
@@ -490,13 +521,13 @@ extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, 
 // grads_bf16: the gradient of fp32 logits as bf16 (the LM head's products take it); pad: zeros behind each of its rows
 static int token_logprobs_bwd(hipStream_t stream, const void* logits, const int32_t* targets, const float* stats, const float* dlogprobs,
                               const float* dentropy, void* dlogits, int64_t T, int32_t V, int64_t ld, int64_t ldd, bool logits_f32, bool grads_f32,
-                              int32_t ignore_index, float temperature, float softcap, int pad) {
+                              int32_t ignore_index, float temperature, float softcap, int pad, int first = 0) {
   const Scale c = scale_of(temperature, softcap);
   const int parts = (int)std::max<int64_t>(1, V / (grads_f32 ? 4 : 8) / (TH * 8));
   OLMAX_CHECK(T * parts < (1LL << 31), OLMAX_ERR_SHAPE, "olmax_token_logprobs_bwd: T=%ld rows of V=%d are too many", (long)T, V);
 #define GRAD(TY, TO, CAPV, ENTV)                                                                                                                             \
   hipLaunchKernelGGL((score_grad_kernel<TY, TO, CAPV, ENTV>), dim3((unsigned)(T * parts)), dim3(TH), 0, stream, (const TY*)logits, (TO*)dlogits, targets, stats, \
-                     dlogprobs, dentropy, V, ld, ldd, ignore_index, c, parts, pad)
+                     dlogprobs, dentropy, V, ld, ldd, ignore_index, c, parts, pad, first)
 #define GRAD_E(TY, TO, CAPV) do { if (dentropy) GRAD(TY, TO, CAPV, true); else GRAD(TY, TO, CAPV, false); } while (0)
 #define GRAD_C(TY, TO) do { if (softcap > 0.f) GRAD_E(TY, TO, true); else GRAD_E(TY, TO, false); } while (0)
   if (logits_f32 && grads_f32) GRAD_C(float, float); else if (logits_f32) GRAD_C(float, bf16); else GRAD_C(bf16, bf16);
@@ -519,36 +550,77 @@ extern "C" int32_t olmax_token_logprobs_bwd(hipStream_t stream, const void* logi
                             temperature, softcap, 0);
 }
 
-// ---- with the LM head's product.  The logits are fp32 in the workspace: the framework's bf16 ones are off by 2^-9 of themselves, as much in a
-// log probability as policies of two steps may be apart.
+// ---- with the LM head's product.  The logits are fp32: the framework's bf16 ones are off by 2^-9 of themselves, as much in a
+// log probability as policies of two steps may be apart.  Where the product runs in large tiles they stay in its accumulators (HeadRows), but for the columns behind the last whole
+// round of tiles, which are a product of their own; where it does not, or alternatives are asked for, all of them go through the workspace.  us, logits in the workspace -> not: 2048
+// x 4096 x 100352 1443 -> 1195 (the product alone, fp32 logits written, 1335), gradients of 1024 x 4096 x 100352 2080 -> 1977.
 static int64_t head_stride(int32_t V) { return ((int64_t)V + 63) / 64 * 64; }  // whole lines of bf16 and fp32
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
+// Memory of the forward call: fp32 logits of the columns from `fused` on, then (fused > 0) statistics of its tiles, of the other columns, and target logits
+struct HeadPlan {
+  int fused;
+  int64_t ld, stats_at, rest_at, target_at, bytes;
+};
+static HeadPlan head_plan(int64_t T, int32_t d, int32_t V, int32_t top) {
+  HeadPlan p;
+  p.fused = top > 0 ? 0 : olmax_gemm_head_columns((int)T, V, d);
+  p.ld = head_stride(V - p.fused);
+  p.stats_at = up256(T * p.ld * 4);
+  p.rest_at = p.stats_at + up256((int64_t)((p.fused + 255) / 256) * T * sizeof(Stat));
+  p.target_at = p.rest_at + up256(T * sizeof(Stat));
+  p.bytes = p.fused ? p.target_at + up256(T * 4) : p.stats_at + olmax_token_logprobs_workspace_bytes(T, V, top, 1);
+  return p;
+}
+
 extern "C" int64_t olmax_lmhead_logprobs_workspace_bytes(int64_t T, int32_t d, int32_t V, int32_t top) {
-  if (T <= 0 || V <= 0) return 0;
-  return up256(T * head_stride(V) * 4) + olmax_token_logprobs_workspace_bytes(T, V, top, 1);
+  return T <= 0 || V <= 0 || d <= 0 || T >= (1 << 24) ? 0 : head_plan(T, d, V, top).bytes;
 }
 
 extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, const void* W, const int32_t* targets, float* logprobs, float* entropy,
                                          float* stats, int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes, int64_t T,
                                          int32_t d, int32_t V, int32_t top, int32_t ignore_index, float temperature, float softcap) {
-  OLMAX_CHECK(h && W && workspace, OLMAX_ERR_ARG, "olmax_lmhead_logprobs: null pointer");
+  OLMAX_CHECK(h && W && workspace && entropy && stats && (!logprobs || targets), OLMAX_ERR_ARG, "olmax_lmhead_logprobs: null pointer");
   OLMAX_CHECK(T > 0 && d > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs: bad shape T=%ld d=%d V=%d", (long)T, d, V);
-  OLMAX_CHECK(workspace_bytes >= olmax_lmhead_logprobs_workspace_bytes(T, d, V, top) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
-              "olmax_lmhead_logprobs: workspace needs %ld bytes, 256-byte aligned", (long)olmax_lmhead_logprobs_workspace_bytes(T, d, V, top));
-  const int64_t ld = head_stride(V), at = up256(T * ld * 4);
-  // (the arguments of the rows are checked before the product is launched)
-  OLMAX_CHECK(entropy && stats && (!logprobs || targets) && top >= 0 && top <= MAX_TOP && top <= V && (top == 0 || (top_ids && top_logprobs)) && temperature >= 1e-6f &&
-                  temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG,
-              "olmax_lmhead_logprobs: wants entropy and stats, targets for logprobs, 0 to %d alternatives, a temperature within 1e-6 and 1e6, a softcap that is not negative", MAX_TOP);
-  if (int rc = olmax_gemm_padded(stream, (const bf16*)h, (const bf16*)W, workspace, nullptr, (int)T, V, d, d, d, ld, 0, true, true, true, false)) return rc;
-  return olmax_token_logprobs(stream, workspace, targets, logprobs, entropy, stats, top_ids, top_logprobs, (char*)workspace + at, workspace_bytes - at, T, V,
-                              ld, top, 1, ignore_index, temperature, softcap);
+  OLMAX_CHECK(top >= 0 && top <= MAX_TOP && top <= V && (top == 0 || (top_ids && top_logprobs)), OLMAX_ERR_ARG,
+              "olmax_lmhead_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, top);
+  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_lmhead_logprobs: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(aligned16(h) && aligned16(W), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs: h and W must be 16-byte aligned");
+  const HeadPlan p = head_plan(T, d, V, top);
+  OLMAX_CHECK(workspace_bytes >= p.bytes && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs: workspace needs %ld bytes, 256-byte aligned", (long)p.bytes);
+  const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
+  char* ws = (char*)workspace;
+  const int rest = V - p.fused;
+  if (rest) {
+    if (int rc = olmax_gemm_padded(stream, hp, wp + (int64_t)p.fused * d, ws, nullptr, (int)T, rest, d, d, d, p.ld, 0, true, true, true, false)) return rc;
+  }
+  if (!p.fused)
+    return olmax_token_logprobs(stream, ws, targets, logprobs, entropy, stats, top_ids, top_logprobs, ws + p.stats_at, workspace_bytes - p.stats_at, T, V, p.ld, top, 1,
+                                ignore_index, temperature, softcap);
+  const Scale c = scale_of(temperature, softcap);
+  const Out out{logprobs, entropy, stats, nullptr, nullptr};
+  Stat *tiles = (Stat*)(ws + p.stats_at), *rest_stat = (Stat*)(ws + p.rest_at);
+  float* target_logit = (float*)(ws + p.target_at);
+  HeadRows rows{};
+  rows.targets = targets;
+  rows.ignore_index = ignore_index;
+  rows.V = V;
+  rows.cap = c.cap, rows.cap_k = c.cap_k, rows.inv_tau = c.inv_tau;
+  rows.parts = (float*)tiles;
+  rows.target_logit = target_logit;
+  if (int rc = olmax_gemm_head_stats(stream, hp, wp, (int)T, p.fused, d, rows)) return rc;
+#define JOIN(CAPV)                                                                                                                                                        do {                                                                                                                                                                      if (rest)                                                                                                                                                                 hipLaunchKernelGGL((score_rows_kernel<float, CAPV, false>), dim3((unsigned)T), dim3(TH), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,                          p.ld, ignore_index, c, 0, 1);                                                                                                                      hipLaunchKernelGGL((head_join_kernel<CAPV>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,                        (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, V, p.fused, ignore_index, c);                                                 } while (0)
+  if (softcap > 0.f) JOIN(true); else JOIN(false);
+#undef JOIN
+  OLMAX_LAUNCH_CHECK();
+  return OLMAX_OK;
 }
 
+// The backward call's: bf16 gradients, then fp32 logits of the columns from `fused` on and, in the same place afterwards, room for the products' partial sums
+static int64_t head_grads_room(int64_t T, int fused, int32_t V) { return std::max(up256(T * head_stride(V - fused) * 4), fused ? PRODUCT_SCRATCH : 0); }
 extern "C" int64_t olmax_lmhead_logprobs_bwd_workspace_bytes(int64_t T, int32_t d, int32_t V) {
-  if (T <= 0 || V <= 0) return 0;
-  return up256(T * head_stride(V) * 4) + up256(T * head_stride(V) * 2);
+  if (T <= 0 || V <= 0 || d <= 0 || T >= (1 << 24)) return 0;
+  return up256(T * head_stride(V) * 2) + head_grads_room(T, olmax_gemm_head_columns((int)T, V, d), V);
 }
 
 extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, const void* W, const int32_t* targets, const float* stats,
@@ -557,15 +629,33 @@ extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, 
   OLMAX_CHECK(h && W && targets && stats && dlogprobs && workspace && (dh || dW), OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: null pointer");
   OLMAX_CHECK(T > 0 && d > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs_bwd: bad shape T=%ld d=%d V=%d", (long)T, d, V);
   OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(aligned16(h) && aligned16(W), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs_bwd: h and W must be 16-byte aligned");
   OLMAX_CHECK(workspace_bytes >= olmax_lmhead_logprobs_bwd_workspace_bytes(T, d, V) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
               "olmax_lmhead_logprobs_bwd: workspace needs %ld bytes, 256-byte aligned", (long)olmax_lmhead_logprobs_bwd_workspace_bytes(T, d, V));
   const int64_t ld = head_stride(V);
+  const int fused = olmax_gemm_head_columns((int)T, V, d), rest = V - fused, pad = (8 - V % 8) % 8;
   const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
-  bf16* grads = (bf16*)((char*)workspace + up256(T * ld * 4));
-  if (int rc = olmax_gemm_padded(stream, hp, wp, workspace, nullptr, (int)T, V, d, d, d, ld, 0, true, true, true, false)) return rc;
-  if (int rc = token_logprobs_bwd(stream, workspace, targets, stats, dlogprobs, dentropy, grads, T, V, ld, ld, true, false, ignore_index, temperature, softcap,
-                                  (8 - V % 8) % 8))
-    return rc;
-  // (the fp32 logits are done with.  Without shared reductions the few long ones of dh take 60 % more: dh and dW of 1024 x 4096 x 100352 1.78 -> 1.34 ms)
-  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0, GemmScratch{workspace, std::min<int64_t>(T * ld * 4, PRODUCT_SCRATCH)});
+  bf16* grads = (bf16*)workspace;
+  float* logits = (float*)((char*)workspace + up256(T * ld * 2));
+  if (fused) {
+    const Scale c = scale_of(temperature, softcap);
+    HeadRows rows{};
+    rows.targets = targets;
+    rows.ignore_index = ignore_index;
+    rows.V = V;
+    rows.cap = c.cap, rows.cap_k = c.cap_k, rows.inv_tau = c.inv_tau;
+    rows.stats = stats, rows.dlogprobs = dlogprobs, rows.dentropy = dentropy;
+    if (int rc = olmax_gemm_head_grads(stream, hp, wp, grads, ld, (int)T, fused, d, rows)) return rc;
+  }
+  if (rest) {
+    const int64_t ldr = head_stride(rest);
+    if (int rc = olmax_gemm_padded(stream, hp, wp + (int64_t)fused * d, logits, nullptr, (int)T, rest, d, d, d, ldr, 0, true, true, true, false)) return rc;
+    if (int rc = token_logprobs_bwd(stream, logits, targets, stats, dlogprobs, dentropy, grads + fused, T, rest, ldr, ld, true, false, ignore_index, temperature, softcap, pad, fused))
+      return rc;
+  } else if (pad) {
+    hipLaunchKernelGGL(zero_columns_kernel, dim3((unsigned)((T * pad + 255) / 256)), dim3(256), 0, stream, grads + V, T, ld, pad);
+  }
+  // (without shared reductions the few long ones of dh take 60 % more: dh and dW of 1024 x 4096 x 100352 1.78 -> 1.34 ms)
+  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0,
+                               GemmScratch{logits, std::min(head_grads_room(T, fused, V), PRODUCT_SCRATCH)});
 }

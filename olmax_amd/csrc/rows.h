@@ -124,4 +124,19 @@ template <int NW> __device__ __forceinline__ Stat block_join(Stat a, Stat* red) 
   return a;
 }
 
+// d / d x of g ln p[target] + h entropy: (g (i == target) - p (g + h (ln p + H))) dz/dx, from the row's m, ln S and H
+template <bool CAP, bool ENT>
+__device__ __forceinline__ float score_grad(float x, const Scale& c, float m, float log_sum, float entropy, float g, float h, bool target) {
+  float chain = c.inv_tau, y = x;
+  if (CAP) {
+    const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f);
+    y = c.cap * t;
+    chain *= 1.f - t * t;
+  }
+  const float logp = __builtin_fmaf(y, c.inv_tau, -m) - log_sum;
+  float d = -exp_of(logp) * (ENT ? __builtin_fmaf(h, fmaxf(logp, -200.f) + entropy, g) : g);
+  if (target) d += g;
+  return d * chain;
+}
+
 }  // namespace rows

@@ -365,6 +365,49 @@ def head(T, d, V, seed=0):
 
 
 HEADS = [(1, 64, 100), (5, 256, 4096), (37, 200, 1003), (300, 320, 1030), (513, 1024, 5000), (1024, 512, 2304), (700, 72, 50304)]
+# large tiles, the logits in the accumulators: whole rounds of tiles and columns behind them; partial tiles and k-tiles; a row length that is no multiple of 8, with and without
+# columns behind the last round; one round exactly
+IN_TILES = [(256, 64, 70000), (511, 72, 40007), (700, 128, 50301), (512, 256, 32768)]
+
+
+@pytest.mark.parametrize("T,d,V", IN_TILES)
+@pytest.mark.parametrize("temperature,softcap", [(1.0, 0.0), (0.7, 20.0)])
+def test_lmhead_in_tiles(T, d, V, temperature, softcap):
+    """The bounds of the two tests below, on the GPU in 64 bits; targets in every 256 columns, some ignored, some out of range, no cotangent of the entropy."""
+    from olmax_amd import ops
+    print(f"[case] tiles {T} {d} {V}", flush=True)
+    assert ops._size("olmax_lmhead_logprobs_workspace_bytes", T, d, V, 0) < 2 * T * V  # (fp32 logits would need 4)
+    h, W, t = head(T, d, V)
+    t = ((torch.arange(T, device="cuda") * 977 + 255) % V).to(torch.int32)
+    t[0], t[1], t[2], t[3], t[4], t[T - 1] = V - 1, -100, V, -7, 0, V - 2
+    tau, cap = f32(temperature), f32(softcap)
+    r = ops.lmhead_logprobs(h, W, t, temperature=temperature, softcap=softcap)
+    z = h.double() @ W.double().t()
+    of_z = (4 * math.sqrt(d) * U * (h.double().abs() @ W.double().abs().t()).max(1).values).cpu() / tau
+    s = ref.token_scores(z, tau, cap)
+    logp = torch.log_softmax(s, 1)
+    p = logp.exp()
+    entropy = -(p * logp).sum(1)
+    inside = (t >= 0) & (t < V)
+    at = t.clamp(0, V - 1).long()[:, None]
+    lp = torch.where(inside, logp.gather(1, at)[:, 0], 0.0)
+    kept = t != -100
+    b = Row(z[:300].cpu(), tau, cap)
+    few = slice(0, b.lse.shape[0])
+    near(r.logprobs[few], (lp * kept)[few].cpu(), b.of_lp((lp * kept)[few].cpu()) + 2 * of_z[few], "logprobs")
+    near(r.entropy[few], (entropy * kept)[few].cpu(), b.of_entropy + 2 * of_z[few] * (1 + b.first + b.lse), "entropy")
+    near(r.logprobs, (lp * kept).cpu(), b.of_lp((lp * kept)[few].cpu()).max() + 2 * of_z, "logprobs of all rows, the largest bound of some")
+    assert torch.equal((r.stats[:, 2]), r.entropy) and (r.stats[1] == 0).all()
+    g = torch.randn(T, device="cuda")
+    dh, dW = ops.lmhead_logprobs_bwd(h, W, t, r.stats, g, temperature=temperature, softcap=softcap)
+    gd = (g.double() * inside * kept)[:, None]
+    dz = (-gd * p).scatter_add(1, at, gd) / tau
+    if softcap:
+        dz = dz * (1 - torch.tanh(z / cap) ** 2)
+    for got, want in ((dh, dz @ W.double()), (dW, dz.t() @ h.double())):
+        assert (got.double() - want).norm() <= 2.0 ** -8 * want.norm()
+        assert (got[-40:].double() - want[-40:]).norm() <= 2.0 ** -7 * want[-40:].norm()
+    assert (dh[1:4] == 0).all()
 
 
 @pytest.mark.parametrize("T,d,V", HEADS)
