@@ -15,29 +15,39 @@ using namespace rows;
 namespace {
 
 constexpr int MAX_TOP = 128;
+constexpr int COUNTERS = 64;
 constexpr int COUNT_IN_ROWS = 1024;  // up to so many rows each workgroup counts them itself
 constexpr float LEAST_TAIL = 0x1p-20f;  // fp32 log probabilities leave less than this undetermined: a tail below it is none (a student without other tokens would lose infinitely by it)
 constexpr int MAX_BITS = 1 << 20;    // tokens that a workgroup can keep a bit of (128 KB)
 
-template <int NW> __device__ __forceinline__ float counted_rows(const int32_t* ids, int64_t T, int k, float* red) {
-  float n = 0.f;
-  for (int64_t i = threadIdx.x; i < T; i += NW * 64) n += ids[i * k] >= 0 ? 1.f : 0.f;
-  return block_sum<NW>(n, red);
+// Rows that are not left out, in COUNTERS shares (a line of memory a row: one workgroup takes 10 us for 4096 rows, these 5).
+__global__ __launch_bounds__(256) void distill_count_kernel(const int32_t* __restrict__ ids, int64_t T, int k, float* __restrict__ n) {
+  __shared__ float red[4];
+  float c = 0.f;
+  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < T; i += COUNTERS * 256) c += ids[i * k] >= 0 ? 1.f : 0.f;
+  c = block_sum<4>(c, red);
+  if (threadIdx.x == 0) n[blockIdx.x] = c;
 }
 
-__global__ __launch_bounds__(1024) void distill_count_kernel(const int32_t* __restrict__ ids, int64_t T, int k, float* __restrict__ n) {
-  __shared__ float red[16];
-  const float c = counted_rows<16>(ids, T, k, red);
-  if (threadIdx.x == 0) *n = c;
-}
-
-__global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ row_loss, const int32_t* __restrict__ ids, int64_t T, int k, float* __restrict__ loss,
-                                                           int mean) {
-  __shared__ float red[16];
-  float s = 0.f;
-  for (int64_t i = threadIdx.x; i < T; i += 1024) s += row_loss[i];
-  s = block_sum<16>(s, red);
-  const float n = mean ? counted_rows<16>(ids, T, k, red) : 1.f;
+// loss = sum of the rows' (/ rows that are not left out); one workgroup, whose loads of both are in flight together.
+__global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ row_loss, const int32_t* __restrict__ ids, const float* __restrict__ counted, int64_t T, int k,
+                                                           float* __restrict__ loss, int mean) {
+  __shared__ float sums[16], counts[16];
+  float s = 0.f, n = 0.f;
+  const bool count = mean && !counted;
+  for (int64_t i = threadIdx.x; i < T; i += blockDim.x) {
+    const int id = count ? ids[i * k] : 0;
+    s += row_loss[i];
+    n += id >= 0 ? 1.f : 0.f;
+  }
+  s = wave_sum(s);
+  n = wave_sum(n);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s, counts[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const int waves = blockDim.x >> 6;
+  s = wave_sum((int)threadIdx.x < waves ? sums[threadIdx.x] : 0.f);
+  n = !mean ? 1.f : wave_sum(counted ? counted[threadIdx.x] : (int)threadIdx.x < waves ? counts[threadIdx.x] : 0.f);
   if (threadIdx.x == 0) *loss = n > 0.f ? s / n : 0.f;
 }
 
@@ -47,160 +57,302 @@ struct Teacher {
   int k;
 };
 
+// What a workgroup knows of its row's teacher: tokens (-1: dropped), probabilities, their logarithms, the student's logits.  (In LDS, so that they take no registers while a
+// row is held there.)
+template <int NW> struct Lds {
+  int id[MAX_TOP];
+  float q[MAX_TOP], logq[MAX_TOP], x[MAX_TOP];
+  float weight, rest, counted;
+  Stat red[NW];
+  float sums[NW];
+};
+
+// The teacher's side of a row, by one wave, two tokens a lane (BUCKET: its tokens' bits too, element i at i + shift; they are zero).  Others read it behind a barrier.
+template <typename T, bool BUCKET, int NW>
+__device__ __forceinline__ void teacher_of(const Teacher& teacher, int64_t row, const T* zr, int V, float inv_tau, unsigned* bits, int shift, Lds<NW>& l) {
+  const int lane = threadIdx.x & 63, k = teacher.k;
+  int id[2];
+  bool mine[2];
+  float t[2], q[2], logq[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int j = lane + 64 * i;
+    id[i] = j < k ? teacher.ids[row * k + j] : -1;
+    t[i] = j < k ? teacher.t[row * k + j] : -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    mine[i] = id[i] >= 0 && id[i] < V;
+    l.x[lane + 64 * i] = mine[i] ? (float)zr[id[i]] : 0.f;
+    if (!mine[i]) t[i] = -INFINITY;
+  }
+  for (int j = 0; j < min(k, 64); j++) {  // a token that is named again counts once
+    const int other = __builtin_amdgcn_readlane(id[0], j);
+    mine[0] = mine[0] && !(j < lane && id[0] == other);
+    mine[1] = mine[1] && id[1] != other;
+  }
+  for (int j = 0; j < k - 64; j++) mine[1] = mine[1] && !(j < lane && id[1] == __builtin_amdgcn_readlane(id[1], j));
+  float sum = 0.f, best = 0.f;
+  if (!BUCKET) best = wave_max(fmaxf(mine[0] ? t[0] : -INFINITY, mine[1] ? t[1] : -INFINITY));
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    logq[i] = BUCKET ? t[i] : (t[i] - best) * inv_tau;
+    q[i] = mine[i] && best > -INFINITY ? exp_of(logq[i]) : 0.f;
+    sum += q[i];
+  }
+  sum = wave_sum(sum);
+  const float r = BUCKET && 1.f - sum >= LEAST_TAIL ? 1.f - sum : 0.f;
+  const float part = BUCKET ? 1.f : sum > 0.f ? 1.f / sum : 0.f, log_part = BUCKET ? 0.f : log_of(sum);
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int j = lane + 64 * i;
+    l.id[j] = mine[i] ? id[i] : -1;
+    l.q[j] = q[i] * part;
+    l.logq[j] = logq[i] - log_part;
+    if (BUCKET && mine[i]) atomicOr(&bits[(id[i] + shift) >> 5], 1u << ((id[i] + shift) & 31));
+  }
+  if (lane == 0) l.weight = BUCKET ? sum + r : sum > 0.f ? 1.f : 0.f, l.rest = r;  // sum of all probabilities; 0: nothing to learn
+}
+
+// A row's loss from its statistics (BUCKET: of the other tokens, against the largest score of all), and what its gradient is made of: exp(z - m) * out dz/dy for the other tokens,
+// (exp(z - m) * in - q * scale) dz/dy for the teacher's.  Every wave sums the tokens by itself.
+struct Factors {
+  float m, out, in, scale;
+};
+template <bool CAP, bool BUCKET, int NW>
+__device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, const Scale& c, float scale, float* row_loss) {
+  const int lane = threadIdx.x & 63;
+  const float weight = l.weight, r = l.rest;
+  Factors f;
+  f.m = uniform(a.ref());
+  float d[2], inside = 0.f, loss = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const bool mine = l.id[lane + 64 * i] >= 0;
+    d[i] = behind<CAP>(l.x[lane + 64 * i], c, f.m);
+    if (BUCKET && mine) inside += exp_of(d[i]);
+  }
+  const float sum = uniform(BUCKET ? a.s + wave_sum(inside) : a.s);
+  const bool none = sum == 0.f;  // no score above minus infinity: no distribution, nothing to learn from
+  const float log_sum = log_of(sum);
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const float q = l.q[lane + 64 * i];
+    if (q > 0.f) loss += q * (l.logq[lane + 64 * i] - (d[i] - log_sum));
+  }
+  loss = wave_sum(loss);
+  if (BUCKET && r > 0.f) loss += r * (log_of(r) - (log_of(a.s) - log_sum));
+  if (threadIdx.x == 0) *row_loss = none ? 0.f : loss;
+  f.scale = none || weight == 0.f ? 0.f : scale * c.inv_tau;
+  const float inv_sum = none ? 0.f : 1.f / sum;
+  f.in = uniform(f.scale * weight * inv_sum);
+  f.out = uniform(f.scale * (weight * inv_sum - (BUCKET && a.s > 1e-30f ? r / a.s : 0.f)));
+  return f;
+}
+template <bool CAP> __device__ __forceinline__ float slope(float x, const Scale& c) {
+  if (!CAP) return 1.f;
+  const float y = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f);
+  return 1.f - y * y;
+}
+template <bool CAP> __device__ __forceinline__ float outside(float x, const Scale& c, const Factors& f) {
+  return exp_of(behind<CAP>(x, c, f.m)) * f.out * slope<CAP>(x, c);
+}
+
+struct RowArgs {
+  Teacher teacher;
+  float* row_loss;
+  const float *drow, *n_counted;
+  int64_t rows;
+  int V;
+  int64_t ld, ldd;
+  float dloss;
+  int mean, pad;
+};
+
 // One workgroup a row.  The first pass takes the statistics and the loss, the second writes the gradient of all tokens, and the k tokens' own follow.
-template <typename T, typename TO, bool CAP, bool BUCKET, int TH>
-__global__ __launch_bounds__(TH) void distill_rows_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, Teacher teacher, float* __restrict__ row_loss,
-                                                          const float* __restrict__ drow, const float* __restrict__ n_counted, int64_t rows, int V, int64_t ld,
-                                                          int64_t ldd, Scale c, float dloss, int mean, int pad) {
+// HELD > 0: a thread keeps that many vectors of the row in registers between the two, all of the row; otherwise the row is streamed, and read again.
+template <typename T, typename TO, bool CAP, bool BUCKET, int TH, int HELD>
+__global__ __launch_bounds__(TH, HELD ? 4 : 1) void distill_rows_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const RowArgs p, const Scale c) {
   constexpr int N = Vec<TO>::N, NW = TH / 64, UNROLL = 4, SPAN = TH * UNROLL;
-  extern __shared__ unsigned bits[];  // BUCKET: of the k tokens, element i at i + shift
-  __shared__ int ids[MAX_TOP];
-  __shared__ Stat red[NW];
-  __shared__ float sums[NW];
+  extern __shared__ unsigned bits[];  // BUCKET
+  __shared__ Lds<NW> l;
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, k = teacher.k;
-  const T* zr = logits + row * ld;
-  TO* dr = dlogits ? dlogits + row * ldd : nullptr;
+  const int tid = threadIdx.x, V = p.V;
+  const T* zr = logits + row * p.ld;
+  TO* dr = dlogits ? dlogits + row * p.ldd : nullptr;
   const Cut cutting = dr ? cut<TO, N>(dr, V) : cut<T, N>(zr, V);
-  if (teacher.ids[row * k] < 0) {  // left out
-    if (tid == 0) row_loss[row] = 0.f;
+  if (p.teacher.ids[row * p.teacher.k] < 0) {  // left out
+    if (tid == 0) p.row_loss[row] = 0.f;
     if (dr) {
       float zero[N] = {};
       for (int v = tid; v < cutting.nvec; v += TH) *reinterpret_cast<u32x4*>(dr + cutting.head + v * N) = Vec<TO>::pack(zero);
       if (tid < cutting.edges) dr[cutting.edge(tid, V)] = (TO)0.f;
-      if (tid < pad) dr[V + tid] = (TO)0.f;
+      if (tid < p.pad) dr[V + tid] = (TO)0.f;
     }
     return;
   }
-  // ---- the teacher's side; thread j has token j
-  const int id = tid < k ? teacher.ids[row * k + tid] : -1;
-  bool mine = id >= 0 && id < V;
-  const float t = mine ? teacher.t[row * k + tid] : -INFINITY;
-  const float xj = mine ? (float)zr[id] : 0.f;
-  if (tid < MAX_TOP) ids[tid] = mine ? id : -1;
-  const int shift = (N - cutting.head) & (N - 1);
-  if (BUCKET)
-    for (int i = tid; i < (V + N + 31) / 32; i += TH) bits[i] = 0;
-  __syncthreads();
-  for (int j = 0; j < tid && mine; j++) mine = ids[j] != id;  // a token that is named again counts once
-  if (BUCKET && mine) atomicOr(&bits[(id + shift) >> 5], 1u << ((id + shift) & 31));
-  float q, logq, r = 0.f;
-  if (BUCKET) {
-    q = mine ? __expf(t) : 0.f;
-    logq = t;
-    r = 1.f - block_sum<NW>(q, sums);
-    if (r < LEAST_TAIL) r = 0.f;
-  } else {
-    const float best = block_max<NW>(mine ? t : -INFINITY, sums);
-    const float d = (t - best) * c.inv_tau, e = mine && best > -INFINITY ? exp_of(d) : 0.f;
-    const float sum = block_sum<NW>(e, sums);
-    q = sum > 0.f ? e / sum : 0.f;
-    logq = d - log_of(sum);
-  }
-  const float weight = block_sum<NW>(q, sums) + r;  // 1, but for rounding; 0: nothing to learn
-  float n = 1.f;
-  if (mean && dr) n = n_counted ? *n_counted : counted_rows<NW>(teacher.ids, rows, k, sums);
-
-  // ---- pass 1: largest score, sum of exponentials (BUCKET: of the other tokens)
   const T* body = zr + cutting.head;
-  const unsigned char* byte_of = reinterpret_cast<const unsigned char*>(bits);
-  auto inside = [&](int v) {  // which elements of a vector are among the k
-    const int at = cutting.head + v * N + shift;
-    return N == 8 ? (unsigned)byte_of[at >> 3] : (byte_of[at >> 3] >> (at & 4)) & 15u;
-  };
-  Raw<T, N> next[UNROLL];
+  Raw<T, N> next[HELD ? 1 : UNROLL], held[HELD ? HELD : 1];
   auto fetch = [&](int at) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; u++)
+    for (int u = 0; u < (HELD ? 1 : UNROLL); u++)
       if (at + u * TH + tid < cutting.nvec) next[u].load(body + (int64_t)(at + u * TH + tid) * N);
   };
-  fetch(0);
-  Stat a = Stat::none();
-  const bool has_edge = tid < cutting.edges;
-  const int edge = has_edge ? cutting.edge(tid, V) : 0;
-  const float edge_x = has_edge ? (float)zr[edge] : -INFINITY;
-  if (has_edge && (CAP || edge_x > -INFINITY)) a.m = score<CAP>(edge_x, c);
-  if (has_edge && !(BUCKET && (bits[(edge + shift) >> 5] >> ((edge + shift) & 31) & 1))) a.s = exp_of(behind<CAP>(edge_x, c, a.ref()));
-  for (int at = 0; at < cutting.nvec; at += SPAN) {
-    Raw<T, N> now[UNROLL];
+  if (HELD) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; u++) now[u] = next[u];
-    fetch(at + SPAN);
-    float cm = -INFINITY;
-    bool any = false;
-#pragma unroll
-    for (int u = 0; u < UNROLL; u++) {
-      if (at + u * TH + tid >= cutting.nvec) continue;
-      any = true;
-      float x[N];
-      now[u].unpack(x);
-#pragma unroll
-      for (int e = 0; e < N; e++) cm = fmaxf(cm, x[e]);
-    }
-    const float top = score<CAP>(cm, c);
-    if (any && top > a.m) a.raise(top);
-    const float ref = a.ref();
-#pragma unroll
-    for (int u = 0; u < UNROLL; u++) {
-      const int v = at + u * TH + tid;
-      if (v >= cutting.nvec) continue;
-      float x[N];
-      now[u].unpack(x);
-#pragma unroll
-      for (int e = 0; e < N; e++) x[e] = exp_of(behind<CAP>(x[e], c, ref));
-      if (BUCKET) {
-        const unsigned in = inside(v);
-        if (in)
-#pragma unroll
-          for (int e = 0; e < N; e++) x[e] = in >> e & 1 ? 0.f : x[e];
-      }
-#pragma unroll
-      for (int w = N / 2; w > 0; w >>= 1)
-#pragma unroll
-        for (int e = 0; e < w; e++) x[e] += x[e + w];
-      a.s += x[0];
-    }
+    for (int i = 0; i < HELD; i++)
+      if (i * TH + tid < cutting.nvec) held[i].load_once(body + (int64_t)(i * TH + tid) * N);
+  } else {
+    fetch(0);
   }
-  a = block_join<NW>(a, red);
-  const float dj = behind<CAP>(xj, c, a.ref()), ej = mine ? exp_of(dj) : 0.f;
-  const float rest = a.s, sum = BUCKET ? rest + block_sum<NW>(ej, sums) : rest;
-  const bool none = sum == 0.f;  // no score above minus infinity: no distribution, nothing to learn from
-  const float log_sum = log_of(sum);
-  float loss = block_sum<NW>(q > 0.f ? q * (logq - (dj - log_sum)) : 0.f, sums);
-  if (BUCKET && r > 0.f) loss += r * (log_of(r) - (log_of(rest) - log_sum));
-  if (tid == 0) row_loss[row] = none ? 0.f : loss;
-  if (!dr) return;
+  const int shift = (N - cutting.head) & (N - 1);
+  if (BUCKET) {
+    for (int i = tid; i < (V + 8 + 31) / 32; i += TH) bits[i] = 0;
+    __syncthreads();
+  }
+  if (tid < 64) teacher_of<T, BUCKET, NW>(p.teacher, row, zr, V, c.inv_tau, bits, shift, l);
+  if (tid >> 6 == 1 && dr && p.mean) {  // the rows that count, by another wave
+    float n = 0.f;
+    if (p.n_counted) n = p.n_counted[tid & 63];
+    else
+      for (int i = tid & 63; i < p.rows; i += 64) n += p.teacher.ids[(int64_t)i * p.teacher.k] >= 0 ? 1.f : 0.f;
+    n = wave_sum(n);
+    if (tid == 64) l.counted = n;
+  }
+  if (BUCKET) __syncthreads();
 
-  // ---- pass 2: the gradient, in place allowed (every thread reads what it writes, the k logits are in registers)
-  const float scale = none || weight == 0.f ? 0.f : dloss * (drow ? drow[row] : 1.f) / n;
-  const float inv_sum = none ? 0.f : 1.f / sum;
-  const float out_scale = scale * (weight * inv_sum - (BUCKET && rest > 1e-30f ? r / rest : 0.f)) * c.inv_tau;
-  auto chain = [&](float x) {
-    if (!CAP) return 1.f;
-    const float y = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f);
-    return 1.f - y * y;
-  };
-  const float m = a.ref();
-  for (int v = tid; v < cutting.nvec; v += TH) {
-    const int i = cutting.head + v * N;
-    Raw<T, N> w;
-    w.load(zr + i);
+  // ---- largest score, sum of exponentials (BUCKET: of the other tokens)
+  const unsigned char* byte_of = reinterpret_cast<const unsigned char*>(bits);
+  auto summed = [&](const Raw<T, N>& w, int first, float ref) {  // of vector first + tid; first is even
     float x[N];
     w.unpack(x);
 #pragma unroll
-    for (int e = 0; e < N; e++) x[e] = exp_of(behind<CAP>(x[e], c, m)) * out_scale * chain(x[e]);
-    *reinterpret_cast<u32x4*>(dr + i) = Vec<TO>::pack(x);
+    for (int e = 0; e < N; e++) x[e] = exp_of(behind<CAP>(x[e], c, ref));
+    if (BUCKET) {  // which elements of the vector are the teacher's
+      const int at = tid + (cutting.head ? 1 : 0);
+      const unsigned in = N == 8 ? (unsigned)byte_of[at + first] : (byte_of[(at >> 1) + (first >> 1)] >> (at & 1) * 4) & 15u;
+      if (in)
+#pragma unroll
+        for (int e = 0; e < N; e++) x[e] = in >> e & 1 ? 0.f : x[e];
+    }
+#pragma unroll
+    for (int w2 = N / 2; w2 > 0; w2 >>= 1)
+#pragma unroll
+      for (int e = 0; e < w2; e++) x[e] += x[e + w2];
+    return x[0];
+  };
+  auto largest = [&](const Raw<T, N>& w, float most) {
+    float x[N];
+    w.unpack(x);
+#pragma unroll
+    for (int e = 0; e < N; e++) most = fmaxf(most, x[e]);
+    return most;
+  };
+  // each pass unpacks a vector when its turn comes: hidden from the compiler, which otherwise keeps all unpacked logits of a pass for the next
+  auto keep = [](Raw<T, N>& w) {
+#pragma unroll
+    for (int i = 0; i < Raw<T, N>::W; i++) asm volatile("" : "+v"(w.w[i]));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // the row's single elements, one to a thread, as max, sum and gradient
+  auto edge_value = [&](int* at) {
+    *at = cutting.edge(tid, V);
+    return (float)zr[*at];
+  };
+  auto edge_sum = [&](float x, int at, float ref) {
+    return BUCKET && (bits[(at + shift) >> 5] >> ((at + shift) & 31) & 1) ? 0.f : exp_of(behind<CAP>(x, c, ref));
+  };
+  const bool has_edge = tid < cutting.edges;
+  int edge;
+  Stat a = Stat::none();
+  if (HELD) {
+    float most = -INFINITY;
+    if (has_edge) most = fmaxf(most, edge_value(&edge));
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      keep(held[i]);
+      if (i * TH + tid < cutting.nvec) most = largest(held[i], most);
+    }
+    most = uniform(block_reduce<NW, true>(most, l.sums));
+    if (CAP || most > -INFINITY) a.m = score<CAP>(most, c);
+    const float ref = a.ref();
+    float sum = 0.f;
+    if (has_edge) {
+      const float x = edge_value(&edge);
+      sum = edge_sum(x, edge, ref);
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      keep(held[i]);
+      if (i * TH + tid < cutting.nvec) sum += summed(held[i], i * TH, ref);
+    }
+    a.s = uniform(block_reduce<NW, false>(sum, l.sums));
+  } else {
+    if (has_edge) {
+      const float x = edge_value(&edge);
+      if (CAP || x > -INFINITY) a.m = score<CAP>(x, c);
+      a.s = edge_sum(x, edge, a.ref());
+    }
+    for (int at = 0; at < cutting.nvec; at += SPAN) {
+      Raw<T, N> now[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; u++) now[u] = next[HELD ? 0 : u];
+      fetch(at + SPAN);
+      float most = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < UNROLL; u++)
+        if (at + u * TH + tid < cutting.nvec) most = largest(now[u], most);
+      const float top = score<CAP>(most, c);
+      if (at + tid < cutting.nvec && top > a.m) a.raise(top);
+      const float ref = a.ref();
+#pragma unroll
+      for (int u = 0; u < UNROLL; u++)
+        if (at + u * TH + tid < cutting.nvec) a.s += summed(now[u], at + u * TH, ref);
+    }
+    a = block_join<NW>(a, l.red);
   }
-  if (has_edge) dr[edge] = (TO)(exp_of(behind<CAP>(edge_x, c, m)) * out_scale * chain(edge_x));
-  if (tid < pad) dr[V + tid] = (TO)0.f;
+  // (a barrier of the reduction lies between the teacher's wave and here)
+  float scale = 0.f;
+  if (dr) scale = uniform(p.dloss * (p.drow ? p.drow[row] : 1.f) / (p.mean ? l.counted : 1.f));
+  const Factors f = factors_of<CAP, BUCKET, NW>(a, l, c, scale, p.row_loss + row);
+  if (!dr) return;
+
+  // ---- the gradient, in place allowed (every thread reads what it writes, the k logits are in registers)
+  auto write = [&](const Raw<T, N>& w, int v) {
+    float x[N];
+    w.unpack(x);
+#pragma unroll
+    for (int e = 0; e < N; e++) x[e] = outside<CAP>(x[e], c, f);
+    *reinterpret_cast<u32x4*>(dr + cutting.head + v * N) = Vec<TO>::pack(x);
+  };
+  if (HELD) {
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      int at = tid;
+      asm volatile("" : "+v"(at));  // (the offsets, which would be kept from the loads, are computed again)
+      keep(held[i]);
+      if (i * TH + at < cutting.nvec) write(held[i], i * TH + at);
+    }
+  } else {
+    for (int v = tid; v < cutting.nvec; v += TH) {
+      Raw<T, N> w;
+      w.load(body + (int64_t)v * N);
+      write(w, v);
+    }
+  }
+  if (has_edge) {
+    const float x = edge_value(&edge);
+    dr[edge] = (TO)outside<CAP>(x, c, f);
+  }
+  if (tid < p.pad) dr[V + tid] = (TO)0.f;
   __syncthreads();  // behind the vectors that hold them
-  if (mine) dr[id] = (TO)((ej * inv_sum * weight - q) * scale * c.inv_tau * chain(xj));
+  if (tid < MAX_TOP && l.id[tid] >= 0) dr[l.id[tid]] = (TO)((exp_of(behind<CAP>(l.x[tid], c, f.m)) * f.in - l.q[tid] * f.scale) * slope<CAP>(l.x[tid], c));
 }
 
 }  // namespace
 
-// Workspace: T floats (row losses) and the number of counted rows.
-extern "C" int64_t olmax_distill_workspace_bytes(int64_t T) { return ((T * 4 + 15) / 16) * 16 + 16; }
+// Workspace: T floats (row losses) and the shares of the number of counted rows.
+extern "C" int64_t olmax_distill_workspace_bytes(int64_t T) { return ((T * 4 + 15) / 16) * 16 + COUNTERS * 4; }
 
 static int distill_check(const char* name, int64_t T, int32_t V, int32_t k, int32_t tail, float temperature, float softcap) {
   OLMAX_CHECK(T > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "%s: bad shape T=%ld V=%d", name, (long)T, V);
@@ -220,20 +372,32 @@ static int distill(hipStream_t stream, const void* logits, void* dlogits, const 
   c.inv_tau = 1.f / temperature;
   float* row_loss = reduction == 2 ? loss : (float*)workspace;
   float* n = nullptr;
-  if (reduction == 0 && dlogits && T > COUNT_IN_ROWS) {
+  if (reduction == 0 && T > COUNT_IN_ROWS) {
     n = (float*)((char*)workspace + ((T * 4 + 15) / 16) * 16);
-    hipLaunchKernelGGL(distill_count_kernel, dim3(1), dim3(1024), 0, stream, ids, T, k, n);
+    hipLaunchKernelGGL(distill_count_kernel, dim3(COUNTERS), dim3(256), 0, stream, ids, T, k, n);
   }
-  const Teacher teacher{ids, t, k};
-#define ROWS(TY, TO, CAPV, BUCKETV, THV)                                                                                                               \
+  const RowArgs args{{ids, t, k}, row_loss, dloss_rows, n, T, V, ld, ldd, dloss, (int)(reduction == 0), pad};
+#define ROWS(TY, TO, CAPV, BUCKETV, THV, HELDV)                                                                                                        \
   do {                                                                                                                                                 \
-    auto kern = distill_rows_kernel<TY, TO, CAPV, BUCKETV, THV>;                                                                                       \
+    auto kern = distill_rows_kernel<TY, TO, CAPV, BUCKETV, THV, HELDV>;                                                                                \
     static std::once_flag attr_once; /* per instantiation */                                                                                           \
     std::call_once(attr_once, [&] { (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, MAX_BITS / 8); });        \
-    hipLaunchKernelGGL(kern, dim3((unsigned)T), dim3(THV), BUCKETV ? (V + 8 + 31) / 32 * 4 : 0, stream, (const TY*)logits, (TO*)dlogits, teacher, row_loss, \
-                       dloss_rows, (const float*)n, T, V, ld, ldd, c, dloss, (int)(reduction == 0), pad);                                              \
+    hipLaunchKernelGGL(kern, dim3((unsigned)T), dim3(THV), BUCKETV ? (V + 8 + 31) / 32 * 4 : 0, stream, (const TY*)logits, (TO*)dlogits, args, c);      \
   } while (0)
-#define ROWS_H(TY, TO, CAPV, BUCKETV) do { if (V <= 16384) ROWS(TY, TO, CAPV, BUCKETV, 256); else ROWS(TY, TO, CAPV, BUCKETV, 512); } while (0)
+  const int vecs = V / (grads_f32 ? 4 : 8);  // of a row, at most
+  // The fewest threads that hold the row; rows that none do are streamed.  us, streamed | held, with gradient: 4096 x 100352 bf16 422 | 338, 4096 x 128256 bf16 558 | 500,
+  // 2048 x 100352 fp32 498 | 338.  1024 threads that hold a row have a CU to themselves: 300 rows of 128256 52 | 61 (64 rows 31 | 31,
+  // 700 115 | 99), so a last round of few rows is streamed instead.  With the LM head, fp32 logits and bf16 gradients: 2048 x 256 x 100352
+  // with its products 876 | 753.
+  const bool alone = T <= 256 || T >= 384;
+#define ROWS_H(TY, TO, CAPV, BUCKETV)                                                                                                              \
+  do {                                                                                                                                             \
+    constexpr bool WIDE = sizeof(TY) != sizeof(TO), HALF = sizeof(TO) == 2; /* a vector of WIDE takes eight registers */                           \
+    if (vecs <= 256 * 8) ROWS(TY, TO, CAPV, BUCKETV, 256, 8);                                                                                      \
+    else if (vecs <= 512 * (WIDE ? 13 : 25)) ROWS(TY, TO, CAPV, BUCKETV, 512, (WIDE ? 13 : 25));                                                   \
+    else if (alone && vecs <= 1024 * (WIDE ? 13 : HALF ? 20 : 25)) ROWS(TY, TO, CAPV, BUCKETV, 1024, (WIDE ? 13 : HALF ? 20 : 25)); \
+    else ROWS(TY, TO, CAPV, BUCKETV, 512, 0);                                                                                                      \
+  } while (0)
 #define ROWS_B(TY, TO, CAPV) do { if (tail) ROWS_H(TY, TO, CAPV, true); else ROWS_H(TY, TO, CAPV, false); } while (0)
 #define ROWS_C(TY, TO) do { if (softcap > 0.f) ROWS_B(TY, TO, true); else ROWS_B(TY, TO, false); } while (0)
   if (logits_f32 && grads_f32) ROWS_C(float, float); else if (logits_f32) ROWS_C(float, bf16); else ROWS_C(bf16, bf16);
@@ -241,7 +405,7 @@ static int distill(hipStream_t stream, const void* logits, void* dlogits, const 
 #undef ROWS_H
 #undef ROWS_B
 #undef ROWS_C
-  if (reduction != 2) hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, stream, (const float*)row_loss, ids, T, k, loss, (int)(reduction == 0));
+  if (reduction != 2) hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(T <= 256 ? 256 : 1024), 0, stream, (const float*)row_loss, ids, (const float*)n, T, k, loss, (int)(reduction == 0));
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }

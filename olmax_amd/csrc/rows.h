@@ -52,6 +52,10 @@ template <typename T, int N> struct Raw {
 #pragma unroll
     for (int i = 0; i < W; i++) w[i] = *reinterpret_cast<const u32x4_any*>(p + i * Vec<T>::N);
   }
+  __device__ __forceinline__ void load_once(const T* p) {
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p + i * Vec<T>::N));
+  }
   __device__ __forceinline__ void unpack(float* f) const {
 #pragma unroll
     for (int i = 0; i < W; i++) Vec<T>::unpack(w[i], f + i * Vec<T>::N);
@@ -78,6 +82,8 @@ template <bool CAP> __device__ __forceinline__ float capped(float x, const Scale
   return CAP ? c.cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f)) : x;
 }
 template <bool CAP> __device__ __forceinline__ float score(float x, const Scale& c) { return capped<CAP>(x, c) * c.inv_tau; }
+// a value that all threads of the workgroup have, in a scalar register
+__device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 // z - m
 template <bool CAP> __device__ __forceinline__ float behind(float x, const Scale& c, float m) { return __builtin_fmaf(capped<CAP>(x, c), c.inv_tau, -m); }
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
@@ -105,6 +111,18 @@ struct Stat {
     t += b.t;
   }
 };
+// Largest value and sum of a workgroup of NW waves (a power of two), with one register for the waves' results, which each lane has one of.
+template <int NW, bool MAX> __device__ __forceinline__ float block_reduce(float v, float* red) {
+  auto both = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+  v = MAX ? wave_max(v) : wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[threadIdx.x & (NW - 1)];
+#pragma unroll
+  for (int o = NW / 2; o > 0; o >>= 1) v = both(v, __shfl_xor(v, o, 64));
+  return v;
+}
 template <int NW> __device__ __forceinline__ Stat block_join(Stat a, Stat* red) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
