@@ -193,21 +193,6 @@ int olmax_gemm_grads(hipStream_t s, const bf16* dy, const bf16* w, const bf16* x
 int olmax_lmhead_ce_scratch(hipStream_t stream, const void* h, const void* W, const int32_t* labels, float* loss, void* dh, void* dW,
                             void* workspace, int64_t workspace_bytes, int64_t T, int32_t d, int32_t V, int32_t ignore_index,
                             float softcap, int32_t dw_f32, GemmScratch scratch);
-// gemm.hip: the LM head's product with a row's part of its softmax in the epilogue (logprobs.hip): logits leave the kernel only as what is formed of them.
-struct HeadRows {
-  const int32_t* targets;     // [M]
-  int32_t ignore_index, V;    // V: of the whole product; a target from there on has no logit
-  float cap, cap_k, inv_tau;  // z = cap(x) * inv_tau; cap_k = 2 log2(e) / cap; cap 0: none
-  float *parts, *target_logit;  // statistics: [ceil(N / 256)][M][3], (largest score, sum of exponentials behind it, that sum weighted by z - m) of 256 columns; the
-                                // logit x of each target that is one of the columns
-  const float *stats, *dlogprobs, *dentropy;  // gradients: from [M, 3], [M], [M] (optional)
-};
-// Whether the forms run on a product of that size (operands 16-byte aligned, rows of K numbers), and how many of the N columns they take: whole rounds of tiles, or all;
-// 0: the plain product does better.
-int olmax_gemm_head_columns(int M, int N, int K);
-int olmax_gemm_head_stats(hipStream_t s, const bf16* h, const bf16* w, int M, int N, int K, const HeadRows& rows);
-// d [M, ldd] (16-byte aligned, ldd a multiple of 8): columns 0 .. N
-int olmax_gemm_head_grads(hipStream_t s, const bf16* h, const bf16* w, bf16* d, int64_t ldd, int M, int N, int K, const HeadRows& rows);
 // lmhead_ce.hip: dh [T, d] = dlogits W and dW [V, d] = dlogits^T h of dlogits [T, V] whose rows are zero up to a multiple of 8; either may be null
 int olmax_lmhead_products(hipStream_t stream, const bf16* dlogits, const bf16* W, const bf16* h, bf16* dh, void* dW, int T, int d, int V, int64_t ldl,
                           bool dw_f32, GemmScratch scratch = GemmScratch());

@@ -114,8 +114,8 @@ __device__ __forceinline__ void teacher_of(const Teacher& teacher, int64_t row, 
   if (lane == 0) l.weight = BUCKET ? sum + r : sum > 0.f ? 1.f : 0.f, l.rest = r;  // sum of all probabilities; 0: nothing to learn
 }
 
-// A row's loss from its statistics (BUCKET: of the other tokens, against the largest score of all), and what its gradient is made of: exp(z - m) * out dz/dy for the other tokens,
-// (exp(z - m) * in - q * scale) dz/dy for the teacher's.  Every wave sums the tokens by itself.
+// A row's loss from its statistics (BUCKET: of the other tokens, against the largest score of all), and what its gradient is made of: exp(z - m) * out dz/dx for the other tokens,
+// (exp(z - m) * in - q * scale) dz/dx for the teacher's.  Every wave sums the tokens by itself.
 struct Factors {
   float m, out, in, scale;
 };
@@ -143,16 +143,11 @@ __device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, c
   loss = wave_sum(loss);
   if (BUCKET && r > 0.f) loss += r * (log_of(r) - (log_of(a.s) - log_sum));
   if (threadIdx.x == 0) *row_loss = none ? 0.f : loss;
-  f.scale = none || weight == 0.f ? 0.f : scale * c.inv_tau;
+  f.scale = none || weight == 0.f ? 0.f : scale;
   const float inv_sum = none ? 0.f : 1.f / sum;
   f.in = uniform(f.scale * weight * inv_sum);
   f.out = uniform(f.scale * (weight * inv_sum - (BUCKET && a.s > 1e-30f ? r / a.s : 0.f)));
   return f;
-}
-template <bool CAP> __device__ __forceinline__ float slope(float x, const Scale& c) {
-  if (!CAP) return 1.f;
-  const float y = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f);
-  return 1.f - y * y;
 }
 template <bool CAP> __device__ __forceinline__ float outside(float x, const Scale& c, const Factors& f) {
   return exp_of(behind<CAP>(x, c, f.m)) * f.out * slope<CAP>(x, c);
@@ -366,10 +361,7 @@ static int distill_check(const char* name, int64_t T, int32_t V, int32_t k, int3
 static int distill(hipStream_t stream, const void* logits, void* dlogits, const int32_t* ids, const float* t, float* loss, const float* dloss_rows,
                    void* workspace, int64_t T, int32_t V, int32_t k, int64_t ld, int64_t ldd, bool logits_f32, bool grads_f32, int32_t tail, float temperature,
                    float softcap, float dloss, int32_t reduction, int pad) {
-  Scale c;
-  c.cap = softcap;
-  c.cap_k = softcap > 0.f ? 2.f * LOG2E / softcap : 0.f;
-  c.inv_tau = 1.f / temperature;
+  const Scale c = scale_of(temperature, softcap);
   float* row_loss = reduction == 2 ? loss : (float*)workspace;
   float* n = nullptr;
   if (reduction == 0 && T > COUNT_IN_ROWS) {

@@ -684,8 +684,8 @@ __device__ __forceinline__ void gemm_tile(
     for (int i = 0; i < TM; i++) targets[i] = head->targets ? head->targets[m0 + wm * WM + i * 16 + l16e] : -1;
     __syncthreads();  // every wave is done reading the operand stages
     rows::Stat* strip = reinterpret_cast<rows::Stat*>(smem);  // [WAVES_N][BM]
-    const rows::Scale c{head->cap, head->cap_k, head->inv_tau};
-    const bool cap = head->cap > 0.f;
+    const rows::Scale c = head->scale;
+    const bool cap = c.cap > 0.f;
     const int first = wn * WN + g16e * 4;  // this lane's first column of the block
     auto here = [&](int j, int r) { return !RAG || first + j * 16 + r >= col_lo; };
     auto of_row = [&](auto capped, const f32x4* x, int row, int target) {
@@ -740,8 +740,8 @@ __device__ __forceinline__ void gemm_tile(
   }
   if constexpr (ROW_GRADS) {
     // d = p (-g - h (ln p + H)), and g more at the target, times the scores' slope; then out as any bf16 result
-    const rows::Scale c{head->cap, head->cap_k, head->inv_tau};
-    const bool cap = head->cap > 0.f;
+    const rows::Scale c = head->scale;
+    const bool cap = c.cap > 0.f;
     const int first = n0 + wn * WN + g16e * 4;
     auto of_row = [&](auto capped, f32x4* x, int64_t row) {
       constexpr bool CAP = decltype(capped)::value;

@@ -9,7 +9,7 @@ using namespace rows;
 
 namespace {
 
-constexpr int TH = 256;       // threads of a workgroup
+constexpr int GROUPS = 256;   // of threads whose largest logits bound the alternatives
 constexpr int UNROLL = 4;     // vectors of a thread that are in flight, and reduced against one maximum
 constexpr int MAX_TOP = 128;
 constexpr int CAND = 1024;    // candidates for the alternatives that a workgroup can hold
@@ -26,19 +26,25 @@ constexpr unsigned KEY_NEG_INF = 0x007fffffu;
 __device__ __forceinline__ uint64_t entry_of(unsigned key, int index) { return ((uint64_t)key << 32) | (0xffffffffu - (unsigned)index); }
 __device__ __forceinline__ int index_of(uint64_t e) { return (int)(0xffffffffu - (unsigned)e); }
 
-struct Lds {
-  alignas(16) unsigned best[TH];  // key of each thread's largest
+template <int TH> struct Lds {
+  alignas(16) unsigned best[GROUPS];  // key of the largest of each group of threads
   uint64_t cand[CAND];
   unsigned hist[256];
   Stat red[TH / 64];
   int n, sums[TH / 64];
 };
 
-// A lower bound of the k-th largest value that the workgroup has seen, from the largest of each thread: at least k values are not below the k-th
-// largest of those.  Found on the upper 16 bits of the keys, by bits: each wave counts all TH of them, four a lane.
+// A lower bound of the k-th largest value that the workgroup has seen, from the largest of each group of threads: at least k values are not below the k-th
+// largest of those.  Found on the upper 16 bits of the keys, by bits: each wave counts all groups, four a lane.
+template <int TH>
 __device__ __forceinline__ unsigned kth_best(unsigned* best, unsigned own, int k) {
+  static_assert(TH == GROUPS || TH == 4 * GROUPS, "a thread or four to a group");
+  if (TH > GROUPS) {
+    own = max(own, (unsigned)__shfl_xor((int)own, 1, 64));
+    own = max(own, (unsigned)__shfl_xor((int)own, 2, 64));
+  }
   __syncthreads();
-  best[threadIdx.x] = own;
+  if (TH == GROUPS || (threadIdx.x & 3) == 0) best[threadIdx.x / (TH / GROUPS)] = own;
   __syncthreads();
   const u32x4 q = *reinterpret_cast<const u32x4*>(best + (threadIdx.x & 63) * 4);
   unsigned at = 0;
@@ -56,13 +62,13 @@ __device__ __forceinline__ unsigned kth_best(unsigned* best, unsigned own, int k
 // The exact way, for rows with more values that tie at the bound than there is room: the k largest of elements [lo, hi) above minus infinity go
 // to cand, in any order; returns how many.  The k-th largest key by four passes of 8 bits, then all above it, then as many equal ones as are
 // missing, from the lowest index on.
-template <typename T>
-__device__ int select_exact(const T* zr, int lo, int hi, int k, Lds& l) {
+template <typename T, int TH>
+__device__ int select_exact(const T* zr, int lo, int hi, int k, Lds<TH>& l) {
   unsigned at = 0;
   int need = k;
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
-    l.hist[threadIdx.x] = 0;
+    if (threadIdx.x < 256) l.hist[threadIdx.x] = 0;
     __syncthreads();
     for (int i = lo + threadIdx.x; i < hi; i += TH) {
       const float x = (float)zr[i];
@@ -109,7 +115,7 @@ __device__ int select_exact(const T* zr, int lo, int hi, int k, Lds& l) {
 }
 
 // Leaves of cand[0 .. n) those whose key is at least `bound`, in any order, and returns how many.  Each thread holds its share meanwhile.
-template <int ROOM>
+template <int ROOM, int TH>
 __device__ __forceinline__ int narrow(uint64_t* cand, int n, unsigned bound, int* counter) {
   uint64_t own[ROOM / TH];
   __syncthreads();
@@ -127,13 +133,22 @@ __device__ __forceinline__ int narrow(uint64_t* cand, int n, unsigned bound, int
   return *counter;
 }
 
-// emit(rank, entry) for the k largest of cand[0 .. n): an entry's rank is the number of larger ones (all are different).
-template <typename F>
-__device__ __forceinline__ void ranked(const uint64_t* cand, int n, int k, F emit) {
+// emit(rank, entry) for the k largest of cand[0 .. n): an entry's rank is the number of larger ones (all are different).  Room for a multiple of 8; eight are read at a
+// time (one by one 128 of them take 5 us).
+template <int TH, typename F>
+__device__ __forceinline__ void ranked(uint64_t* cand, int n, int k, F emit) {
+  if (threadIdx.x < 8 && (n & 7) && (n & ~7) + (int)threadIdx.x >= n) cand[(n & ~7) + threadIdx.x] = 0;
+  __syncthreads();
   for (int i = threadIdx.x; i < n; i += TH) {
     const uint64_t e = cand[i];
     int rank = 0;
-    for (int j = 0; j < n; j++) rank += cand[j] > e;
+    for (int j = 0; j < n; j += 8) {
+      uint64_t o[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) o[u] = cand[j + u];
+#pragma unroll
+      for (int u = 0; u < 8; u++) rank += o[u] > e;
+    }
     if (rank < k) emit(rank, e);
   }
 }
@@ -167,13 +182,13 @@ __device__ __forceinline__ void write_row(const Out& o, int64_t row, bool has_ta
   o.stats[row * 3 + 2] = entropy;
 }
 // The n <= k largest logits above minus infinity are cand[0 .. n) or are the largest of them; the rest of k slots gets the lowest indices that are not among them.
-template <bool CAP>
-__device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, const uint64_t* cand, int n, const Scale& c, const Stat& a) {
+template <bool CAP, int TH>
+__device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, uint64_t* cand, int n, const Scale& c, const Stat& a) {
   int32_t* ids = o.top_ids + row * k;
   float* lp = o.top_logprobs + row * k;
   const float log_sum = log_of(a.s);
   const bool none = a.s == 0.f;
-  ranked(cand, n, k, [&](int rank, uint64_t e) {
+  ranked<TH>(cand, n, k, [&](int rank, uint64_t e) {
     ids[rank] = index_of(e);
     lp[rank] = none ? -INFINITY : behind<CAP>(value_of((unsigned)(e >> 32)), c, a.m) - log_sum;
   });
@@ -194,11 +209,11 @@ __device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, cons
 }
 
 // One workgroup to a row, or to one of `parts` equal shares of it; with part_stat a share leaves its statistics and its candidates for a kernel that joins them.
-template <typename T, bool CAP, bool TOP>
+template <typename T, bool CAP, bool TOP, int TH>
 __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out, uint64_t* __restrict__ part_top,
                                                         Stat* __restrict__ part_stat, int V, int64_t ld, int32_t ignore_index, Scale c, int k, int parts) {
   constexpr int N = Vec<T>::N, SPAN = TH * UNROLL;
-  __shared__ Lds l;
+  __shared__ Lds<TH> l;
   const int64_t row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
   const int target = targets ? targets[row] : -1;
@@ -225,12 +240,6 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
   float most = -INFINITY;  // of the logits themselves
   unsigned bound = KEY_NEG_INF;
   float bound_value = -INFINITY;
-  auto offer = [&](float x, int i) {
-    if (x >= bound_value && x > -INFINITY) {
-      const int at = atomicAdd(&l.n, 1);
-      if (at < CAND) l.cand[at] = entry_of(key_of(x), i);
-    }
-  };
   // the single elements at the row's ends, one to a thread
   const bool has_edge = part == 0 && (int)threadIdx.x < cutting.edges;
   const int edge = has_edge ? cutting.edge(threadIdx.x, V) : 0;
@@ -249,14 +258,16 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) now[u] = next[u];
     if (ch + 1 < chunks) fetch(at + SPAN);
-    float cm = -INFINITY;
+    float cm = -INFINITY, vm[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
+      vm[u] = -INFINITY;
       if (at + u * TH + (int)threadIdx.x >= v1) continue;
       float x[N];
       now[u].unpack(x);
 #pragma unroll
-      for (int e = 0; e < N; e++) cm = fmaxf(cm, x[e]);
+      for (int e = 0; e < N; e++) vm[u] = fmaxf(vm[u], x[e]);
+      cm = fmaxf(cm, vm[u]);
     }
     if (cm > most || (CAP && a.m == -INFINITY)) {  // (a soft-cap makes a score of minus infinity too)
       most = fmaxf(most, cm);
@@ -282,30 +293,59 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
       a.t += t[0];
     }
     if (TOP) {
-      if ((ch & (ch + 1)) == 0) {  // 1, 2, 4, .. chunks seen: about k candidates between two bounds
-        bound = kth_best(l.best, key_of(most), k);
+      if ((ch & (ch + 1)) == 0) {  // 1, 2, 4, .. chunks seen: about k candidates between two bounds, and those below the new one go where many ties came with them
+        bound = kth_best<TH>(l.best, key_of(most), k);
         bound_value = value_of(bound);
+        if (l.n > CAND / 2 && l.n <= CAND) narrow<CAND, TH>(l.cand, l.n, bound, &l.n);  // (all read l.n between two barriers)
       }
-      if (ch == 0 && has_edge) offer(edge_x, edge);
-      if (cm >= bound_value) {
+      // vectors with a candidate are noted, with their largest; which of their elements are is seen at the end, against the last bound.  (Element by element here: 1600 x 128256
+      // with 20 alternatives 120 us, so 96.)
+      if (cm >= bound_value && cm > -INFINITY) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-          const int v = at + u * TH + threadIdx.x;
-          if (v >= v1) continue;
-          float x[N];
-          now[u].unpack(x);
-#pragma unroll
-          for (int e = 0; e < N; e++) offer(x[e], cutting.head + v * N + e);
-        }
+        for (int u = 0; u < UNROLL; u++)
+          if (vm[u] >= bound_value && vm[u] > -INFINITY) {
+            const int to = atomicAdd(&l.n, 1);
+            if (to < CAND) l.cand[to] = entry_of(key_of(vm[u]), at + u * TH + threadIdx.x);
+          }
       }
     }
   }
   const Stat all = block_join<TH / 64>(a, l.red);
   int n = 0;
   if (TOP) {
-    if (((chunks - 1) & chunks) != 0) bound = kth_best(l.best, key_of(most), k);  // of all that was seen
+    if (((chunks - 1) & chunks) != 0) bound = kth_best<TH>(l.best, key_of(most), k);  // of all that was seen
     __syncthreads();
     n = l.n;
+    __syncthreads();
+    if (n <= CAND) {
+      bound_value = value_of(bound);
+      auto offer = [&](float x, int i) {
+        if (x >= bound_value && x > -INFINITY) {
+          const int to = atomicAdd(&l.n, 1);
+          if (to < CAND) l.cand[to] = entry_of(key_of(x), i);
+        }
+      };
+      uint64_t own[CAND / TH];
+#pragma unroll
+      for (int i = 0; i < CAND / TH; i++) own[i] = i * TH + (int)threadIdx.x < n ? l.cand[i * TH + threadIdx.x] : 0;
+      if (threadIdx.x == 0) l.n = 0;
+      __syncthreads();
+      Raw<T, N> r[CAND / TH];
+#pragma unroll
+      for (int i = 0; i < CAND / TH; i++)
+        if ((unsigned)(own[i] >> 32) >= bound) r[i].load(body + (int64_t)index_of(own[i]) * N);
+#pragma unroll
+      for (int i = 0; i < CAND / TH; i++)
+        if ((unsigned)(own[i] >> 32) >= bound) {
+          float x[N];
+          r[i].unpack(x);
+#pragma unroll
+          for (int e = 0; e < N; e++) offer(x[e], cutting.head + index_of(own[i]) * N + e);
+        }
+      if (has_edge) offer(edge_x, edge);
+      __syncthreads();
+      n = l.n;
+    }
     if (n > CAND) {
       const int first = part == 0 ? 0 : cutting.head + v0 * N;  // part 0 has the edges: the row's first elements and its last
       const int last = cutting.head + v1 * N;
@@ -327,31 +367,29 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
           n = l.n;
         }
       }
-    } else {
-      n = narrow<CAND>(l.cand, n, bound, &l.n);
     }
   }
   if (!part_stat) {
     const bool has_target = target >= 0 && target < V;
     if (threadIdx.x == 0) write_row<CAP>(out, row, has_target, has_target ? (float)zr[target] : 0.f, c, all);
-    if (TOP) write_top<CAP>(out, row, k, l.cand, n, c, all);
+    if (TOP) write_top<CAP, TH>(out, row, k, l.cand, n, c, all);
     return;
   }
   if (threadIdx.x == 0) part_stat[blockIdx.x] = all;
   if (TOP) {
     uint64_t* mine = part_top + (int64_t)blockIdx.x * k;
-    ranked(l.cand, n, k, [&](int rank, uint64_t e) { mine[rank] = e; });
+    ranked<TH>(l.cand, n, k, [&](int rank, uint64_t e) { mine[rank] = e; });
     for (int i = n + threadIdx.x; i < k; i += TH) mine[i] = 0;
   }
 }
 
 // The parts of a row, one workgroup a row.
-template <typename T, bool CAP, bool TOP>
+template <typename T, bool CAP, bool TOP, int TH = 256>
 __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out,
                                                         const uint64_t* __restrict__ part_top, const Stat* __restrict__ part_stat, int V, int64_t ld,
                                                         int32_t ignore_index, Scale c, int k, int parts) {
   __shared__ uint64_t cand[JOINED];
-  __shared__ alignas(16) unsigned best[TH];
+  __shared__ alignas(16) unsigned best[GROUPS];
   __shared__ Stat red[TH / 64];
   __shared__ int counter;
   const int64_t row = blockIdx.x;
@@ -373,9 +411,9 @@ __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ lo
   const bool has_target = target >= 0 && target < V;
   if (threadIdx.x == 0) write_row<CAP>(out, row, has_target, has_target ? (float)logits[row * ld + target] : 0.f, c, a);
   if (TOP) {
-    const unsigned bound = kth_best(best, max((unsigned)(most >> 32), KEY_NEG_INF), k);
-    const int n = narrow<JOINED>(cand, parts * k, bound, &counter);
-    write_top<CAP>(out, row, k, cand, n, c, a);
+    const unsigned bound = kth_best<TH>(best, max((unsigned)(most >> 32), KEY_NEG_INF), k);
+    const int n = narrow<JOINED, TH>(cand, parts * k, bound, &counter);
+    write_top<CAP, TH>(out, row, k, cand, n, c, a);
   }
 }
 
@@ -423,7 +461,7 @@ __global__ __launch_bounds__(256) void zero_columns_kernel(bf16* __restrict__ d,
 
 // d loss / d logits of logprob and entropy: dz_i = g (delta_it - p_i) - h p_i (ln p_i + H), from the statistics that the forward pass kept.
 // A workgroup takes one of `parts` shares of a row.  first: the column of the whole row that these logits begin with (they are its last).
-template <typename T, typename TO, bool CAP, bool ENT>
+template <typename T, typename TO, bool CAP, bool ENT, int TH = 256>
 __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const int32_t* __restrict__ targets,
                                                         const float* __restrict__ stats, const float* __restrict__ dlogprobs,
                                                         const float* __restrict__ dentropy, int V, int64_t ld, int64_t ldd, int32_t ignore_index, Scale c,
@@ -460,27 +498,28 @@ __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ lo
   if (part == 0 && (int)threadIdx.x < pad) dr[V + threadIdx.x] = (TO)0.f;
 }
 
-Scale scale_of(float temperature, float softcap) {
-  Scale c;
-  c.cap = softcap;
-  c.cap_k = softcap > 0.f ? 2.f * LOG2E / softcap : 0.f;
-  c.inv_tau = 1.f / temperature;
-  return c;
-}
-
-// Shares of a row in the forward pass: rows that fill the GPU by themselves are whole.
-int parts_of(int64_t T, int V, int top, bool f32) {
+// Threads of a workgroup and shares of a row in the forward pass.
+struct Form {
+  int threads, parts;
+};
+// Rows that fill the GPU by themselves take a workgroup of 256 threads each; up to 256 long ones one of 1024; few ones come in shares of one round of loads (1024 vectors), whose
+// candidates a second launch joins: many of those cost more than longer shares of 1024 threads.  us in a graph, bf16, 256 threads x 1 | 1024 x 1 | 256 x 16 | 1024 x 4: 1 x 128256 without
+// alternatives 17.0 | 13.5 | 7.4 | 10.2, with 20 28.8 | 23.2 | 13.4 | 17, with 128 35.8 | 25.7 | 45 | 20.9; 200 x 128256 with 20 31.1 | 25.4 | 30 | 37; 400 x 128256 with 20 38.5 | 47.8;
+// 37 x 50304 without 9.8 | 9.2 | (8 shares) 8.2; 100 x 4096 without 4.7 | 6.2.
+Form form_of(int64_t T, int V, int top, bool f32) {
   const int64_t vecs = V / (f32 ? 4 : 8);
-  int64_t p = std::min<int64_t>(1024 / T, vecs / (TH * 2));
-  if (top > 0) p = std::min<int64_t>(p, JOINED / top);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(p, 64));
+  if (T > 256 || vecs < 2048) return {256, 1};
+  if (T > 128) return {vecs < 6000 ? 256 : 1024, 1};
+  const int64_t shares = std::min<int64_t>(std::min<int64_t>(vecs / 1024, 1024 / T), 32);
+  if (shares * top <= 640) return {256, (int)shares};
+  return {1024, (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(vecs / 4096, 512 / top), 256 / T))};
 }
 
 }  // namespace
 
 extern "C" int64_t olmax_token_logprobs_workspace_bytes(int64_t T, int32_t V, int32_t top, int32_t logits_f32) {
   if (T <= 0 || V <= 0) return 0;
-  const int parts = parts_of(T, V, top, logits_f32 != 0);
+  const int parts = form_of(T, V, top, logits_f32 != 0).parts;
   return parts == 1 ? 0 : T * parts * ((int64_t)std::max(top, 0) * 8 + (int64_t)sizeof(Stat));
 }
 
@@ -493,24 +532,28 @@ extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, 
               "olmax_token_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, top);
   OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_token_logprobs: temperature within 1e-6 and 1e6, softcap not negative");
   OLMAX_CHECK(((uintptr_t)logits & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_token_logprobs: logits not aligned to their type");
-  const int parts = parts_of(T, V, top, logits_f32 != 0);
+  const Form form = form_of(T, V, top, logits_f32 != 0);
+  const int parts = form.parts;
   OLMAX_CHECK(workspace_bytes >= olmax_token_logprobs_workspace_bytes(T, V, top, logits_f32) && (parts == 1 || (workspace && aligned16(workspace))), OLMAX_ERR_WORKSPACE,
               "olmax_token_logprobs: workspace needs %ld bytes, 16-byte aligned", (long)olmax_token_logprobs_workspace_bytes(T, V, top, logits_f32));
   uint64_t* part_top = (uint64_t*)workspace;
   Stat* part_stat = parts == 1 ? nullptr : (Stat*)((char*)workspace + T * parts * (int64_t)top * 8);
   const Out out{logprobs, entropy, stats, top ? top_logprobs : nullptr, top ? top_ids : nullptr};
   const Scale c = scale_of(temperature, softcap);
+#define ROWS(TY, CAPV, TOPV, THV)                                                                                                                             \
+  hipLaunchKernelGGL((score_rows_kernel<TY, CAPV, TOPV, THV>), dim3((unsigned)(T * parts)), dim3(THV), 0, stream, (const TY*)logits, targets, out, part_top, \
+                     part_stat, V, ld, ignore_index, c, top, parts)
 #define SCORE(TY, CAPV, TOPV)                                                                                                                             \
   do {                                                                                                                                                    \
-    hipLaunchKernelGGL((score_rows_kernel<TY, CAPV, TOPV>), dim3((unsigned)(T * parts)), dim3(TH), 0, stream, (const TY*)logits, targets, out, part_top, \
-                       part_stat, V, ld, ignore_index, c, top, parts);                                                                                    \
+    if (form.threads == 256) ROWS(TY, CAPV, TOPV, 256); else ROWS(TY, CAPV, TOPV, 1024);                                                                  \
     if (parts > 1)                                                                                                                                        \
-      hipLaunchKernelGGL((score_join_kernel<TY, CAPV, TOPV>), dim3((unsigned)T), dim3(TH), 0, stream, (const TY*)logits, targets, out,                    \
+      hipLaunchKernelGGL((score_join_kernel<TY, CAPV, TOPV>), dim3((unsigned)T), dim3(256), 0, stream, (const TY*)logits, targets, out,                   \
                          (const uint64_t*)part_top, (const Stat*)part_stat, V, ld, ignore_index, c, top, parts);                                          \
   } while (0)
 #define SCORE_T(TY, CAPV) do { if (top) SCORE(TY, CAPV, true); else SCORE(TY, CAPV, false); } while (0)
 #define SCORE_C(TY) do { if (softcap > 0.f) SCORE_T(TY, true); else SCORE_T(TY, false); } while (0)
   if (logits_f32) SCORE_C(float); else SCORE_C(bf16);
+#undef ROWS
 #undef SCORE
 #undef SCORE_T
 #undef SCORE_C
@@ -523,10 +566,10 @@ static int token_logprobs_bwd(hipStream_t stream, const void* logits, const int3
                               const float* dentropy, void* dlogits, int64_t T, int32_t V, int64_t ld, int64_t ldd, bool logits_f32, bool grads_f32,
                               int32_t ignore_index, float temperature, float softcap, int pad, int first = 0) {
   const Scale c = scale_of(temperature, softcap);
-  const int parts = (int)std::max<int64_t>(1, V / (grads_f32 ? 4 : 8) / (TH * 8));
+  const int parts = (int)std::max<int64_t>(1, V / (grads_f32 ? 4 : 8) / 2048);
   OLMAX_CHECK(T * parts < (1LL << 31), OLMAX_ERR_SHAPE, "olmax_token_logprobs_bwd: T=%ld rows of V=%d are too many", (long)T, V);
 #define GRAD(TY, TO, CAPV, ENTV)                                                                                                                             \
-  hipLaunchKernelGGL((score_grad_kernel<TY, TO, CAPV, ENTV>), dim3((unsigned)(T * parts)), dim3(TH), 0, stream, (const TY*)logits, (TO*)dlogits, targets, stats, \
+  hipLaunchKernelGGL((score_grad_kernel<TY, TO, CAPV, ENTV>), dim3((unsigned)(T * parts)), dim3(256), 0, stream, (const TY*)logits, (TO*)dlogits, targets, stats, \
                      dlogprobs, dentropy, V, ld, ldd, ignore_index, c, parts, pad, first)
 #define GRAD_E(TY, TO, CAPV) do { if (dentropy) GRAD(TY, TO, CAPV, true); else GRAD(TY, TO, CAPV, false); } while (0)
 #define GRAD_C(TY, TO) do { if (softcap > 0.f) GRAD_E(TY, TO, true); else GRAD_E(TY, TO, false); } while (0)
@@ -605,11 +648,11 @@ extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, cons
   rows.targets = targets;
   rows.ignore_index = ignore_index;
   rows.V = V;
-  rows.cap = c.cap, rows.cap_k = c.cap_k, rows.inv_tau = c.inv_tau;
+  rows.scale = c;
   rows.parts = (float*)tiles;
   rows.target_logit = target_logit;
   if (int rc = olmax_gemm_head_stats(stream, hp, wp, (int)T, p.fused, d, rows)) return rc;
-#define JOIN(CAPV)                                                                                                                                                        do {                                                                                                                                                                      if (rest)                                                                                                                                                                 hipLaunchKernelGGL((score_rows_kernel<float, CAPV, false>), dim3((unsigned)T), dim3(TH), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,                          p.ld, ignore_index, c, 0, 1);                                                                                                                      hipLaunchKernelGGL((head_join_kernel<CAPV>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,                        (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, V, p.fused, ignore_index, c);                                                 } while (0)
+#define JOIN(CAPV)                                                                                                                                                        do {                                                                                                                                                                      if (rest)                                                                                                                                                                 hipLaunchKernelGGL((score_rows_kernel<float, CAPV, false, 256>), dim3((unsigned)T), dim3(256), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,                          p.ld, ignore_index, c, 0, 1);                                                                                                                      hipLaunchKernelGGL((head_join_kernel<CAPV>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,                        (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, V, p.fused, ignore_index, c);                                                 } while (0)
   if (softcap > 0.f) JOIN(true); else JOIN(false);
 #undef JOIN
   OLMAX_LAUNCH_CHECK();
@@ -643,7 +686,7 @@ extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, 
     rows.targets = targets;
     rows.ignore_index = ignore_index;
     rows.V = V;
-    rows.cap = c.cap, rows.cap_k = c.cap_k, rows.inv_tau = c.inv_tau;
+    rows.scale = c;
     rows.stats = stats, rows.dlogprobs = dlogprobs, rows.dentropy = dentropy;
     if (int rc = olmax_gemm_head_grads(stream, hp, wp, grads, ld, (int)T, fused, d, rows)) return rc;
   }

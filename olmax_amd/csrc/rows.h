@@ -75,17 +75,36 @@ template <typename T, int N> __device__ __forceinline__ Cut cut(const T* row, in
   return c;
 }
 
+// tanh(x / softcap) = 1 - 2 r, r = 1 / (exp(2 x / softcap) + 1), so that a capped score is one fma on r, and its slope dy / dx is 4 r (1 - r)
 struct Scale {
-  float cap, cap_k, inv_tau;  // cap_k = 2 log2(e) / cap
+  float cap, cap_k, inv_tau;  // cap_k = 2 log2(e) / cap; cap 0: none
+  float r_k, top;             // a score is r_k r + top: r_k = -2 cap / temperature, top = cap / temperature
 };
-template <bool CAP> __device__ __forceinline__ float capped(float x, const Scale& c) {
-  return CAP ? c.cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f)) : x;
+inline Scale scale_of(float temperature, float softcap) {
+  Scale c;
+  c.cap = softcap;
+  c.cap_k = softcap > 0.f ? 2.f * LOG2E / softcap : 0.f;
+  c.inv_tau = 1.f / temperature;
+  c.top = softcap * c.inv_tau;
+  c.r_k = -2.f * c.top;
+  return c;
 }
-template <bool CAP> __device__ __forceinline__ float score(float x, const Scale& c) { return capped<CAP>(x, c) * c.inv_tau; }
+__device__ __forceinline__ float tail_of_tanh(float x, const Scale& c) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f); }
+template <bool CAP> __device__ __forceinline__ float score(float x, const Scale& c) {
+  return CAP ? __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top) : x * c.inv_tau;
+}
 // a value that all threads of the workgroup have, in a scalar register
 __device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 // z - m
-template <bool CAP> __device__ __forceinline__ float behind(float x, const Scale& c, float m) { return __builtin_fmaf(capped<CAP>(x, c), c.inv_tau, -m); }
+template <bool CAP> __device__ __forceinline__ float behind(float x, const Scale& c, float m) {
+  return CAP ? __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top - m) : __builtin_fmaf(x, c.inv_tau, -m);
+}
+// dz / dx
+template <bool CAP> __device__ __forceinline__ float slope(float x, const Scale& c) {
+  if (!CAP) return c.inv_tau;
+  const float r = tail_of_tanh(x, c);
+  return 4.f * r * (1.f - r) * c.inv_tau;
+}
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 __device__ __forceinline__ float log_of(float s) { return __builtin_amdgcn_logf(s) * LN2; }
 
@@ -145,16 +164,26 @@ template <int NW> __device__ __forceinline__ Stat block_join(Stat a, Stat* red) 
 // d / d x of g ln p[target] + h entropy: (g (i == target) - p (g + h (ln p + H))) dz/dx, from the row's m, ln S and H
 template <bool CAP, bool ENT>
 __device__ __forceinline__ float score_grad(float x, const Scale& c, float m, float log_sum, float entropy, float g, float h, bool target) {
-  float chain = c.inv_tau, y = x;
-  if (CAP) {
-    const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f);
-    y = c.cap * t;
-    chain *= 1.f - t * t;
-  }
-  const float logp = __builtin_fmaf(y, c.inv_tau, -m) - log_sum;
+  const float logp = behind<CAP>(x, c, m) - log_sum;
   float d = -exp_of(logp) * (ENT ? __builtin_fmaf(h, fmaxf(logp, -200.f) + entropy, g) : g);
   if (target) d += g;
-  return d * chain;
+  return d * slope<CAP>(x, c);
 }
 
 }  // namespace rows
+
+// gemm.hip: the LM head's product with a row's part of its softmax in the epilogue (logprobs.hip): logits leave the kernel only as what is formed of them.
+struct HeadRows {
+  const int32_t* targets;     // [M]
+  int32_t ignore_index, V;    // V: of the whole product; a target from there on has no logit
+  rows::Scale scale;
+  float *parts, *target_logit;  // statistics: [ceil(N / 256)][M][3], (largest score, sum of exponentials behind it, that sum weighted by z - m) of 256 columns; the
+                                // logit x of each target that is one of the columns
+  const float *stats, *dlogprobs, *dentropy;  // gradients: from [M, 3], [M], [M] (optional)
+};
+// Whether the forms run on a product of that size (operands 16-byte aligned, rows of K numbers), and how many of the N columns they take: whole rounds of tiles, or all;
+// 0: the plain product does better.
+int olmax_gemm_head_columns(int M, int N, int K);
+int olmax_gemm_head_stats(hipStream_t s, const bf16* h, const bf16* w, int M, int N, int K, const HeadRows& rows);
+// d [M, ldd] (16-byte aligned, ldd a multiple of 8): columns 0 .. N
+int olmax_gemm_head_grads(hipStream_t s, const bf16* h, const bf16* w, bf16* d, int64_t ldd, int M, int N, int K, const HeadRows& rows);
