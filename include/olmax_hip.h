@@ -227,7 +227,7 @@ int32_t olmax_token_logprobs_bwd(olmax_stream_t stream, const void* logits, cons
  * outside [0, V), and those named before in the row, are dropped.  A row without a logit above minus infinity has no loss and no gradient.
  * reduction 0 mean over the rows that are not left out, 1 sum, 2 none (loss [T], cotangent dloss * dloss_rows[t]).  dlogits (optional; type of the
  * logits; may be them, with the same stride) receives dloss * dL/dlogits.  (Softened targets are commonly weighted by temperature^2: through dloss.) */
-int64_t olmax_distill_workspace_bytes(int64_t T);
+int64_t olmax_distill_workspace_bytes(int64_t T, int32_t V, int32_t k, int32_t logits_f32);
 int32_t olmax_distill(olmax_stream_t stream, const void* logits, void* dlogits, const int32_t* top_ids,
                       const float* top_logprobs, float* loss, const float* dloss_rows, void* workspace,
                       int64_t workspace_bytes, int64_t T, int32_t V, int32_t k, int64_t ld, int64_t ldd,
@@ -261,7 +261,7 @@ int32_t olmax_lmhead_logprobs_bwd(olmax_stream_t stream, const void* h, const vo
                                   void* dW, void* workspace, int64_t workspace_bytes, int64_t T, int32_t d,
                                   int32_t V, int32_t ignore_index, float temperature, float softcap,
                                   int32_t dw_f32);
-int64_t olmax_lmhead_distill_workspace_bytes(int64_t T, int32_t d, int32_t V);
+int64_t olmax_lmhead_distill_workspace_bytes(int64_t T, int32_t d, int32_t V, int32_t k);
 int32_t olmax_lmhead_distill(olmax_stream_t stream, const void* h, const void* W, const int32_t* top_ids,
                              const float* top_logprobs, float* loss, void* dh, void* dW, void* workspace,
                              int64_t workspace_bytes, int64_t T, int32_t d, int32_t V, int32_t k, int32_t tail,

@@ -9,6 +9,7 @@
 #include "rows.h"
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 using namespace rows;
 
@@ -55,6 +56,7 @@ struct Teacher {
   const int32_t* ids;
   const float* t;
   int k;
+  float* x;  // the student's logits of the tokens, kept by a launch ahead of the one that may overwrite them; null: from the row
 };
 
 // What a workgroup knows of its row's teacher: tokens (-1: dropped), probabilities, their logarithms, the student's logits.  (In LDS, so that they take no registers while a
@@ -67,7 +69,7 @@ template <int NW> struct Lds {
   float sums[NW];
 };
 
-// The teacher's side of a row, by one wave, two tokens a lane (BUCKET: its tokens' bits too, element i at i + shift; they are zero).  Others read it behind a barrier.
+// The teacher's side of a row, by one wave, two tokens a lane (with `bits` its tokens' too, element i at i + shift; they are zero).  Others read it behind a barrier.
 template <typename T, bool BUCKET, int NW>
 __device__ __forceinline__ void teacher_of(const Teacher& teacher, int64_t row, const T* zr, int V, float inv_tau, unsigned* bits, int shift, Lds<NW>& l) {
   const int lane = threadIdx.x & 63, k = teacher.k;
@@ -83,7 +85,7 @@ __device__ __forceinline__ void teacher_of(const Teacher& teacher, int64_t row, 
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     mine[i] = id[i] >= 0 && id[i] < V;
-    l.x[lane + 64 * i] = mine[i] ? (float)zr[id[i]] : 0.f;
+    l.x[lane + 64 * i] = !mine[i] ? 0.f : teacher.x ? teacher.x[row * k + lane + 64 * i] : (float)zr[id[i]];
     if (!mine[i]) t[i] = -INFINITY;
   }
   for (int j = 0; j < min(k, 64); j++) {  // a token that is named again counts once
@@ -109,7 +111,7 @@ __device__ __forceinline__ void teacher_of(const Teacher& teacher, int64_t row, 
     l.id[j] = mine[i] ? id[i] : -1;
     l.q[j] = q[i] * part;
     l.logq[j] = logq[i] - log_part;
-    if (BUCKET && mine[i]) atomicOr(&bits[(id[i] + shift) >> 5], 1u << ((id[i] + shift) & 31));
+    if (BUCKET && bits && mine[i]) atomicOr(&bits[(id[i] + shift) >> 5], 1u << ((id[i] + shift) & 31));
   }
   if (lane == 0) l.weight = BUCKET ? sum + r : sum > 0.f ? 1.f : 0.f, l.rest = r;  // sum of all probabilities; 0: nothing to learn
 }
@@ -153,6 +155,10 @@ template <bool CAP> __device__ __forceinline__ float outside(float x, const Scal
   return exp_of(behind<CAP>(x, c, f.m)) * f.out * slope<CAP>(x, c);
 }
 
+template <bool CAP> __device__ __forceinline__ float inside(float x, float q, const Scale& c, const Factors& f) {
+  return (exp_of(behind<CAP>(x, c, f.m)) * f.in - q * f.scale) * slope<CAP>(x, c);
+}
+
 struct RowArgs {
   Teacher teacher;
   float* row_loss;
@@ -164,11 +170,172 @@ struct RowArgs {
   int mean, pad;
 };
 
-// One workgroup a row.  The first pass takes the statistics and the loss, the second writes the gradient of all tokens, and the k tokens' own follow.
-// HELD > 0: a thread keeps that many vectors of the row in registers between the two, all of the row; otherwise the row is streamed, and read again.
+// The number of rows that are not left out, by the second wave.
+template <int NW> __device__ __forceinline__ void count_rows(const RowArgs& p, Lds<NW>& l) {
+  float n = 0.f;
+  if (p.n_counted) n = p.n_counted[threadIdx.x & 63];
+  else
+    for (int i = threadIdx.x & 63; i < p.rows; i += 64) n += p.teacher.ids[(int64_t)i * p.teacher.k] >= 0 ? 1.f : 0.f;
+  n = wave_sum(n);
+  if (threadIdx.x == 64) l.counted = n;
+}
+template <typename TO, int TH> __device__ __forceinline__ void write_zeros(TO* dr, const Cut& cutting, int v0, int v1, bool ends, int V, int pad) {
+  constexpr int N = Vec<TO>::N;
+  const float zero[N] = {};
+  for (int v = v0 + threadIdx.x; v < v1; v += TH) *reinterpret_cast<u32x4*>(dr + cutting.head + v * N) = Vec<TO>::pack(zero);
+  if (ends && (int)threadIdx.x < cutting.edges) dr[cutting.edge(threadIdx.x, V)] = (TO)0.f;
+  if (ends && (int)threadIdx.x < pad) dr[V + threadIdx.x] = (TO)0.f;
+}
+
+// Rows that no workgroup holds, and few rows: two launches of shares of rows.  The first leaves statistics (BUCKET: sums of the other tokens) of each share, and the teacher's tokens'
+// logits; or (part_stat null) the loss of whole rows, and there is no second.
+template <typename T, bool CAP, bool BUCKET, int TH>
+__global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__ logits, const RowArgs p, const Scale c, Stat* __restrict__ part_stat, int parts) {
+  constexpr int N = Vec<T>::N, UNROLL = 4, SPAN = TH * UNROLL;
+  extern __shared__ unsigned bits[];  // BUCKET: of the teacher's tokens in the share, the row's single elements behind its vectors
+  __shared__ Lds<TH / 64> l;
+  const int64_t row = blockIdx.x / parts;
+  const int part = blockIdx.x % parts, tid = threadIdx.x, V = p.V;
+  const int32_t* ids = p.teacher.ids + row * p.teacher.k;
+  if (ids[0] < 0) {
+    if (!part_stat && tid == 0) p.row_loss[row] = 0.f;
+    return;
+  }
+  const T* zr = logits + row * p.ld;
+  const Cut cutting = cut<T, N>(zr, V);
+  const T* body = zr + cutting.head;
+  const int per = (cutting.nvec + parts - 1) / parts;
+  const int v0 = min(part * per, cutting.nvec), v1 = min(v0 + per, cutting.nvec);
+  Raw<T, N> next[UNROLL];
+  auto fetch = [&](int at) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++)
+      if (at + u * TH + tid < v1) next[u].load(body + (int64_t)(at + u * TH + tid) * N);
+  };
+  fetch(v0);
+  if (!part_stat && tid < 64) teacher_of<T, BUCKET, TH / 64>(p.teacher, row, zr, V, c.inv_tau, nullptr, 0, l);  // (beside the others' first loads)
+  if (part_stat && part == 0 && tid < p.teacher.k) p.teacher.x[row * p.teacher.k + tid] = ids[tid] >= 0 && ids[tid] < V ? (float)zr[ids[tid]] : 0.f;
+  if (BUCKET) {
+    for (int i = tid; i < (per * N + 2 * N + 31) / 32; i += TH) bits[i] = 0;
+    __syncthreads();
+    if (tid < p.teacher.k) {
+      const int id = ids[tid], in = id - cutting.head;
+      int at = -1;
+      if (id >= 0 && id < V) at = in < 0 ? per * N + id : in >= cutting.nvec * N ? per * N + id - cutting.nvec * N : in >= v0 * N && in < v1 * N ? in - v0 * N : -1;
+      if (at >= 0) atomicOr(&bits[at >> 5], 1u << (at & 31));
+    }
+    __syncthreads();
+  }
+  const unsigned char* byte_of = reinterpret_cast<const unsigned char*>(bits);
+  Stat a = Stat::none();
+  if (part == 0 && tid < cutting.edges) {
+    const float x = (float)zr[cutting.edge(tid, V)];
+    const int at = per * N + tid;
+    if (CAP || x > -INFINITY) a.m = score<CAP>(x, c);
+    a.s = BUCKET && (bits[at >> 5] >> (at & 31) & 1) ? 0.f : exp_of(behind<CAP>(x, c, a.ref()));
+  }
+  for (int at = v0; at < v1; at += SPAN) {
+    Raw<T, N> now[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) now[u] = next[u];
+    fetch(at + SPAN);
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      if (at + u * TH + tid >= v1) continue;
+      float x[N];
+      now[u].unpack(x);
+#pragma unroll
+      for (int e = 0; e < N; e++) most = fmaxf(most, x[e]);
+    }
+    const float top = score<CAP>(most, c);
+    if (at + tid < v1 && top > a.m) a.raise(top);
+    const float ref = a.ref();
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      const int v = at + u * TH + tid;
+      if (v >= v1) continue;
+      float x[N];
+      now[u].unpack(x);
+#pragma unroll
+      for (int e = 0; e < N; e++) x[e] = exp_of(behind<CAP>(x[e], c, ref));
+      if (BUCKET) {
+        const int b = v - v0;
+        const unsigned in = N == 8 ? (unsigned)byte_of[b] : (byte_of[b >> 1] >> (b & 1) * 4) & 15u;
+        if (in)
+#pragma unroll
+          for (int e = 0; e < N; e++) x[e] = in >> e & 1 ? 0.f : x[e];
+      }
+#pragma unroll
+      for (int w = N / 2; w > 0; w >>= 1)
+#pragma unroll
+        for (int e = 0; e < w; e++) x[e] += x[e + w];
+      a.s += x[0];
+    }
+  }
+  a = block_join<TH / 64>(a, l.red);
+  if (part_stat && tid == 0) part_stat[blockIdx.x] = a;
+  if (!part_stat) factors_of<CAP, BUCKET, TH / 64>(a, l, c, 0.f, p.row_loss + row);
+}
+
+// The second joins them (every workgroup for itself), writes the loss, and the gradient of one of `shares` shares of the row.
+template <typename T, typename TO, bool CAP, bool BUCKET>
+__global__ __launch_bounds__(256) void distill_grads_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const RowArgs p, const Scale c,
+                                                            const Stat* __restrict__ part_stat, int parts, int shares) {
+  constexpr int N = Vec<TO>::N, TH = 256, NW = TH / 64;
+  __shared__ Lds<NW> l;
+  __shared__ float unused;
+  const int64_t row = blockIdx.x / shares;
+  const int share = blockIdx.x % shares, tid = threadIdx.x, V = p.V;
+  const T* zr = logits + row * p.ld;
+  TO* dr = dlogits ? dlogits + row * p.ldd : nullptr;
+  const Cut cutting = dr ? cut<TO, N>(dr, V) : cut<T, N>(zr, V);
+  const int per = (cutting.nvec + shares - 1) / shares;
+  const int v0 = min(share * per, cutting.nvec), v1 = min(v0 + per, cutting.nvec);
+  if (p.teacher.ids[row * p.teacher.k] < 0) {  // left out
+    if (share == 0 && tid == 0) p.row_loss[row] = 0.f;
+    if (dr) write_zeros<TO, TH>(dr, cutting, v0, v1, share == 0, V, p.pad);
+    return;
+  }
+  if (tid < 64) {
+    Stat a = Stat::none();
+    if (tid < parts) a = part_stat[row * parts + tid];
+    a = block_join<1>(a, nullptr);
+    if (tid == 0) l.red[0] = a;
+    teacher_of<T, BUCKET, NW>(p.teacher, row, zr, V, c.inv_tau, nullptr, 0, l);
+  }
+  if (tid >> 6 == 1 && dr && p.mean) count_rows(p, l);
+  __syncthreads();
+  float scale = 0.f;
+  if (dr) scale = uniform(p.dloss * (p.drow ? p.drow[row] : 1.f) / (p.mean ? l.counted : 1.f));
+  const Factors f = factors_of<CAP, BUCKET, NW>(l.red[0], l, c, scale, share == 0 ? p.row_loss + row : &unused);
+  if (!dr) return;
+  for (int v = v0 + tid; v < v1; v += TH) {
+    const int i = cutting.head + v * N;
+    Raw<T, N> w;
+    w.load(zr + i);
+    float x[N];
+    w.unpack(x);
+#pragma unroll
+    for (int e = 0; e < N; e++) x[e] = outside<CAP>(x[e], c, f);
+    *reinterpret_cast<u32x4*>(dr + i) = Vec<TO>::pack(x);
+  }
+  if (share == 0 && tid < cutting.edges) {
+    const int i = cutting.edge(tid, V);
+    dr[i] = (TO)outside<CAP>((float)zr[i], c, f);
+  }
+  if (share == 0 && tid < p.pad) dr[V + tid] = (TO)0.f;
+  __syncthreads();  // behind the vectors that hold them
+  if (tid < MAX_TOP && l.id[tid] >= 0) {
+    const int in = l.id[tid] - cutting.head;
+    if (in >= 0 && in < cutting.nvec * N ? in >= v0 * N && in < v1 * N : share == 0) dr[l.id[tid]] = (TO)inside<CAP>(l.x[tid], l.q[tid], c, f);
+  }
+}
+
+// One workgroup a row, of which a thread keeps HELD vectors in registers: statistics and the loss, then the gradient of all tokens, then the k tokens' own.
 template <typename T, typename TO, bool CAP, bool BUCKET, int TH, int HELD>
-__global__ __launch_bounds__(TH, HELD ? 4 : 1) void distill_rows_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const RowArgs p, const Scale c) {
-  constexpr int N = Vec<TO>::N, NW = TH / 64, UNROLL = 4, SPAN = TH * UNROLL;
+__global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const RowArgs p, const Scale c) {
+  constexpr int N = Vec<TO>::N, NW = TH / 64;
   extern __shared__ unsigned bits[];  // BUCKET
   __shared__ Lds<NW> l;
   const int64_t row = blockIdx.x;
@@ -178,42 +345,21 @@ __global__ __launch_bounds__(TH, HELD ? 4 : 1) void distill_rows_kernel(const T*
   const Cut cutting = dr ? cut<TO, N>(dr, V) : cut<T, N>(zr, V);
   if (p.teacher.ids[row * p.teacher.k] < 0) {  // left out
     if (tid == 0) p.row_loss[row] = 0.f;
-    if (dr) {
-      float zero[N] = {};
-      for (int v = tid; v < cutting.nvec; v += TH) *reinterpret_cast<u32x4*>(dr + cutting.head + v * N) = Vec<TO>::pack(zero);
-      if (tid < cutting.edges) dr[cutting.edge(tid, V)] = (TO)0.f;
-      if (tid < p.pad) dr[V + tid] = (TO)0.f;
-    }
+    if (dr) write_zeros<TO, TH>(dr, cutting, 0, cutting.nvec, true, V, p.pad);
     return;
   }
   const T* body = zr + cutting.head;
-  Raw<T, N> next[HELD ? 1 : UNROLL], held[HELD ? HELD : 1];
-  auto fetch = [&](int at) {
+  Raw<T, N> held[HELD];
 #pragma unroll
-    for (int u = 0; u < (HELD ? 1 : UNROLL); u++)
-      if (at + u * TH + tid < cutting.nvec) next[u].load(body + (int64_t)(at + u * TH + tid) * N);
-  };
-  if (HELD) {
-#pragma unroll
-    for (int i = 0; i < HELD; i++)
-      if (i * TH + tid < cutting.nvec) held[i].load_once(body + (int64_t)(i * TH + tid) * N);
-  } else {
-    fetch(0);
-  }
+  for (int i = 0; i < HELD; i++)
+    if (i * TH + tid < cutting.nvec) held[i].load_once(body + (int64_t)(i * TH + tid) * N);
   const int shift = (N - cutting.head) & (N - 1);
   if (BUCKET) {
     for (int i = tid; i < (V + 8 + 31) / 32; i += TH) bits[i] = 0;
     __syncthreads();
   }
   if (tid < 64) teacher_of<T, BUCKET, NW>(p.teacher, row, zr, V, c.inv_tau, bits, shift, l);
-  if (tid >> 6 == 1 && dr && p.mean) {  // the rows that count, by another wave
-    float n = 0.f;
-    if (p.n_counted) n = p.n_counted[tid & 63];
-    else
-      for (int i = tid & 63; i < p.rows; i += 64) n += p.teacher.ids[(int64_t)i * p.teacher.k] >= 0 ? 1.f : 0.f;
-    n = wave_sum(n);
-    if (tid == 64) l.counted = n;
-  }
+  if (tid >> 6 == 1 && dr && p.mean) count_rows(p, l);
   if (BUCKET) __syncthreads();
 
   // ---- largest score, sum of exponentials (BUCKET: of the other tokens)
@@ -259,53 +405,28 @@ __global__ __launch_bounds__(TH, HELD ? 4 : 1) void distill_rows_kernel(const T*
   };
   const bool has_edge = tid < cutting.edges;
   int edge;
-  Stat a = Stat::none();
-  if (HELD) {
-    float most = -INFINITY;
-    if (has_edge) most = fmaxf(most, edge_value(&edge));
+  float most = -INFINITY;
+  if (has_edge) most = fmaxf(most, edge_value(&edge));
 #pragma unroll
-    for (int i = 0; i < HELD; i++) {
-      keep(held[i]);
-      if (i * TH + tid < cutting.nvec) most = largest(held[i], most);
-    }
-    most = uniform(block_reduce<NW, true>(most, l.sums));
-    if (CAP || most > -INFINITY) a.m = score<CAP>(most, c);
-    const float ref = a.ref();
-    float sum = 0.f;
-    if (has_edge) {
-      const float x = edge_value(&edge);
-      sum = edge_sum(x, edge, ref);
-    }
-#pragma unroll
-    for (int i = 0; i < HELD; i++) {
-      keep(held[i]);
-      if (i * TH + tid < cutting.nvec) sum += summed(held[i], i * TH, ref);
-    }
-    a.s = uniform(block_reduce<NW, false>(sum, l.sums));
-  } else {
-    if (has_edge) {
-      const float x = edge_value(&edge);
-      if (CAP || x > -INFINITY) a.m = score<CAP>(x, c);
-      a.s = edge_sum(x, edge, a.ref());
-    }
-    for (int at = 0; at < cutting.nvec; at += SPAN) {
-      Raw<T, N> now[UNROLL];
-#pragma unroll
-      for (int u = 0; u < UNROLL; u++) now[u] = next[HELD ? 0 : u];
-      fetch(at + SPAN);
-      float most = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < UNROLL; u++)
-        if (at + u * TH + tid < cutting.nvec) most = largest(now[u], most);
-      const float top = score<CAP>(most, c);
-      if (at + tid < cutting.nvec && top > a.m) a.raise(top);
-      const float ref = a.ref();
-#pragma unroll
-      for (int u = 0; u < UNROLL; u++)
-        if (at + u * TH + tid < cutting.nvec) a.s += summed(now[u], at + u * TH, ref);
-    }
-    a = block_join<NW>(a, l.red);
+  for (int i = 0; i < HELD; i++) {
+    keep(held[i]);
+    if (i * TH + tid < cutting.nvec) most = largest(held[i], most);
   }
+  most = uniform(block_reduce<NW, true>(most, l.sums));
+  Stat a = Stat::none();
+  if (CAP || most > -INFINITY) a.m = score<CAP>(most, c);
+  const float ref = a.ref();
+  float sum = 0.f;
+  if (has_edge) {
+    const float x = edge_value(&edge);
+    sum = edge_sum(x, edge, ref);
+  }
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    keep(held[i]);
+    if (i * TH + tid < cutting.nvec) sum += summed(held[i], i * TH, ref);
+  }
+  a.s = uniform(block_reduce<NW, false>(sum, l.sums));
   // (a barrier of the reduction lies between the teacher's wave and here)
   float scale = 0.f;
   if (dr) scale = uniform(p.dloss * (p.drow ? p.drow[row] : 1.f) / (p.mean ? l.counted : 1.f));
@@ -320,20 +441,12 @@ __global__ __launch_bounds__(TH, HELD ? 4 : 1) void distill_rows_kernel(const T*
     for (int e = 0; e < N; e++) x[e] = outside<CAP>(x[e], c, f);
     *reinterpret_cast<u32x4*>(dr + cutting.head + v * N) = Vec<TO>::pack(x);
   };
-  if (HELD) {
 #pragma unroll
-    for (int i = 0; i < HELD; i++) {
-      int at = tid;
-      asm volatile("" : "+v"(at));  // (the offsets, which would be kept from the loads, are computed again)
-      keep(held[i]);
-      if (i * TH + at < cutting.nvec) write(held[i], i * TH + at);
-    }
-  } else {
-    for (int v = tid; v < cutting.nvec; v += TH) {
-      Raw<T, N> w;
-      w.load(body + (int64_t)v * N);
-      write(w, v);
-    }
+  for (int i = 0; i < HELD; i++) {
+    int at = tid;
+    asm volatile("" : "+v"(at));  // (the offsets, which would be kept from the loads, are computed again)
+    keep(held[i]);
+    if (i * TH + at < cutting.nvec) write(held[i], i * TH + at);
   }
   if (has_edge) {
     const float x = edge_value(&edge);
@@ -341,13 +454,38 @@ __global__ __launch_bounds__(TH, HELD ? 4 : 1) void distill_rows_kernel(const T*
   }
   if (tid < p.pad) dr[V + tid] = (TO)0.f;
   __syncthreads();  // behind the vectors that hold them
-  if (tid < MAX_TOP && l.id[tid] >= 0) dr[l.id[tid]] = (TO)((exp_of(behind<CAP>(l.x[tid], c, f.m)) * f.in - l.q[tid] * f.scale) * slope<CAP>(l.x[tid], c));
+  if (tid < MAX_TOP && l.id[tid] >= 0) dr[l.id[tid]] = (TO)inside<CAP>(l.x[tid], l.q[tid], c, f);
 }
 
 }  // namespace
 
-// Workspace: T floats (row losses) and the shares of the number of counted rows.
-extern "C" int64_t olmax_distill_workspace_bytes(int64_t T) { return ((T * 4 + 15) / 16) * 16 + COUNTERS * 4; }
+// How a call runs: held = vectors and threads that hold a row, or 0 and the shares of a row for statistics and gradient.
+// The fewest threads that hold the row.  us, two launches of shares | held, with gradient: FIGURES
+struct Form {
+  int threads, held, parts, shares;
+};
+static Form form_of(int64_t T, int V, bool logits_f32, bool grads_f32, bool grad) {
+  const int vecs = V / (grads_f32 ? 4 : 8), reads = V / (logits_f32 ? 4 : 8);
+  const bool wide = logits_f32 && !grads_f32;  // a vector takes eight registers
+  const int most = wide ? 13 : grads_f32 ? 25 : 20;
+  if (vecs <= 256 * 8) return {256, 8, 1, 1};
+  // the loss alone: a row has to be read once anyway, and 256 threads that stream it leave a CU to more rows
+  const bool hold = grad ? T > 128 || vecs <= 512 * 25 : T < 400 && vecs <= 512 * 25;
+  if (hold && vecs <= 512 * (wide ? 13 : 25)) return {512, wide ? 13 : 25, 1, 1};
+  if (hold && vecs <= 1024 * most) return {1024, most, 1, 1};
+  const int64_t parts = T > 256 ? 1 : std::min<int64_t>(std::min<int64_t>(reads / 1024, 1024 / T), 32);
+  const int64_t shares = grad ? std::min<int64_t>(vecs / 2048, 4096 / T) : 1;
+  return {0, 0, (int)std::max<int64_t>(1, parts), (int)std::max<int64_t>(1, shares)};
+}
+
+// Workspace: T floats (row losses), the shares of the number of counted rows, statistics of the shares of rows, the tokens' logits.
+static int64_t stats_at(int64_t T) { return ((T * 4 + 15) / 16) * 16 + COUNTERS * 4; }
+extern "C" int64_t olmax_distill_workspace_bytes(int64_t T, int32_t V, int32_t k, int32_t logits_f32) {
+  if (T <= 0 || V <= 0 || k <= 0) return 0;
+  int64_t parts = 1;
+  for (int grad = 0; grad < 4; grad++) parts = std::max<int64_t>(parts, form_of(T, V, logits_f32 != 0, logits_f32 && grad < 2, grad & 1).parts);
+  return stats_at(T) + T * (parts * (int64_t)sizeof(Stat) + k * 4ll);
+}
 
 static int distill_check(const char* name, int64_t T, int32_t V, int32_t k, int32_t tail, float temperature, float softcap) {
   OLMAX_CHECK(T > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "%s: bad shape T=%ld V=%d", name, (long)T, V);
@@ -368,35 +506,46 @@ static int distill(hipStream_t stream, const void* logits, void* dlogits, const 
     n = (float*)((char*)workspace + ((T * 4 + 15) / 16) * 16);
     hipLaunchKernelGGL(distill_count_kernel, dim3(COUNTERS), dim3(256), 0, stream, ids, T, k, n);
   }
-  const RowArgs args{{ids, t, k}, row_loss, dloss_rows, n, T, V, ld, ldd, dloss, (int)(reduction == 0), pad};
-#define ROWS(TY, TO, CAPV, BUCKETV, THV, HELDV)                                                                                                        \
-  do {                                                                                                                                                 \
-    auto kern = distill_rows_kernel<TY, TO, CAPV, BUCKETV, THV, HELDV>;                                                                                \
-    static std::once_flag attr_once; /* per instantiation */                                                                                           \
-    std::call_once(attr_once, [&] { (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, MAX_BITS / 8); });        \
-    hipLaunchKernelGGL(kern, dim3((unsigned)T), dim3(THV), BUCKETV ? (V + 8 + 31) / 32 * 4 : 0, stream, (const TY*)logits, (TO*)dlogits, args, c);      \
+  const Form form = form_of(T, V, logits_f32, grads_f32, dlogits != nullptr);
+  OLMAX_CHECK(T * std::max(form.parts, form.shares) < (1LL << 31), OLMAX_ERR_SHAPE, "olmax_distill: T=%ld rows of V=%d are too many", (long)T, V);
+  Stat* part_stat = (Stat*)((char*)workspace + stats_at(T));
+  const bool alone = form.parts == 1 && !dlogits;
+  const RowArgs args{{ids, t, k, form.threads || alone ? nullptr : (float*)(part_stat + T * form.parts)}, row_loss, dloss_rows, n, T, V, ld, ldd, dloss, (int)(reduction == 0), pad};
+#define LAUNCH(K, GRID, THV, LDS, ...)                                                                                                          \
+  do {                                                                                                                                          \
+    auto kern = K;                                                                                                                              \
+    static std::once_flag attr_once; /* per instantiation */                                                                                    \
+    std::call_once(attr_once, [&] { (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, MAX_BITS / 8); }); \
+    hipLaunchKernelGGL(kern, dim3((unsigned)(GRID)), dim3(THV), LDS, stream, (const TY*)logits, __VA_ARGS__);                                   \
   } while (0)
-  const int vecs = V / (grads_f32 ? 4 : 8);  // of a row, at most
-  // The fewest threads that hold the row; rows that none do are streamed.  us, streamed | held, with gradient: 4096 x 100352 bf16 422 | 338, 4096 x 128256 bf16 558 | 500,
-  // 2048 x 100352 fp32 498 | 338.  1024 threads that hold a row have a CU to themselves: 300 rows of 128256 52 | 61 (64 rows 31 | 31,
-  // 700 115 | 99), so a last round of few rows is streamed instead.  With the LM head, fp32 logits and bf16 gradients: 2048 x 256 x 100352
-  // with its products 876 | 753.
-  const bool alone = T <= 256 || T >= 384;
-#define ROWS_H(TY, TO, CAPV, BUCKETV)                                                                                                              \
-  do {                                                                                                                                             \
-    constexpr bool WIDE = sizeof(TY) != sizeof(TO), HALF = sizeof(TO) == 2; /* a vector of WIDE takes eight registers */                           \
-    if (vecs <= 256 * 8) ROWS(TY, TO, CAPV, BUCKETV, 256, 8);                                                                                      \
-    else if (vecs <= 512 * (WIDE ? 13 : 25)) ROWS(TY, TO, CAPV, BUCKETV, 512, (WIDE ? 13 : 25));                                                   \
-    else if (alone && vecs <= 1024 * (WIDE ? 13 : HALF ? 20 : 25)) ROWS(TY, TO, CAPV, BUCKETV, 1024, (WIDE ? 13 : HALF ? 20 : 25)); \
-    else ROWS(TY, TO, CAPV, BUCKETV, 512, 0);                                                                                                      \
-  } while (0)
-#define ROWS_B(TY, TO, CAPV) do { if (tail) ROWS_H(TY, TO, CAPV, true); else ROWS_H(TY, TO, CAPV, false); } while (0)
-#define ROWS_C(TY, TO) do { if (softcap > 0.f) ROWS_B(TY, TO, true); else ROWS_B(TY, TO, false); } while (0)
-  if (logits_f32 && grads_f32) ROWS_C(float, float); else if (logits_f32) ROWS_C(float, bf16); else ROWS_C(bf16, bf16);
-#undef ROWS
-#undef ROWS_H
-#undef ROWS_B
-#undef ROWS_C
+#define HELD(THV, HELDV) LAUNCH((distill_rows_kernel<TY, TO, CAP, BUCKET, THV, (HELDV)>), T, THV, BUCKET ? (V + 8 + 31) / 32 * 4 : 0, (TO*)dlogits, args, c)
+  auto go = [&](auto in, auto out, auto capped, auto bucket) {
+    using TY = decltype(in);
+    using TO = decltype(out);
+    constexpr bool CAP = decltype(capped)::value, BUCKET = decltype(bucket)::value, WIDE = sizeof(TY) != sizeof(TO);
+    if (form.threads == 256) HELD(256, 8);
+    else if (form.threads == 512) HELD(512, WIDE ? 13 : 25);
+    else if (form.threads == 1024) HELD(1024, WIDE ? 13 : sizeof(TO) == 2 ? 20 : 25);
+    else {
+      constexpr int N = Vec<TY>::N;
+      const size_t lds = BUCKET ? ((V / N + form.parts) / form.parts * N + 2 * N + 31) / 32 * 4 : 0;
+      Stat* stat = alone ? nullptr : part_stat;
+      if (form.parts > 1) LAUNCH((distill_stats_kernel<TY, CAP, BUCKET, 256>), T * form.parts, 256, lds, args, c, stat, form.parts);
+      else LAUNCH((distill_stats_kernel<TY, CAP, BUCKET, 512>), T, 512, lds, args, c, stat, 1);
+      if (!alone) LAUNCH((distill_grads_kernel<TY, TO, CAP, BUCKET>), T * form.shares, 256, 0, (TO*)dlogits, args, c, (const Stat*)part_stat, form.parts, form.shares);
+    }
+  };
+#undef HELD
+#undef LAUNCH
+  auto kind = [&](auto in, auto out) {
+    const std::true_type yes;
+    const std::false_type no;
+    if (softcap > 0.f) tail ? go(in, out, yes, yes) : go(in, out, yes, no);
+    else tail ? go(in, out, no, yes) : go(in, out, no, no);
+  };
+  if (logits_f32 && grads_f32) kind(0.f, 0.f);
+  else if (logits_f32) kind(0.f, bf16());
+  else kind(bf16(), bf16());
   if (reduction != 2) hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(T <= 256 ? 256 : 1024), 0, stream, (const float*)row_loss, ids, (const float*)n, T, k, loss, (int)(reduction == 0));
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
@@ -412,8 +561,8 @@ extern "C" int32_t olmax_distill(hipStream_t stream, const void* logits, void* d
   OLMAX_CHECK(!dloss_rows || reduction == 2, OLMAX_ERR_ARG, "olmax_distill: a per-row cotangent only goes with reduction none");
   OLMAX_CHECK((((uintptr_t)logits | (uintptr_t)dlogits) & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_distill: operands not aligned to their type");
   OLMAX_CHECK(logits != dlogits || ld == ldd, OLMAX_ERR_ARG, "olmax_distill: in place wants one row stride");
-  OLMAX_CHECK(workspace_bytes >= olmax_distill_workspace_bytes(T) && aligned16(workspace), OLMAX_ERR_WORKSPACE, "olmax_distill: workspace needs %ld bytes, 16-byte aligned",
-              (long)olmax_distill_workspace_bytes(T));
+  OLMAX_CHECK(workspace_bytes >= olmax_distill_workspace_bytes(T, V, k, logits_f32) && aligned16(workspace), OLMAX_ERR_WORKSPACE, "olmax_distill: workspace needs %ld bytes, 16-byte aligned",
+              (long)olmax_distill_workspace_bytes(T, V, k, logits_f32));
   return distill(stream, logits, dlogits, top_ids, top_logprobs, loss, dloss_rows, workspace, T, V, k, ld, ldd, logits_f32 != 0, logits_f32 != 0, tail,
                  temperature, softcap, dloss, reduction, 0);
 }
@@ -422,9 +571,9 @@ extern "C" int32_t olmax_distill(hipStream_t stream, const void* logits, void* d
 static int64_t head_stride(int32_t V) { return ((int64_t)V + 63) / 64 * 64; }
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-extern "C" int64_t olmax_lmhead_distill_workspace_bytes(int64_t T, int32_t d, int32_t V) {
+extern "C" int64_t olmax_lmhead_distill_workspace_bytes(int64_t T, int32_t d, int32_t V, int32_t k) {
   if (T <= 0 || V <= 0) return 0;
-  return up256(T * head_stride(V) * 4) + up256(T * head_stride(V) * 2) + olmax_distill_workspace_bytes(T);
+  return up256(T * head_stride(V) * 4) + up256(T * head_stride(V) * 2) + olmax_distill_workspace_bytes(T, V, k, 1);
 }
 
 extern "C" int32_t olmax_lmhead_distill(hipStream_t stream, const void* h, const void* W, const int32_t* top_ids, const float* top_logprobs, float* loss,
@@ -433,8 +582,8 @@ extern "C" int32_t olmax_lmhead_distill(hipStream_t stream, const void* h, const
   OLMAX_CHECK(h && W && top_ids && top_logprobs && loss && workspace, OLMAX_ERR_ARG, "olmax_lmhead_distill: null pointer");
   if (int rc = distill_check("olmax_lmhead_distill", T, V, k, tail, temperature, softcap)) return rc;
   OLMAX_CHECK(d > 0, OLMAX_ERR_SHAPE, "olmax_lmhead_distill: bad shape d=%d", d);
-  OLMAX_CHECK(workspace_bytes >= olmax_lmhead_distill_workspace_bytes(T, d, V) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
-              "olmax_lmhead_distill: workspace needs %ld bytes, 256-byte aligned", (long)olmax_lmhead_distill_workspace_bytes(T, d, V));
+  OLMAX_CHECK(workspace_bytes >= olmax_lmhead_distill_workspace_bytes(T, d, V, k) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
+              "olmax_lmhead_distill: workspace needs %ld bytes, 256-byte aligned", (long)olmax_lmhead_distill_workspace_bytes(T, d, V, k));
   const int64_t ld = head_stride(V);
   const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
   bf16* grads = (bf16*)((char*)workspace + up256(T * ld * 4));

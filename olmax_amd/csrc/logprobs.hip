@@ -38,13 +38,11 @@ template <int TH> struct Lds {
 // largest of those.  Found on the upper 16 bits of the keys, by bits: each wave counts all groups, four a lane.
 template <int TH>
 __device__ __forceinline__ unsigned kth_best(unsigned* best, unsigned own, int k) {
-  static_assert(TH == GROUPS || TH == 4 * GROUPS, "a thread or four to a group");
-  if (TH > GROUPS) {
-    own = max(own, (unsigned)__shfl_xor((int)own, 1, 64));
-    own = max(own, (unsigned)__shfl_xor((int)own, 2, 64));
-  }
+  static_assert(TH == GROUPS || TH == 2 * GROUPS || TH == 4 * GROUPS, "up to four threads to a group");
+  if (TH > GROUPS) own = max(own, (unsigned)__shfl_xor((int)own, 1, 64));
+  if (TH > 2 * GROUPS) own = max(own, (unsigned)__shfl_xor((int)own, 2, 64));
   __syncthreads();
-  if (TH == GROUPS || (threadIdx.x & 3) == 0) best[threadIdx.x / (TH / GROUPS)] = own;
+  if ((threadIdx.x & (TH / GROUPS - 1)) == 0) best[threadIdx.x / (TH / GROUPS)] = own;
   __syncthreads();
   const u32x4 q = *reinterpret_cast<const u32x4*>(best + (threadIdx.x & 63) * 4);
   unsigned at = 0;
@@ -502,14 +500,14 @@ __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ lo
 struct Form {
   int threads, parts;
 };
-// Rows that fill the GPU by themselves take a workgroup of 256 threads each; up to 256 long ones one of 1024; few ones come in shares of one round of loads (1024 vectors), whose
-// candidates a second launch joins: many of those cost more than longer shares of 1024 threads.  us in a graph, bf16, 256 threads x 1 | 1024 x 1 | 256 x 16 | 1024 x 4: 1 x 128256 without
-// alternatives 17.0 | 13.5 | 7.4 | 10.2, with 20 28.8 | 23.2 | 13.4 | 17, with 128 35.8 | 25.7 | 45 | 20.9; 200 x 128256 with 20 31.1 | 25.4 | 30 | 37; 400 x 128256 with 20 38.5 | 47.8;
-// 37 x 50304 without 9.8 | 9.2 | (8 shares) 8.2; 100 x 4096 without 4.7 | 6.2.
+// Rows that fill the GPU by themselves take a workgroup of 256 threads each, up to 256 long ones one of 512; few ones come in shares of one round of loads (1024 vectors), whose
+// candidates a second launch joins: many of those cost more than longer shares of 1024 threads.  us in a graph, bf16, 256 threads x 1 | 512 x 1 | 1024 x 1 | 256 x 16 | 1024 x 4: 1 x 128256
+// without alternatives 17.0 | - | 13.5 | 7.4 | 10.2, with 20 28.8 | - | 23.2 | 13.4 | 17, with 128 35.8 | - | 25.7 | 45 | 20.9; 200 x 100352 with 20 27.3 | 22.6 | 24.1; 400 x 100352 with
+// 20 33.1 | 31.8 | 44.8, without 21.1 | 21.7 | 24.7; 1600 x 50304 with 20 49.7 | 54.8 | 104; 100 x 4096 without 4.7 | - | 6.2.
 Form form_of(int64_t T, int V, int top, bool f32) {
   const int64_t vecs = V / (f32 ? 4 : 8);
   if (T > 256 || vecs < 2048) return {256, 1};
-  if (T > 128) return {vecs < 6000 ? 256 : 1024, 1};
+  if (T > 128) return {vecs < 6000 ? 256 : 512, 1};
   const int64_t shares = std::min<int64_t>(std::min<int64_t>(vecs / 1024, 1024 / T), 32);
   if (shares * top <= 640) return {256, (int)shares};
   return {1024, (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(vecs / 4096, 512 / top), 256 / T))};
@@ -545,7 +543,7 @@ extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, 
                      part_stat, V, ld, ignore_index, c, top, parts)
 #define SCORE(TY, CAPV, TOPV)                                                                                                                             \
   do {                                                                                                                                                    \
-    if (form.threads == 256) ROWS(TY, CAPV, TOPV, 256); else ROWS(TY, CAPV, TOPV, 1024);                                                                  \
+    if (form.threads == 256) ROWS(TY, CAPV, TOPV, 256); else if (form.threads == 512) ROWS(TY, CAPV, TOPV, 512); else ROWS(TY, CAPV, TOPV, 1024);                                                                  \
     if (parts > 1)                                                                                                                                        \
       hipLaunchKernelGGL((score_join_kernel<TY, CAPV, TOPV>), dim3((unsigned)T), dim3(256), 0, stream, (const TY*)logits, targets, out,                   \
                          (const uint64_t*)part_top, (const Stat*)part_stat, V, ld, ignore_index, c, top, parts);                                          \

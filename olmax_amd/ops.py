@@ -454,7 +454,7 @@ def distill(logits, top_ids, top_logprobs, *, tail: str = "renormalize", tempera
     k = _teacher(top_ids, top_logprobs, T)
     _want(reduction in ("mean", "sum", "none"), f"unknown reduction {reduction!r}")
     red = ("mean", "sum", "none").index(reduction)
-    nbytes = _size("olmax_distill_workspace_bytes", T)
+    nbytes = _size("olmax_distill_workspace_bytes", T, V, k, 1 if logits.dtype == torch.float32 else 0)
     ws = logits.new_empty((nbytes,), dtype=torch.uint8)
     loss = logits.new_empty((T,) if red == 2 else (), dtype=torch.float32)
     d, ldd = None, 0
@@ -504,7 +504,7 @@ def lmhead_distill(h, W, top_ids, top_logprobs, *, tail: str = "renormalize", te
     _place(h, W, top_ids, top_logprobs)
     T, d, V = _head(h, W)
     k = _teacher(top_ids, top_logprobs, T)
-    nbytes = _size("olmax_lmhead_distill_workspace_bytes", T, d, V)
+    nbytes = _size("olmax_lmhead_distill_workspace_bytes", T, d, V, k)
     ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
     loss = torch.empty((), device=h.device, dtype=torch.float32)
     dh, dW = _head_grads(h, W, want_dh, want_dw, dw_f32)

@@ -129,7 +129,7 @@ def test_workspace_queries():
     from olmax_amd import ops
     assert ops._size("olmax_token_logprobs_workspace_bytes", 4096, 50304, 20, 0) == 0
     assert 0 < ops._size("olmax_token_logprobs_workspace_bytes", 1, 128256, 128, 0) <= 64 * (128 * 8 + 12)
-    assert ops._size("olmax_distill_workspace_bytes", 1000) >= 4004
+    assert ops._size("olmax_distill_workspace_bytes", 1000, 5000, 8, 0) >= 4004
     for T, d, V in ((1, 64, 100), (2048, 4096, 100278)):
         n = ops._size("olmax_lmhead_logprobs_bwd_workspace_bytes", T, d, V)
         assert n >= T * V * 2 and n % 256 == 0
