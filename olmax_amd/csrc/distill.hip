@@ -571,9 +571,24 @@ extern "C" int32_t olmax_distill(hipStream_t stream, const void* logits, void* d
 static int64_t head_stride(int32_t V) { return ((int64_t)V + 63) / 64 * 64; }
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
+struct HeadPlan {
+  bool few;       // tokens fewer than a tile has rows: the gradients' products pad them, and the logits' those of more than 64
+  int64_t rows, ld, grads_at, rows_at, h_at, dh_at, bytes;
+};
+static HeadPlan head_plan(int64_t T, int32_t d, int32_t V, int32_t k) {
+  HeadPlan p;
+  p.few = olmax_lmhead_pads(T, d, V);
+  p.rows = p.few && T > 64 ? 256 : T;
+  p.ld = head_stride(V);
+  p.grads_at = up256(std::max<int64_t>(p.rows * p.ld * 4, p.few ? PRODUCT_SCRATCH : 0));
+  p.rows_at = p.grads_at + up256((p.few ? 256 : T) * p.ld * 2);
+  p.h_at = p.rows_at + up256(olmax_distill_workspace_bytes(T, V, k, 1));
+  p.dh_at = p.h_at + (p.few ? up256(256ll * d * 2) : 0);
+  p.bytes = p.dh_at + (p.few ? up256(256ll * d * 2) : 0);
+  return p;
+}
 extern "C" int64_t olmax_lmhead_distill_workspace_bytes(int64_t T, int32_t d, int32_t V, int32_t k) {
-  if (T <= 0 || V <= 0) return 0;
-  return up256(T * head_stride(V) * 4) + up256(T * head_stride(V) * 2) + olmax_distill_workspace_bytes(T, V, k, 1);
+  return T <= 0 || V <= 0 || d <= 0 || k <= 0 || T >= (1 << 24) ? 0 : head_plan(T, d, V, k).bytes;
 }
 
 extern "C" int32_t olmax_lmhead_distill(hipStream_t stream, const void* h, const void* W, const int32_t* top_ids, const float* top_logprobs, float* loss,
@@ -582,15 +597,21 @@ extern "C" int32_t olmax_lmhead_distill(hipStream_t stream, const void* h, const
   OLMAX_CHECK(h && W && top_ids && top_logprobs && loss && workspace, OLMAX_ERR_ARG, "olmax_lmhead_distill: null pointer");
   if (int rc = distill_check("olmax_lmhead_distill", T, V, k, tail, temperature, softcap)) return rc;
   OLMAX_CHECK(d > 0, OLMAX_ERR_SHAPE, "olmax_lmhead_distill: bad shape d=%d", d);
-  OLMAX_CHECK(workspace_bytes >= olmax_lmhead_distill_workspace_bytes(T, d, V, k) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
-              "olmax_lmhead_distill: workspace needs %ld bytes, 256-byte aligned", (long)olmax_lmhead_distill_workspace_bytes(T, d, V, k));
-  const int64_t ld = head_stride(V);
+  const HeadPlan p = head_plan(T, d, V, k);
+  OLMAX_CHECK(workspace_bytes >= p.bytes && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_distill: workspace needs %ld bytes, 256-byte aligned", (long)p.bytes);
+  OLMAX_CHECK(aligned16(h) && aligned16(W) && aligned16(dh), OLMAX_ERR_ALIGN, "olmax_lmhead_distill: h, W and dh must be 16-byte aligned");
   const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
-  bf16* grads = (bf16*)((char*)workspace + up256(T * ld * 4));
-  void* row_ws = (char*)grads + up256(T * ld * 2);
-  if (int rc = olmax_gemm_padded(stream, hp, wp, workspace, nullptr, (int)T, V, d, d, d, ld, 0, true, true, true, false)) return rc;
-  if (int rc = distill(stream, workspace, dh || dW ? grads : nullptr, top_ids, top_logprobs, loss, nullptr, row_ws, T, V, k, ld, ld, true, false, tail, temperature,
-                       softcap, dloss, 0, (8 - V % 8) % 8))
+  char* ws = (char*)workspace;
+  bf16 *grads = (bf16*)(ws + p.grads_at), *h_pad = (bf16*)(ws + p.h_at);
+  const bool grad = dh || dW;
+  const int pad = (8 - V % 8) % 8;
+  if (p.few && (dW || p.rows > T)) olmax_pad_rows(stream, hp, h_pad, T, 256, d);
+  if (int rc = olmax_gemm_padded(stream, p.rows > T ? h_pad : hp, wp, workspace, nullptr, (int)p.rows, V, d, d, d, p.ld, 0, true, true, true, false)) return rc;
+  if (int rc = distill(stream, workspace, grad ? grads : nullptr, top_ids, top_logprobs, loss, nullptr, ws + p.rows_at, T, V, k, p.ld, p.ld, true, false, tail, temperature, softcap,
+                       dloss, 0, pad))
     return rc;
-  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0, GemmScratch{workspace, std::min<int64_t>(T * ld * 4, PRODUCT_SCRATCH)});
+  const GemmScratch scratch{workspace, std::min(p.grads_at, PRODUCT_SCRATCH)};  // (the logits are done with)
+  if (!p.few) return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, scratch);
+  if (dW) olmax_zero_rows(stream, grads, T, 64, V + pad, p.ld);
+  return olmax_lmhead_products_few(stream, grads, wp, hp, h_pad, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, (bf16*)(ws + p.dh_at), scratch);
 }

@@ -681,7 +681,10 @@ __device__ __forceinline__ void gemm_tile(
   if constexpr (ROW_STATS) {
     int targets[TM];
 #pragma unroll
-    for (int i = 0; i < TM; i++) targets[i] = head->targets ? head->targets[m0 + wm * WM + i * 16 + l16e] : -1;
+    for (int i = 0; i < TM; i++) {
+      const int row = m0 + wm * WM + i * 16 + l16e;
+      targets[i] = head->targets && row < head->rows ? head->targets[row] : -1;
+    }
     __syncthreads();  // every wave is done reading the operand stages
     rows::Stat* strip = reinterpret_cast<rows::Stat*>(smem);  // [WAVES_N][BM]
     const rows::Scale c = head->scale;
@@ -745,8 +748,9 @@ __device__ __forceinline__ void gemm_tile(
     const int first = n0 + wn * WN + g16e * 4;
     auto of_row = [&](auto capped, f32x4* x, int64_t row) {
       constexpr bool CAP = decltype(capped)::value;
-      const float m = head->stats[row * 3], log_sum = head->stats[row * 3 + 1], entropy = head->stats[row * 3 + 2];
-      const int target = head->targets[row];
+      const bool there = row < head->rows;
+      const float m = there ? head->stats[row * 3] : -INFINITY, log_sum = there ? head->stats[row * 3 + 1] : 0.f, entropy = there ? head->stats[row * 3 + 2] : 0.f;
+      const int target = there ? head->targets[row] : -1;
       const bool skipped = target == head->ignore_index || m == -INFINITY;
       const float g = target < 0 || target >= head->V || skipped ? 0.f : head->dlogprobs[row], h = head->dentropy && !skipped ? head->dentropy[row] : 0.f;
 #pragma unroll

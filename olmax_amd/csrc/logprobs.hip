@@ -272,6 +272,7 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
       a.raise(score<CAP>(most, c));
     }
     const float ref = a.ref();
+    const float cap_r = c.r_k * LOG2E, cap_top = (c.top - ref) * LOG2E;
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
       if (at + u * TH + (int)threadIdx.x >= v1) continue;
@@ -279,16 +280,22 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
       now[u].unpack(x);
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        const float d = behind<CAP>(x[e], c, ref);
-        x[e] = exp_of(d);
-        t[e] = x[e] * fmaxf(d, -200.f);
+        if (CAP) {  // scores are finite and small: in units of log 2, without a cut (three of 22 issue slots of a logit; these rows are bound by them)
+          const float d = __builtin_fmaf(tail_of_tanh(x[e], c), cap_r, cap_top);
+          x[e] = __builtin_amdgcn_exp2f(d);
+          t[e] = x[e] * d;
+        } else {
+          const float d = behind<CAP>(x[e], c, ref);
+          x[e] = exp_of(d);
+          t[e] = x[e] * fmaxf(d, -200.f);
+        }
       }
 #pragma unroll
       for (int w = N / 2; w > 0; w >>= 1)
 #pragma unroll
         for (int e = 0; e < w; e++) x[e] += x[e + w], t[e] += t[e + w];
       a.s += x[0];
-      a.t += t[0];
+      a.t += CAP ? t[0] * LN2 : t[0];
     }
     if (TOP) {
       if ((ch & (ch + 1)) == 0) {  // 1, 2, 4, .. chunks seen: about k candidates between two bounds, and those below the new one go where many ties came with them
@@ -415,19 +422,19 @@ __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ lo
   }
 }
 
-// The rows of an LM head whose product left statistics of 256 columns a tile (olmax_gemm_head_stats), [tiles][rows], and, for the last columns, logits (`rest`, from column
+// The rows of an LM head whose product left statistics of 256 columns a tile (olmax_gemm_head_stats), [tiles][ld_tiles], and, for the last columns, logits (`rest`, from column
 // `fused` on) with statistics of their own: 16 rows a workgroup, each sixteenth of a wave takes every 64th tile.  (64 rows a workgroup, a lane each: 20 us for 2048 rows of
 // 384 tiles, so 8.)
 template <bool CAP>
 __global__ __launch_bounds__(1024) void head_join_kernel(const Stat* __restrict__ tiles, int n_tiles, const Stat* __restrict__ rest_stat, const float* __restrict__ rest,
                                                          int64_t ld_rest, const float* __restrict__ target_logit, const int32_t* __restrict__ targets, Out out, int64_t rows,
-                                                         int V, int fused, int32_t ignore_index, Scale c) {
+                                                         int64_t ld_tiles, int V, int fused, int32_t ignore_index, Scale c) {
   __shared__ Stat part[16][16];
   const int wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x * 16ll + (threadIdx.x & 15);
   Stat a = Stat::none();
   if (row < rows)
-    for (int i = threadIdx.x >> 4; i < n_tiles; i += 64) a.join(tiles[(int64_t)i * rows + row]);
+    for (int i = threadIdx.x >> 4; i < n_tiles; i += 64) a.join(tiles[(int64_t)i * ld_tiles + row]);
 #pragma unroll
   for (int o = 16; o < 64; o <<= 1) {
     Stat b;
@@ -598,19 +605,22 @@ extern "C" int32_t olmax_token_logprobs_bwd(hipStream_t stream, const void* logi
 static int64_t head_stride(int32_t V) { return ((int64_t)V + 63) / 64 * 64; }  // whole lines of bf16 and fp32
 static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Memory of the forward call: fp32 logits of the columns from `fused` on, then (fused > 0) statistics of its tiles, of the other columns, and target logits
+// Memory of the forward call: fp32 logits of the columns from `fused` on, then (fused > 0) statistics of its tiles, of the other columns, target logits, and tokens that are
+// padded (to `rows`)
 struct HeadPlan {
   int fused;
-  int64_t ld, stats_at, rest_at, target_at, bytes;
+  int64_t rows, ld, stats_at, rest_at, target_at, h_at, bytes;
 };
 static HeadPlan head_plan(int64_t T, int32_t d, int32_t V, int32_t top) {
   HeadPlan p;
-  p.fused = top > 0 ? 0 : olmax_gemm_head_columns((int)T, V, d);
+  p.rows = top == 0 && T > 64 && olmax_lmhead_pads(T, d, V) ? 256 : T;
+  p.fused = top > 0 ? 0 : olmax_gemm_head_columns((int)p.rows, V, d);
   p.ld = head_stride(V - p.fused);
-  p.stats_at = up256(T * p.ld * 4);
-  p.rest_at = p.stats_at + up256((int64_t)((p.fused + 255) / 256) * T * sizeof(Stat));
+  p.stats_at = up256(p.rows * p.ld * 4);
+  p.rest_at = p.stats_at + up256((int64_t)((p.fused + 255) / 256) * p.rows * sizeof(Stat));
   p.target_at = p.rest_at + up256(T * sizeof(Stat));
-  p.bytes = p.fused ? p.target_at + up256(T * 4) : p.stats_at + olmax_token_logprobs_workspace_bytes(T, V, top, 1);
+  p.h_at = p.target_at + up256(T * 4);
+  p.bytes = p.fused ? p.h_at + (p.rows > T ? up256(p.rows * d * 2) : 0) : p.stats_at + olmax_token_logprobs_workspace_bytes(T, V, top, 1);
   return p;
 }
 
@@ -631,9 +641,13 @@ extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, cons
   OLMAX_CHECK(workspace_bytes >= p.bytes && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs: workspace needs %ld bytes, 256-byte aligned", (long)p.bytes);
   const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
   char* ws = (char*)workspace;
+  if (p.rows > T) {
+    olmax_pad_rows(stream, hp, (bf16*)(ws + p.h_at), T, p.rows, d);
+    hp = (bf16*)(ws + p.h_at);
+  }
   const int rest = V - p.fused;
   if (rest) {
-    if (int rc = olmax_gemm_padded(stream, hp, wp + (int64_t)p.fused * d, ws, nullptr, (int)T, rest, d, d, d, p.ld, 0, true, true, true, false)) return rc;
+    if (int rc = olmax_gemm_padded(stream, hp, wp + (int64_t)p.fused * d, ws, nullptr, (int)p.rows, rest, d, d, d, p.ld, 0, true, true, true, false)) return rc;
   }
   if (!p.fused)
     return olmax_token_logprobs(stream, ws, targets, logprobs, entropy, stats, top_ids, top_logprobs, ws + p.stats_at, workspace_bytes - p.stats_at, T, V, p.ld, top, 1,
@@ -646,22 +660,38 @@ extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, cons
   rows.targets = targets;
   rows.ignore_index = ignore_index;
   rows.V = V;
+  rows.rows = (int)T;
   rows.scale = c;
   rows.parts = (float*)tiles;
   rows.target_logit = target_logit;
-  if (int rc = olmax_gemm_head_stats(stream, hp, wp, (int)T, p.fused, d, rows)) return rc;
-#define JOIN(CAPV)                                                                                                                                                        do {                                                                                                                                                                      if (rest)                                                                                                                                                                 hipLaunchKernelGGL((score_rows_kernel<float, CAPV, false, 256>), dim3((unsigned)T), dim3(256), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,                          p.ld, ignore_index, c, 0, 1);                                                                                                                      hipLaunchKernelGGL((head_join_kernel<CAPV>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,                        (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, V, p.fused, ignore_index, c);                                                 } while (0)
+  if (int rc = olmax_gemm_head_stats(stream, hp, wp, (int)p.rows, p.fused, d, rows)) return rc;
+#define JOIN(CAPV)                                                                                                                                                        do {                                                                                                                                                                      if (rest)                                                                                                                                                                 hipLaunchKernelGGL((score_rows_kernel<float, CAPV, false, 256>), dim3((unsigned)T), dim3(256), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,                          p.ld, ignore_index, c, 0, 1);                                                                                                                      hipLaunchKernelGGL((head_join_kernel<CAPV>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,                        (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, p.rows, V, p.fused, ignore_index, c);                                                 } while (0)
   if (softcap > 0.f) JOIN(true); else JOIN(false);
 #undef JOIN
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }
 
-// The backward call's: bf16 gradients, then fp32 logits of the columns from `fused` on and, in the same place afterwards, room for the products' partial sums
-static int64_t head_grads_room(int64_t T, int fused, int32_t V) { return std::max(up256(T * head_stride(V - fused) * 4), fused ? PRODUCT_SCRATCH : 0); }
+// The backward call's: bf16 gradients, then fp32 logits of the columns from `fused` on and, in the same place afterwards, room for the products' partial sums; then (tokens
+// padded to `rows`) the padded tokens, and room for dh
+struct HeadGradPlan {
+  int fused;
+  int64_t rows, ld, logits_at, room, h_at, dh_at, bytes;
+};
+static HeadGradPlan head_grad_plan(int64_t T, int32_t d, int32_t V) {
+  HeadGradPlan p;
+  p.rows = olmax_lmhead_pads(T, d, V) ? 256 : T;
+  p.fused = olmax_gemm_head_columns((int)p.rows, V, d);
+  p.ld = head_stride(V);
+  p.logits_at = up256(p.rows * p.ld * 2);
+  p.room = std::max(up256(p.rows * head_stride(V - p.fused) * 4), p.fused ? PRODUCT_SCRATCH : 0);
+  p.h_at = p.logits_at + p.room;
+  p.dh_at = p.h_at + (p.rows > T ? up256(p.rows * d * 2) : 0);
+  p.bytes = p.dh_at + (p.rows > T ? up256(p.rows * d * 2) : 0);
+  return p;
+}
 extern "C" int64_t olmax_lmhead_logprobs_bwd_workspace_bytes(int64_t T, int32_t d, int32_t V) {
-  if (T <= 0 || V <= 0 || d <= 0 || T >= (1 << 24)) return 0;
-  return up256(T * head_stride(V) * 2) + head_grads_room(T, olmax_gemm_head_columns((int)T, V, d), V);
+  return T <= 0 || V <= 0 || d <= 0 || T >= (1 << 24) ? 0 : head_grad_plan(T, d, V).bytes;
 }
 
 extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, const void* W, const int32_t* targets, const float* stats,
@@ -670,33 +700,40 @@ extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, 
   OLMAX_CHECK(h && W && targets && stats && dlogprobs && workspace && (dh || dW), OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: null pointer");
   OLMAX_CHECK(T > 0 && d > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs_bwd: bad shape T=%ld d=%d V=%d", (long)T, d, V);
   OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
-  OLMAX_CHECK(aligned16(h) && aligned16(W), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs_bwd: h and W must be 16-byte aligned");
-  OLMAX_CHECK(workspace_bytes >= olmax_lmhead_logprobs_bwd_workspace_bytes(T, d, V) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
-              "olmax_lmhead_logprobs_bwd: workspace needs %ld bytes, 256-byte aligned", (long)olmax_lmhead_logprobs_bwd_workspace_bytes(T, d, V));
-  const int64_t ld = head_stride(V);
-  const int fused = olmax_gemm_head_columns((int)T, V, d), rest = V - fused, pad = (8 - V % 8) % 8;
+  OLMAX_CHECK(aligned16(h) && aligned16(W) && aligned16(dh), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs_bwd: h, W and dh must be 16-byte aligned");
+  const HeadGradPlan p = head_grad_plan(T, d, V);
+  OLMAX_CHECK(workspace_bytes >= p.bytes && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs_bwd: workspace needs %ld bytes, 256-byte aligned", (long)p.bytes);
+  const int rest = V - p.fused, pad = (8 - V % 8) % 8, rows_of = (int)p.rows;
   const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
-  bf16* grads = (bf16*)workspace;
-  float* logits = (float*)((char*)workspace + up256(T * ld * 2));
-  if (fused) {
-    const Scale c = scale_of(temperature, softcap);
+  char* ws = (char*)workspace;
+  bf16* grads = (bf16*)ws;
+  float* logits = (float*)(ws + p.logits_at);
+  const bool padded = p.rows > T;
+  bf16* h_pad = (bf16*)(ws + p.h_at);
+  if (padded) olmax_pad_rows(stream, hp, h_pad, T, p.rows, d);
+  const bf16* tokens = padded ? h_pad : hp;
+  if (p.fused) {
     HeadRows rows{};
     rows.targets = targets;
     rows.ignore_index = ignore_index;
     rows.V = V;
-    rows.scale = c;
+    rows.rows = (int)T;
+    rows.scale = scale_of(temperature, softcap);
     rows.stats = stats, rows.dlogprobs = dlogprobs, rows.dentropy = dentropy;
-    if (int rc = olmax_gemm_head_grads(stream, hp, wp, grads, ld, (int)T, fused, d, rows)) return rc;
+    if (int rc = olmax_gemm_head_grads(stream, tokens, wp, grads, p.ld, rows_of, p.fused, d, rows)) return rc;
   }
   if (rest) {
     const int64_t ldr = head_stride(rest);
-    if (int rc = olmax_gemm_padded(stream, hp, wp + (int64_t)fused * d, logits, nullptr, (int)T, rest, d, d, d, ldr, 0, true, true, true, false)) return rc;
-    if (int rc = token_logprobs_bwd(stream, logits, targets, stats, dlogprobs, dentropy, grads + fused, T, rest, ldr, ld, true, false, ignore_index, temperature, softcap, pad, fused))
+    if (int rc = olmax_gemm_padded(stream, tokens, wp + (int64_t)p.fused * d, logits, nullptr, rows_of, rest, d, d, d, ldr, 0, true, true, true, false)) return rc;
+    if (int rc = token_logprobs_bwd(stream, logits, targets, stats, dlogprobs, dentropy, grads + p.fused, T, rest, ldr, p.ld, true, false, ignore_index, temperature, softcap, pad,
+                                    p.fused))
       return rc;
+    if (padded) olmax_zero_rows(stream, grads + p.fused, T, 64, rest + pad, p.ld);
   } else if (pad) {
-    hipLaunchKernelGGL(zero_columns_kernel, dim3((unsigned)((T * pad + 255) / 256)), dim3(256), 0, stream, grads + V, T, ld, pad);
+    hipLaunchKernelGGL(zero_columns_kernel, dim3((unsigned)((p.rows * pad + 255) / 256)), dim3(256), 0, stream, grads + V, p.rows, p.ld, pad);
   }
+  const GemmScratch scratch{logits, std::min(p.room, PRODUCT_SCRATCH)};
+  if (padded) return olmax_lmhead_products_few(stream, grads, wp, hp, h_pad, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, (bf16*)(ws + p.dh_at), scratch);
   // (without shared reductions the few long ones of dh take 60 % more: dh and dW of 1024 x 4096 x 100352 1.78 -> 1.34 ms)
-  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, ld, dw_f32 != 0,
-                               GemmScratch{logits, std::min(head_grads_room(T, fused, V), PRODUCT_SCRATCH)});
+  return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, scratch);
 }

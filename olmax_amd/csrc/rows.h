@@ -174,8 +174,9 @@ __device__ __forceinline__ float score_grad(float x, const Scale& c, float m, fl
 
 // gemm.hip: the LM head's product with a row's part of its softmax in the epilogue (logprobs.hip): logits leave the kernel only as what is formed of them.
 struct HeadRows {
-  const int32_t* targets;     // [M]
+  const int32_t* targets;     // [rows]
   int32_t ignore_index, V;    // V: of the whole product; a target from there on has no logit
+  int32_t rows;               // that there are: up to M, those behind pad the product (their gradients are zeros)
   rows::Scale scale;
   float *parts, *target_logit;  // statistics: [ceil(N / 256)][M][3], (largest score, sum of exponentials behind it, that sum weighted by z - m) of 256 columns; the
                                 // logit x of each target that is one of the columns
@@ -187,3 +188,15 @@ int olmax_gemm_head_columns(int M, int N, int K);
 int olmax_gemm_head_stats(hipStream_t s, const bf16* h, const bf16* w, int M, int N, int K, const HeadRows& rows);
 // d [M, ldd] (16-byte aligned, ldd a multiple of 8): columns 0 .. N
 int olmax_gemm_head_grads(hipStream_t s, const bf16* h, const bf16* w, bf16* d, int64_t ldd, int M, int N, int K, const HeadRows& rows);
+
+// lmhead_rows.hip: the LM head's products on fewer tokens than a tile of 256 has rows.  Whether large tiles do better with the tokens padded to 256 (for the logits of more than
+// 64 tokens, and for the gradients):
+bool olmax_lmhead_pads(int64_t T, int32_t d, int32_t V);
+// dst [padded, d] = src [rows, d] and zeros; d is a multiple of 8 and both are 16-byte aligned
+void olmax_pad_rows(hipStream_t s, const bf16* src, bf16* dst, int64_t rows, int64_t padded, int d);
+// columns [0, n) of rows [from, to) of d = 0
+void olmax_zero_rows(hipStream_t s, bf16* d, int64_t from, int64_t to, int64_t n, int64_t ld);
+// olmax_lmhead_products of T < 256 tokens: dlogits has 256 rows of memory, h_pad [64, d] is h and zeros (read, as rows T to 63 of dlogits are, where T < 64), tmp [256, d] is room
+// for dh
+int olmax_lmhead_products_few(hipStream_t stream, const bf16* dlogits, const bf16* W, const bf16* h, const bf16* h_pad, bf16* dh, void* dW, int T, int d, int V, int64_t ldl,
+                              bool dw_f32, bf16* tmp, GemmScratch scratch);
