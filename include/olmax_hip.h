@@ -372,6 +372,33 @@ int32_t olmax_model_loss(olmax_stream_t stream, const olmax_model_config* cfg, c
                          const void* params_bf16, const int32_t* ids, const int32_t* labels,
                          float* loss, void* workspace, int64_t workspace_bytes);
 
+/* The model with olmax_lmhead_logprobs, its gradients and olmax_lmhead_distill in the place of the cross entropy (arguments as theirs; the soft-cap is
+ * the configuration's final_softcap; no counterparts in the reference).  A policy-gradient step is a logprobs call, cotangents formed from its
+ * outputs, and a grads call on the same parameters; the gradients are laid out as olmax_model_loss_and_grads leaves them.  head_workspace: what
+ * the LM head's call wants for [batch * seq_len] tokens, 256-byte aligned, apart from workspace. */
+int32_t olmax_model_logprobs(olmax_stream_t stream, const olmax_model_config* cfg, const int32_t* windows,
+                             const float* const* cos_tables, const float* const* sin_tables,
+                             const void* params_bf16, const int32_t* ids, const int32_t* targets,
+                             float* logprobs, float* entropy, float* stats, int32_t* top_ids,
+                             float* top_logprobs, void* workspace, int64_t workspace_bytes,
+                             void* head_workspace, int64_t head_workspace_bytes, int32_t top,
+                             int32_t ignore_index, float temperature);
+int32_t olmax_model_logprobs_grads(olmax_stream_t stream, const olmax_model_config* cfg, const int32_t* windows,
+                                   const float* const* cos_tables, const float* const* sin_tables,
+                                   const void* params_bf16, const int32_t* ids, const int32_t* targets,
+                                   const float* stats, const float* dlogprobs, const float* dentropy,
+                                   void* grad_bf16, float* grad_f32, void* workspace, int64_t workspace_bytes,
+                                   void* head_workspace, int64_t head_workspace_bytes, int32_t ignore_index,
+                                   float temperature);
+int32_t olmax_model_distill_loss_and_grads(olmax_stream_t stream, const olmax_model_config* cfg,
+                                           const int32_t* windows, const float* const* cos_tables,
+                                           const float* const* sin_tables, const void* params_bf16,
+                                           const int32_t* ids, const int32_t* top_ids,
+                                           const float* top_logprobs, float* loss, void* grad_bf16,
+                                           float* grad_f32, void* workspace, int64_t workspace_bytes,
+                                           void* head_workspace, int64_t head_workspace_bytes, int32_t k,
+                                           int32_t tail, float temperature, float dloss);
+
 /* step_optimizer, src/olmax/train/trainer.py:742-757: fused AdamW over every leaf.
  * leaf_decay: host array with one entry per leaf in olmax_model_layout order, 0 = the leaf is
  * exempt from weight decay, the mask of OptimConfig.build_weight_decay_mask

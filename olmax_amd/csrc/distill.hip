@@ -591,15 +591,21 @@ extern "C" int64_t olmax_lmhead_distill_workspace_bytes(int64_t T, int32_t d, in
   return T <= 0 || V <= 0 || d <= 0 || k <= 0 || T >= (1 << 24) ? 0 : head_plan(T, d, V, k).bytes;
 }
 
+int olmax_lmhead_distill_check(const HeadDistill& a) {
+  OLMAX_CHECK(a.h && a.W && a.top_ids && a.top_logprobs && a.loss && a.workspace, OLMAX_ERR_ARG, "olmax_lmhead_distill: null pointer");
+  if (int rc = distill_check("olmax_lmhead_distill", a.T, a.V, a.k, a.tail, a.temperature, a.softcap)) return rc;
+  OLMAX_CHECK(a.d > 0, OLMAX_ERR_SHAPE, "olmax_lmhead_distill: bad shape d=%d", a.d);
+  OLMAX_CHECK(aligned16(a.h) && aligned16(a.W) && aligned16(a.dh), OLMAX_ERR_ALIGN, "olmax_lmhead_distill: h, W and dh must be 16-byte aligned");
+  const int64_t need = head_plan(a.T, a.d, a.V, a.k).bytes;
+  OLMAX_CHECK(a.workspace_bytes >= need && (((uintptr_t)a.workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_distill: workspace needs %ld bytes, 256-byte aligned", (long)need);
+  return OLMAX_OK;
+}
+
 extern "C" int32_t olmax_lmhead_distill(hipStream_t stream, const void* h, const void* W, const int32_t* top_ids, const float* top_logprobs, float* loss,
                                         void* dh, void* dW, void* workspace, int64_t workspace_bytes, int64_t T, int32_t d, int32_t V, int32_t k,
                                         int32_t tail, float temperature, float softcap, float dloss, int32_t dw_f32) {
-  OLMAX_CHECK(h && W && top_ids && top_logprobs && loss && workspace, OLMAX_ERR_ARG, "olmax_lmhead_distill: null pointer");
-  if (int rc = distill_check("olmax_lmhead_distill", T, V, k, tail, temperature, softcap)) return rc;
-  OLMAX_CHECK(d > 0, OLMAX_ERR_SHAPE, "olmax_lmhead_distill: bad shape d=%d", d);
+  if (int rc = olmax_lmhead_distill_check({h, W, top_ids, top_logprobs, loss, dh, workspace, workspace_bytes, T, d, V, k, tail, temperature, softcap})) return rc;
   const HeadPlan p = head_plan(T, d, V, k);
-  OLMAX_CHECK(workspace_bytes >= p.bytes && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_distill: workspace needs %ld bytes, 256-byte aligned", (long)p.bytes);
-  OLMAX_CHECK(aligned16(h) && aligned16(W) && aligned16(dh), OLMAX_ERR_ALIGN, "olmax_lmhead_distill: h, W and dh must be 16-byte aligned");
   const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
   char* ws = (char*)workspace;
   bf16 *grads = (bf16*)(ws + p.grads_at), *h_pad = (bf16*)(ws + p.h_at);

@@ -628,17 +628,26 @@ extern "C" int64_t olmax_lmhead_logprobs_workspace_bytes(int64_t T, int32_t d, i
   return T <= 0 || V <= 0 || d <= 0 || T >= (1 << 24) ? 0 : head_plan(T, d, V, top).bytes;
 }
 
+int olmax_lmhead_logprobs_check(const HeadScore& a) {
+  OLMAX_CHECK(a.h && a.W && a.workspace && a.entropy && a.stats && (!a.logprobs || a.targets), OLMAX_ERR_ARG, "olmax_lmhead_logprobs: null pointer");
+  OLMAX_CHECK(a.T > 0 && a.d > 0 && a.V > 0 && a.T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs: bad shape T=%ld d=%d V=%d", (long)a.T, a.d, a.V);
+  OLMAX_CHECK(a.top >= 0 && a.top <= MAX_TOP && a.top <= a.V && (a.top == 0 || (a.top_ids && a.top_logprobs)), OLMAX_ERR_ARG,
+              "olmax_lmhead_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, a.top);
+  OLMAX_CHECK(a.temperature >= 1e-6f && a.temperature <= 1e6f && a.softcap >= 0.f && a.softcap <= 1e30f, OLMAX_ERR_ARG,
+              "olmax_lmhead_logprobs: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(aligned16(a.h) && aligned16(a.W), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs: h and W must be 16-byte aligned");
+  const int64_t need = head_plan(a.T, a.d, a.V, a.top).bytes;
+  OLMAX_CHECK(a.workspace_bytes >= need && (((uintptr_t)a.workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs: workspace needs %ld bytes, 256-byte aligned", (long)need);
+  return OLMAX_OK;
+}
+
 extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, const void* W, const int32_t* targets, float* logprobs, float* entropy,
                                          float* stats, int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes, int64_t T,
                                          int32_t d, int32_t V, int32_t top, int32_t ignore_index, float temperature, float softcap) {
-  OLMAX_CHECK(h && W && workspace && entropy && stats && (!logprobs || targets), OLMAX_ERR_ARG, "olmax_lmhead_logprobs: null pointer");
-  OLMAX_CHECK(T > 0 && d > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs: bad shape T=%ld d=%d V=%d", (long)T, d, V);
-  OLMAX_CHECK(top >= 0 && top <= MAX_TOP && top <= V && (top == 0 || (top_ids && top_logprobs)), OLMAX_ERR_ARG,
-              "olmax_lmhead_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, top);
-  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_lmhead_logprobs: temperature within 1e-6 and 1e6, softcap not negative");
-  OLMAX_CHECK(aligned16(h) && aligned16(W), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs: h and W must be 16-byte aligned");
+  if (int rc = olmax_lmhead_logprobs_check({h, W, targets, logprobs, entropy, stats, top_ids, top_logprobs, workspace, workspace_bytes, T, d, V, top, ignore_index, temperature,
+                                            softcap}))
+    return rc;
   const HeadPlan p = head_plan(T, d, V, top);
-  OLMAX_CHECK(workspace_bytes >= p.bytes && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs: workspace needs %ld bytes, 256-byte aligned", (long)p.bytes);
   const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
   char* ws = (char*)workspace;
   if (p.rows > T) {
@@ -694,15 +703,23 @@ extern "C" int64_t olmax_lmhead_logprobs_bwd_workspace_bytes(int64_t T, int32_t 
   return T <= 0 || V <= 0 || d <= 0 || T >= (1 << 24) ? 0 : head_grad_plan(T, d, V).bytes;
 }
 
+int olmax_lmhead_logprobs_bwd_check(const HeadScoreGrad& a) {
+  OLMAX_CHECK(a.h && a.W && a.targets && a.stats && a.dlogprobs && a.workspace && (a.dh || a.dW), OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: null pointer");
+  OLMAX_CHECK(a.T > 0 && a.d > 0 && a.V > 0 && a.T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs_bwd: bad shape T=%ld d=%d V=%d", (long)a.T, a.d, a.V);
+  OLMAX_CHECK(a.temperature >= 1e-6f && a.temperature <= 1e6f && a.softcap >= 0.f && a.softcap <= 1e30f, OLMAX_ERR_ARG,
+              "olmax_lmhead_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(aligned16(a.h) && aligned16(a.W) && aligned16(a.dh), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs_bwd: h, W and dh must be 16-byte aligned");
+  const int64_t need = head_grad_plan(a.T, a.d, a.V).bytes;
+  OLMAX_CHECK(a.workspace_bytes >= need && (((uintptr_t)a.workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs_bwd: workspace needs %ld bytes, 256-byte aligned",
+              (long)need);
+  return OLMAX_OK;
+}
+
 extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, const void* W, const int32_t* targets, const float* stats,
                                              const float* dlogprobs, const float* dentropy, void* dh, void* dW, void* workspace, int64_t workspace_bytes,
                                              int64_t T, int32_t d, int32_t V, int32_t ignore_index, float temperature, float softcap, int32_t dw_f32) {
-  OLMAX_CHECK(h && W && targets && stats && dlogprobs && workspace && (dh || dW), OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: null pointer");
-  OLMAX_CHECK(T > 0 && d > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs_bwd: bad shape T=%ld d=%d V=%d", (long)T, d, V);
-  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
-  OLMAX_CHECK(aligned16(h) && aligned16(W) && aligned16(dh), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs_bwd: h, W and dh must be 16-byte aligned");
+  if (int rc = olmax_lmhead_logprobs_bwd_check({h, W, targets, stats, dlogprobs, dentropy, dh, dW, workspace, workspace_bytes, T, d, V, temperature, softcap})) return rc;
   const HeadGradPlan p = head_grad_plan(T, d, V);
-  OLMAX_CHECK(workspace_bytes >= p.bytes && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs_bwd: workspace needs %ld bytes, 256-byte aligned", (long)p.bytes);
   const int rest = V - p.fused, pad = (8 - V % 8) % 8, rows_of = (int)p.rows;
   const bf16 *hp = (const bf16*)h, *wp = (const bf16*)W;
   char* ws = (char*)workspace;

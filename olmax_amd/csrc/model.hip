@@ -8,7 +8,7 @@
 // (src/olmax/nn/transformer/model.py:95-136), compute_loss_and_grads and step_optimizer
 // (src/olmax/train/trainer.py:723-757).  The backward pass, which the reference obtains from
 // eqx.filter_value_and_grad, is written out by hand here.
-#include "common.h"
+#include "rows.h"
 #include "olmax_hip.h"
 #include <algorithm>
 
@@ -447,12 +447,54 @@ struct GradReady {
   int operator()(int layer) const { return fn ? fn(ctx, layer) : OLMAX_OK; }
 };
 
+// What follows the final norm: the cross entropy of the labels, or another call on its output and the LM head, checked before anything of the model is launched.
+struct HeadOp {
+  enum Kind { CROSS_ENTROPY, LOGPROBS, LOGPROBS_GRADS, DISTILL } kind = CROSS_ENTROPY;
+  HeadScore score{};
+  HeadScoreGrad grad{};
+  HeadDistill distill{};
+  float dloss = 1.f;
+  int32_t ignore_index = -100;
+
+  int check(const void* h, const void* W, void* dh, void* dW) const {
+    if (kind == LOGPROBS) {
+      HeadScore a = score;
+      a.h = h, a.W = W;
+      return olmax_lmhead_logprobs_check(a);
+    }
+    if (kind == LOGPROBS_GRADS) {
+      HeadScoreGrad a = grad;
+      a.h = h, a.W = W, a.dh = dh, a.dW = dW;
+      return olmax_lmhead_logprobs_bwd_check(a);
+    }
+    HeadDistill a = distill;
+    a.h = h, a.W = W, a.dh = dh;
+    return olmax_lmhead_distill_check(a);
+  }
+  int run(hipStream_t s, const void* h, const void* W, void* dh, void* dW, int dw_f32) const {
+    if (kind == LOGPROBS) {
+      const HeadScore& a = score;
+      return olmax_lmhead_logprobs(s, h, W, a.targets, a.logprobs, a.entropy, a.stats, a.top_ids, a.top_logprobs, a.workspace, a.workspace_bytes, a.T, a.d, a.V, a.top,
+                                   a.ignore_index, a.temperature, a.softcap);
+    }
+    if (kind == LOGPROBS_GRADS) {
+      const HeadScoreGrad& a = grad;
+      return olmax_lmhead_logprobs_bwd(s, h, W, a.targets, a.stats, a.dlogprobs, a.dentropy, dh, dW, a.workspace, a.workspace_bytes, a.T, a.d, a.V, ignore_index, a.temperature,
+                                       a.softcap, dw_f32);
+    }
+    const HeadDistill& a = distill;
+    return olmax_lmhead_distill(s, h, W, a.top_ids, a.top_logprobs, a.loss, dh, dW, a.workspace, a.workspace_bytes, a.T, a.d, a.V, a.k, a.tail, a.temperature, a.softcap, dloss,
+                                dw_f32);
+  }
+};
+
 int model_run(hipStream_t s, const olmax_model_config* c, const int32_t* windows, const float* const* cos_tables,
               const float* const* sin_tables, const void* params_bf16, const int32_t* ids, const int32_t* labels,
               float* loss, void* grad_bf16, float* grad_f32, void* workspace, int64_t workspace_bytes, bool bwd,
-              GradReady ready = GradReady()) {
+              GradReady ready = GradReady(), const HeadOp& head = HeadOp()) {
   RC(check_cfg(c));
-  OLMAX_CHECK(params_bf16 && ids && labels && loss && workspace, OLMAX_ERR_ARG, "olmax_model: null pointer");
+  const bool ce = head.kind == HeadOp::CROSS_ENTROPY;
+  OLMAX_CHECK(params_bf16 && ids && (!ce || (labels && loss)) && workspace, OLMAX_ERR_ARG, "olmax_model: null pointer");
   OLMAX_CHECK(!bwd || (grad_bf16 && grad_f32), OLMAX_ERR_ARG, "olmax_model: gradient buffers are null");
   OLMAX_CHECK(c->n_layers == 0 || (windows && cos_tables && sin_tables), OLMAX_ERR_ARG, "olmax_model: per-layer tables are null");
   OLMAX_CHECK((((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_ALIGN, "olmax_model: workspace must be 256-byte aligned");
@@ -468,6 +510,9 @@ int model_run(hipStream_t s, const olmax_model_config* c, const int32_t* windows
   const int64_t Td = m.T * m.d;
   const int nl = c->n_layers;
   const bool keep = bwd && !c->checkpoint;
+  const bf16* Wout = c->tied ? P + L.embedding : P + L.lm_head;
+  void* dWout = !bwd ? nullptr : c->tied ? (void*)(grad_f32 + L.f_embedding) : (void*)(G + L.lm_head);
+  if (!ce) RC(head.check(w.hn, Wout, bwd ? w.da : nullptr, dWout));
 
   // RAII scope: a failing RC() return still closes the range
   struct Range {
@@ -494,8 +539,8 @@ int model_run(hipStream_t s, const olmax_model_config* c, const int32_t* windows
   Range rg_head("olmax.lm_head_and_loss", 0);
   const bf16* xl = w.xs + (int64_t)nl * Td;
   RC(olmax_rmsnorm_fwd(s, xl, P + L.final_norm, w.hn, m.T, m.d, m.d, m.d, c->eps));
-  const bf16* Wout = c->tied ? P + L.embedding : P + L.lm_head;
   if (!bwd) {
+    if (!ce) return head.run(s, w.hn, Wout, nullptr, nullptr, 0);
     return olmax_lmhead_ce(s, w.hn, Wout, labels, loss, nullptr, nullptr, w.head_ws, w.head_ws_bytes, m.T, m.d, c->vocab,
                            -100, c->final_softcap, 0);
   }
@@ -506,7 +551,9 @@ int model_run(hipStream_t s, const olmax_model_config* c, const int32_t* windows
     const int64_t skip = c->tied ? (int64_t)c->vocab * m.d : 0;
     RC(olmax_fill_zero(s, grad_f32 + L.f_embedding + skip, (L.f_total - skip) * 4));
   }
-  if (c->tied) {
+  if (!ce) {
+    RC(head.run(s, w.hn, Wout, w.da, dWout, c->tied));
+  } else if (c->tied) {
     // head dW is written (fp32) straight into the embedding's accumulator; the scatter-add follows
     RC(olmax_lmhead_ce_scratch(s, w.hn, Wout, labels, loss, w.da, grad_f32 + L.f_embedding, w.head_ws, w.head_ws_bytes, m.T,
                                m.d, c->vocab, -100, c->final_softcap, 1, w.tmp.before()));
@@ -857,6 +904,43 @@ extern "C" int32_t olmax_model_loss(hipStream_t s, const olmax_model_config* c, 
                                     void* workspace, int64_t workspace_bytes) {
   return model_run(s, c, windows, cos_tables, sin_tables, params_bf16, ids, labels, loss, nullptr, nullptr, workspace,
                    workspace_bytes, false);
+}
+
+// (sizes as the configuration has them: a bad one is refused by model_run)
+extern "C" int32_t olmax_model_logprobs(hipStream_t s, const olmax_model_config* c, const int32_t* windows, const float* const* cos_tables, const float* const* sin_tables,
+                                        const void* params_bf16, const int32_t* ids, const int32_t* targets, float* logprobs, float* entropy, float* stats, int32_t* top_ids,
+                                        float* top_logprobs, void* workspace, int64_t workspace_bytes, void* head_workspace, int64_t head_workspace_bytes, int32_t top,
+                                        int32_t ignore_index, float temperature) {
+  RC(check_cfg(c));
+  HeadOp head;
+  head.kind = HeadOp::LOGPROBS;
+  head.score = {nullptr, nullptr, targets, logprobs, entropy, stats, top_ids, top_logprobs, head_workspace, head_workspace_bytes, (int64_t)c->batch * c->seq_len, c->d_model,
+                c->vocab, top, ignore_index, temperature, c->final_softcap};
+  return model_run(s, c, windows, cos_tables, sin_tables, params_bf16, ids, nullptr, nullptr, nullptr, nullptr, workspace, workspace_bytes, false, GradReady(), head);
+}
+extern "C" int32_t olmax_model_logprobs_grads(hipStream_t s, const olmax_model_config* c, const int32_t* windows, const float* const* cos_tables, const float* const* sin_tables,
+                                              const void* params_bf16, const int32_t* ids, const int32_t* targets, const float* stats, const float* dlogprobs,
+                                              const float* dentropy, void* grad_bf16, float* grad_f32, void* workspace, int64_t workspace_bytes, void* head_workspace,
+                                              int64_t head_workspace_bytes, int32_t ignore_index, float temperature) {
+  RC(check_cfg(c));
+  HeadOp head;
+  head.kind = HeadOp::LOGPROBS_GRADS;
+  head.ignore_index = ignore_index;
+  head.grad = {nullptr, nullptr, targets, stats, dlogprobs, dentropy, nullptr, nullptr, head_workspace, head_workspace_bytes, (int64_t)c->batch * c->seq_len, c->d_model, c->vocab,
+               temperature, c->final_softcap};
+  return model_run(s, c, windows, cos_tables, sin_tables, params_bf16, ids, nullptr, nullptr, grad_bf16, grad_f32, workspace, workspace_bytes, true, GradReady(), head);
+}
+extern "C" int32_t olmax_model_distill_loss_and_grads(hipStream_t s, const olmax_model_config* c, const int32_t* windows, const float* const* cos_tables,
+                                                      const float* const* sin_tables, const void* params_bf16, const int32_t* ids, const int32_t* top_ids,
+                                                      const float* top_logprobs, float* loss, void* grad_bf16, float* grad_f32, void* workspace, int64_t workspace_bytes,
+                                                      void* head_workspace, int64_t head_workspace_bytes, int32_t k, int32_t tail, float temperature, float dloss) {
+  RC(check_cfg(c));
+  HeadOp head;
+  head.kind = HeadOp::DISTILL;
+  head.dloss = dloss;
+  head.distill = {nullptr, nullptr, top_ids, top_logprobs, loss, nullptr, head_workspace, head_workspace_bytes, (int64_t)c->batch * c->seq_len, c->d_model, c->vocab, k, tail,
+                  temperature, c->final_softcap};
+  return model_run(s, c, windows, cos_tables, sin_tables, params_bf16, ids, nullptr, nullptr, grad_bf16, grad_f32, workspace, workspace_bytes, true, GradReady(), head);
 }
 
 extern "C" int32_t olmax_model_adamw(hipStream_t s, const olmax_model_config* c, float* master, float* mom, float* var,

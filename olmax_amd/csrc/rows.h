@@ -200,3 +200,38 @@ void olmax_zero_rows(hipStream_t s, bf16* d, int64_t from, int64_t to, int64_t n
 // for dh
 int olmax_lmhead_products_few(hipStream_t stream, const bf16* dlogits, const bf16* W, const bf16* h, const bf16* h_pad, bf16* dh, void* dW, int T, int d, int V, int64_t ldl,
                               bool dw_f32, bf16* tmp, GemmScratch scratch);
+
+// What the LM head's calls are given, for their checks ahead of any launch (olmax_model_logprobs and its like make them ahead of the model's).
+struct HeadScore {
+  const void *h, *W;
+  const int32_t* targets;
+  float *logprobs, *entropy, *stats;
+  int32_t* top_ids;
+  float* top_logprobs;
+  void* workspace;
+  int64_t workspace_bytes, T;
+  int32_t d, V, top, ignore_index;
+  float temperature, softcap;
+};
+struct HeadScoreGrad {
+  const void *h, *W;
+  const int32_t* targets;
+  const float *stats, *dlogprobs, *dentropy;
+  void *dh, *dW, *workspace;
+  int64_t workspace_bytes, T;
+  int32_t d, V;
+  float temperature, softcap;
+};
+struct HeadDistill {
+  const void *h, *W;
+  const int32_t* top_ids;
+  const float* top_logprobs;
+  float* loss;
+  void *dh, *workspace;
+  int64_t workspace_bytes, T;
+  int32_t d, V, k, tail;
+  float temperature, softcap;
+};
+int olmax_lmhead_logprobs_check(const HeadScore& a);
+int olmax_lmhead_logprobs_bwd_check(const HeadScoreGrad& a);
+int olmax_lmhead_distill_check(const HeadDistill& a);

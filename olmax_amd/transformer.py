@@ -386,6 +386,52 @@ class Transformer:
             ptr(ids), ptr(labels), ptr(self.loss), ptr(ws), i64(ws.numel())))
         return self.loss
 
+    def _head_workspace(self, name: str, *more: int) -> torch.Tensor:
+        c = self.config
+        n = ops._size(name, self.batch_size * self.sequence_length, c.d_model, c.vocab_size, *more)
+        return torch.empty(n, device=self.device, dtype=torch.uint8)
+
+    def token_logprobs(self, ids: torch.Tensor, targets: Optional[torch.Tensor] = None, *, top: int = 0, temperature: float = 1.0,
+                       ignore_index: int = -100) -> ops.TokenLogprobs:
+        """The model's log probabilities of targets (flat [batch * sequence], as labels are: the token that follows), entropies and `top` most likely tokens of
+        each position, see ops.token_logprobs; the final soft-cap is the configuration's.  No gradient buffer is touched."""
+        self._check_batch(ids, ids if targets is None else targets)
+        T = self.batch_size * self.sequence_length
+        r = ops._outputs(T, None if targets is None else targets.view(T), top, self.loss)
+        ws, hw = self.workspace(), self._head_workspace("olmax_lmhead_logprobs_workspace_bytes", top)
+        check(self._L.olmax_model_logprobs(
+            stream_ptr(), ctypes.byref(self.c), self._windows, self._cos, self._sin, ptr(self.params_bf16), ptr(ids), ptr(targets), ptr(r.logprobs), ptr(r.entropy),
+            ptr(r.stats), ptr(r.top_ids), ptr(r.top_logprobs), ptr(ws), i64(ws.numel()), ptr(hw), i64(hw.numel()), i32(top), i32(ignore_index), f32(temperature)))
+        return r
+
+    def logprobs_grads(self, ids: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, dlogprobs: torch.Tensor, *, dentropy: Optional[torch.Tensor] = None,
+                       temperature: float = 1.0, ignore_index: int = -100) -> None:
+        """Gradients of sum(dlogprobs * logprobs) + sum(dentropy * entropy) to the gradient buffers, as loss_and_grads leaves them: a policy-gradient step is
+        token_logprobs, cotangents of its loss, this, and adamw_step."""
+        self._check_batch(ids, targets)
+        T = self.batch_size * self.sequence_length
+        ops._want(stats.is_cuda and stats.dtype == torch.float32 and stats.shape == (T, 3) and stats.is_contiguous(), f"stats: expected a contiguous fp32 GPU tensor [{T}, 3]")
+        for what, t in (("dlogprobs", dlogprobs), ("dentropy", dentropy)):
+            ops._need_gpu(t)
+            ops._row_of(t, T, what)
+        ws, hw = self.workspace(), self._head_workspace("olmax_lmhead_logprobs_bwd_workspace_bytes")
+        check(self._L.olmax_model_logprobs_grads(
+            stream_ptr(), ctypes.byref(self.c), self._windows, self._cos, self._sin, ptr(self.params_bf16), ptr(ids), ptr(targets), ptr(stats), ptr(dlogprobs), ptr(dentropy),
+            ptr(self.grad_bf16), ptr(self.grad_f32), ptr(ws), i64(ws.numel()), ptr(hw), i64(hw.numel()), i32(ignore_index), f32(temperature)))
+
+    def distill_loss_and_grads(self, ids: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor, *, tail: str = "renormalize", temperature: float = 1.0,
+                               dloss: float = 1.0) -> torch.Tensor:
+        """loss_and_grads with distillation from a teacher's token_logprobs(top=k) in the place of the cross entropy (ops.distill, reduction "mean")."""
+        self._check_batch(ids, ids)
+        T = self.batch_size * self.sequence_length
+        ops._need_gpu(top_ids, top_logprobs)
+        k = ops._teacher(top_ids, top_logprobs, T)
+        ws, hw = self.workspace(), self._head_workspace("olmax_lmhead_distill_workspace_bytes", k)
+        check(self._L.olmax_model_distill_loss_and_grads(
+            stream_ptr(), ctypes.byref(self.c), self._windows, self._cos, self._sin, ptr(self.params_bf16), ptr(ids), ptr(top_ids), ptr(top_logprobs), ptr(self.loss),
+            ptr(self.grad_bf16), ptr(self.grad_f32), ptr(ws), i64(ws.numel()), ptr(hw), i64(hw.numel()), i32(k), i32(ops._tail(tail)), f32(temperature), f32(dloss)))
+        return self.loss
+
     def train_step(self, ids: torch.Tensor, labels: torch.Tensor, *, step: int, lr: float, b1: float = 0.9,
                    b2: float = 0.999, eps: float = 1e-8, weight_decay: float = 1e-4,
                    no_decay_modules: Optional[Sequence[str]] = None, max_grad_norm: Optional[float] = None,
