@@ -488,7 +488,7 @@ extern "C" int64_t olmax_distill_workspace_bytes(int64_t T, int32_t V, int32_t k
 }
 
 static int distill_check(const char* name, int64_t T, int32_t V, int32_t k, int32_t tail, float temperature, float softcap) {
-  OLMAX_CHECK(T > 0 && V > 0 && T < (1LL << 24), OLMAX_ERR_SHAPE, "%s: bad shape T=%ld V=%d", name, (long)T, V);
+  OLMAX_CHECK(T > 0 && V > 0 && V < (1 << 30) && T < (1LL << 24), OLMAX_ERR_SHAPE, "%s: bad shape T=%ld V=%d", name, (long)T, V);
   OLMAX_CHECK(k >= 1 && k <= MAX_TOP, OLMAX_ERR_ARG, "%s: 1 to %d tokens of the teacher a row (got %d)", name, MAX_TOP, k);
   OLMAX_CHECK(tail == 0 || (tail == 1 && V <= MAX_BITS - 32), OLMAX_ERR_ARG, "%s: tail must be 0 (renormalize) or 1 (bucket, up to %d logits)", name, MAX_BITS - 32);
   OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "%s: temperature within 1e-6 and 1e6, softcap not negative", name);

@@ -35,13 +35,15 @@ template <int TH> struct Lds {
 };
 
 // A lower bound of the k-th largest value that the workgroup has seen, from the largest of each group of threads: at least k values are not below the k-th
-// largest of those.  Found on the upper 16 bits of the keys, by bits: each wave counts all groups, four a lane.
+// largest of those.  Found on the upper 16 bits of the keys, by bits: each wave counts all groups, four a lane.  *seen = *noted as it is between two barriers, the same
+// for all threads (behind the second one of them may already note more).
 template <int TH>
-__device__ __forceinline__ unsigned kth_best(unsigned* best, unsigned own, int k) {
+__device__ __forceinline__ unsigned kth_best(unsigned* best, unsigned own, int k, const int* noted, int* seen) {
   static_assert(TH == GROUPS || TH == 2 * GROUPS || TH == 4 * GROUPS, "up to four threads to a group");
   if (TH > GROUPS) own = max(own, (unsigned)__shfl_xor((int)own, 1, 64));
   if (TH > 2 * GROUPS) own = max(own, (unsigned)__shfl_xor((int)own, 2, 64));
   __syncthreads();
+  if (noted) *seen = *noted;
   if ((threadIdx.x & (TH / GROUPS - 1)) == 0) best[threadIdx.x / (TH / GROUPS)] = own;
   __syncthreads();
   const u32x4 q = *reinterpret_cast<const u32x4*>(best + (threadIdx.x & 63) * 4);
@@ -299,9 +301,10 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
     }
     if (TOP) {
       if ((ch & (ch + 1)) == 0) {  // 1, 2, 4, .. chunks seen: about k candidates between two bounds, and those below the new one go where many ties came with them
-        bound = kth_best<TH>(l.best, key_of(most), k);
+        int noted;
+        bound = kth_best<TH>(l.best, key_of(most), k, &l.n, &noted);
         bound_value = value_of(bound);
-        if (l.n > CAND / 2 && l.n <= CAND) narrow<CAND, TH>(l.cand, l.n, bound, &l.n);  // (all read l.n between two barriers)
+        if (noted > CAND / 2 && noted <= CAND) narrow<CAND, TH>(l.cand, noted, bound, &l.n);
       }
       // vectors with a candidate are noted, with their largest; which of their elements are is seen at the end, against the last bound.  (Element by element here: 1600 x 128256
       // with 20 alternatives 120 us, so 96.)
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
   const Stat all = block_join<TH / 64>(a, l.red);
   int n = 0;
   if (TOP) {
-    if (((chunks - 1) & chunks) != 0) bound = kth_best<TH>(l.best, key_of(most), k);  // of all that was seen
+    if (((chunks - 1) & chunks) != 0) bound = kth_best<TH>(l.best, key_of(most), k, nullptr, nullptr);  // of all that was seen
     __syncthreads();
     n = l.n;
     __syncthreads();
@@ -416,7 +419,7 @@ __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ lo
   const bool has_target = target >= 0 && target < V;
   if (threadIdx.x == 0) write_row<CAP>(out, row, has_target, has_target ? (float)logits[row * ld + target] : 0.f, c, a);
   if (TOP) {
-    const unsigned bound = kth_best<TH>(best, max((unsigned)(most >> 32), KEY_NEG_INF), k);
+    const unsigned bound = kth_best<TH>(best, max((unsigned)(most >> 32), KEY_NEG_INF), k, nullptr, nullptr);
     const int n = narrow<JOINED, TH>(cand, parts * k, bound, &counter);
     write_top<CAP, TH>(out, row, k, cand, n, c, a);
   }
@@ -532,7 +535,7 @@ extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, 
                                         int32_t* top_ids, float* top_logprobs, void* workspace, int64_t workspace_bytes, int64_t T, int32_t V,
                                         int64_t ld, int32_t top, int32_t logits_f32, int32_t ignore_index, float temperature, float softcap) {
   OLMAX_CHECK(logits && entropy && stats && (!logprobs || targets), OLMAX_ERR_ARG, "olmax_token_logprobs: null pointer");
-  OLMAX_CHECK(T > 0 && V > 0 && ld >= V && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_token_logprobs: bad shape T=%ld V=%d ld=%ld", (long)T, V, (long)ld);
+  OLMAX_CHECK(T > 0 && V > 0 && V < (1 << 30) && ld >= V && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_token_logprobs: bad shape T=%ld V=%d ld=%ld", (long)T, V, (long)ld);
   OLMAX_CHECK(top >= 0 && top <= MAX_TOP && top <= V && (top == 0 || (top_ids && top_logprobs)), OLMAX_ERR_ARG,
               "olmax_token_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, top);
   OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_token_logprobs: temperature within 1e-6 and 1e6, softcap not negative");
@@ -590,7 +593,7 @@ extern "C" int32_t olmax_token_logprobs_bwd(hipStream_t stream, const void* logi
                                             const float* dentropy, void* dlogits, int64_t T, int32_t V, int64_t ld, int64_t ldd, int32_t logits_f32,
                                             int32_t ignore_index, float temperature, float softcap) {
   OLMAX_CHECK(logits && targets && stats && dlogprobs && dlogits, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: null pointer");
-  OLMAX_CHECK(T > 0 && V > 0 && ld >= V && ldd >= V && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_token_logprobs_bwd: bad shape T=%ld V=%d", (long)T, V);
+  OLMAX_CHECK(T > 0 && V > 0 && V < (1 << 30) && ld >= V && ldd >= V && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_token_logprobs_bwd: bad shape T=%ld V=%d", (long)T, V);
   OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
   OLMAX_CHECK((((uintptr_t)logits | (uintptr_t)dlogits) & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_token_logprobs_bwd: operands not aligned to their type");
   OLMAX_CHECK(logits != dlogits || ld == ldd, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: in place wants one row stride");
@@ -630,7 +633,7 @@ extern "C" int64_t olmax_lmhead_logprobs_workspace_bytes(int64_t T, int32_t d, i
 
 int olmax_lmhead_logprobs_check(const HeadScore& a) {
   OLMAX_CHECK(a.h && a.W && a.workspace && a.entropy && a.stats && (!a.logprobs || a.targets), OLMAX_ERR_ARG, "olmax_lmhead_logprobs: null pointer");
-  OLMAX_CHECK(a.T > 0 && a.d > 0 && a.V > 0 && a.T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs: bad shape T=%ld d=%d V=%d", (long)a.T, a.d, a.V);
+  OLMAX_CHECK(a.T > 0 && a.d > 0 && a.V > 0 && a.V < (1 << 30) && a.T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs: bad shape T=%ld d=%d V=%d", (long)a.T, a.d, a.V);
   OLMAX_CHECK(a.top >= 0 && a.top <= MAX_TOP && a.top <= a.V && (a.top == 0 || (a.top_ids && a.top_logprobs)), OLMAX_ERR_ARG,
               "olmax_lmhead_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, a.top);
   OLMAX_CHECK(a.temperature >= 1e-6f && a.temperature <= 1e6f && a.softcap >= 0.f && a.softcap <= 1e30f, OLMAX_ERR_ARG,
@@ -705,7 +708,7 @@ extern "C" int64_t olmax_lmhead_logprobs_bwd_workspace_bytes(int64_t T, int32_t 
 
 int olmax_lmhead_logprobs_bwd_check(const HeadScoreGrad& a) {
   OLMAX_CHECK(a.h && a.W && a.targets && a.stats && a.dlogprobs && a.workspace && (a.dh || a.dW), OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: null pointer");
-  OLMAX_CHECK(a.T > 0 && a.d > 0 && a.V > 0 && a.T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs_bwd: bad shape T=%ld d=%d V=%d", (long)a.T, a.d, a.V);
+  OLMAX_CHECK(a.T > 0 && a.d > 0 && a.V > 0 && a.V < (1 << 30) && a.T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs_bwd: bad shape T=%ld d=%d V=%d", (long)a.T, a.d, a.V);
   OLMAX_CHECK(a.temperature >= 1e-6f && a.temperature <= 1e6f && a.softcap >= 0.f && a.softcap <= 1e30f, OLMAX_ERR_ARG,
               "olmax_lmhead_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
   OLMAX_CHECK(aligned16(a.h) && aligned16(a.W) && aligned16(a.dh), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs_bwd: h, W and dh must be 16-byte aligned");

@@ -105,7 +105,7 @@ CALLS = {
 ARG, SHAPE, ALIGN, WORKSPACE = -1, -2, -3, -5
 REFUSED = [(name, change, code) for name, given in CALLS.items() for change, code in (
     *(({n: None}, ARG) for n in ("logits", "h", "W", "targets", "entropy", "stats", "dlogprobs", "dlogits_out", "top_ids", "top_logprobs", "loss") if n in given),
-    ({"T": 0}, SHAPE), ({"V": 0}, SHAPE), ({"T": 1 << 24}, SHAPE), ({"d": 0}, SHAPE), ({"ld": 99}, SHAPE), ({"ldd": 99}, SHAPE),
+    ({"T": 0}, SHAPE), ({"V": 0}, SHAPE), ({"T": 1 << 24}, SHAPE), ({"V": 1 << 30, "ld": 1 << 30, "ldd": 1 << 30}, SHAPE), ({"V": 1 << 30, "d": 64}, SHAPE), ({"d": 0}, SHAPE), ({"ld": 99}, SHAPE), ({"ldd": 99}, SHAPE),
     ({"temperature": 0.0}, ARG), ({"temperature": -1.0}, ARG), ({"temperature": math.nan}, ARG), ({"temperature": math.inf}, ARG), ({"softcap": -1.0}, ARG),
     ({"softcap": math.nan}, ARG), ({"top": -1}, ARG), ({"top": 129}, ARG), ({"top": 101}, ARG), ({"k": 0}, ARG), ({"k": 129}, ARG), ({"tail": 2}, ARG),
     ({"tail": 1, "V": 1 << 20, "ld": 1 << 20, "ldd": 1 << 20}, ARG), ({"reduction": 3}, ARG), ({"dloss_rows": P}, ARG), ({"logits": P + 1}, ALIGN),
@@ -178,3 +178,11 @@ def test_argument_checks():
     for a, b in ((z.float(), w), (z, w.float()), (z[:, ::2], w[:, :8].contiguous()), (z, w[:, :8].contiguous()), (z[0], w)):
         with pytest.raises(bad):
             ops._head(a, b)
+
+
+def test_rows_that_are_held_stay_in_registers(tmp_path):
+    """Nor do the products with a row's softmax in their epilogue spill, or the scores."""
+    import test_spills
+    got = {n: v for n, v in test_spills.kernels(tmp_path).items() if any(k in n for k in ("distill_", "score_", "gemm_head_kernel"))}
+    assert len(got) >= 40
+    assert not any(got.values()), {n: v for n, v in got.items() if v}
