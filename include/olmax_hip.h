@@ -200,7 +200,9 @@ int32_t olmax_cross_entropy_reduce(olmax_stream_t stream, const void* logits, vo
  * from logits.  No counterpart in the reference (its cross_entropy_loss, src/olmax/nn/functional.py:70-91, returns -logprob of the labels).
  * z = cap(x) / temperature, cap(x) = softcap * tanh(x / softcap) where softcap > 0; p = softmax(z) over the V logits of a row.
  * logprobs [T] (optional; needs targets) = ln p[target], 0 for a target outside [0, V); entropy [T] = - sum p ln p;
- * stats [T, 3] = {m = max z, ln sum exp(z - m), entropy}, what the backward call takes (its first two add up to the log-normaliser);
+ * stats [T, 3] = {m = max z, ln sum exp(z - m), entropy}, what the backward call takes (its first two add up to the log-normaliser; m is
+ * rounded, so that gradients of scores beyond 2^20 at a temperature that is no power of two are off by 2^-24 |m|, and a row whose scores
+ * have no room in fp32, which the other results take in their stride, has none);
  * top_ids / top_logprobs [T, top] (top 0 to 128, at most V): the largest logits x in order, ties to the lowest index.  A row whose target
  * is ignore_index is not read: zeros, ids of -1, log probabilities of minus infinity.  Logits of minus infinity are tokens of no
  * probability; a row of nothing else has entropy 0 and log probabilities of minus infinity.  A NaN or an infinite score makes a row's values NaN

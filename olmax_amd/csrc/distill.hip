@@ -152,11 +152,11 @@ __device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, c
   return f;
 }
 template <bool CAP> __device__ __forceinline__ float outside(float x, const Scale& c, const Factors& f) {
-  return exp_of(behind<CAP>(x, c, f.m)) * f.out * slope<CAP>(x, c);
+  return exp_behind<CAP>(x, c, f.m) * f.out * slope<CAP>(x, c);
 }
 
 template <bool CAP> __device__ __forceinline__ float inside(float x, float q, const Scale& c, const Factors& f) {
-  return (exp_of(behind<CAP>(x, c, f.m)) * f.in - q * f.scale) * slope<CAP>(x, c);
+  return (exp_behind<CAP>(x, c, f.m) * f.in - q * f.scale) * slope<CAP>(x, c);
 }
 
 struct RowArgs {
@@ -231,8 +231,8 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
   if (part == 0 && tid < cutting.edges) {
     const float x = (float)zr[cutting.edge(tid, V)];
     const int at = per * N + tid;
-    if (CAP || x > -INFINITY) a.m = score<CAP>(x, c);
-    a.s = BUCKET && (bits[at >> 5] >> (at & 31) & 1) ? 0.f : exp_of(behind<CAP>(x, c, a.ref()));
+    if (CAP || x > -INFINITY) a.m = level<CAP>(x, c);
+    a.s = BUCKET && (bits[at >> 5] >> (at & 31) & 1) ? 0.f : exp_behind<CAP>(x, c, a.ref());
   }
   for (int at = v0; at < v1; at += SPAN) {
     Raw<T, N> now[UNROLL];
@@ -248,8 +248,8 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
 #pragma unroll
       for (int e = 0; e < N; e++) most = fmaxf(most, x[e]);
     }
-    const float top = score<CAP>(most, c);
-    if (at + tid < v1 && top > a.m) a.raise(top);
+    const float top = level<CAP>(most, c);
+    if (at + tid < v1 && top > a.m) a.raise(top, c.unit);
     const float ref = a.ref();
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
       float x[N];
       now[u].unpack(x);
 #pragma unroll
-      for (int e = 0; e < N; e++) x[e] = exp_of(behind<CAP>(x[e], c, ref));
+      for (int e = 0; e < N; e++) x[e] = exp_behind<CAP>(x[e], c, ref);
       if (BUCKET) {
         const int b = v - v0;
         const unsigned in = N == 8 ? (unsigned)byte_of[b] : (byte_of[b >> 1] >> (b & 1) * 4) & 15u;
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
       a.s += x[0];
     }
   }
-  a = block_join<TH / 64>(a, l.red);
+  a = block_join<TH / 64>(a, l.red, c.unit);
   if (part_stat && tid == 0) part_stat[blockIdx.x] = a;
   if (!part_stat) factors_of<CAP, BUCKET, TH / 64>(a, l, c, 0.f, p.row_loss + row);
 }
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256) void distill_grads_kernel(const T* __restrict_
   if (tid < 64) {
     Stat a = Stat::none();
     if (tid < parts) a = part_stat[row * parts + tid];
-    a = block_join<1>(a, nullptr);
+    a = block_join<1>(a, nullptr, c.unit);
     if (tid == 0) l.red[0] = a;
     teacher_of<T, BUCKET, NW>(p.teacher, row, zr, V, c.inv_tau, nullptr, 0, l);
   }
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict
     float x[N];
     w.unpack(x);
 #pragma unroll
-    for (int e = 0; e < N; e++) x[e] = exp_of(behind<CAP>(x[e], c, ref));
+    for (int e = 0; e < N; e++) x[e] = exp_behind<CAP>(x[e], c, ref);
     if (BUCKET) {  // which elements of the vector are the teacher's
       const int at = tid + (cutting.head ? 1 : 0);
       const unsigned in = N == 8 ? (unsigned)byte_of[at + first] : (byte_of[(at >> 1) + (first >> 1)] >> (at & 1) * 4) & 15u;
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict
     return (float)zr[*at];
   };
   auto edge_sum = [&](float x, int at, float ref) {
-    return BUCKET && (bits[(at + shift) >> 5] >> ((at + shift) & 31) & 1) ? 0.f : exp_of(behind<CAP>(x, c, ref));
+    return BUCKET && (bits[(at + shift) >> 5] >> ((at + shift) & 31) & 1) ? 0.f : exp_behind<CAP>(x, c, ref);
   };
   const bool has_edge = tid < cutting.edges;
   int edge;
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict
   }
   most = uniform(block_reduce<NW, true>(most, l.sums));
   Stat a = Stat::none();
-  if (CAP || most > -INFINITY) a.m = score<CAP>(most, c);
+  if (CAP || most > -INFINITY) a.m = level<CAP>(most, c);
   const float ref = a.ref();
   float sum = 0.f;
   if (has_edge) {

@@ -701,16 +701,17 @@ __device__ __forceinline__ void gemm_tile(
       most = fmaxf(most, __shfl_xor(most, 16, 64));
       most = half_swap_max(most);
       rows::Stat a = rows::Stat::none();
-      if (CAP || most > -INFINITY) a.m = rows::score<CAP>(most, c);
+      if (CAP || most > -INFINITY) a.m = rows::level<CAP>(most, c);
       const float ref = a.ref();
 #pragma unroll
       for (int j = 0; j < TN; j++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const float d = rows::behind<CAP>(x[j][r], c, ref), e = here(j, r) ? rows::exp_of(d) : 0.f;
+          const float d = CAP ? rows::behind<CAP>(x[j][r], c, ref) * rows::LOG2E : (x[j][r] - ref) * c.unit2, e = here(j, r) ? __builtin_amdgcn_exp2f(d) : 0.f;
           a.s += e;
           a.t += e * fmaxf(d, -200.f);
         }
+      a.t *= rows::LN2;
       a.s += __shfl_xor(a.s, 16, 64);
       a.t += __shfl_xor(a.t, 16, 64);
       a.s = half_swap_sum(a.s);
@@ -736,7 +737,7 @@ __device__ __forceinline__ void gemm_tile(
     if (tid < BM && stores_row(tid)) {
       rows::Stat a = strip[tid];
 #pragma unroll
-      for (int w = 1; w < WAVES_N; w++) a.join(strip[w * BM + tid]);
+      for (int w = 1; w < WAVES_N; w++) a.join(strip[w * BM + tid], c.unit);
       reinterpret_cast<rows::Stat*>(head->parts)[(int64_t)tile_n * M + m0 + tid] = a;
     }
     return;

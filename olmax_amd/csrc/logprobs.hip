@@ -177,8 +177,10 @@ __device__ __forceinline__ void write_row(const Out& o, int64_t row, bool has_ta
   const float log_sum = log_of(a.s), entropy = none ? 0.f : log_sum - a.t / a.s;
   if (o.logprobs) o.logprobs[row] = !has_target ? 0.f : none ? -INFINITY : behind<CAP>(x, c, a.m) - log_sum;
   o.entropy[row] = entropy;
-  o.stats[row * 3] = a.m;
-  o.stats[row * 3 + 1] = none ? 0.f : log_sum;
+  // the level as a score, and what its rounding leaves in the logarithm
+  const float m = CAP ? a.m : a.m * c.inv_tau, left = CAP || __builtin_isinf(m) ? 0.f : __builtin_fmaf(a.m, c.inv_tau, -m);
+  o.stats[row * 3] = m;
+  o.stats[row * 3 + 1] = none ? 0.f : log_sum + left;
   o.stats[row * 3 + 2] = entropy;
 }
 // The n <= k largest logits above minus infinity are cand[0 .. n) or are the largest of them; the rest of k slots gets the lowest indices that are not among them.
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
   const float edge_x = has_edge ? (float)zr[edge] : -INFINITY;
   if (has_edge) {
     if (edge_x > -INFINITY) most = edge_x;
-    if (CAP || edge_x > -INFINITY) a.m = score<CAP>(edge_x, c);
+    if (CAP || edge_x > -INFINITY) a.m = level<CAP>(edge_x, c);
     const float d = behind<CAP>(edge_x, c, a.ref()), e = exp_of(d);
     a.s = e;
     a.t = e * fmaxf(d, -200.f);
@@ -274,7 +276,7 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
     }
     if (cm > most || (CAP && a.m == -INFINITY)) {  // (a soft-cap makes a score of minus infinity too)
       most = fmaxf(most, cm);
-      a.raise(score<CAP>(most, c));
+      a.raise(level<CAP>(most, c), c.unit);
     }
     const float ref = a.ref();
     const float cap_r = c.r_k * LOG2E, cap_top = (c.top - ref) * LOG2E;
@@ -290,8 +292,8 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
           x[e] = __builtin_amdgcn_exp2f(d);
           t[e] = x[e] * d;
         } else {
-          const float d = behind<CAP>(x[e], c, ref);
-          x[e] = exp_of(d);
+          const float d = (x[e] - ref) * c.unit2;
+          x[e] = __builtin_amdgcn_exp2f(d);
           t[e] = x[e] * fmaxf(d, -200.f);
         }
       }
@@ -300,7 +302,7 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
 #pragma unroll
         for (int e = 0; e < w; e++) x[e] += x[e + w], t[e] += t[e + w];
       a.s += x[0];
-      a.t += CAP ? t[0] * LN2 : t[0];
+      a.t += t[0] * LN2;
     }
     if (TOP) {
       if ((ch & (ch + 1)) == 0) {  // 1, 2, 4, .. chunks seen: about k candidates between two bounds, and those below the new one go where many ties came with them
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
       }
     }
   }
-  const Stat all = block_join<TH / 64>(a, l.red);
+  const Stat all = block_join<TH / 64>(a, l.red, c.unit);
   int n = 0;
   if (TOP) {
     if (((chunks - 1) & chunks) != 0) bound = kth_best<TH>(l.best, key_of(most), k, nullptr, nullptr);  // of all that was seen
@@ -418,7 +420,7 @@ __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ lo
       cand[i] = e;
       most = max(most, e);
     }
-  a = block_join<TH / 64>(a, red);
+  a = block_join<TH / 64>(a, red, c.unit);
   const bool has_target = target >= 0 && target < V;
   if (threadIdx.x == 0) write_row<CAP>(out, row, has_target, has_target ? (float)logits[row * ld + target] : 0.f, c, a);
   if (TOP) {
@@ -440,14 +442,14 @@ __global__ __launch_bounds__(1024) void head_join_kernel(const Stat* __restrict_
   const int64_t row = blockIdx.x * 16ll + (threadIdx.x & 15);
   Stat a = Stat::none();
   if (row < rows)
-    for (int i = threadIdx.x >> 4; i < n_tiles; i += 64) a.join(tiles[(int64_t)i * ld_tiles + row]);
+    for (int i = threadIdx.x >> 4; i < n_tiles; i += 64) a.join(tiles[(int64_t)i * ld_tiles + row], c.unit);
 #pragma unroll
   for (int o = 16; o < 64; o <<= 1) {
     Stat b;
     b.m = __shfl_xor(a.m, o, 64);
     b.s = __shfl_xor(a.s, o, 64);
     b.t = __shfl_xor(a.t, o, 64);
-    a.join(b);
+    a.join(b, c.unit);
   }
   if ((threadIdx.x & 63) < 16) part[wave][threadIdx.x & 15] = a;
   __syncthreads();
@@ -459,8 +461,8 @@ __global__ __launch_bounds__(1024) void head_join_kernel(const Stat* __restrict_
     for (int i = 0; i < 3; i++) out.stats[row * 3 + i] = 0.f;
     return;
   }
-  for (int w = 1; w < 16; w++) a.join(part[w][threadIdx.x]);
-  if (fused < V) a.join(rest_stat[row]);
+  for (int w = 1; w < 16; w++) a.join(part[w][threadIdx.x], c.unit);
+  if (fused < V) a.join(rest_stat[row], c.unit);
   const bool has_target = target >= 0 && target < V;
   write_row<CAP>(out, row, has_target, !has_target ? 0.f : target < fused ? target_logit[row] : rest[row * ld_rest + target - fused], c, a);
 }

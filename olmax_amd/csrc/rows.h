@@ -2,10 +2,10 @@
 // softmax statistics, 16-byte access to rows of any alignment.
 //
 // Scores z = cap(x) / temperature, cap(x) = softcap * tanh(x / softcap) or x.  A thread's statistics are of what it has seen:
-//   m   largest score (the reference that exponentials are taken against), s = sum exp(z - m), t = sum exp(z - m) (z - m)
-// so that ln sum exp z = m + ln s, and the entropy of softmax(z) is ln s - t / s.  Everything is fp32.  z - m is formed by one fma from the
-// logit, so that rows at the type's lowest value or about 1e30 are exact where scores near the largest are; a score of minus infinity has
-// exp = 0 and adds nothing to t (z - m is cut at -200, where exp is 0 in fp32).
+//   m   largest level (what exponentials are taken against: a logit, or with a soft-cap its score), s = sum exp(z - m), t = sum exp(z - m) (z - m)
+// so that ln sum exp z = m + ln s, and the entropy of softmax(z) is ln s - t / s.  Everything is fp32.  z - m is formed from the difference of the
+// logits, so that rows at the type's lowest value or about 1e30 are exact where scores near the largest are, at any temperature; a score of minus
+// infinity has exp = 0 and adds nothing to t (z - m is cut at -200, where exp is 0 in fp32).
 #pragma once
 #include "common.h"
 
@@ -78,7 +78,8 @@ template <typename T, int N> __device__ __forceinline__ Cut cut(const T* row, in
 // tanh(x / softcap) = 1 - 2 r, r = 1 / (exp(2 x / softcap) + 1), so that a capped score is one fma on r, and its slope dy / dx is 4 r (1 - r)
 struct Scale {
   float cap, cap_k, inv_tau;  // cap_k = 2 log2(e) / cap; cap 0: none
-  float r_k, top;             // a score is r_k r + top: r_k = -2 cap / temperature, top = cap / temperature
+  float r_k, top;             // a capped score is r_k r + top: r_k = -2 cap / temperature, top = cap / temperature
+  float unit, unit2;          // of a level (see level), in scores: 1, or 1 / temperature; and in powers of two
 };
 inline Scale scale_of(float temperature, float softcap) {
   Scale c;
@@ -87,17 +88,21 @@ inline Scale scale_of(float temperature, float softcap) {
   c.inv_tau = 1.f / temperature;
   c.top = softcap * c.inv_tau;
   c.r_k = -2.f * c.top;
+  c.unit = softcap > 0.f ? 1.f : c.inv_tau;
+  c.unit2 = c.unit * LOG2E;
   return c;
 }
 __device__ __forceinline__ float tail_of_tanh(float x, const Scale& c) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f); }
-template <bool CAP> __device__ __forceinline__ float score(float x, const Scale& c) {
-  return CAP ? __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top) : x * c.inv_tau;
-}
+// What rows are compared by, and exponentials are taken against: capped scores, or the logits themselves, whose scores may have no room in fp32 (the type's lowest value at a
+// temperature below 1) where their differences have.
+template <bool CAP> __device__ __forceinline__ float level(float x, const Scale& c) { return CAP ? __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top) : x; }
 // a value that all threads of the workgroup have, in a scalar register
 __device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
-// z - m
+// z - m, m the score of level m
 template <bool CAP> __device__ __forceinline__ float behind(float x, const Scale& c, float m) {
-  return CAP ? __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top - m) : __builtin_fmaf(x, c.inv_tau, -m);
+  if (CAP) return __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top - m);
+  const float d = (x - m) * c.unit;
+  return d == -INFINITY && x > -INFINITY ? __builtin_fmaf(x, c.unit, -m * c.unit) : d;  // (at a temperature above 1 the scores may have the room that the logits have not)
 }
 // dz / dx
 template <bool CAP> __device__ __forceinline__ float slope(float x, const Scale& c) {
@@ -106,26 +111,30 @@ template <bool CAP> __device__ __forceinline__ float slope(float x, const Scale&
   return 4.f * r * (1.f - r) * c.inv_tau;
 }
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
+// exp(z - m)
+template <bool CAP> __device__ __forceinline__ float exp_behind(float x, const Scale& c, float m) {
+  return CAP ? exp_of(behind<CAP>(x, c, m)) : __builtin_amdgcn_exp2f((x - m) * c.unit2);
+}
 __device__ __forceinline__ float log_of(float s) { return __builtin_amdgcn_logf(s) * LN2; }
 
-// Statistics of what a thread has seen; m = -inf: nothing above minus infinity yet.
+// Statistics of what a thread has seen: the largest level, the sum of exponentials behind it, that sum weighted by z - m; m = -inf: nothing above minus infinity yet.
 struct Stat {
   float m, s, t;
   static __device__ __forceinline__ Stat none() { return Stat{-INFINITY, 0.f, 0.f}; }
   __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }  // against which every exponential of such a thread is 0
-  // the largest score is m2 now
-  __device__ __forceinline__ void raise(float m2) {
+  // the largest level is m2 now
+  __device__ __forceinline__ void raise(float m2, float unit) {
     if (m != -INFINITY) {
-      const float d = m - m2, f = exp_of(d);
+      const float d = (m - m2) * unit, f = exp_of(d);
       t = f * (t + s * fmaxf(d, -200.f));
       s *= f;
     }
     m = m2;
   }
-  __device__ __forceinline__ void join(const Stat& o) {
+  __device__ __forceinline__ void join(const Stat& o, float unit) {
     Stat b = o;
-    if (b.m > m) raise(b.m);
-    else if (m > b.m) b.raise(m);
+    if (b.m > m) raise(b.m, unit);
+    else if (m > b.m) b.raise(m, unit);
     s += b.s;
     t += b.t;
   }
@@ -142,14 +151,14 @@ template <int NW, bool MAX> __device__ __forceinline__ float block_reduce(float 
   for (int o = NW / 2; o > 0; o >>= 1) v = both(v, __shfl_xor(v, o, 64));
   return v;
 }
-template <int NW> __device__ __forceinline__ Stat block_join(Stat a, Stat* red) {
+template <int NW> __device__ __forceinline__ Stat block_join(Stat a, Stat* red, float unit) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     Stat b;
     b.m = __shfl_xor(a.m, o, 64);
     b.s = __shfl_xor(a.s, o, 64);
     b.t = __shfl_xor(a.t, o, 64);
-    a.join(b);
+    a.join(b, unit);
   }
   if (NW == 1) return a;
   __syncthreads();
@@ -157,14 +166,15 @@ template <int NW> __device__ __forceinline__ Stat block_join(Stat a, Stat* red) 
   __syncthreads();
   a = red[0];
 #pragma unroll
-  for (int i = 1; i < NW; i++) a.join(red[i]);
+  for (int i = 1; i < NW; i++) a.join(red[i], unit);
   return a;
 }
 
-// d / d x of g ln p[target] + h entropy: (g (i == target) - p (g + h (ln p + H))) dz/dx, from the row's m, ln S and H
+// d / d x of g ln p[target] + h entropy: (g (i == target) - p (g + h (ln p + H))) dz/dx, from the row's m (a score, as
+// stats hold it), ln S and H
 template <bool CAP, bool ENT>
 __device__ __forceinline__ float score_grad(float x, const Scale& c, float m, float log_sum, float entropy, float g, float h, bool target) {
-  const float logp = behind<CAP>(x, c, m) - log_sum;
+  const float logp = (CAP ? behind<CAP>(x, c, m) : __builtin_fmaf(x, c.inv_tau, -m)) - log_sum;
   float d = -exp_of(logp) * (ENT ? __builtin_fmaf(h, fmaxf(logp, -200.f) + entropy, g) : g);
   if (target) d += g;
   return d * slope<CAP>(x, c);
@@ -178,7 +188,7 @@ struct HeadRows {
   int32_t ignore_index, V;    // V: of the whole product; a target from there on has no logit
   int32_t rows;               // that there are: up to M, those behind pad the product (their gradients are zeros)
   rows::Scale scale;
-  float *parts, *target_logit;  // statistics: [ceil(N / 256)][M][3], (largest score, sum of exponentials behind it, that sum weighted by z - m) of 256 columns; the
+  float *parts, *target_logit;  // statistics: [ceil(N / 256)][M][3], (Stat) of 256 columns; the
                                 // logit x of each target that is one of the columns
   const float *stats, *dlogprobs, *dentropy;  // gradients: from [M, 3], [M], [M] (optional)
 };

@@ -1,7 +1,8 @@
 """GPU parity tests of log probabilities, entropy, alternatives and distillation, on given logits and with the LM head, against the plain forms in 64 bits.
 
-Tolerances count roundings of 2^-24 (u).  A score behind the row's largest, D = z - m, is one fma on fp32 numbers, its exponential two roundings of the argument (2 u |D| in
-the result's relative error) and a hardware exponential (2 u); a thread adds its share of the row one after another, V / (256 * 8 or 4) vectors behind an 8-fold
+Tolerances count roundings of 2^-24 (u).  A score behind the row's largest, D = z - m, is a difference of logits times 1 / temperature (in
+powers of two for an exponential): two roundings, and at most three of the factor, of which 2 u |D| are counted by themselves and 3 u |D| are within the 24 u below (|D| is 8 at
+most where it has weight); a hardware exponential (2 u); a thread adds its share of the row one after another, V / (256 * 8 or 4) vectors behind an 8-fold
 tree, and twelve more additions join the threads: CHAIN = V / 1024 + 24 u relative at most, for sums of positive numbers.
 A soft-cap's tanh is off by 2^-22 at most (an exponential and a reciprocal, each halved by tanh's slope), its score by CAP = softcap * 2^-21 / temperature with its product's
 rounding.  The temperature is the fp32 number that the kernel gets."""
@@ -47,6 +48,7 @@ class Row:
 def near(got, want, bound, what):
     got = got.cpu().double()
     same = (got == want) | (got.isnan() & want.isnan())
+    same |= got.isinf() & (got.sign() == want.sign()) & (want.abs() + bound > torch.finfo(torch.float32).max)  # (fp32 has no such number)
     off = torch.where(same, torch.zeros_like(want), (got - want).abs() - bound)
     assert (off <= 0).all(), (what, got.flatten()[off.argmax()].item(), want.flatten()[off.argmax()].item(), off.max().item())
 
@@ -142,6 +144,36 @@ def special(V, dtype):
     z[13] = torch.linspace(20, -20, V).to(dtype)
     t = torch.tensor([0, 3, V // 2, V // 3, V - 2, V - 1, 2, 4, 1, 1, 0, V - 1, V - 1, 0], dtype=torch.int32)
     return z, t
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("temperature", [0.7, 3.0])
+@pytest.mark.parametrize("V,copies", [(997, 1), (997, 80), (60001, 1), (60001, 40)])
+def test_masks_and_ties_at_a_temperature(dtype, temperature, V, copies):
+    """Scores beyond fp32 (the type's lowest value over 0.7) and far from 0: only differences of logits count."""
+    from olmax_amd import ops
+    print(f"[case] special V{V} x{copies} temperature {temperature}", flush=True)
+    z, t = special(V, dtype)
+    z[12], z[13] = 1e30, -3e38
+    z[13, 5] = torch.finfo(dtype).max / 2
+    t[12], t[13] = 7, 5
+    r = ops.token_logprobs(z.repeat(copies, 1).cuda(), t.repeat(copies).cuda(), top=20, temperature=temperature)
+    for c in range(min(copies, 4)):
+        check_scores(r, z.double(), t, 20, temperature, rows=torch.arange(14) + 14 * c)
+    k = 8
+    ids = torch.stack([(t.long() + 3 * j) % V for j in range(k)], 1).to(torch.int32)  # the first has a probability where one has
+    q = torch.full((14, k), -math.inf)
+    q[:, 0] = -0.25                                                                  # (what a student rules out costs infinitely much)
+    ids, q = ids[1:], q[1:]                                                          # (a row of nothing has no distribution)
+    for tail in ("renormalize", "bucket"):
+        rows = list(range(13)) if tail == "renormalize" else [0, 4, 5, 7, 8, 9, 10, 11]  # (nor do the others of rows of one token)
+        per, bound, grad, gbound = distill_bounds(z[1:][rows], ids[rows], q[rows], tail, temperature, 0.0, torch.ones(len(rows)))
+        n = len(rows)
+        loss, d = ops.distill(z[1:][rows].repeat(copies, 1).cuda(), ids[rows].repeat(copies, 1).cuda(), q[rows].repeat(copies, 1).cuda(), tail=tail, temperature=temperature,
+                              reduction="none")
+        for c in range(min(copies, 4)):
+            near(loss[n * c:n * c + n], per, bound, tail)
+            near(d[n * c:n * c + n], grad, gbound, tail)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
