@@ -565,6 +565,7 @@ extern "C" int32_t olmax_distill(hipStream_t stream, const void* logits, void* d
   OLMAX_CHECK(!dloss_rows || reduction == 2, OLMAX_ERR_ARG, "olmax_distill: a per-row cotangent only goes with reduction none");
   OLMAX_CHECK((((uintptr_t)logits | (uintptr_t)dlogits) & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_distill: operands not aligned to their type");
   OLMAX_CHECK(logits != dlogits || ld == ldd, OLMAX_ERR_ARG, "olmax_distill: in place wants one row stride");
+  OLMAX_CHECK(!overlap(logits, ld, dlogits, ldd, T, V, logits_f32 ? 4 : 2), OLMAX_ERR_ARG, "olmax_distill: the gradient overlaps the logits, but is not in their place");
   OLMAX_CHECK(workspace_bytes >= olmax_distill_workspace_bytes(T, V, k, logits_f32) && aligned16(workspace), OLMAX_ERR_WORKSPACE, "olmax_distill: workspace needs %ld bytes, 16-byte aligned",
               (long)olmax_distill_workspace_bytes(T, V, k, logits_f32));
   return distill(stream, logits, dlogits, top_ids, top_logprobs, loss, dloss_rows, workspace, T, V, k, ld, ldd, logits_f32 != 0, logits_f32 != 0, tail,

@@ -603,6 +603,7 @@ extern "C" int32_t olmax_token_logprobs_bwd(hipStream_t stream, const void* logi
   OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
   OLMAX_CHECK((((uintptr_t)logits | (uintptr_t)dlogits) & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_token_logprobs_bwd: operands not aligned to their type");
   OLMAX_CHECK(logits != dlogits || ld == ldd, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: in place wants one row stride");
+  OLMAX_CHECK(!overlap(logits, ld, dlogits, ldd, T, V, logits_f32 ? 4 : 2), OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: the gradient overlaps the logits, but is not in their place");
   return token_logprobs_bwd(stream, logits, targets, stats, dlogprobs, dentropy, dlogits, T, V, ld, ldd, logits_f32 != 0, logits_f32 != 0, ignore_index,
                             temperature, softcap, 0);
 }
@@ -683,9 +684,16 @@ extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, cons
   rows.parts = (float*)tiles;
   rows.target_logit = target_logit;
   if (int rc = olmax_gemm_head_stats(stream, hp, wp, (int)p.rows, p.fused, d, rows)) return rc;
-#define JOIN(CAPV)                                                                                                                                                        do {                                                                                                                                                                      if (rest)                                                                                                                                                                 hipLaunchKernelGGL((score_rows_kernel<float, CAPV, false, 256>), dim3((unsigned)T), dim3(256), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,                          p.ld, ignore_index, c, 0, 1);                                                                                                                      hipLaunchKernelGGL((head_join_kernel<CAPV>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,                        (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, p.rows, V, p.fused, ignore_index, c);                                                 } while (0)
-  if (softcap > 0.f) JOIN(true); else JOIN(false);
-#undef JOIN
+  auto join = [&](auto capped) {
+    constexpr bool CAP = decltype(capped)::value;
+    if (rest)
+      hipLaunchKernelGGL((score_rows_kernel<float, CAP, false, 256>), dim3((unsigned)T), dim3(256), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,
+                         p.ld, ignore_index, c, 0, 1);
+    hipLaunchKernelGGL((head_join_kernel<CAP>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,
+                       (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, p.rows, V, p.fused, ignore_index, c);
+  };
+  if (softcap > 0.f) join(std::true_type());
+  else join(std::false_type());
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }

@@ -180,6 +180,14 @@ __device__ __forceinline__ float score_grad(float x, const Scale& c, float m, fl
   return d * slope<CAP>(x, c);
 }
 
+// Whether rows of n numbers of `size` bytes at a and b share memory in another way than being the same (a + b in place is each element over itself).
+inline bool overlap(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t rows, int64_t n, int size) {
+  const int64_t d = ((const char*)b - (const char*)a) / size;  // (both are aligned to their type)
+  if (a == b || !b || d >= (rows - 1) * lda + n || -d >= (rows - 1) * ldb + n) return false;
+  const int64_t at = lda == ldb ? ((d % lda) + lda) % lda : 0;
+  return at < n || at + n > lda;
+}
+
 }  // namespace rows
 
 // gemm.hip: the LM head's product with a row's part of its softmax in the epilogue (logprobs.hip): logits leave the kernel only as what is formed of them.

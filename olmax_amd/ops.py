@@ -389,7 +389,7 @@ def _tail(tail: str) -> int:
 def _outputs(T: int, targets, top: int, like):
     """Views of one allocation (each of its own takes 1.6 us, half of a call on few rows)."""
     _row_of(targets, T, "targets", torch.int32)
-    _want(top >= 0, "top must not be negative")
+    _want(0 <= top <= 128, f"top: 0 to 128 alternatives (got {top})")
     sizes = [T, 3 * T] if targets is None else [T, 3 * T, T]
     if top:
         entropy, stats, *lp, best, ids = like.new_empty((sum(sizes) + 2 * T * top,), dtype=torch.float32).split_with_sizes([*sizes, T * top, T * top])

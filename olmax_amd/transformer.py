@@ -396,6 +396,7 @@ class Transformer:
         """The model's log probabilities of targets (flat [batch * sequence], as labels are: the token that follows), entropies and `top` most likely tokens of
         each position, see ops.token_logprobs; the final soft-cap is the configuration's.  No gradient buffer is touched."""
         self._check_batch(ids, ids if targets is None else targets)
+        ops._place(ids, targets, self.loss)
         T = self.batch_size * self.sequence_length
         r = ops._outputs(T, None if targets is None else targets.view(T), top, self.loss)
         ws, hw = self.workspace(), self._head_workspace("olmax_lmhead_logprobs_workspace_bytes", top)
@@ -410,9 +411,9 @@ class Transformer:
         token_logprobs, cotangents of its loss, this, and adamw_step."""
         self._check_batch(ids, targets)
         T = self.batch_size * self.sequence_length
-        ops._want(stats.is_cuda and stats.dtype == torch.float32 and stats.shape == (T, 3) and stats.is_contiguous(), f"stats: expected a contiguous fp32 GPU tensor [{T}, 3]")
+        ops._place(ids, targets, stats, dlogprobs, dentropy, self.loss)
+        ops._want(stats.dtype == torch.float32 and stats.shape == (T, 3) and stats.is_contiguous(), f"stats: expected a contiguous fp32 tensor [{T}, 3]")
         for what, t in (("dlogprobs", dlogprobs), ("dentropy", dentropy)):
-            ops._need_gpu(t)
             ops._row_of(t, T, what)
         ws, hw = self.workspace(), self._head_workspace("olmax_lmhead_logprobs_bwd_workspace_bytes")
         check(self._L.olmax_model_logprobs_grads(
@@ -424,7 +425,7 @@ class Transformer:
         """loss_and_grads with distillation from a teacher's token_logprobs(top=k) in the place of the cross entropy (ops.distill, reduction "mean")."""
         self._check_batch(ids, ids)
         T = self.batch_size * self.sequence_length
-        ops._need_gpu(top_ids, top_logprobs)
+        ops._place(ids, top_ids, top_logprobs, self.loss)
         k = ops._teacher(top_ids, top_logprobs, T)
         ws, hw = self.workspace(), self._head_workspace("olmax_lmhead_distill_workspace_bytes", k)
         check(self._L.olmax_model_distill_loss_and_grads(

@@ -109,7 +109,8 @@ REFUSED = [(name, change, code) for name, given in CALLS.items() for change, cod
     ({"temperature": 0.0}, ARG), ({"temperature": -1.0}, ARG), ({"temperature": math.nan}, ARG), ({"temperature": math.inf}, ARG), ({"softcap": -1.0}, ARG),
     ({"softcap": math.nan}, ARG), ({"top": -1}, ARG), ({"top": 129}, ARG), ({"top": 101}, ARG), ({"k": 0}, ARG), ({"k": 129}, ARG), ({"tail": 2}, ARG),
     ({"tail": 1, "V": 1 << 20, "ld": 1 << 20, "ldd": 1 << 20}, ARG), ({"reduction": 3}, ARG), ({"dloss_rows": P}, ARG), ({"logits": P + 1}, ALIGN),
-    ({"logits": P, "dlogits": P, "ldd": 104}, ARG), ({"workspace_bytes": 8}, WORKSPACE), ({"workspace": P + 4}, WORKSPACE),
+    ({"logits": P, "dlogits": P, "ldd": 104}, ARG), ({"logits": P, "dlogits": P + 2}, ARG), ({"logits": P, "dlogits": P + 206}, ARG),
+    ({"logits": P, "dlogits": P + 200, "ld": 199, "ldd": 199}, ARG), ({"logits": P + 400, "dlogits": P, "ld": 100, "ldd": 104}, ARG), ({"workspace_bytes": 8}, WORKSPACE), ({"workspace": P + 4}, WORKSPACE),
 ) if all(n in given for n in change)]
 
 
@@ -164,8 +165,9 @@ def test_argument_checks():
             ops._row_of(t, 4, "dlogprobs")
     with pytest.raises(bad):
         ops._outputs(4, torch.zeros(4, dtype=torch.int64), 0, z)
-    with pytest.raises(bad):
-        ops._outputs(4, None, -1, z)
+    for top in (-1, 129, 1 << 40):
+        with pytest.raises(bad):
+            ops._outputs(4, None, top, z)
     ids, t = torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4, 3)
     assert ops._teacher(ids, t, 4) == 3
     for a, b in ((ids.long(), t), (ids[:3], t[:3]), (ids, t[:, :2]), (ids, t.double()), (ids[:, ::2], t[:, ::2])):

@@ -123,6 +123,22 @@ def test_rows_anywhere(dtype, V, T):
     assert torch.equal(view, packed) and (wide[:, :5] == 99).all() and (wide[:, 5 + V:] == 99).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_gradients_between_the_logits(dtype):
+    """Rows of logits and of their gradients that take turns in memory share none; gradients that overlap the logits are refused."""
+    from olmax_amd import _lib, ops
+    T, V = 5, 1003
+    z, targets = make(T, V, dtype)
+    both = torch.full((T, 2 * V), 5.0, dtype=dtype, device="cuda")
+    both[:, :V] = z.cuda()
+    r = ops.token_logprobs(both[:, :V], targets.cuda())
+    g = torch.randn(T, device="cuda")
+    ops.token_logprobs_bwd(both[:, :V], targets.cuda(), r.stats, g, out=both[:, V:])
+    assert torch.equal(both[:, V:], ops.token_logprobs_bwd(z.cuda(), targets.cuda(), r.stats, g)) and torch.equal(both[:, :V].cpu(), z)
+    with pytest.raises(_lib.OlmaxHipError, match="overlaps"):
+        ops.token_logprobs_bwd(both[:, :V], targets.cuda(), r.stats, g, out=both[:, 1:V + 1])
+
+
 def special(V, dtype):
     """Rows that masks and ties make; the targets name a token that has a probability where one has."""
     low = torch.finfo(dtype).min
@@ -342,6 +358,55 @@ def test_distill(dtype, V, k, tail, temperature, softcap):
     ops.distill(wide[:, 3:3 + V], ids.cuda(), t.cuda(), dloss=2.0, inplace=True, **kw)
     near(wide[:, 3:3 + V], *distill_bounds(z, ids, t, tail, temperature, softcap, torch.full((5,), 0.5))[2:], "in place, elsewhere")
     assert (wide[:, :3] == 9).all() and (wide[:, 3 + V:] == 9).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("T,V", [(1, 102401), (40, 262147), (200, 16386), (200, 102408), (200, 163841), (130, 262147), (405, 50304), (405, 102408), (405, 163848), (260, 1000003)])
+@pytest.mark.parametrize("tail", ["renormalize", "bucket"])
+def test_distill_rows_held_and_in_shares(dtype, T, V, tail):
+    """Lengths about those that 256, 512 and 1024 threads hold, of few rows and of many, with the gradient and without."""
+    from olmax_amd import ops
+    print(f"[case] distill T{T} V{V} {tail}", flush=True)
+    z, _ = make(3, V, dtype)
+    ids, t = teacher(z, 33)
+    ids[0, 4], ids[1, 5] = V - 1, 0  # the row's ends
+    per, bound, grad, gbound = distill_bounds(z, ids, t, tail, 1.0, 0.0, torch.ones(3))
+    n = (T + 2) // 3
+    rows, ids, t = z.cuda().repeat(n, 1)[:T], ids.cuda().repeat(n, 1)[:T], t.cuda().repeat(n, 1)[:T]
+    loss, d = ops.distill(rows, ids, t, tail=tail, reduction="none")
+    alone, _ = ops.distill(rows, ids, t, tail=tail, reduction="none", want_grad=False)
+    for i in range(0, T, 1 if T < 50 else 37):
+        for got in (loss, alone):
+            near(got[i:i + 1], per[i % 3:i % 3 + 1], bound[i % 3:i % 3 + 1], f"row loss {i}")
+        near(d[i], grad[i % 3], gbound[i % 3], f"dlogits {i}")
+    mean, dmean = ops.distill(rows, ids, t, tail=tail, inplace=True)
+    assert dmean.data_ptr() == rows.data_ptr()
+    want = per[torch.arange(T) % 3]
+    near(mean, want.mean(), bound[torch.arange(T) % 3].mean() + (T / 1024 + 12) * U * want.abs().mean(), "mean")
+    for i in (0, T // 2, T - 1):
+        near(dmean[i], grad[i % 3] / T, gbound[i % 3] / T + 3 * U * grad[i % 3].abs() / T + 2.0 ** -120, f"dlogits of the mean {i}")
+
+
+def test_offsets_beyond_32_bits():
+    """Rows of 4.4 G logits: the last ones are the first bit for bit, forward and, in place, backward."""
+    from olmax_amd import ops
+    T, V = 22000, 200000
+    z, targets = make(8, V, torch.bfloat16)
+    ids, t = teacher(z, 16)
+    few = z.cuda()
+    targets, ids, t, g = targets.cuda(), ids.cuda(), t.cuda(), torch.randn(8, device="cuda")
+    many = few.repeat(T // 8, 1)
+    large = lambda x: x.repeat(T // 8, *[1] * (x.dim() - 1))  # noqa: E731
+    r = ops.token_logprobs(many, large(targets), top=5)
+    check_scores(r, z.double(), targets.cpu(), 5, rows=torch.arange(T - 8, T))
+    for a in r:
+        assert torch.equal(a[:8], a[T - 8:])
+    loss, d = ops.distill(many, large(ids), large(t), tail="bucket", reduction="none")
+    assert torch.equal(loss[:8], loss[T - 8:]) and torch.equal(d[:8], d[T - 8:]) and torch.equal(d[:8], d[T // 2:T // 2 + 8])
+    del d
+    ops.token_logprobs_bwd(many, large(targets), r.stats, large(g), inplace=True)
+    want = ops.token_logprobs_bwd(few, targets, r.stats[:8].contiguous(), g)
+    assert torch.equal(many[:8], want) and torch.equal(many[T - 8:], want)
 
 
 @pytest.mark.parametrize("tail", ["renormalize", "bucket"])
