@@ -283,26 +283,26 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
       if (at + u * TH + (int)threadIdx.x >= v1) continue;
-      float x[N], t[N];
+      float x[N], t[2] = {0.f, 0.f};  // (two chains of fma)
       now[u].unpack(x);
 #pragma unroll
       for (int e = 0; e < N; e++) {
         if (CAP) {  // scores are finite and small: in units of log 2, without a cut (three of 22 issue slots of a logit; these rows are bound by them)
           const float d = __builtin_fmaf(tail_of_tanh(x[e], c), cap_r, cap_top);
           x[e] = __builtin_amdgcn_exp2f(d);
-          t[e] = x[e] * d;
+          t[e & 1] = __builtin_fmaf(x[e], d, t[e & 1]);
         } else {
           const float d = (x[e] - ref) * c.unit2;
           x[e] = __builtin_amdgcn_exp2f(d);
-          t[e] = x[e] * fmaxf(d, -200.f);
+          t[e & 1] = __builtin_fmaf(x[e], fmaxf(d, -200.f), t[e & 1]);
         }
       }
 #pragma unroll
       for (int w = N / 2; w > 0; w >>= 1)
 #pragma unroll
-        for (int e = 0; e < w; e++) x[e] += x[e + w], t[e] += t[e + w];
+        for (int e = 0; e < w; e++) x[e] += x[e + w];
       a.s += x[0];
-      a.t += t[0] * LN2;
+      a.t = __builtin_fmaf(t[0] + t[1], LN2, a.t);
     }
     if (TOP) {
       if ((ch & (ch + 1)) == 0) {  // 1, 2, 4, .. chunks seen: about k candidates between two bounds, and those below the new one go where many ties came with them
