@@ -17,6 +17,10 @@ namespace {
 
 constexpr int MAX_TOP = 128;
 constexpr int COUNTERS = 64;
+// Held rows' gradients of more bytes than the last-level cache holds are stored past it, where rows that are being read leave them no room.  us, through it | past it, bf16:
+// 4096 x 100352 346 | 329, with a product of the gradients behind it 1320 | 1290; 2048 x 100352 181 | 172, 862 | 874; 4000 x 50304 163 | 155, 604 | 577; fp32 4000 x 50304 313 | 303.
+// Below it: 500 x 50304 32 | 28, with a product 234 | 261; fp32 500 x 100278 81 | 91.
+constexpr int64_t LAST_CACHE = 256ll << 20;
 constexpr int COUNT_IN_ROWS = 1024;  // up to so many rows each workgroup counts them itself
 constexpr float LEAST_TAIL = 0x1p-20f;  // fp32 log probabilities leave less than this undetermined: a tail below it is none (a student without other tokens would lose infinitely by it)
 constexpr int MAX_BITS = 1 << 20;    // tokens that a workgroup can keep a bit of (128 KB)
@@ -167,7 +171,7 @@ struct RowArgs {
   int V;
   int64_t ld, ldd;
   float dloss;
-  int mean, pad;
+  int mean, pad, past_cache;
 };
 
 // The number of rows that are not left out, by the second wave.
@@ -441,7 +445,15 @@ __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict
     w.unpack(x);
 #pragma unroll
     for (int e = 0; e < N; e++) x[e] = outside<CAP>(x[e], c, f);
-    *reinterpret_cast<u32x4*>(dr + cutting.head + v * N) = Vec<TO>::pack(x);
+    u32x4* to = reinterpret_cast<u32x4*>(dr + cutting.head + v * N);
+    const u32x4 all = Vec<TO>::pack(x);
+    if (p.past_cache) {  // (between barriers, or the compiler makes one store of both)
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_nontemporal_store(all, to);
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      *to = all;
+    }
   };
 #pragma unroll
   for (int i = 0; i < HELD; i++) {
@@ -514,7 +526,7 @@ static int distill(hipStream_t stream, const void* logits, void* dlogits, const 
   OLMAX_CHECK(T * std::max(form.parts, form.shares) < (1LL << 31), OLMAX_ERR_SHAPE, "olmax_distill: T=%ld rows of V=%d are too many", (long)T, V);
   Stat* part_stat = (Stat*)((char*)workspace + stats_at(T));
   const bool alone = form.parts == 1 && !dlogits;
-  const RowArgs args{{ids, t, k, form.threads || alone ? nullptr : (float*)(part_stat + T * form.parts)}, row_loss, dloss_rows, n, T, V, ld, ldd, dloss, (int)(reduction == 0), pad};
+  const RowArgs args{{ids, t, k, form.threads || alone ? nullptr : (float*)(part_stat + T * form.parts)}, row_loss, dloss_rows, n, T, V, ld, ldd, dloss, (int)(reduction == 0), pad, (int)(T * V * (grads_f32 ? 4 : 2) > LAST_CACHE)};
 #define LAUNCH(K, GRID, THV, LDS, ...)                                                                                                          \
   do {                                                                                                                                          \
     auto kern = K;                                                                                                                              \
