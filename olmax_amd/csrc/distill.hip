@@ -17,10 +17,6 @@ namespace {
 
 constexpr int MAX_TOP = 128;
 constexpr int COUNTERS = 64;
-// Held rows' gradients of more bytes than the last-level cache holds are stored past it, where rows that are being read leave them no room.  us, through it | past it, bf16:
-// 4096 x 100352 346 | 329, with a product of the gradients behind it 1320 | 1290; 2048 x 100352 181 | 172, 862 | 874; 4000 x 50304 163 | 155, 604 | 577; fp32 4000 x 50304 313 | 303.
-// Below it: 500 x 50304 32 | 28, with a product 234 | 261; fp32 500 x 100278 81 | 91.
-constexpr int64_t LAST_CACHE = 256ll << 20;
 constexpr int COUNT_IN_ROWS = 1024;  // up to so many rows each workgroup counts them itself
 constexpr float LEAST_TAIL = 0x1p-20f;  // fp32 log probabilities leave less than this undetermined: a tail below it is none (a student without other tokens would lose infinitely by it)
 constexpr int MAX_BITS = 1 << 20;    // tokens that a workgroup can keep a bit of (128 KB)
@@ -163,6 +159,9 @@ template <bool CAP> __device__ __forceinline__ float inside(float x, float q, co
   return (exp_behind<CAP>(x, c, f.m) * f.in - q * f.scale) * slope<CAP>(x, c);
 }
 
+// (past_cache) Held rows' gradients of more bytes than LAST_CACHE are stored past it, where rows that are being read leave them no room.  us, through it | past it, bf16:
+// 4096 x 100352 346 | 329, with a product of the gradients behind it 1320 | 1290; 2048 x 100352 181 | 172, 862 | 874; 4000 x 50304 163 | 155, 604 | 577; fp32 4000 x 50304 313 | 303.
+// Below it: 500 x 50304 32 | 28, with a product 234 | 261; fp32 500 x 100278 81 | 91.
 struct RowArgs {
   Teacher teacher;
   float* row_loss;

@@ -3,6 +3,7 @@
 // z = cap(x) / temperature (rows.h), p = softmax(z):  logprob = z[target] - m - ln S,  entropy = ln S - sum p (z - m),
 // alternatives = the `top` largest logits, in order, ties to the lowest index.
 #include "rows.h"
+#include <type_traits>
 #include <algorithm>
 
 using namespace rows;
@@ -216,7 +217,7 @@ __device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, uint
 // alternatives: 197 us, 3.9 TB/s; 19 issue slots a logit, six of them its three transcendental instructions, keep the vector unit busy for 88 %.
 template <typename T, bool CAP, bool TOP, int TH>
 __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out, uint64_t* __restrict__ part_top,
-                                                        Stat* __restrict__ part_stat, int V, int64_t ld, int32_t ignore_index, Scale c, int k, int parts) {
+                                                        Stat* __restrict__ part_stat, int V, int64_t ld, int32_t ignore_index, Scale c, int k, int parts, bool once) {
   constexpr int N = Vec<T>::N, SPAN = TH * UNROLL;
   __shared__ Lds<TH> l;
   const int64_t row = blockIdx.x / parts;
@@ -234,10 +235,20 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
   if (TOP && threadIdx.x == 0) l.n = 0;
   Raw<T, N> next[UNROLL];
   auto fetch = [&](int at) {
+    if (once) {  // (between barriers, or the compiler makes one load of both)
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < UNROLL; u++) {
-      const int v = at + u * TH + threadIdx.x;
-      if (v < v1) next[u].load(body + (int64_t)v * N);
+      for (int u = 0; u < UNROLL; u++) {
+        const int v = at + u * TH + threadIdx.x;
+        if (v < v1) next[u].load_once(body + (int64_t)v * N);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < UNROLL; u++) {
+        const int v = at + u * TH + threadIdx.x;
+        if (v < v1) next[u].load(body + (int64_t)v * N);
+      }
     }
   };
   fetch(v0);
@@ -475,7 +486,7 @@ __global__ __launch_bounds__(256) void zero_columns_kernel(bf16* __restrict__ d,
 // d loss / d logits of logprob and entropy: dz_i = g (delta_it - p_i) - h p_i (ln p_i + H), from the statistics that the forward pass kept.
 // Reads and writes each logit once, without any wait between threads: 4096 x 50304 bf16 159 us, 5.2 TB/s, as a copy; 333 x 100278 fp32 57 us, 4.7 TB/s.
 // A workgroup takes one of `parts` shares of a row.  first: the column of the whole row that these logits begin with (they are its last).
-template <typename T, typename TO, bool CAP, bool ENT, int TH = 256>
+template <typename T, typename TO, bool CAP, bool ENT, bool ONCE, int TH = 256>
 __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const int32_t* __restrict__ targets,
                                                         const float* __restrict__ stats, const float* __restrict__ dlogprobs,
                                                         const float* __restrict__ dentropy, int V, int64_t ld, int64_t ldd, int32_t ignore_index, Scale c,
@@ -498,7 +509,8 @@ __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ lo
     const int i = cutting.head + v * N;
     if (!skipped) {
       Raw<T, N> r;
-      r.load(zr + i);
+      if (ONCE) r.load_once(zr + i);
+      else r.load(zr + i);
       r.unpack(x);
     }
 #pragma unroll
@@ -511,6 +523,11 @@ __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ lo
   }
   if (part == 0 && (int)threadIdx.x < pad) dr[V + threadIdx.x] = (TO)0.f;
 }
+
+// Loads past the last-level cache.  Forward, of logits that it cannot hold: us, 3596 x 100352 bf16 134.4 | 124.6, 1600 x 100352 70 | 64, 1600 x 100278 fp32 123 | 115, and with the
+// gradient behind it 489 | 462 for 4096 x 100352; logits that it can hold may be there from the product: 200 x 100278 fp32 17.3 | 19.3.  Backward, where gradients, which
+// somebody reads next, fit, but not easily beside the logits: 333 x 100278 fp32 57.6 | 46.2, 800 x 50304 bf16 forward, backward and a product behind them 315 | 294, in place
+// 1600 x 50304 64 | 58 (800 x 50304: 30 | 34); where they do not fit: 4096 x 50304 159.1 | 161.1.
 
 // Threads of a workgroup and shares of a row in the forward pass.
 struct Form {
@@ -554,9 +571,10 @@ extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, 
   Stat* part_stat = parts == 1 ? nullptr : (Stat*)((char*)workspace + T * parts * (int64_t)top * 8);
   const Out out{logprobs, entropy, stats, top ? top_logprobs : nullptr, top ? top_ids : nullptr};
   const Scale c = scale_of(temperature, softcap);
+  const bool past_cache = T * V * (logits_f32 ? 4 : 2) > LAST_CACHE;
 #define ROWS(TY, CAPV, TOPV, THV)                                                                                                                             \
   hipLaunchKernelGGL((score_rows_kernel<TY, CAPV, TOPV, THV>), dim3((unsigned)(T * parts)), dim3(THV), 0, stream, (const TY*)logits, targets, out, part_top, \
-                     part_stat, V, ld, ignore_index, c, top, parts)
+                     part_stat, V, ld, ignore_index, c, top, parts, past_cache)
 #define SCORE(TY, CAPV, TOPV)                                                                                                                             \
   do {                                                                                                                                                    \
     if (form.threads == 256) ROWS(TY, CAPV, TOPV, 256); else if (form.threads == 512) ROWS(TY, CAPV, TOPV, 512); else ROWS(TY, CAPV, TOPV, 1024);                                                                  \
@@ -582,15 +600,24 @@ static int token_logprobs_bwd(hipStream_t stream, const void* logits, const int3
   const Scale c = scale_of(temperature, softcap);
   const int parts = (int)std::max<int64_t>(1, V / (grads_f32 ? 4 : 8) / 2048);
   OLMAX_CHECK(T * parts < (1LL << 31), OLMAX_ERR_SHAPE, "olmax_token_logprobs_bwd: T=%ld rows of V=%d are too many", (long)T, V);
-#define GRAD(TY, TO, CAPV, ENTV)                                                                                                                             \
-  hipLaunchKernelGGL((score_grad_kernel<TY, TO, CAPV, ENTV>), dim3((unsigned)(T * parts)), dim3(256), 0, stream, (const TY*)logits, (TO*)dlogits, targets, stats, \
-                     dlogprobs, dentropy, V, ld, ldd, ignore_index, c, parts, pad, first)
-#define GRAD_E(TY, TO, CAPV) do { if (dentropy) GRAD(TY, TO, CAPV, true); else GRAD(TY, TO, CAPV, false); } while (0)
-#define GRAD_C(TY, TO) do { if (softcap > 0.f) GRAD_E(TY, TO, true); else GRAD_E(TY, TO, false); } while (0)
-  if (logits_f32 && grads_f32) GRAD_C(float, float); else if (logits_f32) GRAD_C(float, bf16); else GRAD_C(bf16, bf16);
-#undef GRAD
-#undef GRAD_E
-#undef GRAD_C
+  const int64_t bytes = T * V * (grads_f32 ? 4 : 2);
+  const bool past_cache = bytes <= LAST_CACHE && (logits == dlogits ? bytes : 2 * bytes) > LAST_CACHE / 2;
+  auto go = [&](auto in, auto out, auto capped, auto entropies, auto once) {
+    using TY = decltype(in);
+    using TO = decltype(out);
+    hipLaunchKernelGGL((score_grad_kernel<TY, TO, decltype(capped)::value, decltype(entropies)::value, decltype(once)::value>), dim3((unsigned)(T * parts)), dim3(256), 0, stream,
+                       (const TY*)logits, (TO*)dlogits, targets, stats, dlogprobs, dentropy, V, ld, ldd, ignore_index, c, parts, pad, first);
+  };
+  auto kind = [&](auto in, auto out) {
+    const std::true_type yes;
+    const std::false_type no;
+    auto loads = [&](auto capped, auto entropies) { past_cache ? go(in, out, capped, entropies, yes) : go(in, out, capped, entropies, no); };
+    if (softcap > 0.f) dentropy ? loads(yes, yes) : loads(yes, no);
+    else dentropy ? loads(no, yes) : loads(no, no);
+  };
+  if (logits_f32 && grads_f32) kind(0.f, 0.f);
+  else if (logits_f32) kind(0.f, bf16());
+  else kind(bf16(), bf16());
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }
@@ -688,7 +715,7 @@ extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, cons
     constexpr bool CAP = decltype(capped)::value;
     if (rest)
       hipLaunchKernelGGL((score_rows_kernel<float, CAP, false, 256>), dim3((unsigned)T), dim3(256), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,
-                         p.ld, ignore_index, c, 0, 1);
+                         p.ld, ignore_index, c, 0, 1, false);
     hipLaunchKernelGGL((head_join_kernel<CAP>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,
                        (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, p.rows, V, p.fused, ignore_index, c);
   };

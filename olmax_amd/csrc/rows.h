@@ -11,6 +11,8 @@
 
 namespace rows {
 
+constexpr int64_t LAST_CACHE = 256ll << 20;  // bytes that the cache behind the L2s holds
+
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;  // 16 bytes at any element
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
