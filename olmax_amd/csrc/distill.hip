@@ -160,7 +160,7 @@ template <bool CAP> __device__ __forceinline__ float inside(float x, float q, co
 }
 
 // (past_cache) Held rows' gradients of more bytes than LAST_CACHE are stored past it, where rows that are being read leave them no room.  us, through it | past it, bf16:
-// 4096 x 100352 346 | 329, with a product of the gradients behind it 1320 | 1290; 2048 x 100352 181 | 172, 862 | 874; 4000 x 50304 163 | 155, 604 | 577; fp32 4000 x 50304 313 | 303.
+// 4096 x 100352 346 | 329, with a product of the gradients behind it 1320 | 1290; 2048 x 100352 181 | 172, 862 | 874; 4000 x 50304 163 | 155, 604 | 577; fp32 4000 x 50304 313 | 303; nor are logits kept there that are read once, for the loss alone: 700 x 128256 fp32 69.7 | 65.1.
 // Below it: 500 x 50304 32 | 28, with a product 234 | 261; fp32 500 x 100278 81 | 91.
 struct RowArgs {
   Teacher teacher;
@@ -191,7 +191,7 @@ template <typename TO, int TH> __device__ __forceinline__ void write_zeros(TO* d
 }
 
 // Rows that no workgroup holds, and few rows: two launches of shares of rows.  The first leaves statistics (BUCKET: sums of the other tokens) of each share, and the teacher's tokens'
-// logits; or (part_stat null) the loss of whole rows, and there is no second.  700 x 128256 fp32: 65 us, 5.5 TB/s.
+// logits; or (part_stat null) the loss of whole rows, and there is no second.  700 x 128256 fp32: 60 us, 6.0 TB/s.
 template <typename T, bool CAP, bool BUCKET, int TH>
 __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__ logits, const RowArgs p, const Scale c, Stat* __restrict__ part_stat, int parts) {
   constexpr int N = Vec<T>::N, UNROLL = 4, SPAN = TH * UNROLL;
@@ -210,10 +210,19 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
   const int per = (cutting.nvec + parts - 1) / parts;
   const int v0 = min(part * per, cutting.nvec), v1 = min(v0 + per, cutting.nvec);
   Raw<T, N> next[UNROLL];
+  const bool once = !part_stat && p.past_cache;  // (no second launch reads them)
   auto fetch = [&](int at) {
+    if (once) {  // (between barriers, or the compiler makes one load of both)
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < UNROLL; u++)
-      if (at + u * TH + tid < v1) next[u].load(body + (int64_t)(at + u * TH + tid) * N);
+      for (int u = 0; u < UNROLL; u++)
+        if (at + u * TH + tid < v1) next[u].load_once(body + (int64_t)(at + u * TH + tid) * N);
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < UNROLL; u++)
+        if (at + u * TH + tid < v1) next[u].load(body + (int64_t)(at + u * TH + tid) * N);
+    }
   };
   fetch(v0);
   if (!part_stat && tid < 64) teacher_of<T, BUCKET, TH / 64>(p.teacher, row, zr, V, c.inv_tau, nullptr, 0, l);  // (beside the others' first loads)
@@ -336,7 +345,7 @@ __global__ __launch_bounds__(256) void distill_grads_kernel(const T* __restrict_
 }
 
 // One workgroup a row, of which a thread keeps HELD vectors in registers: statistics and the loss, then the gradient of all tokens, then the k tokens' own.
-// Each logit is read once and its gradient written once, and no exponential is kept: those of the gradient are taken again.  4096 x 100352 bf16 to bf16: 339 us, 4.8 TB/s (a copy:
+// Each logit is read once and its gradient written once, and no exponential is kept: those of the gradient are taken again.  4096 x 100352 bf16 to bf16: 323 us, 5.1 TB/s (a copy:
 // 5.2), the vector unit busy for 60 %: the rows of a CU, of which registers hold two, read and write in turns that overlap only with each other's.
 template <typename T, typename TO, bool CAP, bool BUCKET, int TH, int HELD>
 __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const RowArgs p, const Scale c) {
@@ -525,7 +534,7 @@ static int distill(hipStream_t stream, const void* logits, void* dlogits, const 
   OLMAX_CHECK(T * std::max(form.parts, form.shares) < (1LL << 31), OLMAX_ERR_SHAPE, "olmax_distill: T=%ld rows of V=%d are too many", (long)T, V);
   Stat* part_stat = (Stat*)((char*)workspace + stats_at(T));
   const bool alone = form.parts == 1 && !dlogits;
-  const RowArgs args{{ids, t, k, form.threads || alone ? nullptr : (float*)(part_stat + T * form.parts)}, row_loss, dloss_rows, n, T, V, ld, ldd, dloss, (int)(reduction == 0), pad, (int)(T * V * (grads_f32 ? 4 : 2) > LAST_CACHE)};
+  const RowArgs args{{ids, t, k, form.threads || alone ? nullptr : (float*)(part_stat + T * form.parts)}, row_loss, dloss_rows, n, T, V, ld, ldd, dloss, (int)(reduction == 0), pad, (int)(T * V * (dlogits && !grads_f32 || !logits_f32 ? 2 : 4) > LAST_CACHE)};
 #define LAUNCH(K, GRID, THV, LDS, ...)                                                                                                          \
   do {                                                                                                                                          \
     auto kern = K;                                                                                                                              \

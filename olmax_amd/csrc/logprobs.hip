@@ -213,8 +213,8 @@ __device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, uint
 
 // One workgroup to a row, or to one of `parts` equal shares of it; with part_stat a share leaves its statistics and its candidates for a kernel that joins them.
 // The row is read once, a chunk of four vectors a thread ahead of the one in work; the largest score of a chunk is known before its exponentials, which are taken against the
-// largest so far.  3596 x 100352 bf16: 133 us, 5.4 TB/s, the vector unit busy for 88 % of it (a copy on the card reads and writes 5.2).  1500 x 256000 with a soft-cap and 64
-// alternatives: 197 us, 3.9 TB/s; 19 issue slots a logit, six of them its three transcendental instructions, keep the vector unit busy for 88 %.
+// largest so far.  3596 x 100352 bf16: 124 us, 5.8 TB/s, the vector unit busy for 90 % of it (a copy on the card reads and writes 5.2).  1500 x 256000 with a soft-cap and 64
+// alternatives: 196 us, 3.9 TB/s; 19 issue slots a logit, six of them its three transcendental instructions, keep the vector unit busy for 88 %.
 template <typename T, bool CAP, bool TOP, int TH>
 __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out, uint64_t* __restrict__ part_top,
                                                         Stat* __restrict__ part_stat, int V, int64_t ld, int32_t ignore_index, Scale c, int k, int parts, bool once) {
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256) void zero_columns_kernel(bf16* __restrict__ d,
 }
 
 // d loss / d logits of logprob and entropy: dz_i = g (delta_it - p_i) - h p_i (ln p_i + H), from the statistics that the forward pass kept.
-// Reads and writes each logit once, without any wait between threads: 4096 x 50304 bf16 159 us, 5.2 TB/s, as a copy; 333 x 100278 fp32 57 us, 4.7 TB/s.
+// Reads and writes each logit once, without any wait between threads: 4096 x 50304 bf16 159 us, 5.2 TB/s, as a copy; 333 x 100278 fp32 46 us, 5.8 TB/s.
 // A workgroup takes one of `parts` shares of a row.  first: the column of the whole row that these logits begin with (they are its last).
 template <typename T, typename TO, bool CAP, bool ENT, bool ONCE, int TH = 256>
 __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const int32_t* __restrict__ targets,
