@@ -345,7 +345,7 @@ __global__ __launch_bounds__(256) void distill_grads_kernel(const T* __restrict_
 }
 
 // One workgroup a row, of which a thread keeps HELD vectors in registers: statistics and the loss, then the gradient of all tokens, then the k tokens' own.
-// Each logit is read once and its gradient written once, and no exponential is kept: those of the gradient are taken again.  4096 x 100352 bf16 to bf16: 323 us, 5.1 TB/s (a copy:
+// Each logit is read once and its gradient written once, and no exponential is kept: those of the gradient are taken again.  4096 x 100352 bf16 to bf16: 329 us with the count and the sum, 5.0 TB/s (a copy:
 // 5.2), the vector unit busy for 60 %: the rows of a CU, of which registers hold two, read and write in turns that overlap only with each other's.
 template <typename T, typename TO, bool CAP, bool BUCKET, int TH, int HELD>
 __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const RowArgs p, const Scale c) {
