@@ -598,18 +598,20 @@ static int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct HeadPlan {
   bool few;       // tokens fewer than a tile has rows: the gradients' products pad them, and the logits' those of more than 64
+  bool in64;      // gradients of 64 tokens
   int64_t rows, ld, grads_at, rows_at, h_at, dh_at, bytes;
 };
 static HeadPlan head_plan(int64_t T, int32_t d, int32_t V, int32_t k) {
   HeadPlan p;
   p.few = olmax_lmhead_pads(T, d, V);
+  p.in64 = olmax_lmhead_pads_64(T, d, V);
   p.rows = p.few && T > 64 ? 256 : T;
   p.ld = head_stride(V);
   p.grads_at = up256(std::max<int64_t>(p.rows * p.ld * 4, p.few ? PRODUCT_SCRATCH : 0));
-  p.rows_at = p.grads_at + up256((p.few ? 256 : T) * p.ld * 2);
+  p.rows_at = p.grads_at + up256((p.few ? 256 : p.in64 ? 64 : T) * p.ld * 2);
   p.h_at = p.rows_at + up256(olmax_distill_workspace_bytes(T, V, k, 1));
-  p.dh_at = p.h_at + (p.few ? up256(256ll * d * 2) : 0);
-  p.bytes = p.dh_at + (p.few ? up256(256ll * d * 2) : 0);
+  p.dh_at = p.h_at + (p.few || p.in64 ? up256((p.few ? 256ll : 64ll) * d * 2) : 0);
+  p.bytes = p.dh_at + (p.few || p.in64 ? up256((p.few ? 256ll : 64ll) * d * 2) : 0);
   return p;
 }
 extern "C" int64_t olmax_lmhead_distill_workspace_bytes(int64_t T, int32_t d, int32_t V, int32_t k) {
@@ -642,7 +644,8 @@ extern "C" int32_t olmax_lmhead_distill(hipStream_t stream, const void* h, const
                        dloss, 0, pad))
     return rc;
   const GemmScratch scratch{workspace, std::min(p.grads_at, PRODUCT_SCRATCH)};  // (the logits are done with)
-  if (!p.few) return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, scratch);
+  if (p.in64 && dW) olmax_pad_rows(stream, hp, h_pad, T, 64, d);
+  else if (!p.few) return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, scratch);
   if (dW) olmax_zero_rows(stream, grads, T, 64, V + pad, p.ld);
-  return olmax_lmhead_products_few(stream, grads, wp, hp, h_pad, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, (bf16*)(ws + p.dh_at), scratch);
+  return olmax_lmhead_products_few(stream, grads, wp, hp, h_pad, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, (bf16*)(ws + p.dh_at), p.few ? 256 : 64, scratch);
 }

@@ -22,6 +22,10 @@ __global__ __launch_bounds__(256) void zero_rows_kernel(bf16* __restrict__ d, in
 
 }  // namespace
 
+// us, distillation of 63 tokens as they are | with gradients of 64: 9402 x 4096 118 | 84, 20000 x 4096 236 | 159, 2000 x 4096 41 | 38, 9402 x 1024 61 | 56, 20000 x 1024 103 | 79; narrow and small ones
+// gain less (64 tokens for 63: 36000 x 256 70 for 72, 4096 x 1024 23 for 31) than the three launches that pad cost.
+bool olmax_lmhead_pads_64(int64_t T, int32_t d, int32_t V) { return T < 64 && d % 8 == 0 && d >= 1024 && (int64_t)V * d >= 8000000 && !olmax_lmhead_pads(T, d, V); }
+
 bool olmax_lmhead_pads(int64_t T, int32_t d, int32_t V) { return T < 256 && olmax_gemm_head_columns(256, V, d) > 0; }
 
 void olmax_pad_rows(hipStream_t s, const bf16* src, bf16* dst, int64_t rows, int64_t padded, int d) {
@@ -35,7 +39,13 @@ void olmax_zero_rows(hipStream_t s, bf16* d, int64_t from, int64_t to, int64_t n
 }
 
 int olmax_lmhead_products_few(hipStream_t stream, const bf16* dlogits, const bf16* W, const bf16* h, const bf16* h_pad, bf16* dh, void* dW, int T, int d, int V, int64_t ldl,
-                              bool dw_f32, bf16* tmp, GemmScratch scratch) {
+                              bool dw_f32, bf16* tmp, int rows, GemmScratch scratch) {
+  if (rows == 64) {
+    if (int rc = olmax_lmhead_products(stream, dlogits, W, h_pad, dh ? tmp : nullptr, dW, 64, d, V, ldl, dw_f32, scratch)) return rc;
+    if (dh) olmax_pad_rows(stream, tmp, dh, T, T, d);
+    OLMAX_LAUNCH_CHECK();
+    return OLMAX_OK;
+  }
   if (dh) {  // (rows behind the tokens are products of whatever is there, and are left behind)
     if (int rc = olmax_gemm_padded(stream, dlogits, W, tmp, nullptr, 256, d, V, ldl, d, d, 0, true, false, false, true, scratch)) return rc;
     olmax_pad_rows(stream, tmp, dh, T, T, d);

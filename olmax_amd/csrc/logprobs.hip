@@ -729,6 +729,7 @@ extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, cons
 // padded to `rows`) the padded tokens, and room for dh
 struct HeadGradPlan {
   int fused;
+  bool in64;  // gradients of 64 tokens
   int64_t rows, ld, logits_at, room, h_at, dh_at, bytes;
 };
 static HeadGradPlan head_grad_plan(int64_t T, int32_t d, int32_t V) {
@@ -736,11 +737,12 @@ static HeadGradPlan head_grad_plan(int64_t T, int32_t d, int32_t V) {
   p.rows = olmax_lmhead_pads(T, d, V) ? 256 : T;
   p.fused = olmax_gemm_head_columns((int)p.rows, V, d);
   p.ld = head_stride(V);
-  p.logits_at = up256(p.rows * p.ld * 2);
+  p.in64 = olmax_lmhead_pads_64(T, d, V);
+  p.logits_at = up256((p.in64 ? 64 : p.rows) * p.ld * 2);
   p.room = std::max(up256(p.rows * head_stride(V - p.fused) * 4), p.fused ? PRODUCT_SCRATCH : 0);
   p.h_at = p.logits_at + p.room;
-  p.dh_at = p.h_at + (p.rows > T ? up256(p.rows * d * 2) : 0);
-  p.bytes = p.dh_at + (p.rows > T ? up256(p.rows * d * 2) : 0);
+  p.dh_at = p.h_at + (p.rows > T ? up256(p.rows * d * 2) : p.in64 ? up256(64ll * d * 2) : 0);
+  p.bytes = p.dh_at + (p.rows > T ? up256(p.rows * d * 2) : p.in64 ? up256(64ll * d * 2) : 0);
   return p;
 }
 extern "C" int64_t olmax_lmhead_logprobs_bwd_workspace_bytes(int64_t T, int32_t d, int32_t V) {
@@ -769,9 +771,9 @@ extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, 
   char* ws = (char*)workspace;
   bf16* grads = (bf16*)ws;
   float* logits = (float*)(ws + p.logits_at);
-  const bool padded = p.rows > T;
+  const bool padded = p.rows > T, in64 = p.in64 && dW;  // (dh alone gains nothing by it)
   bf16* h_pad = (bf16*)(ws + p.h_at);
-  if (padded) olmax_pad_rows(stream, hp, h_pad, T, p.rows, d);
+  if (padded || in64) olmax_pad_rows(stream, hp, h_pad, T, padded ? p.rows : 64, d);
   const bf16* tokens = padded ? h_pad : hp;
   if (p.fused) {
     HeadRows rows{};
@@ -789,12 +791,13 @@ extern "C" int32_t olmax_lmhead_logprobs_bwd(hipStream_t stream, const void* h, 
     if (int rc = token_logprobs_bwd(stream, logits, targets, stats, dlogprobs, dentropy, grads + p.fused, T, rest, ldr, p.ld, true, false, ignore_index, temperature, softcap, pad,
                                     p.fused))
       return rc;
-    if (padded) olmax_zero_rows(stream, grads + p.fused, T, 64, rest + pad, p.ld);
+    if (padded || in64) olmax_zero_rows(stream, grads + p.fused, T, 64, rest + pad, p.ld);
   } else if (pad) {
     hipLaunchKernelGGL(zero_columns_kernel, dim3((unsigned)((p.rows * pad + 255) / 256)), dim3(256), 0, stream, grads + V, p.rows, p.ld, pad);
   }
   const GemmScratch scratch{logits, std::min(p.room, PRODUCT_SCRATCH)};
-  if (padded) return olmax_lmhead_products_few(stream, grads, wp, hp, h_pad, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, (bf16*)(ws + p.dh_at), scratch);
+  if (padded || in64)
+    return olmax_lmhead_products_few(stream, grads, wp, hp, h_pad, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, (bf16*)(ws + p.dh_at), padded ? 256 : 64, scratch);
   // (without shared reductions the few long ones of dh take 60 % more: dh and dW of 1024 x 4096 x 100352 1.78 -> 1.34 ms)
   return olmax_lmhead_products(stream, grads, wp, hp, (bf16*)dh, dW, (int)T, d, V, p.ld, dw_f32 != 0, scratch);
 }

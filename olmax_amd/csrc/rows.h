@@ -212,14 +212,16 @@ int olmax_gemm_head_grads(hipStream_t s, const bf16* h, const bf16* w, bf16* d, 
 // lmhead_rows.hip: the LM head's products on fewer tokens than a tile of 256 has rows.  Whether large tiles do better with the tokens padded to 256 (for the logits of more than
 // 64 tokens, and for the gradients):
 bool olmax_lmhead_pads(int64_t T, int32_t d, int32_t V);
+// Whether, where that is not so, the gradients do better with the tokens padded to 64:
+bool olmax_lmhead_pads_64(int64_t T, int32_t d, int32_t V);
 // dst [padded, d] = src [rows, d] and zeros; d is a multiple of 8 and both are 16-byte aligned
 void olmax_pad_rows(hipStream_t s, const bf16* src, bf16* dst, int64_t rows, int64_t padded, int d);
 // columns [0, n) of rows [from, to) of d = 0
 void olmax_zero_rows(hipStream_t s, bf16* d, int64_t from, int64_t to, int64_t n, int64_t ld);
-// olmax_lmhead_products of T < 256 tokens: dlogits has 256 rows of memory, h_pad [64, d] is h and zeros (read, as rows T to 63 of dlogits are, where T < 64), tmp [256, d] is room
-// for dh
+// olmax_lmhead_products of T tokens padded to `rows`, 64 or 256, that dlogits and tmp [rows, d], for dh, have memory of.  h_pad is h and zeros up to row 63; where T < 64 so is dlogits
+// (other rows of it may hold anything).
 int olmax_lmhead_products_few(hipStream_t stream, const bf16* dlogits, const bf16* W, const bf16* h, const bf16* h_pad, bf16* dh, void* dW, int T, int d, int V, int64_t ldl,
-                              bool dw_f32, bf16* tmp, GemmScratch scratch);
+                              bool dw_f32, bf16* tmp, int rows, GemmScratch scratch);
 
 // What the LM head's calls are given, for their checks ahead of any launch (olmax_model_logprobs and its like make them ahead of the model's).
 struct HeadScore {

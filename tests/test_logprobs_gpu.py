@@ -461,7 +461,8 @@ def head(T, d, V, seed=0):
     return h, W, t
 
 
-HEADS = [(1, 64, 100), (5, 256, 4096), (33, 100, 777), (37, 200, 1003), (300, 320, 1030), (513, 1024, 5000), (1024, 512, 2304), (700, 72, 50304)]
+HEADS = [(1, 64, 100), (5, 256, 4096), (33, 100, 777), (37, 200, 1003), (300, 320, 1030), (513, 1024, 5000), (1024, 512, 2304), (700, 72, 50304),
+         (33, 1032, 8001), (63, 2048, 4001)]  # (gradients of 64 tokens)
 # large tiles, the logits in the accumulators: whole rounds of tiles and columns behind them; partial tiles and k-tiles; a row length that is no multiple of 8, with and without
 # columns behind the last round; one round exactly
 IN_TILES = [(256, 64, 70000), (511, 72, 40007), (700, 128, 50301), (512, 256, 32768)]
