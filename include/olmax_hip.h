@@ -200,9 +200,9 @@ int32_t olmax_cross_entropy_reduce(olmax_stream_t stream, const void* logits, vo
  * from logits.  No counterpart in the reference (its cross_entropy_loss, src/olmax/nn/functional.py:70-91, returns -logprob of the labels).
  * z = cap(x) / temperature, cap(x) = softcap * tanh(x / softcap) where softcap > 0; p = softmax(z) over the V logits of a row.
  * logprobs [T] (optional; needs targets) = ln p[target], 0 for a target outside [0, V); entropy [T] = - sum p ln p;
- * stats [T, 3] = {m = max z, ln sum exp(z - m), entropy}, what the backward call takes (its first two add up to the log-normaliser; m is
- * rounded, so that gradients of scores beyond 2^20 at a temperature that is no power of two are off by 2^-24 |m|, and a row whose scores
- * have no room in fp32, which the other results take in their stride, has none);
+ * stats [T, 3] = {m = max z, ln sum exp(z - m), entropy}, what the backward call takes (its first two add up to the log-normaliser).  m is
+ * rounded: gradients of scores beyond 2^20 at a temperature that is no power of two are off by 2^-24 |m|, and a row all of whose scores
+ * are beyond fp32 (its lowest value everywhere, at a temperature below 1) gets no gradient; the results here take differences of logits and are exact for both;
  * top_ids / top_logprobs [T, top] (top 0 to 128, at most V): the largest logits x in order, ties to the lowest index.  A row whose target
  * is ignore_index is not read: zeros, ids of -1, log probabilities of minus infinity.  Logits of minus infinity are tokens of no
  * probability; a row of nothing else has entropy 0 and log probabilities of minus infinity.  A NaN or an infinite score makes a row's values NaN
@@ -214,7 +214,7 @@ int32_t olmax_token_logprobs(olmax_stream_t stream, const void* logits, const in
                              void* workspace, int64_t workspace_bytes, int64_t T, int32_t V, int64_t ld,
                              int32_t top, int32_t logits_f32, int32_t ignore_index, float temperature,
                              float softcap);
-/* dlogits [T, V] (type of the logits; may be them, with the same stride) from the cotangents dlogprobs [T] and dentropy [T] (optional).  Rows of
+/* dlogits [T, V] (type of the logits; may be them, with the same stride, or share no element with them) from the cotangents dlogprobs [T] and dentropy [T] (optional).  Rows of
  * an ignored target get zeros, a target outside [0, V) has no log probability to follow. */
 int32_t olmax_token_logprobs_bwd(olmax_stream_t stream, const void* logits, const int32_t* targets,
                                  const float* stats, const float* dlogprobs, const float* dentropy,
@@ -228,7 +228,7 @@ int32_t olmax_token_logprobs_bwd(olmax_stream_t stream, const void* logits, cons
  * p is the student's softmax of cap(logits) / temperature.  A row whose first id is negative is left out (no loss, zero gradient); other ids
  * outside [0, V), and those named before in the row, are dropped.  A row without a logit above minus infinity has no loss and no gradient.
  * reduction 0 mean over the rows that are not left out, 1 sum, 2 none (loss [T], cotangent dloss * dloss_rows[t]).  dlogits (optional; type of the
- * logits; may be them, with the same stride) receives dloss * dL/dlogits.  (Softened targets are commonly weighted by temperature^2: through dloss.) */
+ * logits; may be them, with the same stride, or share no element with them) receives dloss * dL/dlogits.  (Softened targets are commonly weighted by temperature^2: through dloss.) */
 int64_t olmax_distill_workspace_bytes(int64_t T, int32_t V, int32_t k, int32_t logits_f32);
 int32_t olmax_distill(olmax_stream_t stream, const void* logits, void* dlogits, const int32_t* top_ids,
                       const float* top_logprobs, float* loss, const float* dloss_rows, void* workspace,

@@ -649,3 +649,55 @@ def test_results_repeat():
     for _ in range(5):
         again = ops.token_logprobs(z, t, top=128)
         assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def _all_calls(T, V, d, seed):
+    """Every row operator and every form with the LM head, on inputs of their own: a call that returns all results."""
+    from olmax_amd import ops
+    z, t = make(T, V, torch.bfloat16, seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    h, W = (torch.randn(n, d, generator=g).to(torch.bfloat16).cuda() for n in (T, V))
+    z, t, c = z.cuda(), t.cuda(), torch.randn(T, generator=g).cuda()
+
+    def work():
+        r = ops.token_logprobs(z, t, top=12)
+        s = ops.lmhead_logprobs(h, W, t, temperature=8.0)
+        return [*r, ops.token_logprobs_bwd(z, t, r.stats, c, dentropy=c), *ops.distill(z, r.top_ids, r.top_logprobs, tail="bucket"), s.logprobs, s.entropy, s.stats,
+                *ops.lmhead_logprobs_bwd(h, W, t, s.stats, c, temperature=8.0), *ops.lmhead_distill(h, W, r.top_ids, r.top_logprobs, temperature=8.0)]
+    return work
+
+
+def test_two_streams_at_once():
+    """Calls on two streams whose work overlaps, with workspaces from one allocator, leave the results of calls by themselves."""
+    works = [_all_calls(5, 40000, 64, 1), _all_calls(300, 9001, 128, 2)]
+    want = [[x.clone() for x in w()] for w in works]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in works]
+    got = [[], []]
+    for _ in range(6):
+        for i, (s, w) in enumerate(zip(streams, works)):
+            with torch.cuda.stream(s):
+                got[i].append(w())
+    torch.cuda.synchronize()
+    for many, one in zip(got, want):
+        for results in many:
+            assert all(torch.equal(a, b) for a, b in zip(results, one))
+
+
+def test_two_graphs_that_share_their_memory():
+    """Graphs recorded into one pool, whose workspaces may lie in the same place, replayed in turn: each leaves its own results."""
+    works = [_all_calls(5, 40000, 64, 1), _all_calls(300, 9001, 128, 2)]
+    want = [[x.clone() for x in w()] for w in works]
+    torch.cuda.synchronize()
+    pool, graphs, outs = None, [], []
+    for w in works:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(w())
+        pool = graph.pool()
+        graphs.append(graph)
+    for i in (0, 1, 1, 0, 1, 0):
+        graphs[i].replay()
+        works[1 - i]()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i]))
