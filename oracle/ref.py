@@ -397,15 +397,15 @@ def distill_bwd(logits: Tensor, top_ids: Tensor, top_logprobs: Tensor, *, tail: 
     q, _, r, ok = _teacher(ids, top_logprobs, V, tail, temperature)
     z = token_scores(logits, temperature, softcap)
     none = (z == -math.inf).all(1)
-    p = torch.where(none[:, None], 0.0, torch.softmax(z, 1))
+    logp = _log_softmax(z)
+    p = torch.where(none[:, None], 0.0, logp.exp())
     at = torch.where(ok, ids, V)
-    w = q.sum(1) + r
-    outside = w[:, None].expand(T, V)
-    if tail == "bucket":
+    d = p * (q.sum(1) + r)[:, None]
+    if tail == "bucket":  # p / s from logarithms: both may be beyond 64 bits
         hidden = torch.zeros(T, V + 1, dtype=torch.bool).scatter(1, at, True)[:, :V]
-        s = torch.where(hidden, 0.0, p).sum(1)
-        outside = torch.where(hidden, w[:, None], (w - torch.where(r > 0, r / s, 0.0))[:, None])
-    d = torch.cat([p * outside, torch.zeros(T, 1, dtype=p.dtype)], 1).scatter_add(1, at, -q)[:, :V]
+        log_s = torch.logsumexp(torch.where(hidden, -math.inf, logp), 1)[:, None]
+        d = d - r[:, None] * torch.where(hidden | (log_s == -math.inf), 0.0, (logp - log_s).exp())
+    d = torch.cat([d, torch.zeros(T, 1, dtype=p.dtype)], 1).scatter_add(1, at, -q)[:, :V]
     kept = (ids[:, 0] >= 0) & ~none
     n = (ids[:, 0] >= 0).sum().clamp(min=1) if reduction == "mean" else 1
     scale = torch.as_tensor(dloss, dtype=p.dtype).expand(T) / n
