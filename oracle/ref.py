@@ -401,10 +401,11 @@ def distill_bwd(logits: Tensor, top_ids: Tensor, top_logprobs: Tensor, *, tail: 
     p = torch.where(none[:, None], 0.0, logp.exp())
     at = torch.where(ok, ids, V)
     d = p * (q.sum(1) + r)[:, None]
-    if tail == "bucket":  # p / s from logarithms: both may be beyond 64 bits
+    if tail == "bucket":  # p / s is the others' own softmax: both may be beyond 64 bits
         hidden = torch.zeros(T, V + 1, dtype=torch.bool).scatter(1, at, True)[:, :V]
-        log_s = torch.logsumexp(torch.where(hidden, -math.inf, logp), 1)[:, None]
-        d = d - r[:, None] * torch.where(hidden | (log_s == -math.inf), 0.0, (logp - log_s).exp())
+        others = torch.where(hidden, -math.inf, logp)
+        alone = (others == -math.inf).all(1, keepdim=True)
+        d = d - r[:, None] * torch.where(alone, 0.0, torch.softmax(others, 1))
     d = torch.cat([d, torch.zeros(T, 1, dtype=p.dtype)], 1).scatter_add(1, at, -q)[:, :V]
     kept = (ids[:, 0] >= 0) & ~none
     n = (ids[:, 0] >= 0).sum().clamp(min=1) if reduction == "mean" else 1

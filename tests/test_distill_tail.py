@@ -44,3 +44,11 @@ def test_no_other_token_is_left():
     loss, d = (f(z, ids, t, tail="bucket", reduction="none") for f in (ref.distill_fwd, ref.distill_bwd))
     assert loss[0] == math.inf and torch.isfinite(loss[1]) and torch.isfinite(d).all()
     assert (d[0, :4] == 0).all() and abs(d[1].sum()) < 1e-15 and abs(d[1, 5] - (0.5 - 0.25)) < 1e-15
+
+
+def test_others_at_the_types_lowest_value():
+    """A mask of finite numbers leads as any other: each of the others has its equal share of r."""
+    z = torch.full((1, 50), float(torch.finfo(torch.float32).min), dtype=torch.float64)
+    z[0, 3] = 1.0
+    d = ref.distill_bwd(z, torch.tensor([[3]]), torch.full((1, 1), math.log(0.75), dtype=torch.float64), tail="bucket", temperature=0.5, reduction="none")[0]
+    assert abs(d[3] - 0.5) < 1e-15 and (d[4:] + 0.5 / 49).abs().max() < 1e-15
