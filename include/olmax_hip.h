@@ -225,7 +225,8 @@ int32_t olmax_token_logprobs_bwd(olmax_stream_t stream, const void* logits, cons
  * top_ids / top_logprobs [T, k], k 1 to 128, are the teacher's tokens and what it says of them (olmax_token_logprobs writes both).
  * tail 0, renormalize: q = softmax over the k numbers / temperature; L = sum q ln(q / p[id]).  tail 1, bucket: q = exp(top_logprobs), and all
  * other tokens are one event: L = sum q ln(q / p[id]) + r ln(r / s), r = 1 - sum q (0 below 2^-20), s = sum of the other tokens' p (V up to 2^20 - 32).
- * p is the student's softmax of cap(logits) / temperature.  A row whose first id is negative is left out (no loss, zero gradient); other ids
+ * p is the student's softmax of cap(logits) / temperature; s and the others' gradient p_i (1 - r / s) are as exact where the k tokens lead by more than fp32 has
+ * exponentials for (no other token above minus infinity: an infinite loss, and no gradient).  A row whose first id is negative is left out (no loss, zero gradient); other ids
  * outside [0, V), and those named before in the row, are dropped.  A row without a logit above minus infinity has no loss and no gradient.
  * reduction 0 mean over the rows that are not left out, 1 sum, 2 none (loss [T], cotangent dloss * dloss_rows[t]).  dlogits (optional; type of the
  * logits; may be them, with the same stride, or share no element with them) receives dloss * dL/dlogits.  (Softened targets are commonly weighted by temperature^2: through dloss.) */

@@ -5,7 +5,9 @@
 //     L = sum_j q_j (ln q_j - ln p_j)                     dL/dz_i = p_i - q_i
 //   tail 1 (bucket): q_j = exp(t_j), and all other tokens are one event of probability r = 1 - sum q, s = sum of the others' p
 //     L = sum_j q_j (ln q_j - ln p_j) + r ln(r / s)       dL/dz_i = p_i - q_i for the k tokens, p_i (1 - r / s) for the others
-// s is summed over the others by themselves (1 - sum p_j would leave nothing of a small one): a bit of LDS per token says which those are.
+// s is summed over the others by themselves (1 - sum p_j would leave nothing of a small one): a bit of LDS per token says which those are.  Their sum is kept against their own largest
+// score m' (or one at most 46 above it), S' = sum exp(z - m'): a student that is sure of the teacher's tokens leaves s far below what fp32 holds, but ln s = m' - m + ln S' - ln S
+// and p_i r / s = exp(z_i - m') r / S' are ordinary numbers, and the only ones that still pull such a student back.
 #include "rows.h"
 #include <algorithm>
 #include <mutex>
@@ -20,6 +22,7 @@ constexpr int COUNTERS = 64;
 constexpr int COUNT_IN_ROWS = 1024;  // up to so many rows each workgroup counts them itself
 constexpr float LEAST_TAIL = 0x1p-20f;  // fp32 log probabilities leave less than this undetermined: a tail below it is none (a student without other tokens would lose infinitely by it)
 constexpr int MAX_BITS = 1 << 20;    // tokens that a workgroup can keep a bit of (128 KB)
+constexpr float FAR_BEHIND = 1e-20f;  // a sum of exponentials below it (46 nats) may have lost terms that count: one of 2^-24 of it is still 10^10 times fp32's least normal number
 
 // Rows that are not left out, in COUNTERS shares (a line of memory a row: one workgroup takes 10 us for 4096 rows, these 5).
 __global__ __launch_bounds__(256) void distill_count_kernel(const int32_t* __restrict__ ids, int64_t T, int k, float* __restrict__ n) {
@@ -116,17 +119,26 @@ __device__ __forceinline__ void teacher_of(const Teacher& teacher, int64_t row, 
   if (lane == 0) l.weight = BUCKET ? sum + r : sum > 0.f ? 1.f : 0.f, l.rest = r;  // sum of all probabilities; 0: nothing to learn
 }
 
-// A row's loss from its statistics (BUCKET: of the other tokens, against the largest score of all), and what its gradient is made of: exp(z - m) * out dz/dx for the other tokens,
-// (exp(z - m) * in - q * scale) dz/dx for the teacher's.  Every wave sums the tokens by itself.
+// A row's loss from its statistics (BUCKET: of the other tokens alone), and what its gradient is made of: exp(z - m_out) * out dz/dx for the other tokens,
+// (exp(z - m) * in - q * scale) dz/dx for the teacher's.  Every wave sums the tokens by itself.  m: the largest level of all, m_out: what the statistics are against.
 struct Factors {
-  float m, out, in, scale;
+  float m, m_out, out, in, scale;
 };
 template <bool CAP, bool BUCKET, int NW>
 __device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, const Scale& c, float scale, float* row_loss) {
   const int lane = threadIdx.x & 63;
   const float weight = l.weight, r = l.rest;
   Factors f;
-  f.m = uniform(a.ref());
+  float most = a.m;
+  if (BUCKET) {
+    float own = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; i++) own = fmaxf(own, l.id[lane + 64 * i] >= 0 ? level<CAP>(l.x[lane + 64 * i], c) : -INFINITY);
+    most = fmaxf(most, wave_max(own));
+  }
+  f.m = uniform(most == -INFINITY ? 0.f : most);
+  f.m_out = uniform(a.ref());
+  const float apart = !BUCKET ? 0.f : CAP ? a.m - f.m : behind<false>(a.m, c, f.m);  // of the two, in scores
   float d[2], inside = 0.f, loss = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
@@ -134,7 +146,7 @@ __device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, c
     d[i] = behind<CAP>(l.x[lane + 64 * i], c, f.m);
     if (BUCKET && mine) inside += exp_of(d[i]);
   }
-  const float sum = uniform(BUCKET ? a.s + wave_sum(inside) : a.s);
+  const float sum = uniform(BUCKET ? __builtin_fmaf(a.s, exp_of(apart), wave_sum(inside)) : a.s);
   const bool none = sum == 0.f;  // no score above minus infinity: no distribution, nothing to learn from
   const float log_sum = log_of(sum);
 #pragma unroll
@@ -143,18 +155,21 @@ __device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, c
     if (q > 0.f) loss += q * (l.logq[lane + 64 * i] - (d[i] - log_sum));
   }
   loss = wave_sum(loss);
-  if (BUCKET && r > 0.f) loss += r * (log_of(r) - (log_of(a.s) - log_sum));
+  if (BUCKET && r > 0.f) {  // r (ln r - ln s); a lead that has no room in fp32 (behind masks of the type's lowest value, at a temperature below 1) may have it times r
+    const float lead = CAP || apart > -INFINITY || a.m == -INFINITY ? r * apart : (r * a.m - r * f.m) * c.unit;
+    loss += r * (log_of(r) - (log_of(a.s) - log_sum)) - lead;
+  }
   if (threadIdx.x == 0) *row_loss = none ? 0.f : loss;
   f.scale = none || weight == 0.f ? 0.f : scale;
   const float inv_sum = none ? 0.f : 1.f / sum;
   f.in = uniform(f.scale * weight * inv_sum);
-  f.out = uniform(f.scale * (weight * inv_sum - (BUCKET && a.s > 1e-30f ? r / a.s : 0.f)));
+  // (without others above minus infinity there is nothing to pull on)
+  f.out = uniform(f.scale * (BUCKET ? weight * inv_sum * exp_of(apart) - (a.s > 0.f ? r / a.s : 0.f) : weight * inv_sum));
   return f;
 }
 template <bool CAP> __device__ __forceinline__ float outside(float x, const Scale& c, const Factors& f) {
-  return exp_behind<CAP>(x, c, f.m) * f.out * slope<CAP>(x, c);
+  return exp_behind<CAP>(x, c, f.m_out) * f.out * slope<CAP>(x, c);
 }
-
 template <bool CAP> __device__ __forceinline__ float inside(float x, float q, const Scale& c, const Factors& f) {
   return (exp_behind<CAP>(x, c, f.m) * f.in - q * f.scale) * slope<CAP>(x, c);
 }
@@ -243,8 +258,10 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
   if (part == 0 && tid < cutting.edges) {
     const float x = (float)zr[cutting.edge(tid, V)];
     const int at = per * N + tid;
-    if (CAP || x > -INFINITY) a.m = level<CAP>(x, c);
-    a.s = BUCKET && (bits[at >> 5] >> (at & 31) & 1) ? 0.f : exp_behind<CAP>(x, c, a.ref());
+    if (!(BUCKET && (bits[at >> 5] >> (at & 31) & 1))) {
+      if (CAP || x > -INFINITY) a.m = level<CAP>(x, c);
+      a.s = exp_behind<CAP>(x, c, a.ref());
+    }
   }
   for (int at = v0; at < v1; at += SPAN) {
     Raw<T, N> now[UNROLL];
@@ -252,11 +269,19 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
     for (int u = 0; u < UNROLL; u++) now[u] = next[u];
     fetch(at + SPAN);
     float most = -INFINITY;
+    unsigned in[UNROLL];  // BUCKET: which elements are the teacher's
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
-      if (at + u * TH + tid >= v1) continue;
+      const int v = at + u * TH + tid, b = v - v0;
+      if (v >= v1) continue;
       float x[N];
       now[u].unpack(x);
+      if (BUCKET) {
+        in[u] = N == 8 ? (unsigned)byte_of[b] : (byte_of[b >> 1] >> (b & 1) * 4) & 15u;
+        if (in[u])
+#pragma unroll
+          for (int e = 0; e < N; e++) x[e] = in[u] >> e & 1 ? -INFINITY : x[e];
+      }
 #pragma unroll
       for (int e = 0; e < N; e++) most = fmaxf(most, x[e]);
     }
@@ -271,13 +296,9 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
       now[u].unpack(x);
 #pragma unroll
       for (int e = 0; e < N; e++) x[e] = exp_behind<CAP>(x[e], c, ref);
-      if (BUCKET) {
-        const int b = v - v0;
-        const unsigned in = N == 8 ? (unsigned)byte_of[b] : (byte_of[b >> 1] >> (b & 1) * 4) & 15u;
-        if (in)
+      if (BUCKET && in[u])
 #pragma unroll
-          for (int e = 0; e < N; e++) x[e] = in >> e & 1 ? 0.f : x[e];
-      }
+        for (int e = 0; e < N; e++) x[e] = in[u] >> e & 1 ? 0.f : x[e];
 #pragma unroll
       for (int w = N / 2; w > 0; w >>= 1)
 #pragma unroll
@@ -378,18 +399,19 @@ __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict
 
   // ---- largest score, sum of exponentials (BUCKET: of the other tokens)
   const unsigned char* byte_of = reinterpret_cast<const unsigned char*>(bits);
-  auto summed = [&](const Raw<T, N>& w, int first, float ref) {  // of vector first + tid; first is even
+  auto hide = [&](float* x, int first, float by) {  // those elements of vector first + tid that are the teacher's; first is even
+    const int at = tid + (cutting.head ? 1 : 0);
+    const unsigned in = N == 8 ? (unsigned)byte_of[at + first] : (byte_of[(at >> 1) + (first >> 1)] >> (at & 1) * 4) & 15u;
+    if (in)
+#pragma unroll
+      for (int e = 0; e < N; e++) x[e] = in >> e & 1 ? by : x[e];
+  };
+  auto summed = [&](const Raw<T, N>& w, int first, float ref) {  // of vector first + tid
     float x[N];
     w.unpack(x);
 #pragma unroll
     for (int e = 0; e < N; e++) x[e] = exp_behind<CAP>(x[e], c, ref);
-    if (BUCKET) {  // which elements of the vector are the teacher's
-      const int at = tid + (cutting.head ? 1 : 0);
-      const unsigned in = N == 8 ? (unsigned)byte_of[at + first] : (byte_of[(at >> 1) + (first >> 1)] >> (at & 1) * 4) & 15u;
-      if (in)
-#pragma unroll
-        for (int e = 0; e < N; e++) x[e] = in >> e & 1 ? 0.f : x[e];
-    }
+    if (BUCKET) hide(x, first, 0.f);
 #pragma unroll
     for (int w2 = N / 2; w2 > 0; w2 >>= 1)
 #pragma unroll
@@ -414,9 +436,7 @@ __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict
     *at = cutting.edge(tid, V);
     return (float)zr[*at];
   };
-  auto edge_sum = [&](float x, int at, float ref) {
-    return BUCKET && (bits[(at + shift) >> 5] >> ((at + shift) & 31) & 1) ? 0.f : exp_behind<CAP>(x, c, ref);
-  };
+  auto is_other = [&](int at) { return !(BUCKET && (bits[(at + shift) >> 5] >> ((at + shift) & 31) & 1)); };
   const bool has_edge = tid < cutting.edges;
   int edge;
   float most = -INFINITY;
@@ -428,19 +448,42 @@ __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict
   }
   most = uniform(block_reduce<NW, true>(most, l.sums));
   Stat a = Stat::none();
-  if (CAP || most > -INFINITY) a.m = level<CAP>(most, c);
-  const float ref = a.ref();
-  float sum = 0.f;
-  if (has_edge) {
-    const float x = edge_value(&edge);
-    sum = edge_sum(x, edge, ref);
-  }
+  auto sum_behind = [&](float most) {
+    a.m = -INFINITY;
+    if (CAP || most > -INFINITY) a.m = level<CAP>(most, c);
+    const float ref = a.ref();
+    float sum = 0.f;
+    if (has_edge) {
+      const float x = edge_value(&edge);
+      if (is_other(edge)) sum = exp_behind<CAP>(x, c, ref);
+    }
 #pragma unroll
-  for (int i = 0; i < HELD; i++) {
-    keep(held[i]);
-    if (i * TH + tid < cutting.nvec) sum += summed(held[i], i * TH, ref);
+    for (int i = 0; i < HELD; i++) {
+      keep(held[i]);
+      if (i * TH + tid < cutting.nvec) sum += summed(held[i], i * TH, ref);
+    }
+    a.s = uniform(block_reduce<NW, false>(sum, l.sums));
+  };
+  sum_behind(most);
+  if (BUCKET && a.s < FAR_BEHIND) {  // (the same for all threads) the teacher's tokens lead by far, so that the others' sum is taken again, against their own largest
+    most = -INFINITY;
+    if (has_edge) {
+      const float x = edge_value(&edge);
+      if (is_other(edge)) most = fmaxf(most, x);
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      keep(held[i]);
+      if (i * TH + tid < cutting.nvec) {
+        float x[N];
+        held[i].unpack(x);
+        hide(x, i * TH, -INFINITY);
+#pragma unroll
+        for (int e = 0; e < N; e++) most = fmaxf(most, x[e]);
+      }
+    }
+    sum_behind(uniform(block_reduce<NW, true>(most, l.sums)));
   }
-  a.s = uniform(block_reduce<NW, false>(sum, l.sums));
   // (a barrier of the reduction lies between the teacher's wave and here)
   float scale = 0.f;
   if (dr) scale = uniform(p.dloss * (p.drow ? p.drow[row] : 1.f) / (p.mean ? l.counted : 1.f));
