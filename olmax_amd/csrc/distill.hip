@@ -124,7 +124,7 @@ __device__ __forceinline__ void teacher_of(const Teacher& teacher, int64_t row, 
 struct Factors {
   float m, m_out, out, in, scale;
 };
-template <bool CAP, bool BUCKET, int NW>
+template <int CAP, bool BUCKET, int NW>
 __device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, const Scale& c, float scale, float* row_loss) {
   const int lane = threadIdx.x & 63;
   const float weight = l.weight, r = l.rest;
@@ -138,7 +138,7 @@ __device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, c
   }
   f.m = uniform(most == -INFINITY ? 0.f : most);
   f.m_out = uniform(a.ref());
-  const float apart = !BUCKET ? 0.f : CAP ? a.m - f.m : behind<false>(a.m, c, f.m);  // of the two, in scores
+  const float apart = !BUCKET ? 0.f : CAP ? a.m - f.m : behind<0>(a.m, c, f.m);  // of the two, in scores
   float d[2], inside = 0.f, loss = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
@@ -167,10 +167,10 @@ __device__ __forceinline__ Factors factors_of(const Stat& a, const Lds<NW>& l, c
   f.out = uniform(f.scale * (BUCKET ? weight * inv_sum * exp_of(apart) - (a.s > 0.f ? r / a.s : 0.f) : weight * inv_sum));
   return f;
 }
-template <bool CAP> __device__ __forceinline__ float outside(float x, const Scale& c, const Factors& f) {
+template <int CAP> __device__ __forceinline__ float outside(float x, const Scale& c, const Factors& f) {
   return exp_behind<CAP>(x, c, f.m_out) * f.out * slope<CAP>(x, c);
 }
-template <bool CAP> __device__ __forceinline__ float inside(float x, float q, const Scale& c, const Factors& f) {
+template <int CAP> __device__ __forceinline__ float inside(float x, float q, const Scale& c, const Factors& f) {
   return (exp_behind<CAP>(x, c, f.m) * f.in - q * f.scale) * slope<CAP>(x, c);
 }
 
@@ -207,7 +207,7 @@ template <typename TO, int TH> __device__ __forceinline__ void write_zeros(TO* d
 
 // Rows that no workgroup holds, and few rows: two launches of shares of rows.  The first leaves statistics (BUCKET: sums of the other tokens) of each share, and the teacher's tokens'
 // logits; or (part_stat null) the loss of whole rows, and there is no second.  700 x 128256 fp32: 60 us, 6.0 TB/s.
-template <typename T, bool CAP, bool BUCKET, int TH>
+template <typename T, int CAP, bool BUCKET, int TH>
 __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__ logits, const RowArgs p, const Scale c, Stat* __restrict__ part_stat, int parts) {
   constexpr int N = Vec<T>::N, UNROLL = 4, SPAN = TH * UNROLL;
   extern __shared__ unsigned bits[];  // BUCKET: of the teacher's tokens in the share, the row's single elements behind its vectors
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(TH) void distill_stats_kernel(const T* __restrict__
 }
 
 // The second joins them (every workgroup for itself), writes the loss, and the gradient of one of `shares` shares of the row.
-template <typename T, typename TO, bool CAP, bool BUCKET>
+template <typename T, typename TO, int CAP, bool BUCKET>
 __global__ __launch_bounds__(256) void distill_grads_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const RowArgs p, const Scale c,
                                                             const Stat* __restrict__ part_stat, int parts, int shares) {
   constexpr int N = Vec<TO>::N, TH = 256, NW = TH / 64;
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void distill_grads_kernel(const T* __restrict_
 // One workgroup a row, of which a thread keeps HELD vectors in registers: statistics and the loss, then the gradient of all tokens, then the k tokens' own.
 // Each logit is read once and its gradient written once, and no exponential is kept: those of the gradient are taken again.  4096 x 100352 bf16 to bf16: 329 us with the count and the sum, 5.0 TB/s (a copy:
 // 5.2), the vector unit busy for 60 %: the rows of a CU, of which registers hold two, read and write in turns that overlap only with each other's.
-template <typename T, typename TO, bool CAP, bool BUCKET, int TH, int HELD>
+template <typename T, typename TO, int CAP, bool BUCKET, int TH, int HELD>
 __global__ __launch_bounds__(TH, 4) void distill_rows_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const RowArgs p, const Scale c) {
   constexpr int N = Vec<TO>::N, NW = TH / 64;
   extern __shared__ unsigned bits[];  // BUCKET
@@ -589,7 +589,8 @@ static int distill(hipStream_t stream, const void* logits, void* dlogits, const 
   auto go = [&](auto in, auto out, auto capped, auto bucket) {
     using TY = decltype(in);
     using TO = decltype(out);
-    constexpr bool CAP = decltype(capped)::value, BUCKET = decltype(bucket)::value, WIDE = sizeof(TY) != sizeof(TO);
+    constexpr int CAP = decltype(capped)::value;
+    constexpr bool BUCKET = decltype(bucket)::value, WIDE = sizeof(TY) != sizeof(TO);
     if (form.threads == 256) HELD(256, 8);
     else if (form.threads == 512) HELD(512, WIDE ? 13 : 25);
     else if (form.threads == 1024) HELD(1024, WIDE ? 13 : sizeof(TO) == 2 ? 20 : 25);
@@ -605,10 +606,10 @@ static int distill(hipStream_t stream, const void* logits, void* dlogits, const 
 #undef HELD
 #undef LAUNCH
   auto kind = [&](auto in, auto out) {
-    const std::true_type yes;
-    const std::false_type no;
-    if (softcap > 0.f) tail ? go(in, out, yes, yes) : go(in, out, yes, no);
-    else tail ? go(in, out, no, yes) : go(in, out, no, no);
+    auto tails = [&](auto capped) { tail ? go(in, out, capped, std::true_type()) : go(in, out, capped, std::false_type()); };
+    if (c.kind == 0) tails(std::integral_constant<int, 0>());
+    else if (c.kind == 1) tails(std::integral_constant<int, 1>());
+    else tails(std::integral_constant<int, 2>());
   };
   if (logits_f32 && grads_f32) kind(0.f, 0.f);
   else if (logits_f32) kind(0.f, bf16());

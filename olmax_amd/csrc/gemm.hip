@@ -88,7 +88,8 @@ std::mutex g_prof_mu;
 //
 // EPI == 7 and 8 form a row's part of the softmax of the LM head's logits from the accumulators (HeadRows): 7 the statistics of each row over the tile's 256 columns
 // (largest score, sum of exponentials, entropy's sum) and the targets' logits, 8 the logits' gradient in their place.  A lane has 16 of a row's 64 columns in a wave, four lanes
-// share a row, four waves a tile's: two exchanges between lanes and one through LDS.  An exponential costs the vector unit about what one k-tile's issue does; of the 100 us that a
+// share a row, four waves a tile's: two exchanges between lanes and one through LDS.  9 and 10 are 7 and 8 for soft-caps above WIDE_CAP (as a third branch in these: 2048 x 256 x 100352 without one
+// 197 us -> 202).  An exponential costs the vector unit about what one k-tile's issue does; of the 100 us that a
 // round of tiles of K = 4096 takes they are 3.
 //
 // RAG: 1 where M or N, 2 where K is not a multiple of the tile.  The last tile of a row or column is
@@ -113,7 +114,7 @@ __device__ __forceinline__ void gemm_tile(
   constexpr bool GLU_BWD = EPI == 4 || EPI == 5;
   constexpr bool ROPE = EPI == 3;
   constexpr bool SPLIT = EPI == 6;
-  constexpr bool ROW_STATS = EPI == 7, ROW_GRADS = EPI == 8;
+  constexpr bool ROW_STATS = EPI == 7 || EPI == 9, ROW_GRADS = EPI == 8 || EPI == 10, WIDE_SOFTCAP = EPI >= 9;
   static_assert(EPI == 0 || SPLIT || (BN == 256 && WN == 64 && B_KC && !HAS_RES && !OUT_F32), "fused epilogues: 256-wide NT tiles only");
   constexpr int NW = (BM / WM) * (BN / WN);
   constexpr int TM = WM / 16, TN = WN / 16;  // accumulators of 16x16 per wave
@@ -692,7 +693,7 @@ __device__ __forceinline__ void gemm_tile(
     const int first = wn * WN + g16e * 4;  // this lane's first column of the block
     auto here = [&](int j, int r) { return !RAG || first + j * 16 + r >= col_lo; };
     auto of_row = [&](auto capped, const f32x4* x, int row, int target) {
-      constexpr bool CAP = decltype(capped)::value;
+      constexpr int CAP = decltype(capped)::value;
       float most = -INFINITY;
 #pragma unroll
       for (int j = 0; j < TN; j++)
@@ -730,8 +731,9 @@ __device__ __forceinline__ void gemm_tile(
 #pragma unroll
     for (int i = 0; i < TM; i++) {
       const int row = wm * WM + i * 16 + l16e;
-      if (cap) of_row(std::true_type(), acc[i], row, targets[i]);
-      else of_row(std::false_type(), acc[i], row, targets[i]);
+      if (WIDE_SOFTCAP) of_row(std::integral_constant<int, WIDE_SOFTCAP ? 2 : 0>(), acc[i], row, targets[i]);
+      else if (cap) of_row(std::integral_constant<int, 1>(), acc[i], row, targets[i]);
+      else of_row(std::integral_constant<int, 0>(), acc[i], row, targets[i]);
     }
     __syncthreads();
     if (tid < BM && stores_row(tid)) {
@@ -748,7 +750,7 @@ __device__ __forceinline__ void gemm_tile(
     const bool cap = c.cap > 0.f;
     const int first = n0 + wn * WN + g16e * 4;
     auto of_row = [&](auto capped, f32x4* x, int64_t row) {
-      constexpr bool CAP = decltype(capped)::value;
+      constexpr int CAP = decltype(capped)::value;
       const bool there = row < head->rows;
       const float m = there ? head->stats[row * 3] : -INFINITY, log_sum = there ? head->stats[row * 3 + 1] : 0.f, entropy = there ? head->stats[row * 3 + 2] : 0.f;
       const int target = there ? head->targets[row] : -1;
@@ -765,8 +767,9 @@ __device__ __forceinline__ void gemm_tile(
 #pragma unroll
     for (int i = 0; i < TM; i++) {
       const int64_t row = m0 + wm * WM + i * 16 + l16e;
-      if (cap) of_row(std::true_type(), acc[i], row);
-      else of_row(std::false_type(), acc[i], row);
+      if (WIDE_SOFTCAP) of_row(std::integral_constant<int, WIDE_SOFTCAP ? 2 : 0>(), acc[i], row);
+      else if (cap) of_row(std::integral_constant<int, 1>(), acc[i], row);
+      else of_row(std::integral_constant<int, 0>(), acc[i], row);
     }
   }
   if (GLU) {
@@ -1155,7 +1158,7 @@ int launch_head(hipStream_t s, const bf16* A, const bf16* B, bf16* C, int M, int
   if (g_prof_on) {
     (void)hipEventRecord(rec.e1, s);
     rec.flops = 2.0 * M * N * K;
-    rec.bytes = 2.0 * ((double)M * K + (double)N * K + (EPI == 8 ? (double)M * N : 0.0));
+    rec.bytes = 2.0 * ((double)M * K + (double)N * K + (C ? (double)M * N : 0.0));
     rec.key = 256 | (1 << 12) | (1 << 13) | (1 << 20);
     rec.M = M; rec.N = N; rec.K = K;
     std::lock_guard<std::mutex> lk(g_prof_mu);
@@ -1657,10 +1660,10 @@ int olmax_gemm_head_columns(int M, int N, int K) {
   return cut.cn ? cut.cn * 256 : N;
 }
 int olmax_gemm_head_stats(hipStream_t s, const bf16* h, const bf16* w, int M, int N, int K, const HeadRows& rows) {
-  return launch_head<7>(s, h, w, nullptr, M, N, K, 0, rows);
+  return rows.scale.kind == 2 ? launch_head<9>(s, h, w, nullptr, M, N, K, 0, rows) : launch_head<7>(s, h, w, nullptr, M, N, K, 0, rows);
 }
 int olmax_gemm_head_grads(hipStream_t s, const bf16* h, const bf16* w, bf16* d, int64_t ldd, int M, int N, int K, const HeadRows& rows) {
-  return launch_head<8>(s, h, w, d, M, N, K, ldd, rows);
+  return rows.scale.kind == 2 ? launch_head<10>(s, h, w, d, M, N, K, ldd, rows) : launch_head<8>(s, h, w, d, M, N, K, ldd, rows);
 }
 
 // The two products of olmax_gemm_grads as one launch: what it costs in each kernel that can run it.  Measured, with the two calls, on 312

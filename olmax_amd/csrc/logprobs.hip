@@ -172,7 +172,7 @@ __device__ __forceinline__ void write_skipped(const Out& o, int64_t row, int k) 
 }
 // a: statistics of the whole row, x: the target's logit, if there is one.  A row without a score above minus infinity has no distribution: log probabilities of minus
 // infinity, entropy 0.  By one thread.
-template <bool CAP>
+template <int CAP>
 __device__ __forceinline__ void write_row(const Out& o, int64_t row, bool has_target, float x, const Scale& c, const Stat& a) {
   const bool none = a.s == 0.f;
   const float log_sum = log_of(a.s), entropy = none ? 0.f : log_sum - a.t / a.s;
@@ -185,7 +185,7 @@ __device__ __forceinline__ void write_row(const Out& o, int64_t row, bool has_ta
   o.stats[row * 3 + 2] = entropy;
 }
 // The n <= k largest logits above minus infinity are cand[0 .. n) or are the largest of them; the rest of k slots gets the lowest indices that are not among them.
-template <bool CAP, int TH>
+template <int CAP, int TH>
 __device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, uint64_t* cand, int n, const Scale& c, const Stat& a) {
   int32_t* ids = o.top_ids + row * k;
   float* lp = o.top_logprobs + row * k;
@@ -215,7 +215,7 @@ __device__ __forceinline__ void write_top(const Out& o, int64_t row, int k, uint
 // The row is read once, a chunk of four vectors a thread ahead of the one in work; the largest score of a chunk is known before its exponentials, which are taken against the
 // largest so far.  3596 x 100352 bf16: 124 us, 5.8 TB/s, the vector unit busy for 90 % of it (a copy on the card reads and writes 5.2).  1500 x 256000 with a soft-cap and 64
 // alternatives: 196 us, 3.9 TB/s; 19 issue slots a logit, six of them its three transcendental instructions, keep the vector unit busy for 88 %.
-template <typename T, bool CAP, bool TOP, int TH>
+template <typename T, int CAP, bool TOP, int TH>
 __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out, uint64_t* __restrict__ part_top,
                                                         Stat* __restrict__ part_stat, int V, int64_t ld, int32_t ignore_index, Scale c, int k, int parts, bool once) {
   constexpr int N = Vec<T>::N, SPAN = TH * UNROLL;
@@ -298,8 +298,8 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
       now[u].unpack(x);
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        if (CAP) {  // scores are finite and small: in units of log 2, without a cut (three of 22 issue slots of a logit; these rows are bound by them)
-          const float d = __builtin_fmaf(tail_of_tanh(x[e], c), cap_r, cap_top);
+        if (CAP) {  // scores are finite: in units of log 2, without a cut (three of 22 issue slots of a logit; these rows are bound by them)
+          const float d = CAP == 1 ? __builtin_fmaf(tail_of_tanh(x[e], c), cap_r, cap_top) : behind<CAP>(x[e], c, ref) * LOG2E;
           x[e] = __builtin_amdgcn_exp2f(d);
           t[e & 1] = __builtin_fmaf(x[e], d, t[e & 1]);
         } else {
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(TH) void score_rows_kernel(const T* __restrict__ lo
 }
 
 // The parts of a row, one workgroup a row.
-template <typename T, bool CAP, bool TOP, int TH = 256>
+template <typename T, int CAP, bool TOP, int TH = 256>
 __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ logits, const int32_t* __restrict__ targets, Out out,
                                                         const uint64_t* __restrict__ part_top, const Stat* __restrict__ part_stat, int V, int64_t ld,
                                                         int32_t ignore_index, Scale c, int k, int parts) {
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(TH) void score_join_kernel(const T* __restrict__ lo
 // The rows of an LM head whose product left statistics of 256 columns a tile (olmax_gemm_head_stats), [tiles][ld_tiles], and, for the last columns, logits (`rest`, from column
 // `fused` on) with statistics of their own: 16 rows a workgroup, each sixteenth of a wave takes every 64th tile.  (64 rows a workgroup, a lane each: 20 us for 2048 rows of
 // 384 tiles, so 8.)
-template <bool CAP>
+template <int CAP>
 __global__ __launch_bounds__(1024) void head_join_kernel(const Stat* __restrict__ tiles, int n_tiles, const Stat* __restrict__ rest_stat, const float* __restrict__ rest,
                                                          int64_t ld_rest, const float* __restrict__ target_logit, const int32_t* __restrict__ targets, Out out, int64_t rows,
                                                          int64_t ld_tiles, int V, int fused, int32_t ignore_index, Scale c) {
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(256) void zero_columns_kernel(bf16* __restrict__ d,
 // d loss / d logits of logprob and entropy: dz_i = g (delta_it - p_i) - h p_i (ln p_i + H), from the statistics that the forward pass kept.
 // Reads and writes each logit once, without any wait between threads: 4096 x 50304 bf16 159 us, 5.2 TB/s, as a copy; 333 x 100278 fp32 46 us, 5.8 TB/s.
 // A workgroup takes one of `parts` shares of a row.  first: the column of the whole row that these logits begin with (they are its last).
-template <typename T, typename TO, bool CAP, bool ENT, bool ONCE, int TH = 256>
+template <typename T, typename TO, int CAP, bool ENT, bool ONCE, int TH = 256>
 __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ logits, TO* __restrict__ dlogits, const int32_t* __restrict__ targets,
                                                         const float* __restrict__ stats, const float* __restrict__ dlogprobs,
                                                         const float* __restrict__ dentropy, int V, int64_t ld, int64_t ldd, int32_t ignore_index, Scale c,
@@ -583,7 +583,7 @@ extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, 
                          (const uint64_t*)part_top, (const Stat*)part_stat, V, ld, ignore_index, c, top, parts);                                          \
   } while (0)
 #define SCORE_T(TY, CAPV) do { if (top) SCORE(TY, CAPV, true); else SCORE(TY, CAPV, false); } while (0)
-#define SCORE_C(TY) do { if (softcap > 0.f) SCORE_T(TY, true); else SCORE_T(TY, false); } while (0)
+#define SCORE_C(TY) do { if (c.kind == 0) SCORE_T(TY, 0); else if (c.kind == 1) SCORE_T(TY, 1); else SCORE_T(TY, 2); } while (0)
   if (logits_f32) SCORE_C(float); else SCORE_C(bf16);
 #undef ROWS
 #undef SCORE
@@ -612,8 +612,10 @@ static int token_logprobs_bwd(hipStream_t stream, const void* logits, const int3
     const std::true_type yes;
     const std::false_type no;
     auto loads = [&](auto capped, auto entropies) { past_cache ? go(in, out, capped, entropies, yes) : go(in, out, capped, entropies, no); };
-    if (softcap > 0.f) dentropy ? loads(yes, yes) : loads(yes, no);
-    else dentropy ? loads(no, yes) : loads(no, no);
+    auto entropies = [&](auto capped) { dentropy ? loads(capped, yes) : loads(capped, no); };
+    if (c.kind == 0) entropies(std::integral_constant<int, 0>());
+    else if (c.kind == 1) entropies(std::integral_constant<int, 1>());
+    else entropies(std::integral_constant<int, 2>());
   };
   if (logits_f32 && grads_f32) kind(0.f, 0.f);
   else if (logits_f32) kind(0.f, bf16());
@@ -712,15 +714,16 @@ extern "C" int32_t olmax_lmhead_logprobs(hipStream_t stream, const void* h, cons
   rows.target_logit = target_logit;
   if (int rc = olmax_gemm_head_stats(stream, hp, wp, (int)p.rows, p.fused, d, rows)) return rc;
   auto join = [&](auto capped) {
-    constexpr bool CAP = decltype(capped)::value;
+    constexpr int CAP = decltype(capped)::value;
     if (rest)
       hipLaunchKernelGGL((score_rows_kernel<float, CAP, false, 256>), dim3((unsigned)T), dim3(256), 0, stream, (const float*)ws, targets, out, (uint64_t*)nullptr, rest_stat, rest,
                          p.ld, ignore_index, c, 0, 1, false);
     hipLaunchKernelGGL((head_join_kernel<CAP>), dim3((unsigned)((T + 15) / 16)), dim3(1024), 0, stream, (const Stat*)tiles, (p.fused + 255) / 256, (const Stat*)rest_stat,
                        (const float*)ws, p.ld, (const float*)target_logit, targets, out, T, p.rows, V, p.fused, ignore_index, c);
   };
-  if (softcap > 0.f) join(std::true_type());
-  else join(std::false_type());
+  if (c.kind == 0) join(std::integral_constant<int, 0>());
+  else if (c.kind == 1) join(std::integral_constant<int, 1>());
+  else join(std::integral_constant<int, 2>());
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }

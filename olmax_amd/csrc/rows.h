@@ -77,15 +77,24 @@ template <typename T, int N> __device__ __forceinline__ Cut cut(const T* row, in
   return c;
 }
 
-// tanh(x / softcap) = 1 - 2 r, r = 1 / (exp(2 x / softcap) + 1), so that a capped score is one fma on r, and its slope dy / dx is 4 r (1 - r)
+// tanh(x / softcap) = 1 - 2 r, r = 1 / (exp(2 x / softcap) + 1), so that a capped score is one fma on r, and its slope dy / dx is 4 r (1 - r).  That is off by softcap 2^-21 / temperature
+// whatever the score, so that a soft-cap far above the logits would leave nothing of them: above WIDE_CAP scores of |x| < softcap / 4 are x (1 - y^2 / 3 + 2 y^4 / 15 - ..) / temperature, y = x /
+// softcap (the series left off behind y^8: 8.4e-9 of it at most), and all are as exact as they are large: 2^-19 of themselves.  The series and the choice are ten more issue slots a logit; us
+// with scores of the first kind | of the second, bf16: 1500 x 256000 with 64 alternatives 203 | 214, its gradient 308 | 367, distillation of 4096 x 100352 407 | 533, the LM head's scores of 2048 x 4096
+// x 100352 1237 | 1260, x 256 227 | 257.
+constexpr float WIDE_CAP = 64.f;
 struct Scale {
+  int kind;                   // of the kernels that run: 0 no soft-cap, 1 up to WIDE_CAP, 2 above (CAP)
   float cap, cap_k, inv_tau;  // cap_k = 2 log2(e) / cap; cap 0: none
+  float inv_cap;
   float r_k, top;             // a capped score is r_k r + top: r_k = -2 cap / temperature, top = cap / temperature
   float unit, unit2;          // of a level (see level), in scores: 1, or 1 / temperature; and in powers of two
 };
 inline Scale scale_of(float temperature, float softcap) {
   Scale c;
+  c.kind = softcap > WIDE_CAP ? 2 : softcap > 0.f ? 1 : 0;
   c.cap = softcap;
+  c.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
   c.cap_k = softcap > 0.f ? 2.f * LOG2E / softcap : 0.f;
   c.inv_tau = 1.f / temperature;
   c.top = softcap * c.inv_tau;
@@ -97,24 +106,32 @@ inline Scale scale_of(float temperature, float softcap) {
 __device__ __forceinline__ float tail_of_tanh(float x, const Scale& c) { return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * c.cap_k) + 1.f); }
 // What rows are compared by, and exponentials are taken against: capped scores, or the logits themselves, whose scores may have no room in fp32 (the type's lowest value at a
 // temperature below 1) where their differences have.
-template <bool CAP> __device__ __forceinline__ float level(float x, const Scale& c) { return CAP ? __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top) : x; }
+template <int CAP> __device__ __forceinline__ float level(float x, const Scale& c) {
+  if (CAP == 0) return x;
+  const float far = __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top);
+  if (CAP == 1) return far;
+  const float y = x * c.inv_cap, y2 = y * y, z = x * c.inv_tau;
+  const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(62.f / 2835.f, y2, -17.f / 315.f), y2, 2.f / 15.f), y2, -1.f / 3.f) * y2;
+  return fabsf(y) < 0.25f ? __builtin_fmaf(z, p, z) : far;
+}
 // a value that all threads of the workgroup have, in a scalar register
 __device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 // z - m, m the score of level m
-template <bool CAP> __device__ __forceinline__ float behind(float x, const Scale& c, float m) {
-  if (CAP) return __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top - m);
+template <int CAP> __device__ __forceinline__ float behind(float x, const Scale& c, float m) {
+  if (CAP == 1) return __builtin_fmaf(tail_of_tanh(x, c), c.r_k, c.top - m);
+  if (CAP == 2) return level<2>(x, c) - m;
   const float d = (x - m) * c.unit;
   return d == -INFINITY && x > -INFINITY ? __builtin_fmaf(x, c.unit, -m * c.unit) : d;  // (at a temperature above 1 the scores may have the room that the logits have not)
 }
 // dz / dx
-template <bool CAP> __device__ __forceinline__ float slope(float x, const Scale& c) {
+template <int CAP> __device__ __forceinline__ float slope(float x, const Scale& c) {
   if (!CAP) return c.inv_tau;
   const float r = tail_of_tanh(x, c);
   return 4.f * r * (1.f - r) * c.inv_tau;
 }
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 // exp(z - m)
-template <bool CAP> __device__ __forceinline__ float exp_behind(float x, const Scale& c, float m) {
+template <int CAP> __device__ __forceinline__ float exp_behind(float x, const Scale& c, float m) {
   return CAP ? exp_of(behind<CAP>(x, c, m)) : __builtin_amdgcn_exp2f((x - m) * c.unit2);
 }
 __device__ __forceinline__ float log_of(float s) { return __builtin_amdgcn_logf(s) * LN2; }
@@ -174,7 +191,7 @@ template <int NW> __device__ __forceinline__ Stat block_join(Stat a, Stat* red, 
 
 // d / d x of g ln p[target] + h entropy: (g (i == target) - p (g + h (ln p + H))) dz/dx, from the row's m (a score, as
 // stats hold it), ln S and H
-template <bool CAP, bool ENT>
+template <int CAP, bool ENT>
 __device__ __forceinline__ float score_grad(float x, const Scale& c, float m, float log_sum, float entropy, float g, float h, bool target) {
   const float logp = (CAP ? behind<CAP>(x, c, m) : __builtin_fmaf(x, c.inv_tau, -m)) - log_sum;
   float d = -exp_of(logp) * (ENT ? __builtin_fmaf(h, fmaxf(logp, -200.f) + entropy, g) : g);
