@@ -198,8 +198,9 @@ int32_t olmax_cross_entropy_reduce(olmax_stream_t stream, const void* logits, vo
 
 /* ---- Log probabilities of given tokens, beside the cross entropy: what evaluation, policy-gradient losses and a teacher's pass take
  * from logits.  No counterpart in the reference (its cross_entropy_loss, src/olmax/nn/functional.py:70-91, returns -logprob of the labels).
- * z = cap(x) / temperature, cap(x) = softcap * tanh(x / softcap) where softcap > 0; p = softmax(z) over the V logits of a row.  With a soft-cap of up to 64 a score is off by
- * softcap 2^-21 / temperature at most, above by 2^-19 of itself (2^-22 where |x| < softcap / 4).
+ * z = cap(x) / temperature, cap(x) = softcap * tanh(x / softcap) where softcap > 0 (1e-30 to 1e30; the temperature is 1e-6 to 1e6); p = softmax(z) over
+ * the V logits of a row.  With a soft-cap of up to 64 a score is off by softcap 2^-21 / temperature at most, above by 2^-19 of itself (2^-22 where
+ * |x| < softcap / 4).
  * logprobs [T] (optional; needs targets) = ln p[target], 0 for a target outside [0, V); entropy [T] = - sum p ln p;
  * stats [T, 3] = {m = max z, ln sum exp(z - m), entropy}, what the backward call takes (its first two add up to the log-normaliser).  m is
  * rounded: gradients of scores beyond 2^20 at a temperature that is no power of two are off by 2^-24 |m|, and a row all of whose scores

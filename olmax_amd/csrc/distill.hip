@@ -558,7 +558,7 @@ static int distill_check(const char* name, int64_t T, int32_t V, int32_t k, int3
   OLMAX_CHECK(T > 0 && V > 0 && V < (1 << 30) && T < (1LL << 24), OLMAX_ERR_SHAPE, "%s: bad shape T=%ld V=%d", name, (long)T, V);
   OLMAX_CHECK(k >= 1 && k <= MAX_TOP, OLMAX_ERR_ARG, "%s: 1 to %d tokens of the teacher a row (got %d)", name, MAX_TOP, k);
   OLMAX_CHECK(tail == 0 || (tail == 1 && V <= MAX_BITS - 32), OLMAX_ERR_ARG, "%s: tail must be 0 (renormalize) or 1 (bucket, up to %d logits)", name, MAX_BITS - 32);
-  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "%s: temperature within 1e-6 and 1e6, softcap not negative", name);
+  OLMAX_CHECK(takes(temperature, softcap), OLMAX_ERR_ARG, "%s: temperature within 1e-6 and 1e6, softcap 0 or within 1e-30 and 1e30", name);
   return OLMAX_OK;
 }
 

@@ -561,7 +561,7 @@ extern "C" int32_t olmax_token_logprobs(hipStream_t stream, const void* logits, 
   OLMAX_CHECK(T > 0 && V > 0 && V < (1 << 30) && ld >= V && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_token_logprobs: bad shape T=%ld V=%d ld=%ld", (long)T, V, (long)ld);
   OLMAX_CHECK(top >= 0 && top <= MAX_TOP && top <= V && (top == 0 || (top_ids && top_logprobs)), OLMAX_ERR_ARG,
               "olmax_token_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, top);
-  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_token_logprobs: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(takes(temperature, softcap), OLMAX_ERR_ARG, "olmax_token_logprobs: temperature within 1e-6 and 1e6, softcap 0 or within 1e-30 and 1e30");
   OLMAX_CHECK(((uintptr_t)logits & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_token_logprobs: logits not aligned to their type");
   const Form form = form_of(T, V, top, logits_f32 != 0);
   const int parts = form.parts;
@@ -629,7 +629,7 @@ extern "C" int32_t olmax_token_logprobs_bwd(hipStream_t stream, const void* logi
                                             int32_t ignore_index, float temperature, float softcap) {
   OLMAX_CHECK(logits && targets && stats && dlogprobs && dlogits, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: null pointer");
   OLMAX_CHECK(T > 0 && V > 0 && V < (1 << 30) && ld >= V && ldd >= V && T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_token_logprobs_bwd: bad shape T=%ld V=%d", (long)T, V);
-  OLMAX_CHECK(temperature >= 1e-6f && temperature <= 1e6f && softcap >= 0.f && softcap <= 1e30f, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(takes(temperature, softcap), OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: temperature within 1e-6 and 1e6, softcap 0 or within 1e-30 and 1e30");
   OLMAX_CHECK((((uintptr_t)logits | (uintptr_t)dlogits) & (logits_f32 ? 3 : 1)) == 0, OLMAX_ERR_ALIGN, "olmax_token_logprobs_bwd: operands not aligned to their type");
   OLMAX_CHECK(logits != dlogits || ld == ldd, OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: in place wants one row stride");
   OLMAX_CHECK(!overlap(logits, ld, dlogits, ldd, T, V, logits_f32 ? 4 : 2), OLMAX_ERR_ARG, "olmax_token_logprobs_bwd: the gradient overlaps the logits, but is not in their place");
@@ -672,8 +672,8 @@ int olmax_lmhead_logprobs_check(const HeadScore& a) {
   OLMAX_CHECK(a.T > 0 && a.d > 0 && a.V > 0 && a.V < (1 << 30) && a.T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs: bad shape T=%ld d=%d V=%d", (long)a.T, a.d, a.V);
   OLMAX_CHECK(a.top >= 0 && a.top <= MAX_TOP && a.top <= a.V && (a.top == 0 || (a.top_ids && a.top_logprobs)), OLMAX_ERR_ARG,
               "olmax_lmhead_logprobs: 0 to %d alternatives, not more than there are logits, with both outputs (got %d)", MAX_TOP, a.top);
-  OLMAX_CHECK(a.temperature >= 1e-6f && a.temperature <= 1e6f && a.softcap >= 0.f && a.softcap <= 1e30f, OLMAX_ERR_ARG,
-              "olmax_lmhead_logprobs: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(takes(a.temperature, a.softcap), OLMAX_ERR_ARG,
+              "olmax_lmhead_logprobs: temperature within 1e-6 and 1e6, softcap 0 or within 1e-30 and 1e30");
   OLMAX_CHECK(aligned16(a.h) && aligned16(a.W), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs: h and W must be 16-byte aligned");
   const int64_t need = head_plan(a.T, a.d, a.V, a.top).bytes;
   OLMAX_CHECK(a.workspace_bytes >= need && (((uintptr_t)a.workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs: workspace needs %ld bytes, 256-byte aligned", (long)need);
@@ -755,8 +755,8 @@ extern "C" int64_t olmax_lmhead_logprobs_bwd_workspace_bytes(int64_t T, int32_t 
 int olmax_lmhead_logprobs_bwd_check(const HeadScoreGrad& a) {
   OLMAX_CHECK(a.h && a.W && a.targets && a.stats && a.dlogprobs && a.workspace && (a.dh || a.dW), OLMAX_ERR_ARG, "olmax_lmhead_logprobs_bwd: null pointer");
   OLMAX_CHECK(a.T > 0 && a.d > 0 && a.V > 0 && a.V < (1 << 30) && a.T < (1LL << 24), OLMAX_ERR_SHAPE, "olmax_lmhead_logprobs_bwd: bad shape T=%ld d=%d V=%d", (long)a.T, a.d, a.V);
-  OLMAX_CHECK(a.temperature >= 1e-6f && a.temperature <= 1e6f && a.softcap >= 0.f && a.softcap <= 1e30f, OLMAX_ERR_ARG,
-              "olmax_lmhead_logprobs_bwd: temperature within 1e-6 and 1e6, softcap not negative");
+  OLMAX_CHECK(takes(a.temperature, a.softcap), OLMAX_ERR_ARG,
+              "olmax_lmhead_logprobs_bwd: temperature within 1e-6 and 1e6, softcap 0 or within 1e-30 and 1e30");
   OLMAX_CHECK(aligned16(a.h) && aligned16(a.W) && aligned16(a.dh), OLMAX_ERR_ALIGN, "olmax_lmhead_logprobs_bwd: h, W and dh must be 16-byte aligned");
   const int64_t need = head_grad_plan(a.T, a.d, a.V).bytes;
   OLMAX_CHECK(a.workspace_bytes >= need && (((uintptr_t)a.workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_lmhead_logprobs_bwd: workspace needs %ld bytes, 256-byte aligned",

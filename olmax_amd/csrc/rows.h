@@ -90,6 +90,8 @@ struct Scale {
   float r_k, top;             // a capped score is r_k r + top: r_k = -2 cap / temperature, top = cap / temperature
   float unit, unit2;          // of a level (see level), in scores: 1, or 1 / temperature; and in powers of two
 };
+// (a soft-cap below 8.5e-39 has no factor of x in fp32: 0 would become NaN)
+inline bool takes(float temperature, float softcap) { return temperature >= 1e-6f && temperature <= 1e6f && (softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f)); }
 inline Scale scale_of(float temperature, float softcap) {
   Scale c;
   c.kind = softcap > WIDE_CAP ? 2 : softcap > 0.f ? 1 : 0;
