@@ -1468,9 +1468,9 @@ static SmallForm small_form(int M, int N, int K, bool a_kc, bool b_kc, bool forc
   return {edge, n64 <= 256 && (edge == 64 || kt > 4) ? 8 : 4};
 }
 // Whether the direct-to-LDS kernels can take the operands: whole 16-byte chunks everywhere, i.e. aligned rows, and a chunk never crosses the end
-// of a row (a_padded: see olmax_gemm_padded).
+// of a row (a_padded: see olmax_gemm_padded); a lane's offset within an instruction's up to 64 rows is 32 bits of bytes.
 static bool direct(const bf16* a, const bf16* b, int M, int N, int K, int64_t lda, int64_t ldb, bool a_kc, bool b_kc, bool a_padded) {
-  return aligned16(a) && aligned16(b) && lda % 8 == 0 && ldb % 8 == 0 && (a_padded || (a_kc ? K : M) % 8 == 0) && (b_kc ? K : N) % 8 == 0;
+  return aligned16(a) && aligned16(b) && lda < (1 << 25) && ldb < (1 << 25) && lda % 8 == 0 && ldb % 8 == 0 && (a_padded || (a_kc ? K : M) % 8 == 0) && (b_kc ? K : N) % 8 == 0;
 }
 
 // Wave quantisation: with one 256x256 tile per CU per round, a last round that fills less
@@ -1651,7 +1651,7 @@ int olmax_gemm_padded(hipStream_t stream, const bf16* a, const bf16* b, void* C,
 }
 
 int olmax_gemm_head_columns(int M, int N, int K) {
-  if (M < 256 || N < 256 || K < BK || K % 8) return 0;
+  if (M < 256 || N < 256 || K < BK || K % 8 || K >= (1 << 25)) return 0;
   int parts;
   float cost;
   if (pick_tile(M, N, K, true, true, true, 0, &parts, &cost) != 256) return 0;
