@@ -252,7 +252,7 @@ int32_t olmax_lmhead_ce(olmax_stream_t stream, const void* h, const void* W, con
                         int32_t dw_f32);
 
 /* The LM head with olmax_token_logprobs, its backward pass, and with olmax_distill (reduction mean): h [T, d], W [V, d] bf16, they and dh
- * 16-byte aligned, the logits h W^T summed and kept in fp32.  The backward call runs the product again.  dh [T, d] bf16 and dW [V, d] (bf16, or fp32 with
+ * 16-byte aligned, the logits h W^T summed and kept in fp32, their gradient rounded to bf16 in front of its two products.  The backward call runs the product again.  dh [T, d] bf16 and dW [V, d] (bf16, or fp32 with
  * dw_f32 != 0) may be NULL to skip. */
 int64_t olmax_lmhead_logprobs_workspace_bytes(int64_t T, int32_t d, int32_t V, int32_t top);
 int32_t olmax_lmhead_logprobs(olmax_stream_t stream, const void* h, const void* W, const int32_t* targets,

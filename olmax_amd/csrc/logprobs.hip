@@ -533,8 +533,8 @@ __global__ __launch_bounds__(TH) void score_grad_kernel(const T* __restrict__ lo
 struct Form {
   int threads, parts;
 };
-// Rows that fill the GPU by themselves take a workgroup of 256 threads each, up to 256 long ones one of 512; few ones come in shares of one round of loads (1024 vectors), whose
-// candidates a second launch joins: many of those cost more than longer shares of 1024 threads.  us in a graph, bf16, 256 threads x 1 | 512 x 1 | 1024 x 1 | 256 x 16 | 1024 x 4: 1 x 128256
+// Rows that fill the GPU by themselves take a workgroup of 256 threads each, up to 256 long ones one of 512; few ones come in shares of at least one round of loads (1024 vectors; 128256 bf16 in
+// 15 of 1069, whose second round is 45), whose candidates a second launch joins: many of those cost more than longer shares of 1024 threads.  us in a graph, bf16, 256 threads x 1 | 512 x 1 | 1024 x 1 | 256 x 16 | 1024 x 4: 1 x 128256
 // without alternatives 17.0 | - | 13.5 | 7.4 | 10.2, with 20 28.8 | - | 23.2 | 13.4 | 17, with 128 35.8 | - | 25.7 | 45 | 20.9; 200 x 100352 with 20 27.3 | 22.6 | 24.1; 400 x 100352 with
 // 20 33.1 | 31.8 | 44.8, without 21.1 | 21.7 | 24.7; 1600 x 50304 with 20 49.7 | 54.8 | 104; 100 x 4096 without 4.7 | - | 6.2.
 Form form_of(int64_t T, int V, int top, bool f32) {
@@ -638,7 +638,8 @@ extern "C" int32_t olmax_token_logprobs_bwd(hipStream_t stream, const void* logi
 }
 
 // ---- with the LM head's product.  The logits are fp32: the framework's bf16 ones are off by 2^-9 of themselves, as much in a
-// log probability as policies of two steps may be apart.  Where the product runs in large tiles they stay in its accumulators (HeadRows), but for the columns behind the last whole
+// log probability as policies of two steps may be apart.  Their gradient is rounded to bf16 in front of its two products, which are the matrix cores' only so (fp32 ones would be two or three
+// times as many): dh and dW are off by two roundings, 0.0023 of themselves in the mean at 1024 x 4096 x 100352, and by one, 0.0017, if only they were rounded.  Where the product runs in large tiles they stay in its accumulators (HeadRows), but for the columns behind the last whole
 // round of tiles, which are a product of their own; where it does not, or alternatives are asked for, all of them go through the workspace.  us, logits in the workspace -> not: 2048
 // x 4096 x 100352 1443 -> 1195 (the product alone, fp32 logits written, 1335), gradients of 1024 x 4096 x 100352 2080 -> 1977.
 static int64_t head_stride(int32_t V) { return ((int64_t)V + 63) / 64 * 64; }  // whole lines of bf16 and fp32
