@@ -93,6 +93,22 @@ int32_t olmax_qk_rope_bwd(olmax_stream_t stream, const void* dy, void* dx, const
                           int64_t tokens, int32_t heads, int32_t head_dim, int32_t seq_len,
                           int64_t lddy, int64_t lddx, int64_t ldx, float eps);
 
+/* ---- Rotary positions beyond the reference's: tables for contexts longer than a model was trained on, interleaved pairs, part of a head, given positions.
+ * No counterpart in the reference (its _apply_rope, src/olmax/nn/rope.py:99-115, is layout 0 on whole heads).
+ * Tables [length, rotary_dim / 2] fp32 of size * cos, size * sin of the angle p f_i, f_i = theta^(-2i / rotary_dim), formed in 64 bits.  kind 0: as they are; 1: f_i / factor; of an angle
+ * that turns t = original_length f_i / 2 pi times in the original context, 2 (llama3): f_i / factor up to t = low, f_i from t = high on, between them the two mixed linearly in t;
+ * 3 (yarn): the same by the index i, linearly between floor and ceil of the indices that turn high and low times. */
+int32_t olmax_rotary_tables(olmax_stream_t stream, float* cos_t, float* sin_t, int64_t length, int32_t rotary_dim, double theta, int32_t kind, double factor,
+                            double original_length, double low, double high, float size);
+/* x, y: [tokens, heads * head_dim], bf16 or (f32) fp32, row strides ldx, ldy; in place (x == y) or apart.  The first rotary_dim columns of each head turn by the angle of the token's
+ * position, the others pass: pairs (i, i + rotary_dim / 2) (layout 0) or (2i, 2i + 1) (layout 1), (a, b) -> (a cos - b sin, b cos + a sin).  Position: positions[token], or (positions null)
+ * token % seq_len, seq_len <= table_rows.  Negative positions (padding) pass; one from table_rows on comes out as NaN.  cos_t, sin_t: [table_rows, rotary_dim / 2].
+ * olmax_rotary_bwd turns back: the gradient (times the tables' size, as the forward is). */
+int32_t olmax_rotary_fwd(olmax_stream_t stream, const void* x, void* y, const float* cos_t, const float* sin_t, const int32_t* positions, int64_t tokens, int32_t heads,
+                         int32_t head_dim, int32_t rotary_dim, int32_t table_rows, int32_t seq_len, int64_t ldx, int64_t ldy, int32_t layout, int32_t f32);
+int32_t olmax_rotary_bwd(olmax_stream_t stream, const void* dy, void* dx, const float* cos_t, const float* sin_t, const int32_t* positions, int64_t tokens, int32_t heads,
+                         int32_t head_dim, int32_t rotary_dim, int32_t table_rows, int32_t seq_len, int64_t lddy, int64_t lddx, int32_t layout, int32_t f32);
+
 /* ---- Gated MLP input projection with the activation fused into the GEMM epilogue:
  * GatedMLP.forward, src/olmax/nn/mlp.py:69-73 (gate_proj, up_proj, act(gate) * up in one call).
  * W = [Wgate; Wup] ([2F, K], row stride ldw); act_out [M, F]; gu_out ([M, 2F]) receives gate|up for the
@@ -176,6 +192,20 @@ int32_t olmax_attn_bwd_noalloc(olmax_stream_t stream, const void* q, const void*
                                void* dv, int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D,
                                int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t lddo,
                                int64_t lddq, int64_t lddk, int64_t lddv, int32_t window, float softcap);
+
+/* ---- Differential attention, beside the attention: the difference of two softmax maps with a learned weight.  No counterpart in the reference.
+ * A query head has two queries of width D (32 or 64) side by side, a key head two keys, and values are 2D wide: q, o, o2 [B*S, H*2D], k, v [B*S, KH*2D] bf16, row strides as in
+ * olmax_attn_fwd (16-byte aligned, multiples of 8, below 2^24).  With P_m = softmax(q_m k_m^T / sqrt(D)) under the mask of olmax_attn_fwd (causal, window):
+ *   o = (P_1 - lam_h P_2) v,   o2 = P_2 v (optional; the backward call takes it),   lse [B, H, 2, S]: both maps' log-normalisers
+ * lam: fp32 [H], or (lam_shared) one number for all heads.  No output may share memory with an input or another output. */
+int32_t olmax_diff_attn_fwd(olmax_stream_t stream, const void* q, const void* k, const void* v, const float* lam, void* o, void* o2, float* lse, int32_t B, int32_t S, int32_t H,
+                            int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t ldo2, int32_t lam_shared, int32_t window);
+/* From o, o2 and lse of the forward call and d_o = d loss / d o: dq, dk, dv, and dlam ([H], or one number with lam_shared, fp32).  Deterministic. */
+int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H);
+int32_t olmax_diff_attn_bwd(olmax_stream_t stream, const void* q, const void* k, const void* v, const float* lam, const void* o, const void* o2, const float* lse,
+                            const void* d_o, void* dq, void* dk, void* dv, float* dlam, void* workspace, int64_t workspace_bytes, int32_t B, int32_t S, int32_t H, int32_t KH,
+                            int32_t D, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t ldo2, int64_t lddo, int64_t lddq, int64_t lddk, int64_t lddv,
+                            int32_t lam_shared, int32_t window);
 
 /* ---- Cross entropy: cross_entropy_loss / fused_cross_entropy_loss,
  * src/olmax/nn/functional.py:70-121 (reduction "mean"; see the label quirks there).

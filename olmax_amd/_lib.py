@@ -66,6 +66,10 @@ _SIGNATURES = {
     "olmax_fill_zero": "PPL",
     "olmax_attn_fwd": "PPPPPPIIIIILLLLIF",
     "olmax_attn_bwd": "PPPPPPPPPPPLIIIIILLLLLLLLIF",
+    "olmax_rotary_fwd": "PPPPPPLIIIIILLII",
+    "olmax_rotary_bwd": "PPPPPPLIIIIILLII",
+    "olmax_diff_attn_fwd": "PPPPPPPPIIIIILLLLLII",
+    "olmax_diff_attn_bwd": "PPPPPPPPPPPPPPLIIIIILLLLLLLLLII",
     "olmax_token_logprobs": "PPPPPPPPPLLILIIIFF",
     "olmax_token_logprobs_bwd": "PPPPPPPLILLIIFF",
     "olmax_distill": "PPPPPPPPLLIILLIIFFFI",

@@ -1,0 +1,802 @@
+// Differential attention for gfx950: the difference of two causal softmax maps, with its gradients.  GQA, optional sliding window, BSHD layout, bf16 in and out, fp32
+// statistics.  No counterpart in the reference; beside its attention (src/olmax/nn/attention.py:96-103, attn.hip).
+//
+// A query head h has two queries q_1, q_2 of width D side by side in 2D columns, its key head two keys, and values of width W = 2D (a head of 128 columns is two maps of 64):
+//   s_m = q_m k_m^T / sqrt(D),  P_m = softmax(s_m),  O_m = P_m v,   o = O_1 - lambda_h O_2
+// Key j is visible to query i iff j <= i and (window < 0 or j >= i - window).  With dP = do v^T and delta_m = do . O_m (a row's sum of P_m dP):
+//   dS_1 = P_1 (dP - delta_1),  dS_2 = -lambda P_2 (dP - delta_2),  dq_m = dS_m k_m / sqrt(D),  dk_m = dS_m^T q_m / sqrt(D),
+//   dv = (P_1 - lambda P_2)^T do,  dlambda = - sum of delta_2 over the head's queries
+// so that the gradients take no more products than one map of width W does, but the exponentials of two.
+//
+// The kernels are laid out as those of attn.hip: score tiles are transposed, a lane owns one query (forward, dQ) or one key (dK/dV), and a [rows][W] tile of K or Q holds both
+// maps' halves of a row, k-steps 0 .. W/32 - 1 of the products the first one's.
+#include "attn_tiles.h"
+#include <cmath>
+#include <mutex>
+
+namespace {
+
+struct Sizes {
+  int S, H, KH, window;
+  int64_t ldq, ldk, ldv, ldo, ldo2;
+  float scale;
+  int shared;  // one lambda for all heads
+};
+
+// ---- Rows that come out infinite or NaN: see redo_rows.  What a row does not see must not reach it, and the tile products take hidden pairs along as zeros, which an infinity
+// or a NaN turns into NaN.  A wave that finds such values among those it has stored does their rows over, over visible pairs only: lane l has key or query l of 64 for the scores, columns l and
+// l + 64 of the row for the sums.  Speed does not matter here.
+__device__ __forceinline__ float dot(const bf16* a, const bf16* b, int n) {
+  float s = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < n; c += 8) {
+    Pack8 x, y;
+    x.u = *reinterpret_cast<const u32x4*>(a + c);
+    y.u = *reinterpret_cast<const u32x4*>(b + c);
+#pragma unroll
+    for (int e = 0; e < 8; e++) s += bf2f(x.e[e]) * bf2f(y.e[e]);
+  }
+  return s;
+}
+
+template <int W>
+__device__ __forceinline__ void redo_fwd(const bf16* q, const bf16* K, int64_t ldk, const bf16* V, int64_t ldv, float lam, bf16* o, bf16* o2, float* lse, int S, int i, int window,
+                                         float scale, int lane) {
+  constexpr int D = W / 2;
+  const int first = window >= 0 ? max(0, i - window) : 0;
+  float l[2];
+#pragma unroll 1
+  for (int m = 0; m < 2; m++) {
+    float mx = -INFINITY, sm = 0.f;
+#pragma unroll 1
+    for (int j = first + lane; j <= i; j += 64) mx = fmaxf(mx, dot(q + m * D, K + j * ldk + m * D, D) * scale);
+    mx = wave_max(mx);
+#pragma unroll 1
+    for (int j = first + lane; j <= i; j += 64) sm += __expf(dot(q + m * D, K + j * ldk + m * D, D) * scale - mx);
+    l[m] = mx + __logf(wave_sum(sm));
+    if (lane == 0) lse[m * S] = l[m];
+  }
+  float acc[2][W / 64] = {};
+#pragma unroll 1
+  for (int j0 = first; j0 <= i; j0 += 64) {
+    const int n = min(64, i - j0 + 1);
+    float p1 = 0.f, p2 = 0.f;
+    if (lane < n) {
+      p1 = __expf(dot(q, K + (j0 + lane) * ldk, D) * scale - l[0]);
+      p2 = __expf(dot(q + D, K + (j0 + lane) * ldk + D, D) * scale - l[1]);
+    }
+#pragma unroll 1
+    for (int t = 0; t < n; t++) {
+      const float a = __shfl(p1, t, 64), b = __shfl(p2, t, 64);
+#pragma unroll
+      for (int c = 0; c < W / 64; c++) {
+        const float v = bf2f(V[(j0 + t) * ldv + c * 64 + lane]);
+        acc[0][c] += a * v;
+        acc[1][c] += b * v;
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < W / 64; c++) {
+    o[c * 64 + lane] = f2bf(acc[0][c] - lam * acc[1][c]);
+    if (o2) o2[c * 64 + lane] = f2bf(acc[1][c]);
+  }
+}
+
+// p_m and dP of a pair
+template <int W>
+__device__ __forceinline__ void pair_of(const bf16* q, const bf16* k, const bf16* d_o, const bf16* v, float l1, float l2, float scale, float& p1, float& p2, float& dp) {
+  constexpr int D = W / 2;
+  p1 = __expf(dot(q, k, D) * scale - l1);
+  p2 = __expf(dot(q + D, k + D, D) * scale - l2);
+  dp = dot(d_o, v, W);
+}
+
+template <int W>
+__device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ldk, const bf16* V, int64_t ldv, const bf16* d_o, float l1, float l2, float d1, float d2, float lam,
+                                        bf16* dq, int i, int window, float scale, int lane) {
+  constexpr int D = W / 2;
+  float acc[W / 64] = {};
+#pragma unroll 1
+  for (int j0 = window >= 0 ? max(0, i - window) : 0; j0 <= i; j0 += 64) {
+    const int n = min(64, i - j0 + 1);
+    float s1 = 0.f, s2 = 0.f;
+    if (lane < n) {
+      float p1, p2, dp;
+      pair_of<W>(q, K + (j0 + lane) * ldk, d_o, V + (j0 + lane) * ldv, l1, l2, scale, p1, p2, dp);
+      s1 = p1 * (dp - d1);
+      s2 = -lam * p2 * (dp - d2);
+    }
+#pragma unroll 1
+    for (int t = 0; t < n; t++) {
+      const float a = __shfl(s1, t, 64), b = __shfl(s2, t, 64);
+#pragma unroll
+      for (int c = 0; c < W / 64; c++) acc[c] += (c * 64 + lane < D ? a : b) * bf2f(K[(j0 + t) * ldk + c * 64 + lane]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < W / 64; c++) dq[c * 64 + lane] = f2bf(acc[c] * scale);
+}
+
+// key j; Q, dO of the first of its rep query heads, stats (of a head and map: S numbers) of the first of them
+template <int W>
+__device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16* dO, int64_t lddo, const float* lse, const float* delta, const float* lam, int lam_step, const bf16* k,
+                                         const bf16* v, bf16* dk, bf16* dv, int j, int S, int rep, int window, float scale, int lane) {
+  constexpr int D = W / 2;
+  const int last = window >= 0 ? min(S - 1, j + window) : S - 1;
+  float ak[W / 64] = {}, av[W / 64] = {};
+#pragma unroll 1
+  for (int r = 0; r < rep; r++, Q += W, dO += W, lse += 2 * (int64_t)S, delta += 2 * (int64_t)S, lam += lam_step)
+#pragma unroll 1
+    for (int i0 = j; i0 <= last; i0 += 64) {
+      const int n = min(64, last - i0 + 1);
+      float p = 0.f, s1 = 0.f, s2 = 0.f;
+      if (lane < n) {
+        const int64_t i = i0 + lane;
+        float p1, p2, dp;
+        pair_of<W>(Q + i * ldq, k, dO + i * lddo, v, lse[i], lse[S + i], scale, p1, p2, dp);
+        s1 = p1 * (dp + delta[i]);
+        s2 = -*lam * p2 * ((dp + delta[i]) + delta[S + i]);
+        p = p1 - *lam * p2;
+      }
+#pragma unroll 1
+      for (int t = 0; t < n; t++) {
+        const float a = __shfl(s1, t, 64), b = __shfl(s2, t, 64), pt = __shfl(p, t, 64);
+#pragma unroll
+        for (int c = 0; c < W / 64; c++) {
+          ak[c] += (c * 64 + lane < D ? a : b) * bf2f(Q[(i0 + t) * ldq + c * 64 + lane]);
+          av[c] += pt * bf2f(dO[(i0 + t) * lddo + c * 64 + lane]);
+        }
+      }
+    }
+#pragma unroll
+  for (int c = 0; c < W / 64; c++) {
+    dk[c * 64 + lane] = f2bf(ak[c] * scale);
+    dv[c * 64 + lane] = f2bf(av[c]);
+  }
+}
+
+constexpr int QR = 128, KR = 128;  // queries, keys of a workgroup of four waves
+
+// ---------------------------------------------------------------------------------------
+// Forward.  grid = ceil(S / 128) H B workgroups of 4 waves; a wave owns 32 queries and both their maps.
+// ---------------------------------------------------------------------------------------
+template <int W>
+__global__ __launch_bounds__(256, 2) void diff_attn_fwd_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+                                                               bf16* __restrict__ O, bf16* __restrict__ O2, float* __restrict__ LSE, const Sizes z) {
+  constexpr int TILE = 64 * W * 2;  // bytes of a K or V tile of 64 keys
+  constexpr int KS = W / 32;        // k-steps of a map
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];  // [2][K | V]
+  const int S = z.S, H = z.H, KH = z.KH, window = z.window;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, lhi = lane >> 5;
+  const int nqt = (S + QR - 1) / QR;
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
+  const int qt = nqt - 1 - wg.rank;  // longest rows first
+  const int b = wg.group / KH, kh = wg.group % KH;
+  const int h = kh * (H / KH) + wg.r;
+  const int i0 = qt * QR;
+  const int iw0 = i0 + wave * 32;
+  const int qi = iw0 + l32;  // this lane's query
+  const int qic = min(qi, S - 1);
+
+  bf16x8 qf[W / 16];
+  {
+    const bf16* qp = Q + ((int64_t)b * S + qic) * z.ldq + h * W + lhi * 8;
+#pragma unroll
+    for (int s = 0; s < W / 16; s++) qf[s] = *reinterpret_cast<const bf16x8*>(qp + s * 16);
+  }
+  const int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
+  const int t_hi = min(i0 + QR - 1, S - 1) >> 6;  // inclusive
+
+  f32x16 o[2][W / 32];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) o[m][dt][r] = 0.f;
+  float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+
+  const bf16* kbase = K + (int64_t)b * S * z.ldk + kh * W;
+  const bf16* vbase = V + (int64_t)b * S * z.ldv + kh * W;
+  const unsigned lds0 = lds_addr_of(smem);
+  TileDma<64, W> dk, dv;
+  dk.init(z.ldk, wave, lane);
+  dv.init(z.ldv, wave, lane);
+  auto load_kv = [&](int t, int stage) {
+    const unsigned dst = lds0 + stage * (2 * TILE);
+    if (t * 64 + 64 <= S) {
+      dk.issue(kbase + (int64_t)t * 64 * z.ldk, dst, wave);
+      dv.issue(vbase + (int64_t)t * 64 * z.ldv, dst + TILE, wave);
+    } else {
+      dma_tile<64, W>(kbase, z.ldk, t * 64, S, dst, wave, lane);
+      dma_tile<64, W>(vbase, z.ldv, t * 64, S, dst + TILE, wave, lane);
+    }
+  };
+  const float sc2 = z.scale * LOG2E;
+  FragAddr<W> fa;
+  fa.init(lane);
+
+  load_kv(t_lo, 0);
+  dma_wait_all();
+  __syncthreads();
+  for (int t = t_lo; t <= t_hi; t++) {
+    const int cur = (t - t_lo) & 1, j0 = t * 64;
+    if (t < t_hi) load_kv(t + 1, cur ^ 1);
+    const bool visible = j0 <= iw0 + 31 && (window < 0 || j0 + 63 >= iw0 - window);
+    if (visible) {
+      const unsigned char* sk = smem + cur * (2 * TILE);
+      const unsigned char* sv = sk + TILE;
+      const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
+      bf16x8 pb[2][4];
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        f32x16 st[2];
+#pragma unroll
+        for (int jt = 0; jt < 2; jt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) st[jt][r] = 0.f;
+#pragma unroll
+        for (int s = m * KS; s < (m + 1) * KS; s++)
+#pragma unroll
+          for (int jt = 0; jt < 2; jt++) st[jt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, s), qf[s], st[jt], 0, 0, 0);
+        if (need_mask) {
+#pragma unroll
+          for (int jt = 0; jt < 2; jt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+              const int j = j0 + jt * 32 + (r >> 2) * 8 + lhi * 4 + (r & 3);
+              const bool ok = (j <= qi) && (window < 0 || j >= qi - window);
+              st[jt][r] = ok ? st[jt][r] : -INFINITY;
+            }
+        }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int jt = 0; jt < 2; jt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) mt = fmaxf(mt, st[jt][r]);
+        mt = half_swap_max(mt * sc2);
+        // the reference of the exponentials moves when a row's maximum has grown by 2^8 (as in attn.hip)
+        if (__builtin_amdgcn_ballot_w64(mt > mx[m] + 8.f) != 0) {
+          const float m_new = fmaxf(mx[m], mt);
+          const float alpha = fexp2(mx[m] - (m_new == -INFINITY ? 0.f : m_new));
+          sum[m] *= alpha;
+          mx[m] = m_new;
+#pragma unroll
+          for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[m][dt][r] *= alpha;
+        }
+        const float ref = mx[m] == -INFINITY ? 0.f : mx[m];
+#pragma unroll
+        for (int jt = 0; jt < 2; jt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) st[jt][r] = fexp2(__builtin_fmaf(st[jt][r], sc2, -ref));
+#pragma unroll
+        for (int u = 0; u < 4; u++) pb[m][u] = pack_bf16x8(st[u >> 1], (u & 1) * 8);
+        float ps[16];  // the sum in fp32, pairwise
+#pragma unroll
+        for (int r = 0; r < 16; r++) ps[r] = st[0][r] + st[1][r];
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+          for (int r = 0; r < w; r++) ps[r] += ps[r + w];
+        sum[m] += ps[0];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int dt = 0; dt < W / 32; dt++) {
+          const bf16x8 vf = fa.load_tr(sv, u * 16, dt);
+          o[0][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[0][u], o[0][dt], 0, 0, 0);
+          o[1][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[1][u], o[1][dt], 0, 0, 0);
+        }
+    }
+    dma_wait_all();
+    __syncthreads();
+  }
+  float inv[2], lse[2], zeros = 0.f;
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    const float total = half_swap_sum(sum[m]);
+    inv[m] = total > 0.f ? 1.f / total : 0.f;
+    lse[m] = (mx[m] + log2f(total)) * LN2;
+    zeros = __builtin_fmaf(lse[m], 0.f, zeros);
+  }
+  const float lam = LAM[z.shared ? 0 : h];
+  float* lse_row = LSE + ((int64_t)b * H + h) * 2 * S;
+  if (qi < S) {
+    bf16* op = O + ((int64_t)b * S + qi) * z.ldo + h * W;
+    bf16* o2p = O2 ? O2 + ((int64_t)b * S + qi) * z.ldo2 + h * W : nullptr;
+#pragma unroll
+    for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        Pack4 pk, p2;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float y = o[1][dt][g * 4 + e] * inv[1], x = __builtin_fmaf(o[0][dt][g * 4 + e], inv[0], -lam * y);
+          zeros = __builtin_fmaf(x, 0.f, zeros);
+          pk.e[e] = f2bf(x);
+          p2.e[e] = f2bf(y);
+        }
+        *reinterpret_cast<u32x2*>(op + dt * 32 + g * 8 + lhi * 4) = pk.u;
+        if (O2) *reinterpret_cast<u32x2*>(o2p + dt * 32 + g * 8 + lhi * 4) = p2.u;
+      }
+    if (lhi == 0) {
+      lse_row[qi] = lse[0];
+      lse_row[S + qi] = lse[1];
+    }
+  } else {
+    zeros = 0.f;
+  }
+  redo_rows(zeros, [&](int r) {
+    const int i = iw0 + r;
+    const int64_t at = (int64_t)b * S + i;
+    redo_fwd<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, lam, O + at * z.ldo + h * W, O2 ? O2 + at * z.ldo2 + h * W : nullptr, lse_row + i, S, i, window, z.scale, lane);
+  });
+}
+
+// ---------------------------------------------------------------------------------------
+// dQ, dlambda and delta.  Tiling and grid of the forward.
+// DELTA [B, H, 2, S]: -delta_1, and delta_1 - delta_2 (dP - delta_2 is what dK/dV has of the first map, plus this).  dlambda is taken from P_2 and dP in fp32, not from the rounded O_2:
+// it is a sum of terms of both signs that an error of 2^-9 in each would leave three digits of.  DLAM: a number for each workgroup, [B, H, tiles].
+// ---------------------------------------------------------------------------------------
+struct Grad {
+  int64_t lddo, lddq, lddk, lddv;
+};
+template <int W>
+__global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+                                                              const bf16* __restrict__ O, const bf16* __restrict__ O2, const float* __restrict__ LSE, const bf16* __restrict__ dO,
+                                                              bf16* __restrict__ dQ, float* __restrict__ DELTA, float* __restrict__ DLAM, const Sizes z, const Grad gr) {
+  constexpr int TILE = 64 * W * 2, KS = W / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];  // [2][K | V]
+  __shared__ float red[4];
+  const int S = z.S, H = z.H, KH = z.KH, window = z.window;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, lhi = lane >> 5;
+  const int nqt = (S + QR - 1) / QR;
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
+  const int qt = nqt - 1 - wg.rank;
+  const int b = wg.group / KH, kh = wg.group % KH;
+  const int h = kh * (H / KH) + wg.r;
+  const int i0 = qt * QR;
+  const int iw0 = i0 + wave * 32;
+  const int qi = iw0 + l32;
+  const int qic = min(qi, S - 1);
+  const float lam = LAM[z.shared ? 0 : h];
+
+  bf16x8 qf[W / 16], dof[W / 16];
+  float d1 = 0.f, d2 = 0.f;
+  {
+    const int64_t at = (int64_t)b * S + qic;
+    const bf16* qp = Q + at * z.ldq + h * W + lhi * 8;
+    const bf16* dp = dO + at * gr.lddo + h * W + lhi * 8;
+    const bf16* op = O + at * z.ldo + h * W + lhi * 8;
+    const bf16* o2p = O2 + at * z.ldo2 + h * W + lhi * 8;
+#pragma unroll
+    for (int s = 0; s < W / 16; s++) {
+      qf[s] = *reinterpret_cast<const bf16x8*>(qp + s * 16);
+      dof[s] = *reinterpret_cast<const bf16x8*>(dp + s * 16);
+      const bf16x8 of = *reinterpret_cast<const bf16x8*>(op + s * 16), o2f = *reinterpret_cast<const bf16x8*>(o2p + s * 16);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        d1 += bf2f(of[e]) * bf2f(dof[s][e]);
+        d2 += bf2f(o2f[e]) * bf2f(dof[s][e]);
+      }
+    }
+  }
+  d2 = half_swap_sum(d2);
+  d1 = __builtin_fmaf(lam, d2, half_swap_sum(d1));  // o + lambda O_2 = O_1
+  const int64_t row0 = ((int64_t)b * H + h) * 2 * S;
+  if (lhi == 0 && qi < S) {
+    DELTA[row0 + qi] = -d1;
+    DELTA[row0 + S + qi] = d1 - d2;
+  }
+  const float l1 = LSE[row0 + qic] * LOG2E, l2 = LSE[row0 + S + qic] * LOG2E;
+  const int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
+  const int t_hi = min(i0 + QR - 1, S - 1) >> 6;
+
+  f32x16 dq[W / 32];
+#pragma unroll
+  for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) dq[dt][r] = 0.f;
+  float dl = 0.f;
+
+  const bf16* kbase = K + (int64_t)b * S * z.ldk + kh * W;
+  const bf16* vbase = V + (int64_t)b * S * z.ldv + kh * W;
+  const unsigned lds0 = lds_addr_of(smem);
+  TileDma<64, W> dk, dv;
+  dk.init(z.ldk, wave, lane);
+  dv.init(z.ldv, wave, lane);
+  auto load_kv = [&](int t, int stage) {
+    const unsigned dst = lds0 + stage * (2 * TILE);
+    if (t * 64 + 64 <= S) {
+      dk.issue(kbase + (int64_t)t * 64 * z.ldk, dst, wave);
+      dv.issue(vbase + (int64_t)t * 64 * z.ldv, dst + TILE, wave);
+    } else {
+      dma_tile<64, W>(kbase, z.ldk, t * 64, S, dst, wave, lane);
+      dma_tile<64, W>(vbase, z.ldv, t * 64, S, dst + TILE, wave, lane);
+    }
+  };
+  const float sc2 = z.scale * LOG2E;
+  FragAddr<W> fa;
+  fa.init(lane);
+
+  load_kv(t_lo, 0);
+  dma_wait_all();
+  __syncthreads();
+  for (int t = t_lo; t <= t_hi; t++) {
+    const int cur = (t - t_lo) & 1, j0 = t * 64;
+    if (t < t_hi) load_kv(t + 1, cur ^ 1);
+    const bool visible = j0 <= iw0 + 31 && (window < 0 || j0 + 63 >= iw0 - window);
+    if (visible) {
+      const unsigned char* sk = smem + cur * (2 * TILE);
+      const unsigned char* sv = sk + TILE;
+      const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
+#pragma unroll
+      for (int jt = 0; jt < 2; jt++) {
+        f32x16 s1, s2, dp;
+#pragma unroll
+        for (int r = 0; r < 16; r++) { s1[r] = 0.f; s2[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+          s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, s), qf[s], s1, 0, 0, 0);
+          s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, KS + s), qf[KS + s], s2, 0, 0, 0);
+        }
+#pragma unroll
+        for (int s = 0; s < 2 * KS; s++) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sv, jt * 32, s), dof[s], dp, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const float p1 = fexp2(__builtin_fmaf(s1[r], sc2, -l1)), p2 = fexp2(__builtin_fmaf(s2[r], sc2, -l2));
+          float x = p1 * (dp[r] - d1), y = p2 * (dp[r] - d2), w = p2 * dp[r];
+          if (need_mask) {
+            const int j = j0 + jt * 32 + (r >> 2) * 8 + lhi * 4 + (r & 3);
+            const bool ok = (j <= qi) && (window < 0 || j >= qi - window);
+            x = ok ? x : 0.f;
+            y = ok ? y : 0.f;
+            w = ok ? w : 0.f;
+          }
+          s1[r] = x;
+          s2[r] = y;
+          dl += w;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const bf16x8 a = pack_bf16x8(s1, u * 8), c = pack_bf16x8(s2, u * 8);
+#pragma unroll
+          for (int dt = 0; dt < W / 32; dt++)
+            dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_tr(sk, jt * 32 + u * 16, dt), dt < W / 64 ? a : c, dq[dt], 0, 0, 0);
+        }
+      }
+    }
+    dma_wait_all();
+    __syncthreads();
+  }
+  dl = block_sum<4>(qi < S ? dl : 0.f, red);
+  if (tid == 0) DLAM[((int64_t)b * H + h) * nqt + qt] = -dl;
+  float zeros = 0.f;
+  if (qi < S) {
+    bf16* op = dQ + ((int64_t)b * S + qi) * gr.lddq + h * W;
+#pragma unroll
+    for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        Pack4 pk;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float x = dq[dt][g * 4 + e] * (dt < W / 64 ? z.scale : -lam * z.scale);
+          zeros = __builtin_fmaf(x, 0.f, zeros);
+          pk.e[e] = f2bf(x);
+        }
+        *reinterpret_cast<u32x2*>(op + dt * 32 + g * 8 + lhi * 4) = pk.u;
+      }
+  }
+  redo_rows(zeros, [&](int r) {
+    const int i = iw0 + r;
+    const int64_t at = (int64_t)b * S + i;
+    redo_dq<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, dO + at * gr.lddo + h * W, LSE[row0 + i], LSE[row0 + S + i], __shfl(d1, r, 64), __shfl(d2, r, 64), lam,
+               dQ + at * gr.lddq + h * W, i, window, z.scale, lane);
+  });
+}
+
+// ---------------------------------------------------------------------------------------
+// dK/dV.  grid = ceil(S / 128) KH B workgroups of 4 waves; a wave owns 32 keys (K in registers) and walks the query heads of its group and their 32-row tiles from the diagonal on.
+// LDS: 2 stages of (Q | dO | lse_1, lse_2, -delta_1, delta_1 - delta_2 of the 32 rows), then the V tile.
+// ---------------------------------------------------------------------------------------
+constexpr int smem_q(int W) { return 2 * 2 * 64 * W * 2; }
+constexpr int smem_kv(int W) { return 2 * (2 * 32 * W * 2 + 512) + KR * W * 2; }
+template <int W>
+__global__ __launch_bounds__(256, 2) void diff_attn_dkv_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+                                                               const float* __restrict__ LSE, const float* __restrict__ DELTA, const bf16* __restrict__ dO, bf16* __restrict__ dK,
+                                                               bf16* __restrict__ dV, const Sizes z, const Grad gr) {
+  constexpr int QT = 32, KS = W / 32;
+  constexpr int TILE = QT * W * 2, STAGE = 2 * TILE + 512;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int S = z.S, H = z.H, KH = z.KH, window = z.window;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, lhi = lane >> 5;
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / ((S + KR - 1) / KR)), 1);  // key tile 0 is seen by every query: longest first
+  const int b = wg.group / KH, kh = wg.group % KH;
+  const int rep = H / KH;
+  const int j0 = wg.rank * KR;
+  const int jw0 = j0 + wave * 32;
+  const int kj = jw0 + l32;  // this lane's key
+  const int kjc = min(kj, S - 1);
+
+  bf16x8 kf[W / 16];
+  {
+    const bf16* kp = K + ((int64_t)b * S + kjc) * z.ldk + kh * W + lhi * 8;
+#pragma unroll
+    for (int s = 0; s < W / 16; s++) kf[s] = *reinterpret_cast<const bf16x8*>(kp + s * 16);
+  }
+  f32x16 dk[W / 32], dv[W / 32];
+#pragma unroll
+  for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) { dk[dt][r] = 0.f; dv[dt][r] = 0.f; }
+
+  const int i_hi = window >= 0 ? min(S - 1, j0 + KR - 1 + window) : S - 1;
+  const int t_lo = j0 / QT, t_hi = i_hi / QT;  // inclusive
+  const int ntile = t_hi - t_lo + 1;
+  const int64_t total = (int64_t)ntile * rep;  // (head, tile) pairs, heads outermost
+  const float sc2 = z.scale * LOG2E;
+  const unsigned lds0 = lds_addr_of(smem);
+
+  TileDma<QT, W> tq, tdo;
+  tq.init(z.ldq, wave, lane);
+  tdo.init(gr.lddo, wave, lane);
+  int ld_h = kh * rep, ld_t = t_lo;  // next pair to load
+  float sreg[2];
+  auto load_tile = [&](int stage) {
+    const int hq = ld_h, t = ld_t;
+    if (++ld_t > t_hi) {
+      ld_t = t_lo;
+      ++ld_h;
+    }
+    const unsigned dst = lds0 + stage * STAGE;
+    const bf16 *qp = Q + (int64_t)b * S * z.ldq + hq * W, *dp = dO + (int64_t)b * S * gr.lddo + hq * W;
+    if (t * QT + QT <= S) {
+      tq.issue(qp + (int64_t)t * QT * z.ldq, dst, wave);
+      tdo.issue(dp + (int64_t)t * QT * gr.lddo, dst + TILE, wave);
+    } else {
+      dma_tile<QT, W>(qp, z.ldq, t * QT, S, dst, wave, lane);
+      dma_tile<QT, W>(dp, gr.lddo, t * QT, S, dst + TILE, wave, lane);
+    }
+    if (wave == 0) {  // lanes 0 .. 31 the first map's, 32 .. 63 the second's
+      const int64_t at = (((int64_t)b * H + hq) * 2 + lhi) * S + min(t * QT + l32, S - 1);
+      sreg[0] = LSE[at];
+      sreg[1] = DELTA[at];
+    }
+  };
+  auto store_stats = [&](int stage) {
+    if (wave == 0) {
+      float* p = reinterpret_cast<float*>(smem + stage * STAGE + 2 * TILE);
+      p[lane] = sreg[0] * LOG2E;
+      p[64 + lane] = sreg[1];
+    }
+  };
+
+  FragAddr<W> fa;
+  fa.init(lane);
+  const unsigned char* svt = smem + 2 * STAGE;  // [128 keys][W] V tile
+  dma_tile<KR, W>(V + (int64_t)b * S * z.ldv + kh * W, z.ldv, j0, S, lds0 + 2 * STAGE, wave, lane);
+  load_tile(0);
+  store_stats(0);
+  dma_wait_all();
+  __syncthreads();
+  int hq = kh * rep, t = t_lo;
+  for (int64_t it = 0; it < total; it++) {
+    const int cur = (int)(it & 1);
+    const bool more = it + 1 < total;
+    if (more) load_tile(cur ^ 1);
+    const int ib = t * QT;  // first query of the tile
+    const float nlam = -LAM[z.shared ? 0 : hq];
+    const bool visible = (ib + QT - 1 >= jw0) && (window < 0 || ib <= jw0 + 31 + window);
+    if (visible) {
+      const unsigned char* sq = smem + cur * STAGE;
+      const unsigned char* so = sq + TILE;
+      const float* stats = reinterpret_cast<const float*>(sq + 2 * TILE);
+      const bool need_mask = (ib < jw0 + 31) || (ib + QT > S) || (window >= 0 && ib + QT - 1 > jw0 + window);
+      f32x16 s1, s2, dp;
+      // accumulator rows are queries ib + 8 (r / 4) + 4 lhi + r % 4; column: key kj.  dP starts from -delta_1
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(stats + 64 + g * 8 + lhi * 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) { s1[g * 4 + e] = 0.f; s2[g * 4 + e] = 0.f; dp[g * 4 + e] = d4[e]; }
+      }
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sq, 0, s), kf[s], s1, 0, 0, 0);
+        s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sq, 0, KS + s), kf[KS + s], s2, 0, 0, 0);
+      }
+#pragma unroll
+      for (int s = 0; s < 2 * KS; s++) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(so, 0, s), fa.load_kc(svt, wave * 32, s), dp, 0, 0, 0);
+      f32x16 p;
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int il = g * 8 + lhi * 4;
+        const f32x4 l1 = *reinterpret_cast<const f32x4*>(stats + il), l2 = *reinterpret_cast<const f32x4*>(stats + 32 + il);
+        const f32x4 dd = *reinterpret_cast<const f32x4*>(stats + 96 + il);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int r = g * 4 + e;
+          const float p1 = fexp2(__builtin_fmaf(s1[r], sc2, -l1[e])), p2 = nlam * fexp2(__builtin_fmaf(s2[r], sc2, -l2[e]));
+          float x = p1 * dp[r], y = p2 * (dp[r] + dd[e]), w = p1 + p2;
+          if (need_mask) {
+            const int i = ib + il + e;
+            const bool ok = (kj <= i) && (i < S) && (window < 0 || kj >= i - window);
+            x = ok ? x : 0.f;
+            y = ok ? y : 0.f;
+            w = ok ? w : 0.f;
+          }
+          s1[r] = x;
+          s2[r] = y;
+          p[r] = w;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const bf16x8 a = pack_bf16x8(s1, u * 8), c = pack_bf16x8(s2, u * 8), w = pack_bf16x8(p, u * 8);
+#pragma unroll
+        for (int dt = 0; dt < W / 32; dt++) {
+          dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_tr(so, u * 16, dt), w, dv[dt], 0, 0, 0);
+          dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_tr(sq, u * 16, dt), dt < W / 64 ? a : c, dk[dt], 0, 0, 0);
+        }
+      }
+    }
+    if (++t > t_hi) {
+      t = t_lo;
+      ++hq;
+    }
+    if (more) store_stats(cur ^ 1);
+    dma_wait_all();
+    __syncthreads();
+  }
+  float zeros = 0.f;
+  auto store4 = [&](bf16* p, int dt, int g, const f32x16& v, float mul) {
+    Pack4 pk;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float x = v[g * 4 + e] * mul;
+      zeros = __builtin_fmaf(x, 0.f, zeros);
+      pk.e[e] = f2bf(x);
+    }
+    *reinterpret_cast<u32x2*>(p + dt * 32 + g * 8 + lhi * 4) = pk.u;
+  };
+  if (kj < S) {
+    bf16* kp = dK + ((int64_t)b * S + kj) * gr.lddk + kh * W;
+    bf16* vp = dV + ((int64_t)b * S + kj) * gr.lddv + kh * W;
+#pragma unroll
+    for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        store4(kp, dt, g, dk[dt], z.scale);
+        store4(vp, dt, g, dv[dt], 1.f);
+        __builtin_amdgcn_sched_barrier(0);  // a row leaves in order (see attn.hip)
+      }
+  }
+  redo_rows(zeros, [&](int r) {
+    const int64_t seq = (int64_t)b * S, at = seq + jw0 + r, row = ((int64_t)b * H + kh * rep) * 2 * S;
+    redo_dkv<W>(Q + seq * z.ldq + kh * rep * W, z.ldq, dO + seq * gr.lddo + kh * rep * W, gr.lddo, LSE + row, DELTA + row, LAM + (z.shared ? 0 : kh * rep), z.shared ? 0 : 1,
+                K + at * z.ldk + kh * W, V + at * z.ldv + kh * W, dK + at * gr.lddk + kh * W, dV + at * gr.lddv + kh * W, jw0 + r, S, rep, window, z.scale, lane);
+  });
+}
+
+// dlambda of a head (or of all): the workgroups' sums in their order
+__global__ __launch_bounds__(256) void diff_attn_dlam_kernel(const float* __restrict__ parts, float* __restrict__ dlam, int B, int H, int tiles, int shared) {
+  __shared__ float red[4];
+  const int64_t per = (int64_t)tiles * (shared ? H : 1);  // a sequence's, next to each other
+  float s = 0.f;
+  for (int b = 0; b < B; b++) {
+    const float* p = parts + ((int64_t)b * H + blockIdx.x) * tiles;
+    for (int64_t i = threadIdx.x; i < per; i += 256) s += p[i];
+  }
+  s = block_sum<4>(s, red);
+  if (threadIdx.x == 0) dlam[blockIdx.x] = s;
+}
+
+int64_t tiles_of(int32_t S) { return ((int64_t)S + QR - 1) / QR; }
+int64_t delta_bytes(int32_t B, int32_t S, int32_t H) { return ((int64_t)B * H * 2 * S * 4 + 255) / 256 * 256; }
+
+constexpr int64_t MAX_LD = 1 << 24;  // of a row, in elements: 64 rows are within reach of a 32-bit offset in bytes
+// Whether rows of na and nb bf16 numbers at a and b share memory: exact for one row stride, as views of one buffer have it, otherwise whether their ranges meet.
+bool meet(const void* a, int64_t lda, int64_t na, const void* b, int64_t ldb, int64_t nb, int64_t rows) {
+  if (!a || !b) return false;
+  const int64_t d = ((const char*)b - (const char*)a) / 2;
+  if (d >= (rows - 1) * lda + na || -d >= (rows - 1) * ldb + nb) return false;
+  const int64_t at = lda == ldb ? ((d % lda) + lda) % lda : 0;
+  return at < na || at + nb > lda;
+}
+bool rows_ok(const void* p, int64_t ld, int64_t width) { return aligned16(p) && ld % 8 == 0 && ld >= width && ld < MAX_LD; }
+
+int check_shape(const char* name, int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D) {
+  OLMAX_CHECK(B > 0 && S > 0 && H > 0 && KH > 0 && H % KH == 0 && S <= (1 << 24) && H <= (1 << 16), OLMAX_ERR_SHAPE, "%s: bad shape B=%d S=%d H=%d KH=%d", name, B, S, H, KH);
+  OLMAX_CHECK(D == 32 || D == 64, OLMAX_ERR_SHAPE, "%s: D must be 32 or 64 (got %d)", name, D);
+  OLMAX_CHECK(tiles_of(S) * H * B < (1LL << 31), OLMAX_ERR_SHAPE, "%s: B=%d S=%d H=%d are too many rows", name, B, S, H);
+  return OLMAX_OK;
+}
+
+template <int W>
+void fwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const float* lam, bf16* o, bf16* o2, float* lse, int B, const Sizes& z) {
+  static std::once_flag once;
+  std::call_once(once, [] { (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W)); });
+  hipLaunchKernelGGL(diff_attn_fwd_kernel<W>, dim3((unsigned)(tiles_of(z.S) * z.H * B)), dim3(256), smem_q(W), stream, q, k, v, lam, o, o2, lse, z);
+}
+
+template <int W>
+void bwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const float* lam, const bf16* o, const bf16* o2, const float* lse, const bf16* d_o, bf16* dq, bf16* dk,
+         bf16* dv, float* dlam, float* delta, float* parts, int B, const Sizes& z, const Grad& gr) {
+  static std::once_flag once;
+  std::call_once(once, [] {
+    (void)hipFuncSetAttribute((const void*)diff_attn_dq_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W));
+    (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W));
+  });
+  const int tiles = (int)tiles_of(z.S);
+  hipLaunchKernelGGL(diff_attn_dq_kernel<W>, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(256), smem_q(W), stream, q, k, v, lam, o, o2, lse, d_o, dq, delta, parts, z, gr);
+  hipLaunchKernelGGL(diff_attn_dkv_kernel<W>, dim3((unsigned)((int64_t)((z.S + KR - 1) / KR) * z.KH * B)), dim3(256), smem_kv(W), stream, q, k, v, lam, lse, (const float*)delta, d_o, dk, dv, z, gr);
+  hipLaunchKernelGGL(diff_attn_dlam_kernel, dim3((unsigned)(z.shared ? 1 : z.H)), dim3(256), 0, stream, (const float*)parts, dlam, B, z.H, tiles, z.shared);
+}
+
+}  // namespace
+
+extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const void* k, const void* v, const float* lam, void* o, void* o2, float* lse, int32_t B, int32_t S,
+                                       int32_t H, int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t ldo2, int32_t lam_shared, int32_t window) {
+  OLMAX_CHECK(q && k && v && lam && o && lse, OLMAX_ERR_ARG, "olmax_diff_attn_fwd: null pointer");
+  if (int rc = check_shape("olmax_diff_attn_fwd", B, S, H, KH, D)) return rc;
+  const int64_t W = 2 * D, rows = (int64_t)B * S;
+  OLMAX_CHECK(rows_ok(q, ldq, H * W) && rows_ok(k, ldk, KH * W) && rows_ok(v, ldv, KH * W) && rows_ok(o, ldo, H * W) && (!o2 || rows_ok(o2, ldo2, H * W)), OLMAX_ERR_ALIGN,
+              "olmax_diff_attn_fwd: operands must be 16-byte aligned, with row strides that are multiples of 8, at least heads * 2D and below 2^24");
+  OLMAX_CHECK((((uintptr_t)lam | (uintptr_t)lse) & 3) == 0, OLMAX_ERR_ALIGN, "olmax_diff_attn_fwd: lam and lse not aligned to their type");
+  const void* ins[] = {q, k, v};
+  const int64_t ld_in[] = {ldq, ldk, ldv}, n_in[] = {H * W, KH * W, KH * W};
+  for (int i = 0; i < 3; i++)
+    OLMAX_CHECK(!meet(ins[i], ld_in[i], n_in[i], o, ldo, H * W, rows) && !meet(ins[i], ld_in[i], n_in[i], o2, ldo2, H * W, rows), OLMAX_ERR_ARG,
+                "olmax_diff_attn_fwd: an output shares memory with an input");
+  OLMAX_CHECK(!meet(o, ldo, H * W, o2, ldo2, H * W, rows), OLMAX_ERR_ARG, "olmax_diff_attn_fwd: o and o2 share memory");
+  const Sizes z{S, H, KH, window < 0 || window >= S ? -1 : window, ldq, ldk, ldv, ldo, ldo2, 1.f / sqrtf((float)D), lam_shared != 0};
+  (D == 64 ? fwd<128> : fwd<64>)(stream, (const bf16*)q, (const bf16*)k, (const bf16*)v, lam, (bf16*)o, (bf16*)o2, lse, B, z);
+  OLMAX_LAUNCH_CHECK();
+  return OLMAX_OK;
+}
+
+// Workspace: delta [B, H, 2, S], then dlambda's parts [B, H, ceil(S / 128)], fp32
+extern "C" int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H) {
+  return B <= 0 || S <= 0 || H <= 0 ? 0 : delta_bytes(B, S, H) + ((int64_t)B * H * tiles_of(S) * 4 + 255) / 256 * 256;
+}
+
+extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const void* k, const void* v, const float* lam, const void* o, const void* o2, const float* lse,
+                                       const void* d_o, void* dq, void* dk, void* dv, float* dlam, void* workspace, int64_t workspace_bytes, int32_t B, int32_t S, int32_t H,
+                                       int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t ldo2, int64_t lddo, int64_t lddq, int64_t lddk,
+                                       int64_t lddv, int32_t lam_shared, int32_t window) {
+  OLMAX_CHECK(q && k && v && lam && o && o2 && lse && d_o && dq && dk && dv && dlam && workspace, OLMAX_ERR_ARG, "olmax_diff_attn_bwd: null pointer");
+  if (int rc = check_shape("olmax_diff_attn_bwd", B, S, H, KH, D)) return rc;
+  const int64_t W = 2 * D, rows = (int64_t)B * S;
+  const void *ins[] = {q, k, v, o, o2, d_o}, *outs[] = {dq, dk, dv};
+  const int64_t ld_in[] = {ldq, ldk, ldv, ldo, ldo2, lddo}, n_in[] = {H * W, KH * W, KH * W, H * W, H * W, H * W};
+  const int64_t ld_out[] = {lddq, lddk, lddv}, n_out[] = {H * W, KH * W, KH * W};
+  bool ok = true, apart = true;
+  for (int i = 0; i < 6; i++) ok = ok && rows_ok(ins[i], ld_in[i], n_in[i]);
+  for (int i = 0; i < 3; i++) ok = ok && rows_ok(outs[i], ld_out[i], n_out[i]);
+  OLMAX_CHECK(ok, OLMAX_ERR_ALIGN, "olmax_diff_attn_bwd: operands must be 16-byte aligned, with row strides that are multiples of 8, at least heads * 2D and below 2^24");
+  OLMAX_CHECK((((uintptr_t)lam | (uintptr_t)lse | (uintptr_t)dlam) & 3) == 0, OLMAX_ERR_ALIGN, "olmax_diff_attn_bwd: lam, lse and dlam not aligned to their type");
+  OLMAX_CHECK(workspace_bytes >= olmax_diff_attn_bwd_workspace_bytes(B, S, H) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
+              "olmax_diff_attn_bwd: workspace needs %ld bytes, 256-byte aligned", (long)olmax_diff_attn_bwd_workspace_bytes(B, S, H));
+  for (int x = 0; x < 3; x++) {
+    for (int i = 0; i < 6; i++) apart = apart && !meet(ins[i], ld_in[i], n_in[i], outs[x], ld_out[x], n_out[x], rows);
+    for (int y = 0; y < x; y++) apart = apart && !meet(outs[y], ld_out[y], n_out[y], outs[x], ld_out[x], n_out[x], rows);
+  }
+  OLMAX_CHECK(apart, OLMAX_ERR_ARG, "olmax_diff_attn_bwd: an output shares memory with an input or another output");
+  const Sizes z{S, H, KH, window < 0 || window >= S ? -1 : window, ldq, ldk, ldv, ldo, ldo2, 1.f / sqrtf((float)D), lam_shared != 0};
+  const Grad gr{lddo, lddq, lddk, lddv};
+  (D == 64 ? bwd<128> : bwd<64>)(stream, (const bf16*)q, (const bf16*)k, (const bf16*)v, lam, (const bf16*)o, (const bf16*)o2, lse, (const bf16*)d_o, (bf16*)dq, (bf16*)dk, (bf16*)dv,
+                                 dlam, (float*)workspace, (float*)((char*)workspace + delta_bytes(B, S, H)), B, z, gr);
+  OLMAX_LAUNCH_CHECK();
+  return OLMAX_OK;
+}

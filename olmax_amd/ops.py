@@ -8,12 +8,13 @@ operands may be row-strided views (stride(1) must be 1).
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import check, f32, i32, i64, ptr, raw_stream, stream_ptr, typed
+from ._lib import check, f32, f64, i32, i64, ptr, raw_stream, stream_ptr, typed
 
 BF16 = torch.bfloat16
 
@@ -145,6 +146,83 @@ def qk_rope_bwd(dy, cos, sin, *, heads: int, head_dim: int, seq_len: int, x=None
     return out, dw
 
 
+# ----------------------------------------------------------------------------- rotary positions for other models and lengths
+_SCALING = {"linear": 1, "llama3": 2, "yarn": 3}
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How the angles of a model trained on original_length tokens are slowed down for `factor` times as many.
+
+    kind "linear": all by the factor.  "llama3": those that turn at most low_turns times in the original context by the factor, those that turn high_turns times and more
+    not, linearly between.  "yarn": the same by the index of the angle (low_turns 1, high_turns 32 are its usual ones), and cos and sin times
+    attention_factor, 0.1 ln(factor) + 1 if None."""
+    kind: str
+    factor: float
+    original_length: int = 8192
+    low_turns: float = 1.0
+    high_turns: Optional[float] = None  # 4 for llama3, 32 for yarn
+    attention_factor: Optional[float] = None
+
+    def __post_init__(self):
+        if self.kind not in _SCALING:
+            raise ValueError(f"unknown rope scaling {self.kind!r}")
+        if self.attention_factor is not None and self.kind != "yarn":
+            raise ValueError("attention_factor goes with yarn")
+
+    def c_args(self):
+        high = self.high_turns if self.high_turns is not None else 32.0 if self.kind == "yarn" else 4.0
+        size = 1.0 if self.kind != "yarn" else self.attention_factor if self.attention_factor is not None else 0.1 * math.log(self.factor) + 1.0
+        return _SCALING[self.kind], self.factor, self.original_length, self.low_turns, high, size
+
+
+def rotary_tables(length: int, rotary_dim: int, theta: float, device, *, scaling: Optional[RopeScaling] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """cos/sin [length, rotary_dim / 2] fp32, angles formed in 64 bits (rope_tables forms them in fp32, as the reference does: at position 131072 that is 0.004 off)."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise _lib.OlmaxHipError("olmax_amd ops run on the GPU only; there is no CPU fallback")
+    _want(length > 0 and rotary_dim > 0 and rotary_dim % 2 == 0, f"rotary_tables: length must be positive and rotary_dim even (got {length}, {rotary_dim})")
+    cos, sin = torch.empty(2, length, rotary_dim // 2, device=device, dtype=torch.float32).unbind(0)
+    _place(cos)
+    kind, factor, original, low, high, size = (0, 1.0, 1.0, 1.0, 1.0, 1.0) if scaling is None else scaling.c_args()
+    check(_L().olmax_rotary_tables(stream_ptr(), ptr(cos), ptr(sin), i64(length), i32(rotary_dim), f64(theta), i32(kind), f64(factor), f64(original), f64(low), f64(high), f32(size)))
+    return cos, sin
+
+
+_LAYOUT = {"half": 0, "interleaved": 1}
+
+
+def _rotary(name, x, cos, sin, heads, head_dim, positions, seq_len, layout, out):
+    _place(x, cos, sin, positions, out)
+    width = heads * head_dim
+    _want(x.dim() == 2 and x.dtype in (BF16, torch.float32) and x.shape[1] >= width > 0 and x.stride(1) == 1, f"expected rows of {heads} x {head_dim} and more in bf16 or fp32")
+    T = x.shape[0]
+    _want(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous(),
+          "cos, sin: expected contiguous fp32 tables [positions, rotary_dim / 2]")
+    _want(positions is None or (positions.dtype == torch.int32 and positions.shape == (T,) and positions.is_contiguous()), f"positions: expected a contiguous int32 tensor [{T}]")
+    _want(layout in _LAYOUT, f"layout must be 'half' or 'interleaved' (got {layout!r})")
+    if out is None:
+        out = x.new_empty((T, width))
+    _want(out.dim() == 2 and out.dtype == x.dtype and out.shape[0] == T and out.shape[1] >= width and out.stride(1) == 1, "out: expected rows of x's type")
+    n = cos.shape[0]
+    check(typed(name)(raw_stream(), x.data_ptr(), out.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(positions), T, heads, head_dim, 2 * cos.shape[1], n,
+                      n if seq_len is None else seq_len, x.stride(0), out.stride(0), _LAYOUT[layout], 1 if x.dtype == torch.float32 else 0))
+    return out
+
+
+def rotary_fwd(x, cos, sin, *, heads: int, head_dim: int, positions=None, seq_len: Optional[int] = None, layout: str = "half", out=None):
+    """x: [tokens, >= heads*head_dim] view, bf16 or fp32.  The first rotary_dim = 2 * cos.shape[1] columns of every head are rotated by the angle of the token's position, the others
+    pass; pairs are (i, i + rotary_dim/2) in the "half" layout and (2i, 2i + 1) in the "interleaved" one.
+
+    positions [tokens] int32 (negative: padding, passes; beyond the tables: NaN), or token % seq_len, all rows of the tables if seq_len is None.  `out` may be x."""
+    return _rotary("olmax_rotary_fwd", x, cos, sin, heads, head_dim, positions, seq_len, layout, out)
+
+
+def rotary_bwd(dy, cos, sin, *, heads: int, head_dim: int, positions=None, seq_len: Optional[int] = None, layout: str = "half", out=None):
+    """Gradient of rotary_fwd: the rotation back (times the tables' size, as there)."""
+    return _rotary("olmax_rotary_bwd", dy, cos, sin, heads, head_dim, positions, seq_len, layout, out)
+
+
 # ----------------------------------------------------------------------------- gated MLP activation
 _ACT = {"silu": 0, "gelu": 1}
 
@@ -264,6 +342,63 @@ def attn_bwd(q, k, v, o, lse, do, *, B: int, S: int, H: int, KH: int, D: int, wi
     return dq, dk, dv
 
 
+# ----------------------------------------------------------------------------- differential attention
+class DiffAttention(NamedTuple):
+    """o = (P_1 - lam P_2) v; what the backward call takes beside it: o2 = P_2 v (None without) and both maps' log-normalisers [B, H, 2, S]."""
+    o: torch.Tensor
+    o2: Optional[torch.Tensor]
+    lse: torch.Tensor
+
+
+def _head_rows(t, T: int, width: int, what: str):
+    """A bf16 [T, width] operand, rows apart as far as they like; its row stride."""
+    _want(t.dim() == 2 and t.dtype == BF16 and t.shape == (T, width) and t.stride(1) == 1, f"{what}: expected bf16 rows [{T}, {width}]")
+    return t.stride(0) if T > 1 else width
+
+
+def _diff_sizes(lam, B: int, S: int, H: int, KH: int, D: int):
+    _want(B > 0 and S > 0 and H > 0 and KH > 0 and H % KH == 0 and D in (32, 64), f"bad shape B={B} S={S} H={H} KH={KH} D={D}: KH divides H, D is 32 or 64")
+    _want(lam.dtype == torch.float32 and lam.shape in ((H,), (1,)) and lam.is_contiguous(), f"lam: expected a contiguous fp32 tensor [{H}] or [1]")
+    return B * S, 2 * D * H, 2 * D * KH
+
+
+def diff_attn_fwd(q, k, v, lam, *, B: int, S: int, H: int, KH: int, D: int, window: Optional[int] = None, want_grad: bool = True, out=None) -> DiffAttention:
+    """Differential attention, o = (softmax(q1 k1^T / sqrt(D)) - lam softmax(q2 k2^T / sqrt(D))) v under attn_fwd's mask.
+
+    q [B*S, H*2D]: the two queries of a head lie side by side; k [B*S, KH*2D] likewise; v [B*S, KH*2D], o as q (row-strided views allowed, 16-byte aligned, strides
+    multiples of 8).  D is 32 or 64.  lam: fp32 [H], or [1] for all heads.  want_grad: o2 is kept for diff_attn_bwd."""
+    _place(q, k, v, lam, out)
+    T, wide, narrow = _diff_sizes(lam, B, S, H, KH, D)
+    ldq, ldk, ldv = _head_rows(q, T, wide, "q"), _head_rows(k, T, narrow, "k"), _head_rows(v, T, narrow, "v")
+    if out is None:
+        out = q.new_empty((T, wide))
+    o2 = q.new_empty((T, wide)) if want_grad else None
+    lse = lam.new_empty((B, H, 2, S))
+    check(typed("olmax_diff_attn_fwd")(raw_stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), out.data_ptr(), _ptr(o2), lse.data_ptr(), B, S, H, KH, D,
+                                       ldq, ldk, ldv, _head_rows(out, T, wide, "out"), wide, int(lam.shape[0] != H), -1 if window is None else window))
+    return DiffAttention(out, o2, lse)
+
+
+def diff_attn_bwd(q, k, v, lam, o, o2, lse, do, *, B: int, S: int, H: int, KH: int, D: int, window: Optional[int] = None, dq=None, dk=None, dv=None):
+    """Gradients of diff_attn_fwd from what it returned: (dq, dk, dv, dlam), dlam fp32 of lam's shape.  The same bits on every call."""
+    _place(q, k, v, lam, o, o2, lse, do, dq, dk, dv)
+    T, wide, narrow = _diff_sizes(lam, B, S, H, KH, D)
+    _want(o2 is not None, "o2 is missing: diff_attn_fwd(want_grad=True) keeps it")
+    _want(lse.dtype == torch.float32 and lse.shape == (B, H, 2, S) and lse.is_contiguous(), f"lse: expected a contiguous fp32 tensor [{B}, {H}, 2, {S}]")
+    dq = q.new_empty((T, wide)) if dq is None else dq
+    dk = q.new_empty((T, narrow)) if dk is None else dk
+    dv = q.new_empty((T, narrow)) if dv is None else dv
+    dlam = torch.empty_like(lam)
+    lds = [_head_rows(t, T, n, what) for t, n, what in ((q, wide, "q"), (k, narrow, "k"), (v, narrow, "v"), (o, wide, "o"), (o2, wide, "o2"), (do, wide, "do"),
+                                                        (dq, wide, "dq"), (dk, narrow, "dk"), (dv, narrow, "dv"))]
+    nbytes = _size32("olmax_diff_attn_bwd_workspace_bytes", B, S, H)
+    ws = q.new_empty((nbytes,), dtype=torch.uint8)
+    check(typed("olmax_diff_attn_bwd")(raw_stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), o.data_ptr(), o2.data_ptr(), lse.data_ptr(), do.data_ptr(),
+                                       dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), nbytes, B, S, H, KH, D, *lds, int(lam.shape[0] != H),
+                                       -1 if window is None else window))
+    return dq, dk, dv, dlam
+
+
 # ----------------------------------------------------------------------------- cross entropy / LM head
 def cross_entropy(logits, labels, *, ignore_index: int = -100, softcap: float = 0.0, want_grad: bool = True,
                   inplace: bool = False, dloss: float = 1.0, reduction: str = "mean", dloss_rows=None):
@@ -341,6 +476,16 @@ def _size(name: str, *args) -> int:
     if f is None:
         f = getattr(_L(), name)
         f.restype, f.argtypes = i64, [i64] + [i32] * (len(args) - 1)
+        _sizes[name] = f
+    return f(*args)
+
+
+def _size32(name: str, *args) -> int:
+    """One whose arguments are all 32 bits wide."""
+    f = _sizes.get(name)
+    if f is None:
+        f = getattr(_L(), name)
+        f.restype, f.argtypes = i64, [i32] * len(args)
         _sizes[name] = f
     return f(*args)
 

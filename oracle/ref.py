@@ -771,3 +771,80 @@ def _fnmatch(name: str, pat: str) -> bool:
     import fnmatch
 
     return fnmatch.fnmatch(name, pat)
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions and differential attention (no counterpart in the reference)
+# ---------------------------------------------------------------------------
+def rotary_freqs(rotary_dim, theta, *, kind=None, factor=1.0, original_length=8192, low_turns=1.0, high_turns=4.0):
+    """f_i of the angles p f_i, float64 [rotary_dim / 2]; kinds as olmax_rotary_tables describes them."""
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    f = theta ** (-2.0 * i / rotary_dim)
+    if kind is None:
+        return f
+    if kind == "linear":
+        keep = torch.zeros_like(f)
+    elif kind == "llama3":
+        keep = ((original_length * f / (2 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0, 1)
+    else:
+        at = lambda turns: rotary_dim * math.log(original_length / (2 * math.pi * turns)) / (2 * math.log(theta))  # noqa: E731
+        lo, hi = max(math.floor(at(high_turns)), 0), min(math.ceil(at(low_turns)), rotary_dim - 1)
+        keep = 1 - ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+    return keep * f + (1 - keep) * f / factor
+
+
+def rotary(x, cos, sin, positions, *, heads, head_dim, layout="half", back=False):
+    """x [T, heads * head_dim]; columns 0 .. 2 * cos.shape[1] - 1 of each head turn by row positions[t] of the tables, none where that is negative; a position beyond them: NaN."""
+    T, half = x.shape[0], cos.shape[1]
+    x = x.reshape(T, heads, head_dim)
+    p = positions.long()
+    c, s = cos[p.clamp(0, cos.shape[0] - 1)], sin[p.clamp(0, cos.shape[0] - 1)]
+    c, s = torch.where((p >= cos.shape[0])[:, None], math.nan, c)[:, None], (-s if back else s)[:, None]
+    c, s = torch.where((p < 0)[:, None, None], 1.0, c), torch.where((p < 0)[:, None, None], 0.0, s)
+    y = x.clone()
+    a, b = (slice(0, half), slice(half, 2 * half)) if layout == "half" else (slice(0, 2 * half, 2), slice(1, 2 * half, 2))
+    y[..., a] = x[..., a] * c - x[..., b] * s
+    y[..., b] = x[..., b] * c + x[..., a] * s
+    return y.reshape(T, heads * head_dim)
+
+
+def _diff_maps(q, k, B, S, H, KH, D, window):
+    """Scores of both maps [B, H, 2, S, S] and which pairs are visible [S, S]."""
+    q = q.reshape(B, S, H, 2, D).permute(0, 2, 3, 1, 4)
+    k = k.reshape(B, S, KH, 2, D).permute(0, 2, 3, 1, 4).repeat_interleave(H // KH, 1)
+    i = torch.arange(S)
+    seen = i[:, None] >= i[None, :]
+    if window is not None and window >= 0:
+        seen &= i[:, None] - i[None, :] <= window
+    return q @ k.transpose(-1, -2) * D ** -0.5, seen, q, k
+
+
+def diff_attn_fwd(q, k, v, lam, *, B, S, H, KH, D, window=None):
+    """(o, o2 [B S, H 2D], lse [B, H, 2, S]), see olmax_diff_attn_fwd; lam [H] or [1]."""
+    s, seen, _, _ = _diff_maps(q, k, B, S, H, KH, D, window)
+    s = s.masked_fill(~seen, -math.inf)
+    p = torch.softmax(s, -1)
+    v = v.reshape(B, S, KH, 2 * D).permute(0, 2, 1, 3).repeat_interleave(H // KH, 1)
+    rows = lambda t: t.permute(0, 2, 1, 3).reshape(B * S, H * 2 * D)  # noqa: E731
+    maps = p @ v[:, :, None]
+    w = lam.expand(H)[:, None, None]
+    return rows(maps[:, :, 0] - w * maps[:, :, 1]), rows(maps[:, :, 1]), torch.logsumexp(s, -1)
+
+
+def diff_attn_bwd(q, k, v, lam, do, *, B, S, H, KH, D, window=None):
+    """(dq, dk, dv, dlam) by the formulas of olmax_diff_attn_bwd."""
+    s, seen, qh, kh = _diff_maps(q, k, B, S, H, KH, D, window)
+    p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+    vh = v.reshape(B, S, KH, 2 * D).permute(0, 2, 1, 3).repeat_interleave(H // KH, 1)
+    doh = do.reshape(B, S, H, 2 * D).permute(0, 2, 1, 3)
+    w = lam.expand(H)[:, None, None]
+    dp = (doh @ vh.transpose(-1, -2))[:, :, None]
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    ds = torch.stack([ds[:, :, 0], -w * ds[:, :, 1]], 2) * D ** -0.5
+    shared = lambda t: t.reshape(B, KH, H // KH, *t.shape[2:]).sum(2)  # noqa: E731
+    dq = (ds @ kh).permute(0, 3, 1, 2, 4).reshape(B * S, H * 2 * D)
+    dk = shared(ds.transpose(-1, -2) @ qh).permute(0, 3, 1, 2, 4).reshape(B * S, KH * 2 * D)
+    dv = shared((p[:, :, 0] - w * p[:, :, 1]).transpose(-1, -2) @ doh).permute(0, 2, 1, 3).reshape(B * S, KH * 2 * D)
+    dlam = -delta[:, :, 1, :, 0].sum((0, 2))
+    return dq, dk, dv, dlam.sum().view(1) if lam.shape[0] != H else dlam
