@@ -118,10 +118,10 @@ __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ld
   for (int c = 0; c < W / 64; c++) dq[c * 64 + lane] = f2bf(acc[c] * scale);
 }
 
-// key j; Q, dO of the first of its rep query heads, stats (of a head and map: S numbers) of the first of them
+// key j, columns [lo, hi); Q, dO of the first of its rep query heads, stats (of a head and map: S numbers) of the first of them
 template <int W>
 __device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16* dO, int64_t lddo, const float* lse, const float* delta, const float* lam, int lam_step, const bf16* k,
-                                         const bf16* v, bf16* dk, bf16* dv, int j, int S, int rep, int window, float scale, int lane) {
+                                         const bf16* v, bf16* dk, bf16* dv, int j, int S, int rep, int window, float scale, int lane, int lo, int hi) {
   constexpr int D = W / 2;
   const int last = window >= 0 ? min(S - 1, j + window) : S - 1;
   float ak[W / 64] = {}, av[W / 64] = {};
@@ -151,183 +151,222 @@ __device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16*
     }
 #pragma unroll
   for (int c = 0; c < W / 64; c++) {
-    dk[c * 64 + lane] = f2bf(ak[c] * scale);
-    dv[c * 64 + lane] = f2bf(av[c]);
+    const int at = c * 64 + lane;
+    if (at < lo || at >= hi) continue;
+    dk[at] = f2bf(ak[c] * scale);
+    dv[at] = f2bf(av[c]);
   }
 }
 
-constexpr int QR = 128, KR = 128;  // queries, keys of a workgroup of four waves
+constexpr int QR = 128;  // queries of a workgroup
 
 // ---------------------------------------------------------------------------------------
-// Forward.  grid = ceil(S / 128) H B workgroups of 4 waves; a wave owns 32 queries and both their maps.
+// Forward.  grid = ceil(S / 128) H B workgroups of 8 waves; wave (qw, m) owns 32 queries and one map, and the two waves of a SIMD, qw of either map, take turns: a key tile is two parts, the softmax
+// (vector unit) and the products (matrix unit: this tile's probabilities with V, the next tile's scores), a barrier ends each, and map 1 is one part behind map 0.
+// LDS: 3 stages of K, then of V.  Map 0's waves fetch K, map 1's V.  K(t) is read in parts 2t - 1 and 2t, V(t) in 2t + 1 and 2t + 2 (counted as map 0 does), so that K(t + 3) is issued in 2t + 1 and
+// V(t + 2) too, and each has four parts to land; past the end the last tile is fetched again.
 // ---------------------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ void part_ends() {  // at most the newest N transfers of this wave are under way; its LDS reads are done
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+constexpr int smem_fwd(int W) { return 2 * 3 * 64 * W * 2; }
 template <int W>
-__global__ __launch_bounds__(256, 2) void diff_attn_fwd_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+__global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
                                                                bf16* __restrict__ O, bf16* __restrict__ O2, float* __restrict__ LSE, const Sizes z) {
   constexpr int TILE = 64 * W * 2;  // bytes of a K or V tile of 64 keys
   constexpr int KS = W / 32;        // k-steps of a map
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];  // [2][K | V]
+  constexpr int INS = 64 * W / 2048;  // transfers of a wave and tile
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];  // [3] K, [3] V
   const int S = z.S, H = z.H, KH = z.KH, window = z.window;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lhi = lane >> 5;
+  const int qw = wave & 3, m = wave >> 2;
   const int nqt = (S + QR - 1) / QR;
   const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
   const int qt = nqt - 1 - wg.rank;  // longest rows first
   const int b = wg.group / KH, kh = wg.group % KH;
   const int h = kh * (H / KH) + wg.r;
   const int i0 = qt * QR;
-  const int iw0 = i0 + wave * 32;
+  const int iw0 = i0 + qw * 32;
   const int qi = iw0 + l32;  // this lane's query
   const int qic = min(qi, S - 1);
 
-  bf16x8 qf[W / 16];
+  bf16x8 qf[KS];
   {
-    const bf16* qp = Q + ((int64_t)b * S + qic) * z.ldq + h * W + lhi * 8;
+    const bf16* qp = Q + ((int64_t)b * S + qic) * z.ldq + h * W + m * (W / 2) + lhi * 8;
 #pragma unroll
-    for (int s = 0; s < W / 16; s++) qf[s] = *reinterpret_cast<const bf16x8*>(qp + s * 16);
+    for (int s = 0; s < KS; s++) qf[s] = *reinterpret_cast<const bf16x8*>(qp + s * 16);
   }
   const int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
   const int t_hi = min(i0 + QR - 1, S - 1) >> 6;  // inclusive
 
-  f32x16 o[2][W / 32];
+  f32x16 o[W / 32], st[2];
 #pragma unroll
-  for (int m = 0; m < 2; m++)
+  for (int dt = 0; dt < W / 32; dt++)
 #pragma unroll
-    for (int dt = 0; dt < W / 32; dt++)
-#pragma unroll
-      for (int r = 0; r < 16; r++) o[m][dt][r] = 0.f;
-  float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    for (int r = 0; r < 16; r++) o[dt][r] = 0.f;
+  float mx = -INFINITY, sum = 0.f;
 
   const bf16* kbase = K + (int64_t)b * S * z.ldk + kh * W;
   const bf16* vbase = V + (int64_t)b * S * z.ldv + kh * W;
   const unsigned lds0 = lds_addr_of(smem);
-  TileDma<64, W> dk, dv;
-  dk.init(z.ldk, wave, lane);
-  dv.init(z.ldv, wave, lane);
-  auto load_kv = [&](int t, int stage) {
-    const unsigned dst = lds0 + stage * (2 * TILE);
-    if (t * 64 + 64 <= S) {
-      dk.issue(kbase + (int64_t)t * 64 * z.ldk, dst, wave);
-      dv.issue(vbase + (int64_t)t * 64 * z.ldv, dst + TILE, wave);
-    } else {
-      dma_tile<64, W>(kbase, z.ldk, t * 64, S, dst, wave, lane);
-      dma_tile<64, W>(vbase, z.ldv, t * 64, S, dst + TILE, wave, lane);
-    }
+  const bf16* base = m ? vbase : kbase;
+  const int64_t ld = m ? z.ldv : z.ldk;
+  TileDma<64, W> dma;
+  dma.init(ld, qw, lane);
+  auto load = [&](int t, int stage) {  // of this wave's operand
+    t = min(t, t_hi);
+    const unsigned dst = lds0 + (m * 3 + stage) * TILE;
+    if (t * 64 + 64 <= S) dma.issue(base + (int64_t)t * 64 * ld, dst, qw);
+    else dma_tile<64, W>(base, ld, t * 64, S, dst, qw, lane);
   };
   const float sc2 = z.scale * LOG2E;
   FragAddr<W> fa;
   fa.init(lane);
-
-  load_kv(t_lo, 0);
-  dma_wait_all();
-  __syncthreads();
-  for (int t = t_lo; t <= t_hi; t++) {
-    const int cur = (t - t_lo) & 1, j0 = t * 64;
-    if (t < t_hi) load_kv(t + 1, cur ^ 1);
-    const bool visible = j0 <= iw0 + 31 && (window < 0 || j0 + 63 >= iw0 - window);
-    if (visible) {
-      const unsigned char* sk = smem + cur * (2 * TILE);
-      const unsigned char* sv = sk + TILE;
-      const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
-      bf16x8 pb[2][4];
+  const int kmap = (m * KS) << 5;  // of the swizzled chunk index: this map's k-steps (KS is 2 or 4: the bits are apart)
+  auto visible = [&](int t) { return t * 64 <= iw0 + 31 && (window < 0 || t * 64 + 63 >= iw0 - window); };
+  auto scores = [&](int stage) {
+    const unsigned char* sk = smem + stage * TILE;
 #pragma unroll
-      for (int m = 0; m < 2; m++) {
-        f32x16 st[2];
+    for (int jt = 0; jt < 2; jt++)
 #pragma unroll
-        for (int jt = 0; jt < 2; jt++)
+      for (int r = 0; r < 16; r++) st[jt][r] = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; r++) st[jt][r] = 0.f;
+    for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int s = m * KS; s < (m + 1) * KS; s++)
-#pragma unroll
-          for (int jt = 0; jt < 2; jt++) st[jt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, s), qf[s], st[jt], 0, 0, 0);
-        if (need_mask) {
-#pragma unroll
-          for (int jt = 0; jt < 2; jt++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-              const int j = j0 + jt * 32 + (r >> 2) * 8 + lhi * 4 + (r & 3);
-              const bool ok = (j <= qi) && (window < 0 || j >= qi - window);
-              st[jt][r] = ok ? st[jt][r] : -INFINITY;
-            }
-        }
-        float mt = -INFINITY;
-#pragma unroll
-        for (int jt = 0; jt < 2; jt++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) mt = fmaxf(mt, st[jt][r]);
-        mt = half_swap_max(mt * sc2);
-        // the reference of the exponentials moves when a row's maximum has grown by 2^8 (as in attn.hip)
-        if (__builtin_amdgcn_ballot_w64(mt > mx[m] + 8.f) != 0) {
-          const float m_new = fmaxf(mx[m], mt);
-          const float alpha = fexp2(mx[m] - (m_new == -INFINITY ? 0.f : m_new));
-          sum[m] *= alpha;
-          mx[m] = m_new;
-#pragma unroll
-          for (int dt = 0; dt < W / 32; dt++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[m][dt][r] *= alpha;
-        }
-        const float ref = mx[m] == -INFINITY ? 0.f : mx[m];
-#pragma unroll
-        for (int jt = 0; jt < 2; jt++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) st[jt][r] = fexp2(__builtin_fmaf(st[jt][r], sc2, -ref));
-#pragma unroll
-        for (int u = 0; u < 4; u++) pb[m][u] = pack_bf16x8(st[u >> 1], (u & 1) * 8);
-        float ps[16];  // the sum in fp32, pairwise
-#pragma unroll
-        for (int r = 0; r < 16; r++) ps[r] = st[0][r] + st[1][r];
-#pragma unroll
-        for (int w = 8; w > 0; w >>= 1)
-#pragma unroll
-          for (int r = 0; r < w; r++) ps[r] += ps[r + w];
-        sum[m] += ps[0];
+      for (int jt = 0; jt < 2; jt++) {
+        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(sk + (fa.kc[s] ^ kmap) + jt * 32 * (2 * W));
+        st[jt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[s], st[jt], 0, 0, 0);
       }
+  };
+
+  load(t_lo, 0);
+  load(t_lo + 1, 1);
+  if (m == 0) load(t_lo + 2, 2);
+  part_ends<0>();
+  if (visible(t_lo)) scores(0);
+  if (m == 1) part_ends<0>();
+  int stage = 0;  // of tile t
+  for (int t = t_lo; t <= t_hi; t++) {
+    const int next = stage == 2 ? 0 : stage + 1, after = next == 2 ? 0 : next + 1;
+    const bool vis = visible(t);
+    // ---- softmax
+    if (m == 1) load(t + 2, after);
+    bf16x8 pb[4];
+    if (vis) {
+      const int j0 = t * 64;
+      const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
+      if (need_mask) {
+#pragma unroll
+        for (int jt = 0; jt < 2; jt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int j = j0 + jt * 32 + (r >> 2) * 8 + lhi * 4 + (r & 3);
+            const bool ok = (j <= qi) && (window < 0 || j >= qi - window);
+            st[jt][r] = ok ? st[jt][r] : -INFINITY;
+          }
+      }
+      float mt = -INFINITY;
+#pragma unroll
+      for (int jt = 0; jt < 2; jt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) mt = fmaxf(mt, st[jt][r]);
+      mt = half_swap_max(mt * sc2);
+      // the reference of the exponentials moves when a row's maximum has grown by 2^8 (as in attn.hip)
+      if (__builtin_amdgcn_ballot_w64(mt > mx + 8.f) != 0) {
+        const float m_new = fmaxf(mx, mt);
+        const float alpha = fexp2(mx - (m_new == -INFINITY ? 0.f : m_new));
+        sum *= alpha;
+        mx = m_new;
+#pragma unroll
+        for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[dt][r] *= alpha;
+      }
+      const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int jt = 0; jt < 2; jt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) st[jt][r] = fexp2(__builtin_fmaf(st[jt][r], sc2, -ref));
+#pragma unroll
+      for (int u = 0; u < 4; u++) pb[u] = pack_bf16x8(st[u >> 1], (u & 1) * 8);
+      float ps[16];  // the sum in fp32, pairwise
+#pragma unroll
+      for (int r = 0; r < 16; r++) ps[r] = st[0][r] + st[1][r];
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+        for (int r = 0; r < w; r++) ps[r] += ps[r + w];
+      sum += ps[0];
+    }
+    part_ends<INS>();
+    // ---- products
+    if (m == 0) load(t + 3, stage);
+    if (vis) {
+      const unsigned char* sv = smem + (3 + stage) * TILE;
 #pragma unroll
       for (int u = 0; u < 4; u++)
 #pragma unroll
-        for (int dt = 0; dt < W / 32; dt++) {
-          const bf16x8 vf = fa.load_tr(sv, u * 16, dt);
-          o[0][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[0][u], o[0][dt], 0, 0, 0);
-          o[1][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[1][u], o[1][dt], 0, 0, 0);
-        }
+        for (int dt = 0; dt < W / 32; dt++) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_tr(sv, u * 16, dt), pb[u], o[dt], 0, 0, 0);
     }
-    dma_wait_all();
-    __syncthreads();
+    if (t < t_hi && visible(t + 1)) scores(next);
+    part_ends<INS>();
+    stage = next;
   }
-  float inv[2], lse[2], zeros = 0.f;
-#pragma unroll
-  for (int m = 0; m < 2; m++) {
-    const float total = half_swap_sum(sum[m]);
-    inv[m] = total > 0.f ? 1.f / total : 0.f;
-    lse[m] = (mx[m] + log2f(total)) * LN2;
-    zeros = __builtin_fmaf(lse[m], 0.f, zeros);
-  }
+  if (m == 0) part_ends<0>();
+  dma_wait_all();
+  __syncthreads();
+
+  const float total = half_swap_sum(sum);
+  const float inv = total > 0.f ? 1.f / total : 0.f;
+  const float lse = (mx + log2f(total)) * LN2;
+  float zeros = lse * 0.f;  // NaN where something of a row is not finite; rows behind the sequence are none
   const float lam = LAM[z.shared ? 0 : h];
   float* lse_row = LSE + ((int64_t)b * H + h) * 2 * S;
+  if (lhi == 0 && qi < S) lse_row[m * S + qi] = lse;
+  // the second map's rows through LDS (its lanes own what the first one's do)
+  f32x4* park = reinterpret_cast<f32x4*>(smem) + qw * (W / 8 * 64) + lane;
+  if (m == 1) {
+    bf16* o2p = O2 ? O2 + ((int64_t)b * S + qic) * z.ldo2 + h * W : nullptr;
+#pragma unroll
+    for (int u = 0; u < W / 8; u++) {
+      f32x4 y;
+      Pack4 pk;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        y[e] = o[u >> 2][(u & 3) * 4 + e] * inv;
+        pk.e[e] = f2bf(y[e]);
+        zeros = __builtin_fmaf(y[e], 0.f, zeros);
+      }
+      park[u * 64] = y;
+      if (O2 && qi < S) *reinterpret_cast<u32x2*>(o2p + u * 8 + lhi * 4) = pk.u;
+    }
+    if (qi >= S) zeros = 0.f;
+    reinterpret_cast<float*>(smem + 4 * 32 * W * 4)[qw * 64 + lane] = zeros;
+    if (__builtin_amdgcn_ballot_w64(zeros != 0.f)) dma_wait_all();  // the other wave of these rows is going to store them over
+  }
+  __syncthreads();
+  if (m == 1) return;
+  zeros += reinterpret_cast<float*>(smem + 4 * 32 * W * 4)[qw * 64 + lane];
   if (qi < S) {
     bf16* op = O + ((int64_t)b * S + qi) * z.ldo + h * W;
-    bf16* o2p = O2 ? O2 + ((int64_t)b * S + qi) * z.ldo2 + h * W : nullptr;
 #pragma unroll
-    for (int dt = 0; dt < W / 32; dt++)
+    for (int u = 0; u < W / 8; u++) {
+      const f32x4 y = park[u * 64];
+      Pack4 pk;
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        Pack4 pk, p2;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float y = o[1][dt][g * 4 + e] * inv[1], x = __builtin_fmaf(o[0][dt][g * 4 + e], inv[0], -lam * y);
-          zeros = __builtin_fmaf(x, 0.f, zeros);
-          pk.e[e] = f2bf(x);
-          p2.e[e] = f2bf(y);
-        }
-        *reinterpret_cast<u32x2*>(op + dt * 32 + g * 8 + lhi * 4) = pk.u;
-        if (O2) *reinterpret_cast<u32x2*>(o2p + dt * 32 + g * 8 + lhi * 4) = p2.u;
+      for (int e = 0; e < 4; e++) {
+        const float x = __builtin_fmaf(o[u >> 2][(u & 3) * 4 + e], inv, -lam * y[e]);
+        zeros = __builtin_fmaf(x, 0.f, zeros);
+        pk.e[e] = f2bf(x);
       }
-    if (lhi == 0) {
-      lse_row[qi] = lse[0];
-      lse_row[S + qi] = lse[1];
+      *reinterpret_cast<u32x2*>(op + u * 8 + lhi * 4) = pk.u;
     }
   } else {
     zeros = 0.f;
@@ -505,27 +544,35 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
 }
 
 // ---------------------------------------------------------------------------------------
-// dK/dV.  grid = ceil(S / 128) KH B workgroups of 4 waves; a wave owns 32 keys (K in registers) and walks the query heads of its group and their 32-row tiles from the diagonal on.
-// LDS: 2 stages of (Q | dO | lse_1, lse_2, -delta_1, delta_1 - delta_2 of the 32 rows), then the V tile.
+// dK/dV.  grid = ceil(S / 32 KW) KH B workgroups of KW x QS waves; wave (kw, qs) owns 32 keys (K in registers) and every QS-th of the pairs of a query head of the group and one of its 32-row
+// tiles from the diagonal on.  LDS: per query group 2 stages of (Q | dO | lse_1, lse_2, -delta_1, delta_1 - delta_2 of the 32 rows), then the V tile.
+// KW = 4, QS = 1: two workgroups per CU, no reduction.  KW = 2, QS = 4: one workgroup of eight waves per CU, half the keys and a quarter of the chain; the four partial sums are added through LDS
+// in group order.  See dkv_split.
 // ---------------------------------------------------------------------------------------
 constexpr int smem_q(int W) { return 2 * 2 * 64 * W * 2; }
-constexpr int smem_kv(int W) { return 2 * (2 * 32 * W * 2 + 512) + KR * W * 2; }
-template <int W>
-__global__ __launch_bounds__(256, 2) void diff_attn_dkv_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
-                                                               const float* __restrict__ LSE, const float* __restrict__ DELTA, const bf16* __restrict__ dO, bf16* __restrict__ dK,
-                                                               bf16* __restrict__ dV, const Sizes z, const Grad gr) {
+constexpr int smem_kv(int W, int KW, int QS) {
+  const int run = QS * 2 * (2 * 32 * W * 2 + 512) + KW * 32 * W * 2, sums = QS > 1 ? KW * QS * 32 * W * 4 : 0;
+  return run > sums ? run : sums;
+}
+template <int W, int KW, int QS>
+__global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+                                                                        const float* __restrict__ LSE, const float* __restrict__ DELTA, const bf16* __restrict__ dO,
+                                                                        bf16* __restrict__ dK, bf16* __restrict__ dV, const Sizes z, const Grad gr) {
   constexpr int QT = 32, KS = W / 32;
   constexpr int TILE = QT * W * 2, STAGE = 2 * TILE + 512;
+  constexpr int KT = KW * 32;         // keys of the workgroup
+  constexpr int TEAMS = KW * QS / 4;  // tiles are fetched by teams of 4 waves
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int S = z.S, H = z.H, KH = z.KH, window = z.window;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lhi = lane >> 5;
-  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / ((S + KR - 1) / KR)), 1);  // key tile 0 is seen by every query: longest first
+  const int kw = wave % KW, qs = wave / KW, wv = wave & 3, team = wave >> 2;
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / ((S + KT - 1) / KT)), 1);  // key tile 0 is seen by every query: longest first
   const int b = wg.group / KH, kh = wg.group % KH;
   const int rep = H / KH;
-  const int j0 = wg.rank * KR;
-  const int jw0 = j0 + wave * 32;
+  const int j0 = wg.rank * KT;
+  const int jw0 = j0 + kw * 32;
   const int kj = jw0 + l32;  // this lane's key
   const int kjc = min(kj, S - 1);
 
@@ -541,42 +588,60 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dkv_kernel(const bf16* __res
 #pragma unroll
     for (int r = 0; r < 16; r++) { dk[dt][r] = 0.f; dv[dt][r] = 0.f; }
 
-  const int i_hi = window >= 0 ? min(S - 1, j0 + KR - 1 + window) : S - 1;
+  const int i_hi = window >= 0 ? min(S - 1, j0 + KT - 1 + window) : S - 1;
   const int t_lo = j0 / QT, t_hi = i_hi / QT;  // inclusive
   const int ntile = t_hi - t_lo + 1;
-  const int64_t total = (int64_t)ntile * rep;  // (head, tile) pairs, heads outermost
+  const int total = ntile * rep;  // (head, tile) pairs, heads outermost
   const float sc2 = z.scale * LOG2E;
   const unsigned lds0 = lds_addr_of(smem);
+  const unsigned char* sgrp = smem + qs * (2 * STAGE);  // this query group's stages
 
   TileDma<QT, W> tq, tdo;
-  tq.init(z.ldq, wave, lane);
-  tdo.init(gr.lddo, wave, lane);
-  int ld_h = kh * rep, ld_t = t_lo;  // next pair to load
+  tq.init(z.ldq, wv, lane);
+  tdo.init(gr.lddo, wv, lane);
+  // (head, tile) of the next iteration to load of each query group this team fetches for, and of this wave's own group (its rows' statistics)
+  struct Iter { int h, t; };
+  auto advance = [&](Iter& x, int n) {
+    x.t += n;
+    while (x.t > t_hi) {
+      x.t -= ntile;
+      ++x.h;
+    }
+  };
+  Iter own{kh * rep, t_lo}, ld[QS / TEAMS];
+  advance(own, qs);
+#pragma unroll
+  for (int g = 0; g < QS / TEAMS; g++) {
+    ld[g] = Iter{kh * rep, t_lo};
+    advance(ld[g], g * TEAMS + team);
+  }
   float sreg[2];
-  auto load_tile = [&](int stage) {
-    const int hq = ld_h, t = ld_t;
-    if (++ld_t > t_hi) {
-      ld_t = t_lo;
-      ++ld_h;
+  auto load_tile = [&](int round, int stage) {
+#pragma unroll
+    for (int g = 0; g < QS / TEAMS; g++) {
+      const int grp = g * TEAMS + team;
+      if (QS > 1 && round * QS + grp >= total) break;
+      const int hq = ld[g].h, t = ld[g].t;
+      advance(ld[g], QS);
+      const unsigned dst = lds0 + (grp * 2 + stage) * STAGE;
+      const bf16 *qp = Q + (int64_t)b * S * z.ldq + hq * W, *dp = dO + (int64_t)b * S * gr.lddo + hq * W;
+      if (t * QT + QT <= S) {
+        tq.issue(qp + (int64_t)t * QT * z.ldq, dst, wv);
+        tdo.issue(dp + (int64_t)t * QT * gr.lddo, dst + TILE, wv);
+      } else {
+        dma_tile<QT, W>(qp, z.ldq, t * QT, S, dst, wv, lane);
+        dma_tile<QT, W>(dp, gr.lddo, t * QT, S, dst + TILE, wv, lane);
+      }
     }
-    const unsigned dst = lds0 + stage * STAGE;
-    const bf16 *qp = Q + (int64_t)b * S * z.ldq + hq * W, *dp = dO + (int64_t)b * S * gr.lddo + hq * W;
-    if (t * QT + QT <= S) {
-      tq.issue(qp + (int64_t)t * QT * z.ldq, dst, wave);
-      tdo.issue(dp + (int64_t)t * QT * gr.lddo, dst + TILE, wave);
-    } else {
-      dma_tile<QT, W>(qp, z.ldq, t * QT, S, dst, wave, lane);
-      dma_tile<QT, W>(dp, gr.lddo, t * QT, S, dst + TILE, wave, lane);
-    }
-    if (wave == 0) {  // lanes 0 .. 31 the first map's, 32 .. 63 the second's
-      const int64_t at = (((int64_t)b * H + hq) * 2 + lhi) * S + min(t * QT + l32, S - 1);
+    if (kw == 0 && (QS == 1 || round * QS + qs < total)) {  // lanes 0 .. 31 the first map's, 32 .. 63 the second's
+      const int64_t at = (((int64_t)b * H + own.h) * 2 + lhi) * S + min(own.t * QT + l32, S - 1);
       sreg[0] = LSE[at];
       sreg[1] = DELTA[at];
     }
   };
-  auto store_stats = [&](int stage) {
-    if (wave == 0) {
-      float* p = reinterpret_cast<float*>(smem + stage * STAGE + 2 * TILE);
+  auto store_stats = [&](int stage) {  // (scaled here, an iteration after the load: see attn.hip)
+    if (kw == 0) {
+      float* p = reinterpret_cast<float*>(smem + (qs * 2 + stage) * STAGE + 2 * TILE);
       p[lane] = sreg[0] * LOG2E;
       p[64 + lane] = sreg[1];
     }
@@ -584,22 +649,27 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dkv_kernel(const bf16* __res
 
   FragAddr<W> fa;
   fa.init(lane);
-  const unsigned char* svt = smem + 2 * STAGE;  // [128 keys][W] V tile
-  dma_tile<KR, W>(V + (int64_t)b * S * z.ldv + kh * W, z.ldv, j0, S, lds0 + 2 * STAGE, wave, lane);
-  load_tile(0);
+  const unsigned char* svt = smem + QS * 2 * STAGE;  // [KT keys][W] V tile
+  if (team == 0) dma_tile<KT, W>(V + (int64_t)b * S * z.ldv + kh * W, z.ldv, j0, S, lds0 + QS * 2 * STAGE, wv, lane);
+  load_tile(0, 0);
   store_stats(0);
   dma_wait_all();
   __syncthreads();
-  int hq = kh * rep, t = t_lo;
-  for (int64_t it = 0; it < total; it++) {
-    const int cur = (int)(it & 1);
-    const bool more = it + 1 < total;
-    if (more) load_tile(cur ^ 1);
-    const int ib = t * QT;  // first query of the tile
-    const float nlam = -LAM[z.shared ? 0 : hq];
-    const bool visible = (ib + QT - 1 >= jw0) && (window < 0 || ib <= jw0 + 31 + window);
+  const int rounds = (total + QS - 1) / QS;
+  Iter cur_it{kh * rep, t_lo};  // being consumed
+  advance(cur_it, qs);
+  for (int round = 0; round < rounds; round++) {
+    const int cur = round & 1;
+    const bool more = round + 1 < rounds;
+    if (more) {
+      advance(own, QS);
+      load_tile(round + 1, cur ^ 1);
+    }
+    const int ib = cur_it.t * QT;  // first query of the tile
+    const bool visible = (QS == 1 || round * QS + qs < total) && (ib + QT - 1 >= jw0) && (window < 0 || ib <= jw0 + 31 + window);
     if (visible) {
-      const unsigned char* sq = smem + cur * STAGE;
+      const float nlam = -LAM[z.shared ? 0 : cur_it.h];
+      const unsigned char* sq = sgrp + cur * STAGE;
       const unsigned char* so = sq + TILE;
       const float* stats = reinterpret_cast<const float*>(sq + 2 * TILE);
       const bool need_mask = (ib < jw0 + 31) || (ib + QT > S) || (window >= 0 && ib + QT - 1 > jw0 + window);
@@ -617,8 +687,7 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dkv_kernel(const bf16* __res
         s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sq, 0, KS + s), kf[KS + s], s2, 0, 0, 0);
       }
 #pragma unroll
-      for (int s = 0; s < 2 * KS; s++) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(so, 0, s), fa.load_kc(svt, wave * 32, s), dp, 0, 0, 0);
-      f32x16 p;
+      for (int s = 0; s < 2 * KS; s++) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(so, 0, s), fa.load_kc(svt, kw * 32, s), dp, 0, 0, 0);
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         const int il = g * 8 + lhi * 4;
@@ -638,12 +707,12 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dkv_kernel(const bf16* __res
           }
           s1[r] = x;
           s2[r] = y;
-          p[r] = w;
+          dp[r] = w;
         }
       }
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const bf16x8 a = pack_bf16x8(s1, u * 8), c = pack_bf16x8(s2, u * 8), w = pack_bf16x8(p, u * 8);
+        const bf16x8 a = pack_bf16x8(s1, u * 8), c = pack_bf16x8(s2, u * 8), w = pack_bf16x8(dp, u * 8);
 #pragma unroll
         for (int dt = 0; dt < W / 32; dt++) {
           dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_tr(so, u * 16, dt), w, dv[dt], 0, 0, 0);
@@ -651,41 +720,50 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dkv_kernel(const bf16* __res
         }
       }
     }
-    if (++t > t_hi) {
-      t = t_lo;
-      ++hq;
-    }
+    advance(cur_it, QS);
     if (more) store_stats(cur ^ 1);
     dma_wait_all();
     __syncthreads();
   }
+  bf16* kp = dK + ((int64_t)b * S + kjc) * gr.lddk + kh * W;
+  bf16* vp = dV + ((int64_t)b * S + kjc) * gr.lddv + kh * W;
   float zeros = 0.f;
-  auto store4 = [&](bf16* p, int dt, int g, const f32x16& v, float mul) {
+  auto store4 = [&](bf16* p, int dt, int g, const f32x4& v, float mul) {
     Pack4 pk;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float x = v[g * 4 + e] * mul;
+      const float x = v[e] * mul;
       zeros = __builtin_fmaf(x, 0.f, zeros);
       pk.e[e] = f2bf(x);
     }
     *reinterpret_cast<u32x2*>(p + dt * 32 + g * 8 + lhi * 4) = pk.u;
   };
-  if (kj < S) {
-    bf16* kp = dK + ((int64_t)b * S + kj) * gr.lddk + kh * W;
-    bf16* vp = dV + ((int64_t)b * S + kj) * gr.lddv + kh * W;
+  if constexpr (QS == 1) {
+    if (kj < S) {
 #pragma unroll
-    for (int dt = 0; dt < W / 32; dt++)
+      for (int dt = 0; dt < W / 32; dt++)
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        store4(kp, dt, g, dk[dt], z.scale);
-        store4(vp, dt, g, dv[dt], 1.f);
-        __builtin_amdgcn_sched_barrier(0);  // a row leaves in order (see attn.hip)
-      }
+        for (int g = 0; g < 4; g++) {
+          store4(kp, dt, g, f32x4{dk[dt][g * 4], dk[dt][g * 4 + 1], dk[dt][g * 4 + 2], dk[dt][g * 4 + 3]}, z.scale);
+          store4(vp, dt, g, f32x4{dv[dt][g * 4], dv[dt][g * 4 + 1], dv[dt][g * 4 + 2], dv[dt][g * 4 + 3]}, 1.f);
+          __builtin_amdgcn_sched_barrier(0);  // a row leaves in order (see attn.hip)
+        }
+    }
+  } else {
+    // the stages are free: the last round ended in a barrier; dK first, then dV in the same space
+    add_partials<W, QS>(smem, dk, kw, qs, lane, [&](int u, const f32x4& v) {
+      if (kj < S) store4(kp, u >> 2, u & 3, v, z.scale);
+    });
+    __syncthreads();
+    add_partials<W, QS>(smem, dv, kw, qs, lane, [&](int u, const f32x4& v) {
+      if (kj < S) store4(vp, u >> 2, u & 3, v, 1.f);
+    });
   }
-  redo_rows(zeros, [&](int r) {
+  redo_rows(kj < S ? zeros : 0.f, [&](int r) {
     const int64_t seq = (int64_t)b * S, at = seq + jw0 + r, row = ((int64_t)b * H + kh * rep) * 2 * S;
     redo_dkv<W>(Q + seq * z.ldq + kh * rep * W, z.ldq, dO + seq * gr.lddo + kh * rep * W, gr.lddo, LSE + row, DELTA + row, LAM + (z.shared ? 0 : kh * rep), z.shared ? 0 : 1,
-                K + at * z.ldk + kh * W, V + at * z.ldv + kh * W, dK + at * gr.lddk + kh * W, dV + at * gr.lddv + kh * W, jw0 + r, S, rep, window, z.scale, lane);
+                K + at * z.ldk + kh * W, V + at * z.ldv + kh * W, dK + at * gr.lddk + kh * W, dV + at * gr.lddv + kh * W, jw0 + r, S, rep, window, z.scale, lane,
+                qs * (W / QS), (qs + 1) * (W / QS));
   });
 }
 
@@ -718,16 +796,20 @@ bool rows_ok(const void* p, int64_t ld, int64_t width) { return aligned16(p) && 
 
 int check_shape(const char* name, int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D) {
   OLMAX_CHECK(B > 0 && S > 0 && H > 0 && KH > 0 && H % KH == 0 && S <= (1 << 24) && H <= (1 << 16), OLMAX_ERR_SHAPE, "%s: bad shape B=%d S=%d H=%d KH=%d", name, B, S, H, KH);
+  OLMAX_CHECK(((int64_t)S / 32 + 2) * (H / KH) < (1LL << 31), OLMAX_ERR_SHAPE, "%s: S=%d tokens of %d query heads to a key head are too many", name, S, H / KH);
   OLMAX_CHECK(D == 32 || D == 64, OLMAX_ERR_SHAPE, "%s: D must be 32 or 64 (got %d)", name, D);
-  OLMAX_CHECK(tiles_of(S) * H * B < (1LL << 31), OLMAX_ERR_SHAPE, "%s: B=%d S=%d H=%d are too many rows", name, B, S, H);
+  OLMAX_CHECK(tiles_of(S) * 2 * H * B < (1LL << 31), OLMAX_ERR_SHAPE, "%s: B=%d S=%d H=%d are too many rows", name, B, S, H);
   return OLMAX_OK;
 }
+
+// Whether dK/dV takes the split kernel
+bool dkv_split(int B, const Sizes& z) { return (int64_t)((z.S + 127) / 128) * z.KH * B <= 640; }
 
 template <int W>
 void fwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const float* lam, bf16* o, bf16* o2, float* lse, int B, const Sizes& z) {
   static std::once_flag once;
-  std::call_once(once, [] { (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W)); });
-  hipLaunchKernelGGL(diff_attn_fwd_kernel<W>, dim3((unsigned)(tiles_of(z.S) * z.H * B)), dim3(256), smem_q(W), stream, q, k, v, lam, o, o2, lse, z);
+  std::call_once(once, [] { (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W)); });
+  hipLaunchKernelGGL(diff_attn_fwd_kernel<W>, dim3((unsigned)(tiles_of(z.S) * z.H * B)), dim3(512), smem_fwd(W), stream, q, k, v, lam, o, o2, lse, z);
 }
 
 template <int W>
@@ -736,11 +818,17 @@ void bwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const 
   static std::once_flag once;
   std::call_once(once, [] {
     (void)hipFuncSetAttribute((const void*)diff_attn_dq_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W));
-    (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W));
+    (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 4, 1>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 4, 1));
+    (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 2, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 2, 4));
   });
   const int tiles = (int)tiles_of(z.S);
   hipLaunchKernelGGL(diff_attn_dq_kernel<W>, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(256), smem_q(W), stream, q, k, v, lam, o, o2, lse, d_o, dq, delta, parts, z, gr);
-  hipLaunchKernelGGL(diff_attn_dkv_kernel<W>, dim3((unsigned)((int64_t)((z.S + KR - 1) / KR) * z.KH * B)), dim3(256), smem_kv(W), stream, q, k, v, lam, lse, (const float*)delta, d_o, dk, dv, z, gr);
+  auto kv = [&](auto kern, int kw, int qs) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)((z.S + 32 * kw - 1) / (32 * kw)) * z.KH * B)), dim3(64 * kw * qs), smem_kv(W, kw, qs), stream, q, k, v, lam, lse, (const float*)delta,
+                       d_o, dk, dv, z, gr);
+  };
+  if (dkv_split(B, z)) kv(diff_attn_dkv_kernel<W, 2, 4>, 2, 4);
+  else kv(diff_attn_dkv_kernel<W, 4, 1>, 4, 1);
   hipLaunchKernelGGL(diff_attn_dlam_kernel, dim3((unsigned)(z.shared ? 1 : z.H)), dim3(256), 0, stream, (const float*)parts, dlam, B, z.H, tiles, z.shared);
 }
 
