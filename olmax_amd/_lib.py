@@ -77,6 +77,7 @@ _SIGNATURES = {
     "olmax_lmhead_logprobs_bwd": "PPPPPPPPPPLLIIIFFI",
     "olmax_lmhead_distill": "PPPPPPPPPLLIIIIFFFI",
 }
+_SIGNATURES_OF_64_BITS = {"olmax_rotary_tables": "PPPLIDIDDDDF"}  # D: double
 _typed = {}
 
 
@@ -87,7 +88,7 @@ def typed(name: str):
     if f is None:
         load()
         f = getattr(ctypes.CDLL(str(_LIB_PATH)), name)
-        f.argtypes = [{"P": vp, "I": i32, "L": i64, "F": f32}[c] for c in _SIGNATURES[name]]
+        f.argtypes = [{"P": vp, "I": i32, "L": i64, "F": f32, "D": f64}[c] for c in _SIGNATURES.get(name) or _SIGNATURES_OF_64_BITS[name]]
         f.restype = i32
         _typed[name] = f
     return f

@@ -16,6 +16,11 @@
 
 namespace {
 
+// 4 B per lane straight into LDS, as dma16
+__device__ __forceinline__ void dma4(const void* g, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_addr), "v"(g) : "m0", "memory");
+}
+
 struct Sizes {
   int S, H, KH, window;
   int64_t ldq, ldk, ldv, ldo, ldo2;
@@ -118,25 +123,27 @@ __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ld
   for (int c = 0; c < W / 64; c++) dq[c * 64 + lane] = f2bf(acc[c] * scale);
 }
 
-// key j, columns [lo, hi); Q, dO of the first of its rep query heads, stats (of a head and map: S numbers) of the first of them
+// key j, columns [lo, hi); Q, dO, stats, lam of the first of its rep query heads
 template <int W>
-__device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16* dO, int64_t lddo, const float* lse, const float* delta, const float* lam, int lam_step, const bf16* k,
-                                         const bf16* v, bf16* dk, bf16* dv, int j, int S, int rep, int window, float scale, int lane, int lo, int hi) {
+__device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16* dO, int64_t lddo, const float* stats, const float* lam, int lam_step, const bf16* k, const bf16* v,
+                                         bf16* dk, bf16* dv, int j, int S, int rep, int window, float scale, int lane, int lo, int hi) {
   constexpr int D = W / 2;
   const int last = window >= 0 ? min(S - 1, j + window) : S - 1;
   float ak[W / 64] = {}, av[W / 64] = {};
 #pragma unroll 1
-  for (int r = 0; r < rep; r++, Q += W, dO += W, lse += 2 * (int64_t)S, delta += 2 * (int64_t)S, lam += lam_step)
+  for (int r = 0; r < rep; r++, Q += W, dO += W, stats += 4 * (int64_t)S, lam += lam_step)
 #pragma unroll 1
     for (int i0 = j; i0 <= last; i0 += 64) {
       const int n = min(64, last - i0 + 1);
       float p = 0.f, s1 = 0.f, s2 = 0.f;
       if (lane < n) {
         const int64_t i = i0 + lane;
+        const float* st = stats + i;
         float p1, p2, dp;
-        pair_of<W>(Q + i * ldq, k, dO + i * lddo, v, lse[i], lse[S + i], scale, p1, p2, dp);
-        s1 = p1 * (dp + delta[i]);
-        s2 = -*lam * p2 * ((dp + delta[i]) + delta[S + i]);
+        pair_of<W>(Q + i * ldq, k, dO + i * lddo, v, st[0] * LN2, st[S] * LN2, scale, p1, p2, dp);
+        dp += st[2 * (int64_t)S];
+        s1 = p1 * dp;
+        s2 = -*lam * p2 * (dp + st[3 * (int64_t)S]);
         p = p1 - *lam * p2;
       }
 #pragma unroll 1
@@ -159,6 +166,41 @@ __device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16*
 }
 
 constexpr int QR = 128;  // queries of a workgroup
+
+#ifndef MAPV
+#define MAPV 1
+#endif
+__device__ __forceinline__ WgCoord coord(int id, int ngroups, int rep) {
+  WgCoord c = decode_wg(id, ngroups, rep);
+  if ((ngroups & 7) == 0) {
+    const int per = ngroups >> 3;
+    if (MAPV == 1) c.group = (c.group & 7) * per + (c.group >> 3);
+    if (MAPV == 2) c.group = (c.group + c.rank) % ngroups;
+    if (MAPV == 3) c.group = ((c.group & 7) * per + (c.group >> 3) + c.rank) % ngroups;
+    if (MAPV == 4) c.group = ((c.group & 7) * per + (c.group >> 3) + (per < 8 ? c.rank * per : 0)) % ngroups;
+  }
+  return c;
+}
+
+// Scores of pairs that are not visible become -1e30 (s + I M): two more k-steps, of the identity and a mask with M[k][column] = 0 or -1e30 (hides(k, column)), into the accumulators where they
+// are, so that tiles inside pay nothing.  (As selects on the scores every tile pays; in a branch or a second copy of the tile the accumulators of the two ways meet in copies and spill.)
+// Lane and column are hidden from the compiler, which otherwise keeps what is formed of them through the loop.
+template <typename F>
+__device__ __forceinline__ void hide(f32x16& s1, f32x16& s2, int lane, int column, F hides) {
+  asm volatile("" : "+v"(lane), "+v"(column));
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    bf16x8 one, mask;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int k = u * 16 + (lane >> 5) * 8 + e;
+      one[e] = f2bf(k == (lane & 31) ? 1.f : 0.f);
+      mask[e] = f2bf(hides(k, column) ? -1e30f : 0.f);
+    }
+    s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(one, mask, s1, 0, 0, 0);
+    s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(one, mask, s2, 0, 0, 0);
+  }
+}
 
 // ---------------------------------------------------------------------------------------
 // Forward.  grid = ceil(S / 128) H B workgroups of 8 waves; wave (qw, m) owns 32 queries and one map, and the two waves of a SIMD, qw of either map, take turns: a key tile is two parts, the softmax
@@ -188,7 +230,7 @@ __global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __res
   const int l32 = lane & 31, lhi = lane >> 5;
   const int qw = wave & 3, m = wave >> 2;
   const int nqt = (S + QR - 1) / QR;
-  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
+  const WgCoord wg = coord(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
   const int qt = nqt - 1 - wg.rank;  // longest rows first
   const int b = wg.group / KH, kh = wg.group % KH;
   const int h = kh * (H / KH) + wg.r;
@@ -263,12 +305,14 @@ __global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __res
       const int j0 = t * 64;
       const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
       if (need_mask) {
+        int i = qi, half = lhi;
+        asm volatile("" : "+v"(i), "+v"(half));  // a branch, and nothing formed of them is kept through the loop
 #pragma unroll
         for (int jt = 0; jt < 2; jt++)
 #pragma unroll
           for (int r = 0; r < 16; r++) {
-            const int j = j0 + jt * 32 + (r >> 2) * 8 + lhi * 4 + (r & 3);
-            const bool ok = (j <= qi) && (window < 0 || j >= qi - window);
+            const int j = j0 + jt * 32 + (r >> 2) * 8 + half * 4 + (r & 3);
+            const bool ok = (j <= i) && (window < 0 || j >= i - window);
             st[jt][r] = ok ? st[jt][r] : -INFINITY;
           }
       }
@@ -380,7 +424,7 @@ __global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __res
 
 // ---------------------------------------------------------------------------------------
 // dQ, dlambda and delta.  Tiling and grid of the forward.
-// DELTA [B, H, 2, S]: -delta_1, and delta_1 - delta_2 (dP - delta_2 is what dK/dV has of the first map, plus this).  dlambda is taken from P_2 and dP in fp32, not from the rounded O_2:
+// STATS [B, H, 4, S]: what dK/dV takes of a row: lse_1 and lse_2 in powers of two, -delta_1, and delta_1 - delta_2 (dP - delta_2 is what it has of the first map, plus this).  dlambda is taken from P_2 and dP in fp32, not from the rounded O_2:
 // it is a sum of terms of both signs that an error of 2^-9 in each would leave three digits of.  DLAM: a number for each workgroup, [B, H, tiles].
 // ---------------------------------------------------------------------------------------
 struct Grad {
@@ -389,7 +433,7 @@ struct Grad {
 template <int W>
 __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
                                                               const bf16* __restrict__ O, const bf16* __restrict__ O2, const float* __restrict__ LSE, const bf16* __restrict__ dO,
-                                                              bf16* __restrict__ dQ, float* __restrict__ DELTA, float* __restrict__ DLAM, const Sizes z, const Grad gr) {
+                                                              bf16* __restrict__ dQ, float* __restrict__ STATS, float* __restrict__ DLAM, const Sizes z, const Grad gr) {
   constexpr int TILE = 64 * W * 2, KS = W / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];  // [2][K | V]
   __shared__ float red[4];
@@ -398,7 +442,7 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lhi = lane >> 5;
   const int nqt = (S + QR - 1) / QR;
-  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
+  const WgCoord wg = coord(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
   const int qt = nqt - 1 - wg.rank;
   const int b = wg.group / KH, kh = wg.group % KH;
   const int h = kh * (H / KH) + wg.r;
@@ -431,11 +475,14 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
   d2 = half_swap_sum(d2);
   d1 = __builtin_fmaf(lam, d2, half_swap_sum(d1));  // o + lambda O_2 = O_1
   const int64_t row0 = ((int64_t)b * H + h) * 2 * S;
-  if (lhi == 0 && qi < S) {
-    DELTA[row0 + qi] = -d1;
-    DELTA[row0 + S + qi] = d1 - d2;
-  }
   const float l1 = LSE[row0 + qic] * LOG2E, l2 = LSE[row0 + S + qic] * LOG2E;
+  if (lhi == 0 && qi < S) {
+    float* st = STATS + 2 * row0 + qi;
+    st[0] = l1;
+    st[S] = l2;
+    st[2 * (int64_t)S] = -d1;
+    st[3 * (int64_t)S] = d1 - d2;
+  }
   const int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
   const int t_hi = min(i0 + QR - 1, S - 1) >> 6;
 
@@ -463,7 +510,7 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
     }
   };
   const float sc2 = z.scale * LOG2E;
-  FragAddr<W> fa;
+  FragAddr<W, W == 128> fa;  // (short of registers)
   fa.init(lane);
 
   load_kv(t_lo, 0);
@@ -487,22 +534,19 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
           s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, s), qf[s], s1, 0, 0, 0);
           s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, KS + s), qf[KS + s], s2, 0, 0, 0);
         }
+        if (need_mask)
+          hide(s1, s2, lane, qi, [&](int k, int i) {
+            const int j = j0 + jt * 32 + k;
+            return j > i || (window >= 0 && j < i - window);
+          });
 #pragma unroll
         for (int s = 0; s < 2 * KS; s++) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sv, jt * 32, s), dof[s], dp, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const float p1 = fexp2(__builtin_fmaf(s1[r], sc2, -l1)), p2 = fexp2(__builtin_fmaf(s2[r], sc2, -l2));
-          float x = p1 * (dp[r] - d1), y = p2 * (dp[r] - d2), w = p2 * dp[r];
-          if (need_mask) {
-            const int j = j0 + jt * 32 + (r >> 2) * 8 + lhi * 4 + (r & 3);
-            const bool ok = (j <= qi) && (window < 0 || j >= qi - window);
-            x = ok ? x : 0.f;
-            y = ok ? y : 0.f;
-            w = ok ? w : 0.f;
-          }
-          s1[r] = x;
-          s2[r] = y;
-          dl += w;
+          dl = __builtin_fmaf(p2, dp[r], dl);
+          s1[r] = p1 * (dp[r] - d1);
+          s2[r] = p2 * (dp[r] - d2);
         }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -544,19 +588,21 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
 }
 
 // ---------------------------------------------------------------------------------------
-// dK/dV.  grid = ceil(S / 32 KW) KH B workgroups of KW x QS waves; wave (kw, qs) owns 32 keys (K in registers) and every QS-th of the pairs of a query head of the group and one of its 32-row
-// tiles from the diagonal on.  LDS: per query group 2 stages of (Q | dO | lse_1, lse_2, -delta_1, delta_1 - delta_2 of the 32 rows), then the V tile.
+// dK/dV.  grid = ceil(S / 32 KW) KH B workgroups of KW x QS waves; wave (kw, qs) owns 32 keys and every QS-th of the pairs of a query head of the group and one of its 32-row
+// tiles from the diagonal on.  LDS: per query group 2 stages of (Q | dO | the 32 rows' statistics), then the fragments of V and K.
 // KW = 4, QS = 1: two workgroups per CU, no reduction.  KW = 2, QS = 4: one workgroup of eight waves per CU, half the keys and a quarter of the chain; the four partial sums are added through LDS
 // in group order.  See dkv_split.
 // ---------------------------------------------------------------------------------------
 constexpr int smem_q(int W) { return 2 * 2 * 64 * W * 2; }
+// k-steps of K that lie in LDS, the last of the second map's (W = 128: with all in registers the loop spills, and a reload waits for the tiles under way; two workgroups of 4 x 1 find room on a CU with 3)
+constexpr int k_parked(int W, int KW) { return W != 128 ? 0 : KW == 4 ? 3 : 4; }
 constexpr int smem_kv(int W, int KW, int QS) {
-  const int run = QS * 2 * (2 * 32 * W * 2 + 512) + KW * 32 * W * 2, sums = QS > 1 ? KW * QS * 32 * W * 4 : 0;
+  const int run = QS * 2 * (2 * 32 * W * 2 + 512) + KW * (W / 16 + k_parked(W, KW)) * 1024, sums = QS > 1 ? KW * QS * 32 * W * 4 : 0;
   return run > sums ? run : sums;
 }
 template <int W, int KW, int QS>
 __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
-                                                                        const float* __restrict__ LSE, const float* __restrict__ DELTA, const bf16* __restrict__ dO,
+                                                                        const float* __restrict__ STATS, const bf16* __restrict__ dO,
                                                                         bf16* __restrict__ dK, bf16* __restrict__ dV, const Sizes z, const Grad gr) {
   constexpr int QT = 32, KS = W / 32;
   constexpr int TILE = QT * W * 2, STAGE = 2 * TILE + 512;
@@ -568,7 +614,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lhi = lane >> 5;
   const int kw = wave % KW, qs = wave / KW, wv = wave & 3, team = wave >> 2;
-  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / ((S + KT - 1) / KT)), 1);  // key tile 0 is seen by every query: longest first
+  const WgCoord wg = coord(blockIdx.x, (int)(gridDim.x / ((S + KT - 1) / KT)), 1);  // key tile 0 is seen by every query: longest first
   const int b = wg.group / KH, kh = wg.group % KH;
   const int rep = H / KH;
   const int j0 = wg.rank * KT;
@@ -576,11 +622,22 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   const int kj = jw0 + l32;  // this lane's key
   const int kjc = min(kj, S - 1);
 
-  bf16x8 kf[W / 16];
+  // K's and V's fragments of these keys: K's first in registers, the others in LDS, each the 1 KB that a read takes
+  constexpr int PARKED = k_parked(W, KW), HELD = 2 * KS - PARKED, FIXED = 2 * KS + PARKED;
+  const unsigned lds0 = lds_addr_of(smem);
+  bf16x8 kf[HELD];
   {
     const bf16* kp = K + ((int64_t)b * S + kjc) * z.ldk + kh * W + lhi * 8;
+    const bf16* vp = V + ((int64_t)b * S + kjc) * z.ldv + kh * W + lhi * 8;
+    const unsigned dst = lds0 + QS * 2 * STAGE + kw * (FIXED * 1024);
 #pragma unroll
-    for (int s = 0; s < W / 16; s++) kf[s] = *reinterpret_cast<const bf16x8*>(kp + s * 16);
+    for (int s = 0; s < HELD; s++) kf[s] = *reinterpret_cast<const bf16x8*>(kp + s * 16);
+    if (qs == 0) {
+#pragma unroll
+      for (int s = 0; s < 2 * KS; s++) dma16(vp + s * 16, dst + s * 1024);
+#pragma unroll
+      for (int s = 0; s < PARKED; s++) dma16(kp + (HELD + s) * 16, dst + (2 * KS + s) * 1024);
+    }
   }
   f32x16 dk[W / 32], dv[W / 32];
 #pragma unroll
@@ -591,37 +648,37 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   const int i_hi = window >= 0 ? min(S - 1, j0 + KT - 1 + window) : S - 1;
   const int t_lo = j0 / QT, t_hi = i_hi / QT;  // inclusive
   const int ntile = t_hi - t_lo + 1;
-  const int total = ntile * rep;  // (head, tile) pairs, heads outermost
+  const int total = ntile * rep;
   const float sc2 = z.scale * LOG2E;
-  const unsigned lds0 = lds_addr_of(smem);
   const unsigned char* sgrp = smem + qs * (2 * STAGE);  // this query group's stages
 
   TileDma<QT, W> tq, tdo;
   tq.init(z.ldq, wv, lane);
   tdo.init(gr.lddo, wv, lane);
-  // (head, tile) of the next iteration to load of each query group this team fetches for, and of this wave's own group (its rows' statistics)
+  // (tile, head) pairs, the last tile first and its heads next to each other: the workgroups of a K/V head, which begin at different tiles, read the same ones at the same time, out of one L2
   struct Iter { int h, t; };
   auto advance = [&](Iter& x, int n) {
-    x.t += n;
-    while (x.t > t_hi) {
-      x.t -= ntile;
-      ++x.h;
+    x.h += n;
+    while (x.h >= rep) {
+      x.h -= rep;
+      --x.t;
     }
   };
-  Iter own{kh * rep, t_lo}, ld[QS / TEAMS];
-  advance(own, qs);
+  auto first = [&](int n) {
+    Iter x{0, t_hi};
+    advance(x, n);
+    return x;
+  };
+  // the next one to load of each query group this team fetches for, and of this wave's own group (its rows' statistics)
+  Iter own = first(qs), ld[QS / TEAMS];
 #pragma unroll
-  for (int g = 0; g < QS / TEAMS; g++) {
-    ld[g] = Iter{kh * rep, t_lo};
-    advance(ld[g], g * TEAMS + team);
-  }
-  float sreg[2];
+  for (int g = 0; g < QS / TEAMS; g++) ld[g] = first(g * TEAMS + team);
   auto load_tile = [&](int round, int stage) {
 #pragma unroll
     for (int g = 0; g < QS / TEAMS; g++) {
       const int grp = g * TEAMS + team;
       if (QS > 1 && round * QS + grp >= total) break;
-      const int hq = ld[g].h, t = ld[g].t;
+      const int hq = kh * rep + ld[g].h, t = ld[g].t;
       advance(ld[g], QS);
       const unsigned dst = lds0 + (grp * 2 + stage) * STAGE;
       const bf16 *qp = Q + (int64_t)b * S * z.ldq + hq * W, *dp = dO + (int64_t)b * S * gr.lddo + hq * W;
@@ -629,35 +686,32 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
         tq.issue(qp + (int64_t)t * QT * z.ldq, dst, wv);
         tdo.issue(dp + (int64_t)t * QT * gr.lddo, dst + TILE, wv);
       } else {
-        dma_tile<QT, W>(qp, z.ldq, t * QT, S, dst, wv, lane);
-        dma_tile<QT, W>(dp, gr.lddo, t * QT, S, dst + TILE, wv, lane);
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        dma_tile<QT, W>(qp, z.ldq, t * QT, S, dst, wv, l);
+        dma_tile<QT, W>(dp, gr.lddo, t * QT, S, dst + TILE, wv, l);
       }
     }
-    if (kw == 0 && (QS == 1 || round * QS + qs < total)) {  // lanes 0 .. 31 the first map's, 32 .. 63 the second's
-      const int64_t at = (((int64_t)b * H + own.h) * 2 + lhi) * S + min(own.t * QT + l32, S - 1);
-      sreg[0] = LSE[at];
-      sreg[1] = DELTA[at];
-    }
-  };
-  auto store_stats = [&](int stage) {  // (scaled here, an iteration after the load: see attn.hip)
-    if (kw == 0) {
-      float* p = reinterpret_cast<float*>(smem + (qs * 2 + stage) * STAGE + 2 * TILE);
-      p[lane] = sreg[0] * LOG2E;
-      p[64 + lane] = sreg[1];
+    if (kw == 0 && (QS == 1 || round * QS + qs < total)) {  // the rows' statistics: lanes 0 .. 31 the first of two, 32 .. 63 the second
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      const float* st = STATS + (((int64_t)b * H + kh * rep + own.h) * 4 + (l >> 5)) * S + min(own.t * QT + (l & 31), S - 1);
+      const unsigned dst = lds0 + (qs * 2 + stage) * STAGE + 2 * TILE;
+      dma4(st, dst);
+      dma4(st + 2 * (int64_t)S, dst + 256);
     }
   };
 
-  FragAddr<W> fa;
+  FragAddr<W, W == 128> fa;
   fa.init(lane);
-  const unsigned char* svt = smem + QS * 2 * STAGE;  // [KT keys][W] V tile
-  if (team == 0) dma_tile<KT, W>(V + (int64_t)b * S * z.ldv + kh * W, z.ldv, j0, S, lds0 + QS * 2 * STAGE, wv, lane);
+  const unsigned char* fixed = smem + QS * 2 * STAGE + kw * (FIXED * 1024) + lane * 16;
+  auto v_step = [&](int s) { return *reinterpret_cast<const bf16x8*>(fixed + s * 1024); };
+  auto k_step = [&](int s) { return s < HELD ? kf[s < HELD ? s : 0] : v_step(2 * KS + s - HELD); };
   load_tile(0, 0);
-  store_stats(0);
   dma_wait_all();
   __syncthreads();
   const int rounds = (total + QS - 1) / QS;
-  Iter cur_it{kh * rep, t_lo};  // being consumed
-  advance(cur_it, qs);
+  Iter cur_it = first(qs);  // being consumed
   for (int round = 0; round < rounds; round++) {
     const int cur = round & 1;
     const bool more = round + 1 < rounds;
@@ -668,60 +722,90 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
     const int ib = cur_it.t * QT;  // first query of the tile
     const bool visible = (QS == 1 || round * QS + qs < total) && (ib + QT - 1 >= jw0) && (window < 0 || ib <= jw0 + 31 + window);
     if (visible) {
-      const float nlam = -LAM[z.shared ? 0 : cur_it.h];
+      const float nlam = -LAM[z.shared ? 0 : kh * rep + cur_it.h];
       const unsigned char* sq = sgrp + cur * STAGE;
       const unsigned char* so = sq + TILE;
       const float* stats = reinterpret_cast<const float*>(sq + 2 * TILE);
       const bool need_mask = (ib < jw0 + 31) || (ib + QT > S) || (window >= 0 && ib + QT - 1 > jw0 + window);
-      f32x16 s1, s2, dp;
-      // accumulator rows are queries ib + 8 (r / 4) + 4 lhi + r % 4; column: key kj.  dP starts from -delta_1
+      // A tile is 32 products (W = 128) in four runs: scores, dP, dV, dK.  The exponentials go between those of dP, what is left of dS between those of dV, and each product's fragments are read
+      // some products ahead; the order is pinned, since the compiler's own reads so far ahead that it spills, and a reload waits for the tiles under way.
+      constexpr int STEPS = 2 * KS, EL = 16 / STEPS;  // products of a run, rows of the vector work beside each
+#ifndef AHP
+#define AHP 1
+#define AHV 1
+#define AHK 2
+#endif
+      constexpr int AP = AHP, AV = AHV, AK = AHK;  // products that fragments are read ahead by, of dP, dV and dK
+      f32x16 s1, s2, dp;  // rows are queries ib + 8 (r / 4) + 4 lhi + r % 4; column: key kj
+      bf16x8 w[2], ds1[2], ds2[2];
+      auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
+      auto of4 = [&](int row, int r) { return stats[row * 32 + (r >> 2) * 8 + lhi * 4 + (r & 3)]; };
+      auto tr_step = [&](const unsigned char* tile, int i) { return fa.load_tr(tile, i / (W / 32) * 16, i % (W / 32)); };
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(stats + 64 + g * 8 + lhi * 4);
+      for (int r = 0; r < 16; r++) { s1[r] = 0.f; s2[r] = 0.f; }
+      pin();
+      bf16x8 fq[STEPS], f2[KS], fo[AP + 1], fv[AP + 1], ft[AV + 1], fd[AK + 1];
 #pragma unroll
-        for (int e = 0; e < 4; e++) { s1[g * 4 + e] = 0.f; s2[g * 4 + e] = 0.f; dp[g * 4 + e] = d4[e]; }
-      }
+      for (int s = 0; s < STEPS; s++) fq[s] = fa.load_kc(sq, 0, s);
 #pragma unroll
-      for (int s = 0; s < KS; s++) {
-        s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sq, 0, s), kf[s], s1, 0, 0, 0);
-        s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sq, 0, KS + s), kf[KS + s], s2, 0, 0, 0);
-      }
+      for (int s = 0; s < KS; s++) f2[s] = k_step(KS + s);
+      pin();
 #pragma unroll
-      for (int s = 0; s < 2 * KS; s++) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(so, 0, s), fa.load_kc(svt, kw * 32, s), dp, 0, 0, 0);
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const int il = g * 8 + lhi * 4;
-        const f32x4 l1 = *reinterpret_cast<const f32x4*>(stats + il), l2 = *reinterpret_cast<const f32x4*>(stats + 32 + il);
-        const f32x4 dd = *reinterpret_cast<const f32x4*>(stats + 96 + il);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int r = g * 4 + e;
-          const float p1 = fexp2(__builtin_fmaf(s1[r], sc2, -l1[e])), p2 = nlam * fexp2(__builtin_fmaf(s2[r], sc2, -l2[e]));
-          float x = p1 * dp[r], y = p2 * (dp[r] + dd[e]), w = p1 + p2;
-          if (need_mask) {
-            const int i = ib + il + e;
-            const bool ok = (kj <= i) && (i < S) && (window < 0 || kj >= i - window);
-            x = ok ? x : 0.f;
-            y = ok ? y : 0.f;
-            w = ok ? w : 0.f;
-          }
-          s1[r] = x;
-          s2[r] = y;
-          dp[r] = w;
+      for (int s = 0; s < STEPS; s++) {
+        if (s < KS) s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fq[s], kf[s], s1, 0, 0, 0);
+        else s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fq[s], f2[s - KS], s2, 0, 0, 0);
+        if (s >= STEPS - AP) {
+          fo[s - (STEPS - AP)] = fa.load_kc(so, 0, s - (STEPS - AP));
+          fv[s - (STEPS - AP)] = v_step(s - (STEPS - AP));
         }
+        pin();
+      }
+      if (need_mask)
+        hide(s1, s2, lane, kj, [&](int k, int j) {
+          const int i = ib + k;
+          return j > i || i >= S || (window >= 0 && j < i - window);
+        });
+#pragma unroll
+      for (int r = 0; r < 16; r++) dp[r] = of4(2, r);  // -delta_1
+      pin();
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        if (s + AP < STEPS) {
+          fo[(s + AP) % (AP + 1)] = fa.load_kc(so, 0, s + AP);
+          fv[(s + AP) % (AP + 1)] = v_step(s + AP);
+        } else if (s + AP - STEPS < AV) {
+          ft[s + AP - STEPS] = tr_step(so, s + AP - STEPS);
+        }
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fo[s % (AP + 1)], fv[s % (AP + 1)], dp, 0, 0, 0);
+#pragma unroll
+        for (int r = s * EL; r < (s + 1) * EL; r++) {
+          s1[r] = fexp2(__builtin_fmaf(s1[r], sc2, -of4(0, r)));
+          s2[r] = nlam * fexp2(__builtin_fmaf(s2[r], sc2, -of4(1, r)));
+          w[r >> 3][r & 7] = f2bf(s1[r] + s2[r]);
+        }
+        pin();
       }
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const bf16x8 a = pack_bf16x8(s1, u * 8), c = pack_bf16x8(s2, u * 8), w = pack_bf16x8(dp, u * 8);
+      for (int i = 0; i < STEPS; i++) {
+        if (i + AV < STEPS) ft[(i + AV) % (AV + 1)] = tr_step(so, i + AV);
+        dv[i % (W / 32)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ft[i % (AV + 1)], w[i / (W / 32)], dv[i % (W / 32)], 0, 0, 0);
 #pragma unroll
-        for (int dt = 0; dt < W / 32; dt++) {
-          dv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_tr(so, u * 16, dt), w, dv[dt], 0, 0, 0);
-          dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_tr(sq, u * 16, dt), dt < W / 64 ? a : c, dk[dt], 0, 0, 0);
+        for (int r = i * EL; r < (i + 1) * EL; r++) {
+          ds1[r >> 3][r & 7] = f2bf(s1[r] * dp[r]);
+          ds2[r >> 3][r & 7] = f2bf(s2[r] * (dp[r] + of4(3, r)));
         }
+        if (i >= STEPS - AK) fd[i - (STEPS - AK)] = tr_step(sq, i - (STEPS - AK));
+        pin();
+      }
+#pragma unroll
+      for (int i = 0; i < STEPS; i++) {
+        const int dt = i % (W / 32);
+        if (i + AK < STEPS) fd[(i + AK) % (AK + 1)] = tr_step(sq, i + AK);
+        dk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fd[i % (AK + 1)], dt < W / 64 ? ds1[i / (W / 32)] : ds2[i / (W / 32)], dk[dt], 0, 0, 0);
+        pin();
       }
     }
     advance(cur_it, QS);
-    if (more) store_stats(cur ^ 1);
     dma_wait_all();
     __syncthreads();
   }
@@ -760,8 +844,8 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
     });
   }
   redo_rows(kj < S ? zeros : 0.f, [&](int r) {
-    const int64_t seq = (int64_t)b * S, at = seq + jw0 + r, row = ((int64_t)b * H + kh * rep) * 2 * S;
-    redo_dkv<W>(Q + seq * z.ldq + kh * rep * W, z.ldq, dO + seq * gr.lddo + kh * rep * W, gr.lddo, LSE + row, DELTA + row, LAM + (z.shared ? 0 : kh * rep), z.shared ? 0 : 1,
+    const int64_t seq = (int64_t)b * S, at = seq + jw0 + r, row = ((int64_t)b * H + kh * rep) * 4 * S;
+    redo_dkv<W>(Q + seq * z.ldq + kh * rep * W, z.ldq, dO + seq * gr.lddo + kh * rep * W, gr.lddo, STATS + row, LAM + (z.shared ? 0 : kh * rep), z.shared ? 0 : 1,
                 K + at * z.ldk + kh * W, V + at * z.ldv + kh * W, dK + at * gr.lddk + kh * W, dV + at * gr.lddv + kh * W, jw0 + r, S, rep, window, z.scale, lane,
                 qs * (W / QS), (qs + 1) * (W / QS));
   });
@@ -781,7 +865,7 @@ __global__ __launch_bounds__(256) void diff_attn_dlam_kernel(const float* __rest
 }
 
 int64_t tiles_of(int32_t S) { return ((int64_t)S + QR - 1) / QR; }
-int64_t delta_bytes(int32_t B, int32_t S, int32_t H) { return ((int64_t)B * H * 2 * S * 4 + 255) / 256 * 256; }
+int64_t stats_bytes(int32_t B, int32_t S, int32_t H) { return ((int64_t)B * H * 4 * S * 4 + 255) / 256 * 256; }
 
 constexpr int64_t MAX_LD = 1 << 24;  // of a row, in elements: 64 rows are within reach of a 32-bit offset in bytes
 // Whether rows of na and nb bf16 numbers at a and b share memory: exact for one row stride, as views of one buffer have it, otherwise whether their ranges meet.
@@ -814,7 +898,7 @@ void fwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const 
 
 template <int W>
 void bwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const float* lam, const bf16* o, const bf16* o2, const float* lse, const bf16* d_o, bf16* dq, bf16* dk,
-         bf16* dv, float* dlam, float* delta, float* parts, int B, const Sizes& z, const Grad& gr) {
+         bf16* dv, float* dlam, float* stats, float* parts, int B, const Sizes& z, const Grad& gr) {
   static std::once_flag once;
   std::call_once(once, [] {
     (void)hipFuncSetAttribute((const void*)diff_attn_dq_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W));
@@ -822,10 +906,9 @@ void bwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const 
     (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 2, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 2, 4));
   });
   const int tiles = (int)tiles_of(z.S);
-  hipLaunchKernelGGL(diff_attn_dq_kernel<W>, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(256), smem_q(W), stream, q, k, v, lam, o, o2, lse, d_o, dq, delta, parts, z, gr);
+  hipLaunchKernelGGL(diff_attn_dq_kernel<W>, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(256), smem_q(W), stream, q, k, v, lam, o, o2, lse, d_o, dq, stats, parts, z, gr);
   auto kv = [&](auto kern, int kw, int qs) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)((z.S + 32 * kw - 1) / (32 * kw)) * z.KH * B)), dim3(64 * kw * qs), smem_kv(W, kw, qs), stream, q, k, v, lam, lse, (const float*)delta,
-                       d_o, dk, dv, z, gr);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)((z.S + 32 * kw - 1) / (32 * kw)) * z.KH * B)), dim3(64 * kw * qs), smem_kv(W, kw, qs), stream, q, k, v, lam, (const float*)stats, d_o, dk, dv, z, gr);
   };
   if (dkv_split(B, z)) kv(diff_attn_dkv_kernel<W, 2, 4>, 2, 4);
   else kv(diff_attn_dkv_kernel<W, 4, 1>, 4, 1);
@@ -854,9 +937,9 @@ extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const 
   return OLMAX_OK;
 }
 
-// Workspace: delta [B, H, 2, S], then dlambda's parts [B, H, ceil(S / 128)], fp32
+// Workspace: the rows' statistics [B, H, 4, S], then dlambda's parts [B, H, ceil(S / 128)], fp32
 extern "C" int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H) {
-  return B <= 0 || S <= 0 || H <= 0 ? 0 : delta_bytes(B, S, H) + ((int64_t)B * H * tiles_of(S) * 4 + 255) / 256 * 256;
+  return B <= 0 || S <= 0 || H <= 0 ? 0 : stats_bytes(B, S, H) + ((int64_t)B * H * tiles_of(S) * 4 + 255) / 256 * 256;
 }
 
 extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const void* k, const void* v, const float* lam, const void* o, const void* o2, const float* lse,
@@ -884,7 +967,7 @@ extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const 
   const Sizes z{S, H, KH, window < 0 || window >= S ? -1 : window, ldq, ldk, ldv, ldo, ldo2, 1.f / sqrtf((float)D), lam_shared != 0};
   const Grad gr{lddo, lddq, lddk, lddv};
   (D == 64 ? bwd<128> : bwd<64>)(stream, (const bf16*)q, (const bf16*)k, (const bf16*)v, lam, (const bf16*)o, (const bf16*)o2, lse, (const bf16*)d_o, (bf16*)dq, (bf16*)dk, (bf16*)dv,
-                                 dlam, (float*)workspace, (float*)((char*)workspace + delta_bytes(B, S, H)), B, z, gr);
+                                 dlam, (float*)workspace, (float*)((char*)workspace + stats_bytes(B, S, H)), B, z, gr);
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }

@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import check, f32, f64, i32, i64, ptr, raw_stream, stream_ptr, typed
+from ._lib import check, f32, i32, i64, ptr, raw_stream, stream_ptr, typed
 
 BF16 = torch.bfloat16
 
@@ -178,14 +178,12 @@ class RopeScaling:
 
 def rotary_tables(length: int, rotary_dim: int, theta: float, device, *, scaling: Optional[RopeScaling] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """cos/sin [length, rotary_dim / 2] fp32, angles formed in 64 bits (rope_tables forms them in fp32, as the reference does: at position 131072 that is 0.004 off)."""
-    device = torch.device(device)
-    if device.type != "cuda":
+    if torch.device(device).type != "cuda":
         raise _lib.OlmaxHipError("olmax_amd ops run on the GPU only; there is no CPU fallback")
-    _want(length > 0 and rotary_dim > 0 and rotary_dim % 2 == 0, f"rotary_tables: length must be positive and rotary_dim even (got {length}, {rotary_dim})")
-    cos, sin = torch.empty(2, length, rotary_dim // 2, device=device, dtype=torch.float32).unbind(0)
+    _want(length > 0 and rotary_dim > 0 and rotary_dim % 2 == 0, "rotary_tables: length must be positive and rotary_dim even")
+    cos, sin = torch.empty((2, length, rotary_dim // 2), device=device, dtype=torch.float32).unbind(0)
     _place(cos)
-    kind, factor, original, low, high, size = (0, 1.0, 1.0, 1.0, 1.0, 1.0) if scaling is None else scaling.c_args()
-    check(_L().olmax_rotary_tables(stream_ptr(), ptr(cos), ptr(sin), i64(length), i32(rotary_dim), f64(theta), i32(kind), f64(factor), f64(original), f64(low), f64(high), f32(size)))
+    check(typed("olmax_rotary_tables")(raw_stream(), cos.data_ptr(), sin.data_ptr(), length, rotary_dim, theta, *((0, 1.0, 1.0, 1.0, 1.0, 1.0) if scaling is None else scaling.c_args())))
     return cos, sin
 
 
@@ -195,18 +193,23 @@ _LAYOUT = {"half": 0, "interleaved": 1}
 def _rotary(name, x, cos, sin, heads, head_dim, positions, seq_len, layout, out):
     _place(x, cos, sin, positions, out)
     width = heads * head_dim
-    _want(x.dim() == 2 and x.dtype in (BF16, torch.float32) and x.shape[1] >= width > 0 and x.stride(1) == 1, f"expected rows of {heads} x {head_dim} and more in bf16 or fp32")
-    T = x.shape[0]
-    _want(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous(),
-          "cos, sin: expected contiguous fp32 tables [positions, rotary_dim / 2]")
-    _want(positions is None or (positions.dtype == torch.int32 and positions.shape == (T,) and positions.is_contiguous()), f"positions: expected a contiguous int32 tensor [{T}]")
-    _want(layout in _LAYOUT, f"layout must be 'half' or 'interleaved' (got {layout!r})")
+    dtype, shape = x.dtype, x.shape
+    _want((dtype is BF16 or dtype is torch.float32) and len(shape) == 2 and shape[1] >= width > 0 and x.stride(1) == 1,
+          "rotary: expected rows of heads * head_dim and more numbers in bf16 or fp32")
+    T = shape[0]
+    n, half = cos.shape if cos.dim() == 2 else (0, 0)
+    _want(cos.dtype is torch.float32 and sin.dtype is torch.float32 and sin.shape == (n, half) and cos.is_contiguous() and sin.is_contiguous(),
+          "rotary: cos, sin: expected contiguous fp32 tables [positions, rotary_dim / 2]")
+    _want(positions is None or (positions.dtype is torch.int32 and positions.shape == (T,) and positions.is_contiguous()),
+          "rotary: positions: expected a contiguous int32 tensor, one for each row")
+    _want(layout in _LAYOUT, "rotary: layout must be 'half' or 'interleaved'")
     if out is None:
-        out = x.new_empty((T, width))
-    _want(out.dim() == 2 and out.dtype == x.dtype and out.shape[0] == T and out.shape[1] >= width and out.stride(1) == 1, "out: expected rows of x's type")
-    n = cos.shape[0]
-    check(typed(name)(raw_stream(), x.data_ptr(), out.data_ptr(), cos.data_ptr(), sin.data_ptr(), _ptr(positions), T, heads, head_dim, 2 * cos.shape[1], n,
-                      n if seq_len is None else seq_len, x.stride(0), out.stride(0), _LAYOUT[layout], 1 if x.dtype == torch.float32 else 0))
+        out, ldo = x.new_empty((T, width)), width
+    else:
+        _want(out.dtype is dtype and out.dim() == 2 and out.shape[0] == T and out.shape[1] >= width and out.stride(1) == 1, "rotary: out: expected rows of x's type")
+        ldo = out.stride(0)
+    check(typed(name)(raw_stream(), x.data_ptr(), out.data_ptr(), cos.data_ptr(), sin.data_ptr(), None if positions is None else positions.data_ptr(), T, heads, head_dim, 2 * half, n,
+                      n if seq_len is None else seq_len, x.stride(0), ldo, _LAYOUT[layout], 0 if dtype is BF16 else 1))
     return out
 
 
@@ -352,13 +355,18 @@ class DiffAttention(NamedTuple):
 
 def _head_rows(t, T: int, width: int, what: str):
     """A bf16 [T, width] operand, rows apart as far as they like; its row stride."""
-    _want(t.dim() == 2 and t.dtype == BF16 and t.shape == (T, width) and t.stride(1) == 1, f"{what}: expected bf16 rows [{T}, {width}]")
-    return t.stride(0) if T > 1 else width
+    ok = t.dtype is BF16 and t.shape == (T, width)
+    ld, one = t.stride() if ok else (0, 0)
+    if one != 1:
+        raise _lib.OlmaxHipError(f"{what}: expected bf16 rows [{T}, {width}]")
+    return ld if T > 1 else width
 
 
 def _diff_sizes(lam, B: int, S: int, H: int, KH: int, D: int):
-    _want(B > 0 and S > 0 and H > 0 and KH > 0 and H % KH == 0 and D in (32, 64), f"bad shape B={B} S={S} H={H} KH={KH} D={D}: KH divides H, D is 32 or 64")
-    _want(lam.dtype == torch.float32 and lam.shape in ((H,), (1,)) and lam.is_contiguous(), f"lam: expected a contiguous fp32 tensor [{H}] or [1]")
+    if not (B > 0 and S > 0 and H > 0 and KH > 0 and H % KH == 0 and (D == 32 or D == 64)):
+        raise _lib.OlmaxHipError(f"bad shape B={B} S={S} H={H} KH={KH} D={D}: KH divides H, D is 32 or 64")
+    if not (lam.dtype is torch.float32 and lam.shape in ((H,), (1,)) and lam.is_contiguous()):
+        raise _lib.OlmaxHipError(f"lam: expected a contiguous fp32 tensor [{H}] or [1]")
     return B * S, 2 * D * H, 2 * D * KH
 
 
@@ -492,10 +500,16 @@ def _size32(name: str, *args) -> int:
 
 def _place(*ts):
     """GPU tensors of the current device, whose stream the call is enqueued on."""
-    _need_gpu(*ts)
-    here = torch._C._cuda_getDevice()
+    here = -1
     for t in ts:
-        _want(t is None or t.device.index == here, "olmax_amd ops: a tensor is on another GPU than the current one")
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
+            _need_gpu(t)
+        if here < 0:
+            here = torch._C._cuda_getDevice()
+        _want(at == here, "olmax_amd ops: a tensor is on another GPU than the current one")
 
 
 def _logits(t, like=None):
