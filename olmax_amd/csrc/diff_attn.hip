@@ -13,6 +13,8 @@
 #include "attn_tiles.h"
 #include <cmath>
 #include <mutex>
+#include <type_traits>
+#include <utility>
 
 namespace {
 
@@ -97,11 +99,13 @@ __device__ __forceinline__ void pair_of(const bf16* q, const bf16* k, const bf16
   dp = dot(d_o, v, W);
 }
 
+// d1, d2: delta as dS takes it; sum1, sum2: the row's sums of P_m dP
 template <int W>
 __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ldk, const bf16* V, int64_t ldv, const bf16* d_o, float l1, float l2, float d1, float d2, float lam,
-                                        bf16* dq, int i, int window, float scale, int lane) {
+                                        bf16* dq, int i, int window, float scale, int lane, float& sum1, float& sum2) {
   constexpr int D = W / 2;
   float acc[W / 64] = {};
+  sum1 = sum2 = 0.f;
 #pragma unroll 1
   for (int j0 = window >= 0 ? max(0, i - window) : 0; j0 <= i; j0 += 64) {
     const int n = min(64, i - j0 + 1);
@@ -109,6 +113,8 @@ __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ld
     if (lane < n) {
       float p1, p2, dp;
       pair_of<W>(q, K + (j0 + lane) * ldk, d_o, V + (j0 + lane) * ldv, l1, l2, scale, p1, p2, dp);
+      sum1 += p1 * dp;
+      sum2 += p2 * dp;
       s1 = p1 * (dp - d1);
       s2 = -lam * p2 * (dp - d2);
     }
@@ -119,6 +125,8 @@ __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ld
       for (int c = 0; c < W / 64; c++) acc[c] += (c * 64 + lane < D ? a : b) * bf2f(K[(j0 + t) * ldk + c * 64 + lane]);
     }
   }
+  sum1 = wave_sum(sum1);
+  sum2 = wave_sum(sum2);
 #pragma unroll
   for (int c = 0; c < W / 64; c++) dq[c * 64 + lane] = f2bf(acc[c] * scale);
 }
@@ -163,6 +171,16 @@ __device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16*
     dk[at] = f2bf(ak[c] * scale);
     dv[at] = f2bf(av[c]);
   }
+}
+
+// f(0) .. f(N - 1) with the index as a constant (a loop of 48 products is not unrolled before its arrays would have to be registers)
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  each_of(f, std::make_integer_sequence<int, N>());
 }
 
 constexpr int QR = 128;  // queries of a workgroup
@@ -424,8 +442,11 @@ __global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __res
 
 // ---------------------------------------------------------------------------------------
 // dQ, dlambda and delta.  Tiling and grid of the forward.
-// STATS [B, H, 4, S]: what dK/dV takes of a row: lse_1 and lse_2 in powers of two, -delta_1, and delta_1 - delta_2 (dP - delta_2 is what it has of the first map, plus this).  dlambda is taken from P_2 and dP in fp32, not from the rounded O_2:
-// it is a sum of terms of both signs that an error of 2^-9 in each would leave three digits of.  DLAM: a number for each workgroup, [B, H, tiles].
+// dQ takes delta from the outputs as they were rounded, as dQ of attn.hip does.  The sums of P_m dP come out of the same sweep in fp32: dK/dV takes its delta from them (its error at 4096 tokens 0.0027 of
+// itself -> 0.0024, the rounding of dS and of the result), and dlambda is their sum: terms of both signs, that an error of 2^-9 in each would leave three digits of.  (For dQ, whose error is
+// 0.0027, they come too late: another sweep ahead would be two thirds of this kernel.)
+// STATS [B, H, 4, S]: what dK/dV takes of a row: lse_1 and lse_2 in powers of two, -delta_1, and delta_1 - delta_2 (dP - delta_2 is what it has of the first map, plus this).  DLAM: a number for
+// each workgroup, [B, H, tiles].
 // ---------------------------------------------------------------------------------------
 struct Grad {
   int64_t lddo, lddq, lddk, lddv;
@@ -476,13 +497,6 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
   d1 = __builtin_fmaf(lam, d2, half_swap_sum(d1));  // o + lambda O_2 = O_1
   const int64_t row0 = ((int64_t)b * H + h) * 2 * S;
   const float l1 = LSE[row0 + qic] * LOG2E, l2 = LSE[row0 + S + qic] * LOG2E;
-  if (lhi == 0 && qi < S) {
-    float* st = STATS + 2 * row0 + qi;
-    st[0] = l1;
-    st[S] = l2;
-    st[2 * (int64_t)S] = -d1;
-    st[3 * (int64_t)S] = d1 - d2;
-  }
   const int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
   const int t_hi = min(i0 + QR - 1, S - 1) >> 6;
 
@@ -491,7 +505,7 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
   for (int dt = 0; dt < W / 32; dt++)
 #pragma unroll
     for (int r = 0; r < 16; r++) dq[dt][r] = 0.f;
-  float dl = 0.f;
+  float sum1 = 0.f, sum2 = 0.f;  // of P_m dP
 
   const bf16* kbase = K + (int64_t)b * S * z.ldk + kh * W;
   const bf16* vbase = V + (int64_t)b * S * z.ldv + kh * W;
@@ -524,44 +538,68 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
       const unsigned char* sk = smem + cur * (2 * TILE);
       const unsigned char* sv = sk + TILE;
       const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
+      // 48 products (W = 128) in six runs: scores and dP of either half of the tile's keys, then dQ of either.  The exponentials go between the products of dP, what is left of dS between those of
+      // the next half's scores, or of dQ; each product's fragment is read one ahead, in a pinned order, as in dK/dV.
+      constexpr int STEPS = 2 * KS, EL = 16 / STEPS, AHEAD = 1;
+      f32x16 s1[2], s2[2], dp[2];
+      bf16x8 ds1[2][2], ds2[2][2], fr[AHEAD + 1];
+      auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
+      auto fetch = [&](int n) {  // the fragment of product n
+        const int run = n / STEPS, s = n % STEPS;
+        if (run >= 4) return fa.load_tr(sk, (run - 4) * 32 + s / (W / 32) * 16, s % (W / 32));
+        return fa.load_kc(run & 1 ? sv : sk, run / 2 * 32, s);
+      };
+      auto left = [&](int jt, int s) {
 #pragma unroll
-      for (int jt = 0; jt < 2; jt++) {
-        f32x16 s1, s2, dp;
-#pragma unroll
-        for (int r = 0; r < 16; r++) { s1[r] = 0.f; s2[r] = 0.f; dp[r] = 0.f; }
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-          s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, s), qf[s], s1, 0, 0, 0);
-          s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, KS + s), qf[KS + s], s2, 0, 0, 0);
+        for (int r = s * EL; r < (s + 1) * EL; r++) {
+          sum1 = __builtin_fmaf(s1[jt][r], dp[jt][r], sum1);
+          sum2 = __builtin_fmaf(s2[jt][r], dp[jt][r], sum2);
+          ds1[jt][r >> 3][r & 7] = f2bf(s1[jt][r] * (dp[jt][r] - d1));
+          ds2[jt][r >> 3][r & 7] = f2bf(s2[jt][r] * (dp[jt][r] - d2));
         }
-        if (need_mask)
-          hide(s1, s2, lane, qi, [&](int k, int i) {
+      };
+      pin();
+      each<AHEAD>([&](auto at) { fr[at] = fetch(at); });
+      each<6 * STEPS>([&](auto at) {
+        constexpr int n = decltype(at)::value, run = n / STEPS, s = n % STEPS, jt = run >= 4 ? run - 4 : run / 2;
+        if (n + AHEAD < 6 * STEPS) fr[(n + AHEAD) % (AHEAD + 1)] = fetch(n + AHEAD);
+        if (run >= 4) {
+          constexpr int u = s / (W / 32), dt = s % (W / 32);
+          dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n % (AHEAD + 1)], dt < W / 64 ? ds1[jt][u] : ds2[jt][u], dq[dt], 0, 0, 0);
+          if (run == 4) left(1, s);
+        } else if (run & 1) {
+          if (s == 0)
+#pragma unroll
+            for (int r = 0; r < 16; r++) dp[jt][r] = 0.f;
+          dp[jt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n % (AHEAD + 1)], dof[s], dp[jt], 0, 0, 0);
+#pragma unroll
+          for (int r = s * EL; r < (s + 1) * EL; r++) {
+            s1[jt][r] = fexp2(__builtin_fmaf(s1[jt][r], sc2, -l1));
+            s2[jt][r] = fexp2(__builtin_fmaf(s2[jt][r], sc2, -l2));
+          }
+          if (s + 1 == STEPS) asm volatile("" : "+v"(s1[jt]), "+v"(s2[jt]));  // (here: else they move behind the next branch)
+        } else {
+          if (s == 0)
+#pragma unroll
+            for (int r = 0; r < 16; r++) { s1[jt][r] = 0.f; s2[jt][r] = 0.f; }
+          if (s < KS) s1[jt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n % (AHEAD + 1)], qf[s], s1[jt], 0, 0, 0);
+          else s2[jt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n % (AHEAD + 1)], qf[s], s2[jt], 0, 0, 0);
+          if (run == 2) left(0, s);
+          if (run == 2 && s + 1 == STEPS) asm volatile("" : "+v"(ds1[0][0]), "+v"(ds1[0][1]), "+v"(ds2[0][0]), "+v"(ds2[0][1]), "+v"(sum1), "+v"(sum2));
+        }
+        pin();
+        if (run < 4 && !(run & 1) && s + 1 == STEPS && need_mask)
+          hide(s1[jt], s2[jt], lane, qi, [&](int k, int i) {
             const int j = j0 + jt * 32 + k;
             return j > i || (window >= 0 && j < i - window);
           });
-#pragma unroll
-        for (int s = 0; s < 2 * KS; s++) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sv, jt * 32, s), dof[s], dp, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const float p1 = fexp2(__builtin_fmaf(s1[r], sc2, -l1)), p2 = fexp2(__builtin_fmaf(s2[r], sc2, -l2));
-          dl = __builtin_fmaf(p2, dp[r], dl);
-          s1[r] = p1 * (dp[r] - d1);
-          s2[r] = p2 * (dp[r] - d2);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const bf16x8 a = pack_bf16x8(s1, u * 8), c = pack_bf16x8(s2, u * 8);
-#pragma unroll
-          for (int dt = 0; dt < W / 32; dt++)
-            dq[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_tr(sk, jt * 32 + u * 16, dt), dt < W / 64 ? a : c, dq[dt], 0, 0, 0);
-        }
-      }
+      });
     }
     dma_wait_all();
     __syncthreads();
   }
-  dl = block_sum<4>(qi < S ? dl : 0.f, red);
-  if (tid == 0) DLAM[((int64_t)b * H + h) * nqt + qt] = -dl;
+  sum1 = half_swap_sum(sum1);
+  sum2 = half_swap_sum(sum2);
   float zeros = 0.f;
   if (qi < S) {
     bf16* op = dQ + ((int64_t)b * S + qi) * gr.lddq + h * W;
@@ -579,12 +617,26 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
         *reinterpret_cast<u32x2*>(op + dt * 32 + g * 8 + lhi * 4) = pk.u;
       }
   }
+  if (qi < S) zeros = __builtin_fmaf(sum1, 0.f, __builtin_fmaf(sum2, 0.f, zeros));
   redo_rows(zeros, [&](int r) {
     const int i = iw0 + r;
     const int64_t at = (int64_t)b * S + i;
+    float a, c;
     redo_dq<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, dO + at * gr.lddo + h * W, LSE[row0 + i], LSE[row0 + S + i], __shfl(d1, r, 64), __shfl(d2, r, 64), lam,
-               dQ + at * gr.lddq + h * W, i, window, z.scale, lane);
+               dQ + at * gr.lddq + h * W, i, window, z.scale, lane, a, c);
+    sum1 = l32 == r ? a : sum1;
+    sum2 = l32 == r ? c : sum2;
   });
+  const bool counts = lhi == 0 && qi < S;
+  if (counts) {
+    float* st = STATS + 2 * row0 + qi;
+    st[0] = l1;
+    st[S] = l2;
+    st[2 * (int64_t)S] = -sum1;
+    st[3 * (int64_t)S] = sum1 - sum2;
+  }
+  const float dl = block_sum<4>(counts ? sum2 : 0.f, red);
+  if (tid == 0) DLAM[((int64_t)b * H + h) * nqt + qt] = -dl;
 }
 
 // ---------------------------------------------------------------------------------------
