@@ -56,9 +56,18 @@ TABLES_REFUSED = [
 def test_tables_refuse(change, code):
     L = lib()
     a = {**TABLES, **change}
-    rc = L.load().olmax_rotary_tables(None, L.vp(a["cos"]), L.vp(a["sin"]), L.i64(a["length"]), L.i32(a["rotary_dim"]), L.f64(a["theta"]), L.i32(a["kind"]), L.f64(a["factor"]),
-                                      L.f64(a["original"]), L.f64(a["low"]), L.f64(a["high"]), L.f32(a["size"]))
-    assert rc == code and b"olmax_rotary_tables" in L.load().olmax_last_error_string()
+    assert L.typed("olmax_rotary_tables")(None, *a.values()) == code and b"olmax_rotary_tables" in L.load().olmax_last_error_string()
+
+
+def test_argument_types_of_the_tables_match_the_header():
+    import re
+    from pathlib import Path
+    _lib = lib()
+    text = re.sub(r"/\*.*?\*/", "", (Path(__file__).resolve().parent.parent / "include" / "olmax_hip.h").read_text(), flags=re.S)
+    for name, letters in _lib._SIGNATURES_OF_64_BITS.items():
+        args = re.search(name + r"\s*\(([^;]*)\)\s*;", text)[1]
+        kinds = ["P" if "*" in a or "olmax_stream_t" in a else {"int32_t": "I", "int64_t": "L", "float": "F", "double": "D"}[a.split()[0]] for a in args.split(",")]
+        assert "".join(kinds) == letters, name
 
 
 def test_scalings_by_name():
