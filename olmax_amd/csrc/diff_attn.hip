@@ -48,7 +48,7 @@ __device__ __forceinline__ float dot(const bf16* a, const bf16* b, int n) {
 
 template <int W>
 __device__ __forceinline__ void redo_fwd(const bf16* q, const bf16* K, int64_t ldk, const bf16* V, int64_t ldv, float lam, bf16* o, bf16* o2, float* lse, int S, int i, int window,
-                                         float scale, int lane) {
+                                         float scale, int lane, int lo, int hi) {
   constexpr int D = W / 2;
   const int first = window >= 0 ? max(0, i - window) : 0;
   float l[2];
@@ -61,7 +61,7 @@ __device__ __forceinline__ void redo_fwd(const bf16* q, const bf16* K, int64_t l
 #pragma unroll 1
     for (int j = first + lane; j <= i; j += 64) sm += __expf(dot(q + m * D, K + j * ldk + m * D, D) * scale - mx);
     l[m] = mx + __logf(wave_sum(sm));
-    if (lane == 0) lse[m * S] = l[m];
+    if (lane == 0 && lo == 0) lse[m * S] = l[m];
   }
   float acc[2][W / 64] = {};
 #pragma unroll 1
@@ -85,8 +85,10 @@ __device__ __forceinline__ void redo_fwd(const bf16* q, const bf16* K, int64_t l
   }
 #pragma unroll
   for (int c = 0; c < W / 64; c++) {
-    o[c * 64 + lane] = f2bf(acc[0][c] - lam * acc[1][c]);
-    if (o2) o2[c * 64 + lane] = f2bf(acc[1][c]);
+    const int at = c * 64 + lane;
+    if (at < lo || at >= hi) continue;
+    o[at] = f2bf(acc[0][c] - lam * acc[1][c]);
+    if (o2) o2[at] = f2bf(acc[1][c]);
   }
 }
 
@@ -99,10 +101,10 @@ __device__ __forceinline__ void pair_of(const bf16* q, const bf16* k, const bf16
   dp = dot(d_o, v, W);
 }
 
-// d1, d2: delta as dS takes it; sum1, sum2: the row's sums of P_m dP
+// columns [lo, hi) of the row; d1, d2: delta as dS takes it; sum1, sum2: the row's sums of P_m dP
 template <int W>
 __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ldk, const bf16* V, int64_t ldv, const bf16* d_o, float l1, float l2, float d1, float d2, float lam,
-                                        bf16* dq, int i, int window, float scale, int lane, float& sum1, float& sum2) {
+                                        bf16* dq, int i, int window, float scale, int lane, int lo, int hi, float& sum1, float& sum2) {
   constexpr int D = W / 2;
   float acc[W / 64] = {};
   sum1 = sum2 = 0.f;
@@ -128,7 +130,8 @@ __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ld
   sum1 = wave_sum(sum1);
   sum2 = wave_sum(sum2);
 #pragma unroll
-  for (int c = 0; c < W / 64; c++) dq[c * 64 + lane] = f2bf(acc[c] * scale);
+  for (int c = 0; c < W / 64; c++)
+    if (c * 64 + lane >= lo && c * 64 + lane < hi) dq[c * 64 + lane] = f2bf(acc[c] * scale);
 }
 
 // key j, columns [lo, hi); Q, dO, stats, lam of the first of its rep query heads
@@ -183,24 +186,7 @@ __device__ __forceinline__ void each(F f) {
   each_of(f, std::make_integer_sequence<int, N>());
 }
 
-constexpr int QR = 128;  // queries of a workgroup
-
-#ifndef MAPV
-#define MAPV 1
-#endif
-__device__ __forceinline__ WgCoord coord(int id, int ngroups, int rep) {
-  WgCoord c = decode_wg(id, ngroups, rep);
-  if ((ngroups & 7) == 0) {
-    const int per = ngroups >> 3;
-    if (MAPV == 1) c.group = (c.group & 7) * per + (c.group >> 3);
-    if (MAPV == 2) c.group = (c.group + c.rank) % ngroups;
-    if (MAPV == 3) c.group = ((c.group & 7) * per + (c.group >> 3) + c.rank) % ngroups;
-    if (MAPV == 4) c.group = ((c.group & 7) * per + (c.group >> 3) + (per < 8 ? c.rank * per : 0)) % ngroups;
-  }
-  return c;
-}
-
-// Scores of pairs that are not visible become -1e30 (s + I M): two more k-steps, of the identity and a mask with M[k][column] = 0 or -1e30 (hides(k, column)), into the accumulators where they
+// Scores of pairs that are not visible become -3e38 (s + I M): two more k-steps, of the identity and a mask with M[k][column] = 0 or -3e38 (hides(k, column)), into the accumulators where they
 // are, so that tiles inside pay nothing.  (As selects on the scores every tile pays; in a branch or a second copy of the tile the accumulators of the two ways meet in copies and spill.)
 // Lane and column are hidden from the compiler, which otherwise keeps what is formed of them through the loop.
 template <typename F>
@@ -213,7 +199,7 @@ __device__ __forceinline__ void hide(f32x16& s1, f32x16& s2, int lane, int colum
     for (int e = 0; e < 8; e++) {
       const int k = u * 16 + (lane >> 5) * 8 + e;
       one[e] = f2bf(k == (lane & 31) ? 1.f : 0.f);
-      mask[e] = f2bf(hides(k, column) ? -1e30f : 0.f);
+      mask[e] = f2bf(hides(k, column) ? -3e38f : 0.f);
     }
     s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(one, mask, s1, 0, 0, 0);
     s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(one, mask, s2, 0, 0, 0);
@@ -221,7 +207,7 @@ __device__ __forceinline__ void hide(f32x16& s1, f32x16& s2, int lane, int colum
 }
 
 // ---------------------------------------------------------------------------------------
-// Forward.  grid = ceil(S / 128) H B workgroups of 8 waves; wave (qw, m) owns 32 queries and one map, and the two waves of a SIMD, qw of either map, take turns: a key tile is two parts, the softmax
+// Forward.  grid = ceil(S / 32 QW) H B workgroups of 2 QW waves; wave (qw, m) owns 32 queries and one map, and the two waves of a SIMD (QW = 4), qw of either map, take turns: a key tile is two parts, the softmax
 // (vector unit) and the products (matrix unit: this tile's probabilities with V, the next tile's scores), a barrier ends each, and map 1 is one part behind map 0.
 // LDS: 3 stages of K, then of V.  Map 0's waves fetch K, map 1's V.  K(t) is read in parts 2t - 1 and 2t, V(t) in 2t + 1 and 2t + 2 (counted as map 0 does), so that K(t + 3) is issued in 2t + 1 and
 // V(t + 2) too, and each has four parts to land; past the end the last tile is fetched again.
@@ -235,20 +221,22 @@ __device__ __forceinline__ void part_ends() {  // at most the newest N transfers
   __builtin_amdgcn_sched_barrier(0);
 }
 constexpr int smem_fwd(int W) { return 2 * 3 * 64 * W * 2; }
-template <int W>
-__global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+template <int W, int QW>
+__global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
                                                                bf16* __restrict__ O, bf16* __restrict__ O2, float* __restrict__ LSE, const Sizes z) {
   constexpr int TILE = 64 * W * 2;  // bytes of a K or V tile of 64 keys
   constexpr int KS = W / 32;        // k-steps of a map
-  constexpr int INS = 64 * W / 2048;  // transfers of a wave and tile
+  constexpr int QR = QW * 32;       // queries of the workgroup
+  constexpr int SHARES = 4 / QW;    // of a tile's four that a wave fetches
+  constexpr int INS = 64 * W / 2048 * SHARES;  // its transfers
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];  // [3] K, [3] V
   const int S = z.S, H = z.H, KH = z.KH, window = z.window;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lhi = lane >> 5;
-  const int qw = wave & 3, m = wave >> 2;
+  const int qw = wave % QW, m = wave / QW;
   const int nqt = (S + QR - 1) / QR;
-  const WgCoord wg = coord(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
   const int qt = nqt - 1 - wg.rank;  // longest rows first
   const int b = wg.group / KH, kh = wg.group % KH;
   const int h = kh * (H / KH) + wg.r;
@@ -278,13 +266,17 @@ __global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __res
   const unsigned lds0 = lds_addr_of(smem);
   const bf16* base = m ? vbase : kbase;
   const int64_t ld = m ? z.ldv : z.ldk;
-  TileDma<64, W> dma;
-  dma.init(ld, qw, lane);
+  TileDma<64, W> dma[SHARES];
+#pragma unroll
+  for (int i = 0; i < SHARES; i++) dma[i].init(ld, qw + i * QW, lane);
   auto load = [&](int t, int stage) {  // of this wave's operand
     t = min(t, t_hi);
     const unsigned dst = lds0 + (m * 3 + stage) * TILE;
-    if (t * 64 + 64 <= S) dma.issue(base + (int64_t)t * 64 * ld, dst, qw);
-    else dma_tile<64, W>(base, ld, t * 64, S, dst, qw, lane);
+#pragma unroll
+    for (int i = 0; i < SHARES; i++) {
+      if (t * 64 + 64 <= S) dma[i].issue(base + (int64_t)t * 64 * ld, dst, qw + i * QW);
+      else dma_tile<64, W>(base, ld, t * 64, S, dst, qw + i * QW, lane);
+    }
   };
   const float sc2 = z.scale * LOG2E;
   FragAddr<W> fa;
@@ -410,12 +402,12 @@ __global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __res
       if (O2 && qi < S) *reinterpret_cast<u32x2*>(o2p + u * 8 + lhi * 4) = pk.u;
     }
     if (qi >= S) zeros = 0.f;
-    reinterpret_cast<float*>(smem + 4 * 32 * W * 4)[qw * 64 + lane] = zeros;
+    reinterpret_cast<float*>(smem + QW * 32 * W * 4)[qw * 64 + lane] = zeros;
     if (__builtin_amdgcn_ballot_w64(zeros != 0.f)) dma_wait_all();  // the other wave of these rows is going to store them over
   }
   __syncthreads();
   if (m == 1) return;
-  zeros += reinterpret_cast<float*>(smem + 4 * 32 * W * 4)[qw * 64 + lane];
+  zeros += reinterpret_cast<float*>(smem + QW * 32 * W * 4)[qw * 64 + lane];
   if (qi < S) {
     bf16* op = O + ((int64_t)b * S + qi) * z.ldo + h * W;
 #pragma unroll
@@ -436,12 +428,13 @@ __global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __res
   redo_rows(zeros, [&](int r) {
     const int i = iw0 + r;
     const int64_t at = (int64_t)b * S + i;
-    redo_fwd<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, lam, O + at * z.ldo + h * W, O2 ? O2 + at * z.ldo2 + h * W : nullptr, lse_row + i, S, i, window, z.scale, lane);
+    redo_fwd<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, lam, O + at * z.ldo + h * W, O2 ? O2 + at * z.ldo2 + h * W : nullptr, lse_row + i, S, i, window, z.scale, lane, 0, W);
   });
 }
 
 // ---------------------------------------------------------------------------------------
-// dQ, dlambda and delta.  Tiling and grid of the forward.
+// dQ, dlambda and delta.  grid = ceil(S / 32 QW) H B workgroups of QW x KG waves; wave (qw, kg) owns 32 queries and every KG-th of their key tiles.  KG = 1 (QW = 4): two workgroups per CU, no merge.
+// KG > 1: one workgroup of eight waves with 1 / KG of the chain of tiles; what they have is added through LDS, in key-group order.  See q_split.
 // dQ takes delta from the outputs as they were rounded, as dQ of attn.hip does.  The sums of P_m dP come out of the same sweep in fp32: dK/dV takes its delta from them (its error at 4096 tokens 0.0027 of
 // itself -> 0.0024, the rounding of dS and of the result), and dlambda is their sum: terms of both signs, that an error of 2^-9 in each would leave three digits of.  (For dQ, whose error is
 // 0.0027, they come too late: another sweep ahead would be two thirds of this kernel.)
@@ -451,24 +444,32 @@ __global__ __launch_bounds__(512, 2) void diff_attn_fwd_kernel(const bf16* __res
 struct Grad {
   int64_t lddo, lddq, lddk, lddv;
 };
-template <int W>
-__global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+struct Lambda {
+  const float* parts;
+  float* dlam;
+  int batch, tiles;
+};
+template <int W, int QW, int KG>
+__global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
                                                               const bf16* __restrict__ O, const bf16* __restrict__ O2, const float* __restrict__ LSE, const bf16* __restrict__ dO,
                                                               bf16* __restrict__ dQ, float* __restrict__ STATS, float* __restrict__ DLAM, const Sizes z, const Grad gr) {
   constexpr int TILE = 64 * W * 2, KS = W / 32;
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];  // [2][K | V]
-  __shared__ float red[4];
+  constexpr int QR = QW * 32;         // queries of the workgroup
+  constexpr int TEAMS = QW * KG / 4;  // tiles are fetched by teams of 4 waves
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];  // [KG][2][K | V]
+  __shared__ float red[QW * KG], sums[KG > 1 ? KG : 1][QR][2];
   const int S = z.S, H = z.H, KH = z.KH, window = z.window;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lhi = lane >> 5;
+  const int qw = wave % QW, kg = wave / QW, wv = wave & 3, team = wave >> 2;
   const int nqt = (S + QR - 1) / QR;
-  const WgCoord wg = coord(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
   const int qt = nqt - 1 - wg.rank;
   const int b = wg.group / KH, kh = wg.group % KH;
   const int h = kh * (H / KH) + wg.r;
   const int i0 = qt * QR;
-  const int iw0 = i0 + wave * 32;
+  const int iw0 = i0 + qw * 32;
   const int qi = iw0 + l32;
   const int qic = min(qi, S - 1);
   const float lam = LAM[z.shared ? 0 : h];
@@ -511,31 +512,39 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
   const bf16* vbase = V + (int64_t)b * S * z.ldv + kh * W;
   const unsigned lds0 = lds_addr_of(smem);
   TileDma<64, W> dk, dv;
-  dk.init(z.ldk, wave, lane);
-  dv.init(z.ldv, wave, lane);
-  auto load_kv = [&](int t, int stage) {
-    const unsigned dst = lds0 + stage * (2 * TILE);
-    if (t * 64 + 64 <= S) {
-      dk.issue(kbase + (int64_t)t * 64 * z.ldk, dst, wave);
-      dv.issue(vbase + (int64_t)t * 64 * z.ldv, dst + TILE, wave);
-    } else {
-      dma_tile<64, W>(kbase, z.ldk, t * 64, S, dst, wave, lane);
-      dma_tile<64, W>(vbase, z.ldv, t * 64, S, dst + TILE, wave, lane);
+  dk.init(z.ldk, wv, lane);
+  dv.init(z.ldv, wv, lane);
+  // K/V tiles of round r: tile t_lo + r KG + g for key group g
+  auto load_kv = [&](int round, int stage) {
+#pragma unroll
+    for (int g0 = 0; g0 < KG / TEAMS; g0++) {
+      const int g = g0 * TEAMS + team, t = t_lo + round * KG + g;
+      if (KG > 1 && t > t_hi) break;
+      const unsigned dst = lds0 + (g * 2 + stage) * (2 * TILE);
+      if (t * 64 + 64 <= S) {
+        dk.issue(kbase + (int64_t)t * 64 * z.ldk, dst, wv);
+        dv.issue(vbase + (int64_t)t * 64 * z.ldv, dst + TILE, wv);
+      } else {
+        dma_tile<64, W>(kbase, z.ldk, t * 64, S, dst, wv, lane);
+        dma_tile<64, W>(vbase, z.ldv, t * 64, S, dst + TILE, wv, lane);
+      }
     }
   };
   const float sc2 = z.scale * LOG2E;
   FragAddr<W, W == 128> fa;  // (short of registers)
   fa.init(lane);
 
-  load_kv(t_lo, 0);
+  load_kv(0, 0);
   dma_wait_all();
   __syncthreads();
-  for (int t = t_lo; t <= t_hi; t++) {
-    const int cur = (t - t_lo) & 1, j0 = t * 64;
-    if (t < t_hi) load_kv(t + 1, cur ^ 1);
-    const bool visible = j0 <= iw0 + 31 && (window < 0 || j0 + 63 >= iw0 - window);
+  const int rounds = (t_hi - t_lo + KG) / KG;
+  for (int round = 0; round < rounds; round++) {
+    const int cur = round & 1;
+    if (round + 1 < rounds) load_kv(round + 1, cur ^ 1);
+    const int t = t_lo + round * KG + kg, j0 = t * 64;
+    const bool visible = (KG == 1 || t <= t_hi) && j0 <= iw0 + 31 && (window < 0 || j0 + 63 >= iw0 - window);
     if (visible) {
-      const unsigned char* sk = smem + cur * (2 * TILE);
+      const unsigned char* sk = smem + (kg * 2 + cur) * (2 * TILE);
       const unsigned char* sv = sk + TILE;
       const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
       // 48 products (W = 128) in six runs: scores and dP of either half of the tile's keys, then dQ of either.  The exponentials go between the products of dP, what is left of dS between those of
@@ -600,22 +609,39 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
   }
   sum1 = half_swap_sum(sum1);
   sum2 = half_swap_sum(sum2);
+  if constexpr (KG > 1) {  // the key groups' sums, in their order
+    if (lhi == 0) {
+      sums[kg][qw * 32 + l32][0] = sum1;
+      sums[kg][qw * 32 + l32][1] = sum2;
+    }
+    __syncthreads();
+    sum1 = sum2 = 0.f;
+#pragma unroll
+    for (int g = 0; g < KG; g++) {
+      sum1 += sums[g][qw * 32 + l32][0];
+      sum2 += sums[g][qw * 32 + l32][1];
+    }
+  }
   float zeros = 0.f;
-  if (qi < S) {
-    bf16* op = dQ + ((int64_t)b * S + qi) * gr.lddq + h * W;
+  auto store4 = [&](int u, const f32x4& v) {
+    Pack4 pk;
 #pragma unroll
-    for (int dt = 0; dt < W / 32; dt++)
+    for (int e = 0; e < 4; e++) {
+      const float x = v[e] * (u < W / 16 ? z.scale : -lam * z.scale);
+      zeros = __builtin_fmaf(x, 0.f, zeros);
+      pk.e[e] = f2bf(x);
+    }
+    *reinterpret_cast<u32x2*>(dQ + ((int64_t)b * S + qic) * gr.lddq + h * W + u * 8 + lhi * 4) = pk.u;
+  };
+  if constexpr (KG == 1) {
+    if (qi < S) {
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        Pack4 pk;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float x = dq[dt][g * 4 + e] * (dt < W / 64 ? z.scale : -lam * z.scale);
-          zeros = __builtin_fmaf(x, 0.f, zeros);
-          pk.e[e] = f2bf(x);
-        }
-        *reinterpret_cast<u32x2*>(op + dt * 32 + g * 8 + lhi * 4) = pk.u;
-      }
+      for (int u = 0; u < W / 8; u++) store4(u, f32x4{dq[u >> 2][(u & 3) * 4], dq[u >> 2][(u & 3) * 4 + 1], dq[u >> 2][(u & 3) * 4 + 2], dq[u >> 2][(u & 3) * 4 + 3]});
+    }
+  } else {
+    add_partials<W, KG>(smem, dq, qw, kg, lane, [&](int u, const f32x4& v) {
+      if (qi < S) store4(u, v);
+    });
   }
   if (qi < S) zeros = __builtin_fmaf(sum1, 0.f, __builtin_fmaf(sum2, 0.f, zeros));
   redo_rows(zeros, [&](int r) {
@@ -623,11 +649,11 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
     const int64_t at = (int64_t)b * S + i;
     float a, c;
     redo_dq<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, dO + at * gr.lddo + h * W, LSE[row0 + i], LSE[row0 + S + i], __shfl(d1, r, 64), __shfl(d2, r, 64), lam,
-               dQ + at * gr.lddq + h * W, i, window, z.scale, lane, a, c);
+               dQ + at * gr.lddq + h * W, i, window, z.scale, lane, kg * (W / KG), (kg + 1) * (W / KG), a, c);
     sum1 = l32 == r ? a : sum1;
     sum2 = l32 == r ? c : sum2;
   });
-  const bool counts = lhi == 0 && qi < S;
+  const bool counts = lhi == 0 && kg == 0 && qi < S;
   if (counts) {
     float* st = STATS + 2 * row0 + qi;
     st[0] = l1;
@@ -635,7 +661,7 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
     st[2 * (int64_t)S] = -sum1;
     st[3 * (int64_t)S] = sum1 - sum2;
   }
-  const float dl = block_sum<4>(counts ? sum2 : 0.f, red);
+  const float dl = block_sum<QW * KG>(counts ? sum2 : 0.f, red);
   if (tid == 0) DLAM[((int64_t)b * H + h) * nqt + qt] = -dl;
 }
 
@@ -645,7 +671,7 @@ __global__ __launch_bounds__(256, 2) void diff_attn_dq_kernel(const bf16* __rest
 // KW = 4, QS = 1: two workgroups per CU, no reduction.  KW = 2, QS = 4: one workgroup of eight waves per CU, half the keys and a quarter of the chain; the four partial sums are added through LDS
 // in group order.  See dkv_split.
 // ---------------------------------------------------------------------------------------
-constexpr int smem_q(int W) { return 2 * 2 * 64 * W * 2; }
+constexpr int smem_q(int W, int KG) { return KG * 2 * 2 * 64 * W * 2; }
 // k-steps of K that lie in LDS, the last of the second map's (W = 128: with all in registers the loop spills, and a reload waits for the tiles under way; two workgroups of 4 x 1 find room on a CU with 3)
 constexpr int k_parked(int W, int KW) { return W != 128 ? 0 : KW == 4 ? 3 : 4; }
 constexpr int smem_kv(int W, int KW, int QS) {
@@ -655,7 +681,7 @@ constexpr int smem_kv(int W, int KW, int QS) {
 template <int W, int KW, int QS>
 __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
                                                                         const float* __restrict__ STATS, const bf16* __restrict__ dO,
-                                                                        bf16* __restrict__ dK, bf16* __restrict__ dV, const Sizes z, const Grad gr) {
+                                                                        bf16* __restrict__ dK, bf16* __restrict__ dV, const Sizes z, const Grad gr, const Lambda la) {
   constexpr int QT = 32, KS = W / 32;
   constexpr int TILE = QT * W * 2, STAGE = 2 * TILE + 512;
   constexpr int KT = KW * 32;         // keys of the workgroup
@@ -666,7 +692,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lhi = lane >> 5;
   const int kw = wave % KW, qs = wave / KW, wv = wave & 3, team = wave >> 2;
-  const WgCoord wg = coord(blockIdx.x, (int)(gridDim.x / ((S + KT - 1) / KT)), 1);  // key tile 0 is seen by every query: longest first
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / ((S + KT - 1) / KT)), 1);  // key tile 0 is seen by every query: longest first
   const int b = wg.group / KH, kh = wg.group % KH;
   const int rep = H / KH;
   const int j0 = wg.rank * KT;
@@ -782,12 +808,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
       // A tile is 32 products (W = 128) in four runs: scores, dP, dV, dK.  The exponentials go between those of dP, what is left of dS between those of dV, and each product's fragments are read
       // some products ahead; the order is pinned, since the compiler's own reads so far ahead that it spills, and a reload waits for the tiles under way.
       constexpr int STEPS = 2 * KS, EL = 16 / STEPS;  // products of a run, rows of the vector work beside each
-#ifndef AHP
-#define AHP 1
-#define AHV 1
-#define AHK 2
-#endif
-      constexpr int AP = AHP, AV = AHV, AK = AHK;  // products that fragments are read ahead by, of dP, dV and dK
+      constexpr int AP = 1, AV = 1, AK = 2;  // products that fragments are read ahead by, of dP, dV and dK
       f32x16 s1, s2, dp;  // rows are queries ib + 8 (r / 4) + 4 lhi + r % 4; column: key kj
       bf16x8 w[2], ds1[2], ds2[2];
       auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
@@ -901,22 +922,22 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
                 K + at * z.ldk + kh * W, V + at * z.ldv + kh * W, dK + at * gr.lddk + kh * W, dV + at * gr.lddv + kh * W, jw0 + r, S, rep, window, z.scale, lane,
                 qs * (W / QS), (qs + 1) * (W / QS));
   });
-}
-
-// dlambda of a head (or of all): the workgroups' sums in their order
-__global__ __launch_bounds__(256) void diff_attn_dlam_kernel(const float* __restrict__ parts, float* __restrict__ dlam, int B, int H, int tiles, int shared) {
-  __shared__ float red[4];
-  const int64_t per = (int64_t)tiles * (shared ? H : 1);  // a sequence's, next to each other
-  float s = 0.f;
-  for (int b = 0; b < B; b++) {
-    const float* p = parts + ((int64_t)b * H + blockIdx.x) * tiles;
-    for (int64_t i = threadIdx.x; i < per; i += 256) s += p[i];
+  // dlambda of a head (or of all): dQ's sums, [B][H][tiles], in their order; the last workgroups, which have the least to do
+  __shared__ float red[KW * QS];
+  for (int64_t n = gridDim.x - 1 - blockIdx.x; n < (z.shared ? 1 : H); n += gridDim.x) {
+    const int64_t per = (int64_t)la.tiles * (z.shared ? H : 1);
+    float sum = 0.f;
+    for (int c = 0; c < la.batch; c++) {
+      const float* p = la.parts + ((int64_t)c * H + n) * la.tiles;
+      for (int64_t i = tid; i < per; i += KW * QS * 64) sum += p[i];
+    }
+    sum = block_sum<KW * QS>(sum, red);
+    if (tid == 0) la.dlam[n] = sum;
   }
-  s = block_sum<4>(s, red);
-  if (threadIdx.x == 0) dlam[blockIdx.x] = s;
 }
 
-int64_t tiles_of(int32_t S) { return ((int64_t)S + QR - 1) / QR; }
+
+int64_t tiles_of(int32_t S) { return ((int64_t)S + 127) / 128; }  // of 128 queries
 int64_t stats_bytes(int32_t B, int32_t S, int32_t H) { return ((int64_t)B * H * 4 * S * 4 + 255) / 256 * 256; }
 
 constexpr int64_t MAX_LD = 1 << 24;  // of a row, in elements: 64 rows are within reach of a 32-bit offset in bytes
@@ -938,14 +959,44 @@ int check_shape(const char* name, int32_t B, int32_t S, int32_t H, int32_t KH, i
   return OLMAX_OK;
 }
 
-// Whether dK/dV takes the split kernel
+// Forms of dQ and dK/dV.  us of a backward pass that takes one and the other of the two forms, bf16, causal, B x S, H/KH heads:
+// dQ split over key groups (QSK of them) where the workgroups of 128 queries would not fill 256 CUs: it halves the queries of a workgroup and its chain of key tiles, and its merge and one more
+// barrier per tile are then free.  D = 64: 117 split, 133 whole (1 x 1000, 16/4); 122, 142 (1 x 2048, 16/16, 256 workgroups); with 512 of them 218, 196 (1 x 2048, 32/16).
+// D = 32: 105, 121; 172, 158; 30.5, 33 (3 x 333, 4/2).
+constexpr int QSW = 2;
+constexpr int qs_groups(int W) { return W == 128 ? 2 : 4; }
+bool q_split(int B, const Sizes& z) { return tiles_of(z.S) * z.H * B <= 256; }
+
+// dK/dV split over query groups where the longest chain, of key tile 0 through all queries and heads of the group, would outlast the others' share of work: 4 x 1 has S / 128 KH B workgroups on
+// 512 places, of half the longest chain's work on average.
+// D = 64, 2 x 4 and 4 x 1: 617, 1053 (1 x 4096, 32/8: 256 workgroups of 4 x 1); 1209, 1349 (2 x 4096, 32/8: 512); 667, 586 (1 x 4096, 32/32: 1024); 1234, 1107 (1 x 8192, 16/16: 1024);
+// window 512: 170, 178 (1 x 5000, 16/8: 320); 512, 431 (2 x 4000, 32/32: 2048).  D = 32: 418, 760; 797, 899; 457, 368; 849, 693.
 bool dkv_split(int B, const Sizes& z) { return (int64_t)((z.S + 127) / 128) * z.KH * B <= 640; }
+// and with one block of keys to eight query groups (D = 32: they find room in LDS) where the workgroups of two would not fill the GPU, or only just, and with chains of every length.
+// 1 x 8 and 2 x 4: 43, 57 (1 x 600, 8/2: 20 workgroups of 2 x 4); 280, 341 (1 x 4096, 16/4: 256); 121, 97 (1 x 2048, 16/16: 512); window 512: 87, 78 (1 x 2000, 32/8: 256).
+bool dkv_narrow(int B, const Sizes& z) { return (int64_t)((z.S + 63) / 64) * z.KH * B * (z.window < 0 ? 1 : 2) <= 256; }
+
+// Form of the forward pass: workgroups of 64 queries (a wave to a SIMD; the turns are then between SIMDs and cost nothing) where those of 128 would leave half of the GPU empty, and for D = 32 always:
+// LDS and registers hold three such workgroups on a CU, and one of the others.  us, 64 and 128 queries, B x S, H/KH heads: D = 64: 17.8, 21.0 (1 x 512, 8/8: 32 workgroups of 128);
+// 29.3, 32.1 (1 x 1000, 16/4: 128); 57.1, 53.4 (1 x 2048, 16/16: 256); 120, 76 (1 x 2048, 32/8: 512).  D = 32: 23.1, 25.4 (1 x 1024, 8/8); 51.3, 52.7 (1 x 2048, 32/8); 162, 168 (1 x 4096, 32/8);
+// 36.6, 42.1 (1 x 4000, 16/8, window 512).
+template <int W>
+bool fwd_halves(int B, const Sizes& z) { return W == 64 || tiles_of(z.S) * z.H * B <= 128; }
 
 template <int W>
 void fwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const float* lam, bf16* o, bf16* o2, float* lse, int B, const Sizes& z) {
   static std::once_flag once;
-  std::call_once(once, [] { (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W)); });
-  hipLaunchKernelGGL(diff_attn_fwd_kernel<W>, dim3((unsigned)(tiles_of(z.S) * z.H * B)), dim3(512), smem_fwd(W), stream, q, k, v, lam, o, o2, lse, z);
+  std::call_once(once, [] {
+    if constexpr (W != 64) (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W));
+    (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W));
+  });
+  auto run = [&](auto kern, int qw) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)((z.S + 32 * qw - 1) / (32 * qw)) * z.H * B)), dim3(128 * qw), smem_fwd(W), stream, q, k, v, lam, o, o2, lse, z);
+  };
+  if constexpr (W != 64) {
+    if (!fwd_halves<W>(B, z)) return run(diff_attn_fwd_kernel<W, 4>, 4);
+  }
+  run(diff_attn_fwd_kernel<W, 2>, 2);
 }
 
 template <int W>
@@ -953,18 +1004,27 @@ void bwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const 
          bf16* dv, float* dlam, float* stats, float* parts, int B, const Sizes& z, const Grad& gr) {
   static std::once_flag once;
   std::call_once(once, [] {
-    (void)hipFuncSetAttribute((const void*)diff_attn_dq_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W));
+    (void)hipFuncSetAttribute((const void*)diff_attn_dq_kernel<W, 4, 1>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W, 1));
+    (void)hipFuncSetAttribute((const void*)diff_attn_dq_kernel<W, QSW, qs_groups(W)>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W, qs_groups(W)));
     (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 4, 1>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 4, 1));
+    if constexpr (W == 64) (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 1, 8>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 1, 8));
     (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 2, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 2, 4));
   });
-  const int tiles = (int)tiles_of(z.S);
-  hipLaunchKernelGGL(diff_attn_dq_kernel<W>, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(256), smem_q(W), stream, q, k, v, lam, o, o2, lse, d_o, dq, stats, parts, z, gr);
-  auto kv = [&](auto kern, int kw, int qs) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)((z.S + 32 * kw - 1) / (32 * kw)) * z.KH * B)), dim3(64 * kw * qs), smem_kv(W, kw, qs), stream, q, k, v, lam, (const float*)stats, d_o, dk, dv, z, gr);
+  int tiles = 0;
+  auto dq_of = [&](auto kern, int qw, int kg) {
+    tiles = (z.S + 32 * qw - 1) / (32 * qw);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(64 * qw * kg), smem_q(W, kg), stream, q, k, v, lam, o, o2, lse, d_o, dq, stats, parts, z, gr);
   };
+  if (q_split(B, z)) dq_of(diff_attn_dq_kernel<W, QSW, qs_groups(W)>, QSW, qs_groups(W));
+  else dq_of(diff_attn_dq_kernel<W, 4, 1>, 4, 1);
+  auto kv = [&](auto kern, int kw, int qs) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)((z.S + 32 * kw - 1) / (32 * kw)) * z.KH * B)), dim3(64 * kw * qs), smem_kv(W, kw, qs), stream, q, k, v, lam, (const float*)stats, d_o, dk, dv, z, gr, Lambda{parts, dlam, B, tiles});
+  };
+  if constexpr (W == 64) {
+    if (dkv_narrow(B, z)) return kv(diff_attn_dkv_kernel<W, 1, 8>, 1, 8);
+  }
   if (dkv_split(B, z)) kv(diff_attn_dkv_kernel<W, 2, 4>, 2, 4);
   else kv(diff_attn_dkv_kernel<W, 4, 1>, 4, 1);
-  hipLaunchKernelGGL(diff_attn_dlam_kernel, dim3((unsigned)(z.shared ? 1 : z.H)), dim3(256), 0, stream, (const float*)parts, dlam, B, z.H, tiles, z.shared);
 }
 
 }  // namespace
@@ -991,7 +1051,7 @@ extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const 
 
 // Workspace: the rows' statistics [B, H, 4, S], then dlambda's parts [B, H, ceil(S / 128)], fp32
 extern "C" int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H) {
-  return B <= 0 || S <= 0 || H <= 0 ? 0 : stats_bytes(B, S, H) + ((int64_t)B * H * tiles_of(S) * 4 + 255) / 256 * 256;
+  return B <= 0 || S <= 0 || H <= 0 ? 0 : stats_bytes(B, S, H) + ((int64_t)B * H * ((S + 63) / 64) * 4 + 255) / 256 * 256;
 }
 
 extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const void* k, const void* v, const float* lam, const void* o, const void* o2, const float* lse,
