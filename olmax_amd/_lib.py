@@ -68,7 +68,7 @@ _SIGNATURES = {
     "olmax_attn_bwd": "PPPPPPPPPPPLIIIIILLLLLLLLIF",
     "olmax_rotary_fwd": "PPPPPPLIIIIILLII",
     "olmax_rotary_bwd": "PPPPPPLIIIIILLII",
-    "olmax_diff_attn_fwd": "PPPPPPPPIIIIILLLLLII",
+    "olmax_diff_attn_fwd": "PPPPPPPPPLIIIIILLLLLII",
     "olmax_diff_attn_bwd": "PPPPPPPPPPPPPPLIIIIILLLLLLLLLII",
     "olmax_token_logprobs": "PPPPPPPPPLLILIIIFF",
     "olmax_token_logprobs_bwd": "PPPPPPPLILLIIFF",

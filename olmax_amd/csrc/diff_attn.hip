@@ -11,6 +11,7 @@
 // The kernels are laid out as those of attn.hip: score tiles are transposed, a lane owns one query (forward, dQ) or one key (dK/dV), and a [rows][W] tile of K or Q holds both
 // maps' halves of a row, k-steps 0 .. W/32 - 1 of the products the first one's.
 #include "attn_tiles.h"
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <type_traits>
@@ -21,6 +22,22 @@ namespace {
 // 4 B per lane straight into LDS, as dma16
 __device__ __forceinline__ void dma4(const void* g, unsigned lds_addr) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_addr), "v"(g) : "m0", "memory");
+}
+
+// Where workgroups would be few and their chains long, a chain is dealt to n workgroups, size steps to each; what they have goes to memory in fp32, [row][n], and a second kernel joins it.  See plan_of.
+constexpr int MOST_CHUNKS = 64;
+struct Chunks {
+  float* to;
+  int size, n;
+  int upto[MOST_CHUNKS];  // chains that have a chunk p are the longest upto[p] - upto[p - 1]: workgroup w of a head has the chunk p with w in between, of one of these
+};
+struct Place { int chain, part; };
+template <bool PART>
+__device__ __forceinline__ Place place_of(const Chunks& ch, int w) {
+  if constexpr (!PART) return {w, 0};
+  int p = 0, before = 0;
+  while (p + 1 < ch.n && w >= ch.upto[p]) before = ch.upto[p++];
+  return {w - before, p};
 }
 
 struct Sizes {
@@ -176,6 +193,13 @@ __device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16*
   }
 }
 
+// The lane, formed where it is needed rather than kept in a register
+__device__ __forceinline__ int lane_id() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
+
 // f(0) .. f(N - 1) with the index as a constant (a loop of 48 products is not unrolled before its arrays would have to be registers)
 template <typename F, int... I>
 __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
@@ -221,9 +245,9 @@ __device__ __forceinline__ void part_ends() {  // at most the newest N transfers
   __builtin_amdgcn_sched_barrier(0);
 }
 constexpr int smem_fwd(int W) { return 2 * 3 * 64 * W * 2; }
-template <int W, int QW>
+template <int W, int QW, bool PART>
 __global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
-                                                               bf16* __restrict__ O, bf16* __restrict__ O2, float* __restrict__ LSE, const Sizes z) {
+                                                               bf16* __restrict__ O, bf16* __restrict__ O2, float* __restrict__ LSE, const Sizes z, const Chunks ch) {
   constexpr int TILE = 64 * W * 2;  // bytes of a K or V tile of 64 keys
   constexpr int KS = W / 32;        // k-steps of a map
   constexpr int QR = QW * 32;       // queries of the workgroup
@@ -236,8 +260,9 @@ __global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* 
   const int l32 = lane & 31, lhi = lane >> 5;
   const int qw = wave % QW, m = wave / QW;
   const int nqt = (S + QR - 1) / QR;
-  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
-  const int qt = nqt - 1 - wg.rank;  // longest rows first
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / ((PART ? ch.upto[ch.n - 1] : nqt) * (H / KH))), H / KH);
+  const Place place = place_of<PART>(ch, wg.rank);
+  const int qt = nqt - 1 - place.chain, part = place.part;  // longest rows first
   const int b = wg.group / KH, kh = wg.group % KH;
   const int h = kh * (H / KH) + wg.r;
   const int i0 = qt * QR;
@@ -251,8 +276,13 @@ __global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* 
 #pragma unroll
     for (int s = 0; s < KS; s++) qf[s] = *reinterpret_cast<const bf16x8*>(qp + s * 16);
   }
-  const int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
-  const int t_hi = min(i0 + QR - 1, S - 1) >> 6;  // inclusive
+  int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
+  int t_hi = min(i0 + QR - 1, S - 1) >> 6;  // inclusive
+  if constexpr (PART) {
+    t_lo += part * ch.size;
+    if (t_lo > t_hi) return;
+    t_hi = min(t_hi, t_lo + ch.size - 1);
+  }
 
   f32x16 o[W / 32], st[2];
 #pragma unroll
@@ -378,6 +408,19 @@ __global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* 
   __syncthreads();
 
   const float total = half_swap_sum(sum);
+  if constexpr (PART) {
+    if (qi < S) {
+      float* to = ch.to + ((((int64_t)b * H + h) * S + qi) * ch.n + part) * (2 * W + 4);
+#pragma unroll
+      for (int u = 0; u < W / 8; u++)
+        *reinterpret_cast<f32x4*>(to + m * W + u * 8 + lhi * 4) = f32x4{o[u >> 2][(u & 3) * 4], o[u >> 2][(u & 3) * 4 + 1], o[u >> 2][(u & 3) * 4 + 2], o[u >> 2][(u & 3) * 4 + 3]};
+      if (lhi == 0) {
+        to[2 * W + m] = mx;
+        to[2 * W + 2 + m] = total;
+      }
+    }
+    return;
+  }
   const float inv = total > 0.f ? 1.f / total : 0.f;
   const float lse = (mx + log2f(total)) * LN2;
   float zeros = lse * 0.f;  // NaN where something of a row is not finite; rows behind the sequence are none
@@ -432,6 +475,56 @@ __global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* 
   });
 }
 
+// Joins a row's chunks: a wave to a row, a lane to columns l and l + 64.  qr: queries of a workgroup of the first kernel.  Bound by the latency of loads that mostly hit the caches: 10 us for 1 x 8192
+// tokens of one head of 64 (38 MB).
+template <int W>
+__global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+                                                                 bf16* __restrict__ O, bf16* __restrict__ O2, float* __restrict__ LSE, const Sizes z, const Chunks ch, int qr) {
+  const int S = z.S, H = z.H, window = z.window, lane = threadIdx.x & 63;
+  const int per = (S + 3) / 4, bh = blockIdx.x / per, i = blockIdx.x % per * 4 + (threadIdx.x >> 6);
+  if (i >= S) return;
+  const int b = bh / H, h = bh % H, kh = h / (H / z.KH);
+  const int i0 = i / qr * qr;
+  const int n = ((min(i0 + qr, S) - 1) / 64 - (window >= 0 ? max(0, i0 - window) : 0) / 64) / ch.size + 1;
+  const float* from = ch.to + ((int64_t)bh * S + i) * ch.n * (2 * W + 4);
+  const float lam = LAM[z.shared ? 0 : h];
+  // lane c has the statistics of chunk c (there are at most 64); the chunks' loads do not wait for each other
+  float y[2][W / 64] = {}, w[2], lse[2];
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    const float* st = from + min(lane, n - 1) * (2 * W + 4) + 2 * W + m;
+    const float mine = lane < n ? st[0] : -INFINITY, mx = wave_max(mine);
+    w[m] = fexp2(mine - mx);
+    const float sum = wave_sum(lane < n ? w[m] * st[2] : 0.f);
+    w[m] /= sum;
+    lse[m] = (mx + log2f(sum)) * LN2;
+  }
+#pragma unroll 4
+  for (int c = 0; c < n; c++) {
+    const float* p = from + c * (2 * W + 4) + lane;
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+      for (int x = 0; x < W / 64; x++) y[m][x] = __builtin_fmaf(__shfl(w[m], c, 64), p[m * W + x * 64], y[m][x]);
+  }
+  const int64_t at = (int64_t)b * S + i;
+  bf16 *o = O + at * z.ldo + h * W, *o2 = O2 ? O2 + at * z.ldo2 + h * W : nullptr;
+  float* lse_row = LSE + (int64_t)bh * 2 * S + i;
+  float zeros = (lse[0] + lse[1]) * 0.f;
+#pragma unroll
+  for (int x = 0; x < W / 64; x++) {
+    const float v = __builtin_fmaf(-lam, y[1][x], y[0][x]);
+    zeros = __builtin_fmaf(v, 0.f, __builtin_fmaf(y[1][x], 0.f, zeros));
+    o[x * 64 + lane] = f2bf(v);
+    if (O2) o2[x * 64 + lane] = f2bf(y[1][x]);
+  }
+  if (lane < 2) lse_row[lane * S] = lane ? lse[1] : lse[0];
+  if (__builtin_amdgcn_ballot_w64(zeros != 0.f)) {
+    dma_wait_all();
+    redo_fwd<W>(Q + at * z.ldq + h * W, K + (int64_t)b * S * z.ldk + kh * W, z.ldk, V + (int64_t)b * S * z.ldv + kh * W, z.ldv, lam, o, o2, lse_row, S, i, window, z.scale, lane, 0, W);
+  }
+}
+
 // ---------------------------------------------------------------------------------------
 // dQ, dlambda and delta.  grid = ceil(S / 32 QW) H B workgroups of QW x KG waves; wave (qw, kg) owns 32 queries and every KG-th of their key tiles.  KG = 1 (QW = 4): two workgroups per CU, no merge.
 // KG > 1: one workgroup of eight waves with 1 / KG of the chain of tiles; what they have is added through LDS, in key-group order.  See q_split.
@@ -449,10 +542,10 @@ struct Lambda {
   float* dlam;
   int batch, tiles;
 };
-template <int W, int QW, int KG>
+template <int W, int QW, int KG, bool PART>
 __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
                                                               const bf16* __restrict__ O, const bf16* __restrict__ O2, const float* __restrict__ LSE, const bf16* __restrict__ dO,
-                                                              bf16* __restrict__ dQ, float* __restrict__ STATS, float* __restrict__ DLAM, const Sizes z, const Grad gr) {
+                                                              bf16* __restrict__ dQ, float* __restrict__ STATS, float* __restrict__ DLAM, const Sizes z, const Grad gr, const Chunks ch) {
   constexpr int TILE = 64 * W * 2, KS = W / 32;
   constexpr int QR = QW * 32;         // queries of the workgroup
   constexpr int TEAMS = QW * KG / 4;  // tiles are fetched by teams of 4 waves
@@ -464,8 +557,9 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   const int l32 = lane & 31, lhi = lane >> 5;
   const int qw = wave % QW, kg = wave / QW, wv = wave & 3, team = wave >> 2;
   const int nqt = (S + QR - 1) / QR;
-  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (nqt * (H / KH))), H / KH);
-  const int qt = nqt - 1 - wg.rank;
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / ((PART ? ch.upto[ch.n - 1] : nqt) * (H / KH))), H / KH);
+  const Place place = place_of<PART>(ch, wg.rank);
+  const int qt = nqt - 1 - place.chain, part = place.part;
   const int b = wg.group / KH, kh = wg.group % KH;
   const int h = kh * (H / KH) + wg.r;
   const int i0 = qt * QR;
@@ -473,6 +567,13 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   const int qi = iw0 + l32;
   const int qic = min(qi, S - 1);
   const float lam = LAM[z.shared ? 0 : h];
+  int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
+  int t_hi = min(i0 + QR - 1, S - 1) >> 6;
+  if constexpr (PART) {
+    t_lo += part * ch.size;
+    if (t_lo > t_hi) return;
+    t_hi = min(t_hi, t_lo + ch.size - 1);
+  }
 
   bf16x8 qf[W / 16], dof[W / 16];
   float d1 = 0.f, d2 = 0.f;
@@ -498,9 +599,6 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   d1 = __builtin_fmaf(lam, d2, half_swap_sum(d1));  // o + lambda O_2 = O_1
   const int64_t row0 = ((int64_t)b * H + h) * 2 * S;
   const float l1 = LSE[row0 + qic] * LOG2E, l2 = LSE[row0 + S + qic] * LOG2E;
-  const int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
-  const int t_hi = min(i0 + QR - 1, S - 1) >> 6;
-
   f32x16 dq[W / 32];
 #pragma unroll
   for (int dt = 0; dt < W / 32; dt++)
@@ -609,6 +707,19 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   }
   sum1 = half_swap_sum(sum1);
   sum2 = half_swap_sum(sum2);
+  if constexpr (PART) {
+    if (qi < S) {
+      float* to = ch.to + ((((int64_t)b * H + h) * S + qi) * ch.n + part) * (W + 4);
+#pragma unroll
+      for (int u = 0; u < W / 8; u++)
+        *reinterpret_cast<f32x4*>(to + u * 8 + lhi * 4) = f32x4{dq[u >> 2][(u & 3) * 4], dq[u >> 2][(u & 3) * 4 + 1], dq[u >> 2][(u & 3) * 4 + 2], dq[u >> 2][(u & 3) * 4 + 3]};
+      if (lhi == 0) {
+        to[W] = sum1;
+        to[W + 1] = sum2;
+      }
+    }
+    return;
+  }
   if constexpr (KG > 1) {  // the key groups' sums, in their order
     if (lhi == 0) {
       sums[kg][qw * 32 + l32][0] = sum1;
@@ -665,6 +776,57 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   if (tid == 0) DLAM[((int64_t)b * H + h) * nqt + qt] = -dl;
 }
 
+// Joins dQ's chunks: 16 waves, of 4 rows each, to 64 queries; a lane to columns l and l + 64.
+template <int W>
+__global__ __launch_bounds__(1024) void diff_attn_dq_join_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+                                                                const bf16* __restrict__ O, const bf16* __restrict__ O2, const float* __restrict__ LSE, const bf16* __restrict__ dO,
+                                                                bf16* __restrict__ dQ, float* __restrict__ STATS, float* __restrict__ DLAM, const Sizes z, const Grad gr, const Chunks ch, int qr) {
+  __shared__ float red[16];
+  const int S = z.S, H = z.H, window = z.window, lane = threadIdx.x & 63;
+  const int per = (S + 63) / 64, bh = blockIdx.x / per;
+  const int b = bh / H, h = bh % H, kh = h / (H / z.KH);
+  const float lam = LAM[z.shared ? 0 : h];
+  float total = 0.f;
+  for (int r = 0; r < 4; r++) {
+    const int i = blockIdx.x % per * 64 + r * 16 + (threadIdx.x >> 6);
+    if (i >= S) break;
+    const int i0 = i / qr * qr;
+    const int n = ((min(i0 + qr, S) - 1) / 64 - (window >= 0 ? max(0, i0 - window) : 0) / 64) / ch.size + 1;
+    const float* from = ch.to + ((int64_t)bh * S + i) * ch.n * (W + 4);
+    float y[W / 64] = {}, sum1 = 0.f, sum2 = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < n; c++, from += W + 4) {
+#pragma unroll
+      for (int x = 0; x < W / 64; x++) y[x] += from[x * 64 + lane];
+      sum1 += from[W];
+      sum2 += from[W + 1];
+    }
+    const int64_t at = (int64_t)b * S + i;
+    bf16* dq = dQ + at * gr.lddq + h * W;
+    const float* lse = LSE + (int64_t)bh * 2 * S + i;
+    const float l1 = lse[0], l2 = lse[S];
+    float zeros = (sum1 + sum2) * 0.f;
+#pragma unroll
+    for (int x = 0; x < W / 64; x++) {
+      const float v = y[x] * (x * 64 + lane < W / 2 ? z.scale : -lam * z.scale);
+      zeros = __builtin_fmaf(v, 0.f, zeros);
+      dq[x * 64 + lane] = f2bf(v);
+    }
+    if (__builtin_amdgcn_ballot_w64(zeros != 0.f)) {
+      dma_wait_all();
+      const bf16* d_o = dO + at * gr.lddo + h * W;
+      const float d2 = dot(O2 + at * z.ldo2 + h * W, d_o, W), d1 = __builtin_fmaf(lam, d2, dot(O + at * z.ldo + h * W, d_o, W));
+      redo_dq<W>(Q + at * z.ldq + h * W, K + (int64_t)b * S * z.ldk + kh * W, z.ldk, V + (int64_t)b * S * z.ldv + kh * W, z.ldv, d_o, l1, l2, d1, d2, lam, dq, i, window, z.scale, lane, 0, W, sum1,
+                 sum2);
+    }
+    if (lane < 4) STATS[((int64_t)bh * 4 + lane) * S + i] = lane == 0 ? l1 * LOG2E : lane == 1 ? l2 * LOG2E : lane == 2 ? -sum1 : sum1 - sum2;
+    total += sum2;
+  }
+  const float dl = block_sum<16>(lane == 0 ? total : 0.f, red);
+  if (threadIdx.x == 0) DLAM[blockIdx.x] = -dl;
+}
+
+
 // ---------------------------------------------------------------------------------------
 // dK/dV.  grid = ceil(S / 32 KW) KH B workgroups of KW x QS waves; wave (kw, qs) owns 32 keys and every QS-th of the pairs of a query head of the group and one of its 32-row
 // tiles from the diagonal on.  LDS: per query group 2 stages of (Q | dO | the 32 rows' statistics), then the fragments of V and K.
@@ -678,10 +840,31 @@ constexpr int smem_kv(int W, int KW, int QS) {
   const int run = QS * 2 * (2 * 32 * W * 2 + 512) + KW * (W / 16 + k_parked(W, KW)) * 1024, sums = QS > 1 ? KW * QS * 32 * W * 4 : 0;
   return run > sums ? run : sums;
 }
-template <int W, int KW, int QS>
+// dlambda of a head (or of all): dQ's sums, [B][H][tiles], in their order; the last workgroups, which have the least to do
+template <int WAVES>
+__device__ __forceinline__ void add_dlambda(const Lambda& la, int H, int shared, int wave) {
+  __shared__ float red[WAVES];
+  for (int64_t n = gridDim.x - 1 - blockIdx.x; n < (shared ? 1 : H); n += gridDim.x) {
+    const int64_t per = (int64_t)la.tiles * (shared ? H : 1);
+    const int lane = lane_id();
+    float sum = 0.f;
+    for (int c = 0; c < la.batch; c++) {
+      const float* p = la.parts + ((int64_t)c * H + n) * la.tiles;
+      for (int64_t i = wave * 64 + lane; i < per; i += WAVES * 64) sum += p[i];
+    }
+    sum = wave_sum(sum);
+    __syncthreads();
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    sum = red[0];
+    for (int w = 1; w < WAVES; w++) sum += red[w];
+    if (wave == 0 && lane == 0) la.dlam[n] = sum;
+  }
+}
+template <int W, int KW, int QS, bool PART>
 __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
                                                                         const float* __restrict__ STATS, const bf16* __restrict__ dO,
-                                                                        bf16* __restrict__ dK, bf16* __restrict__ dV, const Sizes z, const Grad gr, const Lambda la) {
+                                                                        bf16* __restrict__ dK, bf16* __restrict__ dV, const Sizes z, const Grad gr, const Lambda la, const Chunks ch) {
   constexpr int QT = 32, KS = W / 32;
   constexpr int TILE = QT * W * 2, STAGE = 2 * TILE + 512;
   constexpr int KT = KW * 32;         // keys of the workgroup
@@ -692,13 +875,22 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, lhi = lane >> 5;
   const int kw = wave % KW, qs = wave / KW, wv = wave & 3, team = wave >> 2;
-  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / ((S + KT - 1) / KT)), 1);  // key tile 0 is seen by every query: longest first
+  const WgCoord wg = decode_wg(blockIdx.x, (int)(gridDim.x / (PART ? ch.upto[ch.n - 1] : (S + KT - 1) / KT)), 1);  // key tile 0 is seen by every query: longest first
   const int b = wg.group / KH, kh = wg.group % KH;
   const int rep = H / KH;
-  const int j0 = wg.rank * KT;
+  const Place place = place_of<PART>(ch, wg.rank);
+  const int j0 = place.chain * KT, part = place.part;
   const int jw0 = j0 + kw * 32;
   const int kj = jw0 + l32;  // this lane's key
   const int kjc = min(kj, S - 1);
+
+  const int i_hi = window >= 0 ? min(S - 1, j0 + KT - 1 + window) : S - 1;
+  const int t_lo = j0 / QT, t_hi = i_hi / QT;  // inclusive
+  int total = (t_hi - t_lo + 1) * rep;
+  if constexpr (PART) {
+    if (part * ch.size >= total) return;
+    total = min(total - part * ch.size, ch.size);
+  }
 
   // K's and V's fragments of these keys: K's first in registers, the others in LDS, each the 1 KB that a read takes
   constexpr int PARKED = k_parked(W, KW), HELD = 2 * KS - PARKED, FIXED = 2 * KS + PARKED;
@@ -723,10 +915,6 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
 #pragma unroll
     for (int r = 0; r < 16; r++) { dk[dt][r] = 0.f; dv[dt][r] = 0.f; }
 
-  const int i_hi = window >= 0 ? min(S - 1, j0 + KT - 1 + window) : S - 1;
-  const int t_lo = j0 / QT, t_hi = i_hi / QT;  // inclusive
-  const int ntile = t_hi - t_lo + 1;
-  const int total = ntile * rep;
   const float sc2 = z.scale * LOG2E;
   const unsigned char* sgrp = smem + qs * (2 * STAGE);  // this query group's stages
 
@@ -743,7 +931,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
     }
   };
   auto first = [&](int n) {
-    Iter x{0, t_hi};
+    Iter x = PART ? Iter{part * ch.size % rep, t_hi - part * ch.size / rep} : Iter{0, t_hi};
     advance(x, n);
     return x;
   };
@@ -764,15 +952,13 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
         tq.issue(qp + (int64_t)t * QT * z.ldq, dst, wv);
         tdo.issue(dp + (int64_t)t * QT * gr.lddo, dst + TILE, wv);
       } else {
-        int l = lane;
-        asm volatile("" : "+v"(l));
+        const int l = lane_id();
         dma_tile<QT, W>(qp, z.ldq, t * QT, S, dst, wv, l);
         dma_tile<QT, W>(dp, gr.lddo, t * QT, S, dst + TILE, wv, l);
       }
     }
     if (kw == 0 && (QS == 1 || round * QS + qs < total)) {  // the rows' statistics: lanes 0 .. 31 the first of two, 32 .. 63 the second
-      int l = lane;
-      asm volatile("" : "+v"(l));
+      const int l = lane_id();
       const float* st = STATS + (((int64_t)b * H + kh * rep + own.h) * 4 + (l >> 5)) * S + min(own.t * QT + (l & 31), S - 1);
       const unsigned dst = lds0 + (qs * 2 + stage) * STAGE + 2 * TILE;
       dma4(st, dst);
@@ -833,11 +1019,13 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
         }
         pin();
       }
-      if (need_mask)
-        hide(s1, s2, lane, kj, [&](int k, int j) {
+      if (need_mask) {
+        const int l = lane_id();
+        hide(s1, s2, l, jw0 + (l & 31), [&](int k, int j) {
           const int i = ib + k;
           return j > i || i >= S || (window >= 0 && j < i - window);
         });
+      }
 #pragma unroll
       for (int r = 0; r < 16; r++) dp[r] = of4(2, r);  // -delta_1
       pin();
@@ -882,8 +1070,20 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
     dma_wait_all();
     __syncthreads();
   }
-  bf16* kp = dK + ((int64_t)b * S + kjc) * gr.lddk + kh * W;
-  bf16* vp = dV + ((int64_t)b * S + kjc) * gr.lddv + kh * W;
+  const int le = lane_id(), ke = jw0 + (le & 31);
+  if constexpr (PART) {
+    if (ke < S) {
+      float* to = ch.to + ((((int64_t)b * KH + kh) * S + ke) * ch.n + part) * (2 * W) + (le >> 5) * 4;
+#pragma unroll
+      for (int u = 0; u < W / 8; u++) {
+        *reinterpret_cast<f32x4*>(to + u * 8) = f32x4{dk[u >> 2][(u & 3) * 4], dk[u >> 2][(u & 3) * 4 + 1], dk[u >> 2][(u & 3) * 4 + 2], dk[u >> 2][(u & 3) * 4 + 3]};
+        *reinterpret_cast<f32x4*>(to + W + u * 8) = f32x4{dv[u >> 2][(u & 3) * 4], dv[u >> 2][(u & 3) * 4 + 1], dv[u >> 2][(u & 3) * 4 + 2], dv[u >> 2][(u & 3) * 4 + 3]};
+      }
+    }
+    return;
+  }
+  bf16* kp = dK + ((int64_t)b * S + min(ke, S - 1)) * gr.lddk + kh * W;
+  bf16* vp = dV + ((int64_t)b * S + min(ke, S - 1)) * gr.lddv + kh * W;
   float zeros = 0.f;
   auto store4 = [&](bf16* p, int dt, int g, const f32x4& v, float mul) {
     Pack4 pk;
@@ -893,10 +1093,10 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
       zeros = __builtin_fmaf(x, 0.f, zeros);
       pk.e[e] = f2bf(x);
     }
-    *reinterpret_cast<u32x2*>(p + dt * 32 + g * 8 + lhi * 4) = pk.u;
+    *reinterpret_cast<u32x2*>(p + dt * 32 + g * 8 + (le >> 5) * 4) = pk.u;
   };
   if constexpr (QS == 1) {
-    if (kj < S) {
+    if (ke < S) {
 #pragma unroll
       for (int dt = 0; dt < W / 32; dt++)
 #pragma unroll
@@ -908,36 +1108,65 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
     }
   } else {
     // the stages are free: the last round ended in a barrier; dK first, then dV in the same space
-    add_partials<W, QS>(smem, dk, kw, qs, lane, [&](int u, const f32x4& v) {
-      if (kj < S) store4(kp, u >> 2, u & 3, v, z.scale);
+    add_partials<W, QS>(smem, dk, kw, qs, le, [&](int u, const f32x4& v) {
+      if (ke < S) store4(kp, u >> 2, u & 3, v, z.scale);
     });
     __syncthreads();
-    add_partials<W, QS>(smem, dv, kw, qs, lane, [&](int u, const f32x4& v) {
-      if (kj < S) store4(vp, u >> 2, u & 3, v, 1.f);
+    add_partials<W, QS>(smem, dv, kw, qs, le, [&](int u, const f32x4& v) {
+      if (ke < S) store4(vp, u >> 2, u & 3, v, 1.f);
     });
   }
-  redo_rows(kj < S ? zeros : 0.f, [&](int r) {
+  redo_rows(ke < S ? zeros : 0.f, [&](int r) {
     const int64_t seq = (int64_t)b * S, at = seq + jw0 + r, row = ((int64_t)b * H + kh * rep) * 4 * S;
     redo_dkv<W>(Q + seq * z.ldq + kh * rep * W, z.ldq, dO + seq * gr.lddo + kh * rep * W, gr.lddo, STATS + row, LAM + (z.shared ? 0 : kh * rep), z.shared ? 0 : 1,
-                K + at * z.ldk + kh * W, V + at * z.ldv + kh * W, dK + at * gr.lddk + kh * W, dV + at * gr.lddv + kh * W, jw0 + r, S, rep, window, z.scale, lane,
+                K + at * z.ldk + kh * W, V + at * z.ldv + kh * W, dK + at * gr.lddk + kh * W, dV + at * gr.lddv + kh * W, jw0 + r, S, rep, window, z.scale, le,
                 qs * (W / QS), (qs + 1) * (W / QS));
   });
-  // dlambda of a head (or of all): dQ's sums, [B][H][tiles], in their order; the last workgroups, which have the least to do
-  __shared__ float red[KW * QS];
-  for (int64_t n = gridDim.x - 1 - blockIdx.x; n < (z.shared ? 1 : H); n += gridDim.x) {
-    const int64_t per = (int64_t)la.tiles * (z.shared ? H : 1);
-    float sum = 0.f;
-    for (int c = 0; c < la.batch; c++) {
-      const float* p = la.parts + ((int64_t)c * H + n) * la.tiles;
-      for (int64_t i = tid; i < per; i += KW * QS * 64) sum += p[i];
+  add_dlambda<KW * QS>(la, H, z.shared, wave);
+}
+
+// Joins dK's and dV's chunks: a wave to a key.  kt: keys of a workgroup of the first kernel.
+template <int W>
+__global__ __launch_bounds__(256) void diff_attn_dkv_join_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
+                                                                 const float* __restrict__ STATS, const bf16* __restrict__ dO, bf16* __restrict__ dK, bf16* __restrict__ dV, const Sizes z,
+                                                                 const Grad gr, const Lambda la, const Chunks ch, int kt) {
+  const int S = z.S, H = z.H, KH = z.KH, window = z.window, rep = H / KH, lane = threadIdx.x & 63;
+  const int per = (S + 3) / 4, bk = blockIdx.x / per, j = blockIdx.x % per * 4 + (threadIdx.x >> 6);
+  const int b = bk / KH, kh = bk % KH;
+  if (j < S) {
+    const int j0 = j / kt * kt, i_hi = window >= 0 ? min(S - 1, j0 + kt - 1 + window) : S - 1;
+    const int n = ((i_hi / 32 - j0 / 32 + 1) * rep + ch.size - 1) / ch.size;
+    const float* from = ch.to + ((int64_t)bk * S + j) * ch.n * (2 * W) + lane;
+    float yk[W / 64] = {}, yv[W / 64] = {}, zeros = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < n; c++, from += 2 * W)
+#pragma unroll
+      for (int x = 0; x < W / 64; x++) {
+        yk[x] += from[x * 64];
+        yv[x] += from[W + x * 64];
+      }
+    const int64_t seq = (int64_t)b * S, at = seq + j;
+    bf16 *dk = dK + at * gr.lddk + kh * W, *dv = dV + at * gr.lddv + kh * W;
+#pragma unroll
+    for (int x = 0; x < W / 64; x++) {
+      zeros = __builtin_fmaf(yk[x] * z.scale, 0.f, __builtin_fmaf(yv[x], 0.f, zeros));
+      dk[x * 64 + lane] = f2bf(yk[x] * z.scale);
+      dv[x * 64 + lane] = f2bf(yv[x]);
     }
-    sum = block_sum<KW * QS>(sum, red);
-    if (tid == 0) la.dlam[n] = sum;
+    if (__builtin_amdgcn_ballot_w64(zeros != 0.f)) {
+      dma_wait_all();
+      redo_dkv<W>(Q + seq * z.ldq + kh * rep * W, z.ldq, dO + seq * gr.lddo + kh * rep * W, gr.lddo, STATS + ((int64_t)b * H + kh * rep) * 4 * S, LAM + (z.shared ? 0 : kh * rep), z.shared ? 0 : 1,
+                  K + at * z.ldk + kh * W, V + at * z.ldv + kh * W, dk, dv, j, S, rep, window, z.scale, lane, 0, W);
+    }
   }
+  add_dlambda<4>(la, H, z.shared, threadIdx.x >> 6);
 }
 
 
+
 int64_t tiles_of(int32_t S) { return ((int64_t)S + 127) / 128; }  // of 128 queries
+// a number for 64 queries at least
+int64_t parts_bytes(int32_t B, int32_t S, int32_t H) { return ((int64_t)B * H * (((int64_t)S + 63) / 64) * 4 + 255) / 256 * 256; }
 int64_t stats_bytes(int32_t B, int32_t S, int32_t H) { return ((int64_t)B * H * 4 * S * 4 + 255) / 256 * 256; }
 
 constexpr int64_t MAX_LD = 1 << 24;  // of a row, in elements: 64 rows are within reach of a 32-bit offset in bytes
@@ -983,53 +1212,147 @@ bool dkv_narrow(int B, const Sizes& z) { return (int64_t)((z.S + 63) / 64) * z.K
 template <int W>
 bool fwd_halves(int B, const Sizes& z) { return W == 64 || tiles_of(z.S) * z.H * B <= 128; }
 
+// Dealing chains out.  `tiles` chains of steps(i) steps to each of `heads`, on `places` workgroups that the GPU holds at once: chunks of `size` steps, the smallest size (4 at least) with which no
+// workgroup waits for a place, since a second round costs as much as the first.  It is done where the longest chain, which without it is shared by `groups` groups of waves of one workgroup, gets
+// shorter by `margin` steps, or else the chunks' way through memory and the second launch cost more.  us, dealt out and not, B x S, H/KH heads of 64 (32):
+// forward, margin 20: 54, 162 (49, 136) 1 x 8192, 1/1; 39, 85 (36, 71) 1 x 4096, 2/1; 33, 47 (29, 39) 1 x 2048, 4/4; 43, 48 (40, 39) 1 x 2048, 8/2; below it 37, 29 (34, 24) 1 x 1000, 16/4.
+// A backward pass with only dQ's dealt out, margin 12: 233, 327 (145, 179) 1 x 8192, 1/1; 211, 246 1 x 4096, 2/1; below it 115, 112 (65, 61) 1 x 1000, 4/1; 131, 121 (97, 81) 1 x 2048, 16/16.
+// With only dK/dV's, margin 6 (steps of half the size): 375, 484 1 x 4096, 16/4; 106, 210 (67, 106) 1 x 2048, 8/2; 75, 116 (51, 61) 1 x 1000, 16/4; 38, 48 1 x 300, 4/1; below it
+// 226, 206 (142, 131) 1 x 4096, 8/8; 687, 633 1 x 4096, 32/8; 137, 157 (92, 86) 1 x 4000, 8/2 with a window of 1024.
+template <typename F>
+Chunks plan_of(int64_t tiles, int64_t heads, int places, int groups, int margin, F steps) {  // steps(0) the longest chain's
+  Chunks ch{nullptr, 0, 1, {}};
+  ch.upto[0] = (int)tiles;
+  if (tiles * heads > 2 * places) return ch;
+  int64_t total = 0, longest = 0;
+  for (int64_t i = 0; i < tiles; i++) {
+    const int64_t n = steps(i);
+    total += n * heads;
+    longest = std::max(longest, n);
+  }
+  int64_t size = std::max({(total + places - 1) / places, (int64_t)4, (longest + MOST_CHUNKS - 1) / MOST_CHUNKS});
+  for (; longest / groups - size >= margin; size += (size + 15) / 16) {
+    int n = (int)((longest + size - 1) / size), sum = 0;
+    for (int p = 0; p < n; p++) {
+      int64_t last = tiles;
+      while (last > 0 && steps(last - 1) <= p * size) last--;
+      ch.upto[p] = sum += (int)last;
+    }
+    if (sum * heads > places) continue;
+    ch.size = (int)size;
+    ch.n = n;
+    return ch;
+  }
+  ch.upto[0] = (int)tiles;
+  return ch;
+}
+int64_t key_tiles(const Sizes& z, int64_t i0, int64_t qr) {  // of the workgroup of queries i0 .. i0 + qr - 1
+  const int64_t hi = i0 + qr < z.S ? i0 + qr - 1 : z.S - 1, lo = z.window >= 0 && i0 > z.window ? i0 - z.window : 0;
+  return hi / 64 - lo / 64 + 1;
+}
+int fwd_queries(int W) { return W == 64 ? 64 : 128; }
+Chunks fwd_plan(int B, const Sizes& z, int W) {
+  const int64_t qr = fwd_queries(W);
+  return plan_of((z.S + qr - 1) / qr, (int64_t)z.H * B, W == 64 ? 512 : 256, 1, 20, [&](int64_t i) { return key_tiles(z, ((z.S + qr - 1) / qr - 1 - i) * qr, qr); });
+}
+Chunks dq_plan(int B, const Sizes& z, int W) {
+  return plan_of(((int64_t)z.S + 127) / 128, (int64_t)z.H * B, 512, qs_groups(W), 12, [&](int64_t i) { return key_tiles(z, (((int64_t)z.S + 127) / 128 - 1 - i) * 128, 128); });
+}
+Chunks dkv_plan(int B, const Sizes& z, int W) {
+  return plan_of(((int64_t)z.S + 127) / 128, (int64_t)z.KH * B, 512, W == 64 && dkv_narrow(B, z) ? 8 : 4, 6, [&](int64_t i) {
+    const int64_t j0 = i * 128, hi = z.window >= 0 && j0 + 127 + z.window < z.S ? j0 + 127 + z.window : z.S - 1;
+    return (hi / 32 - j0 / 32 + 1) * (z.H / z.KH);
+  });
+}
+int64_t fwd_chunk_bytes(int B, const Sizes& z, int W) {
+  const Chunks c = fwd_plan(B, z, W);
+  return c.n < 2 ? 0 : (int64_t)B * z.H * z.S * c.n * (2 * W + 4) * 4;
+}
+int64_t bwd_chunk_bytes(int B, const Sizes& z, int W) {
+  const Chunks q = dq_plan(B, z, W), k = dkv_plan(B, z, W);
+  const int64_t nq = q.n < 2 ? 0 : (int64_t)B * z.H * z.S * q.n * (W + 4) * 4, nk = k.n < 2 ? 0 : (int64_t)B * z.KH * z.S * k.n * 2 * W * 4;
+  return nq > nk ? nq : nk;
+}
+
 template <int W>
-void fwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const float* lam, bf16* o, bf16* o2, float* lse, int B, const Sizes& z) {
+void fwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const float* lam, bf16* o, bf16* o2, float* lse, float* workspace, int B, const Sizes& z) {
+  constexpr int QW = W == 64 ? 2 : 4;
   static std::once_flag once;
   std::call_once(once, [] {
-    if constexpr (W != 64) (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W));
-    (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W));
+    (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W, QW, false>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W));
+    (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W, 2, false>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W));
+    (void)hipFuncSetAttribute((const void*)diff_attn_fwd_kernel<W, QW, true>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_fwd(W));
   });
+  Chunks ch = fwd_plan(B, z, W);
+  ch.to = workspace;
   auto run = [&](auto kern, int qw) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)((z.S + 32 * qw - 1) / (32 * qw)) * z.H * B)), dim3(128 * qw), smem_fwd(W), stream, q, k, v, lam, o, o2, lse, z);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((ch.n > 1 ? ch.upto[ch.n - 1] : (int64_t)((z.S + 32 * qw - 1) / (32 * qw))) * z.H * B)), dim3(128 * qw), smem_fwd(W), stream, q, k, v, lam, o, o2, lse, z, ch);
   };
-  if constexpr (W != 64) {
-    if (!fwd_halves<W>(B, z)) return run(diff_attn_fwd_kernel<W, 4>, 4);
-  }
-  run(diff_attn_fwd_kernel<W, 2>, 2);
+  if (ch.n > 1) {
+    run(diff_attn_fwd_kernel<W, QW, true>, QW);
+    hipLaunchKernelGGL(diff_attn_fwd_join_kernel<W>, dim3((unsigned)((int64_t)((z.S + 3) / 4) * z.H * B)), dim3(256), 0, stream, q, k, v, lam, o, o2, lse, z, ch, 32 * QW);
+  } else if (fwd_halves<W>(B, z)) run(diff_attn_fwd_kernel<W, 2, false>, 2);
+  else run(diff_attn_fwd_kernel<W, QW, false>, QW);
 }
 
 template <int W>
 void bwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const float* lam, const bf16* o, const bf16* o2, const float* lse, const bf16* d_o, bf16* dq, bf16* dk,
-         bf16* dv, float* dlam, float* stats, float* parts, int B, const Sizes& z, const Grad& gr) {
+         bf16* dv, float* dlam, float* stats, float* parts, float* chunks, int B, const Sizes& z, const Grad& gr) {
+  constexpr int QG = qs_groups(W);
   static std::once_flag once;
   std::call_once(once, [] {
-    (void)hipFuncSetAttribute((const void*)diff_attn_dq_kernel<W, 4, 1>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W, 1));
-    (void)hipFuncSetAttribute((const void*)diff_attn_dq_kernel<W, QSW, qs_groups(W)>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_q(W, qs_groups(W)));
-    (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 4, 1>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 4, 1));
-    if constexpr (W == 64) (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 1, 8>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 1, 8));
-    (void)hipFuncSetAttribute((const void*)diff_attn_dkv_kernel<W, 2, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, smem_kv(W, 2, 4));
+    auto room = [](auto kern, int bytes) { (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); };
+    room(diff_attn_dq_kernel<W, 4, 1, false>, smem_q(W, 1));
+    room(diff_attn_dq_kernel<W, 4, 1, true>, smem_q(W, 1));
+    room(diff_attn_dq_kernel<W, QSW, QG, false>, smem_q(W, QG));
+    room(diff_attn_dkv_kernel<W, 4, 1, false>, smem_kv(W, 4, 1));
+    room(diff_attn_dkv_kernel<W, 4, 1, true>, smem_kv(W, 4, 1));
+    room(diff_attn_dkv_kernel<W, 2, 4, false>, smem_kv(W, 2, 4));
+    if constexpr (W == 64) room(diff_attn_dkv_kernel<W, 1, 8, false>, smem_kv(W, 1, 8));
   });
+  Chunks cq = dq_plan(B, z, W), ck = dkv_plan(B, z, W);
+  cq.to = ck.to = chunks;  // (dK/dV's are written when dQ's have been joined)
   int tiles = 0;
   auto dq_of = [&](auto kern, int qw, int kg) {
     tiles = (z.S + 32 * qw - 1) / (32 * qw);
-    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(64 * qw * kg), smem_q(W, kg), stream, q, k, v, lam, o, o2, lse, d_o, dq, stats, parts, z, gr);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)(cq.n > 1 ? cq.upto[cq.n - 1] : tiles) * z.H * B)), dim3(64 * qw * kg), smem_q(W, kg), stream, q, k, v, lam, o, o2, lse, d_o, dq, stats, parts, z, gr, cq);
   };
-  if (q_split(B, z)) dq_of(diff_attn_dq_kernel<W, QSW, qs_groups(W)>, QSW, qs_groups(W));
-  else dq_of(diff_attn_dq_kernel<W, 4, 1>, 4, 1);
+  if (cq.n > 1) {
+    dq_of(diff_attn_dq_kernel<W, 4, 1, true>, 4, 1);
+    tiles = (z.S + 63) / 64;
+    hipLaunchKernelGGL(diff_attn_dq_join_kernel<W>, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(1024), 0, stream, q, k, v, lam, o, o2, lse, d_o, dq, stats, parts, z, gr, cq, 128);
+  } else if (q_split(B, z)) dq_of(diff_attn_dq_kernel<W, QSW, QG, false>, QSW, QG);
+  else dq_of(diff_attn_dq_kernel<W, 4, 1, false>, 4, 1);
+  const Lambda la{parts, dlam, B, tiles};
   auto kv = [&](auto kern, int kw, int qs) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)((z.S + 32 * kw - 1) / (32 * kw)) * z.KH * B)), dim3(64 * kw * qs), smem_kv(W, kw, qs), stream, q, k, v, lam, (const float*)stats, d_o, dk, dv, z, gr, Lambda{parts, dlam, B, tiles});
+    hipLaunchKernelGGL(kern, dim3((unsigned)((ck.n > 1 ? ck.upto[ck.n - 1] : (int64_t)((z.S + 32 * kw - 1) / (32 * kw))) * z.KH * B)), dim3(64 * kw * qs), smem_kv(W, kw, qs), stream, q, k, v, lam, (const float*)stats, d_o,
+                       dk, dv, z, gr, la, ck);
   };
-  if constexpr (W == 64) {
-    if (dkv_narrow(B, z)) return kv(diff_attn_dkv_kernel<W, 1, 8>, 1, 8);
+  if (ck.n > 1) {
+    kv(diff_attn_dkv_kernel<W, 4, 1, true>, 4, 1);
+    hipLaunchKernelGGL(diff_attn_dkv_join_kernel<W>, dim3((unsigned)((int64_t)((z.S + 3) / 4) * z.KH * B)), dim3(256), 0, stream, q, k, v, lam, (const float*)stats, d_o, dk, dv, z, gr, la, ck, 128);
+    return;
   }
-  if (dkv_split(B, z)) kv(diff_attn_dkv_kernel<W, 2, 4>, 2, 4);
-  else kv(diff_attn_dkv_kernel<W, 4, 1>, 4, 1);
+  if constexpr (W == 64) {
+    if (dkv_narrow(B, z)) return kv(diff_attn_dkv_kernel<W, 1, 8, false>, 1, 8);
+  }
+  if (dkv_split(B, z)) kv(diff_attn_dkv_kernel<W, 2, 4, false>, 2, 4);
+  else kv(diff_attn_dkv_kernel<W, 4, 1, false>, 4, 1);
 }
 
 }  // namespace
 
-extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const void* k, const void* v, const float* lam, void* o, void* o2, float* lse, int32_t B, int32_t S,
+// (shapes that the calls refuse need none)
+static bool sizes_of(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window, Sizes& z) {
+  if (B <= 0 || S <= 0 || H <= 0 || KH <= 0 || H % KH || (D != 32 && D != 64)) return false;
+  z = Sizes{S, H, KH, window < 0 || window >= S ? -1 : window, 0, 0, 0, 0, 0, 0.f, 0};
+  return true;
+}
+extern "C" int64_t olmax_diff_attn_fwd_workspace_bytes(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window) {
+  Sizes z;
+  return sizes_of(B, S, H, KH, D, window, z) ? fwd_chunk_bytes(B, z, 2 * D) : 0;
+}
+extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const void* k, const void* v, const float* lam, void* o, void* o2, float* lse, void* workspace, int64_t workspace_bytes, int32_t B, int32_t S,
                                        int32_t H, int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t ldo2, int32_t lam_shared, int32_t window) {
   OLMAX_CHECK(q && k && v && lam && o && lse, OLMAX_ERR_ARG, "olmax_diff_attn_fwd: null pointer");
   if (int rc = check_shape("olmax_diff_attn_fwd", B, S, H, KH, D)) return rc;
@@ -1044,14 +1367,18 @@ extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const 
                 "olmax_diff_attn_fwd: an output shares memory with an input");
   OLMAX_CHECK(!meet(o, ldo, H * W, o2, ldo2, H * W, rows), OLMAX_ERR_ARG, "olmax_diff_attn_fwd: o and o2 share memory");
   const Sizes z{S, H, KH, window < 0 || window >= S ? -1 : window, ldq, ldk, ldv, ldo, ldo2, 1.f / sqrtf((float)D), lam_shared != 0};
-  (D == 64 ? fwd<128> : fwd<64>)(stream, (const bf16*)q, (const bf16*)k, (const bf16*)v, lam, (bf16*)o, (bf16*)o2, lse, B, z);
+  const int64_t need = fwd_chunk_bytes(B, z, (int)W);
+  OLMAX_CHECK(need == 0 || (workspace && workspace_bytes >= need && (((uintptr_t)workspace) & 15) == 0), OLMAX_ERR_WORKSPACE,
+              "olmax_diff_attn_fwd: workspace needs %ld bytes, 16-byte aligned", (long)need);
+  (D == 64 ? fwd<128> : fwd<64>)(stream, (const bf16*)q, (const bf16*)k, (const bf16*)v, lam, (bf16*)o, (bf16*)o2, lse, (float*)workspace, B, z);
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }
 
 // Workspace: the rows' statistics [B, H, 4, S], then dlambda's parts [B, H, ceil(S / 128)], fp32
-extern "C" int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H) {
-  return B <= 0 || S <= 0 || H <= 0 ? 0 : stats_bytes(B, S, H) + ((int64_t)B * H * ((S + 63) / 64) * 4 + 255) / 256 * 256;
+extern "C" int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window) {
+  Sizes z;
+  return sizes_of(B, S, H, KH, D, window, z) ? stats_bytes(B, S, H) + parts_bytes(B, S, H) + bwd_chunk_bytes(B, z, 2 * D) : 0;
 }
 
 extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const void* k, const void* v, const float* lam, const void* o, const void* o2, const float* lse,
@@ -1069,8 +1396,8 @@ extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const 
   for (int i = 0; i < 3; i++) ok = ok && rows_ok(outs[i], ld_out[i], n_out[i]);
   OLMAX_CHECK(ok, OLMAX_ERR_ALIGN, "olmax_diff_attn_bwd: operands must be 16-byte aligned, with row strides that are multiples of 8, at least heads * 2D and below 2^24");
   OLMAX_CHECK((((uintptr_t)lam | (uintptr_t)lse | (uintptr_t)dlam) & 3) == 0, OLMAX_ERR_ALIGN, "olmax_diff_attn_bwd: lam, lse and dlam not aligned to their type");
-  OLMAX_CHECK(workspace_bytes >= olmax_diff_attn_bwd_workspace_bytes(B, S, H) && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE,
-              "olmax_diff_attn_bwd: workspace needs %ld bytes, 256-byte aligned", (long)olmax_diff_attn_bwd_workspace_bytes(B, S, H));
+  const int64_t need = olmax_diff_attn_bwd_workspace_bytes(B, S, H, KH, D, window);
+  OLMAX_CHECK(workspace_bytes >= need && (((uintptr_t)workspace) & 255) == 0, OLMAX_ERR_WORKSPACE, "olmax_diff_attn_bwd: workspace needs %ld bytes, 256-byte aligned", (long)need);
   for (int x = 0; x < 3; x++) {
     for (int i = 0; i < 6; i++) apart = apart && !meet(ins[i], ld_in[i], n_in[i], outs[x], ld_out[x], n_out[x], rows);
     for (int y = 0; y < x; y++) apart = apart && !meet(outs[y], ld_out[y], n_out[y], outs[x], ld_out[x], n_out[x], rows);
@@ -1079,7 +1406,7 @@ extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const 
   const Sizes z{S, H, KH, window < 0 || window >= S ? -1 : window, ldq, ldk, ldv, ldo, ldo2, 1.f / sqrtf((float)D), lam_shared != 0};
   const Grad gr{lddo, lddq, lddk, lddv};
   (D == 64 ? bwd<128> : bwd<64>)(stream, (const bf16*)q, (const bf16*)k, (const bf16*)v, lam, (const bf16*)o, (const bf16*)o2, lse, (const bf16*)d_o, (bf16*)dq, (bf16*)dk, (bf16*)dv,
-                                 dlam, (float*)workspace, (float*)((char*)workspace + stats_bytes(B, S, H)), B, z, gr);
+                                 dlam, (float*)workspace, (float*)((char*)workspace + stats_bytes(B, S, H)), (float*)((char*)workspace + stats_bytes(B, S, H) + parts_bytes(B, S, H)), B, z, gr);
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }

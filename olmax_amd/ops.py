@@ -382,8 +382,11 @@ def diff_attn_fwd(q, k, v, lam, *, B: int, S: int, H: int, KH: int, D: int, wind
         out = q.new_empty((T, wide))
     o2 = q.new_empty((T, wide)) if want_grad else None
     lse = lam.new_empty((B, H, 2, S))
-    check(typed("olmax_diff_attn_fwd")(raw_stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), out.data_ptr(), _ptr(o2), lse.data_ptr(), B, S, H, KH, D,
-                                       ldq, ldk, ldv, _head_rows(out, T, wide, "out"), wide, int(lam.shape[0] != H), -1 if window is None else window))
+    window = -1 if window is None else window
+    nbytes = _size32("olmax_diff_attn_fwd_workspace_bytes", B, S, H, KH, D, window)
+    ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    check(typed("olmax_diff_attn_fwd")(raw_stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), out.data_ptr(), _ptr(o2), lse.data_ptr(), _ptr(ws), nbytes,
+                                       B, S, H, KH, D, ldq, ldk, ldv, _head_rows(out, T, wide, "out"), wide, int(lam.shape[0] != H), window))
     return DiffAttention(out, o2, lse)
 
 
@@ -399,11 +402,12 @@ def diff_attn_bwd(q, k, v, lam, o, o2, lse, do, *, B: int, S: int, H: int, KH: i
     dlam = torch.empty_like(lam)
     lds = [_head_rows(t, T, n, what) for t, n, what in ((q, wide, "q"), (k, narrow, "k"), (v, narrow, "v"), (o, wide, "o"), (o2, wide, "o2"), (do, wide, "do"),
                                                         (dq, wide, "dq"), (dk, narrow, "dk"), (dv, narrow, "dv"))]
-    nbytes = _size32("olmax_diff_attn_bwd_workspace_bytes", B, S, H)
+    window = -1 if window is None else window
+    nbytes = _size32("olmax_diff_attn_bwd_workspace_bytes", B, S, H, KH, D, window)
     ws = q.new_empty((nbytes,), dtype=torch.uint8)
     check(typed("olmax_diff_attn_bwd")(raw_stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), o.data_ptr(), o2.data_ptr(), lse.data_ptr(), do.data_ptr(),
                                        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), nbytes, B, S, H, KH, D, *lds, int(lam.shape[0] != H),
-                                       -1 if window is None else window))
+                                       window))
     return dq, dk, dv, dlam
 
 

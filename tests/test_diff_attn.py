@@ -18,7 +18,7 @@ def at(i):
 B, S, H, KH, D = 2, 100, 4, 2, 64
 Q, KV = H * 2 * D, KH * 2 * D
 SIZES = dict(B=B, S=S, H=H, KH=KH, D=D)
-FWD = dict(stream=None, q=at(0), k=at(1), v=at(2), lam=at(3), o=at(4), o2=at(5), lse=at(6), **SIZES, ldq=Q, ldk=KV, ldv=KV, ldo=Q, ldo2=Q, shared=0, window=-1)
+FWD = dict(stream=None, q=at(0), k=at(1), v=at(2), lam=at(3), o=at(4), o2=at(5), lse=at(6), ws=at(12), nbytes=1 << 27, **SIZES, ldq=Q, ldk=KV, ldv=KV, ldo=Q, ldo2=Q, shared=0, window=-1)
 BWD = dict(stream=None, q=at(0), k=at(1), v=at(2), lam=at(3), o=at(4), o2=at(5), lse=at(6), do=at(7), dq=at(8), dk=at(9), dv=at(10), dlam=at(11), ws=at(12), nbytes=1 << 27, **SIZES,
            ldq=Q, ldk=KV, ldv=KV, ldo=Q, ldo2=Q, lddo=Q, lddq=Q, lddk=KV, lddv=KV, shared=0, window=-1)
 CALLS = {"olmax_diff_attn_fwd": FWD, "olmax_diff_attn_bwd": BWD}
@@ -32,7 +32,8 @@ ONLY_BWD += [(dict(dlam=at(11) + 1), ALIGN), (dict(nbytes=100), WORKSPACE), (dic
 # memory that an output shares with an input or another output
 ONLY_BWD += [(dict(dq=at(0)), ARG), (dict(dk=at(1)), ARG), (dict(dq=at(7)), ARG), (dict(dv=at(9)), ARG), (dict(dk=at(9), dv=at(9) + 2 * KV, lddk=2 * KV, lddv=4 * KV), ARG),
              (dict(dk=at(8) + 2 * 128), ARG), (dict(dv=at(5) + 2 * Q * 3), ARG)]
-ONLY_FWD = [(dict(o=at(0)), ARG), (dict(o=at(2)), ARG), (dict(o2=at(4)), ARG), (dict(o2=at(4) + 2 * 64), ARG), (dict(o=at(1) - 2 * 64), ARG)]
+FEW = dict(B=1, S=8192, H=1, KH=1)
+ONLY_FWD = [({**FEW, "ws": None}, WORKSPACE), ({**FEW, "nbytes": 1000}, WORKSPACE), ({**FEW, "ws": at(12) + 8}, WORKSPACE), (dict(o=at(0)), ARG), (dict(o=at(2)), ARG), (dict(o2=at(4)), ARG), (dict(o2=at(4) + 2 * 64), ARG), (dict(o=at(1) - 2 * 64), ARG)]
 
 
 @pytest.mark.parametrize("name,change,code", [(n, c, r) for n in CALLS for c, r in BOTH] + [("olmax_diff_attn_bwd", c, r) for c, r in ONLY_BWD] +
@@ -48,9 +49,12 @@ def test_workspace_sizes():
     from olmax_amd import ops
     lib()
     size = lambda *a: ops._size32("olmax_diff_attn_bwd_workspace_bytes", *a)  # noqa: E731
-    assert size(0, 1, 1) == size(1, 0, 1) == size(1, 1, 0) == 0
-    assert size(1, 1, 1) > 0
-    assert size(8, 1 << 20, 128) > 1 << 32  # (beyond 32 bits)
+    assert size(0, 1, 1, 1, 64, -1) == size(1, 0, 1, 1, 64, -1) == size(1, 1, 0, 1, 64, -1) == size(1, 1, 1, 0, 64, -1) == size(1, 1, 1, 1, 48, -1) == 0
+    assert size(1, 1, 1, 1, 64, -1) > 0
+    assert size(8, 1 << 20, 128, 32, 64, -1) > 1 << 32  # (beyond 32 bits)
+    size = lambda *a: ops._size32("olmax_diff_attn_fwd_workspace_bytes", *a)  # noqa: E731
+    assert size(0, 8192, 1, 1, 64, -1) == size(1, 8192, 1, 1, 48, -1) == size(1, 100, 4, 2, 64, -1) == size(2, 4096, 32, 8, 64, -1) == 0
+    assert size(1, 8192, 1, 1, 64, -1) > 8192 * 2 * (256 + 4) * 4 - 1  # a long sequence of one head is split
 
 
 def test_wrappers_refuse():

@@ -115,7 +115,11 @@ SHAPES = [  # B, S, H, KH, D, window, shared
     (1, 1, 1, 1, 32, None, False), (1, 1, 2, 1, 64, None, True), (2, 2, 2, 2, 64, None, False), (2, 33, 4, 2, 64, None, False), (1, 64, 2, 2, 32, None, False), (1, 65, 3, 3, 64, None, True),
     (3, 127, 4, 1, 32, None, False), (1, 128, 8, 8, 64, None, False), (1, 129, 3, 1, 64, None, False), (2, 300, 4, 2, 64, 100, False), (1, 257, 2, 1, 32, 0, False), (1, 200, 2, 2, 64, 1, True),
     (3, 130, 6, 2, 32, 64, False), (1, 700, 4, 4, 64, None, False), (1, 515, 16, 2, 32, 63, False), (1, 640, 8, 4, 64, 128, False), (5, 48, 10, 5, 64, 47, False), (1, 90, 4, 2, 64, 1000, False),
-    (1, 1100, 2, 1, 64, None, True), (1, 1030, 8, 8, 64, 300, False)]
+    (1, 1100, 2, 1, 64, None, True), (1, 1030, 8, 8, 64, 300, False),
+    # grids that fill the GPU: forms of 128 queries and keys to a workgroup
+    (41, 130, 16, 8, 64, None, False), (41, 130, 8, 8, 32, 100, True), (3, 300, 20, 20, 32, None, False), (3, 300, 40, 20, 64, None, False), (33, 65, 40, 20, 64, 0, False),
+    # few rows, long chains: dealt to many workgroups and joined
+    (1, 2111, 1, 1, 64, None, False), (2, 1600, 2, 1, 32, None, True), (1, 4103, 1, 1, 32, None, False), (1, 3001, 2, 2, 64, 2000, False), (1, 1000, 4, 1, 32, 500, False)]
 
 
 @pytest.mark.parametrize("B,S,H,KH,D,window,shared", SHAPES)
@@ -177,23 +181,33 @@ def test_the_parts_of_fused_rows(D):
 @pytest.mark.parametrize("D,window", [(64, None), (32, None), (64, 40)])
 def test_what_a_row_does_not_see_does_not_reach_it(D, window, value):
     """Infinities and NaN in one token's keys and values reach the queries that see it, in its query and dO the keys that it sees, and nothing else."""
-    sizes = dict(B=2, S=200, H=4, KH=2, D=D)
-    W, at = 2 * D, 100
+    unseen(dict(B=2, S=200, H=4, KH=2, D=D), window, 100, value)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("D,window,S,at", [(64, None, 1700, 1500), (32, None, 4100, 70), (64, 1500, 2300, 700)])
+def test_nor_where_chains_are_split(D, window, S, at, value):
+    unseen(dict(B=1, S=S, H=2, KH=1, D=D), window, at, value)
+
+
+def unseen(sizes, window, at, value):
+    B, S, W = sizes["B"], sizes["S"], 2 * sizes["D"]
+    T, last = B * S, min(S, at + window + 1) if window else S
     x = make(**sizes, seed=8)
     p = Plain(*x, window, **sizes)
     q, k, v, lam, do = (t.clone() for t in x)
     k[at, 1] = value
     v[at, 3] = value
     r = forward((q, k, v, lam, do), sizes, window)
-    sees = torch.zeros(400, dtype=torch.bool)
-    sees[at: min(200, at + window + 1) if window else 200] = True
+    sees = torch.zeros(T, dtype=torch.bool)
+    sees[at: last] = True
     rest = ~sees
     near(r.o[rest.cuda()], p.o[rest], p.o_room[rest], "o")
     near(r.o2[rest.cuda()], p.o2[rest], p.o2_room[rest], "o2")
-    near(r.o[:, 2 * W:], p.o[:, 2 * W:], p.o_room[:, 2 * W:], "the other group's heads")
+    if sizes["KH"] > 1:
+        near(r.o[:, 2 * W:], p.o[:, 2 * W:], p.o_room[:, 2 * W:], "the other group's heads")
     assert not r.o[at, : 2 * W].isfinite().all()
-    lse = torch.zeros(2, 200, dtype=torch.bool)
-    lse[0] = sees[:200]
+    lse = sees.view(B, S)
     keep = ~lse[:, None, None, :].expand_as(p.lse)
     near(r.lse[keep.cuda()], p.lse[keep], p.lse_room[keep], "lse")
     # dQ of the queries that do not see it; dK, dV of the keys that a bad query does not see
@@ -203,11 +217,11 @@ def test_what_a_row_does_not_see_does_not_reach_it(D, window, value):
     q[at, 1] = value
     do[at, 2] = value
     g = backward((q, k, v, lam, do), p, sizes, window)
-    seen = torch.zeros(400, dtype=torch.bool)
+    seen = torch.zeros(T, dtype=torch.bool)
     seen[max(0, at - window) if window else 0: at + 1] = True
     for i, name in ((1, "dk"), (2, "dv")):
         near(g[i][~seen.cuda()], p.grads[i][~seen], getattr(p, name + "_room")[~seen], name)
-    rest = torch.ones(400, dtype=torch.bool)
+    rest = torch.ones(T, dtype=torch.bool)
     rest[at] = False
     near(g[0][rest.cuda()], p.grads[0][rest], p.dq_room[rest], "dq of the other queries")
 
@@ -246,8 +260,31 @@ def test_a_graph_replayed_over_new_inputs():
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), rep
 
 
-def test_two_streams_at_once():
-    sizes = dict(B=2, S=500, H=8, KH=2, D=64)
+def test_two_graphs_share_a_pool():
+    """Long chains, whose chunks lie in workspaces, in two graphs that take their memory from one pool, replayed in turn."""
+    sizes = dict(B=1, S=1800, H=2, KH=1, D=64)
+    works = [[t.cuda() for t in make(**sizes, seed=s)] for s in (1, 2)]
+
+    def step(q, k, v, lam, do):
+        r = ops().diff_attn_fwd(q, k, v, lam, **sizes)
+        return (r.o, r.lse, *ops().diff_attn_bwd(q, k, v, lam, r.o, r.o2, r.lse, do, **sizes))
+    want = [step(*w) for w in works]
+    torch.cuda.synchronize()
+    graphs, outs, pool = [torch.cuda.CUDAGraph() for _ in works], [], torch.cuda.graph_pool_handle()
+    for g, w in zip(graphs, works):
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(step(*w))
+    for rep in range(3):
+        for i in (0, 1, 1, 0):
+            for t in outs[i]:
+                t.zero_()
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i])), (rep, i)
+
+
+@pytest.mark.parametrize("sizes", [dict(B=2, S=500, H=8, KH=2, D=64), dict(B=1, S=1800, H=2, KH=1, D=64)])
+def test_two_streams_at_once(sizes):
     works = [[t.cuda() for t in make(**sizes, seed=s)] for s in (1, 2)]
 
     def step(q, k, v, lam, do):
