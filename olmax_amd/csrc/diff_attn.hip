@@ -118,24 +118,32 @@ __device__ __forceinline__ void pair_of(const bf16* q, const bf16* k, const bf16
   dp = dot(d_o, v, W);
 }
 
-// columns [lo, hi) of the row; d1, d2: delta as dS takes it; sum1, sum2: the row's sums of P_m dP
+// columns [lo, hi) of the row; sum1, sum2: the row's sums of P_m dP, which are its delta
 template <int W>
-__device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ldk, const bf16* V, int64_t ldv, const bf16* d_o, float l1, float l2, float d1, float d2, float lam,
-                                        bf16* dq, int i, int window, float scale, int lane, int lo, int hi, float& sum1, float& sum2) {
+__device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ldk, const bf16* V, int64_t ldv, const bf16* d_o, float l1, float l2, float lam, bf16* dq, int i, int window,
+                                        float scale, int lane, int lo, int hi, float& sum1, float& sum2) {
   constexpr int D = W / 2;
+  const int first = window >= 0 ? max(0, i - window) : 0;
   float acc[W / 64] = {};
   sum1 = sum2 = 0.f;
 #pragma unroll 1
-  for (int j0 = window >= 0 ? max(0, i - window) : 0; j0 <= i; j0 += 64) {
+  for (int j = first + lane; j <= i; j += 64) {
+    float p1, p2, dp;
+    pair_of<W>(q, K + j * ldk, d_o, V + j * ldv, l1, l2, scale, p1, p2, dp);
+    sum1 += p1 * dp;
+    sum2 += p2 * dp;
+  }
+  sum1 = wave_sum(sum1);
+  sum2 = wave_sum(sum2);
+#pragma unroll 1
+  for (int j0 = first; j0 <= i; j0 += 64) {
     const int n = min(64, i - j0 + 1);
     float s1 = 0.f, s2 = 0.f;
     if (lane < n) {
       float p1, p2, dp;
       pair_of<W>(q, K + (j0 + lane) * ldk, d_o, V + (j0 + lane) * ldv, l1, l2, scale, p1, p2, dp);
-      sum1 += p1 * dp;
-      sum2 += p2 * dp;
-      s1 = p1 * (dp - d1);
-      s2 = -lam * p2 * (dp - d2);
+      s1 = p1 * (dp - sum1);
+      s2 = -lam * p2 * (dp - sum2);
     }
 #pragma unroll 1
     for (int t = 0; t < n; t++) {
@@ -144,8 +152,6 @@ __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ld
       for (int c = 0; c < W / 64; c++) acc[c] += (c * 64 + lane < D ? a : b) * bf2f(K[(j0 + t) * ldk + c * 64 + lane]);
     }
   }
-  sum1 = wave_sum(sum1);
-  sum2 = wave_sum(sum2);
 #pragma unroll
   for (int c = 0; c < W / 64; c++)
     if (c * 64 + lane >= lo && c * 64 + lane < hi) dq[c * 64 + lane] = f2bf(acc[c] * scale);
@@ -528,9 +534,11 @@ __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __r
 // ---------------------------------------------------------------------------------------
 // dQ, dlambda and delta.  grid = ceil(S / 32 QW) H B workgroups of QW x KG waves; wave (qw, kg) owns 32 queries and every KG-th of their key tiles.  KG = 1 (QW = 4): two workgroups per CU, no merge.
 // KG > 1: one workgroup of eight waves with 1 / KG of the chain of tiles; what they have is added through LDS, in key-group order.  See q_split.
-// dQ takes delta from the outputs as they were rounded, as dQ of attn.hip does.  The sums of P_m dP come out of the same sweep in fp32: dK/dV takes its delta from them (its error at 4096 tokens 0.0027 of
-// itself -> 0.0024, the rounding of dS and of the result), and dlambda is their sum: terms of both signs, that an error of 2^-9 in each would leave three digits of.  (For dQ, whose error is
-// 0.0027, they come too late: another sweep ahead would be two thirds of this kernel.)
+// The sums of P_m dP come out of the same sweep in fp32: dK/dV takes its delta from them, and dlambda is their sum: terms of both signs, that an error of 2^-9 in each would leave three digits of.
+// For dQ they come too late, and it takes delta from the outputs as they were rounded, as dQ of attn.hip does; but where a workgroup has SWEEP key tiles or fewer, a sweep ahead forms them first.
+// A row that sees few keys has most to lose: its dP - delta is small beside delta, and its gradients are the largest.  dQ's error as a share of its norm, and us of a backward pass, without the sweep,
+// with, and with it everywhere (rounding dS and the result alone makes 0.0023): 5 tokens 0.0069, 0.0022; 3 x 333, 4/2 heads of 32 0.0031, 0.0025; 25.8, 30.5 us; 1 x 1000, 8/4, window 333
+// 0.0029, 0.0024; 46, 56 us; 1 x 4096, 32/8 0.0027, 0.0026, 0.0024; 609, 613, 777 us.
 // STATS [B, H, 4, S]: what dK/dV takes of a row: lse_1 and lse_2 in powers of two, -delta_1, and delta_1 - delta_2 (dP - delta_2 is what it has of the first map, plus this).  DLAM: a number for
 // each workgroup, [B, H, tiles].
 // ---------------------------------------------------------------------------------------
@@ -542,6 +550,7 @@ struct Lambda {
   float* dlam;
   int batch, tiles;
 };
+constexpr int SWEEP = 8;
 template <int W, int QW, int KG, bool PART>
 __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
                                                               const bf16* __restrict__ O, const bf16* __restrict__ O2, const float* __restrict__ LSE, const bf16* __restrict__ dO,
@@ -569,6 +578,7 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   const float lam = LAM[z.shared ? 0 : h];
   int t_lo = (window >= 0 ? max(0, i0 - window) : 0) >> 6;
   int t_hi = min(i0 + QR - 1, S - 1) >> 6;
+  const int all_lo = t_lo, all_hi = t_hi;
   if constexpr (PART) {
     t_lo += part * ch.size;
     if (t_lo > t_hi) return;
@@ -599,13 +609,6 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   d1 = __builtin_fmaf(lam, d2, half_swap_sum(d1));  // o + lambda O_2 = O_1
   const int64_t row0 = ((int64_t)b * H + h) * 2 * S;
   const float l1 = LSE[row0 + qic] * LOG2E, l2 = LSE[row0 + S + qic] * LOG2E;
-  f32x16 dq[W / 32];
-#pragma unroll
-  for (int dt = 0; dt < W / 32; dt++)
-#pragma unroll
-    for (int r = 0; r < 16; r++) dq[dt][r] = 0.f;
-  float sum1 = 0.f, sum2 = 0.f;  // of P_m dP
-
   const bf16* kbase = K + (int64_t)b * S * z.ldk + kh * W;
   const bf16* vbase = V + (int64_t)b * S * z.ldv + kh * W;
   const unsigned lds0 = lds_addr_of(smem);
@@ -613,7 +616,7 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   dk.init(z.ldk, wv, lane);
   dv.init(z.ldv, wv, lane);
   // K/V tiles of round r: tile t_lo + r KG + g for key group g
-  auto load_kv = [&](int round, int stage) {
+  auto load_kv = [&](int t_lo, int t_hi, int round, int stage) {
 #pragma unroll
     for (int g0 = 0; g0 < KG / TEAMS; g0++) {
       const int g = g0 * TEAMS + team, t = t_lo + round * KG + g;
@@ -632,13 +635,84 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   FragAddr<W, W == 128> fa;  // (short of registers)
   fa.init(lane);
 
-  load_kv(0, 0);
+  float sum1 = 0.f, sum2 = 0.f;  // of P_m dP
+  auto add_groups = [&] {  // the halves' sums, and the key groups', in their order
+    sum1 = half_swap_sum(sum1);
+    sum2 = half_swap_sum(sum2);
+    if constexpr (KG > 1) {
+      if (lhi == 0) {
+        sums[kg][qw * 32 + l32][0] = sum1;
+        sums[kg][qw * 32 + l32][1] = sum2;
+      }
+      __syncthreads();
+      sum1 = sum2 = 0.f;
+#pragma unroll
+      for (int g = 0; g < KG; g++) {
+        sum1 += sums[g][qw * 32 + l32][0];
+        sum2 += sums[g][qw * 32 + l32][1];
+      }
+    }
+  };
+  if (all_hi - all_lo < SWEEP) {  // delta by a sweep ahead
+    const int rounds = (all_hi - all_lo + KG) / KG;
+    load_kv(all_lo, all_hi, 0, 0);
+    dma_wait_all();
+    __syncthreads();
+    for (int round = 0; round < rounds; round++) {
+      const int cur = round & 1;
+      if (round + 1 < rounds) load_kv(all_lo, all_hi, round + 1, cur ^ 1);
+      const int t = all_lo + round * KG + kg, j0 = t * 64;
+      if ((KG == 1 || t <= all_hi) && j0 <= iw0 + 31 && (window < 0 || j0 + 63 >= iw0 - window)) {
+        const unsigned char* sk = smem + (kg * 2 + cur) * (2 * TILE);
+        const unsigned char* sv = sk + TILE;
+        const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
+#pragma unroll 1
+        for (int jt = 0; jt < 2; jt++) {
+          f32x16 s1, s2, dp;
+#pragma unroll
+          for (int r = 0; r < 16; r++) s1[r] = s2[r] = dp[r] = 0.f;
+#pragma unroll
+          for (int s = 0; s < KS; s++) {
+            s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, s), qf[s], s1, 0, 0, 0);
+            s2 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sk, jt * 32, KS + s), qf[KS + s], s2, 0, 0, 0);
+          }
+#pragma unroll
+          for (int s = 0; s < 2 * KS; s++) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa.load_kc(sv, jt * 32, s), dof[s], dp, 0, 0, 0);
+          if (need_mask)
+            hide(s1, s2, lane, qi, [&](int k, int i) {
+              const int j = j0 + jt * 32 + k;
+              return j > i || (window >= 0 && j < i - window);
+            });
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            sum1 = __builtin_fmaf(fexp2(__builtin_fmaf(s1[r], sc2, -l1)), dp[r], sum1);
+            sum2 = __builtin_fmaf(fexp2(__builtin_fmaf(s2[r], sc2, -l2)), dp[r], sum2);
+          }
+        }
+      }
+      dma_wait_all();
+      __syncthreads();
+    }
+    add_groups();
+    d1 = sum1;
+    d2 = sum2;
+  }
+
+  f32x16 dq[W / 32];
+#pragma unroll
+  for (int dt = 0; dt < W / 32; dt++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) dq[dt][r] = 0.f;
+  sum1 = sum2 = 0.f;
+
+
+  load_kv(t_lo, t_hi, 0, 0);
   dma_wait_all();
   __syncthreads();
   const int rounds = (t_hi - t_lo + KG) / KG;
   for (int round = 0; round < rounds; round++) {
     const int cur = round & 1;
-    if (round + 1 < rounds) load_kv(round + 1, cur ^ 1);
+    if (round + 1 < rounds) load_kv(t_lo, t_hi, round + 1, cur ^ 1);
     const int t = t_lo + round * KG + kg, j0 = t * 64;
     const bool visible = (KG == 1 || t <= t_hi) && j0 <= iw0 + 31 && (window < 0 || j0 + 63 >= iw0 - window);
     if (visible) {
@@ -705,8 +779,7 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
     dma_wait_all();
     __syncthreads();
   }
-  sum1 = half_swap_sum(sum1);
-  sum2 = half_swap_sum(sum2);
+  add_groups();
   if constexpr (PART) {
     if (qi < S) {
       float* to = ch.to + ((((int64_t)b * H + h) * S + qi) * ch.n + part) * (W + 4);
@@ -719,19 +792,6 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
       }
     }
     return;
-  }
-  if constexpr (KG > 1) {  // the key groups' sums, in their order
-    if (lhi == 0) {
-      sums[kg][qw * 32 + l32][0] = sum1;
-      sums[kg][qw * 32 + l32][1] = sum2;
-    }
-    __syncthreads();
-    sum1 = sum2 = 0.f;
-#pragma unroll
-    for (int g = 0; g < KG; g++) {
-      sum1 += sums[g][qw * 32 + l32][0];
-      sum2 += sums[g][qw * 32 + l32][1];
-    }
   }
   float zeros = 0.f;
   auto store4 = [&](int u, const f32x4& v) {
@@ -759,7 +819,7 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
     const int i = iw0 + r;
     const int64_t at = (int64_t)b * S + i;
     float a, c;
-    redo_dq<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, dO + at * gr.lddo + h * W, LSE[row0 + i], LSE[row0 + S + i], __shfl(d1, r, 64), __shfl(d2, r, 64), lam,
+    redo_dq<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, dO + at * gr.lddo + h * W, LSE[row0 + i], LSE[row0 + S + i], lam,
                dQ + at * gr.lddq + h * W, i, window, z.scale, lane, kg * (W / KG), (kg + 1) * (W / KG), a, c);
     sum1 = l32 == r ? a : sum1;
     sum2 = l32 == r ? c : sum2;
@@ -779,7 +839,7 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
 // Joins dQ's chunks: 16 waves, of 4 rows each, to 64 queries; a lane to columns l and l + 64.
 template <int W>
 __global__ __launch_bounds__(1024) void diff_attn_dq_join_kernel(const bf16* __restrict__ Q, const bf16* __restrict__ K, const bf16* __restrict__ V, const float* __restrict__ LAM,
-                                                                const bf16* __restrict__ O, const bf16* __restrict__ O2, const float* __restrict__ LSE, const bf16* __restrict__ dO,
+                                                                const float* __restrict__ LSE, const bf16* __restrict__ dO,
                                                                 bf16* __restrict__ dQ, float* __restrict__ STATS, float* __restrict__ DLAM, const Sizes z, const Grad gr, const Chunks ch, int qr) {
   __shared__ float red[16];
   const int S = z.S, H = z.H, window = z.window, lane = threadIdx.x & 63;
@@ -814,10 +874,8 @@ __global__ __launch_bounds__(1024) void diff_attn_dq_join_kernel(const bf16* __r
     }
     if (__builtin_amdgcn_ballot_w64(zeros != 0.f)) {
       dma_wait_all();
-      const bf16* d_o = dO + at * gr.lddo + h * W;
-      const float d2 = dot(O2 + at * z.ldo2 + h * W, d_o, W), d1 = __builtin_fmaf(lam, d2, dot(O + at * z.ldo + h * W, d_o, W));
-      redo_dq<W>(Q + at * z.ldq + h * W, K + (int64_t)b * S * z.ldk + kh * W, z.ldk, V + (int64_t)b * S * z.ldv + kh * W, z.ldv, d_o, l1, l2, d1, d2, lam, dq, i, window, z.scale, lane, 0, W, sum1,
-                 sum2);
+      redo_dq<W>(Q + at * z.ldq + h * W, K + (int64_t)b * S * z.ldk + kh * W, z.ldk, V + (int64_t)b * S * z.ldv + kh * W, z.ldv, dO + at * gr.lddo + h * W, l1, l2, lam, dq, i, window, z.scale,
+                 lane, 0, W, sum1, sum2);
     }
     if (lane < 4) STATS[((int64_t)bh * 4 + lane) * S + i] = lane == 0 ? l1 * LOG2E : lane == 1 ? l2 * LOG2E : lane == 2 ? -sum1 : sum1 - sum2;
     total += sum2;
@@ -1320,7 +1378,7 @@ void bwd(hipStream_t stream, const bf16* q, const bf16* k, const bf16* v, const 
   if (cq.n > 1) {
     dq_of(diff_attn_dq_kernel<W, 4, 1, true>, 4, 1);
     tiles = (z.S + 63) / 64;
-    hipLaunchKernelGGL(diff_attn_dq_join_kernel<W>, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(1024), 0, stream, q, k, v, lam, o, o2, lse, d_o, dq, stats, parts, z, gr, cq, 128);
+    hipLaunchKernelGGL(diff_attn_dq_join_kernel<W>, dim3((unsigned)((int64_t)tiles * z.H * B)), dim3(1024), 0, stream, q, k, v, lam, lse, d_o, dq, stats, parts, z, gr, cq, 128);
   } else if (q_split(B, z)) dq_of(diff_attn_dq_kernel<W, QSW, QG, false>, QSW, QG);
   else dq_of(diff_attn_dq_kernel<W, 4, 1, false>, 4, 1);
   const Lambda la{parts, dlam, B, tiles};

@@ -6,6 +6,7 @@ once (at most 2 u of |s| and |lse|, both within A + ln S), an exponential and it
 2 u of itself and 16 u of a sum of positive numbers in pairs and (a tile of 64 keys at a time) S / 64 u.
 o: a probability is rounded to bf16 in front of its product, h, and the result is, h; products are added in fp32, S u of the sum of the absolute ones: (h + 2 e + S u) (P_1 + |lam| P_2) |v| + h |o|.
 Gradients take o, o2 (rounded to bf16 here) and lse (to fp32): delta_1 is off by d_1 = (h + 2D u) |do| (|o| + 2 |lam| |o2|), delta_2 by d_2 = (h + 2D u) |do| |o2|, dP by 2D u |do||v| and
+(up to 512 tokens it is the kernel's own sum of P dP, off by e + (2D + S) u of P |do||v|), and
 dS = P (dP - delta) by that and by e of itself, lse's rounding u |lse| in e; then h of itself in front of its products.  dlam is summed in fp32 from P_2 and dP: e + 2D u + (S + 1024) u of P_2 |do||v|."""
 import math
 
@@ -69,6 +70,8 @@ class Plain:
             e = e + self.lse_room[..., None]
             rel = H8 + 2 * e + S * U
         off = torch.stack([d1, d2], 2)[..., None]
+        if S <= 512:  # the kernel's own sums of P dP
+            off = (p * big).sum(-1, keepdim=True) * (e + (2 * D + S) * U)
         ds = (p * (dp - delta)).abs()
         ds_room = (H8 + 2 * e) * ds + p * (off + 2 * D * U * big) * (1 + H8)
         both = torch.stack([torch.ones_like(w).expand(H, 1, 1), w], 1)  # [H, 2, 1, 1]
