@@ -7,6 +7,7 @@ operands may be row-strided views (stride(1) must be 1).
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
@@ -395,7 +396,8 @@ def diff_attn_bwd(q, k, v, lam, o, o2, lse, do, *, B: int, S: int, H: int, KH: i
     _place(q, k, v, lam, o, o2, lse, do, dq, dk, dv)
     T, wide, narrow = _diff_sizes(lam, B, S, H, KH, D)
     _want(o2 is not None, "o2 is missing: diff_attn_fwd(want_grad=True) keeps it")
-    _want(lse.dtype == torch.float32 and lse.shape == (B, H, 2, S) and lse.is_contiguous(), f"lse: expected a contiguous fp32 tensor [{B}, {H}, 2, {S}]")
+    if not (lse.dtype is torch.float32 and lse.shape == (B, H, 2, S) and lse.is_contiguous()):
+        raise _lib.OlmaxHipError(f"lse: expected a contiguous fp32 tensor [{B}, {H}, 2, {S}]")
     dq = q.new_empty((T, wide)) if dq is None else dq
     dk = q.new_empty((T, narrow)) if dk is None else dk
     dv = q.new_empty((T, narrow)) if dv is None else dv
@@ -492,8 +494,9 @@ def _size(name: str, *args) -> int:
     return f(*args)
 
 
+@functools.lru_cache(maxsize=1024)
 def _size32(name: str, *args) -> int:
-    """One whose arguments are all 32 bits wide."""
+    """One whose arguments are all 32 bits wide.  Sizes go by the arguments alone, and a step asks for the same ones again."""
     f = _sizes.get(name)
     if f is None:
         f = getattr(_L(), name)
