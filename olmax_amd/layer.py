@@ -45,8 +45,8 @@ class TransformerBlock:
             self.norms["attention.q_norm"] = torch.ones(D if c.qk_norm_headwise else H * D, device=dev, dtype=BF16)
             self.norms["attention.k_norm"] = torch.ones(D if c.qk_norm_headwise else K * D, device=dev, dtype=BF16)
         self.window = c.windows()[layer_idx] if c.num_layers > layer_idx else (-1 if c.window_size is None else c.window_size)
-        theta = c.thetas()[layer_idx] if c.num_layers > layer_idx else c.rope_theta
-        self.cos, self.sin = ops.rope_tables(sequence_length, D, theta, dev)
+        theta, scaling = (c.thetas()[layer_idx], c.scalings()[layer_idx]) if c.num_layers > layer_idx else (c.rope_theta, c.rope_scaling)
+        self.cos, self.sin = c.rope_tables(sequence_length, theta, scaling, dev)
         self.acts = torch.empty(self._L.olmax_block_acts_bytes(ctypes.byref(self.c)), device=dev, dtype=torch.uint8)
         self.tmp: Optional[torch.Tensor] = None
         self._x: Optional[torch.Tensor] = None

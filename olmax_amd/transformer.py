@@ -82,6 +82,8 @@ class TransformerConfig:
     final_logit_softcap: float = 0.0
     tie_embeddings: bool = False
     layer_ac_policy: Optional[str] = None  # "nothing_saveable" = full-block recompute
+    rope_scaling: Optional[ops.RopeScaling] = None  # slower angles for contexts longer than the model was trained on
+    rope_scaling_per_layer: Optional[Sequence[Optional[ops.RopeScaling]]] = None
 
     def __post_init__(self):
         if self.n_kv_heads is None:
@@ -114,6 +116,18 @@ class TransformerConfig:
             assert len(self.rope_theta_per_layer) == self.num_layers
             return [float(t) for t in self.rope_theta_per_layer]
         return [float(self.rope_theta)] * self.num_layers
+
+    def scalings(self) -> List[Optional[ops.RopeScaling]]:
+        if self.rope_scaling_per_layer is not None:
+            assert len(self.rope_scaling_per_layer) == self.num_layers
+            return list(self.rope_scaling_per_layer)
+        return [self.rope_scaling] * self.num_layers
+
+    def rope_tables(self, seq_len: int, theta: float, scaling: Optional[ops.RopeScaling], device):
+        """cos/sin [seq_len, head_dim / 2] of a layer."""
+        if scaling is None:
+            return ops.rope_tables(seq_len, self.head_dim, theta, device)
+        return ops.rotary_tables(seq_len, self.head_dim, theta, device, scaling=scaling)
 
     def c_config(self, batch: int, seq_len: int) -> CModelConfig:
         return CModelConfig(
@@ -281,13 +295,15 @@ class Transformer:
 
         # per-layer windows and RoPE tables (get_buffer_cache, model.py:138-144)
         self._windows = (ctypes.c_int32 * max(1, config.num_layers))(*config.windows())
-        tables: Dict[float, tuple] = {}
-        for th in config.thetas():
-            if th not in tables:
-                tables[th] = ops.rope_tables(sequence_length, config.head_dim, th, dev)
+        tables: Dict[object, tuple] = {}  # by theta, or (theta, scaling)
+        layers = []
+        for th, scaling in zip(config.thetas(), config.scalings()):
+            layers.append(th if scaling is None else (th, scaling))
+            if layers[-1] not in tables:
+                tables[layers[-1]] = config.rope_tables(sequence_length, th, scaling, dev)
         self.buffer_cache = tables
-        self._cos = (ctypes.c_void_p * max(1, config.num_layers))(*[tables[t][0].data_ptr() for t in config.thetas()])
-        self._sin = (ctypes.c_void_p * max(1, config.num_layers))(*[tables[t][1].data_ptr() for t in config.thetas()])
+        self._cos = (ctypes.c_void_p * max(1, config.num_layers))(*[tables[key][0].data_ptr() for key in layers])
+        self._sin = (ctypes.c_void_p * max(1, config.num_layers))(*[tables[key][1].data_ptr() for key in layers])
         self.reset_parameters(seed, init_std)
 
     # ------------------------------------------------------------------ parameters

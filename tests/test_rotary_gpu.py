@@ -207,3 +207,40 @@ def test_agrees_with_the_half_rotation_of_whole_heads():
     a, b = ops().qk_rope_fwd(x, cos, sin, heads=heads, head_dim=D, seq_len=65), ops().rotary_fwd(x, cos, sin, heads=heads, head_dim=D)
     room = torch.maximum(a.double().abs(), b.double().abs()) * torch.finfo(BF).eps + 16 * 6 * U
     assert ((a.double() - b.double()).abs() <= room).all()
+
+
+def _scaled(scaling):
+    """The oracle's table function with a layer's scaling; `scaling` by theta."""
+    def tables(S, D, theta, dtype=torch.float32):
+        c = scaling[theta]
+        kw = {} if c is None else dict(kind=c.kind, factor=c.factor, original_length=c.original_length, low_turns=c.low_turns, high_turns=c.c_args()[4])
+        angle = torch.arange(S, dtype=torch.float64)[:, None] * ref.rotary_freqs(D, theta, **kw)
+        size = 1.0 if c is None else c.c_args()[5]
+        return (size * angle.cos()).to(dtype), (size * angle.sin()).to(dtype)
+    return tables
+
+
+@pytest.mark.parametrize("kind,scalings", [("default", ("yarn", "yarn")), ("reordered_norm", ("yarn", None)), ("reordered_norm", ("llama3", "linear"))])
+def test_a_model_with_scaled_positions(monkeypatch, kind, scalings):
+    """A model's loss and gradients with tables for longer contexts against the oracle's, with the bounds that its unscaled tables have."""
+    from olmax_amd import TransformerConfig
+    sets = {"yarn": ops().RopeScaling("yarn", 4.0, original_length=32), "llama3": ops().RopeScaling("llama3", 8.0, original_length=64), "linear": ops().RopeScaling("linear", 2.0), None: None}
+    per_layer, thetas = [sets[s] for s in scalings], [1e4, 5e5]
+    qk = kind != "default"
+    sizes = dict(n_heads=2, n_kv_heads=2, head_dim=64)
+    ocfg = ref.ModelConfig(vocab=512, d_model=256, n_layers=2, hidden=512, layer_type="reordered" if qk else "pre", act="silu", qk_norm=qk, qk_norm_headwise=True, eps=1e-6, rope_theta_layers=thetas, **sizes)
+    more = dict(rope_scaling=per_layer[0]) if scalings[0] == scalings[1] else dict(rope_scaling_per_layer=per_layer)
+    hcfg = TransformerConfig(vocab_size=512, d_model=256, hidden_size=512, num_layers=2, layer_type=kind, qk_norm_headwise=qk, norm_eps=1e-6, rope_theta_per_layer=thetas, **sizes, **more)
+    P = {k: (v + 0.1 * torch.randn(v.shape, generator=torch.Generator().manual_seed(3)) if "norm" in k else 2 * v).to(torch.bfloat16).double() for k, v in ref.init_params(ocfg, seed=1).items()}
+    gen = torch.Generator().manual_seed(5)
+    ids, labels = (torch.randint(0, 512, (2, 128), generator=gen, dtype=torch.int32) for _ in range(2))
+    model = hcfg.build(batch_size=2, sequence_length=128)
+    model.load_state_dict({k: v.float() for k, v in P.items()})
+    loss = model.loss_and_grads(ids.cuda().reshape(-1), labels.cuda().reshape(-1)).item()
+    monkeypatch.setattr(ref, "rope_tables", _scaled(dict(zip(thetas, per_layer))))
+    rt = lambda t: t.to(torch.bfloat16).to(t.dtype)  # noqa: E731
+    want, grads = ref.model_loss_and_grads(ocfg, P, ids, labels.long(), rt)
+    assert abs(loss - want.item()) < 1e-2 * abs(want.item())
+    for name, g in model.named_gradients().items():
+        a, b = g.double().cpu().flatten(), grads[name].double().flatten()
+        assert a @ b / (a.norm() * b.norm() + 1e-30) >= 0.999, name
