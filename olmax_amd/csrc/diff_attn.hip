@@ -199,6 +199,14 @@ __device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16*
   }
 }
 
+// Fragments that have been loaded, and that the compiler knows to have been: it counts no transfer of inline assembly, and where it finds a load of its own unfinished on some way into a loop it waits
+// there, in every round, for as many as were behind that load, which are the tiles under way.  (Gradients of 1 x 4096 tokens, 32/8 heads of 32: 422 us, 407 with this; heads of 64, whose rounds are longer, the same.)
+template <int N>
+__device__ __forceinline__ void arrived(bf16x8 (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+v"(f[i]));
+}
+
 // The lane, formed where it is needed rather than kept in a register
 __device__ __forceinline__ int lane_id() {
   int l;
@@ -337,6 +345,7 @@ __global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* 
   load(t_lo, 0);
   load(t_lo + 1, 1);
   if (m == 0) load(t_lo + 2, 2);
+  arrived(qf);
   part_ends<0>();
   if (visible(t_lo)) scores(0);
   if (m == 1) part_ends<0>();
@@ -605,6 +614,8 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
       }
     }
   }
+  arrived(qf);
+  arrived(dof);
   d2 = half_swap_sum(d2);
   d1 = __builtin_fmaf(lam, d2, half_swap_sum(d1));  // o + lambda O_2 = O_1
   const int64_t row0 = ((int64_t)b * H + h) * 2 * S;
@@ -1029,6 +1040,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   const unsigned char* fixed = smem + QS * 2 * STAGE + kw * (FIXED * 1024) + lane * 16;
   auto v_step = [&](int s) { return *reinterpret_cast<const bf16x8*>(fixed + s * 1024); };
   auto k_step = [&](int s) { return s < HELD ? kf[s < HELD ? s : 0] : v_step(2 * KS + s - HELD); };
+  arrived(kf);
   load_tile(0, 0);
   dma_wait_all();
   __syncthreads();
