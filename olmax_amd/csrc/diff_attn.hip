@@ -990,48 +990,60 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   TileDma<QT, W> tq, tdo;
   tq.init(z.ldq, wv, lane);
   tdo.init(gr.lddo, wv, lane);
-  // (tile, head) pairs, the last tile first and its heads next to each other: the workgroups of a K/V head, which begin at different tiles, read the same ones at the same time, out of one L2
-  struct Iter { int h, t; };
-  auto advance = [&](Iter& x, int n) {
-    x.h += n;
-    while (x.h >= rep) {
+  // (tile, head) pairs, the last tile first and its heads next to each other: the workgroups of a K/V head, which begin at different tiles, read the same ones at the same time, out of one L2.
+  // A group takes every QS-th pair; addresses move by a step, or by another one where the heads of a tile are done.
+  struct Pair { int h, t; };
+  const int dh = QS % rep, dt = QS / rep, n0 = PART ? place.part * ch.size : 0;
+  auto first = [&](int n) { return Pair{(n0 + n) % rep, t_hi - (n0 + n) / rep}; };
+  auto advance = [&](Pair& x) {
+    x.h += dh;
+    x.t -= dt;
+    const bool next = x.h >= rep;
+    if (next) {
       x.h -= rep;
       --x.t;
     }
+    return next;
   };
-  auto first = [&](int n) {
-    Iter x = PART ? Iter{part * ch.size % rep, t_hi - part * ch.size / rep} : Iter{0, t_hi};
-    advance(x, n);
-    return x;
-  };
+  const int64_t q_step = dh * W - dt * QT * z.ldq, q_next = q_step - rep * W - QT * z.ldq, do_step = dh * W - dt * QT * gr.lddo, do_next = do_step - rep * W - QT * gr.lddo;
+  const int64_t st_step = (int64_t)dh * 4 * S - dt * QT, st_next = st_step - (int64_t)rep * 4 * S - QT;
   // the next one to load of each query group this team fetches for, and of this wave's own group (its rows' statistics)
-  Iter own = first(qs), ld[QS / TEAMS];
+  Pair own = first(qs), ld[QS / TEAMS];
+  const bf16 *q_at[QS / TEAMS], *do_at[QS / TEAMS];
+  const float* st_at = STATS + ((int64_t)b * H + kh * rep + own.h) * 4 * S + own.t * QT;
 #pragma unroll
-  for (int g = 0; g < QS / TEAMS; g++) ld[g] = first(g * TEAMS + team);
+  for (int g = 0; g < QS / TEAMS; g++) {
+    ld[g] = first(g * TEAMS + team);
+    const int64_t row = (int64_t)b * S + ld[g].t * QT, column = (kh * rep + ld[g].h) * W;
+    q_at[g] = Q + row * z.ldq + column;
+    do_at[g] = dO + row * gr.lddo + column;
+  }
   auto load_tile = [&](int round, int stage) {
 #pragma unroll
     for (int g = 0; g < QS / TEAMS; g++) {
       const int grp = g * TEAMS + team;
       if (QS > 1 && round * QS + grp >= total) break;
-      const int hq = kh * rep + ld[g].h, t = ld[g].t;
-      advance(ld[g], QS);
+      const int t = ld[g].t;
       const unsigned dst = lds0 + (grp * 2 + stage) * STAGE;
-      const bf16 *qp = Q + (int64_t)b * S * z.ldq + hq * W, *dp = dO + (int64_t)b * S * gr.lddo + hq * W;
       if (t * QT + QT <= S) {
-        tq.issue(qp + (int64_t)t * QT * z.ldq, dst, wv);
-        tdo.issue(dp + (int64_t)t * QT * gr.lddo, dst + TILE, wv);
+        tq.issue(q_at[g], dst, wv);
+        tdo.issue(do_at[g], dst + TILE, wv);
       } else {
         const int l = lane_id();
-        dma_tile<QT, W>(qp, z.ldq, t * QT, S, dst, wv, l);
-        dma_tile<QT, W>(dp, gr.lddo, t * QT, S, dst + TILE, wv, l);
+        dma_tile<QT, W>(q_at[g] - t * QT * z.ldq, z.ldq, t * QT, S, dst, wv, l);
+        dma_tile<QT, W>(do_at[g] - t * QT * gr.lddo, gr.lddo, t * QT, S, dst + TILE, wv, l);
       }
+      const bool next = advance(ld[g]);
+      q_at[g] += next ? q_next : q_step;
+      do_at[g] += next ? do_next : do_step;
     }
     if (kw == 0 && (QS == 1 || round * QS + qs < total)) {  // the rows' statistics: lanes 0 .. 31 the first of two, 32 .. 63 the second
       const int l = lane_id();
-      const float* st = STATS + (((int64_t)b * H + kh * rep + own.h) * 4 + (l >> 5)) * S + min(own.t * QT + (l & 31), S - 1);
+      const float* st = st_at + (int64_t)(l >> 5) * S + min(l & 31, S - 1 - own.t * QT);
       const unsigned dst = lds0 + (qs * 2 + stage) * STAGE + 2 * TILE;
       dma4(st, dst);
       dma4(st + 2 * (int64_t)S, dst + 256);
+      st_at += advance(own) ? st_next : st_step;
     }
   };
 
@@ -1045,14 +1057,11 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   dma_wait_all();
   __syncthreads();
   const int rounds = (total + QS - 1) / QS;
-  Iter cur_it = first(qs);  // being consumed
+  Pair cur_it = first(qs);  // being consumed
   for (int round = 0; round < rounds; round++) {
     const int cur = round & 1;
     const bool more = round + 1 < rounds;
-    if (more) {
-      advance(own, QS);
-      load_tile(round + 1, cur ^ 1);
-    }
+    if (more) load_tile(round + 1, cur ^ 1);
     const int ib = cur_it.t * QT;  // first query of the tile
     const bool visible = (QS == 1 || round * QS + qs < total) && (ib + QT - 1 >= jw0) && (window < 0 || ib <= jw0 + 31 + window);
     if (visible) {
@@ -1136,7 +1145,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
         pin();
       }
     }
-    advance(cur_it, QS);
+    advance(cur_it);
     dma_wait_all();
     __syncthreads();
   }
