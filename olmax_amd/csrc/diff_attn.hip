@@ -249,6 +249,10 @@ __device__ __forceinline__ void hide(f32x16& s1, f32x16& s2, int lane, int colum
 // (vector unit) and the products (matrix unit: this tile's probabilities with V, the next tile's scores), a barrier ends each, and map 1 is one part behind map 0.
 // LDS: 3 stages of K, then of V.  Map 0's waves fetch K, map 1's V.  K(t) is read in parts 2t - 1 and 2t, V(t) in 2t + 1 and 2t + 2 (counted as map 0 does), so that K(t + 3) is issued in 2t + 1 and
 // V(t + 2) too, and each has four parts to land; past the end the last tile is fetched again.
+// 2 x 4096 tokens, 32 heads of 64: 470 us, 412 GFLOP of products at 880 TFLOP/s, 1.9 GHz; a map's 32 x 64 tile takes a SIMD 1560 clk, 768 of them matrix instructions.  Bound by what a wave can
+// issue, and by the power: without the products 380 us, without the exponentials' part 510 (its own latencies then stand alone), without the LDS reads 7 % less, without the transfers 2 %.
+// No gain: one barrier a tile with the maps half a tile apart (496), 64 queries to a wave on tiles of 32 keys (538; it spills 12 registers), scores ahead of the values' products with the maximum in
+// their shadow (500), addresses moved by steps (472; heads of 32: 3 % less, heads of 64 1 % more).
 // ---------------------------------------------------------------------------------------
 template <int N>
 __device__ __forceinline__ void part_ends() {  // at most the newest N transfers of this wave are under way; its LDS reads are done
@@ -544,6 +548,7 @@ __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __r
 // dQ, dlambda and delta.  grid = ceil(S / 32 QW) H B workgroups of QW x KG waves; wave (qw, kg) owns 32 queries and every KG-th of their key tiles.  KG = 1 (QW = 4): two workgroups per CU, no merge.
 // KG > 1: one workgroup of eight waves with 1 / KG of the chain of tiles; what they have is added through LDS, in key-group order.  See q_split.
 // The sums of P_m dP come out of the same sweep in fp32: dK/dV takes its delta from them, and dlambda is their sum: terms of both signs, that an error of 2^-9 in each would leave three digits of.
+// dQ: 1 x 4096 tokens, 32/8 heads of 64: 265 us, 206 GFLOP at 780 TFLOP/s, bound by issue as the forward.
 // For dQ they come too late, and it takes delta from the outputs as they were rounded, as dQ of attn.hip does; but where a workgroup has SWEEP key tiles or fewer, a sweep ahead forms them first.
 // A row that sees few keys has most to lose: its dP - delta is small beside delta, and its gradients are the largest.  dQ's error as a share of its norm, and us of a backward pass, without the sweep,
 // with, and with it everywhere (rounding dS and the result alone makes 0.0023): 5 tokens 0.0069, 0.0022; 3 x 333, 4/2 heads of 32 0.0031, 0.0025; 25.8, 30.5 us; 1 x 1000, 8/4, window 333
@@ -899,6 +904,7 @@ __global__ __launch_bounds__(1024) void diff_attn_dq_join_kernel(const bf16* __r
 // ---------------------------------------------------------------------------------------
 // dK/dV.  grid = ceil(S / 32 KW) KH B workgroups of KW x QS waves; wave (kw, qs) owns 32 keys and every QS-th of the pairs of a query head of the group and one of its 32-row
 // tiles from the diagonal on.  LDS: per query group 2 stages of (Q | dO | the 32 rows' statistics), then the fragments of V and K.
+// 1 x 4096 tokens, 32/8 heads of 64 (2 x 4): 345 us, 275 GFLOP at 800 TFLOP/s, bound by issue: 272 vector and matrix instructions to 32 products.
 // KW = 4, QS = 1: two workgroups per CU, no reduction.  KW = 2, QS = 4: one workgroup of eight waves per CU, half the keys and a quarter of the chain; the four partial sums are added through LDS
 // in group order.  See dkv_split.
 // ---------------------------------------------------------------------------------------

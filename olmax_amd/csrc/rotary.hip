@@ -86,7 +86,8 @@ __device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
 }
 
 // Vectors of 16 bytes.  A unit is a place in a head: a vector pair (half layout) or a vector (interleaved) that turns, or a vector that passes.  A thread keeps a unit's cosines and sines in
-// registers and takes the unit of `each` heads, `slots` apart, UNROLL at a time, so that the tables are read once per `each` heads and that many loads are in flight.
+// registers and takes every slots-th head, UNROLL at a time, so that the tables are read once for them and that many loads are in flight.
+// Bound by HBM: 8192 tokens, 64 heads of 128 in bf16 (268 MB) 46 us, 5.8 TB/s; 1 token 2.3 us.
 template <typename T, bool HALF>
 __global__ __launch_bounds__(256) void rotary_kernel(const T* x, T* y, const Turn a, int turning, int units, int slots, int per, int copies) {
   constexpr int N = rows::Vec<T>::N, UNROLL = 4, PAIRS = HALF ? N : N / 2;
