@@ -551,7 +551,7 @@ __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __r
 // dQ: 1 x 4096 tokens, 32/8 heads of 64: 265 us, 206 GFLOP at 780 TFLOP/s, bound by issue as the forward.
 // For dQ they come too late, and it takes delta from the outputs as they were rounded, as dQ of attn.hip does; but where a workgroup has SWEEP key tiles or fewer, a sweep ahead forms them first.
 // A row that sees few keys has most to lose: its dP - delta is small beside delta, and its gradients are the largest.  dQ's error as a share of its norm, and us of a backward pass, without the sweep,
-// with, and with it everywhere (rounding dS and the result alone makes 0.0023): 5 tokens 0.0069, 0.0022; 3 x 333, 4/2 heads of 32 0.0031, 0.0025; 25.8, 30.5 us; 1 x 1000, 8/4, window 333
+// with, and with it everywhere (rounding dS and the result alone makes 0.0023): 5 tokens 0.0069, 0.0022; 3 x 333, 4/2 heads of 32 0.0031, 0.0025; 25.8, 29.4 us (30.9 where the tiles are fetched again); 1 x 1000, 8/4, window 333
 // 0.0029, 0.0024; 46, 56 us; 1 x 4096, 32/8 0.0027, 0.0026, 0.0024; 609, 613, 777 us.
 // STATS [B, H, 4, S]: what dK/dV takes of a row: lse_1 and lse_2 in powers of two, -delta_1, and delta_1 - delta_2 (dP - delta_2 is what it has of the first map, plus this).  DLAM: a number for
 // each workgroup, [B, H, tiles].
@@ -599,6 +599,32 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
     t_hi = min(t_hi, t_lo + ch.size - 1);
   }
 
+  const bf16* kbase = K + (int64_t)b * S * z.ldk + kh * W;
+  const bf16* vbase = V + (int64_t)b * S * z.ldv + kh * W;
+  const unsigned lds0 = lds_addr_of(smem);
+  TileDma<64, W> dk, dv;
+  dk.init(z.ldk, wv, lane);
+  dv.init(z.ldv, wv, lane);
+  // K/V tiles of round r: tile t_lo + r KG + g for key group g
+  auto load_kv = [&](int t_lo, int t_hi, int round, int stage) {
+#pragma unroll
+    for (int g0 = 0; g0 < KG / TEAMS; g0++) {
+      const int g = g0 * TEAMS + team, t = t_lo + round * KG + g;
+      if (KG > 1 && t > t_hi) break;
+      const unsigned dst = lds0 + (g * 2 + stage) * (2 * TILE);
+      if (t * 64 + 64 <= S) {
+        dk.issue(kbase + (int64_t)t * 64 * z.ldk, dst, wv);
+        dv.issue(vbase + (int64_t)t * 64 * z.ldv, dst + TILE, wv);
+      } else {
+        dma_tile<64, W>(kbase, z.ldk, t * 64, S, dst, wv, lane);
+        dma_tile<64, W>(vbase, z.ldv, t * 64, S, dst + TILE, wv, lane);
+      }
+    }
+  };
+  const bool sweeps = all_hi - all_lo < SWEEP;
+  const int first_lo = sweeps ? all_lo : t_lo, first_hi = sweeps ? all_hi : t_hi;
+  load_kv(first_lo, first_hi, 0, 0);
+
   bf16x8 qf[W / 16], dof[W / 16];
   float d1 = 0.f, d2 = 0.f;
   {
@@ -625,28 +651,6 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   d1 = __builtin_fmaf(lam, d2, half_swap_sum(d1));  // o + lambda O_2 = O_1
   const int64_t row0 = ((int64_t)b * H + h) * 2 * S;
   const float l1 = LSE[row0 + qic] * LOG2E, l2 = LSE[row0 + S + qic] * LOG2E;
-  const bf16* kbase = K + (int64_t)b * S * z.ldk + kh * W;
-  const bf16* vbase = V + (int64_t)b * S * z.ldv + kh * W;
-  const unsigned lds0 = lds_addr_of(smem);
-  TileDma<64, W> dk, dv;
-  dk.init(z.ldk, wv, lane);
-  dv.init(z.ldv, wv, lane);
-  // K/V tiles of round r: tile t_lo + r KG + g for key group g
-  auto load_kv = [&](int t_lo, int t_hi, int round, int stage) {
-#pragma unroll
-    for (int g0 = 0; g0 < KG / TEAMS; g0++) {
-      const int g = g0 * TEAMS + team, t = t_lo + round * KG + g;
-      if (KG > 1 && t > t_hi) break;
-      const unsigned dst = lds0 + (g * 2 + stage) * (2 * TILE);
-      if (t * 64 + 64 <= S) {
-        dk.issue(kbase + (int64_t)t * 64 * z.ldk, dst, wv);
-        dv.issue(vbase + (int64_t)t * 64 * z.ldv, dst + TILE, wv);
-      } else {
-        dma_tile<64, W>(kbase, z.ldk, t * 64, S, dst, wv, lane);
-        dma_tile<64, W>(vbase, z.ldv, t * 64, S, dst + TILE, wv, lane);
-      }
-    }
-  };
   const float sc2 = z.scale * LOG2E;
   FragAddr<W, W == 128> fa;  // (short of registers)
   fa.init(lane);
@@ -669,11 +673,12 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
       }
     }
   };
-  if (all_hi - all_lo < SWEEP) {  // delta by a sweep ahead
+  dma_wait_all();
+  __syncthreads();
+  const int rounds = (t_hi - t_lo + KG) / KG;
+  bool there = false;  // whether both stages have what the chain takes
+  if (sweeps) {        // delta by a sweep ahead
     const int rounds = (all_hi - all_lo + KG) / KG;
-    load_kv(all_lo, all_hi, 0, 0);
-    dma_wait_all();
-    __syncthreads();
     for (int round = 0; round < rounds; round++) {
       const int cur = round & 1;
       if (round + 1 < rounds) load_kv(all_lo, all_hi, round + 1, cur ^ 1);
@@ -712,6 +717,12 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
     add_groups();
     d1 = sum1;
     d2 = sum2;
+    there = !PART && rounds <= 2;
+    if (!there) {
+      load_kv(t_lo, t_hi, 0, 0);
+      dma_wait_all();
+      __syncthreads();
+    }
   }
 
   f32x16 dq[W / 32];
@@ -722,13 +733,9 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
   sum1 = sum2 = 0.f;
 
 
-  load_kv(t_lo, t_hi, 0, 0);
-  dma_wait_all();
-  __syncthreads();
-  const int rounds = (t_hi - t_lo + KG) / KG;
   for (int round = 0; round < rounds; round++) {
     const int cur = round & 1;
-    if (round + 1 < rounds) load_kv(t_lo, t_hi, round + 1, cur ^ 1);
+    if (round + 1 < rounds && !there) load_kv(t_lo, t_hi, round + 1, cur ^ 1);
     const int t = t_lo + round * KG + kg, j0 = t * 64;
     const bool visible = (KG == 1 || t <= t_hi) && j0 <= iw0 + 31 && (window < 0 || j0 + 63 >= iw0 - window);
     if (visible) {
@@ -1058,8 +1065,8 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   const unsigned char* fixed = smem + QS * 2 * STAGE + kw * (FIXED * 1024) + lane * 16;
   auto v_step = [&](int s) { return *reinterpret_cast<const bf16x8*>(fixed + s * 1024); };
   auto k_step = [&](int s) { return s < HELD ? kf[s < HELD ? s : 0] : v_step(2 * KS + s - HELD); };
-  arrived(kf);
   load_tile(0, 0);
+  arrived(kf);
   dma_wait_all();
   __syncthreads();
   const int rounds = (total + QS - 1) / QS;
