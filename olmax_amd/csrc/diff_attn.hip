@@ -177,7 +177,7 @@ __device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16*
         pair_of<W>(Q + i * ldq, k, dO + i * lddo, v, st[0] * LN2, st[S] * LN2, scale, p1, p2, dp);
         dp += st[2 * (int64_t)S];
         s1 = p1 * dp;
-        s2 = -*lam * p2 * (dp + st[3 * (int64_t)S]);
+        s2 = p2 * (st[3 * (int64_t)S] - *lam * dp);
         p = p1 - *lam * p2;
       }
 #pragma unroll 1
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __r
 // A row that sees few keys has most to lose: its dP - delta is small beside delta, and its gradients are the largest.  dQ's error as a share of its norm, and us of a backward pass, without the sweep,
 // with, and with it everywhere (rounding dS and the result alone makes 0.0023): 5 tokens 0.0069, 0.0022; 3 x 333, 4/2 heads of 32 0.0031, 0.0025; 25.8, 29.4 us (30.9 where the tiles are fetched again); 1 x 1000, 8/4, window 333
 // 0.0029, 0.0024; 46, 56 us; 1 x 4096, 32/8 0.0027, 0.0026, 0.0024; 609, 613, 777 us.
-// STATS [B, H, 4, S]: what dK/dV takes of a row: lse_1 and lse_2 in powers of two, -delta_1, and delta_1 - delta_2 (dP - delta_2 is what it has of the first map, plus this).  DLAM: a number for
+// STATS [B, H, 4, S]: what dK/dV takes of a row: lse_1 and lse_2 in powers of two, -delta_1, and -lambda (delta_1 - delta_2) (-lambda (dP - delta_2) is -lambda times what it has of the first map, plus this).  DLAM: a number for
 // each workgroup, [B, H, tiles].
 // ---------------------------------------------------------------------------------------
 struct Grad {
@@ -853,7 +853,7 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
     st[0] = l1;
     st[S] = l2;
     st[2 * (int64_t)S] = -sum1;
-    st[3 * (int64_t)S] = sum1 - sum2;
+    st[3 * (int64_t)S] = lam * (sum2 - sum1);
   }
   const float dl = block_sum<QW * KG>(counts ? sum2 : 0.f, red);
   if (tid == 0) DLAM[((int64_t)b * H + h) * nqt + qt] = -dl;
@@ -900,7 +900,7 @@ __global__ __launch_bounds__(1024) void diff_attn_dq_join_kernel(const bf16* __r
       redo_dq<W>(Q + at * z.ldq + h * W, K + (int64_t)b * S * z.ldk + kh * W, z.ldk, V + (int64_t)b * S * z.ldv + kh * W, z.ldv, dO + at * gr.lddo + h * W, l1, l2, lam, dq, i, window, z.scale,
                  lane, 0, W, sum1, sum2);
     }
-    if (lane < 4) STATS[((int64_t)bh * 4 + lane) * S + i] = lane == 0 ? l1 * LOG2E : lane == 1 ? l2 * LOG2E : lane == 2 ? -sum1 : sum1 - sum2;
+    if (lane < 4) STATS[((int64_t)bh * 4 + lane) * S + i] = lane == 0 ? l1 * LOG2E : lane == 1 ? l2 * LOG2E : lane == 2 ? -sum1 : lam * (sum2 - sum1);
     total += sum2;
   }
   const float dl = block_sum<16>(lane == 0 ? total : 0.f, red);
@@ -1133,8 +1133,8 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
 #pragma unroll
         for (int r = s * EL; r < (s + 1) * EL; r++) {
           s1[r] = fexp2(__builtin_fmaf(s1[r], sc2, -of4(0, r)));
-          s2[r] = nlam * fexp2(__builtin_fmaf(s2[r], sc2, -of4(1, r)));
-          w[r >> 3][r & 7] = f2bf(s1[r] + s2[r]);
+          s2[r] = fexp2(__builtin_fmaf(s2[r], sc2, -of4(1, r)));
+          w[r >> 3][r & 7] = f2bf(__builtin_fmaf(nlam, s2[r], s1[r]));
         }
         pin();
       }
@@ -1145,7 +1145,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
 #pragma unroll
         for (int r = i * EL; r < (i + 1) * EL; r++) {
           ds1[r >> 3][r & 7] = f2bf(s1[r] * dp[r]);
-          ds2[r >> 3][r & 7] = f2bf(s2[r] * (dp[r] + of4(3, r)));
+          ds2[r >> 3][r & 7] = f2bf(s2[r] * __builtin_fmaf(nlam, dp[r], of4(3, r)));
         }
         if (i >= STEPS - AK) fd[i - (STEPS - AK)] = tr_step(sq, i - (STEPS - AK));
         pin();
