@@ -1087,6 +1087,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
       // some products ahead; the order is pinned, since the compiler's own reads so far ahead that it spills, and a reload waits for the tiles under way.
       constexpr int STEPS = 2 * KS, EL = 16 / STEPS;  // products of a run, rows of the vector work beside each
       constexpr int AP = 1, AV = 1, AK = 2;  // products that fragments are read ahead by, of dP, dV and dK
+      static_assert(AV <= AP && AK < STEPS, "the first fragments of a run are read beside the last products of the one before");
       f32x16 s1, s2, dp;  // rows are queries ib + 8 (r / 4) + 4 lhi + r % 4; column: key kj
       bf16x8 w[2], ds1[2], ds2[2];
       auto pin = [] { __builtin_amdgcn_sched_barrier(0); };

@@ -193,6 +193,12 @@ def test_nor_where_chains_are_split(D, window, S, at, value):
     unseen(dict(B=1, S=S, H=2, KH=1, D=D), window, at, value)
 
 
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+@pytest.mark.parametrize("B,S,H,KH,D,window,at", [(41, 130, 16, 8, 64, None, 70), (41, 130, 16, 8, 32, 60, 3), (3, 300, 20, 20, 32, None, 128), (3, 300, 40, 20, 64, 33, 255)])
+def test_nor_where_the_gpu_is_full(B, S, H, KH, D, window, at, value):
+    unseen(dict(B=B, S=S, H=H, KH=KH, D=D), window, at, value)
+
+
 def unseen(sizes, window, at, value):
     B, S, W = sizes["B"], sizes["S"], 2 * sizes["D"]
     T, last = B * S, min(S, at + window + 1) if window else S
