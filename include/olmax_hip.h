@@ -201,7 +201,8 @@ int32_t olmax_attn_bwd_noalloc(olmax_stream_t stream, const void* q, const void*
  * Long sequences of few heads take a workspace (16-byte aligned); where the query returns 0 none is read. */
 int64_t olmax_diff_attn_fwd_workspace_bytes(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window);
 int32_t olmax_diff_attn_fwd(olmax_stream_t stream, const void* q, const void* k, const void* v, const float* lam, void* o, void* o2, float* lse,
-                            void* workspace, int64_t workspace_bytes, int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t ldo2, int32_t lam_shared, int32_t window);
+                            void* workspace, int64_t workspace_bytes, int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv,
+                            int64_t ldo, int64_t ldo2, int32_t lam_shared, int32_t window);
 /* From o, o2 and lse of the forward call and d_o = d loss / d o: dq, dk, dv, and dlam ([H], or one number with lam_shared, fp32).  Deterministic. */
 int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window);
 int32_t olmax_diff_attn_bwd(olmax_stream_t stream, const void* q, const void* k, const void* v, const float* lam, const void* o, const void* o2, const float* lse,
