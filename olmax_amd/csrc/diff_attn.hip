@@ -548,7 +548,7 @@ __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __r
 // dQ, dlambda and delta.  grid = ceil(S / 32 QW) H B workgroups of QW x KG waves; wave (qw, kg) owns 32 queries and every KG-th of their key tiles.  KG = 1 (QW = 4): two workgroups per CU, no merge.
 // KG > 1: one workgroup of eight waves with 1 / KG of the chain of tiles; what they have is added through LDS, in key-group order.  See q_split.
 // The sums of P_m dP come out of the same sweep in fp32: dK/dV takes its delta from them, and dlambda is their sum: terms of both signs, that an error of 2^-9 in each would leave three digits of.
-// dQ: 1 x 4096 tokens, 32/8 heads of 64: 265 us, 206 GFLOP at 780 TFLOP/s, bound by issue as the forward.
+// dQ: 1 x 4096 tokens, 32/8 heads of 64: 255 us, 206 GFLOP at 810 TFLOP/s, bound by issue as the forward; fragments one product ahead 10 us more, four spill.
 // For dQ they come too late, and it takes delta from the outputs as they were rounded, as dQ of attn.hip does; but where a workgroup has SWEEP key tiles or fewer, a sweep ahead forms them first.
 // A row that sees few keys has most to lose: its dP - delta is small beside delta, and its gradients are the largest.  dQ's error as a share of its norm, and us of a backward pass, without the sweep,
 // with, and with it everywhere (rounding dS and the result alone makes 0.0023): 5 tokens 0.0069, 0.0022; 3 x 333, 4/2 heads of 32 0.0031, 0.0025; 25.8, 29.4 us (30.9 where the tiles are fetched again); 1 x 1000, 8/4, window 333
@@ -743,8 +743,8 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
       const unsigned char* sv = sk + TILE;
       const bool need_mask = (j0 + 63 > iw0) || (window >= 0 && j0 < iw0 + 31 - window);
       // 48 products (W = 128) in six runs: scores and dP of either half of the tile's keys, then dQ of either.  The exponentials go between the products of dP, what is left of dS between those of
-      // the next half's scores, or of dQ; each product's fragment is read one ahead, in a pinned order, as in dK/dV.
-      constexpr int STEPS = 2 * KS, EL = 16 / STEPS, AHEAD = 1;
+      // the next half's scores, or of dQ; each product's fragment is read two ahead, in a pinned order, as in dK/dV.
+      constexpr int STEPS = 2 * KS, EL = 16 / STEPS, AHEAD = 2;
       f32x16 s1[2], s2[2], dp[2];
       bf16x8 ds1[2][2], ds2[2][2], fr[AHEAD + 1];
       auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
