@@ -1282,7 +1282,7 @@ int check_shape(const char* name, int32_t B, int32_t S, int32_t H, int32_t KH, i
 }
 
 // Forms of dQ and dK/dV.  us of a backward pass that takes one and the other of the two forms, bf16, causal, B x S, H/KH heads:
-// dQ split over key groups (QSK of them) where the workgroups of 128 queries would not fill 256 CUs: it halves the queries of a workgroup and its chain of key tiles, and its merge and one more
+// dQ split over key groups (two of them, four for D = 32) where the workgroups of 128 queries would not fill 256 CUs: it halves the queries of a workgroup and its chain of key tiles, and its merge and one more
 // barrier per tile are then free.  D = 64: 117 split, 133 whole (1 x 1000, 16/4); 122, 142 (1 x 2048, 16/16, 256 workgroups); with 512 of them 218, 196 (1 x 2048, 32/16).
 // D = 32: 105, 121; 172, 158; 30.5, 33 (3 x 333, 4/2).
 constexpr int QSW = 2;
@@ -1299,7 +1299,7 @@ bool dkv_split(int B, const Sizes& z) { return (int64_t)((z.S + 127) / 128) * z.
 bool dkv_narrow(int B, const Sizes& z) { return (int64_t)((z.S + 63) / 64) * z.KH * B * (z.window < 0 ? 1 : 2) <= 256; }
 
 // Form of the forward pass: workgroups of 64 queries (a wave to a SIMD; the turns are then between SIMDs and cost nothing) where those of 128 would leave half of the GPU empty, and for D = 32 always:
-// LDS and registers hold three such workgroups on a CU, and one of the others.  us, 64 and 128 queries, B x S, H/KH heads: D = 64: 17.8, 21.0 (1 x 512, 8/8: 32 workgroups of 128);
+// a CU's LDS and registers hold three of those, and one of 128 queries.  us, 64 and 128 queries, B x S, H/KH heads: D = 64: 17.8, 21.0 (1 x 512, 8/8: 32 workgroups of 128);
 // 29.3, 32.1 (1 x 1000, 16/4: 128); 57.1, 53.4 (1 x 2048, 16/16: 256); 120, 76 (1 x 2048, 32/8: 512).  D = 32: 23.1, 25.4 (1 x 1024, 8/8); 51.3, 52.7 (1 x 2048, 32/8); 162, 168 (1 x 4096, 32/8);
 // 36.6, 42.1 (1 x 4000, 16/8, window 512).
 template <int W>
