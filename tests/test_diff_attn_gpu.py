@@ -180,6 +180,32 @@ def test_the_parts_of_fused_rows(D):
     assert out[:, H * W:].eq(5.0).all() and dqkv[:, -8:].eq(5.0).all() and qkv[:, -8:].eq(5.0).all()
 
 
+@pytest.mark.parametrize("S,window", [(150, None), (1700, 1600)])
+def test_rows_far_apart(S, window):
+    """Operands and results as columns of rows whose distance is the largest that is taken, or that puts the last row behind 2^33 bytes: offsets that leave 32 bits, in bytes and in numbers."""
+    sizes = dict(B=1, S=S, H=2, KH=1, D=32)
+    ld, W = ((1 << 24) - 8 if S < 200 else 2_600_000), 64
+    x = make(**sizes, seed=12)
+    p = Plain(*x, window, **sizes)
+    rows = torch.empty(S * ld, dtype=BF, device="cuda").view(S, ld)
+    at = 0
+
+    def place(t):
+        nonlocal at
+        at += t.shape[1] + 64
+        place = rows[:, at - t.shape[1] - 64: at - 64]
+        place.copy_(t)
+        return place
+    q, k, v, do = (place(x[i].cuda()) for i in (0, 1, 2, 4))
+    lam = x[3].cuda()
+    r = ops().diff_attn_fwd(q, k, v, lam, window=window, **sizes, out=place(torch.zeros(S, 2 * W)))
+    check(r, p)
+    grads = [place(torch.zeros(S, n * W)) for n in (2, 1, 1)]
+    g = ops().diff_attn_bwd(q, k, v, lam, place(p.o.to(BF).cuda()), place(p.o2.to(BF).cuda()), p.lse.float().cuda(), do, window=window, **sizes, dq=grads[0], dk=grads[1], dv=grads[2])
+    check_grads(g, p)
+    assert all(a.data_ptr() == b.data_ptr() for a, b in zip(g, grads))
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("D,window", [(64, None), (32, None), (64, 40)])
 def test_what_a_row_does_not_see_does_not_reach_it(D, window, value):
