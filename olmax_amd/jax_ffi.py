@@ -454,20 +454,27 @@ class HipTrainStep:
         self.nf = int(L.olmax_model_grad_f32_elems(ctypes.byref(c)))
         pats = list(no_decay_modules or [])
         decay = [0 if any(fnmatch.fnmatch(l.name, p) for p in pats) else 1 for l in self.table] if pats else []
-        thetas = config.thetas()
-        uniq = sorted(set(thetas))
+        layers = list(zip(config.thetas(), config.scalings()))
+        uniq = sorted(dict.fromkeys(layers), key=lambda pair: pair[0])  # one table for each theta and scaling
         ints = [getattr(c, f) for f, _ in c._fields_[:14]]
         # attributes of the custom call are host values (numpy), fixed when the step is traced
         attrs = dict(config=np.asarray(ints, np.int32), eps=np.float32(c.eps), attn_softcap=np.float32(c.attn_softcap),
                      final_softcap=np.float32(c.final_softcap), windows=np.asarray(config.windows(), np.int32),
-                     table_index=np.asarray([uniq.index(t) for t in thetas], np.int32),
+                     table_index=np.asarray([uniq.index(pair) for pair in layers], np.int32),
                      leaf_decay=np.asarray(decay, np.int32), b1=np.float32(b1), b2=np.float32(b2),
                      adam_eps=np.float32(eps), wd=np.float32(weight_decay), max_grad_norm=np.float32(max_grad_norm or 0.0),
                      overlap=np.int32(int(overlap_optimizer and not max_grad_norm)))
-        # cos/sin tables, formed in fp32 as src/olmax/nn/rope.py:127-133 does
+        # cos/sin tables, formed in fp32 as src/olmax/nn/rope.py:127-133 does; scaled ones in 64 bits on the host, as olmax_rotary_tables has them
         half = jnp.arange(0.0, config.head_dim, 2) / config.head_dim
-        ang = jnp.stack([jnp.outer(jnp.arange(float(sequence_length)), 1.0 / (jnp.float32(t) ** half)) for t in uniq])
-        self.cos, self.sin = jnp.cos(ang), jnp.sin(ang)
+
+        def tables(theta, scaling):
+            if scaling is None:
+                angle = jnp.outer(jnp.arange(float(sequence_length)), 1.0 / (jnp.float32(theta) ** half))
+                return jnp.cos(angle), jnp.sin(angle)
+            angle = np.outer(np.arange(sequence_length, dtype=np.float64), scaling.frequencies(config.head_dim, theta))
+            return tuple(jnp.asarray((scaling.size * f(angle)).astype(np.float32)) for f in (np.cos, np.sin))
+
+        self.cos, self.sin = (jnp.stack(t) for t in zip(*(tables(*pair) for pair in uniq)))
         n, nf, T = self.n, self.nf, batch_size * sequence_length
 
         def step_fn(master, m, v, params, ids, labels, cos, sin, count):

@@ -10,7 +10,7 @@ from __future__ import annotations
 import functools
 import math
 from dataclasses import dataclass
-from typing import NamedTuple, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -171,10 +171,33 @@ class RopeScaling:
         if self.attention_factor is not None and self.kind != "yarn":
             raise ValueError("attention_factor goes with yarn")
 
+    @property
+    def size(self) -> float:
+        """What cos and sin are multiplied by."""
+        return 1.0 if self.kind != "yarn" else self.attention_factor if self.attention_factor is not None else 0.1 * math.log(self.factor) + 1.0
+
     def c_args(self):
         high = self.high_turns if self.high_turns is not None else 32.0 if self.kind == "yarn" else 4.0
-        size = 1.0 if self.kind != "yarn" else self.attention_factor if self.attention_factor is not None else 0.1 * math.log(self.factor) + 1.0
-        return _SCALING[self.kind], self.factor, self.original_length, self.low_turns, high, size
+        return _SCALING[self.kind], self.factor, self.original_length, self.low_turns, high, self.size
+
+    def frequencies(self, rotary_dim: int, theta: float) -> List[float]:
+        """f_i, i < rotary_dim / 2, of the angles p f_i that olmax_rotary_tables forms on the GPU, for tables that are made on the host."""
+        kind, s, L, low, high, size = self.c_args()
+        if not (rotary_dim > 0 and rotary_dim % 2 == 0 and 1.0 < theta <= 1e30 and 1.0 <= s <= 1e6 and 0.0 < size <= 1e30):
+            raise ValueError(f"{self}: rotary_dim must be even, theta within 1 and 1e30, factor within 1 and 1e6, the tables' size positive")
+        if kind >= 2 and not (1.0 <= L <= 2.0 ** 31 and 0.0 < low < high <= 1e30):
+            raise ValueError(f"{self}: original_length must be within 1 and 2^31, and 0 < low_turns < high_turns")
+        turns = L / (2.0 * math.pi)  # of an angle of 1 in the original context
+        if kind == 3:  # indices at which the original context has so many turns
+            at = lambda n: rotary_dim * math.log(turns / n) / (2.0 * math.log(theta))  # noqa: E731
+            low, high = max(math.floor(at(high)), 0), min(math.ceil(at(low)), rotary_dim - 1)
+        out = []
+        for i in range(rotary_dim // 2):
+            f = theta ** (-2.0 * i / rotary_dim)
+            slow = 1.0 if kind == 1 else 1.0 - (f * turns - low) / (high - low) if kind == 2 else (i - low) / max(high - low, 0.001)
+            slow = min(max(slow, 0.0), 1.0)
+            out.append((1.0 - slow) * f + slow * f / s)
+        return out
 
 
 def rotary_tables(length: int, rotary_dim: int, theta: float, device, *, scaling: Optional[RopeScaling] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -297,3 +297,47 @@ def test_adamw_transformation_and_train_step_make_the_calls_the_handlers_bind(ja
     _check_calls(jax, ["olmax_train_step"])
     back = step.unpack(new_state)
     assert set(back) == set(named) and all(back[k].shape == named[k].shape for k in named)
+
+
+@pytest.mark.parametrize("kinds,index", [((None, "llama3", "llama3"), [0, 1, 1]), (("yarn", "linear", None), [0, 1, 2]), (("yarn", "yarn", "yarn"), [0, 0, 0])])
+def test_train_step_takes_scaled_positions(jax_model, kinds, index):
+    """The whole step's tables are those of each layer's scaling, one for each theta and scaling: the oracle's angles in 64 bits, rounded to fp32 once (2^-24 of the size; its products and sums in
+    64 bits leave less than 2^-26 more)."""
+    torch = pytest.importorskip("torch")
+    from olmax_amd import TransformerConfig, jax_ffi
+    from olmax_amd.ops import RopeScaling
+    from oracle import ref
+    sets = {None: None, "linear": RopeScaling("linear", 2.0), "llama3": RopeScaling("llama3", 8.0, original_length=64), "yarn": RopeScaling("yarn", 4.0, original_length=64)}
+    per_layer = [sets[k] for k in kinds]
+    more = dict(rope_scaling=per_layer[0]) if len(set(kinds)) == 1 else dict(rope_scaling_per_layer=per_layer)
+    cfg = TransformerConfig(vocab_size=64, d_model=32, hidden_size=48, num_layers=3, n_heads=4, n_kv_heads=2, head_dim=32, rope_theta=1e4, **more)
+    S = 128
+    step = jax_ffi.HipTrainStep(cfg, batch_size=2, sequence_length=S)
+    assert step.cos.shape == step.sin.shape == (len(set(kinds)), S, 16)
+    if None not in kinds:  # (the model's arange is in 64 bits)
+        assert step.cos.dtype == step.sin.dtype == np.float32
+    state = tuple(np.zeros(step.n, t) for t in (np.float32, np.float32, np.float32, jax_model.numpy.bfloat16))
+    step(state, np.zeros((2, S), np.int64), np.zeros((2, S), np.int64), np.zeros([], np.int32))
+    call = jax_model.ffi.CALLS[0]
+    assert list(call["attrs"]["table_index"]) == index
+    _check_calls(jax_model, ["olmax_train_step"])
+    for layer, c in enumerate(per_layer):
+        if c is None:  # as without scalings anywhere
+            cos, sin = ref.rope_tables(S, 32, 1e4)
+            room = 128 * 2.0 ** -22  # angles in fp32, up to 128
+        else:
+            kw = dict(kind=c.kind, factor=c.factor, original_length=c.original_length, low_turns=c.low_turns, high_turns=c.c_args()[4])
+            angle = torch.arange(S, dtype=torch.float64)[:, None] * ref.rotary_freqs(32, 1e4, **kw)
+            cos, sin, room = c.c_args()[5] * angle.cos(), c.c_args()[5] * angle.sin(), 1.25 * c.c_args()[5] * 2.0 ** -24
+        for got, want in ((step.cos, cos), (step.sin, sin)):
+            assert np.abs(got[index[layer]].astype(np.float64) - want.double().numpy()).max() <= room
+
+
+@pytest.mark.parametrize("bad", [dict(kind="linear", factor=0.5), dict(kind="llama3", factor=2.0, original_length=0), dict(kind="llama3", factor=2.0, low_turns=5.0),
+                                 dict(kind="yarn", factor=2.0, attention_factor=0.0), dict(kind="yarn", factor=2.0, low_turns=0.0), dict(kind="linear", factor=2e6)])
+def test_train_step_refuses_scalings_that_the_library_refuses(jax_model, bad):
+    from olmax_amd import TransformerConfig, jax_ffi
+    from olmax_amd.ops import RopeScaling
+    cfg = TransformerConfig(vocab_size=64, d_model=32, hidden_size=48, num_layers=1, n_heads=4, head_dim=8, rope_scaling=RopeScaling(**bad))
+    with pytest.raises(ValueError):
+        jax_ffi.HipTrainStep(cfg, batch_size=2, sequence_length=16)
