@@ -63,9 +63,11 @@ __device__ __forceinline__ float dot(const bf16* a, const bf16* b, int n) {
   return s;
 }
 
+// second: whether something of the second map's is not finite either.  Otherwise its o2 and log-normaliser stand, and
+// stay as they are: another wave may still be storing them.  A log-normaliser that is finite stands as well.
 template <int W>
 __device__ __forceinline__ void redo_fwd(const bf16* q, const bf16* K, int64_t ldk, const bf16* V, int64_t ldv, float lam, bf16* o, bf16* o2, float* lse, int S, int i, int window,
-                                         float scale, int lane, int lo, int hi) {
+                                         float scale, int lane, bool second) {
   constexpr int D = W / 2;
   const int first = window >= 0 ? max(0, i - window) : 0;
   float l[2];
@@ -78,7 +80,7 @@ __device__ __forceinline__ void redo_fwd(const bf16* q, const bf16* K, int64_t l
 #pragma unroll 1
     for (int j = first + lane; j <= i; j += 64) sm += __expf(dot(q + m * D, K + j * ldk + m * D, D) * scale - mx);
     l[m] = mx + __logf(wave_sum(sm));
-    if (lane == 0 && lo == 0) lse[m * S] = l[m];
+    if (lane == 0 && (m == 0 || second) && !(fabsf(lse[m * S]) < INFINITY)) lse[m * S] = l[m];
   }
   float acc[2][W / 64] = {};
 #pragma unroll 1
@@ -103,9 +105,8 @@ __device__ __forceinline__ void redo_fwd(const bf16* q, const bf16* K, int64_t l
 #pragma unroll
   for (int c = 0; c < W / 64; c++) {
     const int at = c * 64 + lane;
-    if (at < lo || at >= hi) continue;
     o[at] = f2bf(acc[0][c] - lam * acc[1][c]);
-    if (o2) o2[at] = f2bf(acc[1][c]);
+    if (o2 && second) o2[at] = f2bf(acc[1][c]);
   }
 }
 
@@ -469,7 +470,8 @@ __global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* 
   }
   __syncthreads();
   if (m == 1) return;
-  zeros += reinterpret_cast<float*>(smem + QW * 32 * W * 4)[qw * 64 + lane];
+  const float zeros2 = reinterpret_cast<float*>(smem + QW * 32 * W * 4)[qw * 64 + lane];
+  zeros += zeros2;
   if (qi < S) {
     bf16* op = O + ((int64_t)b * S + qi) * z.ldo + h * W;
 #pragma unroll
@@ -487,10 +489,11 @@ __global__ __launch_bounds__(QW * 128, 2) void diff_attn_fwd_kernel(const bf16* 
   } else {
     zeros = 0.f;
   }
+  const uint64_t bad2 = __builtin_amdgcn_ballot_w64(zeros2 != 0.f);
   redo_rows(zeros, [&](int r) {
     const int i = iw0 + r;
     const int64_t at = (int64_t)b * S + i;
-    redo_fwd<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, lam, O + at * z.ldo + h * W, O2 ? O2 + at * z.ldo2 + h * W : nullptr, lse_row + i, S, i, window, z.scale, lane, 0, W);
+    redo_fwd<W>(Q + at * z.ldq + h * W, kbase, z.ldk, vbase, z.ldv, lam, O + at * z.ldo + h * W, O2 ? O2 + at * z.ldo2 + h * W : nullptr, lse_row + i, S, i, window, z.scale, lane, ((bad2 | bad2 >> 32) >> r & 1) != 0);
   });
 }
 
@@ -529,18 +532,20 @@ __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __r
   const int64_t at = (int64_t)b * S + i;
   bf16 *o = O + at * z.ldo + h * W, *o2 = O2 ? O2 + at * z.ldo2 + h * W : nullptr;
   float* lse_row = LSE + (int64_t)bh * 2 * S + i;
-  float zeros = (lse[0] + lse[1]) * 0.f;
+  float zeros = lse[0] * 0.f, zeros2 = lse[1] * 0.f;
 #pragma unroll
   for (int x = 0; x < W / 64; x++) {
     const float v = __builtin_fmaf(-lam, y[1][x], y[0][x]);
-    zeros = __builtin_fmaf(v, 0.f, __builtin_fmaf(y[1][x], 0.f, zeros));
+    zeros = __builtin_fmaf(v, 0.f, zeros);
+    zeros2 = __builtin_fmaf(y[1][x], 0.f, zeros2);
     o[x * 64 + lane] = f2bf(v);
     if (O2) o2[x * 64 + lane] = f2bf(y[1][x]);
   }
   if (lane < 2) lse_row[lane * S] = lane ? lse[1] : lse[0];
-  if (__builtin_amdgcn_ballot_w64(zeros != 0.f)) {
+  const bool bad2 = __builtin_amdgcn_ballot_w64(zeros2 != 0.f) != 0;
+  if (__builtin_amdgcn_ballot_w64(zeros != 0.f) || bad2) {
     dma_wait_all();
-    redo_fwd<W>(Q + at * z.ldq + h * W, K + (int64_t)b * S * z.ldk + kh * W, z.ldk, V + (int64_t)b * S * z.ldv + kh * W, z.ldv, lam, o, o2, lse_row, S, i, window, z.scale, lane, 0, W);
+    redo_fwd<W>(Q + at * z.ldq + h * W, K + (int64_t)b * S * z.ldk + kh * W, z.ldk, V + (int64_t)b * S * z.ldv + kh * W, z.ldv, lam, o, o2, lse_row, S, i, window, z.scale, lane, bad2);
   }
 }
 

@@ -403,3 +403,31 @@ def test_a_block_of_them_all():
     room = want.abs() * H8
     room[:, : heads * D] += 3 * U * pairs
     near(dqkv, want, room, "turned back")
+
+
+@pytest.mark.parametrize("sizes,window", [(dict(B=1, S=200, H=4, KH=2, D=64), None), (dict(B=2, S=150, H=4, KH=2, D=32), 60), (dict(B=41, S=130, H=16, KH=8, D=64), None),
+                                          (dict(B=1, S=1700, H=2, KH=1, D=64), None), (dict(B=1, S=4100, H=2, KH=1, D=32), None)])
+def test_what_is_wrong_with_the_first_map_leaves_the_second_ones_results(sizes, window):
+    """An infinity or NaN that only the first map or the weight has reaches o and the first map's log-normalisers; o2 and the second map's are the same bits as without it, whichever wave has stored
+    them.  (Rows of o that do not see it may differ by roundings: a wave moves the reference of its exponentials for all of its rows.)  With a weight that is NaN nothing but its head's o changes."""
+    H, D, S = sizes["H"], sizes["D"], sizes["S"]
+    x = make(**sizes, seed=13)
+    want = forward(x, sizes, window)
+    at = 70
+    last = min(S, at + window + 1) if window else S
+    for name, value in (("q", math.inf), ("k", math.nan), ("k", -math.inf), ("lam", math.nan)):
+        y = dict(zip(("q", "k", "v", "lam", "do"), (t.clone() for t in x)))
+        if name == "lam":
+            y["lam"][0] = value
+        else:
+            y[name][at, 1] = value  # (column 1 of a head: the first map's)
+        r = forward(tuple(y.values()), sizes, window)
+        assert torch.equal(r.o2, want.o2) and torch.equal(r.lse[:, :, 1], want.lse[:, :, 1]), name
+        bad = torch.zeros(sizes["B"], S, dtype=torch.bool, device="cuda")
+        bad[:1 if name != "lam" else None, at if name == "q" else at if name == "k" else 0: at + 1 if name == "q" else last if name == "k" else S] = True
+        heads = slice(0, 1) if name != "k" else slice(0, H // sizes["KH"])
+        o, clean = (t.view(-1, H, 2 * D) for t in (r.o, want.o))
+        if value != -math.inf:  # (scores of minus infinity alone leave a row as it is)
+            assert not o[bad.view(-1)][:, heads].isfinite().any(), name
+        if name == "lam":
+            assert torch.equal(o[:, 1:], clean[:, 1:]) and torch.equal(r.lse, want.lse)
