@@ -92,7 +92,7 @@ template <typename T, bool HALF>
 __global__ __launch_bounds__(256) void rotary_kernel(const T* x, T* y, const Turn a, int turning, int units, int slots, int per, int copies) {
   constexpr int N = rows::Vec<T>::N, UNROLL = 4, PAIRS = HALF ? N : N / 2;
   const int u = threadIdx.x % units, slot = threadIdx.x / units % slots, row = threadIdx.x / (units * slots);
-  const int64_t token = (int64_t)blockIdx.x * per + row;
+  const int64_t token = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * per + row;
   if (row >= per || token >= a.tokens) return;
   bool off;
   const int p = position_of(a, token, off);
@@ -167,6 +167,7 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(const T* x, T* y, const
   }
 }
 
+constexpr int64_t MOST_GROUPS = 1 << 23;  // workgroups of 256 in a dimension of the grid
 template <typename T>
 void launch(hipStream_t stream, const T* x, T* y, const Turn& a, bool half_layout) {
   constexpr int N = rows::Vec<T>::N;
@@ -178,7 +179,8 @@ void launch(hipStream_t stream, const T* x, T* y, const Turn& a, bool half_layou
     return;
   }
   const int slots = std::min((a.heads + 3) / 4, 256 / units), per = 256 / (units * slots);
-  const dim3 grid((unsigned)((a.tokens + per - 1) / per));
+  const int64_t groups = (a.tokens + per - 1) / per;  // below 2^31; a dimension of the grid has room for 2^32 threads, less one
+  const dim3 grid((unsigned)std::min(groups, MOST_GROUPS), (unsigned)((groups + MOST_GROUPS - 1) / MOST_GROUPS));
   const int copies = (const void*)x != (const void*)y;
   if (half_layout) hipLaunchKernelGGL((rotary_kernel<T, true>), grid, dim3(256), 0, stream, x, y, a, turning, units, slots, per, copies);
   else hipLaunchKernelGGL((rotary_kernel<T, false>), grid, dim3(256), 0, stream, x, y, a, turning, units, slots, per, copies);

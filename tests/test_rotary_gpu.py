@@ -244,3 +244,24 @@ def test_a_model_with_scaled_positions(monkeypatch, kind, scalings):
     for name, g in model.named_gradients().items():
         a, b = g.double().cpu().flatten(), grads[name].double().flatten()
         assert a @ b / (a.norm() * b.norm() + 1e-30) >= 0.999, name
+
+
+@pytest.mark.parametrize("head_dim,dtype", [(1040, BF), (520, BF), (520, F32)])
+def test_more_tokens_than_a_dimension_of_the_grid_has_threads_for(head_dim, dtype):
+    """Heads so wide that a workgroup of 256 has one token (or three), and so many tokens that their workgroups have 2^32 threads and more: the first tokens, those about 2^23 and 2^24 workgroups, and
+    the last against the plain form, in place; all others, which hold one number, against 37 rows of it."""
+    per = 256 // (head_dim // (8 if dtype == BF else 4))
+    T = per * 2 ** 24 + 5
+    cos, sin = tables(60, 32)
+    x = torch.full((T, head_dim), 3.0, dtype=dtype, device="cuda")
+    at = torch.cat([torch.arange(max(0, m - 20), min(T, m + 20)) for m in (0, per * 2 ** 23, per * 2 ** 24)])
+    some = torch.randn(at.numel(), head_dim, generator=torch.Generator().manual_seed(1)).to(dtype)
+    x[at.cuda()] = some.cuda()
+    assert ops().rotary_fwd(x, cos, sin, heads=1, head_dim=head_dim, seq_len=37, out=x) is x
+    check(x[at.cuda()], some, cos, sin, at % 37, 1, head_dim, "half", False)
+    want = ops().rotary_fwd(torch.full((37, head_dim), 3.0, dtype=dtype, device="cuda"), cos, sin, heads=1, head_dim=head_dim)
+    x[at.cuda()] = want[at.cuda() % 37]
+    for first in range(0, T, 37 * 2 ** 15):  # all rows, each once
+        chunk = x[first: first + 37 * 2 ** 15]
+        n = chunk.shape[0] // 37 * 37
+        assert (chunk[:n].view(-1, 37, head_dim) == want).all() and torch.equal(chunk[n:], want[: chunk.shape[0] - n]), first
