@@ -1278,11 +1278,13 @@ bool meet(const void* a, int64_t lda, int64_t na, const void* b, int64_t ldb, in
 }
 bool rows_ok(const void* p, int64_t ld, int64_t width) { return aligned16(p) && ld % 8 == 0 && ld >= width && ld < MAX_LD; }
 
-int check_shape(const char* name, int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D) {
+// rows, threads: queries and threads of a workgroup of the call's largest grid, which holds fewer than 2^32 threads
+int check_shape(const char* name, int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int rows, int threads) {
   OLMAX_CHECK(B > 0 && S > 0 && H > 0 && KH > 0 && H % KH == 0 && S <= (1 << 24) && H <= (1 << 16), OLMAX_ERR_SHAPE, "%s: bad shape B=%d S=%d H=%d KH=%d", name, B, S, H, KH);
   OLMAX_CHECK(((int64_t)S / 32 + 2) * (H / KH) < (1LL << 31), OLMAX_ERR_SHAPE, "%s: S=%d tokens of %d query heads to a key head are too many", name, S, H / KH);
   OLMAX_CHECK(D == 32 || D == 64, OLMAX_ERR_SHAPE, "%s: D must be 32 or 64 (got %d)", name, D);
-  OLMAX_CHECK(tiles_of(S) * 2 * H * B < (1LL << 31), OLMAX_ERR_SHAPE, "%s: B=%d S=%d H=%d are too many rows", name, B, S, H);
+  OLMAX_CHECK(((int64_t)S + rows - 1) / rows * H < (1LL << 32) / threads && ((int64_t)S + rows - 1) / rows * H * B < (1LL << 32) / threads, OLMAX_ERR_SHAPE,
+              "%s: B=%d S=%d H=%d are too many rows", name, B, S, H);
   return OLMAX_OK;
 }
 
@@ -1453,7 +1455,7 @@ extern "C" int64_t olmax_diff_attn_fwd_workspace_bytes(int32_t B, int32_t S, int
 extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const void* k, const void* v, const float* lam, void* o, void* o2, float* lse, void* workspace, int64_t workspace_bytes, int32_t B, int32_t S,
                                        int32_t H, int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t ldo2, int32_t lam_shared, int32_t window) {
   OLMAX_CHECK(q && k && v && lam && o && lse, OLMAX_ERR_ARG, "olmax_diff_attn_fwd: null pointer");
-  if (int rc = check_shape("olmax_diff_attn_fwd", B, S, H, KH, D)) return rc;
+  if (int rc = check_shape("olmax_diff_attn_fwd", B, S, H, KH, D, D == 32 ? 64 : 128, D == 32 ? 256 : 512)) return rc;
   const int64_t W = 2 * D, rows = (int64_t)B * S;
   OLMAX_CHECK(rows_ok(q, ldq, H * W) && rows_ok(k, ldk, KH * W) && rows_ok(v, ldv, KH * W) && rows_ok(o, ldo, H * W) && (!o2 || rows_ok(o2, ldo2, H * W)), OLMAX_ERR_ALIGN,
               "olmax_diff_attn_fwd: operands must be 16-byte aligned, with row strides that are multiples of 8, at least heads * 2D and below 2^24");
@@ -1484,7 +1486,7 @@ extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const 
                                        int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, int64_t ldo2, int64_t lddo, int64_t lddq, int64_t lddk,
                                        int64_t lddv, int32_t lam_shared, int32_t window) {
   OLMAX_CHECK(q && k && v && lam && o && o2 && lse && d_o && dq && dk && dv && dlam && workspace, OLMAX_ERR_ARG, "olmax_diff_attn_bwd: null pointer");
-  if (int rc = check_shape("olmax_diff_attn_bwd", B, S, H, KH, D)) return rc;
+  if (int rc = check_shape("olmax_diff_attn_bwd", B, S, H, KH, D, 128, 256)) return rc;
   const int64_t W = 2 * D, rows = (int64_t)B * S;
   const void *ins[] = {q, k, v, o, o2, d_o}, *outs[] = {dq, dk, dv};
   const int64_t ld_in[] = {ldq, ldk, ldv, ldo, ldo2, lddo}, n_in[] = {H * W, KH * W, KH * W, H * W, H * W, H * W};

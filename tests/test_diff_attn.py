@@ -107,3 +107,18 @@ def test_plain_form_is_two_attentions():
              for x in (0, 4)]
         assert (o[:, h * 8: h * 8 + 8] - (m[0] - lam[h] * m[1])).abs().max() < 1e-12 and (o2[:, h * 8: h * 8 + 8] - m[1]).abs().max() < 1e-12
         assert abs(lse[0, h, 1, 0] - (q[0, h * 8 + 4: h * 8 + 8] * k[0, h * 8 + 4: h * 8 + 8]).sum() / 2) < 1e-12
+
+
+ONE_ROW = dict(S=1, KH=64, H=64)
+
+
+@pytest.mark.parametrize("name,change,code", [  # 2^32 threads and more; one workgroup's fewer pass on to what is refused next
+    ("olmax_diff_attn_fwd", dict(B=1 << 17, D=64, **ONE_ROW), SHAPE), ("olmax_diff_attn_fwd", dict(B=(1 << 17) - 1, D=64, **ONE_ROW), ALIGN),
+    ("olmax_diff_attn_fwd", dict(B=1 << 18, D=32, **ONE_ROW), SHAPE), ("olmax_diff_attn_fwd", dict(B=(1 << 18) - 1, D=32, **ONE_ROW), ALIGN),
+    ("olmax_diff_attn_bwd", dict(B=1 << 18, D=64, **ONE_ROW), SHAPE), ("olmax_diff_attn_bwd", dict(B=(1 << 18) - 1, D=64, **ONE_ROW), ALIGN),
+    ("olmax_diff_attn_bwd", dict(B=1 << 18, D=32, **ONE_ROW), SHAPE), ("olmax_diff_attn_bwd", dict(B=(1 << 18) - 1, D=32, **ONE_ROW), ALIGN),
+    ("olmax_diff_attn_fwd", dict(B=1 << 6, S=1 << 24, H=1, KH=1, D=64), SHAPE), ("olmax_diff_attn_fwd", dict(B=(1 << 6) - 1, S=1 << 24, H=1, KH=1, D=64), ALIGN),
+    ("olmax_diff_attn_fwd", dict(B=(1 << 31) - 1, S=1 << 24, H=1 << 16, KH=1 << 16), SHAPE), ("olmax_diff_attn_bwd", dict(B=(1 << 31) - 1, S=1 << 24, H=1 << 16, KH=1 << 16), SHAPE)])
+def test_refuses_more_workgroups_than_a_launch_takes(name, change, code):
+    L = lib()
+    assert L.typed(name)(*{**CALLS[name], **change, "q": at(0) + 8}.values()) == code, L.load().olmax_last_error_string()
