@@ -197,7 +197,7 @@ int32_t olmax_attn_bwd_noalloc(olmax_stream_t stream, const void* q, const void*
  * A query head has two queries of width D (32 or 64) side by side, a key head two keys, and values are 2D wide: q, o, o2 [B*S, H*2D], k, v [B*S, KH*2D] bf16, row strides as in
  * olmax_attn_fwd (16-byte aligned, multiples of 8, below 2^24).  With P_m = softmax(q_m k_m^T / sqrt(D)) under the mask of olmax_attn_fwd (causal, window):
  *   o = (P_1 - lam_h P_2) v,   o2 = P_2 v (optional; the backward call takes it),   lse [B, H, 2, S]: both maps' log-normalisers
- * lam: fp32 [H], or (lam_shared) one number for all heads.  No output may share memory with an input or another output.
+ * lam: fp32 [H], or (lam_shared) one number for all heads.  No output (lse, dlam and the workspace among them) may share memory with an input or another output.
  * Long sequences of few heads take a workspace (16-byte aligned); where the query returns 0 none is read. */
 int64_t olmax_diff_attn_fwd_workspace_bytes(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window);
 int32_t olmax_diff_attn_fwd(olmax_stream_t stream, const void* q, const void* k, const void* v, const float* lam, void* o, void* o2, float* lse,

@@ -1276,6 +1276,13 @@ bool meet(const void* a, int64_t lda, int64_t na, const void* b, int64_t ldb, in
   const int64_t at = lda == ldb ? ((d % lda) + lda) % lda : 0;
   return at < na || at + nb > lda;
 }
+// The same of rows and a range of bytes, and of two ranges.
+bool meet(const void* a, int64_t lda, int64_t na, int64_t rows, const void* range, int64_t bytes) {
+  if (!a || !range || bytes <= 0) return false;
+  const int64_t d = (const char*)range - (const char*)a, first = d > 0 ? d : 0, ld = 2 * lda, n = 2 * na, end = std::min(d + bytes, (rows - 1) * ld + n);
+  return first < end && (first % ld < n || (first / ld + 1) * ld < end);
+}
+bool meet(const void* a, int64_t na, const void* b, int64_t nb) { return a && b && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na; }
 bool rows_ok(const void* p, int64_t ld, int64_t width) { return aligned16(p) && ld % 8 == 0 && ld >= width && ld < MAX_LD; }
 
 // rows, threads: queries and threads of a workgroup of the call's largest grid, which holds fewer than 2^32 threads
@@ -1470,6 +1477,13 @@ extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const 
   const int64_t need = fwd_chunk_bytes(B, z, (int)W);
   OLMAX_CHECK(need == 0 || (workspace && workspace_bytes >= need && (((uintptr_t)workspace) & 15) == 0), OLMAX_ERR_WORKSPACE,
               "olmax_diff_attn_fwd: workspace needs %ld bytes, 16-byte aligned", (long)need);
+  // what is not rows of heads
+  struct { const void* p; int64_t n; } const flat[] = {{lse, (int64_t)B * H * 2 * S * 4}, {workspace, need}, {lam, (lam_shared ? 1 : H) * 4ll}};
+  bool apart = !meet(lse, flat[0].n, workspace, need) && !meet(lse, flat[0].n, lam, flat[2].n) && !meet(workspace, need, lam, flat[2].n);
+  for (const auto& f : flat) apart = apart && !meet(o, ldo, H * W, rows, f.p, f.n) && !meet(o2, ldo2, H * W, rows, f.p, f.n);
+  for (int i = 0; i < 3; i++)
+    for (int f = 0; f < 2; f++) apart = apart && !meet(ins[i], ld_in[i], n_in[i], rows, flat[f].p, flat[f].n);
+  OLMAX_CHECK(apart, OLMAX_ERR_ARG, "olmax_diff_attn_fwd: lse, lam or the workspace shares memory with an output or an input");
   (D == 64 ? fwd<128> : fwd<64>)(stream, (const bf16*)q, (const bf16*)k, (const bf16*)v, lam, (bf16*)o, (bf16*)o2, lse, (float*)workspace, B, z);
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
@@ -1501,6 +1515,12 @@ extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const 
   for (int x = 0; x < 3; x++) {
     for (int i = 0; i < 6; i++) apart = apart && !meet(ins[i], ld_in[i], n_in[i], outs[x], ld_out[x], n_out[x], rows);
     for (int y = 0; y < x; y++) apart = apart && !meet(outs[y], ld_out[y], n_out[y], outs[x], ld_out[x], n_out[x], rows);
+  }
+  struct { const void* p; int64_t n; } const flat[] = {{dlam, (lam_shared ? 1 : H) * 4ll}, {workspace, need}, {lam, (lam_shared ? 1 : H) * 4ll}, {lse, (int64_t)B * H * 2 * S * 4}};  // two that are written
+  for (int f = 0; f < 4; f++) {
+    for (int x = 0; x < 3; x++) apart = apart && !meet(outs[x], ld_out[x], n_out[x], rows, flat[f].p, flat[f].n);
+    for (int i = 0; i < 6 && f < 2; i++) apart = apart && !meet(ins[i], ld_in[i], n_in[i], rows, flat[f].p, flat[f].n);
+    for (int g = 0; g < f && g < 2; g++) apart = apart && !meet(flat[g].p, flat[g].n, flat[f].p, flat[f].n);
   }
   OLMAX_CHECK(apart, OLMAX_ERR_ARG, "olmax_diff_attn_bwd: an output shares memory with an input or another output");
   const Sizes z{S, H, KH, window < 0 || window >= S ? -1 : window, ldq, ldk, ldv, ldo, ldo2, 1.f / sqrtf((float)D), lam_shared != 0};

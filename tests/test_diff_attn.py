@@ -122,3 +122,28 @@ ONE_ROW = dict(S=1, KH=64, H=64)
 def test_refuses_more_workgroups_than_a_launch_takes(name, change, code):
     L = lib()
     assert L.typed(name)(*{**CALLS[name], **change, "q": at(0) + 8}.values()) == code, L.load().olmax_last_error_string()
+
+
+WIDE = dict(ldq=Q + 64, ldk=Q + 64, ldv=Q + 64)  # rows of a wider buffer: room for 64 numbers behind each
+LAST = 2 * (B * S - 1)  # bytes to the last row of a stride of 1
+
+
+@pytest.mark.parametrize("name,change,code", [
+    ("olmax_diff_attn_fwd", dict(lse=at(0)), ARG), ("olmax_diff_attn_fwd", dict(lse=at(1) + LAST * KV + 2 * KV - 4), ARG), ("olmax_diff_attn_fwd", dict(lse=at(2) - 4 * B * H * 2 * S + 4), ARG),
+    ("olmax_diff_attn_fwd", dict(lse=at(4) + 1024), ARG), ("olmax_diff_attn_fwd", dict(lse=at(5) + 1024), ARG), ("olmax_diff_attn_fwd", dict(lse=at(3) - 8), ARG),
+    ("olmax_diff_attn_fwd", dict(lam=at(4) + 2 * Q), ARG), ("olmax_diff_attn_fwd", dict(lam=at(5) + 4, shared=1), ARG),
+    ("olmax_diff_attn_fwd", dict(lse=at(0) + 2 * Q, **WIDE), ARG), ("olmax_diff_attn_fwd", dict(lam=at(4) + 2 * Q - 4, ldo=Q + 64), ARG),
+    ("olmax_diff_attn_fwd", dict(lam=at(6) + 4 * B * H * 2 * S - 4, shared=1), ARG),
+    ("olmax_diff_attn_bwd", dict(dlam=at(3)), ARG), ("olmax_diff_attn_bwd", dict(dlam=at(3) + 12), ARG), ("olmax_diff_attn_bwd", dict(dlam=at(6) + 64), ARG), ("olmax_diff_attn_bwd", dict(dlam=at(8)), ARG),
+    ("olmax_diff_attn_bwd", dict(dlam=at(0) + 256), ARG), ("olmax_diff_attn_bwd", dict(dlam=at(12) + 1024), ARG), ("olmax_diff_attn_bwd", dict(ws=at(7)), ARG), ("olmax_diff_attn_bwd", dict(ws=at(10) - 256), ARG),
+    ("olmax_diff_attn_bwd", dict(ws=at(6)), ARG), ("olmax_diff_attn_bwd", dict(lse=at(9) + 4), ARG), ("olmax_diff_attn_bwd", dict(lam=at(8) + LAST * Q), ARG)])
+def test_refuses_memory_that_log_normalisers_weights_and_workspaces_share(name, change, code):
+    L = lib()
+    assert L.typed(name)(*{**CALLS[name], **change}.values()) == code and b"share" in L.load().olmax_last_error_string()
+
+
+@pytest.mark.parametrize("change", [dict(ws=at(0)), dict(ws=at(4)), dict(ws=at(6)), dict(ws=at(3) - 64), dict(ws=at(2) - 64)])
+def test_refuses_a_forward_workspace_in_other_memory(change):
+    L = lib()
+    few = {**FWD, **FEW, **{n: 2 * 64 for n in ("ldq", "ldk", "ldv", "ldo", "ldo2")}}
+    assert L.typed("olmax_diff_attn_fwd")(*{**few, **change}.values()) == ARG and b"share" in L.load().olmax_last_error_string()

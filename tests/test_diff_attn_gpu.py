@@ -431,3 +431,20 @@ def test_what_is_wrong_with_the_first_map_leaves_the_second_ones_results(sizes, 
             assert not o[bad.view(-1)][:, heads].isfinite().any(), name
         if name == "lam":
             assert torch.equal(o[:, 1:], clean[:, 1:]) and torch.equal(r.lse, want.lse)
+
+
+def test_weights_between_the_rows_of_the_queries():
+    """lam in the columns that a fused row has behind the queries: no operand's memory."""
+    sizes = dict(B=2, S=90, H=4, KH=2, D=64)
+    x = make(**sizes, seed=14)
+    p = Plain(*x, None, **sizes)
+    q, k, v, lam, do = (t.cuda() for t in x)
+    wide = torch.zeros(180, 512 + 64, dtype=BF, device="cuda")
+    wide[:, :512] = q
+    for row in (0, 57, 179):
+        between = wide[row, 512:520].view(torch.float32)
+        between.copy_(lam)
+        y = (wide[:, :512], k, v, between, do)
+        r = ops().diff_attn_fwd(*y[:4], **sizes)
+        check(r, p)
+        check_grads(ops().diff_attn_bwd(*y[:4], p.o.to(BF).cuda(), p.o2.to(BF).cuda(), p.lse.float().cuda(), do, **sizes), p)
