@@ -531,6 +531,10 @@ int32_t olmax_gemm_profile_end_shapes(int32_t* keys, int32_t* mnk, double* ms, i
 /* How olmax_attn_bwd runs on 16-byte aligned operands whose outputs share no memory with its inputs: bit 0 dQ, bit 1 dK/dV
  * with a workgroup's chain split over its waves, bit 2 both in one launch; -1: neither (another head_dim).  Host only. */
 int32_t olmax_attn_bwd_form(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window);
+/* How differential attention runs: bit 0 forward with 64 queries to a workgroup (128 otherwise), bit 1 with chains dealt out to workgroups and joined; bit 2 dQ split over the waves of a workgroup,
+ * bit 3 dealt out, bit 4 chains longer than a sweep ahead forms delta of (at weights up to 1); bit 5 dK/dV with four query groups to a workgroup, bit 6 with eight, bit 7 dealt out.  -1: refused
+ * shapes.  Host only. */
+int32_t olmax_diff_attn_form(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window);
 /* Profiler ranges: the counterpart of the reference's jax.named_scope annotations and
  * ProfilerCallback (src/olmax/train/callbacks/profiler.py:33-50).  on != 0: the whole-model entry
  * points emit roctx ranges ("olmax.layers.<l>.forward" / ".backward", "olmax.lm_head_and_loss")

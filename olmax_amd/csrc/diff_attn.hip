@@ -1535,3 +1535,18 @@ extern "C" int32_t olmax_diff_attn_bwd(hipStream_t stream, const void* q, const 
   OLMAX_LAUNCH_CHECK();
   return OLMAX_OK;
 }
+
+extern "C" int32_t olmax_diff_attn_form(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window) {
+  Sizes z;
+  if (!sizes_of(B, S, H, KH, D, window, z)) return -1;
+  const int W = 2 * D;
+  const bool q_parts = dq_plan(B, z, W).n > 1, kv_parts = dkv_plan(B, z, W).n > 1, split = !q_parts && q_split(B, z), narrow = !kv_parts && D == 32 && dkv_narrow(B, z);
+  const int64_t qr = split ? 32 * QSW : 128;
+  int64_t chain = 0;
+  for (int64_t i0 = 0; i0 < S; i0 += qr) chain = std::max(chain, key_tiles(z, i0, qr));
+  const bool fwd_parts = fwd_plan(B, z, W).n > 1;
+  const bool bits[] = {!fwd_parts && (D == 32 || fwd_halves<128>(B, z)), fwd_parts, split, q_parts, chain > SWEEP, !kv_parts && !narrow && dkv_split(B, z), narrow, kv_parts};
+  int32_t form = 0;
+  for (int i = 0; i < 8; i++) form |= bits[i] << i;
+  return form;
+}

@@ -93,3 +93,59 @@ def test_a_large_weight_beside_small_ones():
     lam = torch.tensor([0.5, -30.0] * 8)
     run_and_compare(sizes, None, [3], lam=lam, seed=22)
     run_and_compare({**sizes, "H": 1, "KH": 1}, None, [0], lam=torch.tensor([30.0]), seed=23, dq_room=dq_room_of_own_sums)
+
+
+# olmax_diff_attn_form's bits
+FWD64, FWD_DEALT, DQ_SPLIT, DQ_DEALT, LONG, KV4, KV8, KV_DEALT = (1 << i for i in range(8))
+FORMS = [  # B, S, H, KH, D, window, form, weights shared, key heads that are compared
+    (2, 1100, 40, 40, 64, None, LONG, False, (0, 39)), (2, 1100, 40, 40, 64, 700, LONG, True, (7, 39)), (2, 1100, 80, 40, 64, None, LONG, False, (0, 20)),
+    (2, 1100, 16, 8, 64, None, LONG | KV4, False, (0, 7)), (2, 1100, 16, 8, 64, 600, LONG | KV4, False, (0, 7)), (2, 1300, 24, 12, 64, 900, LONG | KV4, True, (11,)),
+    (1, 3000, 32, 8, 64, None, LONG | KV_DEALT, False, (5,)), (1, 4001, 32, 16, 64, 1024, LONG | KV4, False, (9,)),
+    (2, 1100, 16, 16, 32, None, FWD64 | LONG | KV4, False, (0, 15)), (2, 1100, 32, 16, 32, None, FWD64 | LONG | KV4, False, (0, 15)), (1, 1500, 24, 12, 32, 400, LONG | FWD64 | KV4, False, (3,)),
+    (2, 1100, 48, 12, 32, None, FWD64 | LONG | KV4, True, (0,)), (2, 1100, 40, 40, 32, None, FWD64 | LONG, False, (0, 39)), (2, 1100, 80, 40, 32, 700, FWD64 | LONG, False, (13,)),
+    (1, 1100, 4, 4, 64, 700, DQ_SPLIT | FWD64 | LONG | KV4, False, (0, 3)), (1, 1300, 16, 2, 32, 900, FWD64 | DQ_SPLIT | LONG | KV_DEALT, False, (1,)),
+    (1, 4000, 8, 2, 64, 1024, DQ_SPLIT | LONG | KV_DEALT, False, (0,)), (1, 4000, 8, 2, 32, 1024, FWD64 | DQ_SPLIT | LONG | KV8, False, (0,))]
+
+
+@pytest.mark.parametrize("B,S,H,KH,D,window,form,shared,groups", FORMS)
+def test_forms_of_large_grids_and_long_sequences(B, S, H, KH, D, window, form, shared, groups):
+    print(f"[case] diff B{B} S{S} H{H} KH{KH} D{D} w{window} form{form}", flush=True)
+    lam = torch.full((1,), 0.7) if shared else torch.rand(H, generator=torch.Generator().manual_seed(S)) * 1.2 - 0.3
+    run_and_compare(dict(B=B, S=S, H=H, KH=KH, D=D), window, groups, lam=lam, seed=S + H)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("sizes,window,at", [(dict(B=2, S=1100, H=16, KH=8, D=64), None, 800), (dict(B=2, S=1100, H=40, KH=20, D=32), 700, 90), (dict(B=2, S=1100, H=40, KH=40, D=64), None, 1000)])
+def test_what_a_row_does_not_see_does_not_reach_it_in_long_rows(sizes, window, at, value):
+    """As test_what_a_row_does_not_see_does_not_reach_it, in the forms of large grids."""
+    B, S, H, KH, D = (sizes[n] for n in ("B", "S", "H", "KH", "D"))
+    T, rep, W, last = B * S, H // KH, 2 * D, min(S, at + window + 1) if window else S
+    x = make(**sizes, seed=31)
+    part, small = part_of(x, 0, sizes)
+    p = Plain(*part, window, **small)
+
+    def backward(**changed):
+        q, k, v, lam, do = (changed.get(n, t).cuda() for n, t in zip(("q", "k", "v", "lam", "do"), x))
+        r = ops().diff_attn_fwd(q, k, v, lam, window=window, **sizes)
+        o, o2, lse = r.o.clone(), r.o2.clone(), r.lse.clone()
+        o[:, : rep * W], o2[:, : rep * W], lse[:, :rep] = p.o.to(BF).cuda(), p.o2.to(BF).cuda(), p.lse.float().cuda()
+        return r, ops().diff_attn_bwd(q, k, v, lam, o, o2, lse, do, window=window, **sizes)
+    k, v = x[1].clone(), x[2].clone()
+    k[at, 1] = v[at, 3] = value
+    r, g = backward(k=k, v=v)
+    rest = torch.ones(T, dtype=torch.bool)
+    rest[at: last] = False
+    for got, name in ((r.o, "o"), (r.o2, "o2"), (g[0], "dq")):
+        want = getattr(p, name) if name != "dq" else p.grads[0]
+        near(got[rest.cuda()][:, : rep * W], want[rest], getattr(p, name + "_room")[rest], name)
+    assert not r.o[at: last, : rep * W].isfinite().all(1).any() and r.o[:, rep * W:].isfinite().all()
+    q, do = x[0].clone(), x[4].clone()
+    q[at, 1] = do[at, 2] = value
+    _, g = backward(q=q, do=do)
+    rest = torch.ones(T, dtype=torch.bool)
+    rest[max(0, at - window) if window else 0: at + 1] = False
+    for i, name in ((1, "dk"), (2, "dv")):
+        near(g[i][rest.cuda()][:, :W], p.grads[i][rest], getattr(p, name + "_room")[rest], name)
+    rest = torch.ones(T, dtype=torch.bool)
+    rest[at] = False
+    near(g[0][rest.cuda()][:, : rep * W], p.grads[0][rest], p.dq_room[rest], "dq of the other queries")
