@@ -265,3 +265,53 @@ def test_more_tokens_than_a_dimension_of_the_grid_has_threads_for(head_dim, dtyp
         chunk = x[first: first + 37 * 2 ** 15]
         n = chunk.shape[0] // 37 * 37
         assert (chunk[:n].view(-1, 37, head_dim) == want).all() and torch.equal(chunk[n:], want[: chunk.shape[0] - n]), first
+
+
+def _model_of_scaled_positions(kind, per_layer, thetas=(1e4, 5e5)):
+    qk = kind != "default"
+    sizes = dict(n_heads=2, n_kv_heads=2, head_dim=64)
+    ocfg = ref.ModelConfig(vocab=512, d_model=256, n_layers=2, hidden=512, layer_type="reordered" if qk else "pre", act="silu", qk_norm=qk, qk_norm_headwise=True, eps=1e-6,
+                           rope_theta_layers=list(thetas), **sizes)
+    gen = torch.Generator().manual_seed(5)
+    ids, labels = (torch.randint(0, 512, (2, 128), generator=gen, dtype=torch.int32) for _ in range(2))
+    P = {k: (v + 0.1 * torch.randn(v.shape, generator=torch.Generator().manual_seed(3)) if "norm" in k else 2 * v).to(BF).double() for k, v in ref.init_params(ocfg, seed=1).items()}
+    more = dict(vocab_size=512, d_model=256, hidden_size=512, num_layers=2, layer_type=kind, qk_norm_headwise=qk, norm_eps=1e-6, rope_theta_per_layer=list(thetas),
+                rope_scaling_per_layer=per_layer, **sizes)
+    return ocfg, P, ids, labels, more
+
+
+@pytest.mark.parametrize("kind", ["default", "reordered_norm"])
+def test_a_models_gradients_are_as_large_as_the_tables_make_them(monkeypatch, kind):
+    """Norms of a model's gradients with yarn's tables, whose size (1.139 here) enters the scores twice and the gradients of queries and keys again.  A cosine of 0.999 leaves an error of sqrt(0.002)
+    across the gradient, and roundings leave no more along it: norms agree within 0.045.  The oracle with tables of size 1, and one that leaves the size out of the backward pass alone, do not."""
+    from olmax_amd import TransformerConfig
+    yarn = ops().RopeScaling("yarn", 4.0, original_length=32)
+    ocfg, P, ids, labels, more = _model_of_scaled_positions(kind, [yarn, yarn])
+    model = TransformerConfig(**more).build(batch_size=2, sequence_length=128)
+    model.load_state_dict({k: v.float() for k, v in P.items()})
+    model.loss_and_grads(ids.cuda().reshape(-1), labels.cuda().reshape(-1))
+    got = {name: g.double().cpu().norm().item() for name, g in model.named_gradients().items()}
+    rt = lambda t: t.to(BF).to(t.dtype)  # noqa: E731
+    of = _scaled({1e4: yarn, 5e5: yarn})
+    monkeypatch.setattr(ref, "rope_tables", of)
+    want = {name: g.double().norm().item() for name, g in ref.model_loss_and_grads(ocfg, P, ids, labels.long(), rt)[1].items()}
+    monkeypatch.setattr(ref, "rope_tables", lambda S, D, theta, dtype=F32: tuple((t.double() / yarn.size).to(dtype) for t in of(S, D, theta, torch.float64)))
+    bare = {name: g.double().norm().item() for name, g in ref.model_loss_and_grads(ocfg, P, ids, labels.long(), rt)[1].items()}
+    for name in want:
+        assert abs(got[name] / want[name] - 1) < 0.045, (name, got[name], want[name])
+    turned = [name for name in want if "q_proj" in name or "k_proj" in name or "q_norm" in name or "k_norm" in name]
+    assert len(turned) == (4 if kind == "default" else 8)
+    for name in turned:  # planted in the oracle: the forward's size, and the backward's
+        assert abs(bare[name] / want[name] - 1) > 0.045 and abs(1 / yarn.size - 1) > 2 * 0.045, (name, bare[name], want[name])
+
+
+def test_a_layer_has_its_own_scaling():
+    """One layer by itself takes the tables that the model gives it."""
+    from olmax_amd import TransformerConfig
+    from olmax_amd.layer import TransformerBlock
+    yarn = ops().RopeScaling("yarn", 4.0, original_length=32)
+    *_, more = _model_of_scaled_positions("default", [None, yarn])
+    c = TransformerConfig(**more)
+    for i, want in enumerate((ops().rope_tables(128, 64, 1e4, "cuda"), ops().rotary_tables(128, 64, 5e5, "cuda", scaling=yarn))):
+        block = TransformerBlock(c, layer_idx=i, batch_size=2, sequence_length=128)
+        assert torch.equal(block.cos, want[0]) and torch.equal(block.sin, want[1])
