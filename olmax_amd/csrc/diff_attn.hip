@@ -561,6 +561,9 @@ __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __r
 // STATS [B, H, 4, S]: what dK/dV takes of a row: lse_1 and lse_2 in powers of two, -delta_1, and -lambda (delta_1 - delta_2) (-lambda (dP - delta_2) is -lambda times what it has of the first map, plus this).  DLAM: a number for
 // each workgroup, [B, H, tiles].
 // ---------------------------------------------------------------------------------------
+// A log-normaliser in powers of two is rounded, by up to 2^-24 of itself, and all of its row's probabilities are off by that: what their sums are multiplied by for it.
+// (log2(e) is off as much in the scores' factor: the two cancel.)
+__device__ __forceinline__ float mend(float lse, float l) { return __builtin_fmaf(-LN2, __builtin_fmaf(lse, LOG2E, -l), 1.f); }
 struct Grad {
   int64_t lddo, lddq, lddk, lddv;
 };
@@ -714,11 +717,14 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
               const int j = j0 + jt * 32 + k;
               return j > i || (window >= 0 && j < i - window);
             });
+          float t1 = 0.f, t2 = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; r++) {
-            sum1 = __builtin_fmaf(fexp2(__builtin_fmaf(s1[r], sc2, -l1)), dp[r], sum1);
-            sum2 = __builtin_fmaf(fexp2(__builtin_fmaf(s2[r], sc2, -l2)), dp[r], sum2);
+            t1 = __builtin_fmaf(fexp2(__builtin_fmaf(s1[r], sc2, -l1)), dp[r], t1);
+            t2 = __builtin_fmaf(fexp2(__builtin_fmaf(s2[r], sc2, -l2)), dp[r], t2);
           }
+          sum1 += t1;
+          sum2 += t2;
         }
       }
       dma_wait_all();
@@ -757,6 +763,7 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
       constexpr int STEPS = 2 * KS, EL = 16 / STEPS, AHEAD = 2;
       f32x16 s1[2], s2[2], dp[2];
       bf16x8 ds1[2][2], ds2[2][2], fr[AHEAD + 1];
+      float t1 = 0.f, t2 = 0.f;  // the sums of half a tile
       auto pin = [] { __builtin_amdgcn_sched_barrier(0); };
       auto fetch = [&](int n) {  // the fragment of product n
         const int run = n / STEPS, s = n % STEPS;
@@ -766,10 +773,14 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
       auto left = [&](int jt, int s) {
 #pragma unroll
         for (int r = s * EL; r < (s + 1) * EL; r++) {
-          sum1 = __builtin_fmaf(s1[jt][r], dp[jt][r], sum1);
-          sum2 = __builtin_fmaf(s2[jt][r], dp[jt][r], sum2);
+          t1 = r == 0 ? s1[jt][r] * dp[jt][r] : __builtin_fmaf(s1[jt][r], dp[jt][r], t1);
+          t2 = r == 0 ? s2[jt][r] * dp[jt][r] : __builtin_fmaf(s2[jt][r], dp[jt][r], t2);
           ds1[jt][r >> 3][r & 7] = f2bf(s1[jt][r] * (dp[jt][r] - d1));
           ds2[jt][r >> 3][r & 7] = f2bf(s2[jt][r] * (dp[jt][r] - d2));
+        }
+        if (s + 1 == STEPS) {
+          sum1 += t1;
+          sum2 += t2;
         }
       };
       pin();
@@ -825,6 +836,11 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
       }
     }
     return;
+  }
+  {
+    const float* lse = LSE + row0 + min(iw0 + (lane_id() & 31), S - 1);
+    sum1 *= mend(lse[0], l1);
+    sum2 *= mend(lse[S], l2);
   }
   float zeros = 0.f;
   auto store4 = [&](int u, const f32x4& v) {
@@ -898,6 +914,8 @@ __global__ __launch_bounds__(1024) void diff_attn_dq_join_kernel(const bf16* __r
     bf16* dq = dQ + at * gr.lddq + h * W;
     const float* lse = LSE + (int64_t)bh * 2 * S + i;
     const float l1 = lse[0], l2 = lse[S];
+    sum1 *= mend(l1, l1 * LOG2E);
+    sum2 *= mend(l2, l2 * LOG2E);
     float zeros = (sum1 + sum2) * 0.f;
 #pragma unroll
     for (int x = 0; x < W / 64; x++) {

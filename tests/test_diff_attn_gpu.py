@@ -448,3 +448,37 @@ def test_weights_between_the_rows_of_the_queries():
         r = ops().diff_attn_fwd(*y[:4], **sizes)
         check(r, p)
         check_grads(ops().diff_attn_bwd(*y[:4], p.o.to(BF).cuda(), p.o2.to(BF).cuda(), p.lse.float().cuda(), do, **sizes), p)
+
+
+@pytest.mark.parametrize("sizes", [dict(B=1, S=300, H=8, KH=8, D=64), dict(B=41, S=130, H=16, KH=8, D=64), dict(B=2, S=1100, H=16, KH=8, D=64)])
+@pytest.mark.parametrize("window", [0, 150])
+def test_weights_gradient_at_large_scores(sizes, window):
+    """Equal scores m, whole numbers that differ by head and go up to 1000, and dP = 64: every probability is one over the number of keys n that a row sees, and dlam is -64 times the number of rows (the
+    log-normalisers are given, m + ln n rounded to fp32, and P = exp(m - that), which dlam is computed from here).  m's exponent is rounded by up to 2^-24 m log2(e), 9e-5 at 1000, which all of a
+    head's rows share.  What is left: an exponential's 2^-23, three roundings of the row's factor and sum, the second order 2^-26 of that factor, at most 64 for n equal numbers, in
+    tiles of 16, and for the rows', log2 (64 x rows) + 64 of u."""
+    B, S, H, KH, D = (sizes[n] for n in ("B", "S", "H", "KH", "D"))
+    T = B * S
+    g = torch.Generator().manual_seed(15)
+    m = torch.randint(500, 1000, (KH,), generator=g).repeat_interleave(H // KH)
+    # a score of m: q k / 8 with k = 8 in eight columns and q = m / 8 as a bf16 number above, and below, its lowest bits
+    k = torch.zeros(T, KH, 2, D)
+    k[..., :8] = 8.0
+    q = torch.zeros(T, H, 2, D)
+    q[..., 0] = (m - m % 8).float()[:, None]
+    q[..., 1] = (m % 8).float()[:, None]
+    v, do = torch.full((T, KH * 2 * D), 1.0), torch.zeros(T, H, 2 * D)
+    do[..., 0] = 64.0
+    lam = torch.linspace(0.1, 0.9, H)
+    i = torch.arange(S)
+    n = (torch.clamp(i, max=window) + 1).double()
+    exact = m.double()[:, None] + n.log()[None, :]  # [H, S]
+    lse = exact.float()
+    p = torch.exp(m.double()[:, None] - lse.double())
+    want = -64.0 * B * (p * n).sum(1)
+    x = [t.reshape(T, -1).to(BF).cuda() for t in (q, k, v)]
+    full = lse[None, :, None, :].expand(B, H, 2, S).contiguous().cuda()
+    o = (torch.ones(T, H, 2 * D) * (1 - lam)[None, :, None]).reshape(T, -1).to(BF).cuda()
+    got = ops().diff_attn_bwd(*x, lam.cuda(), o, torch.ones(T, H * 2 * D, dtype=BF, device="cuda"), full, do.reshape(T, -1).to(BF).cuda(), window=window, **sizes)[3]
+    room = want.abs() * U * (2 + 3 + 1 + 64 + math.log2(64 * T) + 64)
+    near(got, want, room, "dlam")
