@@ -198,12 +198,13 @@ int32_t olmax_attn_bwd_noalloc(olmax_stream_t stream, const void* q, const void*
  * olmax_attn_fwd (16-byte aligned, multiples of 8, below 2^24).  With P_m = softmax(q_m k_m^T / sqrt(D)) under the mask of olmax_attn_fwd (causal, window):
  *   o = (P_1 - lam_h P_2) v,   o2 = P_2 v (optional; the backward call takes it),   lse [B, H, 2, S]: both maps' log-normalisers
  * lam: fp32 [H], or (lam_shared) one number for all heads.  No output (lse, dlam and the workspace among them) may share memory with an input or another output.
- * Long sequences of few heads take a workspace (16-byte aligned); where the query returns 0 none is read. */
+ * Long sequences of few heads take a workspace (16-byte aligned); where the query returns 0 none is read.  (D = 128, with values of 256, is refused: the kernels' tiles and accumulators have no room.) */
 int64_t olmax_diff_attn_fwd_workspace_bytes(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window);
 int32_t olmax_diff_attn_fwd(olmax_stream_t stream, const void* q, const void* k, const void* v, const float* lam, void* o, void* o2, float* lse,
                             void* workspace, int64_t workspace_bytes, int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int64_t ldq, int64_t ldk, int64_t ldv,
                             int64_t ldo, int64_t ldo2, int32_t lam_shared, int32_t window);
-/* From o, o2 and lse of the forward call and d_o = d loss / d o: dq, dk, dv, and dlam ([H], or one number with lam_shared, fp32).  Deterministic. */
+/* From o, o2 and lse of the forward call and d_o = d loss / d o: dq, dk, dv, and dlam ([H], or one number with lam_shared, fp32).  Deterministic.  The workspace is 256-byte aligned, and every call
+ * takes one. */
 int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window);
 int32_t olmax_diff_attn_bwd(olmax_stream_t stream, const void* q, const void* k, const void* v, const float* lam, const void* o, const void* o2, const float* lse,
                             const void* d_o, void* dq, void* dk, void* dv, float* dlam, void* workspace, int64_t workspace_bytes, int32_t B, int32_t S, int32_t H, int32_t KH,

@@ -7,6 +7,8 @@
 //   dS_1 = P_1 (dP - delta_1),  dS_2 = -lambda P_2 (dP - delta_2),  dq_m = dS_m k_m / sqrt(D),  dk_m = dS_m^T q_m / sqrt(D),
 //   dv = (P_1 - lambda P_2)^T do,  dlambda = - sum of delta_2 over the head's queries
 // so that the gradients take no more products than one map of width W does, but the exponentials of two.
+// D is 32 or 64.  Maps of 128 have values of 256: a wave's accumulators of 32 queries would be 128 registers in the forward pass and 256 in dK/dV's, and three stages of K and V 192 KB of the 160 that
+// there are, so that they would want kernels of another layout.
 //
 // The kernels are laid out as those of attn.hip: score tiles are transposed, a lane owns one query (forward, dQ) or one key (dK/dV), and a [rows][W] tile of K or Q holds both
 // maps' halves of a row, k-steps 0 .. W/32 - 1 of the products the first one's.
@@ -551,7 +553,8 @@ __global__ __launch_bounds__(256) void diff_attn_fwd_join_kernel(const bf16* __r
 
 // ---------------------------------------------------------------------------------------
 // dQ, dlambda and delta.  grid = ceil(S / 32 QW) H B workgroups of QW x KG waves; wave (qw, kg) owns 32 queries and every KG-th of their key tiles.  KG = 1 (QW = 4): two workgroups per CU, no merge.
-// KG > 1: one workgroup of eight waves with 1 / KG of the chain of tiles; what they have is added through LDS, in key-group order.  See q_split.
+// KG > 1 (QW = 2): a workgroup of 64 queries, four waves for heads of 64 (KG = 2; its LDS leaves room for one on a CU) and eight for heads of 32 (KG = 4), a wave with 1 / KG of the chain of tiles;
+// what they have is added through LDS, in key-group order.  See q_split.
 // The sums of P_m dP come out of the same sweep in fp32: dK/dV takes its delta from them, and dlambda is their sum: terms of both signs, that an error of 2^-9 in each would leave three digits of.
 // dQ: 1 x 4096 tokens, 32/8 heads of 64: 255 us, 206 GFLOP at 810 TFLOP/s, bound by issue as the forward; fragments one product ahead 10 us more, four spill.
 // For dQ they come too late, and it takes delta from the outputs as they were rounded, as dQ of attn.hip does; but where a workgroup has SWEEP key tiles or fewer, a sweep ahead forms them first.
@@ -1348,7 +1351,7 @@ bool fwd_halves(int B, const Sizes& z) { return W == 64 || tiles_of(z.S) * z.H *
 // forward, margin 20: 54, 162 (49, 136) 1 x 8192, 1/1; 39, 85 (36, 71) 1 x 4096, 2/1; 33, 47 (29, 39) 1 x 2048, 4/4; 43, 48 (40, 39) 1 x 2048, 8/2; below it 37, 29 (34, 24) 1 x 1000, 16/4.
 // A backward pass with only dQ's dealt out, margin 12: 233, 327 (145, 179) 1 x 8192, 1/1; 211, 246 1 x 4096, 2/1; below it 115, 112 (65, 61) 1 x 1000, 4/1; 131, 121 (97, 81) 1 x 2048, 16/16.
 // With only dK/dV's, margin 6 (steps of half the size): 375, 484 1 x 4096, 16/4; 106, 210 (67, 106) 1 x 2048, 8/2; 75, 116 (51, 61) 1 x 1000, 16/4; 38, 48 1 x 300, 4/1; below it
-// 226, 206 (142, 131) 1 x 4096, 8/8; 687, 633 1 x 4096, 32/8; 137, 157 (92, 86) 1 x 4000, 8/2 with a window of 1024.
+// 226, 206 (142, 131) 1 x 4096, 8/8; 687, 633 1 x 4096, 32/8; (92, 86) 1 x 4000, 8/2 of 32 with a window of 1024, where heads of 64, above it, take 137 dealt out and 157 not.
 template <typename F>
 Chunks plan_of(int64_t tiles, int64_t heads, int places, int groups, int margin, F steps) {  // steps(0) the longest chain's
   Chunks ch{nullptr, 0, 1, {}};
@@ -1512,7 +1515,7 @@ extern "C" int32_t olmax_diff_attn_fwd(hipStream_t stream, const void* q, const 
   return OLMAX_OK;
 }
 
-// Workspace: the rows' statistics [B, H, 4, S], then dlambda's parts [B, H, ceil(S / 128)], fp32
+// Workspace: the rows' statistics [B, H, 4, S], then dlambda's parts, up to [B, H, ceil(S / 64)], then the chunks of chains that are dealt out (dQ's, and in the same place dK/dV's), fp32
 extern "C" int64_t olmax_diff_attn_bwd_workspace_bytes(int32_t B, int32_t S, int32_t H, int32_t KH, int32_t D, int32_t window) {
   Sizes z;
   return sizes_of(B, S, H, KH, D, window, z) ? stats_bytes(B, S, H) + parts_bytes(B, S, H) + bwd_chunk_bytes(B, z, 2 * D) : 0;

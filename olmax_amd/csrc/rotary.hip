@@ -13,7 +13,7 @@ namespace {
 //   1 all by the factor;  2 (llama3) those that turn less than `low` times in the original context by the factor, those that turn more than `high` times not, linearly in the
 //   turns between;  3 (yarn) by the index, linearly between those of so many turns, `low` and `high` then (not up to low, by the factor from high on).
 // The angle is formed in quarters of a turn and in 64 bits: at position 131072 fp32 leaves an error of 0.004.  A quarter's fraction, to the nearest, is exact, so that what fp32 adds is
-// two Taylor polynomials on [-pi/4, pi/4], whose next terms are 2e-9 and 5e-10.
+// two Taylor polynomials on [-pi/4, pi/4], whose next terms are 2e-9 and 1.2e-10.
 struct Scaling {
   int kind;
   double log_theta, factor, turns, low, high;  // turns: of an angle of 1 in the original context, L / 2 pi
