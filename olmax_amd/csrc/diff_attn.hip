@@ -1308,7 +1308,9 @@ bool meet(const void* a, int64_t lda, int64_t na, int64_t rows, const void* rang
   const int64_t d = (const char*)range - (const char*)a, first = d > 0 ? d : 0, ld = 2 * lda, n = 2 * na, end = std::min(d + bytes, (rows - 1) * ld + n);
   return first < end && (first % ld < n || (first / ld + 1) * ld < end);
 }
-bool meet(const void* a, int64_t na, const void* b, int64_t nb) { return a && b && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na; }
+bool meet(const void* a, int64_t na, const void* b, int64_t nb) {
+  return a && b && na > 0 && nb > 0 && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na;
+}
 bool rows_ok(const void* p, int64_t ld, int64_t width) { return aligned16(p) && ld % 8 == 0 && ld >= width && ld < MAX_LD; }
 
 // rows, threads: queries and threads of a workgroup of the call's largest grid, which holds fewer than 2^32 threads

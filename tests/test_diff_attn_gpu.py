@@ -482,3 +482,17 @@ def test_weights_gradient_at_large_scores(sizes, window):
     got = ops().diff_attn_bwd(*x, lam.cuda(), o, torch.ones(T, H * 2 * D, dtype=BF, device="cuda"), full, do.reshape(T, -1).to(BF).cuda(), window=window, **sizes)[3]
     room = want.abs() * U * (2 + 3 + 1 + 64 + math.log2(64 * T) + 64)
     near(got, want, room, "dlam")
+
+
+def test_a_workspace_that_is_not_needed_may_lie_anywhere():
+    """Where the query returns 0 the workspace is no memory of the call's, whatever it points to."""
+    from olmax_amd import _lib
+    sizes = dict(B=2, S=90, H=4, KH=2, D=64)
+    q, k, v, lam, _ = (t.cuda() for t in make(**sizes, seed=16))
+    want = ops().diff_attn_fwd(q, k, v, lam, **sizes)
+    assert ops()._size32("olmax_diff_attn_fwd_workspace_bytes", *sizes.values(), -1) == 0
+    o, o2, lse = (torch.empty_like(t) for t in want)
+    for at in (None, lse.data_ptr() + 64, o.data_ptr() + 64, q.data_ptr(), lam.data_ptr() + 4):
+        _lib.check(_lib.typed("olmax_diff_attn_fwd")(_lib.raw_stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), o.data_ptr(), o2.data_ptr(), lse.data_ptr(), at, 0, *sizes.values(),
+                                                     512, 256, 256, 512, 512, 0, -1))
+        assert all(torch.equal(a, b) for a, b in zip((o, o2, lse), want))
