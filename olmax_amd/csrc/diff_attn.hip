@@ -1335,6 +1335,8 @@ bool q_split(int B, const Sizes& z) { return tiles_of(z.S) * z.H * B <= 256; }
 // 512 places, of half the longest chain's work on average.
 // D = 64, 2 x 4 and 4 x 1: 617, 1053 (1 x 4096, 32/8: 256 workgroups of 4 x 1); 1209, 1349 (2 x 4096, 32/8: 512); 667, 586 (1 x 4096, 32/32: 1024); 1234, 1107 (1 x 8192, 16/16: 1024);
 // window 512: 170, 178 (1 x 5000, 16/8: 320); 512, 431 (2 x 4000, 32/32: 2048).  D = 32: 418, 760; 797, 899; 457, 368; 849, 693.
+// About the border, 1 x 4096 with 18/18, 20/20 and 22/22 heads (576, 640, 704): 387, 388; 414, 405; 451, 423; window 1024: 236, 219; 250, 251; 267, 267.  D = 32: 251, 254; 271, 263; 291, 270;
+// window 1024: 153, 141; 163, 161; 176, 176.
 bool dkv_split(int B, const Sizes& z) { return (int64_t)((z.S + 127) / 128) * z.KH * B <= 640; }
 // and with one block of keys to eight query groups (D = 32: they find room in LDS) where the workgroups of two would not fill the GPU, or only just, and with chains of every length.
 // 1 x 8 and 2 x 4: 43, 57 (1 x 600, 8/2: 20 workgroups of 2 x 4); 280, 341 (1 x 4096, 16/4: 256); 121, 97 (1 x 2048, 16/16: 512); window 512: 87, 78 (1 x 2000, 32/8: 256).
