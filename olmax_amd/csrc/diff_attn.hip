@@ -112,6 +112,11 @@ __device__ __forceinline__ void redo_fwd(const bf16* q, const bf16* K, int64_t l
   }
 }
 
+// What gradients of queries and keys are multiplied by: a query that sees one key alone has P = 1 whatever they are, and gradients of exactly 0, where an exponential, and dP in two places, leave
+// roundings; so has a key that only such queries see, where there are no others.  (Not a select: what is not finite stays so.)
+__device__ __forceinline__ float query_moves(int i, int window) { return i == 0 || window == 0 ? 0.f : 1.f; }
+__device__ __forceinline__ float key_moves(int S, int window) { return S == 1 || window == 0 ? 0.f : 1.f; }
+
 // p_m and dP of a pair
 template <int W>
 __device__ __forceinline__ void pair_of(const bf16* q, const bf16* k, const bf16* d_o, const bf16* v, float l1, float l2, float scale, float& p1, float& p2, float& dp) {
@@ -157,7 +162,7 @@ __device__ __forceinline__ void redo_dq(const bf16* q, const bf16* K, int64_t ld
   }
 #pragma unroll
   for (int c = 0; c < W / 64; c++)
-    if (c * 64 + lane >= lo && c * 64 + lane < hi) dq[c * 64 + lane] = f2bf(acc[c] * scale);
+    if (c * 64 + lane >= lo && c * 64 + lane < hi) dq[c * 64 + lane] = f2bf(acc[c] * (scale * query_moves(i, window)));
 }
 
 // key j, columns [lo, hi); Q, dO, stats, lam of the first of its rep query heads
@@ -197,7 +202,7 @@ __device__ __forceinline__ void redo_dkv(const bf16* Q, int64_t ldq, const bf16*
   for (int c = 0; c < W / 64; c++) {
     const int at = c * 64 + lane;
     if (at < lo || at >= hi) continue;
-    dk[at] = f2bf(ak[c] * scale);
+    dk[at] = f2bf(ak[c] * (scale * key_moves(S, window)));
     dv[at] = f2bf(av[c]);
   }
 }
@@ -846,11 +851,12 @@ __global__ __launch_bounds__(QW * KG * 64, 2) void diff_attn_dq_kernel(const bf1
     sum2 *= mend(lse[S], l2);
   }
   float zeros = 0.f;
+  const float moves = z.scale * query_moves(qi, window);
   auto store4 = [&](int u, const f32x4& v) {
     Pack4 pk;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float x = v[e] * (u < W / 16 ? z.scale : -lam * z.scale);
+      const float x = v[e] * (u < W / 16 ? moves : -lam * moves);
       zeros = __builtin_fmaf(x, 0.f, zeros);
       pk.e[e] = f2bf(x);
     }
@@ -922,7 +928,7 @@ __global__ __launch_bounds__(1024) void diff_attn_dq_join_kernel(const bf16* __r
     float zeros = (sum1 + sum2) * 0.f;
 #pragma unroll
     for (int x = 0; x < W / 64; x++) {
-      const float v = y[x] * (x * 64 + lane < W / 2 ? z.scale : -lam * z.scale);
+      const float moves = z.scale * query_moves(i, window), v = y[x] * (x * 64 + lane < W / 2 ? moves : -lam * moves);
       zeros = __builtin_fmaf(v, 0.f, zeros);
       dq[x * 64 + lane] = f2bf(v);
     }
@@ -1209,6 +1215,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   bf16* kp = dK + ((int64_t)b * S + min(ke, S - 1)) * gr.lddk + kh * W;
   bf16* vp = dV + ((int64_t)b * S + min(ke, S - 1)) * gr.lddv + kh * W;
   float zeros = 0.f;
+  const float moves = z.scale * key_moves(S, window);
   auto store4 = [&](bf16* p, int dt, int g, const f32x4& v, float mul) {
     Pack4 pk;
 #pragma unroll
@@ -1225,7 +1232,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
       for (int dt = 0; dt < W / 32; dt++)
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-          store4(kp, dt, g, f32x4{dk[dt][g * 4], dk[dt][g * 4 + 1], dk[dt][g * 4 + 2], dk[dt][g * 4 + 3]}, z.scale);
+          store4(kp, dt, g, f32x4{dk[dt][g * 4], dk[dt][g * 4 + 1], dk[dt][g * 4 + 2], dk[dt][g * 4 + 3]}, moves);
           store4(vp, dt, g, f32x4{dv[dt][g * 4], dv[dt][g * 4 + 1], dv[dt][g * 4 + 2], dv[dt][g * 4 + 3]}, 1.f);
           __builtin_amdgcn_sched_barrier(0);  // a row leaves in order (see attn.hip)
         }
@@ -1233,7 +1240,7 @@ __global__ __launch_bounds__(KW * QS * 64, 2) void diff_attn_dkv_kernel(const bf
   } else {
     // the stages are free: the last round ended in a barrier; dK first, then dV in the same space
     add_partials<W, QS>(smem, dk, kw, qs, le, [&](int u, const f32x4& v) {
-      if (ke < S) store4(kp, u >> 2, u & 3, v, z.scale);
+      if (ke < S) store4(kp, u >> 2, u & 3, v, moves);
     });
     __syncthreads();
     add_partials<W, QS>(smem, dv, kw, qs, le, [&](int u, const f32x4& v) {
@@ -1273,8 +1280,9 @@ __global__ __launch_bounds__(256) void diff_attn_dkv_join_kernel(const bf16* __r
     bf16 *dk = dK + at * gr.lddk + kh * W, *dv = dV + at * gr.lddv + kh * W;
 #pragma unroll
     for (int x = 0; x < W / 64; x++) {
-      zeros = __builtin_fmaf(yk[x] * z.scale, 0.f, __builtin_fmaf(yv[x], 0.f, zeros));
-      dk[x * 64 + lane] = f2bf(yk[x] * z.scale);
+      const float k = yk[x] * (z.scale * key_moves(S, window));
+      zeros = __builtin_fmaf(k, 0.f, __builtin_fmaf(yv[x], 0.f, zeros));
+      dk[x * 64 + lane] = f2bf(k);
       dv[x * 64 + lane] = f2bf(yv[x]);
     }
     if (__builtin_amdgcn_ballot_w64(zeros != 0.f)) {

@@ -496,3 +496,31 @@ def test_a_workspace_that_is_not_needed_may_lie_anywhere():
         _lib.check(_lib.typed("olmax_diff_attn_fwd")(_lib.raw_stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), o.data_ptr(), o2.data_ptr(), lse.data_ptr(), at, 0, *sizes.values(),
                                                      512, 256, 256, 512, 512, 0, -1))
         assert all(torch.equal(a, b) for a, b in zip((o, o2, lse), want))
+
+
+@pytest.mark.parametrize("sizes,window", [(dict(B=1, S=1, H=4, KH=2, D=64), None), (dict(B=5, S=1, H=2, KH=1, D=32), 1024), (dict(B=700, S=1, H=8, KH=8, D=64), 0), (dict(B=2, S=2, H=8, KH=4, D=64), 0),
+                                          (dict(B=1, S=200, H=4, KH=2, D=64), 0), (dict(B=1, S=333, H=4, KH=2, D=32), 0), (dict(B=41, S=130, H=16, KH=8, D=64), 0), (dict(B=2, S=1100, H=20, KH=10, D=32), 0),
+                                          (dict(B=2, S=1100, H=16, KH=8, D=64), None), (dict(B=1, S=2111, H=1, KH=1, D=64), None), (dict(B=2, S=90, H=4, KH=2, D=32), 20)])
+def test_a_query_that_sees_one_key_moves_nothing(sizes, window):
+    """Its probabilities are 1 whatever queries and keys are: their gradients are exactly 0, not what roundings leave.  So they are where something that it does not see is not finite."""
+    B, S = sizes["B"], sizes["S"]
+    q, k, v, lam, do = (t.cuda() for t in make(**sizes, seed=17))
+    r = ops().diff_attn_fwd(q, k, v, lam, window=window, **sizes)
+    alone = torch.arange(S) == 0 if window != 0 else torch.ones(S, dtype=torch.bool)
+    alone = alone.repeat(B).cuda()
+
+    def grads(**changed):
+        return ops().diff_attn_bwd(*(changed.get(n, t) for n, t in (("q", q), ("k", k), ("v", v))), lam, *r, changed.get("do", do), window=window, **sizes)
+    g = grads()
+    assert g[0][alone].eq(0).all() and (alone.all() or not g[0][~alone].eq(0).all(1).any())
+    if alone.all():
+        assert g[1].eq(0).all()
+        assert torch.equal(g[2].eq(0).all(), torch.tensor(False, device="cuda"))
+    if S > 5:
+        k2, v2, q2, do2 = (t.clone() for t in (k, v, q, do))
+        k2[5, 1] = v2[5, 3] = math.nan
+        assert grads(k=k2, v=v2)[0][alone & (torch.arange(B * S, device="cuda") != 5)].eq(0).all()
+        if window == 0:
+            q2[5, 1] = do2[5, 2] = math.nan
+            dk = grads(q=q2, do=do2)[1]
+            assert dk[torch.arange(B * S, device="cuda") != 5].eq(0).all() and not dk[5].isfinite().all()
